@@ -906,6 +906,39 @@ int koemi_herm_combine_norm_fusion(const void* expert_outputs, const int64_t* pa
                                    void* next_input_bf16, int64_t pairs, int64_t width, int64_t tokens,
                                    int64_t top_k, int64_t num_segments, float eps, koemi_stream_t stream);
 
+/* The bounded recurrent state from its gate pre-activations, to be trained:
+ * BoundedRecurrentState.gates (model/memory.py:14-30), the masking and scan of
+ * network.py:306-310, and the gradients that autograd forms through them in the
+ * reference. preactivations (F32, F16 or BF16): row (b, t) starts at
+ * b batch_stride + t row_stride (elements) and holds u W_r^T + b_r in its first
+ * `width` columns and u W_c^T + b_c in the next. a = 2^-8 + (1 - 2^-7) sigmoid,
+ * b = (1 - a) tanh, (1, 0) where valid [batch, length] is 0 (NULL: all valid),
+ * h_t = a_t h_{t-1} + b_t in fp32 from initial [batch, width] fp32 (NULL:
+ * zeros). states [batch, length, width] in the input's type, final_states
+ * [batch, width] fp32 (length 0: the initial states). kept (NULL: not wanted)
+ * [batch, koemi_gated_recurrence_kept_rows(length), width] fp32 receives the
+ * states that the backward starts from. `workspace` holds the maps of a sequence cut
+ * into parts (0 bytes where the batch's columns alone fill the chip). What lies in
+ * masked positions does not matter, NaN included. */
+int64_t koemi_gated_recurrence_kept_rows(int64_t length);
+size_t koemi_gated_recurrence_workspace_bytes(int64_t batch, int64_t length, int64_t width);
+int koemi_gated_recurrence_forward(const void* preactivations, int64_t batch_stride, int64_t row_stride, int dtype,
+                                   const uint8_t* valid, const float* initial, void* states, float* final_states,
+                                   float* kept, int64_t batch, int64_t length, int64_t width, void* workspace,
+                                   size_t workspace_bytes, koemi_stream_t stream);
+
+/* Its gradients: from grad_states [batch, length, width] (the input's type;
+ * NULL: zeros) and grad_final [batch, width] fp32 (NULL: zeros) to
+ * grad_preactivations [batch, length, 2 width] contiguous, in the input's type
+ * (0 in masked positions), and grad_initial [batch, width] fp32 (NULL: not
+ * wanted). preactivations, valid and kept as the forward had them. The states are
+ * formed again from `kept`; sums and products in fp32, in a fixed order. */
+int koemi_gated_recurrence_backward(const void* preactivations, int64_t batch_stride, int64_t row_stride, int dtype,
+                                    const uint8_t* valid, const float* kept, const void* grad_states,
+                                    const float* grad_final, void* grad_preactivations, float* grad_initial,
+                                    int64_t batch, int64_t length, int64_t width, void* workspace,
+                                    size_t workspace_bytes, koemi_stream_t stream);
+
 /* Measurement only (no counterpart in the reference): reads `bytes` (a
  * multiple of 16) from `src` with `grid` workgroups of `block` threads, each
  * thread issuing `unroll` (1, 2, 4 or 8) 16-byte loads per pass of a

@@ -1,0 +1,615 @@
+// The bounded recurrent state with its gradients, from gate pre-activations.
+//
+//   s = sigmoid(r), a = 2^-8 + (1 - 2^-7) s, k = 1 - a, u = tanh(c)
+//   h_t = a_t h_{t-1} + k_t u_t                 (a masked position: h_t = h_{t-1})
+//   g_t = dh_t + a_{t+1} g_{t+1},  g_{L-1} = dh_{L-1} + dfinal
+//   dr_t = g_t (h_{t-1} - u_t) (1 - 2^-7) s (1 - s),  dc_t = g_t k_t (1 - u_t^2),
+//   dh0 = a_0 g_0
+//
+// (model/memory.py:14-30 and network.py:306-310 of the reference, whose
+// gradients its autograd forms.) Both directions are scans of affine maps
+// x -> p x + q, which compose as (p2, q2) o (p1, q1) = (p2 p1, p2 q1 + q2).
+//
+// A workgroup owns a strip of columns of one batch row and walks a part of the
+// sequence in chunks. A chunk's steps lie on LPC lane groups of eight waves,
+// kSteps consecutive steps each, a lane two adjacent columns (one where the layout
+// allows no pairs): each lane folds its steps into one map, the groups of a wave
+// compose theirs by shuffles, the waves theirs through LDS, and then every lane
+// runs its steps again from its own entry state. The next chunk's loads are in
+// flight meanwhile. Bound by memory and, for 16-bit inputs, as much by the gates
+// (four transcendental instructions and about twenty others an element).
+//
+// The backward pass forms h again instead of reading it: the forward keeps the
+// fp32 state before every kKeep-th position (1/64 of an element's traffic),
+// and a chunk starts from there. That saves the read of h, and the gradients see the
+// fp32 states, not states rounded to 16 bits.
+//
+// Strips are as wide as still fill the chip; where even narrow ones do not (few
+// long rows), the sequence is cut into parts that run at once: a first launch
+// folds each part but the last (first, for the gradients) into its map, and each
+// part's workgroup composes the maps before it (after it).
+#include "common.hpp"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace koemi {
+namespace {
+
+constexpr int kSteps = 8;                     // steps of a lane and chunk
+constexpr int kWaves = 8;                     // waves of a workgroup
+constexpr int kThreads = kWave * kWaves;
+constexpr int kKeep = kSteps * kWaves;        // positions between kept states
+constexpr int kMaxParts = 64;                 // parts a sequence is cut into at most
+
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC) Pack {
+    T e[VEC];
+};
+
+// One element's gates. e stays finite (an infinite one would make 0 x inf of k);
+// the comparisons keep NaN.
+struct Gates {
+    float a, k, u;    // retention, 1 - retention, candidate
+    float ds, du;     // s (1 - s), 1 - u^2
+};
+__device__ __forceinline__ void exp_pair(float r, float c, float& e, float& d) {
+    const float x = r * -1.44269504088896341f;
+    e = __builtin_amdgcn_exp2f(x > 126.0f ? 126.0f : x);
+    d = __builtin_amdgcn_exp2f(fabsf(c) * -2.88539008177792682f);
+}
+// s = 1 / (1 + e) and 1 - s = e / (1 + e) each to fp32's relative precision, so that
+// k (down to 2^-8) loses nothing to a subtraction from 1.
+template <bool GRADIENTS>
+__device__ __forceinline__ Gates gates_of(float r, float c) {
+    Gates o;
+    float e, d;
+    exp_pair(r, c, e, d);
+    const float s = __builtin_amdgcn_rcpf(1.0f + e), w = __builtin_amdgcn_rcpf(1.0f + d), rest = e * s;
+    o.a = fmaf(kGateRetentionSpan, s, kGateMinRetention);
+    o.k = fmaf(kGateRetentionSpan, rest, kGateMinRetention);
+    o.u = copysignf((1.0f - d) * w, c);
+    if constexpr (GRADIENTS) {
+        o.ds = s * rest;
+        o.du = 4.0f * d * w * w;
+    }
+    return o;
+}
+__device__ __forceinline__ float retention_of(float r) {
+    return fmaf(kGateRetentionSpan, gate_sigmoid(r), kGateMinRetention);
+}
+
+// What both directions work on. z: r in the first `width` columns of a row, c in
+// the next; rows z_row elements apart, batch rows z_batch.
+struct Sequence {
+    const void* z;
+    int64_t z_batch, z_row;
+    const uint8_t* valid;  // [batch, length] or null
+    int64_t batch, length, width;
+    int64_t strips, parts, part_steps;
+};
+
+template <int VEC, int LPC>
+struct Place {
+    static constexpr int kLanes = kWave / LPC;       // lanes of a group
+    static constexpr int kColumns = kLanes * VEC;    // columns of a strip
+    static constexpr int kChunk = kKeep * LPC;       // steps of a chunk
+    int wave, group, lane;       // lane: of its group
+    int64_t b, part, f;          // f: the lane's first column
+    bool inside;                 // its columns exist
+    uint32_t segment;            // the lane's first step in a chunk
+
+    // Workgroup i runs on XCD i % 8: each XCD takes a contiguous range of
+    // (batch row, part, strip), so that strips that share cache lines share an L2.
+    __device__ __forceinline__ bool place(const Sequence& q) {
+        const uint32_t total = static_cast<uint32_t>(q.batch * q.parts * q.strips), per = (total + 7) / 8;
+        const uint32_t i = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+        if ((blockIdx.x >> 3) >= per || i >= total) return false;
+        const uint32_t strip = i % static_cast<uint32_t>(q.strips), rest = i / static_cast<uint32_t>(q.strips);
+        part = rest % static_cast<uint32_t>(q.parts);
+        b = rest / static_cast<uint32_t>(q.parts);
+        wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+        group = lane_id() / kLanes;
+        lane = lane_id() % kLanes;
+        f = static_cast<int64_t>(strip) * kColumns + lane * VEC;
+        inside = f < q.width;
+        if (!inside) f = 0;
+        segment = static_cast<uint32_t>((wave * LPC + group) * kSteps);
+        return true;
+    }
+};
+
+// The steps [t, t + kSteps) of one array's columns; steps past `end` repeat the last.
+// `whole` (uniform): none is.
+template <typename T, int VEC>
+__device__ __forceinline__ void load_steps(Pack<T, VEC> (&o)[kSteps], const T* base, int64_t row, int64_t t, int64_t end,
+                                           bool whole) {
+    if (whole) {
+        const T* p = base + t * row;
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i, p += row) o[i] = *reinterpret_cast<const Pack<T, VEC>*>(p);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i)
+            o[i] = *reinterpret_cast<const Pack<T, VEC>*>(base + min(t + i, end - 1) * row);
+    }
+}
+// Bit i: step t + i is before `end` and valid.
+__device__ __forceinline__ uint32_t load_mask(const uint8_t* valid, int64_t t, int64_t end) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+        const bool v = valid == nullptr ? true : valid[min(t + i, end - 1)] != 0;
+        m |= (v && t + i < end) ? 1u << i : 0u;
+    }
+    return m;
+}
+
+// (p, q) of this lane's group composed with those of the groups before it
+// (REVERSE: after it) in the wave, itself included; before/after alone in (xp, xq).
+template <int LPC, bool REVERSE>
+__device__ __forceinline__ void scan_groups(float& p, float& q, float& xp, float& xq, int group) {
+    constexpr int kLanes = kWave / LPC;
+    xp = 1.0f, xq = 0.0f;
+    if constexpr (LPC > 1) {
+#pragma unroll
+        for (int off = 1; off < LPC; off <<= 1) {
+            const float op = REVERSE ? __shfl_down(p, off * kLanes, kWave) : __shfl_up(p, off * kLanes, kWave);
+            const float oq = REVERSE ? __shfl_down(q, off * kLanes, kWave) : __shfl_up(q, off * kLanes, kWave);
+            const bool has = REVERSE ? group + off < LPC : group >= off;
+            q = has ? fmaf(p, oq, q) : q;
+            p = has ? p * op : p;
+        }
+        const float op = REVERSE ? __shfl_down(p, kLanes, kWave) : __shfl_up(p, kLanes, kWave);
+        const float oq = REVERSE ? __shfl_down(q, kLanes, kWave) : __shfl_up(q, kLanes, kWave);
+        const bool has = REVERSE ? group + 1 < LPC : group > 0;
+        xp = has ? op : 1.0f;
+        xq = has ? oq : 0.0f;
+    }
+}
+
+// The state before every kKeep-th position lies at kept[(b * rows + t / kKeep) * width + f].
+__device__ __forceinline__ int64_t kept_rows(int64_t length) { return (length + kKeep - 1) / kKeep; }
+
+// Forward. FOLD: only the map of each part but the last, into maps[2, batch, parts,
+// width] (p, then q); else the states from the initial state through the maps before.
+template <typename T, int VEC, int LPC, bool FOLD>
+__global__ __launch_bounds__(kThreads) void recurrence_forward_kernel(Sequence s, const float* __restrict__ initial,
+                                                                      T* __restrict__ states, float* __restrict__ final_state,
+                                                                      float* __restrict__ kept, float* __restrict__ maps) {
+    using P = Place<VEC, LPC>;
+    __shared__ float wave_p[2][kWaves][P::kColumns], wave_q[2][kWaves][P::kColumns];
+    P at;
+    if (!at.place(s)) return;
+    if (FOLD && at.part == s.parts - 1) return;
+    const int64_t begin = at.part * s.part_steps, end = min(s.length, begin + s.part_steps);
+    const T* zr = static_cast<const T*>(s.z) + at.b * s.z_batch + at.f;
+    const T* zc = zr + s.width;
+    const uint8_t* valid = s.valid ? s.valid + at.b * s.length : nullptr;
+    const int64_t cells = s.batch * s.parts * s.width;
+    float carry[VEC], prod[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+        carry[v] = FOLD || !initial || !at.inside ? 0.0f : initial[at.b * s.width + at.f + v];
+        prod[v] = 1.0f;
+        if constexpr (!FOLD)
+            for (int64_t j = 0; j < at.part; ++j) {
+                const int64_t cell = (at.b * s.parts + j) * s.width + at.f + v;
+                carry[v] = fmaf(maps[cell], carry[v], maps[cells + cell]);
+            }
+    }
+    struct Raw {
+        Pack<T, VEC> r[kSteps], c[kSteps];
+        uint32_t mask;
+    };
+    auto fetch = [&](int64_t t0, Raw& o) {
+        const bool whole = t0 + P::kChunk <= end;
+        load_steps(o.r, zr, s.z_row, t0 + at.segment, end, whole);
+        load_steps(o.c, zc, s.z_row, t0 + at.segment, end, whole);
+        o.mask = load_mask(valid, t0 + at.segment, end);
+    };
+    int turn = 0;
+    auto chunk = [&](const Raw& raw, int64_t t0) {
+        float a[kSteps][VEC], b[kSteps][VEC], p[VEC], q[VEC], xp[VEC], xq[VEC];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) p[v] = 1.0f, q[v] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                const Gates g = gates_of<false>(to_f32(raw.r[i].e[v]), to_f32(raw.c[i].e[v]));
+                const bool keep = raw.mask >> i & 1;
+                a[i][v] = keep ? g.a : 1.0f;
+                b[i][v] = keep ? g.k * g.u : 0.0f;
+                q[v] = fmaf(a[i][v], q[v], b[i][v]);
+                p[v] *= a[i][v];
+            }
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            scan_groups<LPC, false>(p[v], q[v], xp[v], xq[v], at.group);
+            if (at.group == LPC - 1) {
+                wave_p[turn][at.wave][at.lane * VEC + v] = p[v];
+                wave_q[turn][at.wave][at.lane * VEC + v] = q[v];
+            }
+        }
+        __syncthreads();  // the other buffer's readers are past it: they have written this one
+        float in[VEC];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            float x = carry[v];
+            in[v] = x;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                if (w == at.wave) in[v] = x;
+                const float wp = wave_p[turn][w][at.lane * VEC + v];
+                x = fmaf(wp, x, wave_q[turn][w][at.lane * VEC + v]);
+                if constexpr (FOLD) prod[v] *= wp;
+            }
+            carry[v] = x;
+            in[v] = fmaf(xp[v], in[v], xq[v]);
+        }
+        turn ^= 1;
+        if constexpr (!FOLD) {
+            if (!at.inside) return;
+            const int64_t t = t0 + at.segment;
+            if (kept && t % kKeep == 0 && t < end) {
+                Pack<float, VEC> k;
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) k.e[v] = in[v];
+                *reinterpret_cast<Pack<float, VEC>*>(kept + (at.b * kept_rows(s.length) + t / kKeep) * s.width + at.f) = k;
+            }
+            T* out = states + (at.b * s.length + t) * s.width + at.f;
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i, out += s.width) {
+                Pack<T, VEC> h;
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) {
+                    in[v] = fmaf(a[i][v], in[v], b[i][v]);
+                    h.e[v] = from_f32<T>(in[v]);
+                }
+                if (t + i < end) *reinterpret_cast<Pack<T, VEC>*>(out) = h;
+            }
+        }
+    };
+    if (begin < end) {
+        Raw x, y;
+        fetch(begin, x);
+        for (int64_t t0 = begin;;) {
+            if (t0 + P::kChunk < end) fetch(t0 + P::kChunk, y);
+            chunk(x, t0);
+            if ((t0 += P::kChunk) >= end) break;
+            if (t0 + P::kChunk < end) fetch(t0 + P::kChunk, x);
+            chunk(y, t0);
+            if ((t0 += P::kChunk) >= end) break;
+        }
+    }
+    if (!at.inside || at.wave != 0 || at.group != 0) return;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+        if constexpr (FOLD) {
+            const int64_t cell = (at.b * s.parts + at.part) * s.width + at.f + v;
+            maps[cell] = prod[v];
+            maps[cells + cell] = carry[v];
+        } else if (at.part == s.parts - 1) {
+            final_state[at.b * s.width + at.f + v] = carry[v];
+        }
+    }
+}
+
+// Backward, from the last chunk to the first. The carry is a_{t+1} g_{t+1}. FOLD:
+// only the map of each part but the first.
+template <typename T, int VEC, int LPC, bool FOLD>
+__global__ __launch_bounds__(kThreads) void recurrence_backward_kernel(
+    Sequence s, const float* __restrict__ kept, const T* __restrict__ d_states, const float* __restrict__ d_final,
+    T* __restrict__ d_z, float* __restrict__ d_initial, float* __restrict__ maps) {
+    using P = Place<VEC, LPC>;
+    __shared__ float wave_p[2][kWaves][P::kColumns], wave_q[2][kWaves][P::kColumns], wave_h[2][kWaves][P::kColumns];
+    P at;
+    if (!at.place(s)) return;
+    if (FOLD && at.part == 0) return;
+    const int64_t begin = at.part * s.part_steps, end = min(s.length, begin + s.part_steps);
+    const T* zr = static_cast<const T*>(s.z) + at.b * s.z_batch + at.f;
+    const T* zc = zr + s.width;
+    const T* up = d_states ? d_states + at.b * s.length * s.width + at.f : nullptr;
+    const uint8_t* valid = s.valid ? s.valid + at.b * s.length : nullptr;
+    const int64_t cells = s.batch * s.parts * s.width;
+    float carry[VEC], prod[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+        carry[v] = FOLD || !d_final || !at.inside ? 0.0f : d_final[at.b * s.width + at.f + v];
+        prod[v] = 1.0f;
+        if constexpr (!FOLD)
+            for (int64_t j = s.parts - 1; j > at.part; --j) {
+                const int64_t cell = (at.b * s.parts + j) * s.width + at.f + v;
+                carry[v] = fmaf(maps[cell], carry[v], maps[cells + cell]);
+            }
+    }
+    struct Raw {
+        Pack<T, VEC> r[kSteps], c[kSteps], d[kSteps];
+        Pack<float, VEC> h;
+        uint32_t mask;
+    };
+    auto fetch = [&](int64_t t0, Raw& o) {
+        const bool whole = t0 + P::kChunk <= end;
+        const int64_t t = t0 + at.segment;
+        load_steps(o.r, zr, s.z_row, t, end, whole);
+        if (up) load_steps(o.d, up, s.width, t, end, whole);
+        if constexpr (!FOLD) {
+            load_steps(o.c, zc, s.z_row, t, end, whole);
+            o.h = *reinterpret_cast<const Pack<float, VEC>*>(kept + (at.b * kept_rows(s.length) + t0 / kKeep) * s.width + at.f);
+        }
+        o.mask = load_mask(valid, t, end);
+    };
+    int turn = 0;
+    auto chunk = [&](const Raw& raw, int64_t t0) {
+        Gates g[kSteps][VEC];
+        float d[kSteps][VEC], p[VEC], q[VEC], fp[VEC], fq[VEC], xp[VEC], xq[VEC], yp[VEC], yq[VEC];
+        const int64_t t = t0 + at.segment;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) p[v] = 1.0f, q[v] = 0.0f, fq[v] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                const bool keep = raw.mask >> i & 1;
+                if constexpr (FOLD) {
+                    g[i][v].a = keep ? retention_of(to_f32(raw.r[i].e[v])) : 1.0f;
+                } else {
+                    g[i][v] = gates_of<true>(to_f32(raw.r[i].e[v]), to_f32(raw.c[i].e[v]));
+                    g[i][v].a = keep ? g[i][v].a : 1.0f;
+                    fq[v] = fmaf(g[i][v].a, fq[v], keep ? g[i][v].k * g[i][v].u : 0.0f);
+                }
+                p[v] *= g[i][v].a;
+                d[i][v] = up && t + i < end ? to_f32(raw.d[i].e[v]) : 0.0f;
+            }
+#pragma unroll
+        for (int i = kSteps - 1; i >= 0; --i)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) q[v] = g[i][v].a * (d[i][v] + q[v]);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            fp[v] = p[v];
+            scan_groups<LPC, true>(p[v], q[v], xp[v], xq[v], at.group);
+            if constexpr (!FOLD) scan_groups<LPC, false>(fp[v], fq[v], yp[v], yq[v], at.group);
+            if (at.group == 0) {
+                wave_p[turn][at.wave][at.lane * VEC + v] = p[v];
+                wave_q[turn][at.wave][at.lane * VEC + v] = q[v];
+            }
+            if (!FOLD && at.group == LPC - 1) wave_h[turn][at.wave][at.lane * VEC + v] = fq[v];
+        }
+        __syncthreads();
+        float in[VEC], h[VEC];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            float x = carry[v];
+            in[v] = x;
+            float y = FOLD ? 0.0f : raw.h.e[v];
+            h[v] = y;
+            float wp[kWaves];
+#pragma unroll
+            for (int w = kWaves - 1; w >= 0; --w) {
+                if (w == at.wave) in[v] = x;
+                wp[w] = wave_p[turn][w][at.lane * VEC + v];
+                x = fmaf(wp[w], x, wave_q[turn][w][at.lane * VEC + v]);
+                if constexpr (FOLD) prod[v] *= wp[w];
+            }
+            carry[v] = x;
+            if constexpr (!FOLD) {
+#pragma unroll
+                for (int w = 0; w < kWaves - 1; ++w) {
+                    y = fmaf(wp[w], y, wave_h[turn][w][at.lane * VEC + v]);
+                    if (w + 1 == at.wave) h[v] = y;
+                }
+                in[v] = fmaf(xp[v], in[v], xq[v]);
+                h[v] = fmaf(yp[v], h[v], yq[v]);
+            }
+        }
+        turn ^= 1;
+        if constexpr (!FOLD) {
+            if (!at.inside) return;
+            float before[kSteps][VEC];
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) {
+                    before[i][v] = h[v];
+                    h[v] = fmaf(g[i][v].a, h[v], raw.mask >> i & 1 ? g[i][v].k * g[i][v].u : 0.0f);
+                }
+            T* out = d_z + (at.b * s.length + t) * 2 * s.width + at.f;
+#pragma unroll
+            for (int i = kSteps - 1; i >= 0; --i) {
+                Pack<T, VEC> dr, dc;
+                const bool keep = raw.mask >> i & 1;
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) {
+                    const Gates& w = g[i][v];
+                    const float gt = d[i][v] + in[v];
+                    in[v] = w.a * gt;
+                    dr.e[v] = from_f32<T>(keep ? gt * (before[i][v] - w.u) * (kGateRetentionSpan * w.ds) : 0.0f);
+                    dc.e[v] = from_f32<T>(keep ? gt * (w.k * w.du) : 0.0f);
+                }
+                if (t + i < end) {
+                    *reinterpret_cast<Pack<T, VEC>*>(out + i * 2 * s.width) = dr;
+                    *reinterpret_cast<Pack<T, VEC>*>(out + i * 2 * s.width + s.width) = dc;
+                }
+            }
+        }
+    };
+    if (begin < end) {
+        Raw x, y;
+        int64_t t0 = begin + (end - begin - 1) / P::kChunk * P::kChunk;
+        fetch(t0, x);
+        for (;;) {
+            if (t0 > begin) fetch(t0 - P::kChunk, y);
+            chunk(x, t0);
+            if ((t0 -= P::kChunk) < begin) break;
+            if (t0 > begin) fetch(t0 - P::kChunk, x);
+            chunk(y, t0);
+            if ((t0 -= P::kChunk) < begin) break;
+        }
+    }
+    if (!at.inside || at.wave != 0 || at.group != 0) return;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+        if constexpr (FOLD) {
+            const int64_t cell = (at.b * s.parts + at.part) * s.width + at.f + v;
+            maps[cell] = prod[v];
+            maps[cells + cell] = carry[v];
+        } else if (at.part == 0 && d_initial) {
+            d_initial[at.b * s.width + at.f + v] = carry[v];
+        }
+    }
+}
+
+// How a call is laid out: two columns a lane where rows allow it, the widest strip
+// that still gives two workgroups a CU, and parts where the narrowest does not.
+struct Plan {
+    int vec, lpc;
+    int64_t strips, parts, part_steps;
+};
+constexpr int64_t kFill = 512;  // workgroups that keep 256 CUs loaded
+
+inline Plan plan_of(int64_t batch, int64_t length, int64_t width, int vec) {
+    Plan p;
+    p.vec = vec;
+    for (p.lpc = 1;; p.lpc *= 2) {
+        const int64_t columns = kWave / p.lpc * vec;
+        p.strips = (width + columns - 1) / columns;
+        if (batch * p.strips >= kFill || p.lpc == 4) break;
+    }
+    const int64_t chunk = static_cast<int64_t>(kKeep) * p.lpc, chunks = (length + chunk - 1) / chunk;
+    p.parts = 1;
+    if (batch * p.strips < kFill / 2 && chunks >= 8)
+        p.parts = std::min<int64_t>(std::min<int64_t>(kMaxParts, chunks / 4), (kFill + batch * p.strips - 1) / (batch * p.strips));
+    const int64_t per = (chunks + p.parts - 1) / std::max<int64_t>(p.parts, 1);
+    p.part_steps = std::max<int64_t>(per, 1) * chunk;
+    p.parts = std::max<int64_t>((length + p.part_steps - 1) / p.part_steps, 1);
+    return p;
+}
+// Every row of the arrays starts where two elements load at once.
+inline bool pairs_fit(const void* z, int64_t z_batch, int64_t z_row, int64_t width, int dtype, const void* x,
+                      const void* y, const void* kept) {
+    const uintptr_t two = dtype == KOEMI_F32 ? 8 : 4;
+    const uintptr_t bases = reinterpret_cast<uintptr_t>(z) | reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y);
+    return width % 2 == 0 && z_batch % 2 == 0 && z_row % 2 == 0 && bases % two == 0 &&
+           reinterpret_cast<uintptr_t>(kept) % 8 == 0;
+}
+inline size_t maps_bytes(const Plan& p, int64_t batch, int64_t width) {
+    return p.parts > 1 ? static_cast<size_t>(2 * batch * p.parts * width) * sizeof(float) : 0;
+}
+
+int check_sequence(const char* what, const void* z, int64_t z_batch, int64_t z_row, int dtype, int64_t batch, int64_t length,
+                   int64_t width) {
+    if (!float_dtype(dtype)) return fail(KOEMI_ERR_UNSUPPORTED, "%s: unsupported dtype %s", what, dtype_name(dtype));
+    if (batch < 0 || length < 0 || width < 0) return fail(KOEMI_ERR_INVALID, "%s: negative dimension", what);
+    if (batch == 0 || width == 0) return KOEMI_OK;
+    if (length > 0 && !z) return fail(KOEMI_ERR_INVALID, "%s: null pre-activations", what);
+    if (length > 1 && z_row < 2 * width) return fail(KOEMI_ERR_INVALID, "%s: pre-activation rows overlap", what);
+    const __int128 cells = static_cast<__int128>(batch) * width * (length + 1) * 8;
+    if (cells > (static_cast<__int128>(1) << 60)) return fail(KOEMI_ERR_INVALID, "%s: too many elements", what);
+    if (static_cast<__int128>(batch) * width > (int64_t(1) << 30))
+        return fail(KOEMI_ERR_UNSUPPORTED, "%s: batch x width above 2^30", what);
+    return KOEMI_OK;
+}
+
+unsigned grid_of(const Sequence& s) { return static_cast<unsigned>((s.batch * s.parts * s.strips + 7) / 8 * 8); }
+
+// Calls run(std::integral_constant VEC, LPC) of the plan.
+template <typename Run>
+void by_plan(const Plan& p, Run run) {
+    auto lanes = [&](auto vec) {
+        if (p.lpc == 1) run(vec, std::integral_constant<int, 1>{});
+        else if (p.lpc == 2) run(vec, std::integral_constant<int, 2>{});
+        else run(vec, std::integral_constant<int, 4>{});
+    };
+    if (p.vec == 2) lanes(std::integral_constant<int, 2>{});
+    else lanes(std::integral_constant<int, 1>{});
+}
+
+template <typename T>
+int forward(Sequence s, const Plan& p, const float* initial, void* states, float* final_state, float* kept, float* maps,
+            hipStream_t stream) {
+    by_plan(p, [&](auto vec, auto lpc) {
+        constexpr int V = decltype(vec)::value, C = decltype(lpc)::value;
+        if (s.parts > 1)
+            hipLaunchKernelGGL((recurrence_forward_kernel<T, V, C, true>), dim3(grid_of(s)), dim3(kThreads), 0, stream, s,
+                               initial, static_cast<T*>(states), final_state, kept, maps);
+        hipLaunchKernelGGL((recurrence_forward_kernel<T, V, C, false>), dim3(grid_of(s)), dim3(kThreads), 0, stream, s,
+                           initial, static_cast<T*>(states), final_state, kept, maps);
+    });
+    return check_launch("koemi_gated_recurrence_forward");
+}
+template <typename T>
+int backward(Sequence s, const Plan& p, const float* kept, const void* d_states, const float* d_final, void* d_z,
+             float* d_initial, float* maps, hipStream_t stream) {
+    by_plan(p, [&](auto vec, auto lpc) {
+        constexpr int V = decltype(vec)::value, C = decltype(lpc)::value;
+        if (s.parts > 1)
+            hipLaunchKernelGGL((recurrence_backward_kernel<T, V, C, true>), dim3(grid_of(s)), dim3(kThreads), 0, stream, s,
+                               kept, static_cast<const T*>(d_states), d_final, static_cast<T*>(d_z), d_initial, maps);
+        hipLaunchKernelGGL((recurrence_backward_kernel<T, V, C, false>), dim3(grid_of(s)), dim3(kThreads), 0, stream, s,
+                           kept, static_cast<const T*>(d_states), d_final, static_cast<T*>(d_z), d_initial, maps);
+    });
+    return check_launch("koemi_gated_recurrence_backward");
+}
+
+}  // namespace
+}  // namespace koemi
+
+using namespace koemi;
+
+extern "C" int64_t koemi_gated_recurrence_kept_rows(int64_t length) {
+    return length > 0 ? (length + kKeep - 1) / kKeep : 0;
+}
+
+extern "C" size_t koemi_gated_recurrence_workspace_bytes(int64_t batch, int64_t length, int64_t width) {
+    if (batch <= 0 || length <= 0 || width <= 0) return 0;
+    size_t most = 0;  // of either layout: which one a call takes depends on its alignment
+    for (int vec = 1; vec <= 2; ++vec) most = std::max(most, maps_bytes(plan_of(batch, length, width, vec), batch, width));
+    return most;
+}
+
+extern "C" int koemi_gated_recurrence_forward(const void* preactivations, int64_t batch_stride, int64_t row_stride,
+                                              int dtype, const uint8_t* valid, const float* initial, void* states,
+                                              float* final_states, float* kept, int64_t batch, int64_t length,
+                                              int64_t width, void* workspace, size_t workspace_bytes,
+                                              koemi_stream_t stream) {
+    clear_error();
+    const char* what = "koemi_gated_recurrence_forward";
+    const int st = check_sequence(what, preactivations, batch_stride, row_stride, dtype, batch, length, width);
+    if (st != KOEMI_OK || batch == 0 || width == 0) return st;
+    if (!final_states || (length > 0 && !states)) return fail(KOEMI_ERR_INVALID, "%s: null output", what);
+    const bool pairs = pairs_fit(preactivations, batch_stride, row_stride, width, dtype, states, nullptr, kept);
+    const Plan p = plan_of(batch, length, width, pairs ? 2 : 1);
+    const size_t need = maps_bytes(p, batch, width);
+    if (need && (!workspace || workspace_bytes < need)) return fail(KOEMI_ERR_INVALID, "%s: workspace too small", what);
+    const Sequence s{preactivations, batch_stride, row_stride, valid, batch, length, width, p.strips, p.parts, p.part_steps};
+    float* maps = static_cast<float*>(workspace);
+    if (dtype == KOEMI_F32) return forward<float>(s, p, initial, states, final_states, kept, maps, as_stream(stream));
+    if (dtype == KOEMI_F16) return forward<f16>(s, p, initial, states, final_states, kept, maps, as_stream(stream));
+    return forward<bf16>(s, p, initial, states, final_states, kept, maps, as_stream(stream));
+}
+
+extern "C" int koemi_gated_recurrence_backward(const void* preactivations, int64_t batch_stride, int64_t row_stride,
+                                               int dtype, const uint8_t* valid, const float* kept,
+                                               const void* grad_states, const float* grad_final,
+                                               void* grad_preactivations, float* grad_initial, int64_t batch,
+                                               int64_t length, int64_t width, void* workspace, size_t workspace_bytes,
+                                               koemi_stream_t stream) {
+    clear_error();
+    const char* what = "koemi_gated_recurrence_backward";
+    const int st = check_sequence(what, preactivations, batch_stride, row_stride, dtype, batch, length, width);
+    if (st != KOEMI_OK || batch == 0 || width == 0) return st;
+    if (length > 0 && (!kept || !grad_preactivations)) return fail(KOEMI_ERR_INVALID, "%s: null pointer", what);
+    const bool pairs =
+        pairs_fit(preactivations, batch_stride, row_stride, width, dtype, grad_states, grad_preactivations, kept);
+    const Plan p = plan_of(batch, length, width, pairs ? 2 : 1);
+    const size_t need = maps_bytes(p, batch, width);
+    if (need && (!workspace || workspace_bytes < need)) return fail(KOEMI_ERR_INVALID, "%s: workspace too small", what);
+    const Sequence s{preactivations, batch_stride, row_stride, valid, batch, length, width, p.strips, p.parts, p.part_steps};
+    float* maps = static_cast<float*>(workspace);
+    hipStream_t q = as_stream(stream);
+    if (dtype == KOEMI_F32) return backward<float>(s, p, kept, grad_states, grad_final, grad_preactivations, grad_initial, maps, q);
+    if (dtype == KOEMI_F16) return backward<f16>(s, p, kept, grad_states, grad_final, grad_preactivations, grad_initial, maps, q);
+    return backward<bf16>(s, p, kept, grad_states, grad_final, grad_preactivations, grad_initial, maps, q);
+}

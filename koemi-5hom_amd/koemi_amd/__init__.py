@@ -20,7 +20,7 @@ from koemi_amd.core import fused_rmsnorm_silu, load_core_extension
 from koemi_amd.cuda_scan import cuda_affine_scan, diagnose_cuda_affine_scan
 from koemi_amd.dense import dense_affine_scan, native_cuda_available
 from koemi_amd.memory import read_local_window, read_salient_window, salient_tail
-from koemi_amd.recurrent import recurrent_gates, recurrent_scan
+from koemi_amd.recurrent import gated_recurrence, recurrent_gates, recurrent_scan
 from koemi_amd.moe import (
     combine_topk,
     expert_activation_counts,
@@ -42,6 +42,7 @@ __all__ = [
     "diagnose_cuda_affine_scan",
     "expert_activation_counts",
     "fused_rmsnorm_silu",
+    "gated_recurrence",
     "grouped_expert_mlp_inference",
     "load_core_extension",
     "load_native_extension",

@@ -43,6 +43,7 @@ SOURCES = (
     "herm_glue.hip",
     "linear_rows.hip",
     "gated_projection.hip",
+    "gated_recurrence.hip",
     "stream_probe.hip",
     "refine.hip",
 )

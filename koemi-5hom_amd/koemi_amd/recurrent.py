@@ -7,19 +7,22 @@ invalid positions, affine scan from the carried working state). The gates run
 HIP epilogue kernel); the fp32 window scan runs ``koemi_recurrent_scan``, the
 same products followed by one HIP kernel that forms the gates in registers
 inside the affine scan; other dtypes run the gates and then the dense
-affine-scan kernel. There is no torch fallback. Inference only (no autograd
-through the gates).
+affine-scan kernel. There is no torch fallback. These are inference only (no
+autograd through the gates); ``gated_recurrence`` is the trained form: states
+from stacked gate pre-activations, with the gradients of both.
 """
 
 from __future__ import annotations
 
 import torch
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 from koemi_amd import _native
 from koemi_amd.dense import DenseCudaUnavailableError, DenseCudaValidationError, dense_affine_scan
 
-__all__ = ["GatedScanTimeoutError", "check_gated_scan_status", "gated_scan", "recurrent_gates", "recurrent_scan"]
+__all__ = ["GatedScanTimeoutError", "check_gated_scan_status", "gated_recurrence", "gated_scan", "recurrent_gates",
+           "recurrent_scan"]
 
 # koemi_gated_projection_scan: spin_limit bit that stops tiles publishing their
 # transfers (include/koemi_hip.h KOEMI_GP_WITHHOLD_TRANSFERS), so the host can
@@ -364,3 +367,109 @@ def gated_projection_scan(inputs: Tensor, weight: Tensor, bias: Tensor | None, v
         if own_status:
             check_gated_scan_status(status)
     return (states, states16) if with_bf16 else states
+
+
+_RECURRENCE_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def gated_recurrence(preactivations: Tensor, valid_mask: Tensor | None = None,
+                     initial: Tensor | None = None) -> tuple[Tensor, Tensor]:
+    """Working states from stacked gate pre-activations, with first-order autograd.
+
+    ``preactivations`` ``[B, L, 2 width]`` (float32, float16 or bfloat16) holds
+    ``u W_r^T + b_r`` in its first half and ``u W_c^T + b_c`` in its second, as one
+    stacked projection produces them; any strides (rows are read in place where their
+    columns are contiguous). The gates of memory.py:22-26, the masking of
+    network.py:307-309 (``valid_mask`` ``[B, L]`` bool: a masked position keeps
+    the state, and what its pre-activations hold does not matter) and the scan of
+    network.py:310 from ``initial`` ``[B, width]`` float32 (zeros when
+    omitted) run in one kernel (``koemi_gated_recurrence_forward``).
+
+    Returns ``(states, final)``: ``[B, L, width]`` in the input's dtype and the
+    last states ``[B, width]`` in float32, to be carried into the next window.
+    Both are differentiable by ``preactivations`` and ``initial``
+    (``koemi_gated_recurrence_backward``); states and sums are float32 inside.
+    """
+
+    if not isinstance(preactivations, Tensor) or preactivations.ndim != 3 \
+            or preactivations.dtype not in _RECURRENCE_DTYPES:
+        raise DenseCudaValidationError(
+            "preactivations must be a float32, float16 or bfloat16 [batch, length, 2 width] tensor")
+    batch, length, columns = preactivations.shape
+    if columns % 2:
+        raise DenseCudaValidationError("preactivations must hold as many retention as candidate columns")
+    if preactivations.device.type != "cuda":
+        raise DenseCudaValidationError("preactivations must be on CUDA")
+    width, device = columns // 2, preactivations.device
+    if valid_mask is not None and (not isinstance(valid_mask, Tensor) or valid_mask.dtype != torch.bool
+                                   or valid_mask.shape != (batch, length) or valid_mask.device != device):
+        raise DenseCudaValidationError("valid_mask must be a bool [batch, length] tensor on the same device")
+    if initial is not None and (not isinstance(initial, Tensor) or initial.shape != (batch, width)
+                                or initial.dtype != torch.float32 or initial.device != device):
+        raise DenseCudaValidationError("initial must be a float32 [batch, width] tensor on the same device")
+    if batch * width > 1 << 30:
+        raise DenseCudaValidationError("batch x width must not exceed 2^30")
+    try:
+        _native.load_library()
+    except _native.NativeLibraryUnavailableError as error:
+        raise DenseCudaUnavailableError(str(error)) from error
+    trained = torch.is_grad_enabled() and (preactivations.requires_grad or (initial is not None and initial.requires_grad))
+    return _GatedRecurrence.apply(preactivations, initial, valid_mask, trained)
+
+
+def _in_place(z: Tensor) -> Tensor:
+    """``z`` where a kernel can read its rows as they lie, else a contiguous copy."""
+
+    batch, length, columns = z.shape
+    fits = (columns <= 1 or z.stride(2) == 1) and (length <= 1 or z.stride(1) >= columns) and z.stride(0) >= 0
+    return z if fits else z.contiguous()
+
+
+class _GatedRecurrence(torch.autograd.Function):
+    @staticmethod
+    def forward(context, preactivations: Tensor, initial: Tensor | None, valid_mask: Tensor | None,  # type: ignore[override]
+                trained: bool) -> tuple[Tensor, Tensor]:
+        batch, length, columns = preactivations.shape
+        width, device = columns // 2, preactivations.device
+        z = _in_place(preactivations)
+        h0 = initial.contiguous() if initial is not None else None
+        mask = valid_mask.contiguous() if valid_mask is not None else None
+        states = torch.empty((batch, length, width), device=device, dtype=z.dtype)
+        final = torch.empty((batch, width), device=device, dtype=torch.float32)
+        kept = None
+        if trained:
+            rows = _native.query("koemi_gated_recurrence_kept_rows", length)
+            kept = torch.empty((batch, rows, width), device=device, dtype=torch.float32)
+        need = _native.query("koemi_gated_recurrence_workspace_bytes", batch, length, width)
+        workspace = torch.empty(need, device=device, dtype=torch.uint8) if need else None
+        with _native.device_guard(device):
+            _native.call("koemi_gated_recurrence_forward", z.data_ptr(), z.stride(0), z.stride(1),
+                         _native.dtype_code(z.dtype), _native.ptr(mask), _native.ptr(h0), states.data_ptr(),
+                         final.data_ptr(), _native.ptr(kept), batch, length, width, _native.ptr(workspace), need,
+                         _native.stream_of(device))
+        if trained:
+            context.save_for_backward(z, mask, kept)
+            context.set_materialize_grads(False)
+        return states, final
+
+    @staticmethod
+    @once_differentiable
+    def backward(context, d_states: Tensor | None, d_final: Tensor | None):  # type: ignore[override]
+        z, mask, kept = context.saved_tensors
+        if d_states is None and d_final is None:
+            return None, None, None, None
+        batch, length, columns = z.shape
+        width, device = columns // 2, z.device
+        d_states = d_states.contiguous() if d_states is not None else None
+        d_final = d_final.contiguous() if d_final is not None else None
+        d_z = torch.empty((batch, length, columns), device=device, dtype=z.dtype)
+        d_initial = torch.empty((batch, width), device=device, dtype=torch.float32) \
+            if context.needs_input_grad[1] else None
+        need = _native.query("koemi_gated_recurrence_workspace_bytes", batch, length, width)
+        workspace = torch.empty(need, device=device, dtype=torch.uint8) if need else None
+        with _native.device_guard(device):
+            _native.call("koemi_gated_recurrence_backward", z.data_ptr(), z.stride(0), z.stride(1),
+                         _native.dtype_code(z.dtype), _native.ptr(mask), kept.data_ptr(), _native.ptr(d_states),
+                         _native.ptr(d_final), d_z.data_ptr(), _native.ptr(d_initial), batch, length, width,
+                         _native.ptr(workspace), need, _native.stream_of(device))
+        return d_z if context.needs_input_grad[0] else None, d_initial, None, None

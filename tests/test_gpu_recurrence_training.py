@@ -1,0 +1,332 @@
+"""The trained recurrence (recurrent.gated_recurrence) against float64.
+
+The reference walks the positions one by one in float64 and lets autograd form
+the gradients. Bounds count roundings: every gate and every step is within EPS of
+its size, and an error made at one step is carried on by the retentions, so the bound
+of a state is EPS times the scan of what each step can add, and likewise for the
+adjoint. EPS = 2^-20 covers sigmoid and tanh of arguments up to 16 (the product with
+log2 e is rounded: 16 units of 2^-24) and the few roundings of a step. A 16-bit
+output adds half a step of its type.
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from koemi_amd import recurrent
+from koemi_amd.dense import DenseCudaValidationError
+
+EPS = 2.0 ** -20
+HALF_STEP = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+# Results below a type's range: half of fp16's smallest step is 2^-25; fp32 (and bf16, which has its range) stops at
+# 2^-126, and a final state's gradient goes below it: 200 retentions of at most 0.9 are 2^-30 on their own, small ones
+# make 10^-62 of it, which float64 holds and fp32 does not.
+SMALLEST = {torch.float32: 2.0 ** -126, torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -126}
+MIN_RETENTION, SPAN = 2.0 ** -8, 1.0 - 2.0 ** -7
+
+
+def gates(z, valid):
+    r, c = z.chunk(2, dim=-1)
+    a = MIN_RETENTION + SPAN * torch.sigmoid(r)
+    b = (1.0 - a) * torch.tanh(c)
+    if valid is not None:
+        a = torch.where(valid[..., None], a, torch.ones_like(a))
+        b = torch.where(valid[..., None], b, torch.zeros_like(b))
+    return a, b
+
+
+def scan(a, b, h):
+    out = []
+    for t in range(a.shape[1]):
+        h = a[:, t] * h + b[:, t]
+        out.append(h)
+    return torch.stack(out, dim=1) if out else b
+
+
+def reference(z, valid, initial, d_states, d_final):
+    """float64: states, final, their gradients, and the bounds of all four."""
+
+    z64 = z.detach().double()
+    if valid is not None:
+        z64 = torch.where(valid[..., None], z64, torch.zeros_like(z64))
+    z64.requires_grad_()
+    h0 = (torch.zeros(z.shape[0], z.shape[2] // 2, device=z.device, dtype=torch.float64) if initial is None
+          else initial.detach().double()).requires_grad_()
+    a, b = gates(z64, valid)
+    states = scan(a, b, h0)
+    final = states[:, -1] if z.shape[1] else h0
+    up = torch.zeros_like(states) if d_states is None else d_states.double()
+    loss = (states * up).sum() + (0.0 if d_final is None else (final * d_final.double()).sum())
+    d_z, d_h0 = torch.autograd.grad(loss, (z64, h0), allow_unused=True)
+    with torch.no_grad():
+        a = a.detach()
+        size = scan(a, b.abs() + 1.0, h0.abs() + 1.0)  # what a state's terms add up to
+        state_bound = 4 * EPS * scan(a, size, h0.abs())
+        back = a.flip(1)
+        after = torch.cat([torch.zeros_like(back[:, :1]), back[:, :-1]], dim=1)
+        first = up.abs().flip(1)
+        if d_final is not None and z.shape[1]:
+            first = torch.cat([first[:, :1] + d_final.double().abs()[:, None], first[:, 1:]], dim=1)
+        zero = torch.zeros_like(h0)
+        g_size = scan(after, first, zero)
+        g_bound = 4 * EPS * scan(after, g_size, zero).flip(1)
+        g_size = g_size.flip(1)
+        grad_bound = torch.cat([g_bound * (size + 1) + g_size * (state_bound + 4 * EPS * (size + 1)),
+                                g_bound + 4 * EPS * g_size], dim=-1)
+        if z.shape[1]:
+            initial_bound = g_bound[:, 0] + 4 * EPS * g_size[:, 0]
+        else:
+            initial_bound = torch.zeros_like(h0)
+    return states, final, d_z, d_h0, state_bound, grad_bound, initial_bound
+
+
+def close(got, want, bound, what):
+    want = want.detach()
+    dtype = got.dtype
+    allowed = bound + HALF_STEP[dtype] * (want.abs() + bound) + SMALLEST[dtype]
+    off = (got.detach().double() - want).abs()
+    assert torch.isfinite(got).all(), what
+    worst = (off - allowed).max().item() if off.numel() else 0.0
+    assert worst <= 0.0, (what, worst, off.max().item())
+
+
+def draw(shape, dtype, seed, mask):
+    batch, length, width = shape
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    z = torch.randn((batch, length, 2 * width), device="cuda", generator=gen) * 2.0
+    valid = None
+    if mask == "random":
+        valid = torch.rand((batch, length), device="cuda", generator=gen) < 0.7
+    elif mask == "none valid":
+        valid = torch.zeros((batch, length), dtype=torch.bool, device="cuda")
+    elif mask == "tail":
+        valid = torch.arange(length, device="cuda")[None] < torch.randint(0, length + 1, (batch, 1), device="cuda", generator=gen)
+    z = z.to(dtype)
+    if valid is not None:  # what a masked position holds does not matter
+        junk = torch.tensor([float("nan"), float("inf"), float("-inf"), torch.finfo(dtype).min], device="cuda", dtype=dtype)
+        z = torch.where(valid[..., None], z, junk[torch.randint(0, 4, z.shape, device="cuda", generator=gen)])
+    initial = torch.randn((batch, width), device="cuda", generator=gen)
+    d_states = torch.randn((batch, length, width), device="cuda", generator=gen).to(dtype)
+    d_final = torch.randn((batch, width), device="cuda", generator=gen)
+    return z, valid, initial, d_states, d_final
+
+
+def check(z, valid, initial, d_states, d_final):
+    z = z.detach().requires_grad_()
+    h0 = initial.detach().requires_grad_() if initial is not None else None
+    states, final = recurrent.gated_recurrence(z, valid, h0)
+    assert states.dtype == z.dtype and final.dtype == torch.float32
+    ups = [(o, d) for o, d in ((states, d_states), (final, d_final)) if d is not None]
+    leaves = (z,) if h0 is None else (z, h0)
+    grads = torch.autograd.grad([o for o, _ in ups], leaves, [d for _, d in ups])
+    want = reference(z, valid, initial, d_states, d_final)
+    close(states, want[0], want[4], "states")
+    close(final, want[1], want[4][:, -1] if z.shape[1] else torch.zeros_like(want[1]), "final")
+    if z.shape[1]:
+        close(grads[0], want[2], want[5], "d_z")
+        if valid is not None:
+            assert (grads[0][~valid] == 0).all()
+    if h0 is not None:
+        close(grads[1], want[3], want[6], "d_initial")
+
+
+SHAPES = [(1, 1, 1), (3, 1, 64), (2, 7, 3), (5, 8, 2), (2, 64, 10), (1, 65, 130), (4, 129, 66), (2, 300, 257), (40, 70, 1026),
+          (1, 4100, 70), (2, 2500, 33)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("mask", [None, "random", "tail", "none valid"])
+def test_states_and_gradients(shape, dtype, mask):
+    check(*draw(shape, dtype, sum(shape), mask))
+
+
+@pytest.mark.gpu
+def test_lengths_of_zero_and_empty_batches():
+    z = torch.empty((3, 0, 8), device="cuda", requires_grad=True)
+    h0 = torch.randn((3, 4), device="cuda", requires_grad=True)
+    states, final = recurrent.gated_recurrence(z, None, h0)
+    assert states.shape == (3, 0, 4) and torch.equal(final, h0)
+    d = torch.randn_like(final)
+    d_z, d_h0 = torch.autograd.grad(final, (z, h0), d)
+    assert d_z.shape == z.shape and torch.equal(d_h0, d)
+    for shape in ((0, 5, 8), (2, 5, 0)):
+        z = torch.empty(shape, device="cuda", requires_grad=True)
+        states, final = recurrent.gated_recurrence(z)
+        assert states.shape == (shape[0], shape[1], shape[2] // 2) and final.numel() == 0
+        (d_z,) = torch.autograd.grad(states.sum() + final.sum(), z)
+        assert d_z.shape == shape
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_layouts_give_the_same_results(dtype):
+    z, valid, initial, d_states, d_final = draw((3, 150, 50), dtype, 5, "random")
+    batch, length, columns = z.shape
+
+    def run(z):
+        z = z.detach().requires_grad_()
+        h0 = initial.clone().requires_grad_()
+        out = recurrent.gated_recurrence(z, valid, h0)
+        return (*out, *torch.autograd.grad(out, (z, h0), (d_states, d_final)))
+
+    want = run(z)
+    wide = torch.full((batch, length, columns + 36), float("nan"), device="cuda", dtype=dtype)
+    wide[..., 4:4 + columns] = z  # a column block of a wider projection
+    turned = z.transpose(0, 1).contiguous().transpose(0, 1)  # position-major storage
+    last = z.transpose(1, 2).contiguous().transpose(1, 2)  # columns apart: copied
+    for other in (wide[..., 4:4 + columns], turned, last):
+        assert not other.is_contiguous()
+        for got, ref in zip(run(other), want):
+            assert torch.equal(got, ref)
+    wide[..., 3:3 + columns] = z  # rows that start between pairs: one column a lane, other lane groups
+    z1 = wide[..., 3:3 + columns]
+    check(z1, valid, initial, d_states, d_final)
+    one = z[:1].expand(batch, length, columns)
+    check(one, valid[:1].expand(batch, length), initial, d_states, d_final)
+
+
+@pytest.mark.gpu
+def test_each_upstream_gradient_alone_and_no_initial_state():
+    z, valid, initial, d_states, d_final = draw((4, 200, 96), torch.float32, 9, "random")
+    check(z, valid, initial, d_states, None)
+    check(z, valid, initial, None, d_final)
+    check(z, valid, None, d_states, d_final)
+    check(z, valid, initial, torch.ones((), device="cuda").expand(4, 200, 96), None)
+    # only the initial state asks for a gradient; nothing does
+    h0 = initial.clone().requires_grad_()
+    states, final = recurrent.gated_recurrence(z, valid, h0)
+    (d_h0,) = torch.autograd.grad(states, h0, d_states)
+    want = reference(z, valid, initial, d_states, None)
+    close(d_h0, want[3], want[6], "d_initial")
+    with torch.no_grad():
+        states, final = recurrent.gated_recurrence(z.detach().requires_grad_(), valid, h0)
+    assert not states.requires_grad and not final.requires_grad
+
+
+@pytest.mark.gpu
+def test_windows_carried_over_equal_one_sequence():
+    z, valid, initial, d_states, d_final = draw((2, 700, 130), torch.float32, 11, "tail")
+    z = z.requires_grad_()
+    h0 = initial.clone().requires_grad_()
+    parts, h = [], h0
+    for t0, t1 in ((0, 1), (1, 257), (257, 700)):
+        s, h = recurrent.gated_recurrence(z[:, t0:t1], valid[:, t0:t1], h)
+        parts.append(s)
+    states = torch.cat(parts, dim=1)
+    grads = torch.autograd.grad((states, h), (z, h0), (d_states, d_final))
+    want = reference(z, valid, initial, d_states, d_final)
+    # a carried state is rounded once more between windows: within the bounds all the same
+    close(states, want[0], want[4], "states")
+    close(grads[0], want[2], want[5], "d_z")
+    close(grads[1], want[3], want[6], "d_initial")
+
+
+@pytest.mark.gpu
+def test_saturated_and_non_finite_gates():
+    big = torch.tensor([-1e30, -200.0, -90.0, -88.0, 88.0, 90.0, 200.0, 1e30, float("inf"), float("-inf")], device="cuda")
+    z = torch.cat([big, torch.zeros_like(big)]).reshape(1, 1, -1).expand(1, 9, -1).contiguous()
+    z[..., big.numel():] = big.flip(0)
+    z.requires_grad_()
+    states, final = recurrent.gated_recurrence(z)
+    (d_z,) = torch.autograd.grad(states, z, torch.ones_like(states))
+    want, _, d_want, _, bound, d_bound, _ = reference(z, None, None, torch.ones_like(states), None)
+    close(states, want, bound, "states")
+    d_want = torch.nan_to_num(d_want, nan=0.0)  # float64 autograd forms inf x 0 at an infinite argument: its limit is 0
+    close(d_z, d_want, d_bound, "d_z")
+    z = torch.zeros((1, 20, 6), device="cuda")
+    z[0, 7, 1], z[0, 9, 5] = float("nan"), float("nan")
+    states, _ = recurrent.gated_recurrence(z)
+    nan = torch.isnan(states[0])
+    assert nan[7:, 1].all() and nan[9:, 2].all() and not nan[:, 0].any() and not nan[:7].any() and not nan[:9, 2].any()
+
+
+@pytest.mark.gpu
+def test_gradients_against_differences():
+    # float32 states of order one carry errors near 1e-6; a central difference of step 2^-6 over a
+    # sum of 2 x 40 x 6 outputs is off by that / 2^-6 plus a third-order term of order 2^-12
+    z, _, initial, d_states, d_final = draw((2, 40, 6), torch.float32, 3, None)
+    z = z / 2
+    z.requires_grad_()
+    h0 = initial.clone().requires_grad_()
+
+    def loss(z, h0):
+        states, final = recurrent.gated_recurrence(z, None, h0)
+        return ((states * d_states).double().sum() + (final * d_final).double().sum())
+
+    d_z, d_h0 = torch.autograd.grad(loss(z, h0), (z, h0))
+    step = 2.0 ** -6
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    for _ in range(4):
+        v = torch.randn(z.shape, device="cuda", generator=gen) / z.numel() ** 0.5
+        w = torch.randn(h0.shape, device="cuda", generator=gen) / h0.numel() ** 0.5
+        with torch.no_grad():
+            slope = (loss(z + step * v, h0 + step * w) - loss(z - step * v, h0 - step * w)) / (2 * step)
+        want = (d_z * v).double().sum() + (d_h0 * w).double().sum()
+        assert abs(slope.item() - want.item()) < 5e-3 * max(1.0, abs(want.item()))
+
+
+@pytest.mark.gpu
+def test_captured_replayed_and_on_another_stream():
+    z, valid, initial, d_states, d_final = draw((2, 1500, 64), torch.bfloat16, 21, "random")
+    z, h0 = z.requires_grad_(), initial.clone().requires_grad_()
+
+    def step():
+        out = recurrent.gated_recurrence(z, valid, h0)
+        return (*out, *torch.autograd.grad(out, (z, h0), (d_states, d_final)))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for seed in (31, 32, 33):
+        new = draw((2, 1500, 64), torch.bfloat16, seed, "random")
+        with torch.no_grad():
+            z.copy_(new[0])
+            valid.copy_(new[1])
+            h0.copy_(new[2])
+            d_states.copy_(new[3])
+            d_final.copy_(new[4])
+        graph.replay()
+        torch.cuda.synchronize()
+        kept = [t.clone() for t in held]
+        for got, want in zip(kept, step()):
+            assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+def test_results_do_not_depend_on_timing():
+    z, valid, initial, d_states, d_final = draw((1, 9000, 200), torch.float32, 2, "random")
+    z, h0 = z.requires_grad_(), initial.clone().requires_grad_()
+    first = None
+    for _ in range(3):
+        out = recurrent.gated_recurrence(z, valid, h0)
+        got = (*out, *torch.autograd.grad(out, (z, h0), (d_states, d_final)))
+        first = first or got
+        assert all(torch.equal(a, b) for a, b in zip(got, first))
+
+
+def test_refusals():
+    z = torch.zeros((2, 3, 8))
+    for bad in (z[0], z.double(), z.long(), None, torch.zeros((2, 3, 7)), z):
+        with pytest.raises(DenseCudaValidationError):
+            recurrent.gated_recurrence(bad)
+
+
+@pytest.mark.gpu
+def test_refusals_on_the_gpu():
+    z = torch.zeros((2, 3, 8), device="cuda")
+    ok = torch.ones((2, 3), dtype=torch.bool, device="cuda")
+    for mask in (ok.float(), ok[:1], ok.cpu(), ok.reshape(-1), [True]):
+        with pytest.raises(DenseCudaValidationError):
+            recurrent.gated_recurrence(z, mask)
+    h0 = torch.zeros((2, 4), device="cuda")
+    for initial in (h0.half(), h0[:1], h0.cpu(), h0.reshape(-1), 0.0):
+        with pytest.raises(DenseCudaValidationError):
+            recurrent.gated_recurrence(z, ok, initial)
