@@ -79,6 +79,16 @@ __device__ __forceinline__ float retention_of(float r) {
     return fmaf(kGateRetentionSpan, gate_sigmoid(r), kGateMinRetention);
 }
 
+// All bits where step i of the mask is valid. Selects by it cost one instruction and no
+// branch, which the compiler puts around a conditional product, spilling what it needs.
+__device__ __forceinline__ uint32_t lane_bits(uint32_t mask, int i) {
+    return static_cast<uint32_t>(static_cast<int32_t>(mask << (31 - i)) >> 31);
+}
+__device__ __forceinline__ float or_zero(float v, uint32_t bits) { return __uint_as_float(__float_as_uint(v) & bits); }
+__device__ __forceinline__ float or_one(float v, uint32_t bits) {
+    return __uint_as_float((__float_as_uint(v) & bits) | (0x3f800000u & ~bits));
+}
+
 // What both directions work on. z: r in the first `width` columns of a row, c in
 // the next; rows z_row elements apart, batch rows z_batch.
 struct Sequence {
@@ -95,7 +105,8 @@ struct Place {
     static constexpr int kColumns = kLanes * VEC;    // columns of a strip
     static constexpr int kChunk = kKeep * LPC;       // steps of a chunk
     int wave, group, lane;       // lane: of its group
-    int64_t b, part, f;          // f: the lane's first column
+    int64_t b, part;
+    uint32_t f;                  // the lane's first column
     bool inside;                 // its columns exist
     uint32_t segment;            // the lane's first step in a chunk
 
@@ -111,7 +122,7 @@ struct Place {
         wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
         group = lane_id() / kLanes;
         lane = lane_id() % kLanes;
-        f = static_cast<int64_t>(strip) * kColumns + lane * VEC;
+        f = strip * kColumns + lane * VEC;
         inside = f < q.width;
         if (!inside) f = 0;
         segment = static_cast<uint32_t>((wave * LPC + group) * kSteps);
@@ -119,31 +130,67 @@ struct Place {
     }
 };
 
-// The steps [t, t + kSteps) of one array's columns; steps past `end` repeat the last.
-// `whole` (uniform): none is.
-template <typename T, int VEC>
-__device__ __forceinline__ void load_steps(Pack<T, VEC> (&o)[kSteps], const T* base, int64_t row, int64_t t, int64_t end,
-                                           bool whole) {
-    if (whole) {
-        const T* p = base + t * row;
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i, p += row) o[i] = *reinterpret_cast<const Pack<T, VEC>*>(p);
-    } else {
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i)
-            o[i] = *reinterpret_cast<const Pack<T, VEC>*>(base + min(t + i, end - 1) * row);
+// The rows of one chunk of an array as a buffer: row t of the array starts at base + t
+// row (elements; base, t0 and end the same for the whole workgroup). Reads past `end`
+// give 0 and writes there are dropped, so that a chunk needs no bounds of its own, and
+// an address is one 32-bit offset (the entry points bound the rows). A chunk that is
+// not there (t0 outside [0, end), or no array) has no rows: its reads give 0 without a
+// branch, which would let the compiler move the loads away from where they stand.
+template <typename T, int VEC, typename P>
+struct Rows {
+    __amdgpu_buffer_rsrc_t buffer;
+    uint32_t step, first;  // bytes
+
+    __device__ __forceinline__ Rows(const T* base, int64_t row, int64_t t0, int64_t end, const P& at) {
+        const int64_t rows = base && t0 >= 0 && t0 < end ? min(end - t0, static_cast<int64_t>(P::kChunk)) : 0;
+        step = static_cast<uint32_t>(row) * static_cast<uint32_t>(sizeof(T));
+        buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base + t0 * row), 0,
+                                                   static_cast<int>(static_cast<uint32_t>(rows) * step), 0x00020000);
+        first = at.segment * step + at.f * static_cast<uint32_t>(sizeof(T));
+        asm volatile("" : "+v"(first));  // the offsets of a step are formed in the chunk: hoisted they cost 24 registers
     }
-}
-// Bit i: step t + i is before `end` and valid.
-__device__ __forceinline__ uint32_t load_mask(const uint8_t* valid, int64_t t, int64_t end) {
-    uint32_t m = 0;
+    __device__ __forceinline__ void load(Pack<T, VEC> (&o)[kSteps]) const {
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-        const bool v = valid == nullptr ? true : valid[min(t + i, end - 1)] != 0;
-        m |= (v && t + i < end) ? 1u << i : 0u;
+        for (int i = 0; i < kSteps; ++i) {
+            const uint32_t off = first + i * step;
+            if constexpr (sizeof(T) * VEC == 2)
+                o[i] = __builtin_bit_cast(Pack<T, VEC>, __builtin_amdgcn_raw_buffer_load_b16(buffer, off, 0, 0));
+            else if constexpr (sizeof(T) * VEC == 4)
+                o[i] = __builtin_bit_cast(Pack<T, VEC>, __builtin_amdgcn_raw_buffer_load_b32(buffer, off, 0, 0));
+            else
+                o[i] = __builtin_bit_cast(Pack<T, VEC>, __builtin_amdgcn_raw_buffer_load_b64(buffer, off, 0, 0));
+        }
     }
-    return m;
-}
+    __device__ __forceinline__ void store(int i, const Pack<T, VEC>& v) const {
+        const uint32_t off = first + i * step;
+        if constexpr (sizeof(T) * VEC == 2)
+            __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, v), buffer, off, 0, 0);
+        else if constexpr (sizeof(T) * VEC == 4)
+            __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v), buffer, off, 0, 0);
+        else {
+            typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+            __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, v), buffer, off, 0, 0);
+        }
+    }
+};
+// The valid bytes of a chunk: each of a group's first eight lanes loads one step's, and
+// the mask (bit i: the lane's step i is before `end` and valid) is formed when they are
+// used, since forming it waits for them.
+template <typename P>
+struct Valid {
+    uint32_t byte, rows;
+
+    __device__ __forceinline__ void load(const uint8_t* valid, int64_t t0, int64_t end, const P& at) {
+        rows = static_cast<uint32_t>(t0 >= 0 && t0 < end ? min(end - t0, static_cast<int64_t>(P::kChunk)) : 0);
+        const __amdgpu_buffer_rsrc_t buffer = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<uint8_t*>(valid + t0), 0, static_cast<int>(valid ? rows : 0), 0x00020000);
+        byte = __builtin_amdgcn_raw_buffer_load_b8(buffer, at.segment + (at.lane & (kSteps - 1)), 0, 0);
+    }
+    __device__ __forceinline__ uint32_t mask(const uint8_t* valid, const P& at) const {
+        const bool ok = (byte != 0 || !valid) && at.segment + (at.lane & (kSteps - 1)) < rows;
+        return static_cast<uint32_t>(__ballot(ok) >> (at.group * P::kLanes)) & ((1u << kSteps) - 1);
+    }
+};
 
 // (p, q) of this lane's group composed with those of the groups before it
 // (REVERSE: after it) in the wave, itself included; before/after alone in (xp, xq).
@@ -183,7 +230,7 @@ __global__ __launch_bounds__(kThreads) void recurrence_forward_kernel(Sequence s
     if (!at.place(s)) return;
     if (FOLD && at.part == s.parts - 1) return;
     const int64_t begin = at.part * s.part_steps, end = min(s.length, begin + s.part_steps);
-    const T* zr = static_cast<const T*>(s.z) + at.b * s.z_batch + at.f;
+    const T* zr = static_cast<const T*>(s.z) + at.b * s.z_batch;
     const T* zc = zr + s.width;
     const uint8_t* valid = s.valid ? s.valid + at.b * s.length : nullptr;
     const int64_t cells = s.batch * s.parts * s.width;
@@ -200,30 +247,36 @@ __global__ __launch_bounds__(kThreads) void recurrence_forward_kernel(Sequence s
     }
     struct Raw {
         Pack<T, VEC> r[kSteps], c[kSteps];
-        uint32_t mask;
+        Valid<P> valid;
     };
     auto fetch = [&](int64_t t0, Raw& o) {
-        const bool whole = t0 + P::kChunk <= end;
-        load_steps(o.r, zr, s.z_row, t0 + at.segment, end, whole);
-        load_steps(o.c, zc, s.z_row, t0 + at.segment, end, whole);
-        o.mask = load_mask(valid, t0 + at.segment, end);
+        Rows<T, VEC, P>(zr, s.z_row, t0, end, at).load(o.r);
+        Rows<T, VEC, P>(zc, s.z_row, t0, end, at).load(o.c);
+        o.valid.load(valid, t0, end, at);
     };
     int turn = 0;
-    auto chunk = [&](const Raw& raw, int64_t t0) {
+    Raw raw;
+    if (begin < end) fetch(begin, raw);
+    for (int64_t t0 = begin; t0 < end; t0 += P::kChunk) {
         float a[kSteps][VEC], b[kSteps][VEC], p[VEC], q[VEC], xp[VEC], xq[VEC];
+        const uint32_t mask = raw.valid.mask(valid, at);
 #pragma unroll
         for (int v = 0; v < VEC; ++v) p[v] = 1.0f, q[v] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i)
+        for (int i = 0; i < kSteps; ++i) {
+            const uint32_t bits = lane_bits(mask, i);
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
                 const Gates g = gates_of<false>(to_f32(raw.r[i].e[v]), to_f32(raw.c[i].e[v]));
-                const bool keep = raw.mask >> i & 1;
-                a[i][v] = keep ? g.a : 1.0f;
-                b[i][v] = keep ? g.k * g.u : 0.0f;
+                a[i][v] = or_one(g.a, bits);
+                b[i][v] = or_zero(g.k * g.u, bits);
                 q[v] = fmaf(a[i][v], q[v], b[i][v]);
                 p[v] *= a[i][v];
             }
+        }
+        // the gates are formed: the next chunk's loads run under the rest, in the same registers
+        __builtin_amdgcn_sched_barrier(0);
+        fetch(t0 + P::kChunk, raw);
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
             scan_groups<LPC, false>(p[v], q[v], xp[v], xq[v], at.group);
@@ -250,7 +303,7 @@ __global__ __launch_bounds__(kThreads) void recurrence_forward_kernel(Sequence s
         }
         turn ^= 1;
         if constexpr (!FOLD) {
-            if (!at.inside) return;
+            if (!at.inside) continue;
             const int64_t t = t0 + at.segment;
             if (kept && t % kKeep == 0 && t < end) {
                 Pack<float, VEC> k;
@@ -258,29 +311,17 @@ __global__ __launch_bounds__(kThreads) void recurrence_forward_kernel(Sequence s
                 for (int v = 0; v < VEC; ++v) k.e[v] = in[v];
                 *reinterpret_cast<Pack<float, VEC>*>(kept + (at.b * kept_rows(s.length) + t / kKeep) * s.width + at.f) = k;
             }
-            T* out = states + (at.b * s.length + t) * s.width + at.f;
+            const Rows<T, VEC, P> out(states + at.b * s.length * s.width, s.width, t0, end, at);
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i, out += s.width) {
+            for (int i = 0; i < kSteps; ++i) {
                 Pack<T, VEC> h;
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) {
                     in[v] = fmaf(a[i][v], in[v], b[i][v]);
                     h.e[v] = from_f32<T>(in[v]);
                 }
-                if (t + i < end) *reinterpret_cast<Pack<T, VEC>*>(out) = h;
+                out.store(i, h);
             }
-        }
-    };
-    if (begin < end) {
-        Raw x, y;
-        fetch(begin, x);
-        for (int64_t t0 = begin;;) {
-            if (t0 + P::kChunk < end) fetch(t0 + P::kChunk, y);
-            chunk(x, t0);
-            if ((t0 += P::kChunk) >= end) break;
-            if (t0 + P::kChunk < end) fetch(t0 + P::kChunk, x);
-            chunk(y, t0);
-            if ((t0 += P::kChunk) >= end) break;
         }
     }
     if (!at.inside || at.wave != 0 || at.group != 0) return;
@@ -308,9 +349,9 @@ __global__ __launch_bounds__(kThreads) void recurrence_backward_kernel(
     if (!at.place(s)) return;
     if (FOLD && at.part == 0) return;
     const int64_t begin = at.part * s.part_steps, end = min(s.length, begin + s.part_steps);
-    const T* zr = static_cast<const T*>(s.z) + at.b * s.z_batch + at.f;
+    const T* zr = static_cast<const T*>(s.z) + at.b * s.z_batch;
     const T* zc = zr + s.width;
-    const T* up = d_states ? d_states + at.b * s.length * s.width + at.f : nullptr;
+    const T* up = d_states ? d_states + at.b * s.length * s.width : nullptr;
     const uint8_t* valid = s.valid ? s.valid + at.b * s.length : nullptr;
     const int64_t cells = s.batch * s.parts * s.width;
     float carry[VEC], prod[VEC];
@@ -327,45 +368,62 @@ __global__ __launch_bounds__(kThreads) void recurrence_backward_kernel(
     struct Raw {
         Pack<T, VEC> r[kSteps], c[kSteps], d[kSteps];
         Pack<float, VEC> h;
-        uint32_t mask;
+        Valid<P> valid;
     };
     auto fetch = [&](int64_t t0, Raw& o) {
-        const bool whole = t0 + P::kChunk <= end;
-        const int64_t t = t0 + at.segment;
-        load_steps(o.r, zr, s.z_row, t, end, whole);
-        if (up) load_steps(o.d, up, s.width, t, end, whole);
+        Rows<T, VEC, P>(zr, s.z_row, t0, end, at).load(o.r);
+        Rows<T, VEC, P>(up, s.width, t0, end, at).load(o.d);
         if constexpr (!FOLD) {
-            load_steps(o.c, zc, s.z_row, t, end, whole);
-            o.h = *reinterpret_cast<const Pack<float, VEC>*>(kept + (at.b * kept_rows(s.length) + t0 / kKeep) * s.width + at.f);
+            Rows<T, VEC, P>(zc, s.z_row, t0, end, at).load(o.c);
+            const int64_t row = at.b * kept_rows(s.length) + max(t0, int64_t(0)) / kKeep;
+            o.h = *reinterpret_cast<const Pack<float, VEC>*>(kept + row * s.width + at.f);
         }
-        o.mask = load_mask(valid, t, end);
+        o.valid.load(valid, t0, end, at);
     };
     int turn = 0;
-    auto chunk = [&](const Raw& raw, int64_t t0) {
-        Gates g[kSteps][VEC];
-        float d[kSteps][VEC], p[VEC], q[VEC], fp[VEC], fq[VEC], xp[VEC], xq[VEC], yp[VEC], yq[VEC];
-        const int64_t t = t0 + at.segment;
+    Raw raw;
+    const int64_t last = begin + (end - begin - 1) / P::kChunk * P::kChunk;
+    if (begin < end) fetch(last, raw);
+    for (int64_t t0 = last; begin < end && t0 >= begin; t0 -= P::kChunk) {
+        // x: an element's increment, then the state before it; cr, cc: what g times
+        // (h_{t-1} - u) and g are multiplied by for dr and dc
+        constexpr int kFull = FOLD ? 1 : kSteps;
+        float a[kSteps][VEC], d[kSteps][VEC], x[kFull][VEC], u[kFull][VEC], cr[kFull][VEC], cc[kFull][VEC];
+        float p[VEC], q[VEC], fp[VEC], fq[VEC], xp[VEC], xq[VEC], yp[VEC], yq[VEC];
+        const uint32_t mask = raw.valid.mask(valid, at);
 #pragma unroll
         for (int v = 0; v < VEC; ++v) p[v] = 1.0f, q[v] = 0.0f, fq[v] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i)
+        for (int i = 0; i < kSteps; ++i) {
+            const uint32_t bits = lane_bits(mask, i);
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
-                const bool keep = raw.mask >> i & 1;
                 if constexpr (FOLD) {
-                    g[i][v].a = keep ? retention_of(to_f32(raw.r[i].e[v])) : 1.0f;
+                    a[i][v] = or_one(retention_of(to_f32(raw.r[i].e[v])), bits);
                 } else {
-                    g[i][v] = gates_of<true>(to_f32(raw.r[i].e[v]), to_f32(raw.c[i].e[v]));
-                    g[i][v].a = keep ? g[i][v].a : 1.0f;
-                    fq[v] = fmaf(g[i][v].a, fq[v], keep ? g[i][v].k * g[i][v].u : 0.0f);
+                    const Gates g = gates_of<true>(to_f32(raw.r[i].e[v]), to_f32(raw.c[i].e[v]));
+                    a[i][v] = or_one(g.a, bits);
+                    x[i][v] = or_zero(g.k * g.u, bits);
+                    u[i][v] = g.u;
+                    cr[i][v] = kGateRetentionSpan * g.ds;
+                    cc[i][v] = g.k * g.du;
+                    fq[v] = fmaf(a[i][v], fq[v], x[i][v]);
                 }
-                p[v] *= g[i][v].a;
-                d[i][v] = up && t + i < end ? to_f32(raw.d[i].e[v]) : 0.0f;
+                p[v] *= a[i][v];
+                d[i][v] = to_f32(raw.d[i].e[v]);
             }
+        }
+        float start[VEC];
+        if constexpr (!FOLD)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) start[v] = raw.h.e[v];
+        // the gates are formed: the next chunk's loads run under the rest, in the same registers
+        __builtin_amdgcn_sched_barrier(0);
+        fetch(t0 - P::kChunk, raw);
 #pragma unroll
         for (int i = kSteps - 1; i >= 0; --i)
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) q[v] = g[i][v].a * (d[i][v] + q[v]);
+            for (int v = 0; v < VEC; ++v) q[v] = a[i][v] * (d[i][v] + q[v]);
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
             fp[v] = p[v];
@@ -377,23 +435,23 @@ __global__ __launch_bounds__(kThreads) void recurrence_backward_kernel(
             }
             if (!FOLD && at.group == LPC - 1) wave_h[turn][at.wave][at.lane * VEC + v] = fq[v];
         }
-        __syncthreads();
+        __syncthreads();  // the other buffer's readers are past it: they have written this one
         float in[VEC], h[VEC];
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
-            float x = carry[v];
-            in[v] = x;
-            float y = FOLD ? 0.0f : raw.h.e[v];
+            float c = carry[v];
+            in[v] = c;
+            float y = FOLD ? 0.0f : start[v];
             h[v] = y;
             float wp[kWaves];
 #pragma unroll
             for (int w = kWaves - 1; w >= 0; --w) {
-                if (w == at.wave) in[v] = x;
+                if (w == at.wave) in[v] = c;
                 wp[w] = wave_p[turn][w][at.lane * VEC + v];
-                x = fmaf(wp[w], x, wave_q[turn][w][at.lane * VEC + v]);
+                c = fmaf(wp[w], c, wave_q[turn][w][at.lane * VEC + v]);
                 if constexpr (FOLD) prod[v] *= wp[w];
             }
-            carry[v] = x;
+            carry[v] = c;
             if constexpr (!FOLD) {
 #pragma unroll
                 for (int w = 0; w < kWaves - 1; ++w) {
@@ -406,46 +464,31 @@ __global__ __launch_bounds__(kThreads) void recurrence_backward_kernel(
         }
         turn ^= 1;
         if constexpr (!FOLD) {
-            if (!at.inside) return;
-            float before[kSteps][VEC];
+            if (!at.inside) continue;
 #pragma unroll
             for (int i = 0; i < kSteps; ++i)
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) {
-                    before[i][v] = h[v];
-                    h[v] = fmaf(g[i][v].a, h[v], raw.mask >> i & 1 ? g[i][v].k * g[i][v].u : 0.0f);
+                    const float next = fmaf(a[i][v], h[v], x[i][v]);
+                    x[i][v] = h[v];
+                    h[v] = next;
                 }
-            T* out = d_z + (at.b * s.length + t) * 2 * s.width + at.f;
+            T* out = d_z + at.b * s.length * 2 * s.width;
+            const Rows<T, VEC, P> out_r(out, 2 * s.width, t0, end, at), out_c(out + s.width, 2 * s.width, t0, end, at);
 #pragma unroll
             for (int i = kSteps - 1; i >= 0; --i) {
                 Pack<T, VEC> dr, dc;
-                const bool keep = raw.mask >> i & 1;
+                const uint32_t bits = lane_bits(mask, i);
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) {
-                    const Gates& w = g[i][v];
-                    const float gt = d[i][v] + in[v];
-                    in[v] = w.a * gt;
-                    dr.e[v] = from_f32<T>(keep ? gt * (before[i][v] - w.u) * (kGateRetentionSpan * w.ds) : 0.0f);
-                    dc.e[v] = from_f32<T>(keep ? gt * (w.k * w.du) : 0.0f);
+                    const float g = d[i][v] + in[v];
+                    in[v] = a[i][v] * g;
+                    dr.e[v] = from_f32<T>(or_zero(g * (x[i][v] - u[i][v]) * cr[i][v], bits));
+                    dc.e[v] = from_f32<T>(or_zero(g * cc[i][v], bits));
                 }
-                if (t + i < end) {
-                    *reinterpret_cast<Pack<T, VEC>*>(out + i * 2 * s.width) = dr;
-                    *reinterpret_cast<Pack<T, VEC>*>(out + i * 2 * s.width + s.width) = dc;
-                }
+                out_r.store(i, dr);
+                out_c.store(i, dc);
             }
-        }
-    };
-    if (begin < end) {
-        Raw x, y;
-        int64_t t0 = begin + (end - begin - 1) / P::kChunk * P::kChunk;
-        fetch(t0, x);
-        for (;;) {
-            if (t0 > begin) fetch(t0 - P::kChunk, y);
-            chunk(x, t0);
-            if ((t0 -= P::kChunk) < begin) break;
-            if (t0 > begin) fetch(t0 - P::kChunk, x);
-            chunk(y, t0);
-            if ((t0 -= P::kChunk) < begin) break;
         }
     }
     if (!at.inside || at.wave != 0 || at.group != 0) return;
@@ -509,27 +552,32 @@ int check_sequence(const char* what, const void* z, int64_t z_batch, int64_t z_r
     if (cells > (static_cast<__int128>(1) << 60)) return fail(KOEMI_ERR_INVALID, "%s: too many elements", what);
     if (static_cast<__int128>(batch) * width > (int64_t(1) << 30))
         return fail(KOEMI_ERR_UNSUPPORTED, "%s: batch x width above 2^30", what);
+    // offsets inside a chunk of four lane groups of kKeep rows have 32 bits
+    const int64_t row = std::max<int64_t>(length > 1 ? z_row : 0, 2 * width);
+    if (row > (int64_t(1) << 32) / (4 * kKeep * 4) - 1)
+        return fail(KOEMI_ERR_UNSUPPORTED, "%s: rows of more than 2^22 elements", what);
     return KOEMI_OK;
 }
 
 unsigned grid_of(const Sequence& s) { return static_cast<unsigned>((s.batch * s.parts * s.strips + 7) / 8 * 8); }
 
-// Calls run(std::integral_constant VEC, LPC) of the plan.
-template <typename Run>
+// Calls run(std::integral_constant VEC, LPC) of the plan; MOST: columns of a lane at most.
+template <int MOST, typename Run>
 void by_plan(const Plan& p, Run run) {
     auto lanes = [&](auto vec) {
         if (p.lpc == 1) run(vec, std::integral_constant<int, 1>{});
         else if (p.lpc == 2) run(vec, std::integral_constant<int, 2>{});
         else run(vec, std::integral_constant<int, 4>{});
     };
-    if (p.vec == 2) lanes(std::integral_constant<int, 2>{});
-    else lanes(std::integral_constant<int, 1>{});
+    if constexpr (MOST >= 2)
+        if (p.vec == 2) return lanes(std::integral_constant<int, 2>{});
+    lanes(std::integral_constant<int, 1>{});
 }
 
 template <typename T>
 int forward(Sequence s, const Plan& p, const float* initial, void* states, float* final_state, float* kept, float* maps,
             hipStream_t stream) {
-    by_plan(p, [&](auto vec, auto lpc) {
+    by_plan<2>(p, [&](auto vec, auto lpc) {
         constexpr int V = decltype(vec)::value, C = decltype(lpc)::value;
         if (s.parts > 1)
             hipLaunchKernelGGL((recurrence_forward_kernel<T, V, C, true>), dim3(grid_of(s)), dim3(kThreads), 0, stream, s,
@@ -542,7 +590,7 @@ int forward(Sequence s, const Plan& p, const float* initial, void* states, float
 template <typename T>
 int backward(Sequence s, const Plan& p, const float* kept, const void* d_states, const float* d_final, void* d_z,
              float* d_initial, float* maps, hipStream_t stream) {
-    by_plan(p, [&](auto vec, auto lpc) {
+    by_plan<std::is_same<T, float>::value ? 1 : 2>(p, [&](auto vec, auto lpc) {
         constexpr int V = decltype(vec)::value, C = decltype(lpc)::value;
         if (s.parts > 1)
             hipLaunchKernelGGL((recurrence_backward_kernel<T, V, C, true>), dim3(grid_of(s)), dim3(kThreads), 0, stream, s,
@@ -601,8 +649,9 @@ extern "C" int koemi_gated_recurrence_backward(const void* preactivations, int64
     const int st = check_sequence(what, preactivations, batch_stride, row_stride, dtype, batch, length, width);
     if (st != KOEMI_OK || batch == 0 || width == 0) return st;
     if (length > 0 && (!kept || !grad_preactivations)) return fail(KOEMI_ERR_INVALID, "%s: null pointer", what);
-    const bool pairs =
-        pairs_fit(preactivations, batch_stride, row_stride, width, dtype, grad_states, grad_preactivations, kept);
+    // fp32 takes one column a lane: two spill ([1, 32768, 512] 101 us against 81; bf16 [8, 2048, 1024] 57 with one, 47 with two)
+    const bool pairs = dtype != KOEMI_F32 && pairs_fit(preactivations, batch_stride, row_stride, width, dtype, grad_states,
+                                                       grad_preactivations, kept);
     const Plan p = plan_of(batch, length, width, pairs ? 2 : 1);
     const size_t need = maps_bytes(p, batch, width);
     if (need && (!workspace || workspace_bytes < need)) return fail(KOEMI_ERR_INVALID, "%s: workspace too small", what);

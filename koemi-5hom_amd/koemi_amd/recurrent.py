@@ -14,6 +14,8 @@ from stacked gate pre-activations, with the gradients of both.
 
 from __future__ import annotations
 
+from functools import lru_cache
+
 import torch
 from torch import Tensor
 from torch.autograd.function import once_differentiable
@@ -407,8 +409,8 @@ def gated_recurrence(preactivations: Tensor, valid_mask: Tensor | None = None,
     if initial is not None and (not isinstance(initial, Tensor) or initial.shape != (batch, width)
                                 or initial.dtype != torch.float32 or initial.device != device):
         raise DenseCudaValidationError("initial must be a float32 [batch, width] tensor on the same device")
-    if batch * width > 1 << 30:
-        raise DenseCudaValidationError("batch x width must not exceed 2^30")
+    if batch * width > 1 << 30 or width >= 1 << 20:
+        raise DenseCudaValidationError("width must be below 2^20 and batch x width at most 2^30")
     try:
         _native.load_library()
     except _native.NativeLibraryUnavailableError as error:
@@ -417,11 +419,19 @@ def gated_recurrence(preactivations: Tensor, valid_mask: Tensor | None = None,
     return _GatedRecurrence.apply(preactivations, initial, valid_mask, trained)
 
 
+@lru_cache(maxsize=256)
+def _recurrence_sizes(batch: int, length: int, width: int) -> tuple[int, int]:
+    """(rows of the kept states, bytes of workspace) of a shape."""
+
+    return (_native.query("koemi_gated_recurrence_kept_rows", length),
+            _native.query("koemi_gated_recurrence_workspace_bytes", batch, length, width))
+
+
 def _in_place(z: Tensor) -> Tensor:
     """``z`` where a kernel can read its rows as they lie, else a contiguous copy."""
 
     batch, length, columns = z.shape
-    fits = (columns <= 1 or z.stride(2) == 1) and (length <= 1 or z.stride(1) >= columns) and z.stride(0) >= 0
+    fits = (columns <= 1 or z.stride(2) == 1) and (length <= 1 or columns <= z.stride(1) < 1 << 21)
     return z if fits else z.contiguous()
 
 
@@ -436,11 +446,8 @@ class _GatedRecurrence(torch.autograd.Function):
         mask = valid_mask.contiguous() if valid_mask is not None else None
         states = torch.empty((batch, length, width), device=device, dtype=z.dtype)
         final = torch.empty((batch, width), device=device, dtype=torch.float32)
-        kept = None
-        if trained:
-            rows = _native.query("koemi_gated_recurrence_kept_rows", length)
-            kept = torch.empty((batch, rows, width), device=device, dtype=torch.float32)
-        need = _native.query("koemi_gated_recurrence_workspace_bytes", batch, length, width)
+        rows, need = _recurrence_sizes(batch, length, width)
+        kept = torch.empty((batch, rows, width), device=device, dtype=torch.float32) if trained else None
         workspace = torch.empty(need, device=device, dtype=torch.uint8) if need else None
         with _native.device_guard(device):
             _native.call("koemi_gated_recurrence_forward", z.data_ptr(), z.stride(0), z.stride(1),
@@ -465,7 +472,7 @@ class _GatedRecurrence(torch.autograd.Function):
         d_z = torch.empty((batch, length, columns), device=device, dtype=z.dtype)
         d_initial = torch.empty((batch, width), device=device, dtype=torch.float32) \
             if context.needs_input_grad[1] else None
-        need = _native.query("koemi_gated_recurrence_workspace_bytes", batch, length, width)
+        _, need = _recurrence_sizes(batch, length, width)
         workspace = torch.empty(need, device=device, dtype=torch.uint8) if need else None
         with _native.device_guard(device):
             _native.call("koemi_gated_recurrence_backward", z.data_ptr(), z.stride(0), z.stride(1),
