@@ -939,6 +939,39 @@ int koemi_gated_recurrence_backward(const void* preactivations, int64_t batch_st
                                     int64_t batch, int64_t length, int64_t width, void* workspace,
                                     size_t workspace_bytes, koemi_stream_t stream);
 
+/* LearnedExpertMixture.forward's route and RouterStatistics (model/router.py:11-22,
+ * 43-59), to be trained. router_logits F32, F16 or BF16, rows row_stride elements
+ * apart, expert_count <= 1024. assignments [tokens, top_k] are the experts of the
+ * top_k largest logits in descending order (ties to the lower expert) and weights
+ * their softmax probabilities; -1 and 0 for an invalid token, and for an expert whose
+ * logit is minus infinity: it is never chosen, and a token with no other logit counts
+ * as invalid. probability_mass, assignment_counts [expert_count], valid_count [1] and
+ * balance_loss [1] as koemi_moe_route_learned_stats. Sums run in a fixed order.
+ * Workspace: koemi_moe_route_balanced_workspace_bytes bytes, no zeroing needed. */
+size_t koemi_moe_route_balanced_workspace_bytes(int64_t tokens, int64_t expert_count);
+int koemi_moe_route_balanced_forward(const void* router_logits, int dtype, int64_t row_stride,
+                                     const uint8_t* valid_mask, int64_t* assignments, float* weights,
+                                     float* probability_mass, float* assignment_counts, float* valid_count,
+                                     float* balance_loss, int64_t tokens, int64_t expert_count, int64_t top_k,
+                                     void* workspace, size_t workspace_bytes, koemi_stream_t stream);
+
+/* The gradient of the logits (grad_logits [tokens, expert_count] contiguous, in
+ * their type; 0 for tokens that are not routed) from those of the weights [tokens,
+ * top_k], the mass [expert_count] and the loss [1] (each NULL: zero). The counts are
+ * constants, as in the reference. */
+int koemi_moe_route_balanced_backward(const void* router_logits, int dtype, int64_t row_stride,
+                                      const uint8_t* valid_mask, const int64_t* assignments,
+                                      const float* assignment_counts, const float* valid_count,
+                                      const float* grad_weights, const float* grad_mass, const float* grad_loss,
+                                      void* grad_logits, int64_t tokens, int64_t expert_count, int64_t top_k,
+                                      koemi_stream_t stream);
+
+/* The gradient of koemi_moe_router_balance_loss by the mass:
+ * grad_loss E counts_e / (max(valid, 1) max(sum counts, 1)). */
+int koemi_moe_router_balance_loss_backward(const float* assignment_counts, const float* valid_count,
+                                           const float* grad_loss, int64_t expert_count, float* grad_mass,
+                                           koemi_stream_t stream);
+
 /* Measurement only (no counterpart in the reference): reads `bytes` (a
  * multiple of 16) from `src` with `grid` workgroups of `block` threads, each
  * thread issuing `unroll` (1, 2, 4 or 8) 16-byte loads per pass of a

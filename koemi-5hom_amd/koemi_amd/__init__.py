@@ -27,6 +27,7 @@ from koemi_amd.moe import (
     grouped_expert_mlp_inference,
     load_native_extension,
     permute_topk,
+    route_topk_balanced,
     route_topk_learned,
     route_topk_modulo,
     route_topk_valid,
@@ -48,6 +49,7 @@ __all__ = [
     "load_native_extension",
     "native_cuda_available",
     "permute_topk",
+    "route_topk_balanced",
     "route_topk_learned",
     "route_topk_modulo",
     "route_topk_valid",

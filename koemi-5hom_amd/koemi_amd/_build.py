@@ -32,6 +32,7 @@ SOURCES = (
     "surprise.hip",
     "surprise_head.hip",
     "moe_route.hip",
+    "route_balanced.hip",
     "moe_permute.hip",
     "moe_grouped_mlp.hip",
     "moe_combine.hip",

@@ -17,16 +17,20 @@ Build-side keyword-only extensions (absent from the reference signatures):
 * ``route_topk_learned`` — softmax top-k gate of router.py:46-49, with
   ``return_statistics=True`` also its ``RouterStatistics`` (router.py:11-22,
   50-58; ``merge_router_statistics`` router.py:25-32);
-* ``expert_activation_counts`` — per-expert counts of network.py:48-70.
+* ``expert_activation_counts`` — per-expert counts of network.py:48-70;
+* ``route_topk_balanced`` — the learned gate to be trained: its weights, probability
+  mass and balance loss with the gradient of the logits.
 """
 
 from __future__ import annotations
 
 from dataclasses import dataclass, field
+from functools import lru_cache
 from typing import Any
 
 import torch
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 from koemi_amd import _native
 
@@ -41,6 +45,7 @@ __all__ = [
     "load_native_extension",
     "merge_router_statistics",
     "permute_topk",
+    "route_topk_balanced",
     "route_topk_learned",
     "route_topk_valid",
     "weights_to_fragments",
@@ -239,7 +244,8 @@ class RouterStatistics:
     ``balance_loss`` (0-dim fp32 device tensor) is
     ``E * sum((mass / max(valid, 1)) * (counts / max(sum(counts), 1)))``, formed
     on the device (``koemi_moe_router_balance_loss``) unless the route kernel
-    already formed it."""
+    already formed it; where ``probability_mass`` carries a gradient
+    (``route_topk_balanced``, merged or not), so does the loss."""
 
     probability_mass: Tensor
     assignment_counts: Tensor
@@ -261,11 +267,35 @@ class RouterStatistics:
         if mass.ndim != 1 or counts.shape != mass.shape or mass.numel() < 1:
             raise CudaMoeValidationError("probability_mass and assignment_counts must be [expert_count]")
         _require_library()
-        loss = torch.empty((), device=mass.device, dtype=torch.float32)
-        with _native.device_guard(mass.device):
-            _native.call("koemi_moe_router_balance_loss", mass.data_ptr(), counts.data_ptr(), valid.data_ptr(),
-                         mass.numel(), loss.data_ptr(), _native.stream_of(mass.device))
-        return loss
+        if torch.is_grad_enabled() and mass.requires_grad:
+            return _BalanceLoss.apply(mass, counts, valid)
+        return _balance_loss(mass, counts, valid)
+
+
+def _balance_loss(mass: Tensor, counts: Tensor, valid: Tensor) -> Tensor:
+    loss = torch.empty((), device=mass.device, dtype=torch.float32)
+    with _native.device_guard(mass.device):
+        _native.call("koemi_moe_router_balance_loss", mass.data_ptr(), counts.data_ptr(), valid.data_ptr(),
+                     mass.numel(), loss.data_ptr(), _native.stream_of(mass.device))
+    return loss
+
+
+class _BalanceLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(context, mass: Tensor, counts: Tensor, valid: Tensor) -> Tensor:  # type: ignore[override]
+        context.save_for_backward(counts, valid)
+        return _balance_loss(mass, counts, valid)
+
+    @staticmethod
+    @once_differentiable
+    def backward(context, d_loss: Tensor):  # type: ignore[override]
+        counts, valid = context.saved_tensors
+        d_mass = torch.empty_like(counts)
+        with _native.device_guard(counts.device):
+            _native.call("koemi_moe_router_balance_loss_backward", counts.data_ptr(), valid.data_ptr(),
+                         d_loss.contiguous().data_ptr(), counts.numel(), d_mass.data_ptr(),
+                         _native.stream_of(counts.device))
+        return d_mass, None, None
 
 
 def merge_router_statistics(statistics: list[RouterStatistics]) -> RouterStatistics | None:
@@ -339,6 +369,94 @@ def route_topk_learned(router_logits: Tensor, valid_mask: Tensor, *, top_k: int,
                 _native.stream_of(router_logits.device),
             )
     return assignments.reshape(shape), weights.reshape(shape)
+
+
+def route_topk_balanced(router_logits: Tensor, valid_mask: Tensor, *, top_k: int
+                        ) -> tuple[Tensor, Tensor, RouterStatistics]:
+    """The learned softmax top-k gate of router.py:43-59 with first-order autograd.
+
+    ``router_logits`` ``[..., E]`` float32, float16 or bfloat16 (any strides; E at
+    most 1024), ``valid_mask`` bool of the leading shape. Returns int64 assignments
+    and float32 weights of shape ``[..., top_k]`` and the ``RouterStatistics``: the
+    experts of the ``top_k`` largest logits in descending order (ties to the lower
+    index) with their softmax probabilities, -1 and 0 for an invalid token. An expert
+    whose logit is minus infinity is never chosen (its slot is -1, its weight 0), and
+    a token with no other logit counts as invalid.
+
+    The weights, ``probability_mass`` and ``balance_loss`` are differentiable by the
+    logits; the choices and ``assignment_counts`` are constants, as in the
+    reference. Probabilities and sums are float32, in a fixed order."""
+
+    if not isinstance(router_logits, Tensor) or not isinstance(valid_mask, Tensor):
+        raise TypeError("router_logits and valid_mask must be torch.Tensors")
+    for name, tensor in (("router_logits", router_logits), ("valid_mask", valid_mask)):
+        if not tensor.is_cuda:
+            raise CudaMoeValidationError(f"{name} must be a CUDA tensor")
+    _require_same_cuda_device({"router_logits": router_logits, "valid_mask": valid_mask})
+    _require_supported_context_dtype(router_logits, "router_logits")
+    if router_logits.ndim < 1 or valid_mask.shape != router_logits.shape[:-1]:
+        raise CudaMoeValidationError("valid_mask must match router_logits.shape[:-1]")
+    if valid_mask.dtype != torch.bool:
+        raise CudaMoeValidationError("valid_mask must use boolean dtype")
+    expert_count = _require_positive_bounded(int(router_logits.shape[-1]), "expert_count", 1024)
+    top_k = _require_positive_bounded(top_k, "top_k", 1024)
+    if top_k > expert_count:
+        raise CudaMoeValidationError("top_k must not exceed expert_count")
+    _require_library()
+    assignments, weights, mass, counts, valid_count, loss = _RouteBalanced.apply(router_logits, valid_mask, top_k)
+    return assignments, weights, RouterStatistics(mass, counts, valid_count, loss)
+
+
+@lru_cache(maxsize=256)
+def _size(name: str, *shape: int) -> int:
+    """A workspace query of the library, kept by its arguments."""
+
+    return _native.query(name, *shape)
+
+
+class _RouteBalanced(torch.autograd.Function):
+    @staticmethod
+    def forward(context, router_logits: Tensor, valid_mask: Tensor, top_k: int):  # type: ignore[override]
+        experts, device = router_logits.shape[-1], router_logits.device
+        logits = router_logits.reshape(-1, experts)
+        tokens = logits.shape[0]
+        if logits.stride(1) != 1 or (tokens > 1 and logits.stride(0) < experts):
+            logits = logits.contiguous()
+        valid = valid_mask.contiguous()
+        assignments = torch.empty((*valid_mask.shape, top_k), device=device, dtype=torch.int64)
+        weights = torch.empty(assignments.shape, device=device, dtype=torch.float32)
+        mass = torch.empty((experts,), device=device, dtype=torch.float32)
+        counts = torch.empty((experts,), device=device, dtype=torch.float32)
+        valid_count = torch.empty((), device=device, dtype=torch.float32)
+        loss = torch.empty((), device=device, dtype=torch.float32)
+        need = _size("koemi_moe_route_balanced_workspace_bytes", tokens, experts)
+        workspace = torch.empty((need,), device=device, dtype=torch.uint8)
+        with _native.device_guard(device):
+            _native.call("koemi_moe_route_balanced_forward", logits.data_ptr(), _native.dtype_code(logits.dtype),
+                         logits.stride(0), valid.data_ptr(), assignments.data_ptr(), weights.data_ptr(), mass.data_ptr(),
+                         counts.data_ptr(), valid_count.data_ptr(), loss.data_ptr(), tokens, experts, top_k,
+                         workspace.data_ptr(), need, _native.stream_of(device))
+        context.mark_non_differentiable(assignments, counts, valid_count)
+        context.set_materialize_grads(False)
+        context.save_for_backward(logits, valid, assignments, counts, valid_count)
+        context.shape = router_logits.shape
+        return assignments, weights, mass, counts, valid_count, loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(context, _a, d_weights, d_mass, _c, _v, d_loss):  # type: ignore[override]
+        if d_weights is None and d_mass is None and d_loss is None:
+            return None, None, None
+        logits, valid, assignments, counts, valid_count = context.saved_tensors
+        (tokens, experts), device = logits.shape, logits.device
+        d_logits = torch.empty(context.shape, device=device, dtype=logits.dtype)
+        d_weights, d_mass, d_loss = (d.contiguous() if d is not None else None for d in (d_weights, d_mass, d_loss))
+        with _native.device_guard(device):
+            _native.call("koemi_moe_route_balanced_backward", logits.data_ptr(), _native.dtype_code(logits.dtype),
+                         logits.stride(0), valid.data_ptr(), assignments.data_ptr(), counts.data_ptr(),
+                         valid_count.data_ptr(), _native.ptr(d_weights), _native.ptr(d_mass), _native.ptr(d_loss),
+                         d_logits.data_ptr(), tokens, experts, assignments.shape[-1], _native.stream_of(device))
+        return d_logits, None, None
 
 
 def expert_activation_counts(assignments: Tensor, valid_mask: Tensor, *, expert_count: int) -> Tensor:
