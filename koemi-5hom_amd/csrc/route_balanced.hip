@@ -9,13 +9,13 @@
 // (model/router.py:11-22, 43-59 of the reference and its autograd; the counts are
 // constants there too.) A token lies on a group of 1 to 64 lanes, each with 4, 8 or 16
 // consecutive logits in registers: one read of the logits a direction, the softmax and
-// each of the k choices by butterflies over the group. Experts at minus infinity are
+// each of the k choices by reductions over the group. Experts at minus infinity are
 // never chosen (the slot is -1, its weight 0), and a token with no other is not routed
 // at all, like one that is not valid.
 //
-// A lane always holds the same experts, so the statistics add up in its registers over
+// A lane always holds the same experts, so the mass adds up in its registers over
 // the workgroup's tokens, then over its groups through LDS, then over the workgroups in
-// a second launch: every order is fixed. Bound by memory for many experts, by the two
+// a second launch: every order is fixed (the counts are whole numbers). Bound by memory for many experts, by the two
 // launches' latency for a few tokens.
 #include "common.hpp"
 
@@ -41,13 +41,47 @@ __device__ __forceinline__ float exp_nonpos(float x) {
     return fmaf(e, lo * 0.693147180559945309f, e);
 }
 
-// Ordered like the value it comes from, +0 and -0 alike; never 0, which stands for "not to be chosen".
-__device__ __forceinline__ uint32_t order_key(float v) {
-    const uint32_t b = __float_as_uint(v + 0.0f);
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
+// The other lanes of a reduction over aligned groups of lanes: mirrored within 2, 4,
+// 8 and 16 lanes by data-parallel moves (a mirror pairs the halves as a butterfly does, once
+// each half agrees), then by permutes.
+template <int SPAN>
+__device__ __forceinline__ uint32_t across(uint32_t v) {
+    if constexpr (SPAN == 2) return __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xf, 0xf, true);        // quad_perm 1 0 3 2
+    else if constexpr (SPAN == 4) return __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xf, 0xf, true);   // quad_perm 2 3 0 1
+    else if constexpr (SPAN == 8) return __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, true);  // row_half_mirror
+    else if constexpr (SPAN == 16) return __builtin_amdgcn_update_dpp(0, v, 0x140, 0xf, 0xf, true); // row_mirror
+    else return static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), SPAN / 2, kWave));
 }
+// v combined over the group's G lanes, the same bits in each.
+template <int G, int SPAN = 2, typename V, typename Op>
+__device__ __forceinline__ V over_group(V v, Op op) {
+    if constexpr (SPAN <= G) return over_group<G, SPAN * 2>(op(v, __builtin_bit_cast(V, across<SPAN>(__builtin_bit_cast(uint32_t, v)))), op);
+    else return v;
+}
+
+// A logit's place in the order of choices: greater for a larger logit (+0 and -0
+// alike), 0 for one that is not to be chosen. For 16-bit logits the low half holds the
+// expert, greater for a lower one, so that the largest key names it.
+template <typename T>
+__device__ __forceinline__ uint32_t choice_key(float v, int e) {
+    if (v == -__builtin_inff()) return 0u;
+    v += 0.0f;
+    if constexpr (sizeof(T) == 2) {
+        const uint32_t b = __builtin_bit_cast(uint16_t, from_f32<T>(v));
+        return ((b & 0x8000u ? ~b : b | 0x8000u) & 0xffffu) << 16 | static_cast<uint32_t>(0xffff - e);
+    } else {
+        const uint32_t b = __float_as_uint(v);
+        return b & 0x80000000u ? ~b : b | 0x80000000u;
+    }
+}
+template <typename T>
 __device__ __forceinline__ float key_value(uint32_t k) {
-    return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+    if constexpr (sizeof(T) == 2) {
+        k >>= 16;
+        return to_f32(__builtin_bit_cast(T, static_cast<uint16_t>(k & 0x8000u ? k & 0x7fffu : ~k)));
+    } else {
+        return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+    }
 }
 
 // The layout of a token: G lanes of VPL experts each.
@@ -60,10 +94,10 @@ struct Token {
     // are read one by one; minus infinity past the experts.
     __device__ __forceinline__ void load(const T* row, int e0, int experts, bool vec) {
         if (vec) {
-            struct alignas(sizeof(T) * VPL > 16 ? 16 : sizeof(T) * VPL) Raw {
-                T v[VPL];
-            };
             if (e0 < experts) {
+                struct alignas(sizeof(T) * VPL > 16 ? 16 : sizeof(T) * VPL) Raw {
+                    T v[VPL];
+                };
                 const Raw r = *reinterpret_cast<const Raw*>(row + e0);
 #pragma unroll
                 for (int v = 0; v < VPL; ++v) z[v] = to_f32(r.v[v]);
@@ -76,33 +110,29 @@ struct Token {
             for (int v = 0; v < VPL; ++v) z[v] = e0 + v < experts ? to_f32(row[e0 + v]) : -__builtin_inff();
         }
     }
-    // p over the group (NaN where a logit is NaN or plus infinity); false: no logit above
-    // minus infinity, p is 0.
-    __device__ __forceinline__ bool softmax(float (&p)[VPL]) const {
+    // p over the group (NaN where a logit is NaN or plus infinity), e^(z - most) times
+    // scale; false: no logit above minus infinity, p is 0.
+    float most, scale;
+    __device__ __forceinline__ bool softmax(float (&p)[VPL]) {
         float m = z[0];
-        bool any = false;
+        uint32_t any = 0;
 #pragma unroll
         for (int v = 0; v < VPL; ++v) {
             m = fmaxf(m, z[v]);
             any |= z[v] != -__builtin_inff();
         }
-        uint32_t some = any;
-#pragma unroll
-        for (int off = G / 2; off > 0; off >>= 1) {
-            m = fmaxf(m, __shfl_xor(m, off, kWave));
-            some |= __shfl_xor(some, off, kWave);
-        }
+        most = over_group<G>(m, [](float a, float b) { return fmaxf(a, b); });
+        any = over_group<G>(any, [](uint32_t a, uint32_t b) { return a | b; });
         float sum = 0.0f;
 #pragma unroll
         for (int v = 0; v < VPL; ++v) {
-            p[v] = exp_nonpos(z[v] - m);
+            p[v] = exp_nonpos(z[v] - most);
             sum += p[v];
         }
+        scale = 1.0f / over_group<G>(sum, [](float a, float b) { return a + b; });
 #pragma unroll
-        for (int off = G / 2; off > 0; off >>= 1) sum += __shfl_xor(sum, off, kWave);
-#pragma unroll
-        for (int v = 0; v < VPL; ++v) p[v] = some ? p[v] / sum : 0.0f;
-        return some != 0;
+        for (int v = 0; v < VPL; ++v) p[v] = any ? p[v] * scale : 0.0f;
+        return any != 0;
     }
 };
 
@@ -113,13 +143,15 @@ __global__ __launch_bounds__(kThreads) void route_balanced_kernel(
     uint32_t* __restrict__ part_counts, uint32_t* __restrict__ part_valid) {
     using K = Token<T, G, VPL>;
     __shared__ float mass_sh[kThreads * VPL];
-    __shared__ uint32_t counts_sh[kThreads * VPL];
+    __shared__ uint32_t counts_sh[G * VPL];
     __shared__ uint32_t valid_sh[kThreads / kWave];
     const int tid = threadIdx.x, lane = tid % G, group = tid / G, e0 = lane * VPL;
     float mass[VPL];
-    uint32_t counts[VPL], routed_tokens = 0;
+    uint32_t routed_tokens = 0;
 #pragma unroll
-    for (int v = 0; v < VPL; ++v) mass[v] = 0.0f, counts[v] = 0;
+    for (int v = 0; v < VPL; ++v) mass[v] = 0.0f;
+    for (int e = tid; e < G * VPL; e += kThreads) counts_sh[e] = 0;
+    __syncthreads();
     for (int64_t first = static_cast<int64_t>(blockIdx.x) * K::kPerBlock; first < tokens;
          first += static_cast<int64_t>(gridDim.x) * K::kPerBlock) {
         const int64_t t = first + group;
@@ -135,42 +167,37 @@ __global__ __launch_bounds__(kThreads) void route_balanced_kernel(
 #pragma unroll
         for (int v = 0; v < VPL; ++v) {
             mass[v] += p[v];
-            key[v] = token.z[v] == -__builtin_inff() ? 0u : order_key(token.z[v]);
+            key[v] = choice_key<T>(token.z[v], e0 + v);
         }
         routed_tokens += routed && lane == 0;
-        // the k choices: each lane's best, then the group's; lane s % G keeps choice s
+        // the k choices: the largest key of the group; lane s % G keeps choice s
         int64_t my_idx = -1;
-        float my_w = 0.0f;
+        uint32_t my_key = 0;
         for (int s = 0; s < top_k; ++s) {
-            uint32_t best = key[0];
-            int at = 0;
+            uint32_t top = key[0];
 #pragma unroll
-            for (int v = 1; v < VPL; ++v)
-                if (key[v] > best) best = key[v], at = v;
-            uint64_t top = static_cast<uint64_t>(best) << 32 | static_cast<uint32_t>(~(e0 + at));
+            for (int v = 1; v < VPL; ++v) top = max(top, key[v]);
+            top = over_group<G>(top, [](uint32_t a, uint32_t b) { return max(a, b); });
+            uint32_t e;
+            if constexpr (sizeof(T) == 2) {
+                e = 0xffffu - (top & 0xffffu);
+            } else {  // the lowest expert that has it
+                e = ~0u;
 #pragma unroll
-            for (int off = G / 2; off > 0; off >>= 1) {
-                const uint32_t hi = __shfl_xor(static_cast<uint32_t>(top >> 32), off, kWave);
-                const uint32_t lo = __shfl_xor(static_cast<uint32_t>(top), off, kWave);
-                const uint64_t other = static_cast<uint64_t>(hi) << 32 | lo;
-                top = other > top ? other : top;
+                for (int v = VPL - 1; v >= 0; --v) e = key[v] == top ? e0 + v : e;
+                e = over_group<G>(e, [](uint32_t a, uint32_t b) { return min(a, b); });
             }
-            const bool chosen = (top >> 32) != 0;
-            const int e = static_cast<int>(~static_cast<uint32_t>(top));
-            float w = 0.0f;
 #pragma unroll
-            for (int v = 0; v < VPL; ++v) {
-                const bool mine = chosen && e == e0 + v;
-                key[v] = mine ? 0u : key[v];
-                counts[v] += mine;
-                w = mine ? p[v] : w;
+            for (int v = 0; v < VPL; ++v) key[v] = e == static_cast<uint32_t>(e0 + v) ? 0u : key[v];
+            if (s % G == lane) {
+                my_key = top;
+                my_idx = top ? static_cast<int64_t>(e) : -1;
+                if (top) atomicAdd(&counts_sh[e], 1u);  // whole numbers: any order
             }
-            if constexpr (G > 1) w = __shfl(w, (lane_id() & ~(G - 1)) + (chosen ? e / VPL : 0), kWave);
-            if (s % G == lane) my_idx = chosen ? e : -1, my_w = chosen ? w : 0.0f;
             if ((s % G == G - 1 || s == top_k - 1) && t < tokens && lane <= s % G) {
                 const int64_t o = t * top_k + (s - s % G + lane);
                 out_idx[o] = my_idx;
-                out_w[o] = my_w;
+                out_w[o] = my_key ? exp_nonpos(key_value<T>(my_key) - token.most) * token.scale : 0.0f;
             }
         }
     }
@@ -178,17 +205,13 @@ __global__ __launch_bounds__(kThreads) void route_balanced_kernel(
     for (int off = kWave / 2; off > 0; off >>= 1) routed_tokens += __shfl_xor(routed_tokens, off, kWave);
     if (lane_id() == 0) valid_sh[tid / kWave] = routed_tokens;
 #pragma unroll
-    for (int v = 0; v < VPL; ++v) {
-        mass_sh[group * (G * VPL) + e0 + v] = mass[v];
-        counts_sh[group * (G * VPL) + e0 + v] = counts[v];
-    }
+    for (int v = 0; v < VPL; ++v) mass_sh[group * (G * VPL) + e0 + v] = mass[v];
     __syncthreads();
     for (int e = tid; e < experts; e += kThreads) {
         float m = 0.0f;
-        uint32_t c = 0;
-        for (int g = 0; g < K::kPerBlock; ++g) m += mass_sh[g * (G * VPL) + e], c += counts_sh[g * (G * VPL) + e];
+        for (int g = 0; g < K::kPerBlock; ++g) m += mass_sh[g * (G * VPL) + e];
         part_mass[static_cast<int64_t>(blockIdx.x) * experts + e] = m;
-        part_counts[static_cast<int64_t>(blockIdx.x) * experts + e] = c;
+        part_counts[static_cast<int64_t>(blockIdx.x) * experts + e] = counts_sh[e];
     }
     if (tid == 0) {
         uint32_t n = 0;
@@ -225,7 +248,7 @@ __global__ __launch_bounds__(kFinishThreads) void route_balanced_finish_kernel(
     float m = 0.0f;
     uint32_t c = 0, n = 0;
     if (e < experts)
-#pragma unroll 4
+#pragma unroll 8
         for (int b = slice; b < blocks; b += slices) {
             m += part_mass[static_cast<int64_t>(b) * experts + e];
             c += part_counts[static_cast<int64_t>(b) * experts + e];
@@ -292,16 +315,15 @@ __global__ __launch_bounds__(kThreads) void route_balanced_backward_kernel(
         for (int v = 0; v < VPL; ++v) g[v] = base[v];
         if (grad_w)
             for (int s = 0; s < top_k; ++s) {
-                const int64_t e = idx[tc * top_k + s];
+                const int e = static_cast<int>(idx[tc * top_k + s]);
                 const float d = grad_w[tc * top_k + s];
 #pragma unroll
                 for (int v = 0; v < VPL; ++v) g[v] += e == e0 + v ? d : 0.0f;
             }
         float dot = 0.0f;
 #pragma unroll
-        for (int v = 0; v < VPL; ++v) dot += e0 + v < experts ? p[v] * g[v] : 0.0f;
-#pragma unroll
-        for (int off = G / 2; off > 0; off >>= 1) dot += __shfl_xor(dot, off, kWave);
+        for (int v = 0; v < VPL; ++v) dot += p[v] * g[v];  // past the experts p is 0
+        dot = over_group<G>(dot, [](float a, float b) { return a + b; });
         if (t >= tokens) continue;
         T* out = grad_logits + t * experts + e0;
         struct alignas(sizeof(T) * VPL > 16 ? 16 : sizeof(T) * VPL) Raw {
@@ -328,13 +350,15 @@ __global__ __launch_bounds__(kThreads) void balance_loss_backward_kernel(const f
     for (int64_t e = threadIdx.x; e < experts; e += kThreads) grad_mass[e] = scale * counts[e];
 }
 
-// Lanes of a token: the fewest that hold its experts, 4 each up to 256 experts, then 8 and 16.
+// Lanes of a token: the fewest that hold its experts, 4 each up to 32 experts, 8 up to
+// 64, else 16: fewer lanes reduce in fewer steps, more give small calls more waves
+// ([131072, 128] bf16 with top 4: 107 us with 32 lanes of 4).
 struct Layout {
     int lanes, per_lane, blocks;
 };
 inline Layout layout_of(int64_t tokens, int64_t experts) {
     Layout l;
-    l.per_lane = experts <= 256 ? 4 : experts <= 512 ? 8 : 16;
+    l.per_lane = experts <= 32 ? 4 : experts <= 64 ? 8 : 16;
     for (l.lanes = 1; l.lanes * l.per_lane < experts; l.lanes *= 2) {
     }
     const int64_t per_block = kThreads / l.lanes;
@@ -343,18 +367,21 @@ inline Layout layout_of(int64_t tokens, int64_t experts) {
 }
 template <typename Run>
 void by_layout(const Layout& l, Run run) {
-    auto wide = [&](auto per) { run(std::integral_constant<int, 64>{}, per); };
-    if (l.per_lane == 16) return wide(std::integral_constant<int, 16>{});
-    if (l.per_lane == 8) return wide(std::integral_constant<int, 8>{});
     const std::integral_constant<int, 4> four;
+    const std::integral_constant<int, 16> sixteen;
+    const std::integral_constant<int, 8> eight;
+    if (l.per_lane == 4) switch (l.lanes) {
+            case 1: return run(std::integral_constant<int, 1>{}, four);
+            case 2: return run(std::integral_constant<int, 2>{}, four);
+            case 4: return run(std::integral_constant<int, 4>{}, four);
+            default: return run(eight, four);
+        }
+    if (l.per_lane == 8) return run(eight, eight);
     switch (l.lanes) {
-        case 1: return run(std::integral_constant<int, 1>{}, four);
-        case 2: return run(std::integral_constant<int, 2>{}, four);
-        case 4: return run(std::integral_constant<int, 4>{}, four);
-        case 8: return run(std::integral_constant<int, 8>{}, four);
-        case 16: return run(std::integral_constant<int, 16>{}, four);
-        case 32: return run(std::integral_constant<int, 32>{}, four);
-        default: return run(std::integral_constant<int, 64>{}, four);
+        case 8: return run(eight, sixteen);
+        case 16: return run(sixteen, sixteen);
+        case 32: return run(std::integral_constant<int, 32>{}, sixteen);
+        default: return run(std::integral_constant<int, 64>{}, sixteen);
     }
 }
 inline bool rows_vector(const void* base, int64_t stride, int64_t experts, int per_lane, int size) {
