@@ -972,6 +972,42 @@ int koemi_moe_router_balance_loss_backward(const float* assignment_counts, const
                                            const float* grad_loss, int64_t expert_count, float* grad_mass,
                                            koemi_stream_t stream);
 
+/* The experts' gated feed-forward of every routed pair, weighted and summed per
+ * token, to be trained (LearnedExpertMixture.combine, model/router.py:61-97, before
+ * its normalizer, and its autograd): output[t] = sum over the token's pairs of w
+ * (W_o (silu(W_g x + b_g) (W_v x + b_v)) + b_o). context, output [tokens, width] and
+ * the parameters (gate and value weights [E, hidden, width], output weights [E, width,
+ * hidden], biases [E, hidden], [E, hidden], [E, width]) in one type, F32, F16 or BF16.
+ * The pairs come from koemi_moe_permute_indices (sorted_rows, sorted_experts,
+ * segment_offsets, pair_positions); pair_weights [tokens, top_k] fp32 in token order
+ * (NULL: 1 / top_k). Pairs past the valid ones count nothing, a token without any gets
+ * zeros. saved (NULL: no gradients wanted) keeps koemi_moe_experts_saved_bytes for the
+ * backward. Workspace: koemi_moe_experts_workspace_bytes, no zeroing needed. */
+size_t koemi_moe_experts_saved_bytes(int64_t tokens, int64_t top_k, int64_t width, int64_t hidden,
+                                     int64_t expert_count, int dtype);
+size_t koemi_moe_experts_workspace_bytes(int64_t tokens, int64_t top_k, int64_t width, int64_t hidden,
+                                         int64_t expert_count, int dtype, int backward);
+int koemi_moe_experts_forward(const void* context, const int64_t* sorted_rows, const int64_t* segment_offsets,
+                              const int64_t* pair_positions, const float* pair_weights, const void* gate_weights,
+                              const void* gate_biases, const void* value_weights, const void* value_biases,
+                              const void* output_weights, const void* output_biases, void* output, void* saved,
+                              int64_t tokens, int64_t top_k, int64_t width, int64_t hidden, int64_t expert_count,
+                              int dtype, void* workspace, size_t workspace_bytes, koemi_stream_t stream);
+
+/* Its gradients, each NULL where not wanted: of the context, of the pair weights (fp32,
+ * token order, 0 for pairs past the valid ones) and of the six parameters (zeros for an
+ * expert without pairs). sorted_weights: the pair weights in sorted order (NULL: 1 /
+ * top_k); the other arguments as the forward had them. Sums run in a fixed order. */
+int koemi_moe_experts_backward(const void* grad_output, const void* context, const int64_t* sorted_rows,
+                               const int64_t* sorted_experts, const int64_t* segment_offsets,
+                               const int64_t* pair_positions, const float* sorted_weights, const void* gate_weights,
+                               const void* value_weights, const void* output_weights, const void* output_biases,
+                               const void* saved, void* grad_context, float* grad_pair_weights,
+                               void* grad_gate_weights, void* grad_gate_biases, void* grad_value_weights,
+                               void* grad_value_biases, void* grad_output_weights, void* grad_output_biases,
+                               int64_t tokens, int64_t top_k, int64_t width, int64_t hidden, int64_t expert_count,
+                               int dtype, void* workspace, size_t workspace_bytes, koemi_stream_t stream);
+
 /* Measurement only (no counterpart in the reference): reads `bytes` (a
  * multiple of 16) from `src` with `grid` workgroups of `block` threads, each
  * thread issuing `unroll` (1, 2, 4 or 8) 16-byte loads per pass of a

@@ -1,0 +1,767 @@
+// The experts' gated feed-forward of every routed pair, weighted and summed per token,
+// with its gradients.
+//
+//   g = W_g x + b_g, v = W_v x + b_v, h = silu(g) v, y = W_o h + b_o of each pair's expert
+//   out_t = sum_s w_ts y_ts
+//   d' = W_o^T dout_t (not weighted), dw = <d', h> + <dout_t, b_o>,
+//   dv = w d' silu(g), dg = w d' v s (1 + g (1 - s)), s = sigmoid(g),
+//   dx_t = sum_s W_g^T dg + W_v^T dv,
+//   dW_g = sum dg x^T, dW_v = sum dv x^T, dW_o = sum dout (w h)^T, db_g = sum dg,
+//   db_v = sum dv, db_o = sum w dout  (sums over the expert's pairs)
+//
+// (LearnedExpertMixture.combine, model/router.py:61-97 of the reference, before its
+// normalizer, and what its autograd forms.) dw needs no y: it is the row sum of d' h, and
+// the weighted products take the weight on h's side, so that dout enters them as it came.
+//
+// The pairs of an expert are consecutive rows of the sorted order, so each product is
+// a grouped matrix product: six in all, two of them (W_g and W_v) doubled. The forward
+// keeps g and v in fp32: what dw is made of would otherwise be as inexact as 16-bit
+// values are, and forming them again would cost two of the products.
+//
+// Any type, width and alignment runs on the tiles of split_gemm.hpp, which read an
+// operand either along K or across it; what lies between two products stays fp32 there.
+#include "common.hpp"
+#include "split_gemm.hpp"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace koemi {
+namespace {
+
+using split_gemm::acc_column;
+
+inline size_t align256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
+__host__ __device__ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+inline int64_t padded_hidden(int64_t hidden) { return (hidden + 7) / 8 * 8; }  // rows of whole 32-byte octets
+
+// sigmoid and 1 - sigmoid, each to fp32's relative precision; the exponential stays
+// finite, NaN stays NaN.
+__device__ __forceinline__ void sigmoid_pair(float g, float& s, float& rest) {
+    const float x = g * -1.44269504088896341f;
+    const float e = __builtin_amdgcn_exp2f(x > 126.0f ? 126.0f : x);
+    s = __builtin_amdgcn_rcpf(1.0f + e);
+    rest = e * s;
+}
+__device__ __forceinline__ float glu(float g, float v) {
+    float s, rest;
+    sigmoid_pair(g, s, rest);
+    return g * s * v;
+}
+// From d' of one hidden unit: dg, dv, w h, and what it adds to dw.
+struct GluGradient {
+    float dg, dv, wh, dw;
+};
+__device__ __forceinline__ GluGradient glu_gradient(float g, float v, float d, float w) {
+    float s, rest;
+    sigmoid_pair(g, s, rest);
+    const float silu = g * s, wd = w * d;
+    GluGradient o;
+    o.dw = d * (silu * v);
+    o.dg = wd * v * (s * fmaf(g, rest, 1.0f));
+    o.dv = wd * silu;
+    o.wh = w * (silu * v);
+    return o;
+}
+
+// ------------------------------------------------------------------- slots ---
+// A slot is up to `rows` consecutive pairs of one expert. expert[count] holds the
+// number of slots in use; first[e] the first slot of expert e (experts + 1 of them).
+struct Slots {
+    int32_t* expert;
+    int32_t* first;
+    int64_t* row;
+    int64_t* end;
+};
+constexpr int kSlotThreads = 1024;
+
+__global__ __launch_bounds__(kSlotThreads) void slots_kernel(const int64_t* __restrict__ offsets, int64_t experts,
+                                                             int64_t pairs, int64_t rows, int64_t max_slots, Slots s) {
+    __shared__ int32_t wave_tot[kSlotThreads / kWave];
+    int32_t before = 0;
+    for (int64_t e0 = 0; e0 < experts; e0 += kSlotThreads) {
+        const int64_t e = e0 + threadIdx.x;
+        int64_t lo = 0, hi = 0;
+        if (e < experts) {
+            lo = min(max(offsets[e], int64_t(0)), pairs);
+            hi = min(max(offsets[e + 1], lo), pairs);
+        }
+        const int32_t n = static_cast<int32_t>((hi - lo + rows - 1) / rows);
+        int32_t total;
+        const int32_t at = before + block_exclusive_scan<kSlotThreads>(n, wave_tot, total);
+        if (e < experts) s.first[e] = at;
+        for (int32_t i = 0; i < n && at + i < max_slots; ++i) {
+            s.expert[at + i] = static_cast<int32_t>(e);
+            s.row[at + i] = lo + i * rows;
+            s.end[at + i] = hi;
+        }
+        before += total;
+    }
+    if (threadIdx.x == 0) {
+        s.first[experts] = before;
+        s.expert[max_slots] = static_cast<int32_t>(min(static_cast<int64_t>(before), max_slots));
+    }
+}
+
+// The (slot, column tile) of a workgroup, or false: workgroup b runs on XCD b % 8, and each
+// XCD takes a contiguous range of tiles in groups of kGroup slots, so that tiles that
+// run at once share operands in its L2.
+constexpr uint32_t kGroup = 4;
+__device__ __forceinline__ bool slot_tile(const Slots& s, int64_t max_slots, uint32_t n_tiles, uint32_t& slot,
+                                          uint32_t& tile_n) {
+    const uint32_t slots = static_cast<uint32_t>(s.expert[max_slots]), tiles = slots * n_tiles, per = (tiles + 7) / 8;
+    const uint32_t i = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if ((blockIdx.x >> 3) >= per || i >= tiles) return false;
+    const uint32_t group = kGroup * n_tiles, first = i / group * kGroup, width = min(kGroup, slots - first);
+    slot = first + i % group % width;
+    tile_n = i % group / width;
+    return true;
+}
+
+// --------------------------------------------------- any type and any shape ---
+constexpr int kAnyCols = 128;
+// Rows of a tile: 64 where the experts' segments are mostly shorter than a tile of 128.
+inline int any_rows(int64_t pairs, int64_t experts) { return pairs <= 96 * experts ? 64 : 128; }
+
+// g, v (fp32, kept where wanted) and h (fp32) of a slot's pairs x 64 hidden units; rows
+// are ld apart, zeros from `hidden` on. B rows 0-63 of the tile are W_g's, 64-127 W_v's.
+template <typename T, int BM, int BYTES>
+__global__ __launch_bounds__(split_gemm::kThreads, 2) void any_hidden_kernel(
+    const T* __restrict__ x, const int64_t* __restrict__ rows, int64_t tokens, const T* __restrict__ Wg,
+    const T* __restrict__ bg, const T* __restrict__ Wv, const T* __restrict__ bv, float* __restrict__ keep_g,
+    float* __restrict__ keep_v, float* __restrict__ h, Slots slots, int64_t max_slots, int64_t width, int64_t hidden,
+    int64_t ld, uint32_t n_tiles) {
+    using G = split_gemm::Tile<T, T, BM, kAnyCols>;
+    __shared__ __attribute__((aligned(16))) char lds[G::kLdsBytes];
+    uint32_t slot, tile_n;
+    if (!slot_tile(slots, max_slots, n_tiles, slot, tile_n)) return;
+    const int e = slots.expert[slot];
+    const int64_t row0 = slots.row[slot], end = slots.end[slot], n0 = static_cast<int64_t>(tile_n) * 64;
+    const int wave = threadIdx.x / kWave, wm = wave >> 1, wn = wave & 1;
+    const T* w0 = Wg + e * hidden * width;
+    const T* w1 = Wv + e * hidden * width;
+    auto a_row = [&](int r) { return x + min(max(rows[min(row0 + r, end - 1)], int64_t(0)), tokens - 1) * width; };
+    G tile;
+    uint64_t chains = tile.template run<BYTES, BYTES>(
+        lds, width, width, 0, ceil_div(width, G::BK) * G::BK, a_row,
+        [&](int r) { return (r < 64 ? w0 : w1) + min(n0 + (r & 63), hidden - 1) * width; },
+        [&](int t) { return t * 64 + wn * 32; });
+    if constexpr (G::kNative) split_gemm::lds_barrier();
+    constexpr int kRegion = split_gemm::store_bytes<float, 1>();
+    static_assert(4 * kRegion <= G::kLdsBytes, "the output regions fit the operands' LDS");
+    const int64_t first = n0 + wn * 32;
+    float b0[16], b1[16];
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+        const int64_t c = e * hidden + min(first + acc_column(v), hidden - 1);
+        b0[v] = to_f32(bg[c]);
+        b1[v] = to_f32(bv[c]);
+    }
+#pragma unroll
+    for (int i = 0; i < G::MT; ++i) {
+        const int64_t r = row0 + wm * (BM / 2) + i * 32;
+        float og[1][16], ov[1][16], oh[1][16];
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+            const bool in = first + acc_column(v) < hidden;
+            og[0][v] = in ? tile.acc[i][0][v] + b0[v] : 0.0f;
+            ov[0][v] = in ? tile.acc[i][G::NT - 1][v] + b1[v] : 0.0f;
+            oh[0][v] = glu(og[0][v], ov[0][v]);
+        }
+        char* region = lds + wave * kRegion;
+        if (keep_g) {
+            split_gemm::store_rows<float, 1>(region, og, keep_g + r * ld + first, ld, end - r, ld - first, true);
+            split_gemm::store_rows<float, 1>(region, ov, keep_v + r * ld + first, ld, end - r, ld - first, true);
+        }
+        split_gemm::store_rows<float, 1>(region, oh, h + r * ld + first, ld, end - r, ld - first, true);
+    }
+    if constexpr (!G::kNative) {
+        chains |= chains >> 16 | chains << 16;
+        split_gemm::fix_chains(chains, [&](int block, int v) {
+            if (block % G::NT != 0) return;
+            const int64_t r = wm * (BM / 2) + block / G::NT * 32 + (lane_id() & 31), c = first + acc_column(v);
+            if (row0 + r >= end || c >= hidden) return;
+            const float g = split_gemm::scalar_dot(a_row(static_cast<int>(r)), w0 + c * width, width, to_f32(bg[e * hidden + c]));
+            const float u = split_gemm::scalar_dot(a_row(static_cast<int>(r)), w1 + c * width, width, to_f32(bv[e * hidden + c]));
+            const int64_t o = (row0 + r) * ld + c;
+            if (keep_g) keep_g[o] = g, keep_v[o] = u;
+            h[o] = glu(g, u);
+        });
+    }
+}
+
+// y = W_o h + b_o of a slot's pairs x 128 columns, fp32.
+template <typename T, int BM, int BYTES>
+__global__ __launch_bounds__(split_gemm::kThreads, 2) void any_output_kernel(
+    const float* __restrict__ h, const T* __restrict__ Wo, const T* __restrict__ bo, float* __restrict__ y, Slots slots,
+    int64_t max_slots, int64_t width, int64_t hidden, int64_t ld, uint32_t n_tiles) {
+    using G = split_gemm::Tile<float, T, BM, kAnyCols>;
+    __shared__ __attribute__((aligned(16))) char lds[G::kLdsBytes];
+    uint32_t slot, tile_n;
+    if (!slot_tile(slots, max_slots, n_tiles, slot, tile_n)) return;
+    const int e = slots.expert[slot];
+    const int64_t row0 = slots.row[slot], end = slots.end[slot], n0 = static_cast<int64_t>(tile_n) * kAnyCols;
+    const int wave = threadIdx.x / kWave, wm = wave >> 1, wn = wave & 1;
+    const T* w = Wo + e * width * hidden;
+    G tile;
+    const uint64_t chains = tile.template run<16, BYTES>(
+        lds, ld, hidden, 0, ceil_div(hidden, G::BK) * G::BK, [&](int r) { return h + min(row0 + r, end - 1) * ld; },
+        [&](int r) { return w + min(n0 + r, width - 1) * hidden; }, [&](int t) { return wn * 64 + t * 32; });
+    constexpr int kRegion = split_gemm::store_bytes<float, 1>();
+    const int64_t first = n0 + wn * 64;
+#pragma unroll
+    for (int j = 0; j < G::NT; ++j)
+#pragma unroll
+        for (int i = 0; i < G::MT; ++i) {
+            const int64_t r = row0 + wm * (BM / 2) + i * 32, c = first + j * 32;
+            float o[1][16];
+#pragma unroll
+            for (int v = 0; v < 16; ++v)
+                o[0][v] = tile.acc[i][j][v] + to_f32(bo[e * width + min(c + acc_column(v), width - 1)]);
+            split_gemm::store_rows<float, 1>(lds + wave * kRegion, o, y + r * width + c, width, end - r, width - c, width % 8 == 0);
+        }
+    split_gemm::fix_chains(chains, [&](int block, int v) {
+        const int64_t r = row0 + wm * (BM / 2) + block / G::NT * 32 + (lane_id() & 31);
+        const int64_t c = first + block % G::NT * 32 + acc_column(v);
+        if (r >= end || c >= width) return;
+        y[r * width + c] = split_gemm::scalar_dot(h + r * ld, w + c * hidden, hidden, to_f32(bo[e * width + c]));
+    });
+}
+
+// d' = W_o^T dout of a slot's pairs x 128 hidden units and what follows from it: dg, dv
+// and w h (fp32, rows ld apart, zeros from `hidden` on), and each row's part of dw from
+// a wave's 64 units: dw_part[(2 tile + wave column) pairs + row].
+template <typename T, int BM, int BYTES>
+__global__ __launch_bounds__(split_gemm::kThreads, 2) void any_hidden_gradient_kernel(
+    const T* __restrict__ d_out, const int64_t* __restrict__ rows, int64_t tokens, const T* __restrict__ Wo,
+    const float* __restrict__ keep_g, const float* __restrict__ keep_v, const float* __restrict__ sorted_w, float share,
+    float* __restrict__ dg, float* __restrict__ dv, float* __restrict__ wh, float* __restrict__ dw_part, Slots slots,
+    int64_t max_slots, int64_t pairs, int64_t width, int64_t hidden, int64_t ld, uint32_t n_tiles) {
+    using G = split_gemm::Tile<T, T, BM, kAnyCols, false, true>;
+    __shared__ __attribute__((aligned(16))) char lds[G::kLdsBytes];
+    uint32_t slot, tile_n;
+    if (!slot_tile(slots, max_slots, n_tiles, slot, tile_n)) return;
+    const int e = slots.expert[slot];
+    const int64_t row0 = slots.row[slot], end = slots.end[slot], n0 = static_cast<int64_t>(tile_n) * kAnyCols;
+    const int wave = threadIdx.x / kWave, wm = wave >> 1, wn = wave & 1;
+    const T* w = Wo + e * width * hidden;
+    auto a_row = [&](int r) { return d_out + min(max(rows[min(row0 + r, end - 1)], int64_t(0)), tokens - 1) * width; };
+    G tile;
+    const uint64_t chains = tile.template run<BYTES, 16>(
+        lds, width, width, 0, ceil_div(width, G::BK) * G::BK, a_row, [&](int r) { return w + min(n0 + r, hidden - 1); },
+        [&](int t) { return wn * 64 + t * 32; }, 1, hidden);
+    if constexpr (G::kNative) split_gemm::lds_barrier();
+    constexpr int kRegion = split_gemm::store_bytes<float, 1>();
+    static_assert(4 * kRegion <= G::kLdsBytes, "the output regions fit the operands' LDS");
+    char* region = lds + wave * kRegion;
+    const int64_t first = n0 + wn * 64;
+    float* part = dw_part + (2 * static_cast<int64_t>(tile_n) + wn) * pairs;
+#pragma unroll
+    for (int i = 0; i < G::MT; ++i) {
+        const int64_t r = row0 + wm * (BM / 2) + i * 32, mine = min(r + (lane_id() & 31), end - 1);
+        const float weight = sorted_w ? sorted_w[mine] : share;
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < G::NT; ++j) {
+            const int64_t c = first + j * 32;
+            float a[1][16], b[1][16], h[1][16];
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                const int64_t at = min(c + acc_column(v), hidden - 1);
+                float d = tile.acc[i][j][v];
+                if constexpr (!G::kNative)
+                    if (__builtin_expect(chains >> ((i * G::NT + j) * 16 + v) & 1, 0))
+                        d = split_gemm::scalar_dot(a_row(static_cast<int>(mine - row0)), w + at, width, 0.0f, 1, hidden);
+                const GluGradient o = glu_gradient(keep_g[mine * ld + at], keep_v[mine * ld + at], d, weight);
+                const bool in = c + acc_column(v) < hidden;
+                a[0][v] = in ? o.dg : 0.0f;
+                b[0][v] = in ? o.dv : 0.0f;
+                h[0][v] = in ? o.wh : 0.0f;
+                sum += in ? o.dw : 0.0f;
+            }
+            split_gemm::store_rows<float, 1>(region, a, dg + r * ld + c, ld, end - r, ld - c, true);
+            split_gemm::store_rows<float, 1>(region, b, dv + r * ld + c, ld, end - r, ld - c, true);
+            split_gemm::store_rows<float, 1>(region, h, wh + r * ld + c, ld, end - r, ld - c, true);
+        }
+        sum += __shfl_xor(sum, 32, kWave);
+        if (lane_id() < 32 && r + lane_id() < end) part[r + lane_id()] = sum;
+    }
+}
+
+// dx of a slot's pairs x 128 columns: dg W_g + dv W_v, fp32.
+template <typename T, int BM>
+__global__ __launch_bounds__(split_gemm::kThreads, 2) void any_input_gradient_kernel(
+    const float* __restrict__ dg, const float* __restrict__ dv, const T* __restrict__ Wg, const T* __restrict__ Wv,
+    float* __restrict__ dx, Slots slots, int64_t max_slots, int64_t width, int64_t hidden, int64_t ld, uint32_t n_tiles) {
+    using G = split_gemm::Tile<float, T, BM, kAnyCols, false, true>;
+    __shared__ __attribute__((aligned(16))) char lds[G::kLdsBytes];
+    uint32_t slot, tile_n;
+    if (!slot_tile(slots, max_slots, n_tiles, slot, tile_n)) return;
+    const int e = slots.expert[slot];
+    const int64_t row0 = slots.row[slot], end = slots.end[slot], n0 = static_cast<int64_t>(tile_n) * kAnyCols;
+    const int wave = threadIdx.x / kWave, wm = wave >> 1, wn = wave & 1;
+    split_gemm::f32x16 sum[G::MT][G::NT];
+    uint64_t chains = 0;
+    G tile;
+    for (int half = 0; half < 2; ++half) {
+        const float* a = half ? dv : dg;
+        const T* w = (half ? Wv : Wg) + e * hidden * width;
+        chains |= tile.template run<16, 16>(
+            lds, ld, hidden, 0, ceil_div(hidden, G::BK) * G::BK, [&](int r) { return a + min(row0 + r, end - 1) * ld; },
+            [&](int r) { return w + min(n0 + r, width - 1); }, [&](int t) { return wn * 64 + t * 32; }, 1, width);
+#pragma unroll
+        for (int i = 0; i < G::MT; ++i)
+#pragma unroll
+            for (int j = 0; j < G::NT; ++j) sum[i][j] = half ? sum[i][j] + tile.acc[i][j] : tile.acc[i][j];
+    }
+    constexpr int kRegion = split_gemm::store_bytes<float, 1>();
+    const int64_t first = n0 + wn * 64;
+#pragma unroll
+    for (int j = 0; j < G::NT; ++j)
+#pragma unroll
+        for (int i = 0; i < G::MT; ++i) {
+            const int64_t r = row0 + wm * (BM / 2) + i * 32, c = first + j * 32;
+            float o[1][16];
+#pragma unroll
+            for (int v = 0; v < 16; ++v) o[0][v] = sum[i][j][v];
+            split_gemm::store_rows<float, 1>(lds + wave * kRegion, o, dx + r * width + c, width, end - r, width - c, width % 8 == 0);
+        }
+    split_gemm::fix_chains(chains, [&](int block, int v) {
+        const int64_t r = row0 + wm * (BM / 2) + block / G::NT * 32 + (lane_id() & 31);
+        const int64_t c = first + block % G::NT * 32 + acc_column(v);
+        if (r >= end || c >= width) return;
+        const float part = split_gemm::scalar_dot(dg + r * ld, Wg + e * hidden * width + c, hidden, 0.0f, 1, width);
+        dx[r * width + c] = split_gemm::scalar_dot(dv + r * ld, Wv + e * hidden * width + c, hidden, part, 1, width);
+    });
+}
+
+// One expert's C[m, n] = sum over its pairs of A[pair, m] B[pair, n] (rows lda and ldb
+// apart), in type T; zeros for an expert without pairs.
+template <typename T, typename TA, typename TB, int BM>
+__global__ __launch_bounds__(split_gemm::kThreads, 2) void any_weight_gradient_kernel(
+    const TA* __restrict__ A, const TB* __restrict__ B, const int64_t* __restrict__ offsets, T* __restrict__ C,
+    int64_t pairs, int64_t M, int64_t N, int64_t lda, int64_t ldb, uint32_t m_tiles, uint32_t n_tiles) {
+    using G = split_gemm::Tile<TA, TB, BM, kAnyCols, true, true>;
+    __shared__ __attribute__((aligned(16))) char lds[G::kLdsBytes];
+    const uint32_t per = m_tiles * n_tiles, e = blockIdx.x / per, within = blockIdx.x % per;
+    const int64_t m0 = static_cast<int64_t>(within / n_tiles) * BM, n0 = static_cast<int64_t>(within % n_tiles) * kAnyCols;
+    const int64_t lo = min(max(offsets[e], int64_t(0)), pairs), K = min(max(offsets[e + 1], lo), pairs) - lo;
+    const int wave = threadIdx.x / kWave, wm = wave >> 1, wn = wave & 1;
+    T* out = C + static_cast<int64_t>(e) * M * N;
+    const TA* a = A + lo * lda;
+    const TB* b = B + lo * ldb;
+    G tile;
+    uint64_t chains = 0;
+    if (K > 0) {
+        chains = tile.template run<16, 16>(
+            lds, K, K, 0, ceil_div(K, G::BK) * G::BK, [&](int r) { return a + min(m0 + r, M - 1); },
+            [&](int r) { return b + min(n0 + r, N - 1); }, [&](int t) { return wn * 64 + t * 32; }, lda, ldb);
+    } else {
+#pragma unroll
+        for (int i = 0; i < G::MT; ++i)
+#pragma unroll
+            for (int j = 0; j < G::NT; ++j) tile.acc[i][j] = split_gemm::f32x16{};
+    }
+    if constexpr (G::kNative) split_gemm::lds_barrier();
+    constexpr int kRegion = split_gemm::store_bytes<T, 1>();
+    const int64_t first = n0 + wn * 64;
+#pragma unroll
+    for (int j = 0; j < G::NT; ++j)
+#pragma unroll
+        for (int i = 0; i < G::MT; ++i) {
+            const int64_t r = m0 + wm * (BM / 2) + i * 32, c = first + j * 32;
+            float o[1][16];
+#pragma unroll
+            for (int v = 0; v < 16; ++v) o[0][v] = tile.acc[i][j][v];
+            split_gemm::store_rows<T, 1>(lds + wave * kRegion, o, out + r * N + c, N, M - r, N - c,
+                                         N % 8 == 0 && reinterpret_cast<uintptr_t>(C) % 16 == 0);
+        }
+    if constexpr (!G::kNative)
+        split_gemm::fix_chains(chains, [&](int block, int v) {
+            const int64_t r = m0 + wm * (BM / 2) + block / G::NT * 32 + (lane_id() & 31);
+            const int64_t c = first + block % G::NT * 32 + acc_column(v);
+            if (r < M && c < N) out[r * N + c] = from_f32<T>(split_gemm::scalar_dot(a + r, b + c, K, 0.0f, lda, ldb));
+        });
+}
+
+// ------------------------------------------------------- rows and columns ---
+// out[t] = sum over the token's pairs of weight x row, in the order of its slots, rounded
+// once; pairs past the valid ones count nothing. weights NULL: `share` each.
+template <typename T>
+__global__ __launch_bounds__(256) void combine_rows_kernel(const float* __restrict__ rows, const int64_t* __restrict__ positions,
+                                                           const int64_t* __restrict__ valid_end, const float* __restrict__ weights,
+                                                           float share, T* __restrict__ out, int64_t tokens, int64_t width,
+                                                           int top_k) {
+    const int64_t per_row = (width + 3) / 4, i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const int64_t t = i / per_row, c = i % per_row * 4;
+    if (t >= tokens) return;
+    const int64_t end = *valid_end;
+    float o[4] = {};
+    for (int s = 0; s < top_k; ++s) {
+        const int64_t p = positions[t * top_k + s];
+        if (p < 0 || p >= end) continue;
+        const float w = weights ? weights[t * top_k + s] : share;
+        const float* r = rows + p * width + c;
+        if (width % 4 == 0) {
+            const float4 v = load4(r);
+            o[0] = fmaf(w, v.x, o[0]), o[1] = fmaf(w, v.y, o[1]), o[2] = fmaf(w, v.z, o[2]), o[3] = fmaf(w, v.w, o[3]);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (c + q < width) o[q] = fmaf(w, r[q], o[q]);
+        }
+    }
+    T* y = out + t * width + c;
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        if (c + q < width) y[q] = from_f32<T>(o[q]);
+}
+
+// The rows of x and dout that the pairs came from, in sorted order (either NULL: not
+// wanted), and <dout, b_o> of each pair. A wave per pair.
+template <typename T>
+__global__ __launch_bounds__(256) void gather_pairs_kernel(const T* __restrict__ x, const T* __restrict__ d_out,
+                                                           const int64_t* __restrict__ rows, const int64_t* __restrict__ offsets,
+                                                           int64_t experts, const T* __restrict__ bo,
+                                                           const int64_t* __restrict__ pair_experts, T* __restrict__ xs,
+                                                           T* __restrict__ ds, float* __restrict__ dot, int64_t pairs,
+                                                           int64_t tokens, int64_t width) {
+    const int64_t p = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / kWave;
+    if (p >= pairs || p >= offsets[experts]) return;
+    const int64_t t = min(max(rows[p], int64_t(0)), tokens - 1), e = min(max(pair_experts[p], int64_t(0)), experts - 1);
+    float sum = 0.0f;
+    for (int64_t c = lane_id(); c < width; c += kWave) {
+        if (xs) xs[p * width + c] = x[t * width + c];
+        const T d = d_out[t * width + c];
+        if (ds) ds[p * width + c] = d;
+        if (dot) sum = fmaf(to_f32(d), to_f32(bo[e * width + c]), sum);
+    }
+    if (dot) {
+        sum = wave_sum_xor(sum);
+        if (lane_id() == 0) dot[p] = sum;
+    }
+}
+
+// dw of every pair in token order: its row's parts in order, and <dout, b_o>; 0 past the valid pairs.
+__global__ __launch_bounds__(256) void weight_gradient_kernel(const float* __restrict__ part, int parts,
+                                                              const float* __restrict__ dot,
+                                                              const int64_t* __restrict__ positions,
+                                                              const int64_t* __restrict__ valid_end, float* __restrict__ dw,
+                                                              int64_t pairs) {
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (i >= pairs) return;
+    const int64_t p = positions[i];
+    float sum = 0.0f;
+    if (p >= 0 && p < *valid_end) {
+        for (int j = 0; j < parts; ++j) sum += part[j * pairs + p];
+        sum += dot[p];
+    }
+    dw[i] = sum;
+}
+
+// Column sums of each expert's rows. First each slot's (a workgroup per slot and 64
+// columns, four waves over the rows), then each expert's slots in order.
+template <typename TA>
+__global__ __launch_bounds__(256) void slot_sums_kernel(const TA* __restrict__ a, int64_t lda, const float* __restrict__ weights,
+                                                        float share, bool weighted, Slots slots, int64_t max_slots, int64_t rows,
+                                                        int64_t columns, float* __restrict__ part) {
+    const int64_t slot = blockIdx.x;
+    if (slot >= slots.expert[max_slots]) return;
+    __shared__ float sh[4][kWave];
+    const int wave = threadIdx.x / kWave;
+    const int64_t c = static_cast<int64_t>(blockIdx.y) * kWave + lane_id();
+    const int64_t r0 = slots.row[slot], end = min(slots.end[slot], r0 + rows);
+    float sum = 0.0f;
+    if (c < columns)
+        for (int64_t r = r0 + wave; r < end; r += 4)
+            sum = fmaf(weighted ? (weights ? weights[r] : share) : 1.0f, to_f32(a[r * lda + c]), sum);
+    sh[wave][lane_id()] = sum;
+    __syncthreads();
+    if (wave == 0 && c < columns)
+        part[slot * columns + c] = (sh[0][lane_id()] + sh[1][lane_id()]) + (sh[2][lane_id()] + sh[3][lane_id()]);
+}
+template <typename T>
+__global__ __launch_bounds__(256) void expert_sums_kernel(const float* __restrict__ part, const int32_t* __restrict__ first,
+                                                          T* __restrict__ out, int64_t columns) {
+    const int64_t e = blockIdx.y, c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (c >= columns) return;
+    float sum = 0.0f;
+    for (int32_t s = first[e]; s < first[e + 1]; ++s) sum += part[s * columns + c];
+    out[e * columns + c] = from_f32<T>(sum);
+}
+
+// --------------------------------------------------------------- the calls ---
+struct Shape {
+    int64_t pairs, tokens, width, hidden, experts, top_k;
+    int dtype;
+};
+inline size_t element(int dtype) { return dtype == KOEMI_F32 ? 4 : 2; }
+inline int64_t most_slots(const Shape& s) { return ceil_div(s.pairs, any_rows(s.pairs, s.experts)) + s.experts; }
+
+// Carves a workspace, or only measures it (base null).
+struct Carver {
+    char* base;
+    size_t used = 0;
+    template <typename V>
+    V* take(int64_t n) {
+        V* p = base ? reinterpret_cast<V*>(base + used) : nullptr;
+        used += align256(static_cast<size_t>(std::max<int64_t>(n, 1)) * sizeof(V));
+        return p;
+    }
+    Slots slots(const Shape& s) {
+        Slots o;
+        o.expert = take<int32_t>(most_slots(s) + 1);
+        o.first = take<int32_t>(s.experts + 1);
+        o.row = take<int64_t>(most_slots(s));
+        o.end = take<int64_t>(most_slots(s));
+        return o;
+    }
+};
+struct ForwardSpace {
+    Slots slots;
+    float *h, *y;
+    size_t bytes;
+};
+inline ForwardSpace forward_space(const Shape& s, void* base) {
+    Carver c{static_cast<char*>(base)};
+    ForwardSpace w;
+    w.slots = c.slots(s);
+    w.h = c.take<float>(s.pairs * padded_hidden(s.hidden));
+    w.y = c.take<float>(s.pairs * s.width);
+    w.bytes = c.used;
+    return w;
+}
+struct BackwardSpace {
+    Slots slots;
+    float *dg, *dv, *wh, *dx, *dw_part, *dot, *sums;
+    void *xs, *ds;
+    size_t bytes;
+};
+inline BackwardSpace backward_space(const Shape& s, void* base) {
+    Carver c{static_cast<char*>(base)};
+    BackwardSpace w;
+    const int64_t ld = padded_hidden(s.hidden);
+    w.slots = c.slots(s);
+    w.dg = c.take<float>(s.pairs * ld);
+    w.dv = c.take<float>(s.pairs * ld);
+    w.wh = c.take<float>(s.pairs * ld);
+    w.dx = c.take<float>(s.pairs * s.width);
+    w.dw_part = c.take<float>(2 * ceil_div(s.hidden, kAnyCols) * s.pairs);
+    w.dot = c.take<float>(s.pairs);
+    w.sums = c.take<float>(most_slots(s) * std::max(s.width, s.hidden));
+    w.xs = c.take<char>(s.pairs * s.width * static_cast<int64_t>(element(s.dtype)));
+    w.ds = c.take<char>(s.pairs * s.width * static_cast<int64_t>(element(s.dtype)));
+    w.bytes = c.used;
+    return w;
+}
+
+int check_shape(const char* what, const Shape& s) {
+    if (!float_dtype(s.dtype)) return fail(KOEMI_ERR_UNSUPPORTED, "%s: unsupported dtype %s", what, dtype_name(s.dtype));
+    if (s.tokens < 0 || s.width < 1 || s.hidden < 1 || s.experts < 1 || s.top_k < 1)
+        return fail(KOEMI_ERR_INVALID, "%s: bad dimension", what);
+    const int64_t most = int64_t(1) << 31;
+    if (s.tokens >= most || s.top_k > 256 || s.pairs >= most || s.width >= (1 << 24) || s.hidden >= (1 << 24) ||
+        s.experts >= (1 << 20) ||
+        most_slots(s) * ceil_div(std::max(s.width, s.hidden), 64) >= most ||
+        s.experts * ceil_div(s.width, 64) * ceil_div(s.hidden, kAnyCols) >= most ||
+        s.tokens * ceil_div(s.width, 4) >= (int64_t(1) << 38))
+        return fail(KOEMI_ERR_UNSUPPORTED, "%s: shape too large", what);
+    return KOEMI_OK;
+}
+inline unsigned tiles_grid(int64_t slots, int64_t n_tiles) { return static_cast<unsigned>(ceil_div(slots * n_tiles, 8) * 8); }
+
+// Runs f(BM) for the tile rows of the shape and f's load bytes of a row of `width` elements at base.
+template <typename F>
+void by_rows(const Shape& s, F f) {
+    if (any_rows(s.pairs, s.experts) == 64) f(std::integral_constant<int, 64>{});
+    else f(std::integral_constant<int, 128>{});
+}
+template <typename F>
+void by_bytes(int bytes, F f) {
+    if (bytes == 16) f(std::integral_constant<int, 16>{});
+    else if (bytes == 8) f(std::integral_constant<int, 8>{});
+    else f(std::integral_constant<int, split_gemm::kElementLoads>{});
+}
+void find_slots(const Shape& s, const int64_t* offsets, const Slots& slots, hipStream_t q) {
+    hipLaunchKernelGGL(slots_kernel, dim3(1), dim3(kSlotThreads), 0, q, offsets, s.experts, s.pairs,
+                       static_cast<int64_t>(any_rows(s.pairs, s.experts)), most_slots(s), slots);
+}
+template <typename T>
+void combine(const float* rows, const int64_t* positions, const int64_t* offsets, const float* weights, float share, void* out,
+             const Shape& s, hipStream_t q) {
+    hipLaunchKernelGGL(combine_rows_kernel<T>, dim3(grid_for(s.tokens * ceil_div(s.width, 4), 256)), dim3(256), 0, q, rows,
+                       positions, offsets + s.experts, weights, share, static_cast<T*>(out), s.tokens, s.width,
+                       static_cast<int>(s.top_k));
+}
+
+struct Weights {
+    const void *Wg, *bg, *Wv, *bv, *Wo, *bo;
+};
+struct Gradients {
+    void *x, *Wg, *bg, *Wv, *bv, *Wo, *bo;
+    float* weights;
+};
+
+template <typename T>
+int any_forward(const Shape& s, const void* x, const int64_t* rows, const int64_t* offsets, const int64_t* positions,
+                const float* pair_weights, const Weights& m, void* out, float* keep, const ForwardSpace& w, hipStream_t q) {
+    const int64_t ld = padded_hidden(s.hidden), slots = most_slots(s);
+    float* keep_v = keep ? keep + s.pairs * ld : nullptr;
+    find_slots(s, offsets, w.slots, q);
+    by_rows(s, [&](auto rows_tag) {
+        constexpr int BM = decltype(rows_tag)::value;
+        const int in_bytes = std::min({split_gemm::load_bytes<T>(x, s.width), split_gemm::load_bytes<T>(m.Wg, s.width),
+                                       split_gemm::load_bytes<T>(m.Wv, s.width)});
+        by_bytes(in_bytes, [&](auto bytes) {
+            const uint32_t n = static_cast<uint32_t>(ceil_div(s.hidden, 64));
+            hipLaunchKernelGGL((any_hidden_kernel<T, BM, decltype(bytes)::value>), dim3(tiles_grid(slots, n)),
+                               dim3(split_gemm::kThreads), 0, q, static_cast<const T*>(x), rows, s.tokens,
+                               static_cast<const T*>(m.Wg), static_cast<const T*>(m.bg), static_cast<const T*>(m.Wv),
+                               static_cast<const T*>(m.bv), keep, keep_v, w.h, w.slots, slots, s.width, s.hidden, ld, n);
+        });
+        by_bytes(split_gemm::load_bytes<T>(m.Wo, s.hidden), [&](auto bytes) {
+            const uint32_t n = static_cast<uint32_t>(ceil_div(s.width, kAnyCols));
+            hipLaunchKernelGGL((any_output_kernel<T, BM, decltype(bytes)::value>), dim3(tiles_grid(slots, n)),
+                               dim3(split_gemm::kThreads), 0, q, w.h, static_cast<const T*>(m.Wo),
+                               static_cast<const T*>(m.bo), w.y, w.slots, slots, s.width, s.hidden, ld, n);
+        });
+    });
+    combine<T>(w.y, positions, offsets, pair_weights, 1.0f / static_cast<float>(s.top_k), out, s, q);
+    return check_launch("koemi_moe_experts_forward");
+}
+
+template <typename T>
+int any_backward(const Shape& s, const void* d_out, const void* x, const int64_t* rows, const int64_t* pair_experts,
+                 const int64_t* offsets, const int64_t* positions, const float* sorted_w, const Weights& m, const float* keep,
+                 const Gradients& d, const BackwardSpace& w, hipStream_t q) {
+    const int64_t ld = padded_hidden(s.hidden), slots = most_slots(s);
+    const float share = 1.0f / static_cast<float>(s.top_k);
+    const T* dy = static_cast<const T*>(d_out);
+    T *xs = static_cast<T*>(w.xs), *ds = static_cast<T*>(w.ds);
+    find_slots(s, offsets, w.slots, q);
+    const bool want_in = d.Wg || d.Wv, want_out = d.Wo || d.bo;
+    if (want_in || want_out || d.weights)
+        hipLaunchKernelGGL(gather_pairs_kernel<T>, dim3(grid_for(s.pairs, 4)), dim3(256), 0, q, static_cast<const T*>(x), dy,
+                           rows, offsets, s.experts, static_cast<const T*>(m.bo), pair_experts, want_in ? xs : nullptr,
+                           want_out ? ds : nullptr, d.weights ? w.dot : nullptr, s.pairs, s.tokens, s.width);
+    const uint32_t h_tiles = static_cast<uint32_t>(ceil_div(s.hidden, kAnyCols));
+    const uint32_t w_tiles = static_cast<uint32_t>(ceil_div(s.width, kAnyCols));
+    by_rows(s, [&](auto rows_tag) {
+        constexpr int BM = decltype(rows_tag)::value;
+        by_bytes(split_gemm::load_bytes<T>(d_out, s.width), [&](auto bytes) {
+            hipLaunchKernelGGL((any_hidden_gradient_kernel<T, BM, decltype(bytes)::value>), dim3(tiles_grid(slots, h_tiles)),
+                               dim3(split_gemm::kThreads), 0, q, dy, rows, s.tokens, static_cast<const T*>(m.Wo), keep,
+                               keep + s.pairs * ld, sorted_w, share, w.dg, w.dv, w.wh, w.dw_part, w.slots, slots, s.pairs,
+                               s.width, s.hidden, ld, h_tiles);
+        });
+        if (d.x)
+            hipLaunchKernelGGL((any_input_gradient_kernel<T, BM>), dim3(tiles_grid(slots, w_tiles)), dim3(split_gemm::kThreads),
+                               0, q, w.dg, w.dv, static_cast<const T*>(m.Wg), static_cast<const T*>(m.Wv), w.dx, w.slots, slots,
+                               s.width, s.hidden, ld, w_tiles);
+    });
+    if (d.x) combine<T>(w.dx, positions, offsets, nullptr, 1.0f, d.x, s, q);
+    if (d.weights)
+        hipLaunchKernelGGL(weight_gradient_kernel, dim3(grid_for(s.pairs, 256)), dim3(256), 0, q, w.dw_part,
+                           static_cast<int>(2 * h_tiles), w.dot, positions, offsets + s.experts, d.weights, s.pairs);
+    auto product = [&](auto* a, auto* b, void* c, int64_t M, int64_t N, int64_t lda, int64_t ldb) {
+        using TA = std::remove_pointer_t<decltype(a)>;
+        using TB = std::remove_pointer_t<decltype(b)>;
+        const uint32_t mt = static_cast<uint32_t>(ceil_div(M, 128)), nt = static_cast<uint32_t>(ceil_div(N, kAnyCols));
+        hipLaunchKernelGGL((any_weight_gradient_kernel<T, TA, TB, 128>), dim3(static_cast<unsigned>(s.experts * mt * nt)),
+                           dim3(split_gemm::kThreads), 0, q, a, b, offsets, static_cast<T*>(c), s.pairs, M, N, lda, ldb, mt, nt);
+    };
+    if (d.Wg) product(w.dg, xs, d.Wg, s.hidden, s.width, ld, s.width);
+    if (d.Wv) product(w.dv, xs, d.Wv, s.hidden, s.width, ld, s.width);
+    if (d.Wo) product(ds, w.wh, d.Wo, s.width, s.hidden, s.width, ld);
+    auto columns = [&](auto* a, int64_t lda, bool weighted, int64_t n, void* c) {
+        using TA = std::remove_pointer_t<decltype(a)>;
+        hipLaunchKernelGGL(slot_sums_kernel<TA>, dim3(static_cast<unsigned>(slots), static_cast<unsigned>(ceil_div(n, kWave))),
+                           dim3(256), 0, q, a, lda, sorted_w, share, weighted, w.slots, slots,
+                           static_cast<int64_t>(any_rows(s.pairs, s.experts)), n, w.sums);
+        hipLaunchKernelGGL(expert_sums_kernel<T>, dim3(grid_for(n, 256), static_cast<unsigned>(s.experts)), dim3(256), 0, q,
+                           w.sums, w.slots.first, static_cast<T*>(c), n);
+    };
+    if (d.bg) columns(w.dg, ld, false, s.hidden, d.bg);
+    if (d.bv) columns(w.dv, ld, false, s.hidden, d.bv);
+    if (d.bo) columns(ds, s.width, true, s.width, d.bo);
+    return check_launch("koemi_moe_experts_backward");
+}
+
+}  // namespace
+}  // namespace koemi
+
+using namespace koemi;
+
+extern "C" size_t koemi_moe_experts_saved_bytes(int64_t tokens, int64_t top_k, int64_t width, int64_t hidden,
+                                                int64_t expert_count, int dtype) {
+    const Shape s{tokens * top_k, tokens, width, hidden, expert_count, top_k, dtype};
+    if (check_shape("koemi_moe_experts_saved_bytes", s) != KOEMI_OK) return 0;
+    return static_cast<size_t>(2 * s.pairs * padded_hidden(hidden)) * sizeof(float);
+}
+
+extern "C" size_t koemi_moe_experts_workspace_bytes(int64_t tokens, int64_t top_k, int64_t width, int64_t hidden,
+                                                    int64_t expert_count, int dtype, int backward) {
+    const Shape s{tokens * top_k, tokens, width, hidden, expert_count, top_k, dtype};
+    if (check_shape("koemi_moe_experts_workspace_bytes", s) != KOEMI_OK) return 0;
+    return backward ? backward_space(s, nullptr).bytes : forward_space(s, nullptr).bytes;
+}
+
+extern "C" int koemi_moe_experts_forward(const void* context, const int64_t* sorted_rows, const int64_t* segment_offsets,
+                                         const int64_t* pair_positions, const float* pair_weights, const void* gate_weights,
+                                         const void* gate_biases, const void* value_weights, const void* value_biases,
+                                         const void* output_weights, const void* output_biases, void* output, void* saved,
+                                         int64_t tokens, int64_t top_k, int64_t width, int64_t hidden, int64_t expert_count,
+                                         int dtype, void* workspace, size_t workspace_bytes, koemi_stream_t stream) {
+    clear_error();
+    const char* what = "koemi_moe_experts_forward";
+    const Shape s{tokens * top_k, tokens, width, hidden, expert_count, top_k, dtype};
+    const int st = check_shape(what, s);
+    if (st != KOEMI_OK || tokens == 0) return st;
+    const Weights m{gate_weights, gate_biases, value_weights, value_biases, output_weights, output_biases};
+    if (!context || !sorted_rows || !segment_offsets || !pair_positions || !m.Wg || !m.bg || !m.Wv || !m.bv || !m.Wo ||
+        !m.bo || !output)
+        return fail(KOEMI_ERR_INVALID, "%s: null pointer", what);
+    const ForwardSpace w = forward_space(s, workspace);
+    if (!workspace || workspace_bytes < w.bytes) return fail(KOEMI_ERR_INVALID, "%s: workspace too small", what);
+    float* keep = static_cast<float*>(saved);
+    hipStream_t q = as_stream(stream);
+    if (dtype == KOEMI_F32)
+        return any_forward<float>(s, context, sorted_rows, segment_offsets, pair_positions, pair_weights, m, output, keep, w, q);
+    if (dtype == KOEMI_F16)
+        return any_forward<f16>(s, context, sorted_rows, segment_offsets, pair_positions, pair_weights, m, output, keep, w, q);
+    return any_forward<bf16>(s, context, sorted_rows, segment_offsets, pair_positions, pair_weights, m, output, keep, w, q);
+}
+
+extern "C" int koemi_moe_experts_backward(const void* grad_output, const void* context, const int64_t* sorted_rows,
+                                          const int64_t* sorted_experts, const int64_t* segment_offsets,
+                                          const int64_t* pair_positions, const float* sorted_weights, const void* gate_weights,
+                                          const void* value_weights, const void* output_weights, const void* output_biases,
+                                          const void* saved, void* grad_context, float* grad_pair_weights,
+                                          void* grad_gate_weights, void* grad_gate_biases, void* grad_value_weights,
+                                          void* grad_value_biases, void* grad_output_weights, void* grad_output_biases,
+                                          int64_t tokens, int64_t top_k, int64_t width, int64_t hidden, int64_t expert_count,
+                                          int dtype, void* workspace, size_t workspace_bytes, koemi_stream_t stream) {
+    clear_error();
+    const char* what = "koemi_moe_experts_backward";
+    const Shape s{tokens * top_k, tokens, width, hidden, expert_count, top_k, dtype};
+    const int st = check_shape(what, s);
+    if (st != KOEMI_OK || tokens == 0) return st;
+    const Weights m{gate_weights, nullptr, value_weights, nullptr, output_weights, output_biases};
+    if (!grad_output || !context || !sorted_rows || !sorted_experts || !segment_offsets || !pair_positions || !m.Wg ||
+        !m.Wv || !m.Wo || !m.bo || !saved)
+        return fail(KOEMI_ERR_INVALID, "%s: null pointer", what);
+    const Gradients d{grad_context,       grad_gate_weights,   grad_gate_biases,   grad_value_weights,
+                      grad_value_biases,  grad_output_weights, grad_output_biases, grad_pair_weights};
+    const BackwardSpace w = backward_space(s, workspace);
+    if (!workspace || workspace_bytes < w.bytes) return fail(KOEMI_ERR_INVALID, "%s: workspace too small", what);
+    const float* keep = static_cast<const float*>(saved);
+    hipStream_t q = as_stream(stream);
+    if (dtype == KOEMI_F32)
+        return any_backward<float>(s, grad_output, context, sorted_rows, sorted_experts, segment_offsets, pair_positions,
+                                   sorted_weights, m, keep, d, w, q);
+    if (dtype == KOEMI_F16)
+        return any_backward<f16>(s, grad_output, context, sorted_rows, sorted_experts, segment_offsets, pair_positions,
+                                 sorted_weights, m, keep, d, w, q);
+    return any_backward<bf16>(s, grad_output, context, sorted_rows, sorted_experts, segment_offsets, pair_positions,
+                              sorted_weights, m, keep, d, w, q);
+}

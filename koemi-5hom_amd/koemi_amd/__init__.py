@@ -24,6 +24,7 @@ from koemi_amd.recurrent import gated_recurrence, recurrent_gates, recurrent_sca
 from koemi_amd.moe import (
     combine_topk,
     expert_activation_counts,
+    expert_mixture,
     grouped_expert_mlp_inference,
     load_native_extension,
     permute_topk,
@@ -42,6 +43,7 @@ __all__ = [
     "dense_affine_scan",
     "diagnose_cuda_affine_scan",
     "expert_activation_counts",
+    "expert_mixture",
     "fused_rmsnorm_silu",
     "gated_recurrence",
     "grouped_expert_mlp_inference",

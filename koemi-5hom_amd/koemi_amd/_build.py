@@ -36,6 +36,7 @@ SOURCES = (
     "moe_permute.hip",
     "moe_grouped_mlp.hip",
     "moe_combine.hip",
+    "moe_experts.hip",
     "memory.hip",
     "salient_read.hip",
     "gates.hip",

@@ -229,6 +229,16 @@ _SIGNATURES: dict[str, tuple[Any, tuple[Any, ...]]] = {
         c_int,
         (_P, c_int64, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int64, c_int64, c_int64, c_int64, _P, c_size_t, _P),
     ),
+    "koemi_moe_experts_saved_bytes": (c_size_t, (c_int64, c_int64, c_int64, c_int64, c_int64, c_int)),
+    "koemi_moe_experts_workspace_bytes": (c_size_t, (c_int64, c_int64, c_int64, c_int64, c_int64, c_int, c_int)),
+    "koemi_moe_experts_forward": (
+        c_int,
+        (*(_P,) * 13, c_int64, c_int64, c_int64, c_int64, c_int64, c_int, _P, c_size_t, _P),
+    ),
+    "koemi_moe_experts_backward": (
+        c_int,
+        (*(_P,) * 20, c_int64, c_int64, c_int64, c_int64, c_int64, c_int, _P, c_size_t, _P),
+    ),
     "koemi_moe_route_balanced_workspace_bytes": (c_size_t, (c_int64, c_int64)),
     "koemi_moe_route_balanced_forward": (
         c_int,

@@ -19,7 +19,9 @@ Build-side keyword-only extensions (absent from the reference signatures):
   50-58; ``merge_router_statistics`` router.py:25-32);
 * ``expert_activation_counts`` — per-expert counts of network.py:48-70;
 * ``route_topk_balanced`` — the learned gate to be trained: its weights, probability
-  mass and balance loss with the gradient of the logits.
+  mass and balance loss with the gradient of the logits;
+* ``expert_mixture`` — the experts of every token's route, weighted and summed
+  (router.py:61-97 before its normalizer), with the gradients of all its inputs.
 """
 
 from __future__ import annotations
@@ -40,6 +42,7 @@ __all__ = [
     "RouterStatistics",
     "combine_topk",
     "expert_activation_counts",
+    "expert_mixture",
     "grouped_expert_mlp_fragments",
     "grouped_expert_mlp_inference",
     "load_native_extension",
@@ -948,6 +951,157 @@ def combine_topk(
             _native.stream_of(expert_outputs.device),
         )
     return combined
+
+
+def expert_mixture(
+    context: Tensor,
+    assignments: Tensor,
+    pair_weights: Tensor | None,
+    valid_mask: Tensor,
+    gate_weights: Tensor,
+    gate_biases: Tensor,
+    value_weights: Tensor,
+    value_biases: Tensor,
+    output_weights: Tensor,
+    output_biases: Tensor,
+    *,
+    validate: bool = True,
+) -> Tensor:
+    """Every token's experts, weighted and summed, with first-order autograd
+    (LearnedExpertMixture.combine, router.py:61-97, before its normalizer).
+
+    ``context`` ``[..., D]`` float32, float16 or bfloat16; ``assignments`` int32 or
+    int64 ``[..., top_k]`` with ``pair_weights`` float32 of that shape (None: ``1 /
+    top_k`` each), as ``route_topk_balanced`` returns them; ``valid_mask`` bool of the
+    leading shape. Parameters in the context's dtype: ``[E, H, D]``, ``[E, H]``,
+    ``[E, H, D]``, ``[E, H]``, ``[E, D, H]``, ``[E, D]``. Any strides. A slot whose
+    expert lies outside ``[0, E)`` (-1: not routed), that repeats an expert of its
+    token, or whose token is invalid counts nothing; ``validate`` refuses the repeats,
+    and ids other than -1 outside the catalog, of valid tokens (one read-back, so not
+    under graph capture).
+
+    Returns ``context``'s shape and dtype: the sum over a token's slots of
+    ``w (W_o (silu(W_g x + b_g) * (W_v x + b_v)) + b_o)``, zeros without any. All
+    floating arguments are differentiable (``koemi_moe_experts_backward``); sums are
+    float32, in a fixed order."""
+
+    params = {"gate_weights": gate_weights, "gate_biases": gate_biases, "value_weights": value_weights,
+              "value_biases": value_biases, "output_weights": output_weights, "output_biases": output_biases}
+    tensors = {"context": context, "assignments": assignments, "valid_mask": valid_mask, **params}
+    if pair_weights is not None:
+        tensors["pair_weights"] = pair_weights
+    for name, tensor in tensors.items():
+        if not isinstance(tensor, Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor")
+        if not tensor.is_cuda:
+            raise CudaMoeValidationError(f"{name} must be a CUDA tensor")
+    _require_same_cuda_device(tensors)
+    _require_supported_context_dtype(context, "context")
+    if any(tensor.dtype != context.dtype for tensor in params.values()):
+        raise CudaMoeValidationError("context and the expert parameters must share a dtype")
+    if context.ndim < 1 or context.shape[-1] < 1:
+        raise CudaMoeValidationError("context must have a non-empty width")
+    leading = context.shape[:-1]
+    if assignments.dtype not in (torch.int32, torch.int64) or assignments.shape[:-1] != leading \
+            or assignments.ndim != context.ndim:
+        raise CudaMoeValidationError("assignments must be int32 or int64 of shape context.shape[:-1] + (top_k,)")
+    if pair_weights is not None and (pair_weights.dtype != torch.float32 or pair_weights.shape != assignments.shape):
+        raise CudaMoeValidationError("pair_weights must be float32 with the shape of assignments")
+    if valid_mask.dtype != torch.bool or valid_mask.shape != leading:
+        raise CudaMoeValidationError("valid_mask must be boolean with shape context.shape[:-1]")
+    if gate_weights.ndim != 3 or gate_weights.shape[2] != context.shape[-1] or gate_weights.shape[1] < 1:
+        raise CudaMoeValidationError("gate_weights must have shape [expert_count, hidden, width]")
+    experts, hidden, width = gate_weights.shape
+    if value_weights.shape != (experts, hidden, width) or output_weights.shape != (experts, width, hidden):
+        raise CudaMoeValidationError("value and output weights do not match the gate weights")
+    if gate_biases.shape != (experts, hidden) or value_biases.shape != (experts, hidden) \
+            or output_biases.shape != (experts, width):
+        raise CudaMoeValidationError("biases do not match their weights")
+    _require_positive_bounded(experts, "expert_count", _MAX_PERMUTE_EXPERTS)
+    top_k = _require_positive_bounded(int(assignments.shape[-1]), "top_k", 256)
+    if top_k > experts:
+        raise CudaMoeValidationError("top_k must not exceed expert_count")
+    tokens = valid_mask.numel()
+    if tokens * top_k >= 1 << 31 or max(width, hidden) >= 1 << 24:
+        raise CudaMoeValidationError("tokens x top_k must be below 2^31, width and hidden below 2^24")
+    _require_library()
+    if validate and tokens:
+        flat, mask = assignments.reshape(-1, top_k).contiguous(), valid_mask.reshape(-1)
+        # a slot of -1 is no expert: it takes one past the catalog of its own, which repeats nothing
+        spare = torch.arange(experts, experts + top_k, device=flat.device, dtype=flat.dtype)
+        out_of_range, duplicate = _assignment_flags(torch.where(flat == -1, spare, flat), mask.contiguous(), experts + top_k)
+        if out_of_range or bool(((flat >= experts) & mask[:, None]).any()):
+            raise CudaMoeValidationError("valid MoE assignments must be -1 or in [0, expert_count)")
+        if duplicate and top_k >= 2:
+            raise CudaMoeValidationError("expert_mixture received duplicate experts for a valid token")
+    return _ExpertMixture.apply(context, pair_weights, assignments, valid_mask, *params.values())
+
+
+class _ExpertMixture(torch.autograd.Function):
+    @staticmethod
+    def forward(context, x: Tensor, pair_weights: Tensor | None, assignments: Tensor, valid_mask: Tensor,  # type: ignore[override]
+                *params: Tensor) -> Tensor:
+        (experts, hidden, width), top_k = params[0].shape, int(assignments.shape[-1])
+        trained = any(context.needs_input_grad)
+        flat = _aligned(x.reshape(-1, width).contiguous())
+        tokens, device, code = flat.shape[0], x.device, _native.dtype_code(x.dtype)
+        out = torch.empty(x.shape, device=device, dtype=x.dtype)
+        shape = (tokens, top_k, width, hidden, experts, code)
+        if tokens == 0:
+            context.shape = None
+            context.save_for_backward(x, pair_weights, *params)
+            return out
+        weights = pair_weights.reshape(-1, top_k).contiguous() if pair_weights is not None else None
+        rows, pair_experts, offsets, sorted_weights, positions = permute_indices(
+            assignments.reshape(-1, top_k), valid_mask.reshape(-1), expert_count=experts, pair_weights=weights)
+        laid = [_aligned(p.contiguous()) for p in params]
+        saved = torch.empty((_size("koemi_moe_experts_saved_bytes", *shape),), device=device, dtype=torch.uint8) \
+            if trained else None
+        need = _size("koemi_moe_experts_workspace_bytes", *shape, 0)
+        workspace = torch.empty((need,), device=device, dtype=torch.uint8)
+        with _native.device_guard(device):
+            _native.call("koemi_moe_experts_forward", flat.data_ptr(), rows.data_ptr(), offsets.data_ptr(),
+                         positions.data_ptr(), _native.ptr(weights), *(p.data_ptr() for p in laid), out.data_ptr(),
+                         _native.ptr(saved), *shape, workspace.data_ptr(), need, _native.stream_of(device))
+        if trained:
+            context.shape = shape
+            context.like = (x.shape, assignments.shape)
+            gate, _, value, _, output, output_bias = laid
+            context.save_for_backward(flat, rows, pair_experts, offsets, positions, sorted_weights, gate, value, output,
+                                      output_bias, saved)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(context, d_out: Tensor):  # type: ignore[override]
+        wanted = context.needs_input_grad
+        if context.shape is None:  # no tokens
+            x, weights, *params = context.saved_tensors
+            grads = [torch.zeros_like(t) if t is not None and want else None
+                     for t, want in zip((x, weights, None, None, *params), wanted)]
+            return tuple(grads)
+        x, rows, pair_experts, offsets, positions, sorted_weights, gate, value, output, output_bias, saved = context.saved_tensors
+        tokens, top_k, width, hidden, experts, _ = context.shape
+        device = x.device
+        d_out = _aligned(d_out.reshape(tokens, width).contiguous())
+
+        def room(want: bool, shape: tuple[int, ...], dtype: torch.dtype = x.dtype) -> Tensor | None:
+            return torch.empty(shape, device=device, dtype=dtype) if want else None
+
+        d_x = room(wanted[0], context.like[0])
+        d_weights = room(wanted[1], context.like[1], torch.float32)
+        matrix, wide, narrow = (experts, hidden, width), (experts, hidden), (experts, width)
+        d_params = [room(want, shape) for want, shape in
+                    zip(wanted[4:], (matrix, wide, matrix, wide, (experts, width, hidden), narrow))]
+        need = _size("koemi_moe_experts_workspace_bytes", *context.shape, 1)
+        workspace = torch.empty((need,), device=device, dtype=torch.uint8)
+        with _native.device_guard(device):
+            _native.call("koemi_moe_experts_backward", d_out.data_ptr(), x.data_ptr(), rows.data_ptr(),
+                         pair_experts.data_ptr(), offsets.data_ptr(), positions.data_ptr(), _native.ptr(sorted_weights),
+                         gate.data_ptr(), value.data_ptr(), output.data_ptr(), output_bias.data_ptr(), saved.data_ptr(),
+                         _native.ptr(d_x), _native.ptr(d_weights), *(_native.ptr(p) for p in d_params), *context.shape,
+                         workspace.data_ptr(), need, _native.stream_of(device))
+        return d_x, d_weights, None, None, *d_params
 
 
 class _MoeExtension:
