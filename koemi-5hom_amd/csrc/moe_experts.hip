@@ -21,9 +21,11 @@
 // Any type, width and alignment runs on the tiles of split_gemm.hpp, which read an
 // operand either along K or across it; what lies between two products stays fp32 there.
 #include "common.hpp"
+#include "mfma_across.hpp"
 #include "split_gemm.hpp"
 
 #include <algorithm>
+#include <initializer_list>
 #include <type_traits>
 
 namespace koemi {
@@ -384,6 +386,411 @@ __global__ __launch_bounds__(split_gemm::kThreads, 2) void any_weight_gradient_k
         });
 }
 
+// ------------------------------------------------------------ the bf16 tiles ---
+// Width and hidden multiples of 64: 256 x 256 tiles of mfma_stage.hpp and mfma_across.hpp
+// (four waves in 2 x 2, 128 x 128 outputs each, operands through a ring of four LDS
+// stages filled by direct copies). What lies between two products is bf16, g, v, y and dx
+// are fp32. A slot is up to 256 pairs of one expert; the backward works on rows padded to
+// whole slots (row 256 slot + r), so that sums over an expert's pairs take whole K steps:
+// rows past its pairs are zeros.
+using mfma_stage::across_fragment;
+using mfma_stage::along_fragment;
+using mfma_stage::f32x16;
+using mfma_stage::kOperandBytes;
+using mfma_stage::uniform_ptr;
+constexpr int kTile = 256;
+constexpr int kTileK = mfma_stage::kBK;
+constexpr uint32_t kTileLds = mfma_stage::TileShape<256>::kStages * mfma_stage::TileShape<256>::kStageBytes;
+
+struct TilePlace {
+    int lane, wave, wm, wn;
+    uint32_t a_lds, b_lds;
+    __device__ __forceinline__ explicit TilePlace(char* lds) {
+        lane = lane_id();
+        wave = threadIdx.x / kWave;
+        wm = wave >> 1;
+        wn = wave & 1;
+        const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+        a_lds = __builtin_amdgcn_readfirstlane(lds0 + wave * 4 * 1024);
+        b_lds = __builtin_amdgcn_readfirstlane(lds0 + kOperandBytes + wave * 4 * 1024);
+    }
+    // Offsets of the wave's copies of an operand along K: row(r) is the memory row of the
+    // tile's row r, ld elements long.
+    template <typename Row>
+    __device__ __forceinline__ void along(uint32_t (&off)[4], int64_t ld, Row row) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = (wave * 4 + i) * 16 + (lane >> 2), g = (lane & 3) ^ mfma_stage::slot_swizzle(r);
+            off[i] = (static_cast<uint32_t>(row(r)) * static_cast<uint32_t>(ld) + g * 8) * 2u;
+        }
+    }
+    // Of an operand across K: columns from `first` on (those past `columns`, a multiple of 8, repeat the last).
+    __device__ __forceinline__ void across(uint32_t (&off)[4], int64_t ld, int64_t first, int64_t columns) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            int k, c;
+            mfma_stage::across_source(wave * 4 + i, lane, k, c);
+            off[i] = (static_cast<uint32_t>(k) * static_cast<uint32_t>(ld) + static_cast<uint32_t>(min(first + c, columns - 8))) * 2u;
+        }
+    }
+    __device__ __forceinline__ void fragments(uint32_t (&off)[4], bool across, int first) const {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) off[t] = across ? across_fragment(first + t * 32) : along_fragment(first + t * 32);
+    }
+};
+__device__ __forceinline__ void clear(f32x16 (&acc)[4][4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = f32x16{};
+}
+
+// A wave's 128 x (32 TILES) outputs as whole bf16 rows. They pass through the wave's own
+// LDS region (chunk c of row r at c ^ r, so that rows are read without bank conflicts),
+// four consecutive columns c of a row at a time, and leave in 16-byte pieces.
+template <int TILES>
+__device__ __forceinline__ void put_four(char* region, int r, int c, float v0, float v1, float v2, float v3) {
+    constexpr int kRowBytes = TILES * 64, kSwz = kRowBytes / 16 - 1;
+    store4(reinterpret_cast<bf16*>(region + r * kRowBytes + ((c >> 3) ^ (r & kSwz)) * 16 + (c & 4) * 2), v0, v1, v2, v3);
+}
+// rows, cols (a multiple of 8): how many exist from out's first element on.
+template <int TILES>
+__device__ __forceinline__ void flush_wave(const char* region, bf16* out, int64_t ld, int64_t rows, int64_t cols) {
+    constexpr int kRowBytes = TILES * 64, kChunks = kRowBytes / 16, kSwz = kChunks - 1;
+    constexpr int kBatch = 8, kIters = 128 * kChunks / kWave;
+    const int lane = lane_id();
+#pragma unroll
+    for (int b = 0; b < kIters; b += kBatch) {
+        uint4 piece[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int idx = (b + i) * kWave + lane, r = idx / kChunks, c = idx % kChunks;
+            piece[i] = *reinterpret_cast<const uint4*>(region + r * kRowBytes + ((c ^ (r & kSwz)) * 16));
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int idx = (b + i) * kWave + lane, r = idx / kChunks, c = idx % kChunks;
+            if (r < rows && c * 8 < cols) *reinterpret_cast<uint4*>(out + r * ld + c * 8) = piece[i];
+        }
+    }
+}
+// Both, of value(mt, t, v), element v of the wave's tile (mt, t).
+template <int TILES, typename Value>
+__device__ __forceinline__ void store_wave(char* region, bf16* out, int64_t ld, int64_t rows, int64_t cols, Value value) {
+    const int lane = lane_id();
+#pragma unroll
+    for (int t = 0; t < TILES; ++t)
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) {
+            __builtin_amdgcn_sched_barrier(0);  // a tile at a time: all at once they spill
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                put_four<TILES>(region, mt * 32 + (lane & 31), t * 32 + (lane >> 5) * 4 + j * 8, value(mt, t, j * 4),
+                                value(mt, t, j * 4 + 1), value(mt, t, j * 4 + 2), value(mt, t, j * 4 + 3));
+        }
+    flush_wave<TILES>(region, out, ld, rows, cols);
+}
+// A wave's 128 x 128 outputs in fp32, each lane four consecutive columns at a time.
+template <typename Value>
+__device__ __forceinline__ void store_wave_f32(float* out, int64_t ld, int64_t rows, int64_t cols, Value value) {
+    const int lane = lane_id();
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+        const int r = mt * 32 + (lane & 31);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int c = t * 32 + (lane >> 5) * 4 + j * 8;
+                if (r < rows && c < cols)
+                    store4(out + r * ld + c, value(mt, t, j * 4), value(mt, t, j * 4 + 1), value(mt, t, j * 4 + 2),
+                           value(mt, t, j * 4 + 3));
+            }
+        }
+    }
+}
+
+// g and v are kept in the order of the accumulators: float4 (slot, 32-column block, 32-row
+// block, j, lane) holds elements 4 j .. 4 j + 3, so that a wave reads and writes 1 KiB at once.
+__device__ __forceinline__ int64_t kept_at(int64_t slot, int64_t blocks, int64_t c32, int m32, int j, int lane) {
+    return ((((slot * blocks + c32) * 8 + m32) * 4 + j) * kWave + lane) * 4;
+}
+
+// g, v and h of a slot's pairs x 128 hidden units: B rows 0 .. 127 are W_g's, 128 .. 255 W_v's.
+__global__ __launch_bounds__(mfma_stage::kThreads, 1) void tile_hidden_kernel(
+    const bf16* __restrict__ x, const int64_t* __restrict__ rows, int64_t tokens, const bf16* __restrict__ Wg,
+    const bf16* __restrict__ bg, const bf16* __restrict__ Wv, const bf16* __restrict__ bv, float* __restrict__ keep_g,
+    float* __restrict__ keep_v, bf16* __restrict__ h, Slots slots, int64_t max_slots, int64_t width, int64_t hidden,
+    uint32_t n_tiles) {
+    __shared__ __attribute__((aligned(1024))) char lds[kTileLds];
+    uint32_t slot, tile_n;
+    if (!slot_tile(slots, max_slots, n_tiles, slot, tile_n)) return;
+    const int e = slots.expert[slot];
+    const int64_t row0 = slots.row[slot], end = slots.end[slot], n0 = static_cast<int64_t>(tile_n) * 128;
+    const TilePlace at(lds);
+    const bf16* a = static_cast<const bf16*>(uniform_ptr(x));
+    const bf16* b = static_cast<const bf16*>(uniform_ptr((at.wave >= 2 ? Wv : Wg) + static_cast<int64_t>(e) * hidden * width));
+    uint32_t a_off[4], b_off[4], a_frag[4], b_frag[4];
+    at.along(a_off, width, [&](int r) { return min(max(rows[min(row0 + r, end - 1)], int64_t(0)), tokens - 1); });
+    at.along(b_off, width, [&](int r) { return min(n0 + (r & 127), hidden - 1); });
+    at.fragments(a_frag, false, at.wm * 128);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) b_frag[t] = along_fragment((t < 2 ? 0 : 128) + at.wn * 64 + (t & 1) * 32);
+    f32x16 acc[4][4];
+    clear(acc);
+    mfma_stage::across_loop<false, false>(
+        lds, [&](int kt) { return a + kt * kTileK; }, [&](int kt) { return b + kt * kTileK; }, a_off, b_off, at.a_lds,
+        at.b_lds, a_frag, b_frag, static_cast<int>(width / kTileK), acc);
+    __syncthreads();  // every wave is done reading the stages
+    const int64_t first = n0 + at.wn * 64, blocks = hidden / 32;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        if (first + t * 32 >= hidden) break;
+        float b0[16], b1[16];
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+            const int64_t c = static_cast<int64_t>(e) * hidden + first + t * 32 + acc_column(v);
+            b0[v] = to_f32(bg[c]);
+            b1[v] = to_f32(bv[c]);
+        }
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) {
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                acc[mt][t][v] += b0[v];
+                acc[mt][t + 2][v] += b1[v];
+            }
+            if (keep_g)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int64_t o = kept_at(slot, blocks, first / 32 + t, at.wm * 4 + mt, j, at.lane);
+                    store4(keep_g + o, acc[mt][t][j * 4], acc[mt][t][j * 4 + 1], acc[mt][t][j * 4 + 2], acc[mt][t][j * 4 + 3]);
+                    store4(keep_v + o, acc[mt][t + 2][j * 4], acc[mt][t + 2][j * 4 + 1], acc[mt][t + 2][j * 4 + 2],
+                           acc[mt][t + 2][j * 4 + 3]);
+                }
+        }
+    }
+    store_wave<2>(lds + at.wave * (128 * 128), h + (row0 + at.wm * 128) * hidden + first, hidden, end - row0 - at.wm * 128,
+                  hidden - first, [&](int mt, int t, int v) { return glu(acc[mt][t][v], acc[mt][t + 2][v]); });
+}
+
+// y = W_o h + b_o of a slot's pairs x 256 columns.
+__global__ __launch_bounds__(mfma_stage::kThreads, 1) void tile_output_kernel(
+    const bf16* __restrict__ h, const bf16* __restrict__ Wo, const bf16* __restrict__ bo, float* __restrict__ y, Slots slots,
+    int64_t max_slots, int64_t width, int64_t hidden, uint32_t n_tiles) {
+    __shared__ __attribute__((aligned(1024))) char lds[kTileLds];
+    uint32_t slot, tile_n;
+    if (!slot_tile(slots, max_slots, n_tiles, slot, tile_n)) return;
+    const int e = slots.expert[slot];
+    const int64_t row0 = slots.row[slot], end = slots.end[slot], n0 = static_cast<int64_t>(tile_n) * kTile;
+    const TilePlace at(lds);
+    const bf16* a = static_cast<const bf16*>(uniform_ptr(h + row0 * hidden));
+    const bf16* b = static_cast<const bf16*>(uniform_ptr(Wo + static_cast<int64_t>(e) * width * hidden));
+    uint32_t a_off[4], b_off[4], a_frag[4], b_frag[4];
+    at.along(a_off, hidden, [&](int r) { return min(static_cast<int64_t>(r), end - row0 - 1); });
+    at.along(b_off, hidden, [&](int r) { return min(n0 + r, width - 1); });
+    at.fragments(a_frag, false, at.wm * 128);
+    at.fragments(b_frag, false, at.wn * 128);
+    f32x16 acc[4][4];
+    clear(acc);
+    mfma_stage::across_loop<false, false>(
+        lds, [&](int kt) { return a + kt * kTileK; }, [&](int kt) { return b + kt * kTileK; }, a_off, b_off, at.a_lds,
+        at.b_lds, a_frag, b_frag, static_cast<int>(hidden / kTileK), acc);
+    const int64_t first = n0 + at.wn * 128, r0 = row0 + at.wm * 128;
+    float bias[4][16];
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+            bias[t][v] = to_f32(bo[static_cast<int64_t>(e) * width + min(first + t * 32 + acc_column(v), width - 1)]);
+    store_wave_f32(y + r0 * width + first, width, end - r0, width - first,
+                   [&](int mt, int t, int v) { return acc[mt][t][v] + bias[t][v]; });
+}
+
+// The pairs' rows of x and dout, padded to whole slots with zeros, and <dout, b_o>. A wave per row.
+__global__ __launch_bounds__(256) void tile_gather_kernel(const bf16* __restrict__ x, const bf16* __restrict__ d_out,
+                                                          const int64_t* __restrict__ rows, const bf16* __restrict__ bo,
+                                                          bf16* __restrict__ xs, bf16* __restrict__ ds, float* __restrict__ dot,
+                                                          Slots slots, int64_t max_slots, int64_t tokens, int64_t width) {
+    const int64_t padded = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / kWave, slot = padded / kTile;
+    if (slot >= slots.expert[max_slots]) return;
+    const int64_t p = slots.row[slot] + padded % kTile;
+    const bool real = p < slots.end[slot];
+    const int64_t t = real ? min(max(rows[p], int64_t(0)), tokens - 1) : 0, e = slots.expert[slot];
+    float sum = 0.0f;
+    for (int64_t c = lane_id() * 8; c < width; c += kWave * 8) {
+        uint4 a = make_uint4(0, 0, 0, 0), d = a;
+        if (real) {
+            if (xs) a = *reinterpret_cast<const uint4*>(x + t * width + c);
+            d = *reinterpret_cast<const uint4*>(d_out + t * width + c);
+        }
+        if (xs) *reinterpret_cast<uint4*>(xs + padded * width + c) = a;
+        *reinterpret_cast<uint4*>(ds + padded * width + c) = d;
+        if (dot && real) {
+            const uint4 b = *reinterpret_cast<const uint4*>(bo + e * width + c);
+            const uint32_t dw[4] = {d.x, d.y, d.z, d.w}, bw[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                sum = fmaf(__uint_as_float(dw[i] << 16), __uint_as_float(bw[i] << 16), sum);
+                sum = fmaf(__uint_as_float(dw[i] & 0xffff0000u), __uint_as_float(bw[i] & 0xffff0000u), sum);
+            }
+        }
+    }
+    if (dot && real) {
+        sum = wave_sum_xor(sum);
+        if (lane_id() == 0) dot[p] = sum;
+    }
+}
+
+// d' of a slot x 256 hidden units and what follows: dg and dv side by side (rows of 2
+// hidden), w h, all padded, and each pair's part of dw from a wave's 128 units.
+__global__ __launch_bounds__(mfma_stage::kThreads, 1) void tile_hidden_gradient_kernel(
+    const bf16* __restrict__ ds, const bf16* __restrict__ Wo, const float* __restrict__ keep_g, const float* __restrict__ keep_v,
+    const float* __restrict__ sorted_w, float share, bf16* __restrict__ dgv, bf16* __restrict__ wh,
+    float* __restrict__ dw_part, Slots slots, int64_t max_slots, int64_t pairs, int64_t width, int64_t hidden,
+    uint32_t n_tiles) {
+    __shared__ __attribute__((aligned(1024))) char lds[kTileLds];
+    uint32_t slot, tile_n;
+    if (!slot_tile(slots, max_slots, n_tiles, slot, tile_n)) return;
+    const int e = slots.expert[slot];
+    const int64_t row0 = slots.row[slot], end = slots.end[slot], n0 = static_cast<int64_t>(tile_n) * kTile;
+    const int64_t padded = static_cast<int64_t>(slot) * kTile;
+    const TilePlace at(lds);
+    const bf16* a = static_cast<const bf16*>(uniform_ptr(ds + padded * width));
+    const bf16* b = static_cast<const bf16*>(uniform_ptr(Wo + static_cast<int64_t>(e) * width * hidden));
+    uint32_t a_off[4], b_off[4], a_frag[4], b_frag[4];
+    at.along(a_off, width, [&](int r) { return r; });
+    at.across(b_off, hidden, n0, hidden);
+    at.fragments(a_frag, false, at.wm * 128);
+    at.fragments(b_frag, true, at.wn * 128);
+    f32x16 acc[4][4];
+    clear(acc);
+    mfma_stage::across_loop<false, true>(
+        lds, [&](int kt) { return a + kt * kTileK; }, [&](int kt) { return b + kt * kTileK * hidden; }, a_off, b_off, at.a_lds,
+        at.b_lds, a_frag, b_frag, static_cast<int>(width / kTileK), acc);
+    __syncthreads();  // every wave is done reading the stages
+    const int64_t first = n0 + at.wn * 128, blocks = hidden / 32;
+    char* region = lds + at.wave * (3 * 128 * 64);
+    float* part = dw_part + (2 * static_cast<int64_t>(tile_n) + at.wn) * pairs;
+    // 32 columns at a time: dg, dv and w h in three regions of 128 x 32, so that no product is kept beside its sums
+    const int64_t r0 = padded + at.wm * 128;
+    float weight[4], sum[4] = {};
+    bool real[4];
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+        const int64_t p = row0 + at.wm * 128 + mt * 32 + (at.lane & 31);
+        real[mt] = p < end;
+        weight[mt] = !real[mt] ? 0.0f : sorted_w ? sorted_w[p] : share;
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        if (first + t * 32 >= hidden) break;  // the same for the wave
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                __builtin_amdgcn_sched_barrier(0);
+                const int64_t o = kept_at(slot, blocks, first / 32 + t, at.wm * 4 + mt, j, at.lane);
+                const float4 g4 = load4(keep_g + o), v4 = load4(keep_v + o);
+                const float g[4] = {g4.x, g4.y, g4.z, g4.w}, v[4] = {v4.x, v4.y, v4.z, v4.w};
+                float dg[4], dv[4], h[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const GluGradient o4 = glu_gradient(g[q], v[q], acc[mt][t][j * 4 + q], weight[mt]);
+                    sum[mt] += real[mt] ? o4.dw : 0.0f;
+                    dg[q] = real[mt] ? o4.dg : 0.0f;
+                    dv[q] = real[mt] ? o4.dv : 0.0f;
+                    h[q] = real[mt] ? o4.wh : 0.0f;
+                }
+                const int r = mt * 32 + (at.lane & 31), c = (at.lane >> 5) * 4 + j * 8;
+                put_four<1>(region, r, c, dg[0], dg[1], dg[2], dg[3]);
+                put_four<1>(region + 128 * 64, r, c, dv[0], dv[1], dv[2], dv[3]);
+                put_four<1>(region + 2 * 128 * 64, r, c, h[0], h[1], h[2], h[3]);
+            }
+        bf16* out = dgv + r0 * 2 * hidden + first + t * 32;
+        flush_wave<1>(region, out, 2 * hidden, 128, 32);
+        flush_wave<1>(region + 128 * 64, out + hidden, 2 * hidden, 128, 32);
+        flush_wave<1>(region + 2 * 128 * 64, wh + r0 * hidden + first + t * 32, hidden, 128, 32);
+    }
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+        sum[mt] += __shfl_xor(sum[mt], 32, kWave);
+        if (at.lane < 32 && real[mt]) part[row0 + at.wm * 128 + mt * 32 + at.lane] = sum[mt];
+    }
+}
+
+// dx of a slot's pairs x 256 columns: [dg dv] [W_g ; W_v], one sum over 2 hidden.
+__global__ __launch_bounds__(mfma_stage::kThreads, 1) void tile_input_gradient_kernel(
+    const bf16* __restrict__ dgv, const bf16* __restrict__ Wg, const bf16* __restrict__ Wv, float* __restrict__ dx, Slots slots,
+    int64_t max_slots, int64_t width, int64_t hidden, uint32_t n_tiles) {
+    __shared__ __attribute__((aligned(1024))) char lds[kTileLds];
+    uint32_t slot, tile_n;
+    if (!slot_tile(slots, max_slots, n_tiles, slot, tile_n)) return;
+    const int e = slots.expert[slot];
+    const int64_t row0 = slots.row[slot], end = slots.end[slot], n0 = static_cast<int64_t>(tile_n) * kTile;
+    const TilePlace at(lds);
+    const bf16* a = static_cast<const bf16*>(uniform_ptr(dgv + static_cast<int64_t>(slot) * kTile * 2 * hidden));
+    const bf16* b0 = static_cast<const bf16*>(uniform_ptr(Wg + static_cast<int64_t>(e) * hidden * width));
+    const bf16* b1 = static_cast<const bf16*>(uniform_ptr(Wv + static_cast<int64_t>(e) * hidden * width));
+    uint32_t a_off[4], b_off[4], a_frag[4], b_frag[4];
+    at.along(a_off, 2 * hidden, [&](int r) { return r; });
+    at.across(b_off, width, n0, width);
+    at.fragments(a_frag, false, at.wm * 128);
+    at.fragments(b_frag, true, at.wn * 128);
+    f32x16 acc[4][4];
+    clear(acc);
+    const int steps = static_cast<int>(hidden / kTileK);
+    mfma_stage::across_loop<false, true>(
+        lds, [&](int kt) { return a + kt * kTileK; },
+        [&](int kt) { return kt < steps ? b0 + kt * kTileK * width : b1 + (kt - steps) * kTileK * width; }, a_off, b_off,
+        at.a_lds, at.b_lds, a_frag, b_frag, 2 * steps, acc);
+    const int64_t first = n0 + at.wn * 128, r0 = row0 + at.wm * 128;
+    store_wave_f32(dx + r0 * width + first, width, end - r0, width - first,
+                   [&](int mt, int t, int v) { return acc[mt][t][v]; });
+}
+
+// The three weights' gradients of every expert, in tiles of 256 x 256: sums over its
+// padded rows. `which` 0: dW_g, 1: dW_v, 2: dW_o; a NULL one is not wanted.
+__global__ __launch_bounds__(mfma_stage::kThreads, 1) void tile_weight_gradient_kernel(
+    const bf16* __restrict__ dgv, const bf16* __restrict__ wh, const bf16* __restrict__ xs, const bf16* __restrict__ ds,
+    const int64_t* __restrict__ offsets, Slots slots, bf16* __restrict__ dWg, bf16* __restrict__ dWv, bf16* __restrict__ dWo,
+    int64_t pairs, int64_t width, int64_t hidden, uint32_t w_tiles, uint32_t h_tiles, uint32_t tiles) {
+    __shared__ __attribute__((aligned(1024))) char lds[kTileLds];
+    const uint32_t per = (tiles + 7) / 8, i = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if ((blockIdx.x >> 3) >= per || i >= tiles) return;
+    const uint32_t one = w_tiles * h_tiles, e = i / (3 * one), which = i % (3 * one) / one, within = i % one;
+    bf16* C = which == 0 ? dWg : which == 1 ? dWv : dWo;
+    if (!C) return;
+    const bool out = which == 2;
+    const int64_t M = out ? width : hidden, N = out ? hidden : width;
+    const uint32_t n_tiles = out ? h_tiles : w_tiles;
+    const int64_t m0 = static_cast<int64_t>(within / n_tiles) * kTile, n0 = static_cast<int64_t>(within % n_tiles) * kTile;
+    const int64_t lo = min(max(offsets[e], int64_t(0)), pairs), count = min(max(offsets[e + 1], lo), pairs) - lo;
+    const int64_t row = static_cast<int64_t>(slots.first[e]) * kTile;
+    const int64_t lda = out ? width : 2 * hidden, ldb = out ? hidden : width;
+    const TilePlace at(lds);
+    const bf16* a = static_cast<const bf16*>(uniform_ptr((out ? ds : dgv + (which == 1 ? hidden : 0)) + row * lda));
+    const bf16* b = static_cast<const bf16*>(uniform_ptr((out ? wh : xs) + row * ldb));
+    uint32_t a_off[4], b_off[4], a_frag[4], b_frag[4];
+    at.across(a_off, lda, m0, M);
+    at.across(b_off, ldb, n0, N);
+    at.fragments(a_frag, true, at.wm * 128);
+    at.fragments(b_frag, true, at.wn * 128);
+    f32x16 acc[4][4];
+    clear(acc);
+    const int nk = static_cast<int>((count + kTileK - 1) / kTileK);
+    if (nk > 0)  // the same for the workgroup
+        mfma_stage::across_loop<true, true>(
+            lds, [&](int kt) { return a + kt * kTileK * lda; }, [&](int kt) { return b + kt * kTileK * ldb; }, a_off, b_off,
+            at.a_lds, at.b_lds, a_frag, b_frag, nk, acc);
+    __syncthreads();  // every wave is done reading the stages
+    const int64_t r = m0 + at.wm * 128, c = n0 + at.wn * 128;
+    store_wave<4>(lds + at.wave * (128 * 256), C + static_cast<int64_t>(e) * M * N + r * N + c, N, M - r, N - c,
+                  [&](int mt, int t, int v) { return acc[mt][t][v]; });
+}
+
 // ------------------------------------------------------- rows and columns ---
 // out[t] = sum over the token's pairs of weight x row, in the order of its slots, rounded
 // once; pairs past the valid ones count nothing. weights NULL: `share` each.
@@ -463,18 +870,19 @@ __global__ __launch_bounds__(256) void weight_gradient_kernel(const float* __res
 // columns, four waves over the rows), then each expert's slots in order.
 template <typename TA>
 __global__ __launch_bounds__(256) void slot_sums_kernel(const TA* __restrict__ a, int64_t lda, const float* __restrict__ weights,
-                                                        float share, bool weighted, Slots slots, int64_t max_slots, int64_t rows,
-                                                        int64_t columns, float* __restrict__ part) {
+                                                        float share, bool weighted, bool padded, Slots slots, int64_t max_slots,
+                                                        int64_t rows, int64_t columns, float* __restrict__ part) {
     const int64_t slot = blockIdx.x;
     if (slot >= slots.expert[max_slots]) return;
     __shared__ float sh[4][kWave];
     const int wave = threadIdx.x / kWave;
     const int64_t c = static_cast<int64_t>(blockIdx.y) * kWave + lane_id();
     const int64_t r0 = slots.row[slot], end = min(slots.end[slot], r0 + rows);
+    const int64_t shift = padded ? slot * rows - r0 : 0;  // from a pair to its row of `a`
     float sum = 0.0f;
     if (c < columns)
         for (int64_t r = r0 + wave; r < end; r += 4)
-            sum = fmaf(weighted ? (weights ? weights[r] : share) : 1.0f, to_f32(a[r * lda + c]), sum);
+            sum = fmaf(weighted ? (weights ? weights[r] : share) : 1.0f, to_f32(a[(r + shift) * lda + c]), sum);
     sh[wave][lane_id()] = sum;
     __syncthreads();
     if (wave == 0 && c < columns)
@@ -496,7 +904,22 @@ struct Shape {
     int dtype;
 };
 inline size_t element(int dtype) { return dtype == KOEMI_F32 ? 4 : 2; }
-inline int64_t most_slots(const Shape& s) { return ceil_div(s.pairs, any_rows(s.pairs, s.experts)) + s.experts; }
+// Which path a shape takes: the bf16 tiles where their alignment holds, their 32-bit
+// offsets reach and the experts' segments average at least a quarter of a tile's rows.
+inline bool tile_shape(const Shape& s) {
+    const int64_t reach = int64_t(1) << 31;
+    return s.dtype == KOEMI_BF16 && s.width % 64 == 0 && s.hidden % 64 == 0 && s.pairs >= 64 * s.experts &&
+           s.tokens * s.width < reach && s.hidden * s.width < reach && 512 * s.hidden < reach;
+}
+inline int64_t slot_rows(const Shape& s) { return tile_shape(s) ? kTile : any_rows(s.pairs, s.experts); }
+inline int64_t most_slots(const Shape& s) { return ceil_div(s.pairs, slot_rows(s)) + s.experts; }
+
+// Rows of the gathered operands of the backward: whole slots for the tiles.
+inline int64_t gathered_rows(const Shape& s) { return tile_shape(s) ? most_slots(s) * kTile : s.pairs; }
+// Floats of g (and of v) that the forward keeps.
+inline int64_t kept_floats(const Shape& s) {
+    return tile_shape(s) ? most_slots(s) * kTile * s.hidden : s.pairs * padded_hidden(s.hidden);
+}
 
 // Carves a workspace, or only measures it (base null).
 struct Carver {
@@ -526,7 +949,7 @@ inline ForwardSpace forward_space(const Shape& s, void* base) {
     Carver c{static_cast<char*>(base)};
     ForwardSpace w;
     w.slots = c.slots(s);
-    w.h = c.take<float>(s.pairs * padded_hidden(s.hidden));
+    w.h = c.take<float>(tile_shape(s) ? s.pairs * s.hidden / 2 : s.pairs * padded_hidden(s.hidden));
     w.y = c.take<float>(s.pairs * s.width);
     w.bytes = c.used;
     return w;
@@ -540,17 +963,23 @@ struct BackwardSpace {
 inline BackwardSpace backward_space(const Shape& s, void* base) {
     Carver c{static_cast<char*>(base)};
     BackwardSpace w;
-    const int64_t ld = padded_hidden(s.hidden);
+    const int64_t ld = padded_hidden(s.hidden), rows = gathered_rows(s);
     w.slots = c.slots(s);
-    w.dg = c.take<float>(s.pairs * ld);
-    w.dv = c.take<float>(s.pairs * ld);
-    w.wh = c.take<float>(s.pairs * ld);
+    if (tile_shape(s)) {  // dg and dv as bf16 side by side, w h bf16
+        w.dg = c.take<float>(rows * s.hidden);
+        w.dv = nullptr;
+        w.wh = c.take<float>(rows * s.hidden / 2);
+    } else {
+        w.dg = c.take<float>(rows * ld);
+        w.dv = c.take<float>(rows * ld);
+        w.wh = c.take<float>(rows * ld);
+    }
     w.dx = c.take<float>(s.pairs * s.width);
     w.dw_part = c.take<float>(2 * ceil_div(s.hidden, kAnyCols) * s.pairs);
     w.dot = c.take<float>(s.pairs);
-    w.sums = c.take<float>(most_slots(s) * std::max(s.width, s.hidden));
-    w.xs = c.take<char>(s.pairs * s.width * static_cast<int64_t>(element(s.dtype)));
-    w.ds = c.take<char>(s.pairs * s.width * static_cast<int64_t>(element(s.dtype)));
+    w.sums = c.take<float>(most_slots(s) * std::max(s.width, 2 * s.hidden));
+    w.xs = c.take<char>(rows * s.width * static_cast<int64_t>(element(s.dtype)));
+    w.ds = c.take<char>(rows * s.width * static_cast<int64_t>(element(s.dtype)));
     w.bytes = c.used;
     return w;
 }
@@ -584,7 +1013,7 @@ void by_bytes(int bytes, F f) {
 }
 void find_slots(const Shape& s, const int64_t* offsets, const Slots& slots, hipStream_t q) {
     hipLaunchKernelGGL(slots_kernel, dim3(1), dim3(kSlotThreads), 0, q, offsets, s.experts, s.pairs,
-                       static_cast<int64_t>(any_rows(s.pairs, s.experts)), most_slots(s), slots);
+                       slot_rows(s), most_slots(s), slots);
 }
 template <typename T>
 void combine(const float* rows, const int64_t* positions, const int64_t* offsets, const float* weights, float share, void* out,
@@ -676,8 +1105,7 @@ int any_backward(const Shape& s, const void* d_out, const void* x, const int64_t
     auto columns = [&](auto* a, int64_t lda, bool weighted, int64_t n, void* c) {
         using TA = std::remove_pointer_t<decltype(a)>;
         hipLaunchKernelGGL(slot_sums_kernel<TA>, dim3(static_cast<unsigned>(slots), static_cast<unsigned>(ceil_div(n, kWave))),
-                           dim3(256), 0, q, a, lda, sorted_w, share, weighted, w.slots, slots,
-                           static_cast<int64_t>(any_rows(s.pairs, s.experts)), n, w.sums);
+                           dim3(256), 0, q, a, lda, sorted_w, share, weighted, false, w.slots, slots, slot_rows(s), n, w.sums);
         hipLaunchKernelGGL(expert_sums_kernel<T>, dim3(grid_for(n, 256), static_cast<unsigned>(s.experts)), dim3(256), 0, q,
                            w.sums, w.slots.first, static_cast<T*>(c), n);
     };
@@ -685,6 +1113,73 @@ int any_backward(const Shape& s, const void* d_out, const void* x, const int64_t
     if (d.bv) columns(w.dv, ld, false, s.hidden, d.bv);
     if (d.bo) columns(ds, s.width, true, s.width, d.bo);
     return check_launch("koemi_moe_experts_backward");
+}
+
+int tile_forward(const Shape& s, const void* x, const int64_t* rows, const int64_t* offsets, const int64_t* positions,
+                 const float* pair_weights, const Weights& m, void* out, float* keep, const ForwardSpace& w, hipStream_t q) {
+    const int64_t slots = most_slots(s);
+    const uint32_t h_tiles = static_cast<uint32_t>(ceil_div(s.hidden, 128)), w_tiles = static_cast<uint32_t>(ceil_div(s.width, kTile));
+    bf16* h = reinterpret_cast<bf16*>(w.h);
+    find_slots(s, offsets, w.slots, q);
+    hipLaunchKernelGGL(tile_hidden_kernel, dim3(tiles_grid(slots, h_tiles)), dim3(mfma_stage::kThreads), 0, q,
+                       static_cast<const bf16*>(x), rows, s.tokens, static_cast<const bf16*>(m.Wg),
+                       static_cast<const bf16*>(m.bg), static_cast<const bf16*>(m.Wv), static_cast<const bf16*>(m.bv), keep,
+                       keep ? keep + kept_floats(s) : nullptr, h, w.slots, slots, s.width, s.hidden, h_tiles);
+    hipLaunchKernelGGL(tile_output_kernel, dim3(tiles_grid(slots, w_tiles)), dim3(mfma_stage::kThreads), 0, q, h,
+                       static_cast<const bf16*>(m.Wo), static_cast<const bf16*>(m.bo), w.y, w.slots, slots, s.width, s.hidden,
+                       w_tiles);
+    combine<bf16>(w.y, positions, offsets, pair_weights, 1.0f / static_cast<float>(s.top_k), out, s, q);
+    return check_launch("koemi_moe_experts_forward(tiles)");
+}
+
+int tile_backward(const Shape& s, const void* d_out, const void* x, const int64_t* rows, const int64_t* offsets,
+                  const int64_t* positions, const float* sorted_w, const Weights& m, const float* keep, const Gradients& d,
+                  const BackwardSpace& w, hipStream_t q) {
+    const int64_t slots = most_slots(s), padded = gathered_rows(s);
+    const float share = 1.0f / static_cast<float>(s.top_k);
+    const uint32_t h_tiles = static_cast<uint32_t>(ceil_div(s.hidden, kTile)), w_tiles = static_cast<uint32_t>(ceil_div(s.width, kTile));
+    bf16 *xs = static_cast<bf16*>(w.xs), *ds = static_cast<bf16*>(w.ds);
+    bf16 *dgv = reinterpret_cast<bf16*>(w.dg), *wh = reinterpret_cast<bf16*>(w.wh);
+    const dim3 threads(mfma_stage::kThreads);
+    find_slots(s, offsets, w.slots, q);
+    hipLaunchKernelGGL(tile_gather_kernel, dim3(grid_for(padded, 4)), dim3(256), 0, q, static_cast<const bf16*>(x),
+                       static_cast<const bf16*>(d_out), rows, static_cast<const bf16*>(m.bo), d.Wg || d.Wv ? xs : nullptr, ds,
+                       d.weights ? w.dot : nullptr, w.slots, slots, s.tokens, s.width);
+    hipLaunchKernelGGL(tile_hidden_gradient_kernel, dim3(tiles_grid(slots, h_tiles)), threads, 0, q, ds,
+                       static_cast<const bf16*>(m.Wo), keep, keep + kept_floats(s), sorted_w, share, dgv, wh, w.dw_part,
+                       w.slots, slots, s.pairs, s.width, s.hidden, h_tiles);
+    if (d.x) {
+        hipLaunchKernelGGL(tile_input_gradient_kernel, dim3(tiles_grid(slots, w_tiles)), threads, 0, q, dgv,
+                           static_cast<const bf16*>(m.Wg), static_cast<const bf16*>(m.Wv), w.dx, w.slots, slots, s.width,
+                           s.hidden, w_tiles);
+        combine<bf16>(w.dx, positions, offsets, nullptr, 1.0f, d.x, s, q);
+    }
+    if (d.weights)
+        hipLaunchKernelGGL(weight_gradient_kernel, dim3(grid_for(s.pairs, 256)), dim3(256), 0, q, w.dw_part,
+                           static_cast<int>(2 * h_tiles), w.dot, positions, offsets + s.experts, d.weights, s.pairs);
+    if (d.Wg || d.Wv || d.Wo) {
+        const uint32_t tiles = static_cast<uint32_t>(s.experts) * 3 * w_tiles * h_tiles;
+        hipLaunchKernelGGL(tile_weight_gradient_kernel, dim3((tiles + 7) / 8 * 8), threads, 0, q, dgv, wh, xs, ds, offsets,
+                           w.slots, static_cast<bf16*>(d.Wg), static_cast<bf16*>(d.Wv), static_cast<bf16*>(d.Wo), s.pairs,
+                           s.width, s.hidden, w_tiles, h_tiles, tiles);
+    }
+    auto columns = [&](const bf16* a, int64_t lda, bool weighted, int64_t n, void* c) {
+        hipLaunchKernelGGL(slot_sums_kernel<bf16>, dim3(static_cast<unsigned>(slots), static_cast<unsigned>(ceil_div(n, kWave))),
+                           dim3(256), 0, q, a, lda, sorted_w, share, weighted, true, w.slots, slots, slot_rows(s), n, w.sums);
+        hipLaunchKernelGGL(expert_sums_kernel<bf16>, dim3(grid_for(n, 256), static_cast<unsigned>(s.experts)), dim3(256), 0, q,
+                           w.sums, w.slots.first, static_cast<bf16*>(c), n);
+    };
+    if (d.bg) columns(dgv, 2 * s.hidden, false, s.hidden, d.bg);
+    if (d.bv) columns(dgv + s.hidden, 2 * s.hidden, false, s.hidden, d.bv);
+    if (d.bo) columns(ds, s.width, true, s.width, d.bo);
+    return check_launch("koemi_moe_experts_backward(tiles)");
+}
+
+// The tiles' copies take 16 bytes of a row at once.
+inline bool aligned16(std::initializer_list<const void*> pointers) {
+    uintptr_t all = 0;
+    for (const void* p : pointers) all |= reinterpret_cast<uintptr_t>(p);
+    return all % 16 == 0;
 }
 
 }  // namespace
@@ -696,7 +1191,7 @@ extern "C" size_t koemi_moe_experts_saved_bytes(int64_t tokens, int64_t top_k, i
                                                 int64_t expert_count, int dtype) {
     const Shape s{tokens * top_k, tokens, width, hidden, expert_count, top_k, dtype};
     if (check_shape("koemi_moe_experts_saved_bytes", s) != KOEMI_OK) return 0;
-    return static_cast<size_t>(2 * s.pairs * padded_hidden(hidden)) * sizeof(float);
+    return static_cast<size_t>(2 * kept_floats(s)) * sizeof(float);
 }
 
 extern "C" size_t koemi_moe_experts_workspace_bytes(int64_t tokens, int64_t top_k, int64_t width, int64_t hidden,
@@ -725,6 +1220,11 @@ extern "C" int koemi_moe_experts_forward(const void* context, const int64_t* sor
     if (!workspace || workspace_bytes < w.bytes) return fail(KOEMI_ERR_INVALID, "%s: workspace too small", what);
     float* keep = static_cast<float*>(saved);
     hipStream_t q = as_stream(stream);
+    if (tile_shape(s)) {
+        if (!aligned16({context, m.Wg, m.Wv, m.Wo, saved, workspace}))
+            return fail(KOEMI_ERR_INVALID, "%s: operands must be 16-byte aligned", what);
+        return tile_forward(s, context, sorted_rows, segment_offsets, pair_positions, pair_weights, m, output, keep, w, q);
+    }
     if (dtype == KOEMI_F32)
         return any_forward<float>(s, context, sorted_rows, segment_offsets, pair_positions, pair_weights, m, output, keep, w, q);
     if (dtype == KOEMI_F16)
@@ -756,6 +1256,12 @@ extern "C" int koemi_moe_experts_backward(const void* grad_output, const void* c
     if (!workspace || workspace_bytes < w.bytes) return fail(KOEMI_ERR_INVALID, "%s: workspace too small", what);
     const float* keep = static_cast<const float*>(saved);
     hipStream_t q = as_stream(stream);
+    if (tile_shape(s)) {
+        if (!aligned16({grad_output, context, m.Wg, m.Wv, m.Wo, m.bo, saved, workspace, d.Wg, d.Wv, d.Wo}))
+            return fail(KOEMI_ERR_INVALID, "%s: operands must be 16-byte aligned", what);
+        return tile_backward(s, grad_output, context, sorted_rows, segment_offsets, pair_positions, sorted_weights, m, keep, d, w,
+                             q);
+    }
     if (dtype == KOEMI_F32)
         return any_backward<float>(s, grad_output, context, sorted_rows, sorted_experts, segment_offsets, pair_positions,
                                    sorted_weights, m, keep, d, w, q);
