@@ -609,48 +609,106 @@ __global__ __launch_bounds__(mfma_stage::kThreads, 1) void tile_output_kernel(
                    [&](int mt, int t, int v) { return acc[mt][t][v] + bias[t][v]; });
 }
 
-// The pairs' rows of x and dout, padded to whole slots with zeros, and <dout, b_o>. A wave per row.
+// The pairs' rows of x and dout, padded to whole slots with zeros; the rows' parts of <dout,
+// b_o> and the column sums of w dout, both from the values as they pass. A workgroup takes
+// 64 rows and 512 columns, a wave every fourth row, a lane eight columns.
+constexpr int kGatherRows = 64, kGatherColumns = 512;
 __global__ __launch_bounds__(256) void tile_gather_kernel(const bf16* __restrict__ x, const bf16* __restrict__ d_out,
                                                           const int64_t* __restrict__ rows, const bf16* __restrict__ bo,
-                                                          bf16* __restrict__ xs, bf16* __restrict__ ds, float* __restrict__ dot,
-                                                          Slots slots, int64_t max_slots, int64_t tokens, int64_t width) {
-    const int64_t padded = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / kWave, slot = padded / kTile;
+                                                          const float* __restrict__ sorted_w, float share,
+                                                          bf16* __restrict__ xs, bf16* __restrict__ ds,
+                                                          float* __restrict__ dot_part, float* __restrict__ sums, Slots slots,
+                                                          int64_t max_slots, int64_t pairs, int64_t tokens, int64_t width) {
+    __shared__ float sh[3][kWave][8];
+    const int64_t quarter = blockIdx.x, slot = quarter / (kTile / kGatherRows);
     if (slot >= slots.expert[max_slots]) return;
-    const int64_t p = slots.row[slot] + padded % kTile;
-    const bool real = p < slots.end[slot];
-    const int64_t t = real ? min(max(rows[p], int64_t(0)), tokens - 1) : 0, e = slots.expert[slot];
-    float sum = 0.0f;
-    for (int64_t c = lane_id() * 8; c < width; c += kWave * 8) {
+    const int wave = threadIdx.x / kWave, lane = lane_id();
+    const int64_t c = static_cast<int64_t>(blockIdx.y) * kGatherColumns + lane * 8, e = slots.expert[slot];
+    const int64_t p0 = slots.row[slot] + quarter % (kTile / kGatherRows) * kGatherRows, end = slots.end[slot];
+    const bool in = c < width;
+    auto spread = [](const uint4& u, float (&f)[8]) {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[2 * i] = __uint_as_float(w[i] << 16), f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    };
+    float bias[8] = {}, sum[8] = {};
+    if (dot_part && in) spread(*reinterpret_cast<const uint4*>(bo + e * width + c), bias);
+#pragma unroll 4
+    for (int i = wave; i < kGatherRows; i += 4) {
+        const int64_t p = p0 + i, padded = quarter * kGatherRows + i;
+        const bool real = p < end;
+        const int64_t t = real ? min(max(rows[p], int64_t(0)), tokens - 1) : 0;
         uint4 a = make_uint4(0, 0, 0, 0), d = a;
-        if (real) {
+        if (real && in) {
             if (xs) a = *reinterpret_cast<const uint4*>(x + t * width + c);
             d = *reinterpret_cast<const uint4*>(d_out + t * width + c);
         }
-        if (xs) *reinterpret_cast<uint4*>(xs + padded * width + c) = a;
-        *reinterpret_cast<uint4*>(ds + padded * width + c) = d;
-        if (dot && real) {
-            const uint4 b = *reinterpret_cast<const uint4*>(bo + e * width + c);
-            const uint32_t dw[4] = {d.x, d.y, d.z, d.w}, bw[4] = {b.x, b.y, b.z, b.w};
+        if (in) {
+            if (xs) *reinterpret_cast<uint4*>(xs + padded * width + c) = a;
+            *reinterpret_cast<uint4*>(ds + padded * width + c) = d;
+        }
+        float f[8], dot = 0.0f;
+        spread(d, f);
+        const float w = !real ? 0.0f : sorted_w ? sorted_w[p] : share;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                sum = fmaf(__uint_as_float(dw[i] << 16), __uint_as_float(bw[i] << 16), sum);
-                sum = fmaf(__uint_as_float(dw[i] & 0xffff0000u), __uint_as_float(bw[i] & 0xffff0000u), sum);
-            }
+        for (int q = 0; q < 8; ++q) {
+            dot = fmaf(f[q], bias[q], dot);
+            sum[q] = real ? fmaf(w, f[q], sum[q]) : sum[q];
+        }
+        if (dot_part) {
+            dot = wave_sum_xor(dot);
+            if (lane == 0 && real) dot_part[blockIdx.y * pairs + p] = dot;
         }
     }
-    if (dot && real) {
-        sum = wave_sum_xor(sum);
-        if (lane_id() == 0) dot[p] = sum;
+    if (!sums) return;
+    if (wave > 0)
+#pragma unroll
+        for (int q = 0; q < 8; ++q) sh[wave - 1][lane][q] = sum[q];
+    __syncthreads();
+    if (wave != 0 || !in) return;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) sum[q] = (sum[q] + sh[0][lane][q]) + (sh[1][lane][q] + sh[2][lane][q]);
+    store4(sums + quarter * width + c, sum[0], sum[1], sum[2], sum[3]);
+    store4(sums + quarter * width + c + 4, sum[4], sum[5], sum[6], sum[7]);
+}
+
+// Column sums of a wave's region of 128 rows x 32 columns (put_four<1>), as products
+// with ones on the matrix cores: the region's rows are K, read transposed.
+__device__ __forceinline__ void region_sums(const char* region, float* out) {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+    const int lane = lane_id(), chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    mfma_stage::bf16x8 ones;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ones[i] = static_cast<bf16>(1.0f);
+    f32x16 acc = {};
+#pragma unroll
+    for (int k0 = 0; k0 < 128; k0 += 16) {
+        union {
+            s16x4 half[2];
+            mfma_stage::bf16x8 whole;
+        } u;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int r = k0 + 8 * (lane >> 5) + 4 * j + ((lane & 15) >> 2);
+            u.half[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(region + r * 64 + ((chunk ^ (r & 3)) * 16) + (lane & 1) * 8));
+        }
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u.whole, ones, acc, 0, 0, 0);
     }
+    if ((lane & 31) == 0)  // every column of the product is the sums
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            store4(out + (lane >> 5) * 4 + j * 8, acc[j * 4], acc[j * 4 + 1], acc[j * 4 + 2], acc[j * 4 + 3]);
 }
 
 // d' of a slot x 256 hidden units and what follows: dg and dv side by side (rows of 2
-// hidden), w h, all padded, and each pair's part of dw from a wave's 128 units.
+// hidden), w h, all padded, each pair's part of dw from a wave's 128 units, and (sums,
+// NULL: not wanted) the column sums of dg and dv over a wave's 128 rows.
 __global__ __launch_bounds__(mfma_stage::kThreads, 1) void tile_hidden_gradient_kernel(
     const bf16* __restrict__ ds, const bf16* __restrict__ Wo, const float* __restrict__ keep_g, const float* __restrict__ keep_v,
     const float* __restrict__ sorted_w, float share, bf16* __restrict__ dgv, bf16* __restrict__ wh,
-    float* __restrict__ dw_part, Slots slots, int64_t max_slots, int64_t pairs, int64_t width, int64_t hidden,
-    uint32_t n_tiles) {
+    float* __restrict__ dw_part, float* __restrict__ sums, Slots slots, int64_t max_slots, int64_t pairs, int64_t width,
+    int64_t hidden, uint32_t n_tiles) {
     __shared__ __attribute__((aligned(1024))) char lds[kTileLds];
     uint32_t slot, tile_n;
     if (!slot_tile(slots, max_slots, n_tiles, slot, tile_n)) return;
@@ -684,17 +742,31 @@ __global__ __launch_bounds__(mfma_stage::kThreads, 1) void tile_hidden_gradient_
         real[mt] = p < end;
         weight[mt] = !real[mt] ? 0.0f : sorted_w ? sorted_w[p] : share;
     }
+    // block 4 t + mt of kept g and v, loaded while the block before is worked on
+    struct Kept {
+        float4 g[4], v[4];
+    } kept[2];
+    auto fetch = [&](int block, Kept& k) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int64_t o = kept_at(slot, blocks, min(first / 32 + block / 4, blocks - 1), at.wm * 4 + block % 4, j, at.lane);
+            k.g[j] = load4(keep_g + o);
+            k.v[j] = load4(keep_v + o);
+        }
+    };
+    fetch(0, kept[0]);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
         if (first + t * 32 >= hidden) break;  // the same for the wave
 #pragma unroll
-        for (int mt = 0; mt < 4; ++mt)
+        for (int mt = 0; mt < 4; ++mt) {
+            __builtin_amdgcn_sched_barrier(0);
+            const Kept& k = kept[mt % 2];
+            if (t * 4 + mt < 15) fetch(t * 4 + mt + 1, kept[(mt + 1) % 2]);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                __builtin_amdgcn_sched_barrier(0);
-                const int64_t o = kept_at(slot, blocks, first / 32 + t, at.wm * 4 + mt, j, at.lane);
-                const float4 g4 = load4(keep_g + o), v4 = load4(keep_v + o);
-                const float g[4] = {g4.x, g4.y, g4.z, g4.w}, v[4] = {v4.x, v4.y, v4.z, v4.w};
+                const float g[4] = {k.g[j].x, k.g[j].y, k.g[j].z, k.g[j].w}, v[4] = {k.v[j].x, k.v[j].y, k.v[j].z, k.v[j].w};
                 float dg[4], dv[4], h[4];
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
@@ -709,6 +781,12 @@ __global__ __launch_bounds__(mfma_stage::kThreads, 1) void tile_hidden_gradient_
                 put_four<1>(region + 128 * 64, r, c, dv[0], dv[1], dv[2], dv[3]);
                 put_four<1>(region + 2 * 128 * 64, r, c, h[0], h[1], h[2], h[3]);
             }
+        }
+        if (sums) {
+            float* to = sums + (2 * static_cast<int64_t>(slot) + at.wm) * 2 * hidden + first + t * 32;
+            region_sums(region, to);
+            region_sums(region + 128 * 64, to + hidden);
+        }
         bf16* out = dgv + r0 * 2 * hidden + first + t * 32;
         flush_wave<1>(region, out, 2 * hidden, 128, 32);
         flush_wave<1>(region + 128 * 64, out + hidden, 2 * hidden, 128, 32);
@@ -849,9 +927,10 @@ __global__ __launch_bounds__(256) void gather_pairs_kernel(const T* __restrict__
     }
 }
 
-// dw of every pair in token order: its row's parts in order, and <dout, b_o>; 0 past the valid pairs.
+// dw of every pair in token order: the parts of its row's <d', h> and <dout, b_o> in order; 0
+// past the valid pairs.
 __global__ __launch_bounds__(256) void weight_gradient_kernel(const float* __restrict__ part, int parts,
-                                                              const float* __restrict__ dot,
+                                                              const float* __restrict__ dot, int dot_parts,
                                                               const int64_t* __restrict__ positions,
                                                               const int64_t* __restrict__ valid_end, float* __restrict__ dw,
                                                               int64_t pairs) {
@@ -861,7 +940,7 @@ __global__ __launch_bounds__(256) void weight_gradient_kernel(const float* __res
     float sum = 0.0f;
     if (p >= 0 && p < *valid_end) {
         for (int j = 0; j < parts; ++j) sum += part[j * pairs + p];
-        sum += dot[p];
+        for (int j = 0; j < dot_parts; ++j) sum += dot[j * pairs + p];
     }
     dw[i] = sum;
 }
@@ -870,31 +949,33 @@ __global__ __launch_bounds__(256) void weight_gradient_kernel(const float* __res
 // columns, four waves over the rows), then each expert's slots in order.
 template <typename TA>
 __global__ __launch_bounds__(256) void slot_sums_kernel(const TA* __restrict__ a, int64_t lda, const float* __restrict__ weights,
-                                                        float share, bool weighted, bool padded, Slots slots, int64_t max_slots,
-                                                        int64_t rows, int64_t columns, float* __restrict__ part) {
+                                                        float share, bool weighted, Slots slots, int64_t max_slots, int64_t rows,
+                                                        int64_t columns, float* __restrict__ part) {
     const int64_t slot = blockIdx.x;
     if (slot >= slots.expert[max_slots]) return;
     __shared__ float sh[4][kWave];
     const int wave = threadIdx.x / kWave;
     const int64_t c = static_cast<int64_t>(blockIdx.y) * kWave + lane_id();
     const int64_t r0 = slots.row[slot], end = min(slots.end[slot], r0 + rows);
-    const int64_t shift = padded ? slot * rows - r0 : 0;  // from a pair to its row of `a`
     float sum = 0.0f;
     if (c < columns)
         for (int64_t r = r0 + wave; r < end; r += 4)
-            sum = fmaf(weighted ? (weights ? weights[r] : share) : 1.0f, to_f32(a[(r + shift) * lda + c]), sum);
+            sum = fmaf(weighted ? (weights ? weights[r] : share) : 1.0f, to_f32(a[r * lda + c]), sum);
     sh[wave][lane_id()] = sum;
     __syncthreads();
     if (wave == 0 && c < columns)
         part[slot * columns + c] = (sh[0][lane_id()] + sh[1][lane_id()]) + (sh[2][lane_id()] + sh[3][lane_id()]);
 }
+// part: `per` rows a slot, ld apart.
 template <typename T>
 __global__ __launch_bounds__(256) void expert_sums_kernel(const float* __restrict__ part, const int32_t* __restrict__ first,
-                                                          T* __restrict__ out, int64_t columns) {
+                                                          T* __restrict__ out, int per, int64_t ld, int64_t columns) {
     const int64_t e = blockIdx.y, c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
     if (c >= columns) return;
+    const int64_t end = static_cast<int64_t>(first[e + 1]) * per;
     float sum = 0.0f;
-    for (int32_t s = first[e]; s < first[e + 1]; ++s) sum += part[s * columns + c];
+#pragma unroll 8
+    for (int64_t s = static_cast<int64_t>(first[e]) * per; s < end; ++s) sum += part[s * ld + c];
     out[e * columns + c] = from_f32<T>(sum);
 }
 
@@ -956,7 +1037,7 @@ inline ForwardSpace forward_space(const Shape& s, void* base) {
 }
 struct BackwardSpace {
     Slots slots;
-    float *dg, *dv, *wh, *dx, *dw_part, *dot, *sums;
+    float *dg, *dv, *wh, *dx, *dw_part, *dot, *sums, *out_sums;
     void *xs, *ds;
     size_t bytes;
 };
@@ -976,8 +1057,15 @@ inline BackwardSpace backward_space(const Shape& s, void* base) {
     }
     w.dx = c.take<float>(s.pairs * s.width);
     w.dw_part = c.take<float>(2 * ceil_div(s.hidden, kAnyCols) * s.pairs);
-    w.dot = c.take<float>(s.pairs);
-    w.sums = c.take<float>(most_slots(s) * std::max(s.width, 2 * s.hidden));
+    if (tile_shape(s)) {
+        w.dot = c.take<float>(ceil_div(s.width, kGatherColumns) * s.pairs);
+        w.sums = c.take<float>(most_slots(s) * 4 * s.hidden);
+        w.out_sums = c.take<float>(most_slots(s) * (kTile / kGatherRows) * s.width);
+    } else {
+        w.dot = c.take<float>(s.pairs);
+        w.sums = c.take<float>(most_slots(s) * std::max(s.width, s.hidden));
+        w.out_sums = nullptr;
+    }
     w.xs = c.take<char>(rows * s.width * static_cast<int64_t>(element(s.dtype)));
     w.ds = c.take<char>(rows * s.width * static_cast<int64_t>(element(s.dtype)));
     w.bytes = c.used;
@@ -1091,7 +1179,7 @@ int any_backward(const Shape& s, const void* d_out, const void* x, const int64_t
     if (d.x) combine<T>(w.dx, positions, offsets, nullptr, 1.0f, d.x, s, q);
     if (d.weights)
         hipLaunchKernelGGL(weight_gradient_kernel, dim3(grid_for(s.pairs, 256)), dim3(256), 0, q, w.dw_part,
-                           static_cast<int>(2 * h_tiles), w.dot, positions, offsets + s.experts, d.weights, s.pairs);
+                           static_cast<int>(2 * h_tiles), w.dot, 1, positions, offsets + s.experts, d.weights, s.pairs);
     auto product = [&](auto* a, auto* b, void* c, int64_t M, int64_t N, int64_t lda, int64_t ldb) {
         using TA = std::remove_pointer_t<decltype(a)>;
         using TB = std::remove_pointer_t<decltype(b)>;
@@ -1105,9 +1193,9 @@ int any_backward(const Shape& s, const void* d_out, const void* x, const int64_t
     auto columns = [&](auto* a, int64_t lda, bool weighted, int64_t n, void* c) {
         using TA = std::remove_pointer_t<decltype(a)>;
         hipLaunchKernelGGL(slot_sums_kernel<TA>, dim3(static_cast<unsigned>(slots), static_cast<unsigned>(ceil_div(n, kWave))),
-                           dim3(256), 0, q, a, lda, sorted_w, share, weighted, false, w.slots, slots, slot_rows(s), n, w.sums);
+                           dim3(256), 0, q, a, lda, sorted_w, share, weighted, w.slots, slots, slot_rows(s), n, w.sums);
         hipLaunchKernelGGL(expert_sums_kernel<T>, dim3(grid_for(n, 256), static_cast<unsigned>(s.experts)), dim3(256), 0, q,
-                           w.sums, w.slots.first, static_cast<T*>(c), n);
+                           w.sums, w.slots.first, static_cast<T*>(c), 1, n, n);
     };
     if (d.bg) columns(w.dg, ld, false, s.hidden, d.bg);
     if (d.bv) columns(w.dv, ld, false, s.hidden, d.bv);
@@ -1142,12 +1230,14 @@ int tile_backward(const Shape& s, const void* d_out, const void* x, const int64_
     bf16 *dgv = reinterpret_cast<bf16*>(w.dg), *wh = reinterpret_cast<bf16*>(w.wh);
     const dim3 threads(mfma_stage::kThreads);
     find_slots(s, offsets, w.slots, q);
-    hipLaunchKernelGGL(tile_gather_kernel, dim3(grid_for(padded, 4)), dim3(256), 0, q, static_cast<const bf16*>(x),
-                       static_cast<const bf16*>(d_out), rows, static_cast<const bf16*>(m.bo), d.Wg || d.Wv ? xs : nullptr, ds,
-                       d.weights ? w.dot : nullptr, w.slots, slots, s.tokens, s.width);
+    const unsigned blocks = static_cast<unsigned>(ceil_div(s.width, kGatherColumns));
+    hipLaunchKernelGGL(tile_gather_kernel, dim3(static_cast<unsigned>(padded / kGatherRows), blocks), dim3(256), 0, q,
+                       static_cast<const bf16*>(x), static_cast<const bf16*>(d_out), rows, static_cast<const bf16*>(m.bo),
+                       sorted_w, share, d.Wg || d.Wv ? xs : nullptr, ds, d.weights ? w.dot : nullptr,
+                       d.bo ? w.out_sums : nullptr, w.slots, slots, s.pairs, s.tokens, s.width);
     hipLaunchKernelGGL(tile_hidden_gradient_kernel, dim3(tiles_grid(slots, h_tiles)), threads, 0, q, ds,
                        static_cast<const bf16*>(m.Wo), keep, keep + kept_floats(s), sorted_w, share, dgv, wh, w.dw_part,
-                       w.slots, slots, s.pairs, s.width, s.hidden, h_tiles);
+                       d.bg || d.bv ? w.sums : nullptr, w.slots, slots, s.pairs, s.width, s.hidden, h_tiles);
     if (d.x) {
         hipLaunchKernelGGL(tile_input_gradient_kernel, dim3(tiles_grid(slots, w_tiles)), threads, 0, q, dgv,
                            static_cast<const bf16*>(m.Wg), static_cast<const bf16*>(m.Wv), w.dx, w.slots, slots, s.width,
@@ -1156,22 +1246,21 @@ int tile_backward(const Shape& s, const void* d_out, const void* x, const int64_
     }
     if (d.weights)
         hipLaunchKernelGGL(weight_gradient_kernel, dim3(grid_for(s.pairs, 256)), dim3(256), 0, q, w.dw_part,
-                           static_cast<int>(2 * h_tiles), w.dot, positions, offsets + s.experts, d.weights, s.pairs);
+                           static_cast<int>(2 * h_tiles), w.dot, static_cast<int>(blocks), positions, offsets + s.experts,
+                           d.weights, s.pairs);
     if (d.Wg || d.Wv || d.Wo) {
         const uint32_t tiles = static_cast<uint32_t>(s.experts) * 3 * w_tiles * h_tiles;
         hipLaunchKernelGGL(tile_weight_gradient_kernel, dim3((tiles + 7) / 8 * 8), threads, 0, q, dgv, wh, xs, ds, offsets,
                            w.slots, static_cast<bf16*>(d.Wg), static_cast<bf16*>(d.Wv), static_cast<bf16*>(d.Wo), s.pairs,
                            s.width, s.hidden, w_tiles, h_tiles, tiles);
     }
-    auto columns = [&](const bf16* a, int64_t lda, bool weighted, int64_t n, void* c) {
-        hipLaunchKernelGGL(slot_sums_kernel<bf16>, dim3(static_cast<unsigned>(slots), static_cast<unsigned>(ceil_div(n, kWave))),
-                           dim3(256), 0, q, a, lda, sorted_w, share, weighted, true, w.slots, slots, slot_rows(s), n, w.sums);
+    auto expert_sums = [&](const float* part, int per, int64_t ld, int64_t n, void* c) {
         hipLaunchKernelGGL(expert_sums_kernel<bf16>, dim3(grid_for(n, 256), static_cast<unsigned>(s.experts)), dim3(256), 0, q,
-                           w.sums, w.slots.first, static_cast<bf16*>(c), n);
+                           part, w.slots.first, static_cast<bf16*>(c), per, ld, n);
     };
-    if (d.bg) columns(dgv, 2 * s.hidden, false, s.hidden, d.bg);
-    if (d.bv) columns(dgv + s.hidden, 2 * s.hidden, false, s.hidden, d.bv);
-    if (d.bo) columns(ds, s.width, true, s.width, d.bo);
+    if (d.bg) expert_sums(w.sums, 2, 2 * s.hidden, s.hidden, d.bg);
+    if (d.bv) expert_sums(w.sums + s.hidden, 2, 2 * s.hidden, s.hidden, d.bv);
+    if (d.bo) expert_sums(w.out_sums, kTile / kGatherRows, s.width, s.width, d.bo);
     return check_launch("koemi_moe_experts_backward(tiles)");
 }
 
