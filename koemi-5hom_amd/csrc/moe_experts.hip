@@ -400,49 +400,59 @@ using mfma_stage::kOperandBytes;
 using mfma_stage::uniform_ptr;
 constexpr int kTile = 256;
 constexpr int kTileK = mfma_stage::kBK;
-constexpr uint32_t kTileLds = mfma_stage::TileShape<256>::kStages * mfma_stage::TileShape<256>::kStageBytes;
+// Columns of the tiles that write g and v: 128, two workgroups a CU, so that one's epilogue
+// runs under the other's products (256 with one: 5% slower here, 10% faster where g and v
+// are read, whose workgroups need the registers to have loads under way).
+constexpr int kHiddenTile = 128;
+template <int BNT>
+constexpr uint32_t kTileLds = mfma_stage::TileShape<BNT>::kStages * mfma_stage::TileShape<BNT>::kStageBytes;
 
+template <int BNT>
 struct TilePlace {
+    static constexpr int NT = BNT / 64;
     int lane, wave, wm, wn;
     uint32_t a_lds, b_lds;
     __device__ __forceinline__ explicit TilePlace(char* lds) {
         lane = lane_id();
-        wave = threadIdx.x / kWave;
+        wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);  // scalar, and what follows from it
         wm = wave >> 1;
         wn = wave & 1;
         const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
         a_lds = __builtin_amdgcn_readfirstlane(lds0 + wave * 4 * 1024);
-        b_lds = __builtin_amdgcn_readfirstlane(lds0 + kOperandBytes + wave * 4 * 1024);
+        b_lds = __builtin_amdgcn_readfirstlane(lds0 + kOperandBytes + wave * NT * 1024);
     }
     // Offsets of the wave's copies of an operand along K: row(r) is the memory row of the
     // tile's row r, ld elements long.
-    template <typename Row>
-    __device__ __forceinline__ void along(uint32_t (&off)[4], int64_t ld, Row row) const {
+    template <int N, typename Row>
+    __device__ __forceinline__ void along(uint32_t (&off)[N], int64_t ld, Row row) const {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = (wave * 4 + i) * 16 + (lane >> 2), g = (lane & 3) ^ mfma_stage::slot_swizzle(r);
+        for (int i = 0; i < N; ++i) {
+            const int r = (wave * N + i) * 16 + (lane >> 2), g = (lane & 3) ^ mfma_stage::slot_swizzle(r);
             off[i] = (static_cast<uint32_t>(row(r)) * static_cast<uint32_t>(ld) + g * 8) * 2u;
         }
     }
     // Of an operand across K: columns from `first` on (those past `columns`, a multiple of 8, repeat the last).
-    __device__ __forceinline__ void across(uint32_t (&off)[4], int64_t ld, int64_t first, int64_t columns) const {
+    template <int N>
+    __device__ __forceinline__ void across(uint32_t (&off)[N], int64_t ld, int64_t first, int64_t columns) const {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < N; ++i) {
             int k, c;
-            mfma_stage::across_source(wave * 4 + i, lane, k, c);
+            mfma_stage::across_source<N * 64>(wave * N + i, lane, k, c);
             off[i] = (static_cast<uint32_t>(k) * static_cast<uint32_t>(ld) + static_cast<uint32_t>(min(first + c, columns - 8))) * 2u;
         }
     }
-    __device__ __forceinline__ void fragments(uint32_t (&off)[4], bool across, int first) const {
+    template <int N>
+    __device__ __forceinline__ void fragments(uint32_t (&off)[N], bool across, int first) const {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) off[t] = across ? across_fragment(first + t * 32) : along_fragment(first + t * 32);
+        for (int t = 0; t < N; ++t) off[t] = across ? across_fragment<N * 64>(first + t * 32) : along_fragment(first + t * 32);
     }
 };
-__device__ __forceinline__ void clear(f32x16 (&acc)[4][4]) {
+template <int NT>
+__device__ __forceinline__ void clear(f32x16 (&acc)[4][NT]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = f32x16{};
+        for (int j = 0; j < NT; ++j) acc[i][j] = f32x16{};
 }
 
 // A wave's 128 x (32 TILES) outputs as whole bf16 rows. They pass through the wave's own
@@ -453,24 +463,30 @@ __device__ __forceinline__ void put_four(char* region, int r, int c, float v0, f
     constexpr int kRowBytes = TILES * 64, kSwz = kRowBytes / 16 - 1;
     store4(reinterpret_cast<bf16*>(region + r * kRowBytes + ((c >> 3) ^ (r & kSwz)) * 16 + (c & 4) * 2), v0, v1, v2, v3);
 }
-// rows, cols (a multiple of 8): how many exist from out's first element on.
-template <int TILES>
+// rows, cols (a multiple of 8): how many of the region's ROWS and its columns exist from
+// out's first element on.
+template <int TILES, int ROWS = 128>
 __device__ __forceinline__ void flush_wave(const char* region, bf16* out, int64_t ld, int64_t rows, int64_t cols) {
     constexpr int kRowBytes = TILES * 64, kChunks = kRowBytes / 16, kSwz = kChunks - 1;
-    constexpr int kBatch = 8, kIters = 128 * kChunks / kWave;
-    const int lane = lane_id();
+    constexpr int kIters = ROWS * kChunks / kWave, kBatch = kIters < 8 ? kIters : 8;
+    constexpr int kStep = kWave / kChunks;  // rows of one store
+    int lane = lane_id();
+    asm volatile("" : "+v"(lane));  // addresses formed here: shared with other calls they are kept, and spill
+    const int r0 = lane / kChunks, c = lane % kChunks;
+    const uint32_t off = (static_cast<uint32_t>(r0) * static_cast<uint32_t>(ld) + c * 8) * 2u;  // below 64 rows
 #pragma unroll
     for (int b = 0; b < kIters; b += kBatch) {
         uint4 piece[kBatch];
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
-            const int idx = (b + i) * kWave + lane, r = idx / kChunks, c = idx % kChunks;
+            const int r = (b + i) * kStep + r0;
             piece[i] = *reinterpret_cast<const uint4*>(region + r * kRowBytes + ((c ^ (r & kSwz)) * 16));
         }
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
-            const int idx = (b + i) * kWave + lane, r = idx / kChunks, c = idx % kChunks;
-            if (r < rows && c * 8 < cols) *reinterpret_cast<uint4*>(out + r * ld + c * 8) = piece[i];
+            const int r = (b + i) * kStep + r0;
+            char* base = reinterpret_cast<char*>(out + (b + i) * kStep * ld);
+            if (r < rows && c * 8 < cols) *reinterpret_cast<uint4*>(base + off) = piece[i];
         }
     }
 }
@@ -493,59 +509,74 @@ __device__ __forceinline__ void store_wave(char* region, bf16* out, int64_t ld, 
 // A wave's 128 x 128 outputs in fp32, each lane four consecutive columns at a time.
 template <typename Value>
 __device__ __forceinline__ void store_wave_f32(float* out, int64_t ld, int64_t rows, int64_t cols, Value value) {
-    const int lane = lane_id();
+    const int lane = lane_id(), r0 = lane & 31, c0 = (lane >> 5) * 4;
+    const uint32_t off = (static_cast<uint32_t>(r0) * static_cast<uint32_t>(ld) + c0) * 4u;
 #pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {
-        const int r = mt * 32 + (lane & 31);
+    for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int c = t * 32 + (lane >> 5) * 4 + j * 8;
-                if (r < rows && c < cols)
-                    store4(out + r * ld + c, value(mt, t, j * 4), value(mt, t, j * 4 + 1), value(mt, t, j * 4 + 2),
-                           value(mt, t, j * 4 + 3));
+                char* base = reinterpret_cast<char*>(out + mt * 32 * ld + t * 32 + j * 8);
+                if (mt * 32 + r0 < rows && t * 32 + j * 8 + c0 < cols)
+                    store4(reinterpret_cast<float*>(base + off), value(mt, t, j * 4), value(mt, t, j * 4 + 1),
+                           value(mt, t, j * 4 + 2), value(mt, t, j * 4 + 3));
             }
         }
-    }
 }
 
 // g and v are kept in the order of the accumulators: float4 (slot, 32-column block, 32-row
-// block, j, lane) holds elements 4 j .. 4 j + 3, so that a wave reads and writes 1 KiB at once.
-__device__ __forceinline__ int64_t kept_at(int64_t slot, int64_t blocks, int64_t c32, int m32, int j, int lane) {
-    return ((((slot * blocks + c32) * 8 + m32) * 4 + j) * kWave + lane) * 4;
+// block, j, lane) holds elements 4 j .. 4 j + 3, so that a wave reads and writes 1 KiB at
+// once. The first float of (slot, column block, row block): j and the lane add to it.
+__device__ __forceinline__ int64_t kept_at(int64_t slot, int64_t blocks, int64_t c32, int m32) {
+    return ((slot * blocks + c32) * 8 + m32) * (4 * kWave * 4);
+}
+__device__ __forceinline__ uint32_t kept_lane(int j) { return static_cast<uint32_t>((j * kWave + lane_id()) * 4); }
+// Past the caches: they are read a whole backward pass later, and once (16384 tokens, 1024
+// -> 2048: written 389 us, 365 so; read 331, 306 so).
+__device__ __forceinline__ float4 kept4(const float* p) {
+    typedef float f32x4 __attribute__((ext_vector_type(4)));
+    const f32x4 v = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(p));
+    return make_float4(v.x, v.y, v.z, v.w);
+}
+__device__ __forceinline__ void keep4(float* p, float a, float b, float c, float d) {
+    store16_nt(p, make_uint4(__float_as_uint(a), __float_as_uint(b), __float_as_uint(c), __float_as_uint(d)));
 }
 
-// g, v and h of a slot's pairs x 128 hidden units: B rows 0 .. 127 are W_g's, 128 .. 255 W_v's.
-__global__ __launch_bounds__(mfma_stage::kThreads, 1) void tile_hidden_kernel(
+// g, v and h of a slot's pairs x BNT / 2 hidden units: the first half of the B rows are
+// W_g's, the other W_v's.
+template <int BNT>
+__global__ __launch_bounds__(mfma_stage::kThreads, mfma_stage::TileShape<BNT>::kWgPerCu) void tile_hidden_kernel(
     const bf16* __restrict__ x, const int64_t* __restrict__ rows, int64_t tokens, const bf16* __restrict__ Wg,
     const bf16* __restrict__ bg, const bf16* __restrict__ Wv, const bf16* __restrict__ bv, float* __restrict__ keep_g,
     float* __restrict__ keep_v, bf16* __restrict__ h, Slots slots, int64_t max_slots, int64_t width, int64_t hidden,
     uint32_t n_tiles) {
-    __shared__ __attribute__((aligned(1024))) char lds[kTileLds];
+    constexpr int NT = BNT / 64;
+    __shared__ __attribute__((aligned(1024))) char lds[kTileLds<BNT>];
     uint32_t slot, tile_n;
     if (!slot_tile(slots, max_slots, n_tiles, slot, tile_n)) return;
     const int e = slots.expert[slot];
-    const int64_t row0 = slots.row[slot], end = slots.end[slot], n0 = static_cast<int64_t>(tile_n) * 128;
-    const TilePlace at(lds);
+    const int64_t row0 = slots.row[slot], end = slots.end[slot], n0 = static_cast<int64_t>(tile_n) * (BNT / 2);
+    const TilePlace<BNT> at(lds);
     const bf16* a = static_cast<const bf16*>(uniform_ptr(x));
     const bf16* b = static_cast<const bf16*>(uniform_ptr((at.wave >= 2 ? Wv : Wg) + static_cast<int64_t>(e) * hidden * width));
-    uint32_t a_off[4], b_off[4], a_frag[4], b_frag[4];
+    uint32_t a_off[4], b_off[NT], a_frag[4], b_frag[NT];
     at.along(a_off, width, [&](int r) { return min(max(rows[min(row0 + r, end - 1)], int64_t(0)), tokens - 1); });
-    at.along(b_off, width, [&](int r) { return min(n0 + (r & 127), hidden - 1); });
+    at.along(b_off, width, [&](int r) { return min(n0 + (r & (BNT / 2 - 1)), hidden - 1); });
     at.fragments(a_frag, false, at.wm * 128);
 #pragma unroll
-    for (int t = 0; t < 4; ++t) b_frag[t] = along_fragment((t < 2 ? 0 : 128) + at.wn * 64 + (t & 1) * 32);
-    f32x16 acc[4][4];
+    for (int t = 0; t < NT; ++t)
+        b_frag[t] = along_fragment((t < NT / 2 ? 0 : BNT / 2) + at.wn * (BNT / 4) + t % (NT / 2) * 32);
+    f32x16 acc[4][NT];
     clear(acc);
-    mfma_stage::across_loop<false, false>(
+    mfma_stage::across_loop<BNT, false, false>(
         lds, [&](int kt) { return a + kt * kTileK; }, [&](int kt) { return b + kt * kTileK; }, a_off, b_off, at.a_lds,
         at.b_lds, a_frag, b_frag, static_cast<int>(width / kTileK), acc);
     __syncthreads();  // every wave is done reading the stages
-    const int64_t first = n0 + at.wn * 64, blocks = hidden / 32;
+    const int64_t first = n0 + at.wn * (BNT / 4), blocks = hidden / 32;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < NT / 2; ++t) {
         if (first + t * 32 >= hidden) break;
         float b0[16], b1[16];
 #pragma unroll
@@ -560,32 +591,32 @@ __global__ __launch_bounds__(mfma_stage::kThreads, 1) void tile_hidden_kernel(
 #pragma unroll
             for (int v = 0; v < 16; ++v) {
                 acc[mt][t][v] += b0[v];
-                acc[mt][t + 2][v] += b1[v];
+                acc[mt][t + NT / 2][v] += b1[v];
             }
             if (keep_g)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int64_t o = kept_at(slot, blocks, first / 32 + t, at.wm * 4 + mt, j, at.lane);
-                    store4(keep_g + o, acc[mt][t][j * 4], acc[mt][t][j * 4 + 1], acc[mt][t][j * 4 + 2], acc[mt][t][j * 4 + 3]);
-                    store4(keep_v + o, acc[mt][t + 2][j * 4], acc[mt][t + 2][j * 4 + 1], acc[mt][t + 2][j * 4 + 2],
-                           acc[mt][t + 2][j * 4 + 3]);
+                    const int64_t o = kept_at(slot, blocks, first / 32 + t, at.wm * 4 + mt);
+                    keep4(keep_g + o + kept_lane(j), acc[mt][t][j * 4], acc[mt][t][j * 4 + 1], acc[mt][t][j * 4 + 2], acc[mt][t][j * 4 + 3]);
+                    keep4(keep_v + o + kept_lane(j), acc[mt][t + NT / 2][j * 4], acc[mt][t + NT / 2][j * 4 + 1], acc[mt][t + NT / 2][j * 4 + 2],
+                          acc[mt][t + NT / 2][j * 4 + 3]);
                 }
         }
     }
-    store_wave<2>(lds + at.wave * (128 * 128), h + (row0 + at.wm * 128) * hidden + first, hidden, end - row0 - at.wm * 128,
-                  hidden - first, [&](int mt, int t, int v) { return glu(acc[mt][t][v], acc[mt][t + 2][v]); });
+    store_wave<NT / 2>(lds + at.wave * (128 * 32 * NT), h + (row0 + at.wm * 128) * hidden + first, hidden, end - row0 - at.wm * 128,
+                  hidden - first, [&](int mt, int t, int v) { return glu(acc[mt][t][v], acc[mt][t + NT / 2][v]); });
 }
 
 // y = W_o h + b_o of a slot's pairs x 256 columns.
 __global__ __launch_bounds__(mfma_stage::kThreads, 1) void tile_output_kernel(
     const bf16* __restrict__ h, const bf16* __restrict__ Wo, const bf16* __restrict__ bo, float* __restrict__ y, Slots slots,
     int64_t max_slots, int64_t width, int64_t hidden, uint32_t n_tiles) {
-    __shared__ __attribute__((aligned(1024))) char lds[kTileLds];
+    __shared__ __attribute__((aligned(1024))) char lds[kTileLds<256>];
     uint32_t slot, tile_n;
     if (!slot_tile(slots, max_slots, n_tiles, slot, tile_n)) return;
     const int e = slots.expert[slot];
     const int64_t row0 = slots.row[slot], end = slots.end[slot], n0 = static_cast<int64_t>(tile_n) * kTile;
-    const TilePlace at(lds);
+    const TilePlace<256> at(lds);
     const bf16* a = static_cast<const bf16*>(uniform_ptr(h + row0 * hidden));
     const bf16* b = static_cast<const bf16*>(uniform_ptr(Wo + static_cast<int64_t>(e) * width * hidden));
     uint32_t a_off[4], b_off[4], a_frag[4], b_frag[4];
@@ -595,7 +626,7 @@ __global__ __launch_bounds__(mfma_stage::kThreads, 1) void tile_output_kernel(
     at.fragments(b_frag, false, at.wn * 128);
     f32x16 acc[4][4];
     clear(acc);
-    mfma_stage::across_loop<false, false>(
+    mfma_stage::across_loop<256, false, false>(
         lds, [&](int kt) { return a + kt * kTileK; }, [&](int kt) { return b + kt * kTileK; }, a_off, b_off, at.a_lds,
         at.b_lds, a_frag, b_frag, static_cast<int>(hidden / kTileK), acc);
     const int64_t first = n0 + at.wn * 128, r0 = row0 + at.wm * 128;
@@ -633,31 +664,41 @@ __global__ __launch_bounds__(256) void tile_gather_kernel(const bf16* __restrict
     };
     float bias[8] = {}, sum[8] = {};
     if (dot_part && in) spread(*reinterpret_cast<const uint4*>(bo + e * width + c), bias);
-#pragma unroll 4
-    for (int i = wave; i < kGatherRows; i += 4) {
-        const int64_t p = p0 + i, padded = quarter * kGatherRows + i;
-        const bool real = p < end;
-        const int64_t t = real ? min(max(rows[p], int64_t(0)), tokens - 1) : 0;
-        uint4 a = make_uint4(0, 0, 0, 0), d = a;
-        if (real && in) {
-            if (xs) a = *reinterpret_cast<const uint4*>(x + t * width + c);
-            d = *reinterpret_cast<const uint4*>(d_out + t * width + c);
-        }
-        if (in) {
-            if (xs) *reinterpret_cast<uint4*>(xs + padded * width + c) = a;
-            *reinterpret_cast<uint4*>(ds + padded * width + c) = d;
-        }
-        float f[8], dot = 0.0f;
-        spread(d, f);
-        const float w = !real ? 0.0f : sorted_w ? sorted_w[p] : share;
+    constexpr int kTurn = 4;  // rows of a wave whose loads are under way at once
+    for (int i0 = wave; i0 < kGatherRows; i0 += 4 * kTurn) {
+        uint4 a[kTurn], d[kTurn];
+        float w[kTurn];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-            dot = fmaf(f[q], bias[q], dot);
-            sum[q] = real ? fmaf(w, f[q], sum[q]) : sum[q];
+        for (int u = 0; u < kTurn; ++u) {
+            const int64_t p = p0 + i0 + 4 * u;
+            const bool real = p < end;
+            const int64_t t = real ? min(max(rows[p], int64_t(0)), tokens - 1) : 0;
+            a[u] = d[u] = make_uint4(0, 0, 0, 0);
+            if (real && in) {
+                if (xs) a[u] = *reinterpret_cast<const uint4*>(x + t * width + c);
+                d[u] = *reinterpret_cast<const uint4*>(d_out + t * width + c);
+            }
+            w[u] = !real ? 0.0f : sorted_w ? sorted_w[p] : share;
         }
-        if (dot_part) {
-            dot = wave_sum_xor(dot);
-            if (lane == 0 && real) dot_part[blockIdx.y * pairs + p] = dot;
+#pragma unroll
+        for (int u = 0; u < kTurn; ++u) {
+            const int64_t p = p0 + i0 + 4 * u, padded = quarter * kGatherRows + i0 + 4 * u;
+            const bool real = p < end;
+            if (in) {
+                if (xs) *reinterpret_cast<uint4*>(xs + padded * width + c) = a[u];
+                *reinterpret_cast<uint4*>(ds + padded * width + c) = d[u];
+            }
+            float f[8], dot = 0.0f;
+            spread(d[u], f);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                dot = fmaf(f[q], bias[q], dot);
+                sum[q] = real ? fmaf(w[u], f[q], sum[q]) : sum[q];
+            }
+            if (dot_part) {
+                dot = wave_sum_xor(dot);
+                if (lane == 0 && real) dot_part[blockIdx.y * pairs + p] = dot;
+            }
         }
     }
     if (!sums) return;
@@ -672,18 +713,19 @@ __global__ __launch_bounds__(256) void tile_gather_kernel(const bf16* __restrict
     store4(sums + quarter * width + c + 4, sum[4], sum[5], sum[6], sum[7]);
 }
 
-// Column sums of a wave's region of 128 rows x 32 columns (put_four<1>), as products
-// with ones on the matrix cores: the region's rows are K, read transposed.
-__device__ __forceinline__ void region_sums(const char* region, float* out) {
+// Adds the column sums of a wave's region of ROWS rows x 32 columns (put_four<1>), as
+// products with ones on the matrix cores: the region's rows are K, read transposed. Every
+// column of the result is the sums.
+template <int ROWS>
+__device__ __forceinline__ void region_sums(const char* region, f32x16& acc) {
     typedef short s16x4 __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
     const int lane = lane_id(), chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
     mfma_stage::bf16x8 ones;
 #pragma unroll
     for (int i = 0; i < 8; ++i) ones[i] = static_cast<bf16>(1.0f);
-    f32x16 acc = {};
 #pragma unroll
-    for (int k0 = 0; k0 < 128; k0 += 16) {
+    for (int k0 = 0; k0 < ROWS; k0 += 16) {
         union {
             s16x4 half[2];
             mfma_stage::bf16x8 whole;
@@ -695,7 +737,10 @@ __device__ __forceinline__ void region_sums(const char* region, float* out) {
         }
         acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u.whole, ones, acc, 0, 0, 0);
     }
-    if ((lane & 31) == 0)  // every column of the product is the sums
+}
+__device__ __forceinline__ void store_sums(const f32x16& acc, float* out) {
+    const int lane = lane_id();
+    if ((lane & 31) == 0)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             store4(out + (lane >> 5) * 4 + j * 8, acc[j * 4], acc[j * 4 + 1], acc[j * 4 + 2], acc[j * 4 + 3]);
@@ -709,31 +754,47 @@ __global__ __launch_bounds__(mfma_stage::kThreads, 1) void tile_hidden_gradient_
     const float* __restrict__ sorted_w, float share, bf16* __restrict__ dgv, bf16* __restrict__ wh,
     float* __restrict__ dw_part, float* __restrict__ sums, Slots slots, int64_t max_slots, int64_t pairs, int64_t width,
     int64_t hidden, uint32_t n_tiles) {
-    __shared__ __attribute__((aligned(1024))) char lds[kTileLds];
+    constexpr int NT = kTile / 64, kRows = 64;
+    __shared__ __attribute__((aligned(1024))) char lds[kTileLds<kTile>];
     uint32_t slot, tile_n;
     if (!slot_tile(slots, max_slots, n_tiles, slot, tile_n)) return;
     const int e = slots.expert[slot];
     const int64_t row0 = slots.row[slot], end = slots.end[slot], n0 = static_cast<int64_t>(tile_n) * kTile;
     const int64_t padded = static_cast<int64_t>(slot) * kTile;
-    const TilePlace at(lds);
+    const TilePlace<kTile> at(lds);
     const bf16* a = static_cast<const bf16*>(uniform_ptr(ds + padded * width));
     const bf16* b = static_cast<const bf16*>(uniform_ptr(Wo + static_cast<int64_t>(e) * width * hidden));
-    uint32_t a_off[4], b_off[4], a_frag[4], b_frag[4];
+    uint32_t a_off[4], b_off[NT], a_frag[4], b_frag[NT];
     at.along(a_off, width, [&](int r) { return r; });
     at.across(b_off, hidden, n0, hidden);
     at.fragments(a_frag, false, at.wm * 128);
-    at.fragments(b_frag, true, at.wn * 128);
-    f32x16 acc[4][4];
+    at.fragments(b_frag, true, at.wn * (kTile / 2));
+    f32x16 acc[4][NT];
     clear(acc);
-    mfma_stage::across_loop<false, true>(
+    mfma_stage::across_loop<kTile, false, true>(
         lds, [&](int kt) { return a + kt * kTileK; }, [&](int kt) { return b + kt * kTileK * hidden; }, a_off, b_off, at.a_lds,
         at.b_lds, a_frag, b_frag, static_cast<int>(width / kTileK), acc);
+    const int64_t first = n0 + at.wn * (kTile / 2), blocks = hidden / 32;
+    // block 4 t + mt of kept g and v, loaded while the block before is worked on
+    struct Kept {
+        float4 g[4], v[4];
+    } kept[2];
+    auto fetch = [&](int block, Kept& k) {
+        const int64_t o = kept_at(slot, blocks, min(first / 32 + block / 4, blocks - 1), at.wm * 4 + block % 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            k.g[j] = kept4(keep_g + o + kept_lane(j));
+            k.v[j] = kept4(keep_v + o + kept_lane(j));
+        }
+    };
+    fetch(0, kept[0]);
     __syncthreads();  // every wave is done reading the stages
-    const int64_t first = n0 + at.wn * 128, blocks = hidden / 32;
-    char* region = lds + at.wave * (3 * 128 * 64);
-    float* part = dw_part + (2 * static_cast<int64_t>(tile_n) + at.wn) * pairs;
-    // 32 columns at a time: dg, dv and w h in three regions of 128 x 32, so that no product is kept beside its sums
+    // 64 rows x 32 columns at a time: dg, dv and w h in three regions, so that no product is kept beside its sums
+    constexpr int kRegion = kRows * 64;
+    static_assert(4 * 3 * kRegion <= kTileLds<kTile>, "the output regions fit the stages");
+    char* region = lds + at.wave * (3 * kRegion);
     const int64_t r0 = padded + at.wm * 128;
+    float* part = dw_part + (2 * static_cast<int64_t>(tile_n) + at.wn) * pairs;
     float weight[4], sum[4] = {};
     bool real[4];
 #pragma unroll
@@ -742,27 +803,15 @@ __global__ __launch_bounds__(mfma_stage::kThreads, 1) void tile_hidden_gradient_
         real[mt] = p < end;
         weight[mt] = !real[mt] ? 0.0f : sorted_w ? sorted_w[p] : share;
     }
-    // block 4 t + mt of kept g and v, loaded while the block before is worked on
-    struct Kept {
-        float4 g[4], v[4];
-    } kept[2];
-    auto fetch = [&](int block, Kept& k) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int64_t o = kept_at(slot, blocks, min(first / 32 + block / 4, blocks - 1), at.wm * 4 + block % 4, j, at.lane);
-            k.g[j] = load4(keep_g + o);
-            k.v[j] = load4(keep_v + o);
-        }
-    };
-    fetch(0, kept[0]);
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
+    for (int t = 0; t < NT; ++t) {
         if (first + t * 32 >= hidden) break;  // the same for the wave
+        f32x16 g_sums = {}, v_sums = {};
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt) {
             __builtin_amdgcn_sched_barrier(0);
             const Kept& k = kept[mt % 2];
-            if (t * 4 + mt < 15) fetch(t * 4 + mt + 1, kept[(mt + 1) % 2]);
+            if (t * 4 + mt < 4 * NT - 1) fetch(t * 4 + mt + 1, kept[(mt + 1) % 2]);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -776,21 +825,27 @@ __global__ __launch_bounds__(mfma_stage::kThreads, 1) void tile_hidden_gradient_
                     dv[q] = real[mt] ? o4.dv : 0.0f;
                     h[q] = real[mt] ? o4.wh : 0.0f;
                 }
-                const int r = mt * 32 + (at.lane & 31), c = (at.lane >> 5) * 4 + j * 8;
+                const int r = mt * 32 % kRows + (at.lane & 31), c = (at.lane >> 5) * 4 + j * 8;
                 put_four<1>(region, r, c, dg[0], dg[1], dg[2], dg[3]);
-                put_four<1>(region + 128 * 64, r, c, dv[0], dv[1], dv[2], dv[3]);
-                put_four<1>(region + 2 * 128 * 64, r, c, h[0], h[1], h[2], h[3]);
+                put_four<1>(region + kRegion, r, c, dv[0], dv[1], dv[2], dv[3]);
+                put_four<1>(region + 2 * kRegion, r, c, h[0], h[1], h[2], h[3]);
             }
+            if ((mt + 1) * 32 % kRows != 0) continue;
+            if (sums) {
+                region_sums<kRows>(region, g_sums);
+                region_sums<kRows>(region + kRegion, v_sums);
+            }
+            const int64_t row = r0 + mt * 32 / kRows * kRows;
+            bf16* out = dgv + row * 2 * hidden + first + t * 32;
+            flush_wave<1, kRows>(region, out, 2 * hidden, kRows, 32);
+            flush_wave<1, kRows>(region + kRegion, out + hidden, 2 * hidden, kRows, 32);
+            flush_wave<1, kRows>(region + 2 * kRegion, wh + row * hidden + first + t * 32, hidden, kRows, 32);
         }
         if (sums) {
             float* to = sums + (2 * static_cast<int64_t>(slot) + at.wm) * 2 * hidden + first + t * 32;
-            region_sums(region, to);
-            region_sums(region + 128 * 64, to + hidden);
+            store_sums(g_sums, to);
+            store_sums(v_sums, to + hidden);
         }
-        bf16* out = dgv + r0 * 2 * hidden + first + t * 32;
-        flush_wave<1>(region, out, 2 * hidden, 128, 32);
-        flush_wave<1>(region + 128 * 64, out + hidden, 2 * hidden, 128, 32);
-        flush_wave<1>(region + 2 * 128 * 64, wh + r0 * hidden + first + t * 32, hidden, 128, 32);
     }
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) {
@@ -803,12 +858,12 @@ __global__ __launch_bounds__(mfma_stage::kThreads, 1) void tile_hidden_gradient_
 __global__ __launch_bounds__(mfma_stage::kThreads, 1) void tile_input_gradient_kernel(
     const bf16* __restrict__ dgv, const bf16* __restrict__ Wg, const bf16* __restrict__ Wv, float* __restrict__ dx, Slots slots,
     int64_t max_slots, int64_t width, int64_t hidden, uint32_t n_tiles) {
-    __shared__ __attribute__((aligned(1024))) char lds[kTileLds];
+    __shared__ __attribute__((aligned(1024))) char lds[kTileLds<256>];
     uint32_t slot, tile_n;
     if (!slot_tile(slots, max_slots, n_tiles, slot, tile_n)) return;
     const int e = slots.expert[slot];
     const int64_t row0 = slots.row[slot], end = slots.end[slot], n0 = static_cast<int64_t>(tile_n) * kTile;
-    const TilePlace at(lds);
+    const TilePlace<256> at(lds);
     const bf16* a = static_cast<const bf16*>(uniform_ptr(dgv + static_cast<int64_t>(slot) * kTile * 2 * hidden));
     const bf16* b0 = static_cast<const bf16*>(uniform_ptr(Wg + static_cast<int64_t>(e) * hidden * width));
     const bf16* b1 = static_cast<const bf16*>(uniform_ptr(Wv + static_cast<int64_t>(e) * hidden * width));
@@ -820,7 +875,7 @@ __global__ __launch_bounds__(mfma_stage::kThreads, 1) void tile_input_gradient_k
     f32x16 acc[4][4];
     clear(acc);
     const int steps = static_cast<int>(hidden / kTileK);
-    mfma_stage::across_loop<false, true>(
+    mfma_stage::across_loop<256, false, true>(
         lds, [&](int kt) { return a + kt * kTileK; },
         [&](int kt) { return kt < steps ? b0 + kt * kTileK * width : b1 + (kt - steps) * kTileK * width; }, a_off, b_off,
         at.a_lds, at.b_lds, a_frag, b_frag, 2 * steps, acc);
@@ -835,7 +890,7 @@ __global__ __launch_bounds__(mfma_stage::kThreads, 1) void tile_weight_gradient_
     const bf16* __restrict__ dgv, const bf16* __restrict__ wh, const bf16* __restrict__ xs, const bf16* __restrict__ ds,
     const int64_t* __restrict__ offsets, Slots slots, bf16* __restrict__ dWg, bf16* __restrict__ dWv, bf16* __restrict__ dWo,
     int64_t pairs, int64_t width, int64_t hidden, uint32_t w_tiles, uint32_t h_tiles, uint32_t tiles) {
-    __shared__ __attribute__((aligned(1024))) char lds[kTileLds];
+    __shared__ __attribute__((aligned(1024))) char lds[kTileLds<256>];
     const uint32_t per = (tiles + 7) / 8, i = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
     if ((blockIdx.x >> 3) >= per || i >= tiles) return;
     const uint32_t one = w_tiles * h_tiles, e = i / (3 * one), which = i % (3 * one) / one, within = i % one;
@@ -848,7 +903,7 @@ __global__ __launch_bounds__(mfma_stage::kThreads, 1) void tile_weight_gradient_
     const int64_t lo = min(max(offsets[e], int64_t(0)), pairs), count = min(max(offsets[e + 1], lo), pairs) - lo;
     const int64_t row = static_cast<int64_t>(slots.first[e]) * kTile;
     const int64_t lda = out ? width : 2 * hidden, ldb = out ? hidden : width;
-    const TilePlace at(lds);
+    const TilePlace<256> at(lds);
     const bf16* a = static_cast<const bf16*>(uniform_ptr((out ? ds : dgv + (which == 1 ? hidden : 0)) + row * lda));
     const bf16* b = static_cast<const bf16*>(uniform_ptr((out ? wh : xs) + row * ldb));
     uint32_t a_off[4], b_off[4], a_frag[4], b_frag[4];
@@ -860,7 +915,7 @@ __global__ __launch_bounds__(mfma_stage::kThreads, 1) void tile_weight_gradient_
     clear(acc);
     const int nk = static_cast<int>((count + kTileK - 1) / kTileK);
     if (nk > 0)  // the same for the workgroup
-        mfma_stage::across_loop<true, true>(
+        mfma_stage::across_loop<256, true, true>(
             lds, [&](int kt) { return a + kt * kTileK * lda; }, [&](int kt) { return b + kt * kTileK * ldb; }, a_off, b_off,
             at.a_lds, at.b_lds, a_frag, b_frag, nk, acc);
     __syncthreads();  // every wave is done reading the stages
@@ -1206,10 +1261,11 @@ int any_backward(const Shape& s, const void* d_out, const void* x, const int64_t
 int tile_forward(const Shape& s, const void* x, const int64_t* rows, const int64_t* offsets, const int64_t* positions,
                  const float* pair_weights, const Weights& m, void* out, float* keep, const ForwardSpace& w, hipStream_t q) {
     const int64_t slots = most_slots(s);
-    const uint32_t h_tiles = static_cast<uint32_t>(ceil_div(s.hidden, 128)), w_tiles = static_cast<uint32_t>(ceil_div(s.width, kTile));
+    const uint32_t h_tiles = static_cast<uint32_t>(ceil_div(s.hidden, kHiddenTile / 2)),
+                   w_tiles = static_cast<uint32_t>(ceil_div(s.width, kTile));
     bf16* h = reinterpret_cast<bf16*>(w.h);
     find_slots(s, offsets, w.slots, q);
-    hipLaunchKernelGGL(tile_hidden_kernel, dim3(tiles_grid(slots, h_tiles)), dim3(mfma_stage::kThreads), 0, q,
+    hipLaunchKernelGGL(tile_hidden_kernel<kHiddenTile>, dim3(tiles_grid(slots, h_tiles)), dim3(mfma_stage::kThreads), 0, q,
                        static_cast<const bf16*>(x), rows, s.tokens, static_cast<const bf16*>(m.Wg),
                        static_cast<const bf16*>(m.bg), static_cast<const bf16*>(m.Wv), static_cast<const bf16*>(m.bv), keep,
                        keep ? keep + kept_floats(s) : nullptr, h, w.slots, slots, s.width, s.hidden, h_tiles);
@@ -1235,7 +1291,7 @@ int tile_backward(const Shape& s, const void* d_out, const void* x, const int64_
                        static_cast<const bf16*>(x), static_cast<const bf16*>(d_out), rows, static_cast<const bf16*>(m.bo),
                        sorted_w, share, d.Wg || d.Wv ? xs : nullptr, ds, d.weights ? w.dot : nullptr,
                        d.bo ? w.out_sums : nullptr, w.slots, slots, s.pairs, s.tokens, s.width);
-    hipLaunchKernelGGL(tile_hidden_gradient_kernel, dim3(tiles_grid(slots, h_tiles)), threads, 0, q, ds,
+        hipLaunchKernelGGL(tile_hidden_gradient_kernel, dim3(tiles_grid(slots, h_tiles)), threads, 0, q, ds,
                        static_cast<const bf16*>(m.Wo), keep, keep + kept_floats(s), sorted_w, share, dgv, wh, w.dw_part,
                        d.bg || d.bv ? w.sums : nullptr, w.slots, slots, s.pairs, s.width, s.hidden, h_tiles);
     if (d.x) {
