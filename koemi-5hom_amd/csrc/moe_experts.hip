@@ -19,7 +19,8 @@
 // values are, and forming them again would cost two of the products.
 //
 // Any type, width and alignment runs on the tiles of split_gemm.hpp, which read an
-// operand either along K or across it; what lies between two products stays fp32 there.
+// operand either along K or across it; what lies between two products stays fp32 there
+// (two bf16 planes of it are multiplied where the result is 16-bit).
 #include "common.hpp"
 #include "mfma_across.hpp"
 #include "split_gemm.hpp"
@@ -121,9 +122,21 @@ __device__ __forceinline__ bool slot_tile(const Slots& s, int64_t max_slots, uin
 }
 
 // --------------------------------------------------- any type and any shape ---
-constexpr int kAnyCols = 128;
 // Rows of a tile: 64 where the experts' segments are mostly shorter than a tile of 128.
 inline int any_rows(int64_t pairs, int64_t experts) { return pairs <= 96 * experts ? 64 : 128; }
+// Such calls have few tiles too: those of 64 rows are 64 columns wide and have four K steps
+// under way (64 tokens bf16, 2048 -> 1024: 53 us with 128 columns and one step).
+__host__ __device__ constexpr int any_cols(int rows) { return rows == 64 ? 64 : 128; }
+__host__ __device__ constexpr int any_depth(int rows) { return rows == 64 ? 4 : 1; }
+
+// What lies between two products, as their operand beside T: fp32 in memory.
+template <typename T>
+using Between = std::conditional_t<std::is_same<T, float>::value, float, split_gemm::coarse_f32>;
+// The LDS of a tile and, after its products, of four waves' output regions.
+template <typename G>
+constexpr int any_lds(int region) {
+    return G::kLdsBytes > 4 * region ? G::kLdsBytes : 4 * region;
+}
 
 // g, v (fp32, kept where wanted) and h (fp32) of a slot's pairs x 64 hidden units; rows
 // are ld apart, zeros from `hidden` on. B rows 0-63 of the tile are W_g's, 64-127 W_v's.
@@ -133,8 +146,9 @@ __global__ __launch_bounds__(split_gemm::kThreads, 2) void any_hidden_kernel(
     const T* __restrict__ bg, const T* __restrict__ Wv, const T* __restrict__ bv, float* __restrict__ keep_g,
     float* __restrict__ keep_v, float* __restrict__ h, Slots slots, int64_t max_slots, int64_t width, int64_t hidden,
     int64_t ld, uint32_t n_tiles) {
-    using G = split_gemm::Tile<T, T, BM, kAnyCols>;
-    __shared__ __attribute__((aligned(16))) char lds[G::kLdsBytes];
+    using G = split_gemm::Tile<T, T, BM, 128, false, false, BM == 64 ? 2 : 1>;
+    constexpr int kRegion = split_gemm::store_bytes<float, 1>();
+    __shared__ __attribute__((aligned(16))) char lds[any_lds<G>(kRegion)];
     uint32_t slot, tile_n;
     if (!slot_tile(slots, max_slots, n_tiles, slot, tile_n)) return;
     const int e = slots.expert[slot];
@@ -149,8 +163,6 @@ __global__ __launch_bounds__(split_gemm::kThreads, 2) void any_hidden_kernel(
         [&](int r) { return (r < 64 ? w0 : w1) + min(n0 + (r & 63), hidden - 1) * width; },
         [&](int t) { return t * 64 + wn * 32; });
     if constexpr (G::kNative) split_gemm::lds_barrier();
-    constexpr int kRegion = split_gemm::store_bytes<float, 1>();
-    static_assert(4 * kRegion <= G::kLdsBytes, "the output regions fit the operands' LDS");
     const int64_t first = n0 + wn * 32;
     float b0[16], b1[16];
 #pragma unroll
@@ -192,25 +204,26 @@ __global__ __launch_bounds__(split_gemm::kThreads, 2) void any_hidden_kernel(
     }
 }
 
-// y = W_o h + b_o of a slot's pairs x 128 columns, fp32.
+// y = W_o h + b_o of a slot's pairs x a tile's columns, fp32.
 template <typename T, int BM, int BYTES>
 __global__ __launch_bounds__(split_gemm::kThreads, 2) void any_output_kernel(
-    const float* __restrict__ h, const T* __restrict__ Wo, const T* __restrict__ bo, float* __restrict__ y, Slots slots,
+    const Between<T>* __restrict__ h, const T* __restrict__ Wo, const T* __restrict__ bo, float* __restrict__ y, Slots slots,
     int64_t max_slots, int64_t width, int64_t hidden, int64_t ld, uint32_t n_tiles) {
-    using G = split_gemm::Tile<float, T, BM, kAnyCols>;
-    __shared__ __attribute__((aligned(16))) char lds[G::kLdsBytes];
+    constexpr int BN = any_cols(BM);
+    using G = split_gemm::Tile<Between<T>, T, BM, BN, false, false, any_depth(BM)>;
+    constexpr int kRegion = split_gemm::store_bytes<float, 1>();
+    __shared__ __attribute__((aligned(16))) char lds[any_lds<G>(kRegion)];
     uint32_t slot, tile_n;
     if (!slot_tile(slots, max_slots, n_tiles, slot, tile_n)) return;
     const int e = slots.expert[slot];
-    const int64_t row0 = slots.row[slot], end = slots.end[slot], n0 = static_cast<int64_t>(tile_n) * kAnyCols;
+    const int64_t row0 = slots.row[slot], end = slots.end[slot], n0 = static_cast<int64_t>(tile_n) * BN;
     const int wave = threadIdx.x / kWave, wm = wave >> 1, wn = wave & 1;
     const T* w = Wo + e * width * hidden;
     G tile;
     const uint64_t chains = tile.template run<16, BYTES>(
         lds, ld, hidden, 0, ceil_div(hidden, G::BK) * G::BK, [&](int r) { return h + min(row0 + r, end - 1) * ld; },
-        [&](int r) { return w + min(n0 + r, width - 1) * hidden; }, [&](int t) { return wn * 64 + t * 32; });
-    constexpr int kRegion = split_gemm::store_bytes<float, 1>();
-    const int64_t first = n0 + wn * 64;
+        [&](int r) { return w + min(n0 + r, width - 1) * hidden; }, [&](int t) { return wn * (BN / 2) + t * 32; });
+    const int64_t first = n0 + wn * (BN / 2);
 #pragma unroll
     for (int j = 0; j < G::NT; ++j)
 #pragma unroll
@@ -230,33 +243,33 @@ __global__ __launch_bounds__(split_gemm::kThreads, 2) void any_output_kernel(
     });
 }
 
-// d' = W_o^T dout of a slot's pairs x 128 hidden units and what follows from it: dg, dv
+// d' = W_o^T dout of a slot's pairs x a tile's hidden units and what follows from it: dg, dv
 // and w h (fp32, rows ld apart, zeros from `hidden` on), and each row's part of dw from
-// a wave's 64 units: dw_part[(2 tile + wave column) pairs + row].
+// a wave's half of them: dw_part[(2 tile + wave column) pairs + row].
 template <typename T, int BM, int BYTES>
 __global__ __launch_bounds__(split_gemm::kThreads, 2) void any_hidden_gradient_kernel(
     const T* __restrict__ d_out, const int64_t* __restrict__ rows, int64_t tokens, const T* __restrict__ Wo,
     const float* __restrict__ keep_g, const float* __restrict__ keep_v, const float* __restrict__ sorted_w, float share,
     float* __restrict__ dg, float* __restrict__ dv, float* __restrict__ wh, float* __restrict__ dw_part, Slots slots,
     int64_t max_slots, int64_t pairs, int64_t width, int64_t hidden, int64_t ld, uint32_t n_tiles) {
-    using G = split_gemm::Tile<T, T, BM, kAnyCols, false, true>;
-    __shared__ __attribute__((aligned(16))) char lds[G::kLdsBytes];
+    constexpr int BN = any_cols(BM);
+    using G = split_gemm::Tile<T, T, BM, BN, false, true, any_depth(BM)>;
+    constexpr int kRegion = split_gemm::store_bytes<float, 1>();
+    __shared__ __attribute__((aligned(16))) char lds[any_lds<G>(kRegion)];
     uint32_t slot, tile_n;
     if (!slot_tile(slots, max_slots, n_tiles, slot, tile_n)) return;
     const int e = slots.expert[slot];
-    const int64_t row0 = slots.row[slot], end = slots.end[slot], n0 = static_cast<int64_t>(tile_n) * kAnyCols;
+    const int64_t row0 = slots.row[slot], end = slots.end[slot], n0 = static_cast<int64_t>(tile_n) * BN;
     const int wave = threadIdx.x / kWave, wm = wave >> 1, wn = wave & 1;
     const T* w = Wo + e * width * hidden;
     auto a_row = [&](int r) { return d_out + min(max(rows[min(row0 + r, end - 1)], int64_t(0)), tokens - 1) * width; };
     G tile;
     const uint64_t chains = tile.template run<BYTES, 16>(
         lds, width, width, 0, ceil_div(width, G::BK) * G::BK, a_row, [&](int r) { return w + min(n0 + r, hidden - 1); },
-        [&](int t) { return wn * 64 + t * 32; }, 1, hidden);
+        [&](int t) { return wn * (BN / 2) + t * 32; }, 1, hidden);
     if constexpr (G::kNative) split_gemm::lds_barrier();
-    constexpr int kRegion = split_gemm::store_bytes<float, 1>();
-    static_assert(4 * kRegion <= G::kLdsBytes, "the output regions fit the operands' LDS");
     char* region = lds + wave * kRegion;
-    const int64_t first = n0 + wn * 64;
+    const int64_t first = n0 + wn * (BN / 2);
     float* part = dw_part + (2 * static_cast<int64_t>(tile_n) + wn) * pairs;
 #pragma unroll
     for (int i = 0; i < G::MT; ++i) {
@@ -290,34 +303,35 @@ __global__ __launch_bounds__(split_gemm::kThreads, 2) void any_hidden_gradient_k
     }
 }
 
-// dx of a slot's pairs x 128 columns: dg W_g + dv W_v, fp32.
+// dx of a slot's pairs x a tile's columns: dg W_g + dv W_v, fp32.
 template <typename T, int BM>
 __global__ __launch_bounds__(split_gemm::kThreads, 2) void any_input_gradient_kernel(
-    const float* __restrict__ dg, const float* __restrict__ dv, const T* __restrict__ Wg, const T* __restrict__ Wv,
+    const Between<T>* __restrict__ dg, const Between<T>* __restrict__ dv, const T* __restrict__ Wg, const T* __restrict__ Wv,
     float* __restrict__ dx, Slots slots, int64_t max_slots, int64_t width, int64_t hidden, int64_t ld, uint32_t n_tiles) {
-    using G = split_gemm::Tile<float, T, BM, kAnyCols, false, true>;
-    __shared__ __attribute__((aligned(16))) char lds[G::kLdsBytes];
+    constexpr int BN = any_cols(BM);
+    using G = split_gemm::Tile<Between<T>, T, BM, BN, false, true, any_depth(BM)>;
+    constexpr int kRegion = split_gemm::store_bytes<float, 1>();
+    __shared__ __attribute__((aligned(16))) char lds[any_lds<G>(kRegion)];
     uint32_t slot, tile_n;
     if (!slot_tile(slots, max_slots, n_tiles, slot, tile_n)) return;
     const int e = slots.expert[slot];
-    const int64_t row0 = slots.row[slot], end = slots.end[slot], n0 = static_cast<int64_t>(tile_n) * kAnyCols;
+    const int64_t row0 = slots.row[slot], end = slots.end[slot], n0 = static_cast<int64_t>(tile_n) * BN;
     const int wave = threadIdx.x / kWave, wm = wave >> 1, wn = wave & 1;
     split_gemm::f32x16 sum[G::MT][G::NT];
     uint64_t chains = 0;
     G tile;
     for (int half = 0; half < 2; ++half) {
-        const float* a = half ? dv : dg;
+        const Between<T>* a = half ? dv : dg;
         const T* w = (half ? Wv : Wg) + e * hidden * width;
         chains |= tile.template run<16, 16>(
             lds, ld, hidden, 0, ceil_div(hidden, G::BK) * G::BK, [&](int r) { return a + min(row0 + r, end - 1) * ld; },
-            [&](int r) { return w + min(n0 + r, width - 1); }, [&](int t) { return wn * 64 + t * 32; }, 1, width);
+            [&](int r) { return w + min(n0 + r, width - 1); }, [&](int t) { return wn * (BN / 2) + t * 32; }, 1, width);
 #pragma unroll
         for (int i = 0; i < G::MT; ++i)
 #pragma unroll
             for (int j = 0; j < G::NT; ++j) sum[i][j] = half ? sum[i][j] + tile.acc[i][j] : tile.acc[i][j];
     }
-    constexpr int kRegion = split_gemm::store_bytes<float, 1>();
-    const int64_t first = n0 + wn * 64;
+    const int64_t first = n0 + wn * (BN / 2);
 #pragma unroll
     for (int j = 0; j < G::NT; ++j)
 #pragma unroll
@@ -343,10 +357,11 @@ template <typename T, typename TA, typename TB, int BM>
 __global__ __launch_bounds__(split_gemm::kThreads, 2) void any_weight_gradient_kernel(
     const TA* __restrict__ A, const TB* __restrict__ B, const int64_t* __restrict__ offsets, T* __restrict__ C,
     int64_t pairs, int64_t M, int64_t N, int64_t lda, int64_t ldb, uint32_t m_tiles, uint32_t n_tiles) {
-    using G = split_gemm::Tile<TA, TB, BM, kAnyCols, true, true>;
-    __shared__ __attribute__((aligned(16))) char lds[G::kLdsBytes];
+    using G = split_gemm::Tile<TA, TB, BM, BM, true, true, BM == 64 ? 2 : 1>;
+    constexpr int kRegion = split_gemm::store_bytes<T, 1>();
+    __shared__ __attribute__((aligned(16))) char lds[any_lds<G>(kRegion)];
     const uint32_t per = m_tiles * n_tiles, e = blockIdx.x / per, within = blockIdx.x % per;
-    const int64_t m0 = static_cast<int64_t>(within / n_tiles) * BM, n0 = static_cast<int64_t>(within % n_tiles) * kAnyCols;
+    const int64_t m0 = static_cast<int64_t>(within / n_tiles) * BM, n0 = static_cast<int64_t>(within % n_tiles) * BM;
     const int64_t lo = min(max(offsets[e], int64_t(0)), pairs), K = min(max(offsets[e + 1], lo), pairs) - lo;
     const int wave = threadIdx.x / kWave, wm = wave >> 1, wn = wave & 1;
     T* out = C + static_cast<int64_t>(e) * M * N;
@@ -357,7 +372,7 @@ __global__ __launch_bounds__(split_gemm::kThreads, 2) void any_weight_gradient_k
     if (K > 0) {
         chains = tile.template run<16, 16>(
             lds, K, K, 0, ceil_div(K, G::BK) * G::BK, [&](int r) { return a + min(m0 + r, M - 1); },
-            [&](int r) { return b + min(n0 + r, N - 1); }, [&](int t) { return wn * 64 + t * 32; }, lda, ldb);
+            [&](int r) { return b + min(n0 + r, N - 1); }, [&](int t) { return wn * (BM / 2) + t * 32; }, lda, ldb);
     } else {
 #pragma unroll
         for (int i = 0; i < G::MT; ++i)
@@ -365,8 +380,7 @@ __global__ __launch_bounds__(split_gemm::kThreads, 2) void any_weight_gradient_k
             for (int j = 0; j < G::NT; ++j) tile.acc[i][j] = split_gemm::f32x16{};
     }
     if constexpr (G::kNative) split_gemm::lds_barrier();
-    constexpr int kRegion = split_gemm::store_bytes<T, 1>();
-    const int64_t first = n0 + wn * 64;
+    const int64_t first = n0 + wn * (BM / 2);
 #pragma unroll
     for (int j = 0; j < G::NT; ++j)
 #pragma unroll
@@ -1000,38 +1014,56 @@ __global__ __launch_bounds__(256) void weight_gradient_kernel(const float* __res
     dw[i] = sum;
 }
 
-// Column sums of each expert's rows. First each slot's (a workgroup per slot and 64
-// columns, four waves over the rows), then each expert's slots in order.
+// Column sums of each expert's rows, for the three biases in one launch each (blockIdx.z; an
+// out of NULL is not wanted). First each slot's (a workgroup per slot and 64 columns, four
+// waves over the rows), then each expert's slots in order.
+struct ColumnSums {
+    const void* a;     // rows of float (T for the third), lda apart
+    float* part;       // `per` rows a slot, ld apart
+    void* out;         // [experts, columns]
+    int64_t lda, ld, columns;
+    int per;
+};
+struct ThreeSums {
+    ColumnSums s[3];
+};
 template <typename TA>
-__global__ __launch_bounds__(256) void slot_sums_kernel(const TA* __restrict__ a, int64_t lda, const float* __restrict__ weights,
-                                                        float share, bool weighted, Slots slots, int64_t max_slots, int64_t rows,
-                                                        int64_t columns, float* __restrict__ part) {
+__device__ __forceinline__ float column_sum(const TA* a, int64_t lda, const float* weights, float share, bool weighted,
+                                            int64_t begin, int64_t end) {
+    float sum = 0.0f;
+    for (int64_t r = begin; r < end; r += 4)
+        sum = fmaf(weighted ? (weights ? weights[r] : share) : 1.0f, to_f32(a[r * lda]), sum);
+    return sum;
+}
+template <typename T>
+__global__ __launch_bounds__(256) void slot_sums_kernel(ThreeSums all, const float* __restrict__ weights, float share,
+                                                        Slots slots, int64_t max_slots, int64_t rows) {
+    const ColumnSums& s = all.s[blockIdx.z];
     const int64_t slot = blockIdx.x;
-    if (slot >= slots.expert[max_slots]) return;
+    if (!s.out || slot >= slots.expert[max_slots] || static_cast<int64_t>(blockIdx.y) * kWave >= s.columns) return;
     __shared__ float sh[4][kWave];
     const int wave = threadIdx.x / kWave;
     const int64_t c = static_cast<int64_t>(blockIdx.y) * kWave + lane_id();
     const int64_t r0 = slots.row[slot], end = min(slots.end[slot], r0 + rows);
     float sum = 0.0f;
-    if (c < columns)
-        for (int64_t r = r0 + wave; r < end; r += 4)
-            sum = fmaf(weighted ? (weights ? weights[r] : share) : 1.0f, to_f32(a[r * lda + c]), sum);
+    if (c < s.columns)
+        sum = blockIdx.z == 2 ? column_sum(static_cast<const T*>(s.a) + c, s.lda, weights, share, true, r0 + wave, end)
+                              : column_sum(static_cast<const float*>(s.a) + c, s.lda, weights, share, false, r0 + wave, end);
     sh[wave][lane_id()] = sum;
     __syncthreads();
-    if (wave == 0 && c < columns)
-        part[slot * columns + c] = (sh[0][lane_id()] + sh[1][lane_id()]) + (sh[2][lane_id()] + sh[3][lane_id()]);
+    if (wave == 0 && c < s.columns)
+        s.part[slot * s.ld + c] = (sh[0][lane_id()] + sh[1][lane_id()]) + (sh[2][lane_id()] + sh[3][lane_id()]);
 }
-// part: `per` rows a slot, ld apart.
 template <typename T>
-__global__ __launch_bounds__(256) void expert_sums_kernel(const float* __restrict__ part, const int32_t* __restrict__ first,
-                                                          T* __restrict__ out, int per, int64_t ld, int64_t columns) {
+__global__ __launch_bounds__(256) void expert_sums_kernel(ThreeSums all, const int32_t* __restrict__ first) {
+    const ColumnSums& s = all.s[blockIdx.z];
     const int64_t e = blockIdx.y, c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    if (c >= columns) return;
-    const int64_t end = static_cast<int64_t>(first[e + 1]) * per;
+    if (!s.out || c >= s.columns) return;
+    const int64_t end = static_cast<int64_t>(first[e + 1]) * s.per;
     float sum = 0.0f;
 #pragma unroll 8
-    for (int64_t s = static_cast<int64_t>(first[e]) * per; s < end; ++s) sum += part[s * ld + c];
-    out[e * columns + c] = from_f32<T>(sum);
+    for (int64_t i = static_cast<int64_t>(first[e]) * s.per; i < end; ++i) sum += s.part[i * s.ld + c];
+    static_cast<T*>(s.out)[e * s.columns + c] = from_f32<T>(sum);
 }
 
 // --------------------------------------------------------------- the calls ---
@@ -1111,15 +1143,15 @@ inline BackwardSpace backward_space(const Shape& s, void* base) {
         w.wh = c.take<float>(rows * ld);
     }
     w.dx = c.take<float>(s.pairs * s.width);
-    w.dw_part = c.take<float>(2 * ceil_div(s.hidden, kAnyCols) * s.pairs);
+    w.dw_part = c.take<float>(2 * ceil_div(s.hidden, tile_shape(s) ? kTile : any_cols(static_cast<int>(slot_rows(s)))) * s.pairs);
     if (tile_shape(s)) {
         w.dot = c.take<float>(ceil_div(s.width, kGatherColumns) * s.pairs);
         w.sums = c.take<float>(most_slots(s) * 4 * s.hidden);
         w.out_sums = c.take<float>(most_slots(s) * (kTile / kGatherRows) * s.width);
     } else {
         w.dot = c.take<float>(s.pairs);
-        w.sums = c.take<float>(most_slots(s) * std::max(s.width, s.hidden));
-        w.out_sums = nullptr;
+        w.sums = c.take<float>(most_slots(s) * 2 * s.hidden);
+        w.out_sums = c.take<float>(most_slots(s) * s.width);
     }
     w.xs = c.take<char>(rows * s.width * static_cast<int64_t>(element(s.dtype)));
     w.ds = c.take<char>(rows * s.width * static_cast<int64_t>(element(s.dtype)));
@@ -1135,7 +1167,7 @@ int check_shape(const char* what, const Shape& s) {
     if (s.tokens >= most || s.top_k > 256 || s.pairs >= most || s.width >= (1 << 24) || s.hidden >= (1 << 24) ||
         s.experts >= (1 << 20) ||
         most_slots(s) * ceil_div(std::max(s.width, s.hidden), 64) >= most ||
-        s.experts * ceil_div(s.width, 64) * ceil_div(s.hidden, kAnyCols) >= most ||
+        s.experts * ceil_div(s.width, 64) * ceil_div(s.hidden, 64) >= most ||
         s.tokens * ceil_div(s.width, 4) >= (int64_t(1) << 38))
         return fail(KOEMI_ERR_UNSUPPORTED, "%s: shape too large", what);
     return KOEMI_OK;
@@ -1166,6 +1198,11 @@ void combine(const float* rows, const int64_t* positions, const int64_t* offsets
                        static_cast<int>(s.top_k));
 }
 
+template <typename T>
+Between<T>* between(float* p) {
+    return reinterpret_cast<Between<T>*>(p);
+}
+
 struct Weights {
     const void *Wg, *bg, *Wv, *bv, *Wo, *bo;
 };
@@ -1192,9 +1229,9 @@ int any_forward(const Shape& s, const void* x, const int64_t* rows, const int64_
                                static_cast<const T*>(m.bv), keep, keep_v, w.h, w.slots, slots, s.width, s.hidden, ld, n);
         });
         by_bytes(split_gemm::load_bytes<T>(m.Wo, s.hidden), [&](auto bytes) {
-            const uint32_t n = static_cast<uint32_t>(ceil_div(s.width, kAnyCols));
+            const uint32_t n = static_cast<uint32_t>(ceil_div(s.width, any_cols(BM)));
             hipLaunchKernelGGL((any_output_kernel<T, BM, decltype(bytes)::value>), dim3(tiles_grid(slots, n)),
-                               dim3(split_gemm::kThreads), 0, q, w.h, static_cast<const T*>(m.Wo),
+                               dim3(split_gemm::kThreads), 0, q, between<T>(w.h), static_cast<const T*>(m.Wo),
                                static_cast<const T*>(m.bo), w.y, w.slots, slots, s.width, s.hidden, ld, n);
         });
     });
@@ -1216,8 +1253,8 @@ int any_backward(const Shape& s, const void* d_out, const void* x, const int64_t
         hipLaunchKernelGGL(gather_pairs_kernel<T>, dim3(grid_for(s.pairs, 4)), dim3(256), 0, q, static_cast<const T*>(x), dy,
                            rows, offsets, s.experts, static_cast<const T*>(m.bo), pair_experts, want_in ? xs : nullptr,
                            want_out ? ds : nullptr, d.weights ? w.dot : nullptr, s.pairs, s.tokens, s.width);
-    const uint32_t h_tiles = static_cast<uint32_t>(ceil_div(s.hidden, kAnyCols));
-    const uint32_t w_tiles = static_cast<uint32_t>(ceil_div(s.width, kAnyCols));
+    const int cols = any_cols(static_cast<int>(slot_rows(s)));
+    const uint32_t h_tiles = static_cast<uint32_t>(ceil_div(s.hidden, cols)), w_tiles = static_cast<uint32_t>(ceil_div(s.width, cols));
     by_rows(s, [&](auto rows_tag) {
         constexpr int BM = decltype(rows_tag)::value;
         by_bytes(split_gemm::load_bytes<T>(d_out, s.width), [&](auto bytes) {
@@ -1228,33 +1265,39 @@ int any_backward(const Shape& s, const void* d_out, const void* x, const int64_t
         });
         if (d.x)
             hipLaunchKernelGGL((any_input_gradient_kernel<T, BM>), dim3(tiles_grid(slots, w_tiles)), dim3(split_gemm::kThreads),
-                               0, q, w.dg, w.dv, static_cast<const T*>(m.Wg), static_cast<const T*>(m.Wv), w.dx, w.slots, slots,
+                               0, q, between<T>(w.dg), between<T>(w.dv), static_cast<const T*>(m.Wg), static_cast<const T*>(m.Wv), w.dx, w.slots, slots,
                                s.width, s.hidden, ld, w_tiles);
     });
     if (d.x) combine<T>(w.dx, positions, offsets, nullptr, 1.0f, d.x, s, q);
     if (d.weights)
         hipLaunchKernelGGL(weight_gradient_kernel, dim3(grid_for(s.pairs, 256)), dim3(256), 0, q, w.dw_part,
                            static_cast<int>(2 * h_tiles), w.dot, 1, positions, offsets + s.experts, d.weights, s.pairs);
+    // tiles of 64 x 64 where those of 128 x 128 would leave CUs idle
+    const int side = s.experts * ceil_div(s.width, 128) * ceil_div(s.hidden, 128) < 256 ? 64 : 128;
     auto product = [&](auto* a, auto* b, void* c, int64_t M, int64_t N, int64_t lda, int64_t ldb) {
         using TA = std::remove_pointer_t<decltype(a)>;
         using TB = std::remove_pointer_t<decltype(b)>;
-        const uint32_t mt = static_cast<uint32_t>(ceil_div(M, 128)), nt = static_cast<uint32_t>(ceil_div(N, kAnyCols));
-        hipLaunchKernelGGL((any_weight_gradient_kernel<T, TA, TB, 128>), dim3(static_cast<unsigned>(s.experts * mt * nt)),
-                           dim3(split_gemm::kThreads), 0, q, a, b, offsets, static_cast<T*>(c), s.pairs, M, N, lda, ldb, mt, nt);
+        const uint32_t mt = static_cast<uint32_t>(ceil_div(M, side)), nt = static_cast<uint32_t>(ceil_div(N, side));
+        auto launch = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(s.experts * mt * nt)), dim3(split_gemm::kThreads), 0, q, a, b,
+                               offsets, static_cast<T*>(c), s.pairs, M, N, lda, ldb, mt, nt);
+        };
+        if (side == 64) launch(any_weight_gradient_kernel<T, TA, TB, 64>);
+        else launch(any_weight_gradient_kernel<T, TA, TB, 128>);
     };
-    if (d.Wg) product(w.dg, xs, d.Wg, s.hidden, s.width, ld, s.width);
-    if (d.Wv) product(w.dv, xs, d.Wv, s.hidden, s.width, ld, s.width);
-    if (d.Wo) product(ds, w.wh, d.Wo, s.width, s.hidden, s.width, ld);
-    auto columns = [&](auto* a, int64_t lda, bool weighted, int64_t n, void* c) {
-        using TA = std::remove_pointer_t<decltype(a)>;
-        hipLaunchKernelGGL(slot_sums_kernel<TA>, dim3(static_cast<unsigned>(slots), static_cast<unsigned>(ceil_div(n, kWave))),
-                           dim3(256), 0, q, a, lda, sorted_w, share, weighted, w.slots, slots, slot_rows(s), n, w.sums);
-        hipLaunchKernelGGL(expert_sums_kernel<T>, dim3(grid_for(n, 256), static_cast<unsigned>(s.experts)), dim3(256), 0, q,
-                           w.sums, w.slots.first, static_cast<T*>(c), 1, n, n);
-    };
-    if (d.bg) columns(w.dg, ld, false, s.hidden, d.bg);
-    if (d.bv) columns(w.dv, ld, false, s.hidden, d.bv);
-    if (d.bo) columns(ds, s.width, true, s.width, d.bo);
+    if (d.Wg) product(between<T>(w.dg), xs, d.Wg, s.hidden, s.width, ld, s.width);
+    if (d.Wv) product(between<T>(w.dv), xs, d.Wv, s.hidden, s.width, ld, s.width);
+    if (d.Wo) product(ds, between<T>(w.wh), d.Wo, s.width, s.hidden, s.width, ld);
+    if (d.bg || d.bv || d.bo) {
+        const int64_t most = std::max(s.hidden, s.width);
+        const ThreeSums sums{{{w.dg, w.sums, d.bg, ld, 2 * s.hidden, s.hidden, 1},
+                              {w.dv, w.sums + s.hidden, d.bv, ld, 2 * s.hidden, s.hidden, 1},
+                              {ds, w.out_sums, d.bo, s.width, s.width, s.width, 1}}};
+        hipLaunchKernelGGL(slot_sums_kernel<T>, dim3(static_cast<unsigned>(slots), static_cast<unsigned>(ceil_div(most, kWave)), 3),
+                           dim3(256), 0, q, sums, sorted_w, share, w.slots, slots, slot_rows(s));
+        hipLaunchKernelGGL(expert_sums_kernel<T>, dim3(grid_for(most, 256), static_cast<unsigned>(s.experts), 3), dim3(256), 0, q,
+                           sums, w.slots.first);
+    }
     return check_launch("koemi_moe_experts_backward");
 }
 
@@ -1310,13 +1353,13 @@ int tile_backward(const Shape& s, const void* d_out, const void* x, const int64_
                            w.slots, static_cast<bf16*>(d.Wg), static_cast<bf16*>(d.Wv), static_cast<bf16*>(d.Wo), s.pairs,
                            s.width, s.hidden, w_tiles, h_tiles, tiles);
     }
-    auto expert_sums = [&](const float* part, int per, int64_t ld, int64_t n, void* c) {
-        hipLaunchKernelGGL(expert_sums_kernel<bf16>, dim3(grid_for(n, 256), static_cast<unsigned>(s.experts)), dim3(256), 0, q,
-                           part, w.slots.first, static_cast<bf16*>(c), per, ld, n);
-    };
-    if (d.bg) expert_sums(w.sums, 2, 2 * s.hidden, s.hidden, d.bg);
-    if (d.bv) expert_sums(w.sums + s.hidden, 2, 2 * s.hidden, s.hidden, d.bv);
-    if (d.bo) expert_sums(w.out_sums, kTile / kGatherRows, s.width, s.width, d.bo);
+    if (d.bg || d.bv || d.bo) {
+        const ThreeSums sums{{{nullptr, w.sums, d.bg, 0, 2 * s.hidden, s.hidden, 2},
+                              {nullptr, w.sums + s.hidden, d.bv, 0, 2 * s.hidden, s.hidden, 2},
+                              {nullptr, w.out_sums, d.bo, 0, s.width, s.width, kTile / kGatherRows}}};
+        hipLaunchKernelGGL(expert_sums_kernel<bf16>, dim3(grid_for(std::max(s.hidden, s.width), 256), static_cast<unsigned>(s.experts), 3),
+                           dim3(256), 0, q, sums, w.slots.first);
+    }
     return check_launch("koemi_moe_experts_backward(tiles)");
 }
 

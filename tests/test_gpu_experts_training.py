@@ -29,7 +29,8 @@ def reference(case, d_out):
     width, top_k = x.shape[-1], assignments.shape[-1]
     flat, ids, ok = x.detach().double().reshape(-1, width), assignments.reshape(-1, top_k).long(), valid.reshape(-1)
     experts, hidden, _ = case["gate_weights"].shape
-    R = 2.0 ** -8 if x.dtype == torch.bfloat16 and width % 64 == 0 and hidden % 64 == 0 else 0.0
+    R = 0.0 if x.dtype == torch.float32 else \
+        2.0 ** -8 if x.dtype == torch.bfloat16 and width % 64 == 0 and hidden % 64 == 0 else 2.0 ** -17
     w64 = w.detach().double().reshape(-1, top_k) if w is not None else torch.full(ids.shape, 1.0 / top_k, device=x.device).double()
     d = d_out.double().reshape(-1, width)
     zeros = torch.zeros_like
