@@ -1,0 +1,15 @@
+// The grouped GLU feed-forward of a few rows per expert (skinny_gemm_kernel of
+// moe_grouped_mlp.hip) for other sources: bf16 context rows by index, fp32 outputs.
+#pragma once
+
+#include "common.hpp"
+
+namespace koemi {
+
+bool few_rows_mlp_fits(int64_t pairs, int64_t width, int64_t hidden, int64_t experts, int dtype);
+// y [pairs, width]: the rows of the valid pairs alone are written; hidden_rows [pairs, hidden] bf16 is scratch.
+int few_rows_mlp(const void* x, const int64_t* rows, int64_t tokens, const int64_t* offsets, const void* Wg, const void* bg,
+                 const void* Wv, const void* bv, const void* Wo, const void* bo, void* hidden_rows, float* y, int64_t pairs,
+                 int64_t width, int64_t hidden, int64_t experts, hipStream_t stream);
+
+}  // namespace koemi

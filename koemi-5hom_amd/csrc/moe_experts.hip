@@ -22,6 +22,7 @@
 // operand either along K or across it; what lies between two products stays fp32 there
 // (two bf16 planes of it are multiplied where the result is 16-bit).
 #include "common.hpp"
+#include "few_rows_mlp.hpp"
 #include "mfma_across.hpp"
 #include "split_gemm.hpp"
 
@@ -280,6 +281,14 @@ __global__ __launch_bounds__(split_gemm::kThreads, 2) void any_hidden_gradient_k
         for (int j = 0; j < G::NT; ++j) {
             const int64_t c = first + j * 32;
             float a[1][16], b[1][16], h[1][16];
+            float kg[16], kv[16];
+#pragma unroll
+            for (int v = 0; v < 16; v += 4) {  // four units at once: rows are padded to eight
+                const int64_t at = mine * ld + min(c + acc_column(v), ld - 4);
+                const float4 g4 = load4(keep_g + at), v4 = load4(keep_v + at);
+                kg[v] = g4.x, kg[v + 1] = g4.y, kg[v + 2] = g4.z, kg[v + 3] = g4.w;
+                kv[v] = v4.x, kv[v + 1] = v4.y, kv[v + 2] = v4.z, kv[v + 3] = v4.w;
+            }
 #pragma unroll
             for (int v = 0; v < 16; ++v) {
                 const int64_t at = min(c + acc_column(v), hidden - 1);
@@ -287,7 +296,7 @@ __global__ __launch_bounds__(split_gemm::kThreads, 2) void any_hidden_gradient_k
                 if constexpr (!G::kNative)
                     if (__builtin_expect(chains >> ((i * G::NT + j) * 16 + v) & 1, 0))
                         d = split_gemm::scalar_dot(a_row(static_cast<int>(mine - row0)), w + at, width, 0.0f, 1, hidden);
-                const GluGradient o = glu_gradient(keep_g[mine * ld + at], keep_v[mine * ld + at], d, weight);
+                const GluGradient o = glu_gradient(kg[v], kv[v], d, weight);
                 const bool in = c + acc_column(v) < hidden;
                 a[0][v] = in ? o.dg : 0.0f;
                 b[0][v] = in ? o.dv : 0.0f;
@@ -303,11 +312,12 @@ __global__ __launch_bounds__(split_gemm::kThreads, 2) void any_hidden_gradient_k
     }
 }
 
-// dx of a slot's pairs x a tile's columns: dg W_g + dv W_v, fp32.
-template <typename T, int BM>
+// dx of a slot's pairs x a tile's columns: dg W_g, then (ADD) dv W_v added to it, fp32. In one
+// launch the first product's sums beside the second's spill (fp16 3000 tokens: 301 us).
+template <typename T, int BM, bool ADD>
 __global__ __launch_bounds__(split_gemm::kThreads, 2) void any_input_gradient_kernel(
-    const Between<T>* __restrict__ dg, const Between<T>* __restrict__ dv, const T* __restrict__ Wg, const T* __restrict__ Wv,
-    float* __restrict__ dx, Slots slots, int64_t max_slots, int64_t width, int64_t hidden, int64_t ld, uint32_t n_tiles) {
+    const Between<T>* __restrict__ d, const T* __restrict__ W, float* __restrict__ dx, Slots slots, int64_t max_slots,
+    int64_t width, int64_t hidden, int64_t ld, uint32_t n_tiles) {
     constexpr int BN = any_cols(BM);
     using G = split_gemm::Tile<Between<T>, T, BM, BN, false, true, any_depth(BM)>;
     constexpr int kRegion = split_gemm::store_bytes<float, 1>();
@@ -317,38 +327,28 @@ __global__ __launch_bounds__(split_gemm::kThreads, 2) void any_input_gradient_ke
     const int e = slots.expert[slot];
     const int64_t row0 = slots.row[slot], end = slots.end[slot], n0 = static_cast<int64_t>(tile_n) * BN;
     const int wave = threadIdx.x / kWave, wm = wave >> 1, wn = wave & 1;
-    split_gemm::f32x16 sum[G::MT][G::NT];
-    uint64_t chains = 0;
+    const T* w = W + e * hidden * width;
     G tile;
-    for (int half = 0; half < 2; ++half) {
-        const Between<T>* a = half ? dv : dg;
-        const T* w = (half ? Wv : Wg) + e * hidden * width;
-        chains |= tile.template run<16, 16>(
-            lds, ld, hidden, 0, ceil_div(hidden, G::BK) * G::BK, [&](int r) { return a + min(row0 + r, end - 1) * ld; },
-            [&](int r) { return w + min(n0 + r, width - 1); }, [&](int t) { return wn * (BN / 2) + t * 32; }, 1, width);
-#pragma unroll
-        for (int i = 0; i < G::MT; ++i)
-#pragma unroll
-            for (int j = 0; j < G::NT; ++j) sum[i][j] = half ? sum[i][j] + tile.acc[i][j] : tile.acc[i][j];
-    }
+    const uint64_t chains = tile.template run<16, 16>(
+        lds, ld, hidden, 0, ceil_div(hidden, G::BK) * G::BK, [&](int r) { return d + min(row0 + r, end - 1) * ld; },
+        [&](int r) { return w + min(n0 + r, width - 1); }, [&](int t) { return wn * (BN / 2) + t * 32; }, 1, width);
     const int64_t first = n0 + wn * (BN / 2);
 #pragma unroll
     for (int j = 0; j < G::NT; ++j)
 #pragma unroll
         for (int i = 0; i < G::MT; ++i) {
-            const int64_t r = row0 + wm * (BM / 2) + i * 32, c = first + j * 32;
+            const int64_t r = row0 + wm * (BM / 2) + i * 32, c = first + j * 32, mine = min(r + (lane_id() & 31), end - 1);
             float o[1][16];
 #pragma unroll
-            for (int v = 0; v < 16; ++v) o[0][v] = sum[i][j][v];
+            for (int v = 0; v < 16; ++v) {
+                const int64_t at = min(c + acc_column(v), width - 1);
+                float sum = tile.acc[i][j][v];
+                if (__builtin_expect(chains >> ((i * G::NT + j) * 16 + v) & 1, 0))
+                    sum = split_gemm::scalar_dot(d + mine * ld, w + at, hidden, 0.0f, 1, width);
+                o[0][v] = ADD ? dx[mine * width + at] + sum : sum;
+            }
             split_gemm::store_rows<float, 1>(lds + wave * kRegion, o, dx + r * width + c, width, end - r, width - c, width % 8 == 0);
         }
-    split_gemm::fix_chains(chains, [&](int block, int v) {
-        const int64_t r = row0 + wm * (BM / 2) + block / G::NT * 32 + (lane_id() & 31);
-        const int64_t c = first + block % G::NT * 32 + acc_column(v);
-        if (r >= end || c >= width) return;
-        const float part = split_gemm::scalar_dot(dg + r * ld, Wg + e * hidden * width + c, hidden, 0.0f, 1, width);
-        dx[r * width + c] = split_gemm::scalar_dot(dv + r * ld, Wv + e * hidden * width + c, hidden, part, 1, width);
-    });
 }
 
 // One expert's C[m, n] = sum over its pairs of A[pair, m] B[pair, n] (rows lda and ldb
@@ -996,22 +996,26 @@ __global__ __launch_bounds__(256) void gather_pairs_kernel(const T* __restrict__
     }
 }
 
-// dw of every pair in token order: the parts of its row's <d', h> and <dout, b_o> in order; 0
-// past the valid pairs.
+// dw of every pair: the parts of its row's <d', h> and <dout, b_o> in order, 0 past the valid
+// pairs. A thread per sorted row (the parts lie in that order), which looks for its slot
+// among its token's.
 __global__ __launch_bounds__(256) void weight_gradient_kernel(const float* __restrict__ part, int parts,
                                                               const float* __restrict__ dot, int dot_parts,
+                                                              const int64_t* __restrict__ rows,
                                                               const int64_t* __restrict__ positions,
                                                               const int64_t* __restrict__ valid_end, float* __restrict__ dw,
-                                                              int64_t pairs) {
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    if (i >= pairs) return;
-    const int64_t p = positions[i];
+                                                              int64_t pairs, int top_k) {
+    const int64_t p = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (p >= pairs) return;
     float sum = 0.0f;
-    if (p >= 0 && p < *valid_end) {
+    if (p < *valid_end) {
+#pragma unroll 4
         for (int j = 0; j < parts; ++j) sum += part[j * pairs + p];
         for (int j = 0; j < dot_parts; ++j) sum += dot[j * pairs + p];
     }
-    dw[i] = sum;
+    const int64_t t = min(max(rows[p], int64_t(0)), pairs / top_k - 1);
+    for (int s = 0; s < top_k; ++s)
+        if (positions[t * top_k + s] == p) dw[t * top_k + s] = sum;
 }
 
 // Column sums of each expert's rows, for the three biases in one launch each (blockIdx.z; an
@@ -1263,15 +1267,19 @@ int any_backward(const Shape& s, const void* d_out, const void* x, const int64_t
                                keep + s.pairs * ld, sorted_w, share, w.dg, w.dv, w.wh, w.dw_part, w.slots, slots, s.pairs,
                                s.width, s.hidden, ld, h_tiles);
         });
-        if (d.x)
-            hipLaunchKernelGGL((any_input_gradient_kernel<T, BM>), dim3(tiles_grid(slots, w_tiles)), dim3(split_gemm::kThreads),
-                               0, q, between<T>(w.dg), between<T>(w.dv), static_cast<const T*>(m.Wg), static_cast<const T*>(m.Wv), w.dx, w.slots, slots,
-                               s.width, s.hidden, ld, w_tiles);
+        if (d.x) {
+            const dim3 grid(tiles_grid(slots, w_tiles)), threads(split_gemm::kThreads);
+            hipLaunchKernelGGL((any_input_gradient_kernel<T, BM, false>), grid, threads, 0, q, between<T>(w.dg),
+                               static_cast<const T*>(m.Wg), w.dx, w.slots, slots, s.width, s.hidden, ld, w_tiles);
+            hipLaunchKernelGGL((any_input_gradient_kernel<T, BM, true>), grid, threads, 0, q, between<T>(w.dv),
+                               static_cast<const T*>(m.Wv), w.dx, w.slots, slots, s.width, s.hidden, ld, w_tiles);
+        }
     });
     if (d.x) combine<T>(w.dx, positions, offsets, nullptr, 1.0f, d.x, s, q);
     if (d.weights)
         hipLaunchKernelGGL(weight_gradient_kernel, dim3(grid_for(s.pairs, 256)), dim3(256), 0, q, w.dw_part,
-                           static_cast<int>(2 * h_tiles), w.dot, 1, positions, offsets + s.experts, d.weights, s.pairs);
+                           static_cast<int>(2 * h_tiles), w.dot, 1, rows, positions, offsets + s.experts, d.weights, s.pairs,
+                           static_cast<int>(s.top_k));
     // tiles of 64 x 64 where those of 128 x 128 would leave CUs idle
     const int side = s.experts * ceil_div(s.width, 128) * ceil_div(s.hidden, 128) < 256 ? 64 : 128;
     auto product = [&](auto* a, auto* b, void* c, int64_t M, int64_t N, int64_t lda, int64_t ldb) {
@@ -1345,8 +1353,8 @@ int tile_backward(const Shape& s, const void* d_out, const void* x, const int64_
     }
     if (d.weights)
         hipLaunchKernelGGL(weight_gradient_kernel, dim3(grid_for(s.pairs, 256)), dim3(256), 0, q, w.dw_part,
-                           static_cast<int>(2 * h_tiles), w.dot, static_cast<int>(blocks), positions, offsets + s.experts,
-                           d.weights, s.pairs);
+                           static_cast<int>(2 * h_tiles), w.dot, static_cast<int>(blocks), rows, positions, offsets + s.experts,
+                           d.weights, s.pairs, static_cast<int>(s.top_k));
     if (d.Wg || d.Wv || d.Wo) {
         const uint32_t tiles = static_cast<uint32_t>(s.experts) * 3 * w_tiles * h_tiles;
         hipLaunchKernelGGL(tile_weight_gradient_kernel, dim3((tiles + 7) / 8 * 8), threads, 0, q, dgv, wh, xs, ds, offsets,
@@ -1408,11 +1416,18 @@ extern "C" int koemi_moe_experts_forward(const void* context, const int64_t* sor
     if (!workspace || workspace_bytes < w.bytes) return fail(KOEMI_ERR_INVALID, "%s: workspace too small", what);
     float* keep = static_cast<float*>(saved);
     hipStream_t q = as_stream(stream);
-    if (tile_shape(s)) {
-        if (!aligned16({context, m.Wg, m.Wv, m.Wo, saved, workspace}))
-            return fail(KOEMI_ERR_INVALID, "%s: operands must be 16-byte aligned", what);
-        return tile_forward(s, context, sorted_rows, segment_offsets, pair_positions, pair_weights, m, output, keep, w, q);
+    const bool few = !saved && few_rows_mlp_fits(s.pairs, width, hidden, expert_count, dtype);
+    if ((tile_shape(s) || few) && !aligned16({context, m.Wg, m.Wv, m.Wo, saved, workspace}))
+        return fail(KOEMI_ERR_INVALID, "%s: operands must be 16-byte aligned", what);
+    if (few) {  // a decode step: bound by the weights, read once
+        const int rc = few_rows_mlp(context, sorted_rows, tokens, segment_offsets, m.Wg, m.bg, m.Wv, m.bv, m.Wo, m.bo, w.h, w.y,
+                                    s.pairs, width, hidden, expert_count, q);
+        if (rc != KOEMI_OK) return rc;
+        combine<bf16>(w.y, pair_positions, segment_offsets, pair_weights, 1.0f / static_cast<float>(top_k), output, s, q);
+        return check_launch("koemi_moe_experts_forward(few rows)");
     }
+    if (tile_shape(s))
+        return tile_forward(s, context, sorted_rows, segment_offsets, pair_positions, pair_weights, m, output, keep, w, q);
     if (dtype == KOEMI_F32)
         return any_forward<float>(s, context, sorted_rows, segment_offsets, pair_positions, pair_weights, m, output, keep, w, q);
     if (dtype == KOEMI_F16)

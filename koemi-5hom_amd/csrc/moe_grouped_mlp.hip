@@ -18,6 +18,7 @@
 // valid pairs are zero-filled. float32, float16 and shapes off the bf16 tiles run
 // on tiles of split_gemm.hpp (the any-shape path below).
 #include "common.hpp"
+#include "few_rows_mlp.hpp"
 #include "mfma_stage.hpp"
 #include "split_gemm.hpp"
 
@@ -728,11 +729,11 @@ constexpr int64_t kSkinnyMaxRowsPerExpert = 64;  // average over experts below w
 #define KOEMI_SKINNY_OUT 4, 1, 2  // S, G, PF of the output GEMM
 #endif
 
-template <bool GLU, bool FRAG, int S, int G, int PF>
+template <bool GLU, bool FRAG, typename C, int S, int G, int PF>
 __global__ __launch_bounds__(S * G * kWave) void skinny_gemm_kernel(
     const bf16* __restrict__ a, const int64_t* __restrict__ a_index, int64_t a_count,
     const bf16* __restrict__ w0, const bf16* __restrict__ w1,
-    const bf16* __restrict__ bias0, const bf16* __restrict__ bias1, bf16* __restrict__ c,
+    const bf16* __restrict__ bias0, const bf16* __restrict__ bias1, C* __restrict__ c,
     const int64_t* __restrict__ offsets, int64_t n_out, int64_t K, int64_t col_groups, int64_t experts,
     int64_t pairs) {
     static_assert(S == 1 || G == 1, "waves that split K share one task per workgroup (the barriers)");
@@ -745,7 +746,7 @@ __global__ __launch_bounds__(S * G * kWave) void skinny_gemm_kernel(
         const int64_t extra = gridDim.x - task_blocks;
         const int64_t start = min(max(offsets[experts], int64_t(0)), pairs);
         for (int64_t p = start + (blockIdx.x - task_blocks); p < pairs; p += extra)
-            for (int64_t q = threadIdx.x; q < n_out; q += blockDim.x) c[p * n_out + q] = from_f32<bf16>(0.0f);
+            for (int64_t q = threadIdx.x; q < n_out; q += blockDim.x) c[p * n_out + q] = from_f32<C>(0.0f);
         return;
     }
     const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
@@ -828,7 +829,7 @@ __global__ __launch_bounds__(S * G * kWave) void skinny_gemm_kernel(
                 float out;
                 if constexpr (GLU) out = silu_f(acc[0][i] + b0) * (acc[kMats - 1][i] + b1);
                 else out = acc[0][i] + b0;
-                c[(row0 + pass + row) * n_out + col] = from_f32<bf16>(out);
+                c[(row0 + pass + row) * n_out + col] = from_f32<C>(out);
             }
         } else {
 #pragma unroll
@@ -851,41 +852,41 @@ __global__ __launch_bounds__(S * G * kWave) void skinny_gemm_kernel(
                 float out;
                 if constexpr (GLU) out = silu_f(v0 + b0) * (v1 + b1);
                 else out = v0 + b0;
-                c[(row0 + pass + row) * n_out + col] = from_f32<bf16>(out);
+                c[(row0 + pass + row) * n_out + col] = from_f32<C>(out);
             }
             __syncthreads();  // red is rewritten by the next pass
         }
     }
 }
 
-// Launch of skinny_gemm_kernel<GLU, FRAG, S, G, PF> over every task (plus
+// Launch of skinny_gemm_kernel<GLU, FRAG, C, S, G, PF> over every task (plus
 // `tail_wgs` workgroups that zero the rows past the valid pairs).
-template <bool GLU, bool FRAG, int S, int G, int PF>
+template <bool GLU, bool FRAG, typename C, int S, int G, int PF>
 void launch_skinny(const bf16* a, const int64_t* a_index, int64_t a_count, const bf16* w0, const bf16* w1,
-                   const bf16* bias0, const bf16* bias1, bf16* c, const int64_t* offsets, int64_t n_out, int64_t K,
+                   const bf16* bias0, const bf16* bias1, C* c, const int64_t* offsets, int64_t n_out, int64_t K,
                    int64_t experts, int64_t pairs, int64_t tail_wgs, hipStream_t s) {
     const int64_t groups = n_out / kSkinnyCols;
     const int64_t blocks = (experts * groups + G - 1) / G + tail_wgs;
-    hipLaunchKernelGGL((skinny_gemm_kernel<GLU, FRAG, S, G, PF>), dim3(static_cast<unsigned>(blocks)), dim3(S * G * kWave),
+    hipLaunchKernelGGL((skinny_gemm_kernel<GLU, FRAG, C, S, G, PF>), dim3(static_cast<unsigned>(blocks)), dim3(S * G * kWave),
                        0, s, a, a_index, a_count, w0, w1, bias0, bias1, c, offsets, n_out, K, groups, experts, pairs);
 }
 
 // Both GEMMs of the skinny path: GEMM 1 into the bf16 hidden rows H, GEMM 2
 // into y (with zero_tail, extra workgroups of its launch zero the rows past
 // the valid pairs).
-template <bool FRAG>
+template <bool FRAG, typename Y = bf16>
 int run_skinny(const void* x, const int64_t* x_index, int64_t x_rows, const int64_t* offsets, const void* Wg,
                const void* bg, const void* Wv, const void* bv, const void* Wo, const void* bo, void* y, int64_t P,
                int64_t D, int64_t Hd, int64_t E, bf16* H, hipStream_t s, bool zero_tail) {
-    launch_skinny<true, FRAG, KOEMI_SKINNY_GLU>(static_cast<const bf16*>(x), x_index, x_rows, static_cast<const bf16*>(Wg),
+    launch_skinny<true, FRAG, bf16, KOEMI_SKINNY_GLU>(static_cast<const bf16*>(x), x_index, x_rows, static_cast<const bf16*>(Wg),
                                                 static_cast<const bf16*>(Wv), static_cast<const bf16*>(bg),
                                                 static_cast<const bf16*>(bv), H, offsets, Hd, D, E, P, 0, s);
     int st = check_launch("koemi_moe_grouped_mlp(skinny gemm1)");
     if (st != KOEMI_OK) return st;
     const int64_t tail_wgs = zero_tail ? (P < 64 ? P : 64) : 0;
-    launch_skinny<false, FRAG, KOEMI_SKINNY_OUT>(H, nullptr, P, static_cast<const bf16*>(Wo),
+    launch_skinny<false, FRAG, Y, KOEMI_SKINNY_OUT>(H, nullptr, P, static_cast<const bf16*>(Wo),
                                                  static_cast<const bf16*>(Wo), static_cast<const bf16*>(bo),
-                                                 static_cast<const bf16*>(bo), static_cast<bf16*>(y), offsets, D, Hd, E,
+                                                 static_cast<const bf16*>(bo), static_cast<Y*>(y), offsets, D, Hd, E,
                                                  P, tail_wgs, s);
     return check_launch("koemi_moe_grouped_mlp(skinny gemm2)");
 }
@@ -1100,6 +1101,17 @@ int run_mfma(const void* x, const int64_t* x_index, int64_t x_rows, const int64_
 }
 
 }  // namespace
+
+bool few_rows_mlp_fits(int64_t pairs, int64_t width, int64_t hidden, int64_t experts, int dtype) {
+    return mfma_shape(width, hidden, dtype) && pairs <= kSkinnyMaxRowsPerExpert * experts;
+}
+int few_rows_mlp(const void* x, const int64_t* rows, int64_t tokens, const int64_t* offsets, const void* Wg, const void* bg,
+                 const void* Wv, const void* bv, const void* Wo, const void* bo, void* hidden_rows, float* y, int64_t pairs,
+                 int64_t width, int64_t hidden, int64_t experts, hipStream_t stream) {
+    return run_skinny<false, float>(x, rows, tokens, offsets, Wg, bg, Wv, bv, Wo, bo, y, pairs, width, hidden, experts,
+                                    static_cast<bf16*>(hidden_rows), stream, false);
+}
+
 }  // namespace koemi
 
 using namespace koemi;
