@@ -79,7 +79,7 @@ template <int B, int BYTES>
 __global__ __launch_bounds__(split_gemm::kThreads, 2) void gate_products_kernel(
     const float* __restrict__ u, const float* __restrict__ wr, const float* __restrict__ wc, float* __restrict__ zr,
     float* __restrict__ zc, int64_t rows, int64_t D, uint32_t row_tiles, uint32_t half_tiles) {
-    using Tile = split_gemm::Tile<float, float, B, B, false, false, B == 64 ? 4 : 1>;
+    using Tile = split_gemm::Tile<float, float, B, B, split_gemm::kAlong, split_gemm::kAlong, B == 64 ? 4 : 1>;
     constexpr int kRegion = split_gemm::store_bytes<float, 1>();
     static_assert(4 * kRegion <= Tile::kLdsBytes, "the output regions fit the operands' LDS");
     __shared__ __attribute__((aligned(16))) char lds[Tile::kLdsBytes];

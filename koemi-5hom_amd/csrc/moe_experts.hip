@@ -130,6 +130,19 @@ inline int any_rows(int64_t pairs, int64_t experts) { return pairs <= 96 * exper
 __host__ __device__ constexpr int any_cols(int rows) { return rows == 64 ? 64 : 128; }
 __host__ __device__ constexpr int any_depth(int rows) { return rows == 64 ? 4 : 1; }
 
+// The gradients' tiles are 64 columns wide throughout: more of them, and more workgroups a CU
+// (fp16 3000 tokens, 768 -> 2000: hidden 130 us and input 276 with 128 columns, 91 and 241 with
+// 64). Where the rows that lie across K allow it they are read eight columns at once: hidden
+// 75 us, input 200, each weight's 109 -> 72.
+constexpr int kGradientCols = 64;
+using split_gemm::kAcross;
+using split_gemm::kStrided;
+// The column that a thread reads from, of `columns` across K: for those past the last, the last octet (kAcross) or the last.
+template <int LIES>
+__device__ __forceinline__ int64_t column_of(int64_t c, int64_t columns) {
+    return min(c, columns - (LIES == kAcross ? 8 : 1));
+}
+
 // What lies between two products, as their operand beside T: fp32 in memory.
 template <typename T>
 using Between = std::conditional_t<std::is_same<T, float>::value, float, split_gemm::coarse_f32>;
@@ -147,7 +160,7 @@ __global__ __launch_bounds__(split_gemm::kThreads, 2) void any_hidden_kernel(
     const T* __restrict__ bg, const T* __restrict__ Wv, const T* __restrict__ bv, float* __restrict__ keep_g,
     float* __restrict__ keep_v, float* __restrict__ h, Slots slots, int64_t max_slots, int64_t width, int64_t hidden,
     int64_t ld, uint32_t n_tiles) {
-    using G = split_gemm::Tile<T, T, BM, 128, false, false, BM == 64 ? 2 : 1>;
+    using G = split_gemm::Tile<T, T, BM, 128, split_gemm::kAlong, split_gemm::kAlong, BM == 64 ? 2 : 1>;
     constexpr int kRegion = split_gemm::store_bytes<float, 1>();
     __shared__ __attribute__((aligned(16))) char lds[any_lds<G>(kRegion)];
     uint32_t slot, tile_n;
@@ -211,7 +224,7 @@ __global__ __launch_bounds__(split_gemm::kThreads, 2) void any_output_kernel(
     const Between<T>* __restrict__ h, const T* __restrict__ Wo, const T* __restrict__ bo, float* __restrict__ y, Slots slots,
     int64_t max_slots, int64_t width, int64_t hidden, int64_t ld, uint32_t n_tiles) {
     constexpr int BN = any_cols(BM);
-    using G = split_gemm::Tile<Between<T>, T, BM, BN, false, false, any_depth(BM)>;
+    using G = split_gemm::Tile<Between<T>, T, BM, BN, split_gemm::kAlong, split_gemm::kAlong, any_depth(BM)>;
     constexpr int kRegion = split_gemm::store_bytes<float, 1>();
     __shared__ __attribute__((aligned(16))) char lds[any_lds<G>(kRegion)];
     uint32_t slot, tile_n;
@@ -247,14 +260,14 @@ __global__ __launch_bounds__(split_gemm::kThreads, 2) void any_output_kernel(
 // d' = W_o^T dout of a slot's pairs x a tile's hidden units and what follows from it: dg, dv
 // and w h (fp32, rows ld apart, zeros from `hidden` on), and each row's part of dw from
 // a wave's half of them: dw_part[(2 tile + wave column) pairs + row].
-template <typename T, int BM, int BYTES>
+template <typename T, int BM, int BYTES, int LIES>
 __global__ __launch_bounds__(split_gemm::kThreads, 2) void any_hidden_gradient_kernel(
     const T* __restrict__ d_out, const int64_t* __restrict__ rows, int64_t tokens, const T* __restrict__ Wo,
     const float* __restrict__ keep_g, const float* __restrict__ keep_v, const float* __restrict__ sorted_w, float share,
     float* __restrict__ dg, float* __restrict__ dv, float* __restrict__ wh, float* __restrict__ dw_part, Slots slots,
     int64_t max_slots, int64_t pairs, int64_t width, int64_t hidden, int64_t ld, uint32_t n_tiles) {
-    constexpr int BN = any_cols(BM);
-    using G = split_gemm::Tile<T, T, BM, BN, false, true, any_depth(BM)>;
+    constexpr int BN = kGradientCols;
+    using G = split_gemm::Tile<T, T, BM, BN, split_gemm::kAlong, LIES, any_depth(BM)>;
     constexpr int kRegion = split_gemm::store_bytes<float, 1>();
     __shared__ __attribute__((aligned(16))) char lds[any_lds<G>(kRegion)];
     uint32_t slot, tile_n;
@@ -266,7 +279,7 @@ __global__ __launch_bounds__(split_gemm::kThreads, 2) void any_hidden_gradient_k
     auto a_row = [&](int r) { return d_out + min(max(rows[min(row0 + r, end - 1)], int64_t(0)), tokens - 1) * width; };
     G tile;
     const uint64_t chains = tile.template run<BYTES, 16>(
-        lds, width, width, 0, ceil_div(width, G::BK) * G::BK, a_row, [&](int r) { return w + min(n0 + r, hidden - 1); },
+        lds, width, width, 0, ceil_div(width, G::BK) * G::BK, a_row, [&](int r) { return w + column_of<LIES>(n0 + r, hidden); },
         [&](int t) { return wn * (BN / 2) + t * 32; }, 1, hidden);
     if constexpr (G::kNative) split_gemm::lds_barrier();
     char* region = lds + wave * kRegion;
@@ -314,12 +327,12 @@ __global__ __launch_bounds__(split_gemm::kThreads, 2) void any_hidden_gradient_k
 
 // dx of a slot's pairs x a tile's columns: dg W_g, then (ADD) dv W_v added to it, fp32. In one
 // launch the first product's sums beside the second's spill (fp16 3000 tokens: 301 us).
-template <typename T, int BM, bool ADD>
+template <typename T, int BM, int LIES, bool ADD>
 __global__ __launch_bounds__(split_gemm::kThreads, 2) void any_input_gradient_kernel(
     const Between<T>* __restrict__ d, const T* __restrict__ W, float* __restrict__ dx, Slots slots, int64_t max_slots,
     int64_t width, int64_t hidden, int64_t ld, uint32_t n_tiles) {
-    constexpr int BN = any_cols(BM);
-    using G = split_gemm::Tile<Between<T>, T, BM, BN, false, true, any_depth(BM)>;
+    constexpr int BN = kGradientCols;
+    using G = split_gemm::Tile<Between<T>, T, BM, BN, split_gemm::kAlong, LIES, any_depth(BM)>;
     constexpr int kRegion = split_gemm::store_bytes<float, 1>();
     __shared__ __attribute__((aligned(16))) char lds[any_lds<G>(kRegion)];
     uint32_t slot, tile_n;
@@ -331,7 +344,7 @@ __global__ __launch_bounds__(split_gemm::kThreads, 2) void any_input_gradient_ke
     G tile;
     const uint64_t chains = tile.template run<16, 16>(
         lds, ld, hidden, 0, ceil_div(hidden, G::BK) * G::BK, [&](int r) { return d + min(row0 + r, end - 1) * ld; },
-        [&](int r) { return w + min(n0 + r, width - 1); }, [&](int t) { return wn * (BN / 2) + t * 32; }, 1, width);
+        [&](int r) { return w + column_of<LIES>(n0 + r, width); }, [&](int t) { return wn * (BN / 2) + t * 32; }, 1, width);
     const int64_t first = n0 + wn * (BN / 2);
 #pragma unroll
     for (int j = 0; j < G::NT; ++j)
@@ -353,11 +366,11 @@ __global__ __launch_bounds__(split_gemm::kThreads, 2) void any_input_gradient_ke
 
 // One expert's C[m, n] = sum over its pairs of A[pair, m] B[pair, n] (rows lda and ldb
 // apart), in type T; zeros for an expert without pairs.
-template <typename T, typename TA, typename TB, int BM>
+template <typename T, typename TA, typename TB, int BM, int A_LIES, int B_LIES>
 __global__ __launch_bounds__(split_gemm::kThreads, 2) void any_weight_gradient_kernel(
     const TA* __restrict__ A, const TB* __restrict__ B, const int64_t* __restrict__ offsets, T* __restrict__ C,
     int64_t pairs, int64_t M, int64_t N, int64_t lda, int64_t ldb, uint32_t m_tiles, uint32_t n_tiles) {
-    using G = split_gemm::Tile<TA, TB, BM, BM, true, true, BM == 64 ? 2 : 1>;
+    using G = split_gemm::Tile<TA, TB, BM, BM, A_LIES, B_LIES, BM == 64 ? 2 : 1>;
     constexpr int kRegion = split_gemm::store_bytes<T, 1>();
     __shared__ __attribute__((aligned(16))) char lds[any_lds<G>(kRegion)];
     const uint32_t per = m_tiles * n_tiles, e = blockIdx.x / per, within = blockIdx.x % per;
@@ -371,8 +384,8 @@ __global__ __launch_bounds__(split_gemm::kThreads, 2) void any_weight_gradient_k
     uint64_t chains = 0;
     if (K > 0) {
         chains = tile.template run<16, 16>(
-            lds, K, K, 0, ceil_div(K, G::BK) * G::BK, [&](int r) { return a + min(m0 + r, M - 1); },
-            [&](int r) { return b + min(n0 + r, N - 1); }, [&](int t) { return wn * (BM / 2) + t * 32; }, lda, ldb);
+            lds, K, K, 0, ceil_div(K, G::BK) * G::BK, [&](int r) { return a + column_of<A_LIES>(m0 + r, M); },
+            [&](int r) { return b + column_of<B_LIES>(n0 + r, N); }, [&](int t) { return wn * (BM / 2) + t * 32; }, lda, ldb);
     } else {
 #pragma unroll
         for (int i = 0; i < G::MT; ++i)
@@ -1147,7 +1160,7 @@ inline BackwardSpace backward_space(const Shape& s, void* base) {
         w.wh = c.take<float>(rows * ld);
     }
     w.dx = c.take<float>(s.pairs * s.width);
-    w.dw_part = c.take<float>(2 * ceil_div(s.hidden, tile_shape(s) ? kTile : any_cols(static_cast<int>(slot_rows(s)))) * s.pairs);
+    w.dw_part = c.take<float>(2 * ceil_div(s.hidden, tile_shape(s) ? kTile : kGradientCols) * s.pairs);
     if (tile_shape(s)) {
         w.dot = c.take<float>(ceil_div(s.width, kGatherColumns) * s.pairs);
         w.sums = c.take<float>(most_slots(s) * 4 * s.hidden);
@@ -1183,6 +1196,16 @@ template <typename F>
 void by_rows(const Shape& s, F f) {
     if (any_rows(s.pairs, s.experts) == 64) f(std::integral_constant<int, 64>{});
     else f(std::integral_constant<int, 128>{});
+}
+// Whether the rows of an operand across K can be read eight columns at once.
+template <typename T>
+bool octets(const void* base, int64_t columns, int64_t ld) {
+    return columns % 8 == 0 && reinterpret_cast<uintptr_t>(base) % 16 == 0 && ld * sizeof(T) % 16 == 0;
+}
+template <typename F>
+void by_lies(bool across, F f) {
+    if (across) f(std::integral_constant<int, kAcross>{});
+    else f(std::integral_constant<int, kStrided>{});
 }
 template <typename F>
 void by_bytes(int bytes, F f) {
@@ -1257,23 +1280,26 @@ int any_backward(const Shape& s, const void* d_out, const void* x, const int64_t
         hipLaunchKernelGGL(gather_pairs_kernel<T>, dim3(grid_for(s.pairs, 4)), dim3(256), 0, q, static_cast<const T*>(x), dy,
                            rows, offsets, s.experts, static_cast<const T*>(m.bo), pair_experts, want_in ? xs : nullptr,
                            want_out ? ds : nullptr, d.weights ? w.dot : nullptr, s.pairs, s.tokens, s.width);
-    const int cols = any_cols(static_cast<int>(slot_rows(s)));
-    const uint32_t h_tiles = static_cast<uint32_t>(ceil_div(s.hidden, cols)), w_tiles = static_cast<uint32_t>(ceil_div(s.width, cols));
+    const uint32_t h_tiles = static_cast<uint32_t>(ceil_div(s.hidden, kGradientCols));
+    const uint32_t w_tiles = static_cast<uint32_t>(ceil_div(s.width, kGradientCols));
     by_rows(s, [&](auto rows_tag) {
         constexpr int BM = decltype(rows_tag)::value;
         by_bytes(split_gemm::load_bytes<T>(d_out, s.width), [&](auto bytes) {
-            hipLaunchKernelGGL((any_hidden_gradient_kernel<T, BM, decltype(bytes)::value>), dim3(tiles_grid(slots, h_tiles)),
-                               dim3(split_gemm::kThreads), 0, q, dy, rows, s.tokens, static_cast<const T*>(m.Wo), keep,
-                               keep + s.pairs * ld, sorted_w, share, w.dg, w.dv, w.wh, w.dw_part, w.slots, slots, s.pairs,
-                               s.width, s.hidden, ld, h_tiles);
+            by_lies(octets<T>(m.Wo, s.hidden, s.hidden), [&](auto lies) {
+                hipLaunchKernelGGL((any_hidden_gradient_kernel<T, BM, decltype(bytes)::value, decltype(lies)::value>),
+                                   dim3(tiles_grid(slots, h_tiles)), dim3(split_gemm::kThreads), 0, q, dy, rows, s.tokens,
+                                   static_cast<const T*>(m.Wo), keep, keep + s.pairs * ld, sorted_w, share, w.dg, w.dv, w.wh,
+                                   w.dw_part, w.slots, slots, s.pairs, s.width, s.hidden, ld, h_tiles);
+            });
         });
-        if (d.x) {
+        if (d.x) by_lies(octets<T>(m.Wg, s.width, s.width) && octets<T>(m.Wv, s.width, s.width), [&](auto lies) {
+            constexpr int kLies = decltype(lies)::value;
             const dim3 grid(tiles_grid(slots, w_tiles)), threads(split_gemm::kThreads);
-            hipLaunchKernelGGL((any_input_gradient_kernel<T, BM, false>), grid, threads, 0, q, between<T>(w.dg),
+            hipLaunchKernelGGL((any_input_gradient_kernel<T, BM, kLies, false>), grid, threads, 0, q, between<T>(w.dg),
                                static_cast<const T*>(m.Wg), w.dx, w.slots, slots, s.width, s.hidden, ld, w_tiles);
-            hipLaunchKernelGGL((any_input_gradient_kernel<T, BM, true>), grid, threads, 0, q, between<T>(w.dv),
+            hipLaunchKernelGGL((any_input_gradient_kernel<T, BM, kLies, true>), grid, threads, 0, q, between<T>(w.dv),
                                static_cast<const T*>(m.Wv), w.dx, w.slots, slots, s.width, s.hidden, ld, w_tiles);
-        }
+        });
     });
     if (d.x) combine<T>(w.dx, positions, offsets, nullptr, 1.0f, d.x, s, q);
     if (d.weights)
@@ -1290,8 +1316,11 @@ int any_backward(const Shape& s, const void* d_out, const void* x, const int64_t
             hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(s.experts * mt * nt)), dim3(split_gemm::kThreads), 0, q, a, b,
                                offsets, static_cast<T*>(c), s.pairs, M, N, lda, ldb, mt, nt);
         };
-        if (side == 64) launch(any_weight_gradient_kernel<T, TA, TB, 64>);
-        else launch(any_weight_gradient_kernel<T, TA, TB, 128>);
+        by_lies(octets<TA>(a, M, lda) && octets<TB>(b, N, ldb), [&](auto lies) {
+            constexpr int kLies = decltype(lies)::value;
+            if (side == 64) launch(any_weight_gradient_kernel<T, TA, TB, 64, kLies, kLies>);
+            else launch(any_weight_gradient_kernel<T, TA, TB, 128, kLies, kLies>);
+        });
     };
     if (d.Wg) product(between<T>(w.dg), xs, d.Wg, s.hidden, s.width, ld, s.width);
     if (d.Wv) product(between<T>(w.dv), xs, d.Wv, s.hidden, s.width, ld, s.width);

@@ -127,6 +127,22 @@ __device__ __forceinline__ void load_octet_strided(Octet<T>& o, const T* __restr
                      static_cast<uint32_t>(__builtin_bit_cast(uint16_t, e[2 * i + 1])) << 16;
     }
 }
+// Eight columns of K row k of an operand that lies across K: the row starts at p + k ld, 16
+// bytes aligned. Past K the last row, which clear_row clears.
+template <typename T>
+__device__ __forceinline__ void load_octet_across(Octet<T>& o, const T* __restrict__ p, int64_t ld, int64_t k, int64_t K) {
+    const uint4* q = reinterpret_cast<const uint4*>(p + min(k, K - 1) * ld);
+#pragma unroll
+    for (int i = 0; i < Octet<T>::kWords / 4; ++i) {
+        const uint4 v = q[i];
+        o.w[i * 4] = v.x, o.w[i * 4 + 1] = v.y, o.w[i * 4 + 2] = v.z, o.w[i * 4 + 3] = v.w;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void clear_row(Octet<T>& o, int64_t k, int64_t K) {
+#pragma unroll
+    for (int i = 0; i < Octet<T>::kWords; ++i) o.w[i] = k >= K ? 0u : o.w[i];
+}
 template <typename T>
 __device__ __forceinline__ void clear_past(Octet<T>& o, int64_t k, int64_t K) {
     constexpr int kPerWord = 4 / static_cast<int>(sizeof(T));
@@ -182,21 +198,29 @@ __device__ __noinline__ float scalar_dot(const TA* a, const TB* b, int64_t K, fl
     return start;
 }
 
+// How an operand lies in memory relative to K.
+constexpr int kAlong = 0, kStrided = 1, kAcross = 2;
+
 // A block tile of BM rows of A by BN rows of B, K in steps of BK through one LDS
 // buffer; the next step's operands are loaded into registers before this step's
 // products and split on their way into LDS. BK = 64 where neither operand is
 // split (eight MFMAs a wave and step otherwise), else 32. An LDS row is BK
 // 16-bit values of one plane; 16-byte group g of row r sits at group
 // g ^ swizzle(r), so that the sixteen rows read by sixteen consecutive lanes
-// fill 256 distinct bytes of banks. A_STRIDED / B_STRIDED: the operand is stored
-// K-major ([K, rows]); its octets are gathered by eight loads, each coalesced
-// over the rows of consecutive lanes.
+// fill 256 distinct bytes of banks. A_LIES / B_LIES: along K (kAlong); stored K-major ([K,
+// rows]), its octets gathered by eight loads, each coalesced over the rows of
+// consecutive lanes (kStrided); or K-major with 16-byte aligned rows and a multiple of
+// eight columns (kAcross): octets of eight columns are loaded and staged as they lie, and
+// fragments read transposed (ds_read_b64_tr_b16: the rows of four lanes each to sixteen
+// lanes). An LDS row is then one K value of the tile's columns, whose 32-byte unit u sits at
+// u ^ unit_swizzle, so that the rows that 32 lanes read lie in distinct banks (fp16 [5100,
+// 2000] x [2000, 768] with two planes an operand: 120 us strided, 100 us across).
 // DEPTH: K steps whose operands are on their way in registers; more than one where
 // a launch has too few tiles to hide the loads behind other workgroups. Split
 // operands then also start a new sum every DEPTH steps (kFold): for so few tiles
 // the library splits K over workgroups, and its shorter sums err less ([168, 512]
 // gates: 2.45e-7 from float64 with its product, 3.25e-7 in one sum, 2.16e-7 so).
-template <typename TA, typename TB, int BM, int BN, bool A_STRIDED = false, bool B_STRIDED = false, int DEPTH = 1>
+template <typename TA, typename TB, int BM, int BN, int A_LIES = kAlong, int B_LIES = kAlong, int DEPTH = 1>
 struct Tile {
     static constexpr int NA = planes<TA, TB>(), NB = planes<TB, TA>();
     static constexpr bool kNative = NA == 1 && NB == 1;
@@ -218,16 +242,66 @@ struct Tile {
 
     f32x16 acc[MT][NT];
 
-    // Octet i of the thread, of an operand of R rows: its row and K group. Eight
-    // or four consecutive threads share a row of a K-contiguous operand (its
-    // 16-byte pieces), consecutive threads take consecutive rows of a strided one.
-    template <int R, bool STRIDED>
+    // Octet i of the thread, of an operand of R rows: its row and K group (across K: its first
+    // column and its K value). Eight or four consecutive threads share a row of a
+    // K-contiguous operand (its 16-byte pieces), consecutive threads take consecutive rows of
+    // a strided one and consecutive octets of one across K.
+    template <int R, int LIES>
     __device__ static int octet_row(int i, int tid = threadIdx.x) {
-        return STRIDED ? (tid + i * kThreads) % R : (tid + i * kThreads) / kGroups;
+        if (LIES == kAcross) return (tid + i * kThreads) % (R / 8) * 8;
+        return LIES == kStrided ? (tid + i * kThreads) % R : (tid + i * kThreads) / kGroups;
     }
-    template <int R, bool STRIDED>
+    template <int R, int LIES>
     __device__ static int octet_group(int i, int tid = threadIdx.x) {
-        return STRIDED ? (tid + i * kThreads) / R : tid % kGroups;
+        if (LIES == kAcross) return (tid + i * kThreads) / (R / 8);
+        return LIES == kStrided ? (tid + i * kThreads) / R : tid % kGroups;
+    }
+    // The first K value of octet i relative to its step, its place in a plane, its load and what clears it past K.
+    template <int R, int LIES>
+    __device__ static int octet_k(int i, int tid = threadIdx.x) {
+        return octet_group<R, LIES>(i, tid) * (LIES == kAcross ? 1 : 8);
+    }
+    template <int R>
+    __device__ static int unit_swizzle(int k) {
+        return R == 128 ? 2 * (k & 3) + ((k & 3) >> 1) : k & 2;
+    }
+    template <int R, int LIES>
+    __device__ static int octet_at(int i, int tid = threadIdx.x) {
+        const int r = octet_row<R, LIES>(i, tid), g = octet_group<R, LIES>(i, tid);
+        if constexpr (LIES == kAcross) return g * (R * 2) + ((r / 16 ^ unit_swizzle<R>(g)) << 5) + (r & 8) * 2;
+        else return at(r, g);
+    }
+    template <int BYTES, int LIES, typename T>
+    __device__ static __forceinline__ void load_octet_of(Octet<T>& o, const T* p, int64_t ld, int64_t k, int64_t K, bool tail) {
+        if constexpr (LIES == kAcross) load_octet_across(o, p, ld, k, K);
+        else if constexpr (LIES == kStrided) load_octet_strided(o, p, ld, k, K, tail);
+        else load_octet<BYTES>(o, p, k, K);
+    }
+    template <int LIES, typename T>
+    __device__ static __forceinline__ void clear_octet(Octet<T>& o, int64_t k, int64_t K) {
+        if constexpr (LIES == kAcross) clear_row(o, k, K);
+        else clear_past(o, k, K);
+    }
+    // The fragment of K group kk of the 32 rows from `first` on of a plane of R rows.
+    template <int R, int LIES>
+    __device__ static __forceinline__ uint4 fragment(const char* plane, int first, int kk) {
+        const int lane = lane_id();
+        if constexpr (LIES == kAcross) {
+            static_assert(R == 64 || R == 128, "columns of a tile");
+            typedef short s16x4 __attribute__((ext_vector_type(4)));
+            typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+            const int k = 16 * kk + 8 * (lane >> 5) + ((lane & 15) >> 2), unit = first / 16 + ((lane >> 4) & 1);
+            const char* p = plane + k * (R * 2) + ((unit ^ unit_swizzle<R>(k)) << 5) + (lane & 3) * 8;
+            union {
+                s16x4 half[2];
+                uint4 whole;
+            } u;
+            u.half[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p));
+            u.half[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 4 * (R * 2)));
+            return u.whole;
+        } else {
+            return *reinterpret_cast<const uint4*>(plane + at(first + (lane & 31), kk * 2 + (lane >> 5)));
+        }
     }
 
     // a_row(r), b_row(r): pointers to row r of the block tile's operands, for
@@ -246,56 +320,47 @@ struct Tile {
         const TA* ap[OA];
         const TB* bp[OB];
 #pragma unroll
-        for (int i = 0; i < OA; ++i) ap[i] = a_row(octet_row<BM, A_STRIDED>(i));
+        for (int i = 0; i < OA; ++i) ap[i] = a_row(octet_row<BM, A_LIES>(i));
 #pragma unroll
-        for (int i = 0; i < OB; ++i) bp[i] = b_row(octet_row<BN, B_STRIDED>(i));
+        for (int i = 0; i < OB; ++i) bp[i] = b_row(octet_row<BN, B_LIES>(i));
         clear(acc);
         char* const lds_b = lds + NA * BM * kRowBytes;
         Octet<TA> a_ring[DEPTH][OA];
         Octet<TB> b_ring[DEPTH][OB];
         auto load = [&](int64_t k0, Octet<TA> (&ao)[OA], Octet<TB> (&bo)[OB]) {
 #pragma unroll
-            for (int i = 0; i < OA; ++i) {
-                const int64_t k = k0 + octet_group<BM, A_STRIDED>(i) * 8;
-                if constexpr (A_STRIDED) load_octet_strided(ao[i], ap[i], a_ld, k, KA, k0 + BK > KA);
-                else load_octet<A_BYTES>(ao[i], ap[i], k, KA);
-            }
+            for (int i = 0; i < OA; ++i)
+                load_octet_of<A_BYTES, A_LIES>(ao[i], ap[i], a_ld, k0 + octet_k<BM, A_LIES>(i), KA, k0 + BK > KA);
 #pragma unroll
-            for (int i = 0; i < OB; ++i) {
-                const int64_t k = k0 + octet_group<BN, B_STRIDED>(i) * 8;
-                if constexpr (B_STRIDED) load_octet_strided(bo[i], bp[i], b_ld, k, KB, k0 + BK > KB);
-                else load_octet<B_BYTES>(bo[i], bp[i], k, KB);
-            }
+            for (int i = 0; i < OB; ++i)
+                load_octet_of<B_BYTES, B_LIES>(bo[i], bp[i], b_ld, k0 + octet_k<BN, B_LIES>(i), KB, k0 + BK > KB);
         };
         auto step = [&](int64_t k0, Octet<TA> (&ao)[OA], Octet<TB> (&bo)[OB]) {
             lds_barrier();  // every wave is done with the previous step's planes
             if (k0 + BK > KA || k0 + BK > KB) {  // only the last step reaches past K
 #pragma unroll
-                for (int i = 0; i < OA; ++i) clear_past(ao[i], k0 + octet_group<BM, A_STRIDED>(i) * 8, KA);
+                for (int i = 0; i < OA; ++i) clear_octet<A_LIES>(ao[i], k0 + octet_k<BM, A_LIES>(i), KA);
 #pragma unroll
-                for (int i = 0; i < OB; ++i) clear_past(bo[i], k0 + octet_group<BN, B_STRIDED>(i) * 8, KB);
+                for (int i = 0; i < OB; ++i) clear_octet<B_LIES>(bo[i], k0 + octet_k<BN, B_LIES>(i), KB);
             }
-            stage<TA, NA, OA, BM, A_STRIDED>(lds, ao);
-            stage<TB, NB, OB, BN, B_STRIDED>(lds_b, bo);
+            stage<TA, NA, OA, BM, A_LIES>(lds, ao);
+            stage<TB, NB, OB, BN, B_LIES>(lds_b, bo);
             if (k0 + DEPTH * BK < k_end) load(k0 + DEPTH * BK, ao, bo);
             lds_barrier();
             // the fragments of K group kk + 1 are read under the products of group kk
             // where two sets fit the registers (one product each)
             uint4 af[kSets][NA][MT], bf[kSets][NB][NT];
             auto read = [&](int kk, int set) {
-                const int fg = kk * 2 + (lane >> 5);
 #pragma unroll
                 for (int p = 0; p < NA; ++p)
 #pragma unroll
                     for (int t = 0; t < MT; ++t)
-                        af[set][p][t] = *reinterpret_cast<const uint4*>(
-                            lds + p * BM * kRowBytes + at(wm * (BM / 2) + t * 32 + (lane & 31), fg));
+                        af[set][p][t] = fragment<BM, A_LIES>(lds + p * BM * kRowBytes, wm * (BM / 2) + t * 32, kk);
 #pragma unroll
                 for (int p = 0; p < NB; ++p)
 #pragma unroll
                     for (int t = 0; t < NT; ++t)
-                        bf[set][p][t] = *reinterpret_cast<const uint4*>(lds_b + p * BN * kRowBytes +
-                                                                       at(b_first(t) + (lane & 31), fg));
+                        bf[set][p][t] = fragment<BN, B_LIES>(lds_b + p * BN * kRowBytes, b_first(t), kk);
             };
             read(0, 0);
 #pragma unroll
@@ -383,21 +448,19 @@ struct Tile {
                 asm volatile("" : "+v"(tid));
                 for (int64_t k0 = k_begin; k0 < k_end; k0 += BK) {
                     lds_barrier();  // every wave is done with the previous step's classes
-                    class_step<A_BYTES, BM, OA, A_STRIDED>(lds, tid, k0, KA, a_ld, a_row);
-                    class_step<B_BYTES, BN, OB, B_STRIDED>(lds_b, tid, k0, KB, b_ld, b_row);
+                    class_step<A_BYTES, BM, OA, A_LIES>(lds, tid, k0, KA, a_ld, a_row);
+                    class_step<B_BYTES, BN, OB, B_LIES>(lds_b, tid, k0, KB, b_ld, b_row);
                     lds_barrier();
 #pragma unroll
-                    for (int kk = 0; kk < BK / 16; ++kk) {
-                        const int fg = kk * 2 + (lane >> 5);
+                    for (int kk = 0; kk < BK / 16; ++kk)
 #pragma unroll
                         for (int i = 0; i < MT; ++i)
 #pragma unroll
                             for (int j = 0; j < NT; ++j)
                                 acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                                    *reinterpret_cast<const bf16x8*>(lds_b + at(b_first(j) + (lane & 31), fg)),
-                                    *reinterpret_cast<const bf16x8*>(lds + at(wm * (BM / 2) + i * 32 + (lane & 31), fg)),
+                                    __builtin_bit_cast(bf16x8, fragment<BN, B_LIES>(lds_b, b_first(j), kk)),
+                                    __builtin_bit_cast(bf16x8, fragment<BM, A_LIES>(lds, wm * (BM / 2) + i * 32, kk)),
                                     acc[i][j], 0, 0, 0);
-                    }
                 }
                 // a NaN of finite operands (infinities of both signs, planes past bf16's range):
                 // the caller's
@@ -416,21 +479,17 @@ struct Tile {
 
   private:
     // One operand's classes of the K step at k0 into LDS.
-    template <int BYTES, int R, int O, bool STRIDED, typename Row>
+    template <int BYTES, int R, int O, int LIES, typename Row>
     __device__ static __forceinline__ void class_step(char* lds, int tid, int64_t k0, int64_t K, int64_t ld, Row row) {
         using T = std::remove_const_t<std::remove_pointer_t<decltype(row(0))>>;
         Octet<T> o[O];
 #pragma unroll
-        for (int i = 0; i < O; ++i) {
-            const int64_t k = k0 + octet_group<R, STRIDED>(i, tid) * 8;
-            if constexpr (STRIDED) load_octet_strided(o[i], row(octet_row<R, STRIDED>(i, tid)), ld, k, K, k0 + BK > K);
-            else load_octet<BYTES>(o[i], row(octet_row<R, STRIDED>(i, tid)), k, K);
-        }
+        for (int i = 0; i < O; ++i)
+            load_octet_of<BYTES, LIES>(o[i], row(octet_row<R, LIES>(i, tid)), ld, k0 + octet_k<R, LIES>(i, tid), K, k0 + BK > K);
 #pragma unroll
         for (int i = 0; i < O; ++i) {
-            clear_past(o[i], k0 + octet_group<R, STRIDED>(i, tid) * 8, K);
-            *reinterpret_cast<uint4*>(lds + at(octet_row<R, STRIDED>(i, tid), octet_group<R, STRIDED>(i, tid))) =
-                classes(o[i]);
+            clear_octet<LIES>(o[i], k0 + octet_k<R, LIES>(i, tid), K);
+            *reinterpret_cast<uint4*>(lds + octet_at<R, LIES>(i, tid)) = classes(o[i]);
         }
     }
 
@@ -441,11 +500,11 @@ struct Tile {
             for (int j = 0; j < NT; ++j) a[i][j] = f32x16{};
     }
 
-    template <typename T, int P, int O, int R, bool STRIDED>
+    template <typename T, int P, int O, int R, int LIES>
     __device__ static __forceinline__ void stage(char* lds, Octet<T> (&o)[O]) {
 #pragma unroll
         for (int i = 0; i < O; ++i) {
-            const int off = at(octet_row<R, STRIDED>(i), octet_group<R, STRIDED>(i));
+            const int off = octet_at<R, LIES>(i);
             if constexpr (P == 1) {
                 *reinterpret_cast<uint4*>(lds + off) = make_uint4(o[i].w[0], o[i].w[1], o[i].w[2], o[i].w[3]);
             } else {

@@ -33,7 +33,7 @@ constexpr int kRows = 64;  // rows of a head tile
 constexpr int kWide = 256, kNarrow = 64;
 
 template <typename T, int BN>
-using HeadTile = split_gemm::Tile<T, T, kRows, BN, false, false, BN == kNarrow ? 4 : 1>;
+using HeadTile = split_gemm::Tile<T, T, kRows, BN, split_gemm::kAlong, split_gemm::kAlong, BN == kNarrow ? 4 : 1>;
 // fp32 rows of 128 to 255 wide tiles gain from the narrow ones ([8192, 1024], vocabulary
 // 256, with gradients: 208 and 163 us), 16-bit ones only lose a launch.
 inline int head_columns(int64_t rows, int64_t V, bool fp32) {
@@ -378,7 +378,7 @@ __global__ __launch_bounds__(kThreads, 2) void surprise_head_grad_prior_kernel(
     const float* __restrict__ G, const T* __restrict__ weight, Out* __restrict__ grad_prior, int64_t rows, int64_t D,
     int64_t V, int64_t d_tiles, int64_t tiles, int64_t chunk_v, int vec_out) {
     constexpr int BM = B, BN = B;
-    using Tile = split_gemm::Tile<float, T, BM, BN, false, true, B == 64 ? 4 : 1>;
+    using Tile = split_gemm::Tile<float, T, BM, BN, split_gemm::kAlong, split_gemm::kStrided, B == 64 ? 4 : 1>;
     constexpr int J = Tile::NT < 2 ? 1 : 2;
     constexpr int kRegion = split_gemm::store_bytes<Out, J>();
     __shared__ __attribute__((aligned(16))) char lds[Tile::kLdsBytes > 4 * kRegion ? Tile::kLdsBytes : 4 * kRegion];
@@ -424,7 +424,7 @@ __global__ __launch_bounds__(kThreads, 2) void surprise_head_grad_weight_kernel(
     const float* __restrict__ G, const T* __restrict__ prior, Out* __restrict__ partial, int64_t rows, int64_t D,
     int64_t V, int64_t d_tiles, int64_t v_tiles, int64_t chunk_rows, int vec_out) {
     constexpr int BM = 128, BN = 128;
-    using Tile = split_gemm::Tile<float, T, BM, BN, true, true>;
+    using Tile = split_gemm::Tile<float, T, BM, BN, split_gemm::kStrided, split_gemm::kStrided>;
     __shared__ __attribute__((aligned(16))) char lds[Tile::kLdsBytes];
     const int64_t chunk = blockIdx.x / (d_tiles * v_tiles), tile_id = blockIdx.x % (d_tiles * v_tiles);
     const int64_t v0 = tile_id / d_tiles * BM, d0 = tile_id % d_tiles * BN;

@@ -154,6 +154,20 @@ def test_outputs_and_gradients(shape, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(9, 8, 16, 3, 2), (150, 200, 136, 2, 2), (600, 72, 328, 2, 2)])
+def test_rows_of_whole_octets_and_weights_behind_an_offset(shape, dtype):
+    """Weights read eight values at a time, and from an address that does not allow it."""
+    case, d_out = draw(*shape, dtype, sum(shape))
+    check(case, d_out)
+    moved = dict(case)
+    for name in ("gate_weights", "value_weights", "output_weights"):
+        flat = torch.empty(case[name].numel() + 1, device="cuda", dtype=dtype)
+        moved[name] = flat[1:].view(case[name].shape).copy_(case[name])
+    check(moved, d_out)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("width,hidden", [(64, 128), (50, 90)])
 def test_one_expert_takes_all_and_equal_shares(width, hidden, dtype):
@@ -216,7 +230,7 @@ def test_each_gradient_alone(width, hidden):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype,width,hidden", [(torch.float32, 50, 90), (torch.float16, 64, 128), (torch.bfloat16, 50, 90),
-                                                (torch.bfloat16, 64, 128)])
+                                                (torch.bfloat16, 64, 128), (torch.float32, 72, 88), (torch.float16, 200, 136)])
 def test_non_finite_values_stay_where_they_belong(dtype, width, hidden):
     case, d_out = draw(90, width, hidden, 3, 1, dtype, 10)
     case["valid"][:] = True
