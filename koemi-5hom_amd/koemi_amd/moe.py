@@ -293,10 +293,10 @@ class _BalanceLoss(torch.autograd.Function):
     @once_differentiable
     def backward(context, d_loss: Tensor):  # type: ignore[override]
         counts, valid = context.saved_tensors
-        d_mass = torch.empty_like(counts)
+        d_mass, d_loss = torch.empty_like(counts), d_loss.contiguous()
         with _native.device_guard(counts.device):
             _native.call("koemi_moe_router_balance_loss_backward", counts.data_ptr(), valid.data_ptr(),
-                         d_loss.contiguous().data_ptr(), counts.numel(), d_mass.data_ptr(),
+                         d_loss.data_ptr(), counts.numel(), d_mass.data_ptr(),
                          _native.stream_of(counts.device))
         return d_mass, None, None
 
@@ -713,6 +713,9 @@ def permute_indices(assignments: Tensor, valid_mask: Tensor, *, expert_count: in
     _require_library()
     device = assignments.device
     pairs = tokens * top_k
+    # named, so that a copy's memory is not given to the next one before the launch
+    ids, mask = assignments.contiguous(), valid_mask.contiguous()
+    weights = pair_weights.contiguous() if pair_weights is not None else None
     sorted_rows = torch.empty((pairs,), device=device, dtype=torch.int64)
     sorted_experts = torch.empty((pairs,), device=device, dtype=torch.int64)
     segment_offsets = torch.empty((expert_count + 1,), device=device, dtype=torch.int64)
@@ -721,9 +724,8 @@ def permute_indices(assignments: Tensor, valid_mask: Tensor, *, expert_count: in
     need = _native.query("koemi_moe_permute_workspace_bytes", tokens, top_k, expert_count)
     workspace = torch.empty((need,), device=device, dtype=torch.uint8)
     with _native.device_guard(device):
-        _native.call("koemi_moe_permute_indices", assignments.contiguous().data_ptr(),
-                     _native.dtype_code(assignments.dtype), valid_mask.contiguous().data_ptr(),
-                     _native.ptr(pair_weights.contiguous() if pair_weights is not None else None),
+        _native.call("koemi_moe_permute_indices", ids.data_ptr(), _native.dtype_code(ids.dtype), mask.data_ptr(),
+                     _native.ptr(weights),
                      sorted_rows.data_ptr(), sorted_experts.data_ptr(), segment_offsets.data_ptr(),
                      _native.ptr(sorted_weights), pair_positions.data_ptr(), tokens, top_k, expert_count,
                      workspace.data_ptr(), need, _native.stream_of(device))
@@ -748,6 +750,7 @@ def permute_hash_indices(token_ids: Tensor, previous_token_ids: Tensor, valid_ma
     _require_library()
     device = ids.device
     pairs = tokens * top_k
+    ids, prev, mask = ids.contiguous(), prev.contiguous(), valid_mask.reshape(-1).contiguous()
     sorted_rows = torch.empty((pairs,), device=device, dtype=torch.int64)
     sorted_experts = torch.empty((pairs,), device=device, dtype=torch.int64)
     segment_offsets = torch.empty((expert_count + 1,), device=device, dtype=torch.int64)
@@ -755,8 +758,8 @@ def permute_hash_indices(token_ids: Tensor, previous_token_ids: Tensor, valid_ma
     need = _native.query("koemi_moe_permute_workspace_bytes", tokens, top_k, expert_count)
     workspace = torch.empty((need,), device=device, dtype=torch.uint8)
     with _native.device_guard(device):
-        _native.call("koemi_moe_permute_hash_indices", ids.contiguous().data_ptr(), prev.contiguous().data_ptr(),
-                     _native.dtype_code(ids.dtype), valid_mask.reshape(-1).contiguous().data_ptr(),
+        _native.call("koemi_moe_permute_hash_indices", ids.data_ptr(), prev.data_ptr(),
+                     _native.dtype_code(ids.dtype), mask.data_ptr(),
                      sorted_rows.data_ptr(), sorted_experts.data_ptr(), segment_offsets.data_ptr(),
                      pair_positions.data_ptr(), tokens, top_k, expert_count, workspace.data_ptr(), need,
                      _native.stream_of(device))

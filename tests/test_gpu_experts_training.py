@@ -216,6 +216,25 @@ def test_layouts(width, hidden):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [5, 16, 32, 64, 200])
+def test_sorting_strided_ids_and_masks(tokens):
+    """Each strided argument's copy lives until the sort has read it."""
+    case, _ = draw(tokens, 64, 64, 6, 2, torch.bfloat16, tokens)
+    ids, weights, valid = case["assignments"], case["pair_weights"], case["valid"]
+    want = moe.permute_indices(ids, valid, expert_count=6, pair_weights=weights)
+    strided = [torch.stack([t, t], dim=-1)[..., 0] for t in (ids, valid, weights)]
+    got = moe.permute_indices(strided[0], strided[1], expert_count=6, pair_weights=strided[2])
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    tokens_now, before = ids[:, 0].abs(), ids[:, 1].abs()
+    want = moe.permute_hash_indices(tokens_now.contiguous(), before.contiguous(), valid, expert_count=6, top_k=2)
+    got = moe.permute_hash_indices(tokens_now[:, None].expand(-1, 2).contiguous()[:, 0],
+                                   before[:, None].expand(-1, 2).contiguous()[:, 0], strided[1], expert_count=6, top_k=2)
+    for a, b in zip(got[:3] + got[4:], want[:3] + want[4:]):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("width,hidden", [(64, 128), (50, 90)])
 def test_each_gradient_alone(width, hidden):
     case, d_out = draw(150, width, hidden, 4, 2, torch.bfloat16, 9)
