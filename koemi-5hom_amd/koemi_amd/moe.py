@@ -1037,15 +1037,16 @@ def expert_mixture(
             raise CudaMoeValidationError("valid MoE assignments must be -1 or in [0, expert_count)")
         if duplicate and top_k >= 2:
             raise CudaMoeValidationError("expert_mixture received duplicate experts for a valid token")
-    return _ExpertMixture.apply(context, pair_weights, assignments, valid_mask, *params.values())
+    floating = (context, pair_weights, *params.values())
+    trained = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in floating)
+    return _ExpertMixture.apply(context, pair_weights, assignments, valid_mask, trained, *params.values())
 
 
 class _ExpertMixture(torch.autograd.Function):
     @staticmethod
     def forward(context, x: Tensor, pair_weights: Tensor | None, assignments: Tensor, valid_mask: Tensor,  # type: ignore[override]
-                *params: Tensor) -> Tensor:
+                trained: bool, *params: Tensor) -> Tensor:
         (experts, hidden, width), top_k = params[0].shape, int(assignments.shape[-1])
-        trained = any(context.needs_input_grad)
         flat = _aligned(x.reshape(-1, width).contiguous())
         tokens, device, code = flat.shape[0], x.device, _native.dtype_code(x.dtype)
         out = torch.empty(x.shape, device=device, dtype=x.dtype)
@@ -1081,7 +1082,7 @@ class _ExpertMixture(torch.autograd.Function):
         if context.shape is None:  # no tokens
             x, weights, *params = context.saved_tensors
             grads = [torch.zeros_like(t) if t is not None and want else None
-                     for t, want in zip((x, weights, None, None, *params), wanted)]
+                     for t, want in zip((x, weights, None, None, None, *params), wanted)]
             return tuple(grads)
         x, rows, pair_experts, offsets, positions, sorted_weights, gate, value, output, output_bias, saved = context.saved_tensors
         tokens, top_k, width, hidden, experts, _ = context.shape
@@ -1095,7 +1096,7 @@ class _ExpertMixture(torch.autograd.Function):
         d_weights = room(wanted[1], context.like[1], torch.float32)
         matrix, wide, narrow = (experts, hidden, width), (experts, hidden), (experts, width)
         d_params = [room(want, shape) for want, shape in
-                    zip(wanted[4:], (matrix, wide, matrix, wide, (experts, width, hidden), narrow))]
+                    zip(wanted[5:], (matrix, wide, matrix, wide, (experts, width, hidden), narrow))]
         need = _size("koemi_moe_experts_workspace_bytes", *context.shape, 1)
         workspace = torch.empty((need,), device=device, dtype=torch.uint8)
         with _native.device_guard(device):
@@ -1104,7 +1105,7 @@ class _ExpertMixture(torch.autograd.Function):
                          gate.data_ptr(), value.data_ptr(), output.data_ptr(), output_bias.data_ptr(), saved.data_ptr(),
                          _native.ptr(d_x), _native.ptr(d_weights), *(_native.ptr(p) for p in d_params), *context.shape,
                          workspace.data_ptr(), need, _native.stream_of(device))
-        return d_x, d_weights, None, None, *d_params
+        return d_x, d_weights, None, None, None, *d_params
 
 
 class _MoeExtension:

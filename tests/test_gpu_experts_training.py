@@ -235,6 +235,25 @@ def test_sorting_strided_ids_and_masks(tokens):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,width,hidden", [(torch.bfloat16, 256, 512), (torch.float32, 100, 300)])
+def test_nothing_is_kept_without_gradients(dtype, width, hidden):
+    """Parameters that require gradients cost an evaluation no more memory than plain tensors do."""
+    case, _ = draw(300, width, hidden, 4, 2, dtype, 31)
+    trained, _, _ = leaves_of(case)
+    peaks = []
+    for which in (case, trained):
+        with torch.no_grad():
+            call(which)
+            torch.cuda.synchronize()
+            torch.cuda.reset_peak_memory_stats()
+            start = torch.cuda.memory_allocated()
+            y = call(which)
+            peaks.append(torch.cuda.max_memory_allocated() - start)
+            del y
+    assert peaks[0] == peaks[1]
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("width,hidden", [(64, 128), (50, 90)])
 def test_each_gradient_alone(width, hidden):
     case, d_out = draw(150, width, hidden, 4, 2, torch.bfloat16, 9)
