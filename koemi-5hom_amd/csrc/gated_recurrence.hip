@@ -550,8 +550,9 @@ int check_sequence(const char* what, const void* z, int64_t z_batch, int64_t z_r
     if (length > 1 && z_row < 2 * width) return fail(KOEMI_ERR_INVALID, "%s: pre-activation rows overlap", what);
     const __int128 cells = static_cast<__int128>(batch) * width * (length + 1) * 8;
     if (cells > (static_cast<__int128>(1) << 60)) return fail(KOEMI_ERR_INVALID, "%s: too many elements", what);
-    if (static_cast<__int128>(batch) * width > (int64_t(1) << 30))
-        return fail(KOEMI_ERR_UNSUPPORTED, "%s: batch x width above 2^30", what);
+    // a launch has fewer than 2^32 threads: 2^23 workgroups, strips of 64 columns or more where many fill the chip
+    if (static_cast<__int128>(batch) * ((width + 63) / 64) > (int64_t(1) << 23) - 8)
+        return fail(KOEMI_ERR_UNSUPPORTED, "%s: more than 2^23 strips of 64 columns", what);
     // offsets inside a chunk of four lane groups of kKeep rows have 32 bits
     const int64_t row = std::max<int64_t>(length > 1 ? z_row : 0, 2 * width);
     if (row > (int64_t(1) << 32) / (4 * kKeep * 4) - 1)

@@ -1180,12 +1180,13 @@ int check_shape(const char* what, const Shape& s) {
     if (!float_dtype(s.dtype)) return fail(KOEMI_ERR_UNSUPPORTED, "%s: unsupported dtype %s", what, dtype_name(s.dtype));
     if (s.tokens < 0 || s.width < 1 || s.hidden < 1 || s.experts < 1 || s.top_k < 1)
         return fail(KOEMI_ERR_INVALID, "%s: bad dimension", what);
-    const int64_t most = int64_t(1) << 31;
-    if (s.tokens >= most || s.top_k > 256 || s.pairs >= most || s.width >= (1 << 24) || s.hidden >= (1 << 24) ||
-        s.experts >= (1 << 20) ||
-        most_slots(s) * ceil_div(std::max(s.width, s.hidden), 64) >= most ||
-        s.experts * ceil_div(s.width, 64) * ceil_div(s.hidden, 64) >= most ||
-        s.tokens * ceil_div(s.width, 4) >= (int64_t(1) << 38))
+    if (s.tokens >= (int64_t(1) << 26) || s.top_k > 256 || s.pairs >= (int64_t(1) << 26) || s.width >= (1 << 22) ||
+        s.hidden >= (1 << 22) || s.experts >= (1 << 16))
+        return fail(KOEMI_ERR_UNSUPPORTED, "%s: shape too large", what);
+    // a launch has fewer than 2^32 threads along a dimension: 2^24 workgroups of 256
+    const int64_t most = (int64_t(1) << 24) - 8, most_columns = ceil_div(std::max(s.width, s.hidden), 64);
+    if (most_slots(s) * most_columns > most || 3 * s.experts * ceil_div(s.width, 64) * ceil_div(s.hidden, 64) > most ||
+        s.tokens * ceil_div(s.width, 4) >= (int64_t(1) << 32) - 256)
         return fail(KOEMI_ERR_UNSUPPORTED, "%s: shape too large", what);
     return KOEMI_OK;
 }

@@ -1025,8 +1025,11 @@ def expert_mixture(
     if top_k > experts:
         raise CudaMoeValidationError("top_k must not exceed expert_count")
     tokens = valid_mask.numel()
-    if tokens * top_k >= 1 << 31 or max(width, hidden) >= 1 << 24:
-        raise CudaMoeValidationError("tokens x top_k must be below 2^31, width and hidden below 2^24")
+    if tokens * top_k >= 1 << 26 or max(width, hidden) >= 1 << 22:
+        raise CudaMoeValidationError("tokens x top_k must be below 2^26, width and hidden below 2^22")
+    if tokens * -(-width // 4) >= (1 << 32) - 256 or \
+            3 * experts * -(-width // 64) * -(-hidden // 64) > (1 << 24) - 8:
+        raise CudaMoeValidationError("tokens x width must be below 2^34 and the parameters' 64 x 64 blocks below 2^22 each")
     _require_library()
     if validate and tokens:
         flat, mask = assignments.reshape(-1, top_k).contiguous(), valid_mask.reshape(-1)

@@ -409,8 +409,8 @@ def gated_recurrence(preactivations: Tensor, valid_mask: Tensor | None = None,
     if initial is not None and (not isinstance(initial, Tensor) or initial.shape != (batch, width)
                                 or initial.dtype != torch.float32 or initial.device != device):
         raise DenseCudaValidationError("initial must be a float32 [batch, width] tensor on the same device")
-    if batch * width > 1 << 30 or width >= 1 << 20:
-        raise DenseCudaValidationError("width must be below 2^20 and batch x width at most 2^30")
+    if batch * -(-width // 64) > (1 << 23) - 8 or width >= 1 << 20:
+        raise DenseCudaValidationError("width must be below 2^20 and batch x width at most 2^29")
     try:
         _native.load_library()
     except _native.NativeLibraryUnavailableError as error:

@@ -13,7 +13,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from koemi_amd import moe
+from koemi_amd import _native, moe
 
 U = 2.0 ** -24
 HALF_STEP = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
@@ -388,3 +388,19 @@ def test_refusals():
         args[i] = bad
         with pytest.raises(moe.CudaMoeValidationError):
             moe.expert_mixture(*args)
+    many = list(good)  # nothing is allocated for shapes past what a launch takes
+    many[:4] = good[0][:1].expand(1 << 25, 8), good[1][:1].expand(1 << 25, 2), good[2][:1].expand(1 << 25, 2), good[3][:1].expand(1 << 25)
+    with pytest.raises(moe.CudaMoeValidationError, match="2\\^26"):
+        moe.expert_mixture(*many)
+    wide = [t(1, 1).expand(1 << 19, 1 << 15), good[1][:1].expand(1 << 19, 2), None, good[3][:1].expand(1 << 19), t(4, 6, 1).expand(4, 6, 1 << 15),
+            good[5], t(4, 6, 1).expand(4, 6, 1 << 15), good[7], t(4, 1, 6).expand(4, 1 << 15, 6), t(4, 1).expand(4, 1 << 15)]
+    with pytest.raises(moe.CudaMoeValidationError, match="2\\^34"):
+        moe.expert_mixture(*wide)
+
+
+@pytest.mark.parametrize("shape", [(1 << 26, 1, 64, 64, 4), (1 << 20, 2, 1 << 16, 64, 4), (4, 257, 64, 64, 512), (8, 2, 1 << 22, 64, 4),
+                                   (8, 2, 1 << 17, 1 << 17, 4), (-1, 2, 64, 64, 4), (8, 0, 64, 64, 4), (8, 2, 64, 64, 0)])
+def test_sizes_past_a_launch_are_refused(shape):
+    for name, last in (("koemi_moe_experts_saved_bytes", ()), ("koemi_moe_experts_workspace_bytes", (1,))):
+        assert _native.query(name, *shape, _native.dtype_code(torch.bfloat16), *last) == 0
+        assert _native.query(name, 1000, 2, 64, 128, 4, _native.dtype_code(torch.bfloat16), *last) > 0

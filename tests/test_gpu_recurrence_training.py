@@ -330,3 +330,5 @@ def test_refusals_on_the_gpu():
     for initial in (h0.half(), h0[:1], h0.cpu(), h0.reshape(-1), 0.0):
         with pytest.raises(DenseCudaValidationError):
             recurrent.gated_recurrence(z, ok, initial)
+    with pytest.raises(DenseCudaValidationError, match="2\\^29"):
+        recurrent.gated_recurrence(z[:1, :1, :2].expand(1 << 23, 1, 2))
