@@ -275,7 +275,7 @@ def test_captured_replayed_and_on_another_stream():
 
     def step():
         out = recurrent.gated_recurrence(z, valid, h0)
-        return (*out, *torch.autograd.grad(out, (z, h0), (d_states, d_final)))
+        return [t.detach() for t in (*out, *torch.autograd.grad(out, (z, h0), (d_states, d_final)))]
 
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
