@@ -24,10 +24,9 @@
 // and a chunk starts from there. That saves the read of h, and the gradients see the
 // fp32 states, not states rounded to 16 bits.
 //
-// Strips are as wide as still fill the chip; where even narrow ones do not (few
-// long rows), the sequence is cut into parts that run at once: a first launch
-// folds each part but the last (first, for the gradients) into its map, and each
-// part's workgroup composes the maps before it (after it).
+// Where even narrow strips do not fill the chip (few long rows), the sequence is cut into
+// parts that run at once: a first launch folds each part but the last (first, for the
+// gradients) into its map, and each part's workgroup composes the maps before it (after it).
 #include "common.hpp"
 
 #include <algorithm>
@@ -218,9 +217,119 @@ __device__ __forceinline__ void scan_groups(float& p, float& q, float& xp, float
 // The state before every kKeep-th position lies at kept[(b * rows + t / kKeep) * width + f].
 __device__ __forceinline__ int64_t kept_rows(int64_t length) { return (length + kKeep - 1) / kKeep; }
 
-// Forward. FOLD: only the map of each part but the last, into maps[2, batch, parts,
-// width] (p, then q); else the states from the initial state through the maps before.
-template <typename T, int VEC, int LPC, bool FOLD>
+// x through `count` parts' maps, the first at maps[cell], the next `step` after it: eight
+// parts' loads are under way at once ([1, 32768, 512] fp32, 32 parts, one by one: forward 51
+// us, backward 81; so 43 and 78).
+template <int VEC>
+__device__ __forceinline__ void through_maps(float (&x)[VEC], const float* __restrict__ maps, int64_t cells, int64_t cell,
+                                             int64_t step, int64_t count) {
+    constexpr int kAhead = 8;
+    for (int64_t j = 0; j < count; j += kAhead) {
+        Pack<float, VEC> p[kAhead], q[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int64_t at = cell + min(j + i, count - 1) * step;
+            p[i] = *reinterpret_cast<const Pack<float, VEC>*>(maps + at);
+            q[i] = *reinterpret_cast<const Pack<float, VEC>*>(maps + cells + at);
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) x[v] = j + i < count ? fmaf(p[i].e[v], x[v], q[i].e[v]) : x[v];
+    }
+}
+
+// Each part's map but the last's (REVERSE: the adjoint's, x -> a (d + x) from the last step to
+// the first, but the first's) into maps[2, batch, parts, width] (p, then q). A wave folds an
+// eighth of the part by itself and the waves' maps meet once, at the end. [1, 32768, 512]
+// fp32, 134 MB either way: 37 us (43 in chunks of the workgroup; half of it the gates) and
+// 24; loads two or three blocks ahead 39 to 45 and no faster.
+template <typename T, int VEC, int LPC, bool REVERSE>
+__global__ __launch_bounds__(kThreads) void recurrence_fold_kernel(Sequence s, const T* __restrict__ d_states,
+                                                                   float* __restrict__ maps) {
+    using P = Place<VEC, LPC>;
+    constexpr int kBlock = kSteps * LPC;
+    __shared__ float wave_p[kWaves][P::kColumns], wave_q[kWaves][P::kColumns];
+    P at;
+    if (!at.place(s)) return;
+    if (at.part == (REVERSE ? 0 : s.parts - 1)) return;
+    at.segment = static_cast<uint32_t>(at.group * kSteps);
+    const int64_t share = s.part_steps / kWaves, begin = at.part * s.part_steps + at.wave * share;
+    const int64_t end = min(s.length, begin + share), blocks = max((end - begin + kBlock - 1) / kBlock, int64_t(0));
+    const T* zr = static_cast<const T*>(s.z) + at.b * s.z_batch;
+    const T* other = REVERSE ? d_states ? d_states + at.b * s.length * s.width : nullptr : zr + s.width;
+    const int64_t other_row = REVERSE ? s.width : s.z_row;
+    const uint8_t* valid = s.valid ? s.valid + at.b * s.length : nullptr;
+    struct Raw {
+        Pack<T, VEC> r[kSteps], o[kSteps];
+        Valid<P> valid;
+    } raw;
+    auto fetch = [&](int64_t i) {  // block i in the order of the fold; none past the last: an identity
+        const int64_t t0 = i < blocks ? begin + (REVERSE ? blocks - 1 - i : i) * kBlock : -1;
+        Rows<T, VEC, P>(zr, s.z_row, t0, end, at).load(raw.r);
+        Rows<T, VEC, P>(other, other_row, t0, end, at).load(raw.o);
+        raw.valid.load(valid, t0, end, at);
+    };
+    float whole_p[VEC], whole_q[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) whole_p[v] = 1.0f, whole_q[v] = 0.0f;
+    fetch(0);
+    for (int64_t i = 0; i < blocks; ++i) {
+        float p[VEC], q[VEC], xp[VEC], xq[VEC];
+        const uint32_t mask = raw.valid.mask(valid, at);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) p[v] = 1.0f, q[v] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+            const int step = REVERSE ? kSteps - 1 - k : k;
+            const uint32_t bits = lane_bits(mask, step);
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                const float r = to_f32(raw.r[step].e[v]), o = to_f32(raw.o[step].e[v]);
+                if constexpr (REVERSE) {
+                    const float a = or_one(retention_of(r), bits);
+                    q[v] = a * (o + q[v]);
+                    p[v] *= a;
+                } else {
+                    const Gates g = gates_of<false>(r, o);
+                    const float a = or_one(g.a, bits);
+                    q[v] = fmaf(a, q[v], or_zero(g.k * g.u, bits));
+                    p[v] *= a;
+                }
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);  // as in the walks: the next loads run under the rest
+        fetch(i + 1);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            scan_groups<LPC, REVERSE>(p[v], q[v], xp[v], xq[v], at.group);
+            whole_q[v] = fmaf(p[v], whole_q[v], q[v]);  // right in the last group (REVERSE: the first)
+            whole_p[v] *= p[v];
+        }
+    }
+    if (at.group == (REVERSE ? 0 : LPC - 1))
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) wave_p[at.wave][at.lane * VEC + v] = whole_p[v], wave_q[at.wave][at.lane * VEC + v] = whole_q[v];
+    __syncthreads();
+    if (!at.inside || at.wave != 0 || at.group != 0) return;
+    const int64_t cell = (at.b * s.parts + at.part) * s.width + at.f, cells = s.batch * s.parts * s.width;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+        float p = 1.0f, q = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kWaves; ++k) {
+            const int w = REVERSE ? kWaves - 1 - k : k;
+            const float wp = wave_p[w][at.lane * VEC + v];
+            q = fmaf(wp, q, wave_q[w][at.lane * VEC + v]);
+            p *= wp;
+        }
+        maps[cell + v] = p;
+        maps[cells + cell + v] = q;
+    }
+}
+
+// Forward, each part from the initial state through the maps before it.
+template <typename T, int VEC, int LPC>
 __global__ __launch_bounds__(kThreads) void recurrence_forward_kernel(Sequence s, const float* __restrict__ initial,
                                                                       T* __restrict__ states, float* __restrict__ final_state,
                                                                       float* __restrict__ kept, float* __restrict__ maps) {
@@ -228,23 +337,14 @@ __global__ __launch_bounds__(kThreads) void recurrence_forward_kernel(Sequence s
     __shared__ float wave_p[2][kWaves][P::kColumns], wave_q[2][kWaves][P::kColumns];
     P at;
     if (!at.place(s)) return;
-    if (FOLD && at.part == s.parts - 1) return;
     const int64_t begin = at.part * s.part_steps, end = min(s.length, begin + s.part_steps);
     const T* zr = static_cast<const T*>(s.z) + at.b * s.z_batch;
     const T* zc = zr + s.width;
     const uint8_t* valid = s.valid ? s.valid + at.b * s.length : nullptr;
     const int64_t cells = s.batch * s.parts * s.width;
-    float carry[VEC], prod[VEC];
+    float carry[VEC];
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-        carry[v] = FOLD || !initial || !at.inside ? 0.0f : initial[at.b * s.width + at.f + v];
-        prod[v] = 1.0f;
-        if constexpr (!FOLD)
-            for (int64_t j = 0; j < at.part; ++j) {
-                const int64_t cell = (at.b * s.parts + j) * s.width + at.f + v;
-                carry[v] = fmaf(maps[cell], carry[v], maps[cells + cell]);
-            }
-    }
+    for (int v = 0; v < VEC; ++v) carry[v] = !initial || !at.inside ? 0.0f : initial[at.b * s.width + at.f + v];
     struct Raw {
         Pack<T, VEC> r[kSteps], c[kSteps];
         Valid<P> valid;
@@ -257,6 +357,7 @@ __global__ __launch_bounds__(kThreads) void recurrence_forward_kernel(Sequence s
     int turn = 0;
     Raw raw;
     if (begin < end) fetch(begin, raw);
+    through_maps<VEC>(carry, maps, cells, at.b * s.parts * s.width + at.f, s.width, at.part);
     for (int64_t t0 = begin; t0 < end; t0 += P::kChunk) {
         float a[kSteps][VEC], b[kSteps][VEC], p[VEC], q[VEC], xp[VEC], xq[VEC];
         const uint32_t mask = raw.valid.mask(valid, at);
@@ -294,52 +395,40 @@ __global__ __launch_bounds__(kThreads) void recurrence_forward_kernel(Sequence s
 #pragma unroll
             for (int w = 0; w < kWaves; ++w) {
                 if (w == at.wave) in[v] = x;
-                const float wp = wave_p[turn][w][at.lane * VEC + v];
-                x = fmaf(wp, x, wave_q[turn][w][at.lane * VEC + v]);
-                if constexpr (FOLD) prod[v] *= wp;
+                x = fmaf(wave_p[turn][w][at.lane * VEC + v], x, wave_q[turn][w][at.lane * VEC + v]);
             }
             carry[v] = x;
             in[v] = fmaf(xp[v], in[v], xq[v]);
         }
         turn ^= 1;
-        if constexpr (!FOLD) {
-            if (!at.inside) continue;
-            const int64_t t = t0 + at.segment;
-            if (kept && t % kKeep == 0 && t < end) {
-                Pack<float, VEC> k;
+        if (!at.inside) continue;
+        const int64_t t = t0 + at.segment;
+        if (kept && t % kKeep == 0 && t < end) {
+            Pack<float, VEC> k;
 #pragma unroll
-                for (int v = 0; v < VEC; ++v) k.e[v] = in[v];
-                *reinterpret_cast<Pack<float, VEC>*>(kept + (at.b * kept_rows(s.length) + t / kKeep) * s.width + at.f) = k;
+            for (int v = 0; v < VEC; ++v) k.e[v] = in[v];
+            *reinterpret_cast<Pack<float, VEC>*>(kept + (at.b * kept_rows(s.length) + t / kKeep) * s.width + at.f) = k;
+        }
+        const Rows<T, VEC, P> out(states + at.b * s.length * s.width, s.width, t0, end, at);
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            Pack<T, VEC> h;
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                in[v] = fmaf(a[i][v], in[v], b[i][v]);
+                h.e[v] = from_f32<T>(in[v]);
             }
-            const Rows<T, VEC, P> out(states + at.b * s.length * s.width, s.width, t0, end, at);
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
-                Pack<T, VEC> h;
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) {
-                    in[v] = fmaf(a[i][v], in[v], b[i][v]);
-                    h.e[v] = from_f32<T>(in[v]);
-                }
-                out.store(i, h);
-            }
+            out.store(i, h);
         }
     }
-    if (!at.inside || at.wave != 0 || at.group != 0) return;
+    if (!at.inside || at.wave != 0 || at.group != 0 || at.part != s.parts - 1) return;
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-        if constexpr (FOLD) {
-            const int64_t cell = (at.b * s.parts + at.part) * s.width + at.f + v;
-            maps[cell] = prod[v];
-            maps[cells + cell] = carry[v];
-        } else if (at.part == s.parts - 1) {
-            final_state[at.b * s.width + at.f + v] = carry[v];
-        }
-    }
+    for (int v = 0; v < VEC; ++v) final_state[at.b * s.width + at.f + v] = carry[v];
 }
 
-// Backward, from the last chunk to the first. The carry is a_{t+1} g_{t+1}. FOLD:
-// only the map of each part but the first.
-template <typename T, int VEC, int LPC, bool FOLD>
+// Backward, from the last chunk to the first, through the maps of the parts after. The carry
+// is a_{t+1} g_{t+1}.
+template <typename T, int VEC, int LPC>
 __global__ __launch_bounds__(kThreads) void recurrence_backward_kernel(
     Sequence s, const float* __restrict__ kept, const T* __restrict__ d_states, const float* __restrict__ d_final,
     T* __restrict__ d_z, float* __restrict__ d_initial, float* __restrict__ maps) {
@@ -347,24 +436,15 @@ __global__ __launch_bounds__(kThreads) void recurrence_backward_kernel(
     __shared__ float wave_p[2][kWaves][P::kColumns], wave_q[2][kWaves][P::kColumns], wave_h[2][kWaves][P::kColumns];
     P at;
     if (!at.place(s)) return;
-    if (FOLD && at.part == 0) return;
     const int64_t begin = at.part * s.part_steps, end = min(s.length, begin + s.part_steps);
     const T* zr = static_cast<const T*>(s.z) + at.b * s.z_batch;
     const T* zc = zr + s.width;
     const T* up = d_states ? d_states + at.b * s.length * s.width : nullptr;
     const uint8_t* valid = s.valid ? s.valid + at.b * s.length : nullptr;
     const int64_t cells = s.batch * s.parts * s.width;
-    float carry[VEC], prod[VEC];
+    float carry[VEC];
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-        carry[v] = FOLD || !d_final || !at.inside ? 0.0f : d_final[at.b * s.width + at.f + v];
-        prod[v] = 1.0f;
-        if constexpr (!FOLD)
-            for (int64_t j = s.parts - 1; j > at.part; --j) {
-                const int64_t cell = (at.b * s.parts + j) * s.width + at.f + v;
-                carry[v] = fmaf(maps[cell], carry[v], maps[cells + cell]);
-            }
-    }
+    for (int v = 0; v < VEC; ++v) carry[v] = !d_final || !at.inside ? 0.0f : d_final[at.b * s.width + at.f + v];
     struct Raw {
         Pack<T, VEC> r[kSteps], c[kSteps], d[kSteps];
         Pack<float, VEC> h;
@@ -373,22 +453,20 @@ __global__ __launch_bounds__(kThreads) void recurrence_backward_kernel(
     auto fetch = [&](int64_t t0, Raw& o) {
         Rows<T, VEC, P>(zr, s.z_row, t0, end, at).load(o.r);
         Rows<T, VEC, P>(up, s.width, t0, end, at).load(o.d);
-        if constexpr (!FOLD) {
-            Rows<T, VEC, P>(zc, s.z_row, t0, end, at).load(o.c);
-            const int64_t row = at.b * kept_rows(s.length) + max(t0, int64_t(0)) / kKeep;
-            o.h = *reinterpret_cast<const Pack<float, VEC>*>(kept + row * s.width + at.f);
-        }
+        Rows<T, VEC, P>(zc, s.z_row, t0, end, at).load(o.c);
+        const int64_t row = at.b * kept_rows(s.length) + max(t0, int64_t(0)) / kKeep;
+        o.h = *reinterpret_cast<const Pack<float, VEC>*>(kept + row * s.width + at.f);
         o.valid.load(valid, t0, end, at);
     };
     int turn = 0;
     Raw raw;
     const int64_t last = begin + (end - begin - 1) / P::kChunk * P::kChunk;
     if (begin < end) fetch(last, raw);
+    through_maps<VEC>(carry, maps, cells, ((at.b + 1) * s.parts - 1) * s.width + at.f, -s.width, s.parts - 1 - at.part);
     for (int64_t t0 = last; begin < end && t0 >= begin; t0 -= P::kChunk) {
         // x: an element's increment, then the state before it; cr, cc: what g times
         // (h_{t-1} - u) and g are multiplied by for dr and dc
-        constexpr int kFull = FOLD ? 1 : kSteps;
-        float a[kSteps][VEC], d[kSteps][VEC], x[kFull][VEC], u[kFull][VEC], cr[kFull][VEC], cc[kFull][VEC];
+        float a[kSteps][VEC], d[kSteps][VEC], x[kSteps][VEC], u[kSteps][VEC], cr[kSteps][VEC], cc[kSteps][VEC];
         float p[VEC], q[VEC], fp[VEC], fq[VEC], xp[VEC], xq[VEC], yp[VEC], yq[VEC];
         const uint32_t mask = raw.valid.mask(valid, at);
 #pragma unroll
@@ -398,25 +476,20 @@ __global__ __launch_bounds__(kThreads) void recurrence_backward_kernel(
             const uint32_t bits = lane_bits(mask, i);
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
-                if constexpr (FOLD) {
-                    a[i][v] = or_one(retention_of(to_f32(raw.r[i].e[v])), bits);
-                } else {
-                    const Gates g = gates_of<true>(to_f32(raw.r[i].e[v]), to_f32(raw.c[i].e[v]));
-                    a[i][v] = or_one(g.a, bits);
-                    x[i][v] = or_zero(g.k * g.u, bits);
-                    u[i][v] = g.u;
-                    cr[i][v] = kGateRetentionSpan * g.ds;
-                    cc[i][v] = g.k * g.du;
-                    fq[v] = fmaf(a[i][v], fq[v], x[i][v]);
-                }
+                const Gates g = gates_of<true>(to_f32(raw.r[i].e[v]), to_f32(raw.c[i].e[v]));
+                a[i][v] = or_one(g.a, bits);
+                x[i][v] = or_zero(g.k * g.u, bits);
+                u[i][v] = g.u;
+                cr[i][v] = kGateRetentionSpan * g.ds;
+                cc[i][v] = g.k * g.du;
+                fq[v] = fmaf(a[i][v], fq[v], x[i][v]);
                 p[v] *= a[i][v];
                 d[i][v] = to_f32(raw.d[i].e[v]);
             }
         }
         float start[VEC];
-        if constexpr (!FOLD)
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) start[v] = raw.h.e[v];
+        for (int v = 0; v < VEC; ++v) start[v] = raw.h.e[v];
         // the gates are formed: the next chunk's loads run under the rest, in the same registers
         __builtin_amdgcn_sched_barrier(0);
         fetch(t0 - P::kChunk, raw);
@@ -428,12 +501,12 @@ __global__ __launch_bounds__(kThreads) void recurrence_backward_kernel(
         for (int v = 0; v < VEC; ++v) {
             fp[v] = p[v];
             scan_groups<LPC, true>(p[v], q[v], xp[v], xq[v], at.group);
-            if constexpr (!FOLD) scan_groups<LPC, false>(fp[v], fq[v], yp[v], yq[v], at.group);
+            scan_groups<LPC, false>(fp[v], fq[v], yp[v], yq[v], at.group);
             if (at.group == 0) {
                 wave_p[turn][at.wave][at.lane * VEC + v] = p[v];
                 wave_q[turn][at.wave][at.lane * VEC + v] = q[v];
             }
-            if (!FOLD && at.group == LPC - 1) wave_h[turn][at.wave][at.lane * VEC + v] = fq[v];
+            if (at.group == LPC - 1) wave_h[turn][at.wave][at.lane * VEC + v] = fq[v];
         }
         __syncthreads();  // the other buffer's readers are past it: they have written this one
         float in[VEC], h[VEC];
@@ -441,7 +514,7 @@ __global__ __launch_bounds__(kThreads) void recurrence_backward_kernel(
         for (int v = 0; v < VEC; ++v) {
             float c = carry[v];
             in[v] = c;
-            float y = FOLD ? 0.0f : start[v];
+            float y = start[v];
             h[v] = y;
             float wp[kWaves];
 #pragma unroll
@@ -449,83 +522,92 @@ __global__ __launch_bounds__(kThreads) void recurrence_backward_kernel(
                 if (w == at.wave) in[v] = c;
                 wp[w] = wave_p[turn][w][at.lane * VEC + v];
                 c = fmaf(wp[w], c, wave_q[turn][w][at.lane * VEC + v]);
-                if constexpr (FOLD) prod[v] *= wp[w];
             }
             carry[v] = c;
-            if constexpr (!FOLD) {
 #pragma unroll
-                for (int w = 0; w < kWaves - 1; ++w) {
-                    y = fmaf(wp[w], y, wave_h[turn][w][at.lane * VEC + v]);
-                    if (w + 1 == at.wave) h[v] = y;
-                }
-                in[v] = fmaf(xp[v], in[v], xq[v]);
-                h[v] = fmaf(yp[v], h[v], yq[v]);
+            for (int w = 0; w < kWaves - 1; ++w) {
+                y = fmaf(wp[w], y, wave_h[turn][w][at.lane * VEC + v]);
+                if (w + 1 == at.wave) h[v] = y;
             }
+            in[v] = fmaf(xp[v], in[v], xq[v]);
+            h[v] = fmaf(yp[v], h[v], yq[v]);
         }
         turn ^= 1;
-        if constexpr (!FOLD) {
-            if (!at.inside) continue;
+        if (!at.inside) continue;
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i)
+        for (int i = 0; i < kSteps; ++i)
 #pragma unroll
-                for (int v = 0; v < VEC; ++v) {
-                    const float next = fmaf(a[i][v], h[v], x[i][v]);
-                    x[i][v] = h[v];
-                    h[v] = next;
-                }
-            T* out = d_z + at.b * s.length * 2 * s.width;
-            const Rows<T, VEC, P> out_r(out, 2 * s.width, t0, end, at), out_c(out + s.width, 2 * s.width, t0, end, at);
-#pragma unroll
-            for (int i = kSteps - 1; i >= 0; --i) {
-                Pack<T, VEC> dr, dc;
-                const uint32_t bits = lane_bits(mask, i);
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) {
-                    const float g = d[i][v] + in[v];
-                    in[v] = a[i][v] * g;
-                    dr.e[v] = from_f32<T>(or_zero(g * (x[i][v] - u[i][v]) * cr[i][v], bits));
-                    dc.e[v] = from_f32<T>(or_zero(g * cc[i][v], bits));
-                }
-                out_r.store(i, dr);
-                out_c.store(i, dc);
+            for (int v = 0; v < VEC; ++v) {
+                const float next = fmaf(a[i][v], h[v], x[i][v]);
+                x[i][v] = h[v];
+                h[v] = next;
             }
-        }
-    }
-    if (!at.inside || at.wave != 0 || at.group != 0) return;
+        T* out = d_z + at.b * s.length * 2 * s.width;
+        const Rows<T, VEC, P> out_r(out, 2 * s.width, t0, end, at), out_c(out + s.width, 2 * s.width, t0, end, at);
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-        if constexpr (FOLD) {
-            const int64_t cell = (at.b * s.parts + at.part) * s.width + at.f + v;
-            maps[cell] = prod[v];
-            maps[cells + cell] = carry[v];
-        } else if (at.part == 0 && d_initial) {
-            d_initial[at.b * s.width + at.f + v] = carry[v];
+        for (int i = kSteps - 1; i >= 0; --i) {
+            Pack<T, VEC> dr, dc;
+            const uint32_t bits = lane_bits(mask, i);
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                const float g = d[i][v] + in[v];
+                in[v] = a[i][v] * g;
+                dr.e[v] = from_f32<T>(or_zero(g * (x[i][v] - u[i][v]) * cr[i][v], bits));
+                dc.e[v] = from_f32<T>(or_zero(g * cc[i][v], bits));
+            }
+            out_r.store(i, dr);
+            out_c.store(i, dc);
         }
     }
+    if (!at.inside || at.wave != 0 || at.group != 0 || at.part != 0 || !d_initial) return;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) d_initial[at.b * s.width + at.f + v] = carry[v];
 }
 
-// How a call is laid out: two columns a lane where rows allow it, the widest strip
-// that still gives two workgroups a CU, and parts where the narrowest does not.
+// How a call is laid out: two columns a lane where rows allow it, strips that leave a CU the
+// least work, and parts where they leave most of the chip idle.
 struct Plan {
     int vec, lpc;
     int64_t strips, parts, part_steps;
 };
-constexpr int64_t kFill = 512;  // workgroups that keep 256 CUs loaded
+// whole: workgroups that run at once on 256 CUs. The registers let two of the forward's share
+// a CU and one of the backward's (bf16 [16, 2048, 1024] backward: 82 us as 256, 92 as 512).
+// parts: from how many on they pay for the fold (bf16 [4, 2048, 1024] in two: forward 12 + 16 us
+// against 26, backward 8 + 23 against 38). They fill the chip once: more only hand on more maps
+// (bf16 [1, 32768, 512] backward: 43 us in 32 parts of eight strips, 55 in 64).
+struct Fill {
+    int64_t whole, parts;
+};
+constexpr Fill kForwardFill{512, 3}, kBackwardFill{256, 2};
+constexpr int64_t kPartFill = 256;
 
-inline Plan plan_of(int64_t batch, int64_t length, int64_t width, int vec) {
+inline Plan plan_of(int64_t batch, int64_t length, int64_t width, int vec, int size, Fill fill) {
     Plan p;
     p.vec = vec;
-    for (p.lpc = 1;; p.lpc *= 2) {
-        const int64_t columns = kWave / p.lpc * vec;
-        p.strips = (width + columns - 1) / columns;
-        if (batch * p.strips >= kFill || p.lpc == 4) break;
+    auto strips_of = [&](int lpc) {
+        const int64_t columns = kWave / lpc * vec;
+        return (width + columns - 1) / columns;
+    };
+    int64_t least = 0;
+    for (int lpc = 1; lpc <= 4; lpc *= 2) {  // rounds of the chip times columns
+        const int64_t cost = (batch * strips_of(lpc) + fill.whole - 1) / fill.whole * (kWave / lpc);
+        if (lpc == 1 || cost < least) p.lpc = lpc, least = cost;
+    }
+    p.strips = strips_of(p.lpc);
+    p.parts = 1;
+    if (batch * p.strips * fill.parts <= kPartFill) {
+        // where parts fill the chip all the same, a strip's row has a cache line's 128 bytes
+        // ([1, 32768, 512] fp32 backward: 80 us and 31 for the maps with 64 bytes, 63 and 24)
+        const int whole = vec * size / 2;
+        if (batch * strips_of(whole) * std::min<int64_t>(kMaxParts, length / (kKeep * whole) / 4) >= kPartFill / 2) {
+            p.lpc = whole;
+            p.strips = strips_of(whole);
+        }
+        const int64_t chunks = (length + kKeep * p.lpc - 1) / (kKeep * p.lpc);
+        if (chunks >= 8) p.parts = std::min<int64_t>(std::min<int64_t>(kMaxParts, chunks / 4), kPartFill / (batch * p.strips));
     }
     const int64_t chunk = static_cast<int64_t>(kKeep) * p.lpc, chunks = (length + chunk - 1) / chunk;
-    p.parts = 1;
-    if (batch * p.strips < kFill / 2 && chunks >= 8)
-        p.parts = std::min<int64_t>(std::min<int64_t>(kMaxParts, chunks / 4), (kFill + batch * p.strips - 1) / (batch * p.strips));
-    const int64_t per = (chunks + p.parts - 1) / std::max<int64_t>(p.parts, 1);
-    p.part_steps = std::max<int64_t>(per, 1) * chunk;
+    p.part_steps = std::max<int64_t>((chunks + p.parts - 1) / p.parts, 1) * chunk;
     p.parts = std::max<int64_t>((length + p.part_steps - 1) / p.part_steps, 1);
     return p;
 }
@@ -581,9 +663,9 @@ int forward(Sequence s, const Plan& p, const float* initial, void* states, float
     by_plan<2>(p, [&](auto vec, auto lpc) {
         constexpr int V = decltype(vec)::value, C = decltype(lpc)::value;
         if (s.parts > 1)
-            hipLaunchKernelGGL((recurrence_forward_kernel<T, V, C, true>), dim3(grid_of(s)), dim3(kThreads), 0, stream, s,
-                               initial, static_cast<T*>(states), final_state, kept, maps);
-        hipLaunchKernelGGL((recurrence_forward_kernel<T, V, C, false>), dim3(grid_of(s)), dim3(kThreads), 0, stream, s,
+            hipLaunchKernelGGL((recurrence_fold_kernel<T, V, C, false>), dim3(grid_of(s)), dim3(kThreads), 0, stream, s,
+                               static_cast<const T*>(nullptr), maps);
+        hipLaunchKernelGGL((recurrence_forward_kernel<T, V, C>), dim3(grid_of(s)), dim3(kThreads), 0, stream, s,
                            initial, static_cast<T*>(states), final_state, kept, maps);
     });
     return check_launch("koemi_gated_recurrence_forward");
@@ -594,9 +676,9 @@ int backward(Sequence s, const Plan& p, const float* kept, const void* d_states,
     by_plan<std::is_same<T, float>::value ? 1 : 2>(p, [&](auto vec, auto lpc) {
         constexpr int V = decltype(vec)::value, C = decltype(lpc)::value;
         if (s.parts > 1)
-            hipLaunchKernelGGL((recurrence_backward_kernel<T, V, C, true>), dim3(grid_of(s)), dim3(kThreads), 0, stream, s,
-                               kept, static_cast<const T*>(d_states), d_final, static_cast<T*>(d_z), d_initial, maps);
-        hipLaunchKernelGGL((recurrence_backward_kernel<T, V, C, false>), dim3(grid_of(s)), dim3(kThreads), 0, stream, s,
+            hipLaunchKernelGGL((recurrence_fold_kernel<T, V, C, true>), dim3(grid_of(s)), dim3(kThreads), 0, stream, s,
+                               static_cast<const T*>(d_states), maps);
+        hipLaunchKernelGGL((recurrence_backward_kernel<T, V, C>), dim3(grid_of(s)), dim3(kThreads), 0, stream, s,
                            kept, static_cast<const T*>(d_states), d_final, static_cast<T*>(d_z), d_initial, maps);
     });
     return check_launch("koemi_gated_recurrence_backward");
@@ -613,8 +695,11 @@ extern "C" int64_t koemi_gated_recurrence_kept_rows(int64_t length) {
 
 extern "C" size_t koemi_gated_recurrence_workspace_bytes(int64_t batch, int64_t length, int64_t width) {
     if (batch <= 0 || length <= 0 || width <= 0) return 0;
-    size_t most = 0;  // of either layout: which one a call takes depends on its alignment
-    for (int vec = 1; vec <= 2; ++vec) most = std::max(most, maps_bytes(plan_of(batch, length, width, vec), batch, width));
+    size_t most = 0;  // of every layout: which one a call takes depends on its type and alignment
+    for (int vec = 1; vec <= 2; ++vec)
+        for (int size = 2; size <= 4; size += 2)
+            for (const Fill& fill : {kForwardFill, kBackwardFill})
+                most = std::max(most, maps_bytes(plan_of(batch, length, width, vec, size, fill), batch, width));
     return most;
 }
 
@@ -629,7 +714,7 @@ extern "C" int koemi_gated_recurrence_forward(const void* preactivations, int64_
     if (st != KOEMI_OK || batch == 0 || width == 0) return st;
     if (!final_states || (length > 0 && !states)) return fail(KOEMI_ERR_INVALID, "%s: null output", what);
     const bool pairs = pairs_fit(preactivations, batch_stride, row_stride, width, dtype, states, nullptr, kept);
-    const Plan p = plan_of(batch, length, width, pairs ? 2 : 1);
+    const Plan p = plan_of(batch, length, width, pairs ? 2 : 1, dtype == KOEMI_F32 ? 4 : 2, kForwardFill);
     const size_t need = maps_bytes(p, batch, width);
     if (need && (!workspace || workspace_bytes < need)) return fail(KOEMI_ERR_INVALID, "%s: workspace too small", what);
     const Sequence s{preactivations, batch_stride, row_stride, valid, batch, length, width, p.strips, p.parts, p.part_steps};
@@ -650,10 +735,10 @@ extern "C" int koemi_gated_recurrence_backward(const void* preactivations, int64
     const int st = check_sequence(what, preactivations, batch_stride, row_stride, dtype, batch, length, width);
     if (st != KOEMI_OK || batch == 0 || width == 0) return st;
     if (length > 0 && (!kept || !grad_preactivations)) return fail(KOEMI_ERR_INVALID, "%s: null pointer", what);
-    // fp32 takes one column a lane: two spill ([1, 32768, 512] 101 us against 81; bf16 [8, 2048, 1024] 57 with one, 47 with two)
+    // fp32 takes one column a lane: two spill ([1, 32768, 512] 101 us against 81 in strips as wide; bf16 [8, 2048, 1024] 57 with one, 47 with two)
     const bool pairs = dtype != KOEMI_F32 && pairs_fit(preactivations, batch_stride, row_stride, width, dtype, grad_states,
                                                        grad_preactivations, kept);
-    const Plan p = plan_of(batch, length, width, pairs ? 2 : 1);
+    const Plan p = plan_of(batch, length, width, pairs ? 2 : 1, dtype == KOEMI_F32 ? 4 : 2, kBackwardFill);
     const size_t need = maps_bytes(p, batch, width);
     if (need && (!workspace || workspace_bytes < need)) return fail(KOEMI_ERR_INVALID, "%s: workspace too small", what);
     const Sequence s{preactivations, batch_stride, row_stride, valid, batch, length, width, p.strips, p.parts, p.part_steps};

@@ -144,6 +144,12 @@ def test_states_and_gradients(shape, dtype, mask):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,width", [(torch.float32, 129), (torch.bfloat16, 129), (torch.float16, 258)])
+def test_long_sequences_in_parts(dtype, width):
+    check(*draw((1, 16500, width), dtype, 77, "random"))
+
+
+@pytest.mark.gpu
 def test_lengths_of_zero_and_empty_batches():
     z = torch.empty((3, 0, 8), device="cuda", requires_grad=True)
     h0 = torch.randn((3, 4), device="cuda", requires_grad=True)
