@@ -1035,8 +1035,9 @@ def expert_mixture(
         flat, mask = assignments.reshape(-1, top_k).contiguous(), valid_mask.reshape(-1)
         # a slot of -1 is no expert: it takes one past the catalog of its own, which repeats nothing
         spare = torch.arange(experts, experts + top_k, device=flat.device, dtype=flat.dtype)
-        out_of_range, duplicate = _assignment_flags(torch.where(flat == -1, spare, flat), mask.contiguous(), experts + top_k)
-        if out_of_range or bool(((flat >= experts) & mask[:, None]).any()):
+        named = torch.where(flat == -1, spare, flat.masked_fill(flat >= experts, -2))
+        out_of_range, duplicate = _assignment_flags(named, mask.contiguous(), experts + top_k)
+        if out_of_range:
             raise CudaMoeValidationError("valid MoE assignments must be -1 or in [0, expert_count)")
         if duplicate and top_k >= 2:
             raise CudaMoeValidationError("expert_mixture received duplicate experts for a valid token")

@@ -372,6 +372,20 @@ def test_repeats_and_ids_outside_the_catalog():
     call(case)  # what an invalid token's slots say does not matter
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+@pytest.mark.parametrize("ids", [(3, 3), (7, 2), (2, 4), (5, -1), (-5, 1), (-2, -1)])
+def test_each_bad_choice_is_refused(ids, dtype):
+    case, _ = draw(10, 64, 64, 4, 2, torch.bfloat16, 18)
+    case["valid"][:], case["valid"][1] = True, False
+    case["context"] = torch.nan_to_num(case["context"], nan=1.0)
+    case["assignments"] = torch.tensor([[0, -1], list(ids), [-1, -1]] + [[0, 1]] * 7, device="cuda", dtype=dtype)
+    call(case)
+    case["valid"][1] = True
+    with pytest.raises(moe.CudaMoeValidationError):
+        call(case)
+
+
 def test_refusals_on_the_cpu():
     t = torch.zeros
     args = [t(3, 8), t(3, 2, dtype=torch.int64), t(3, 2), torch.ones(3, dtype=torch.bool), t(4, 6, 8), t(4, 6), t(4, 6, 8), t(4, 6),
