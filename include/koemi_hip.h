@@ -982,7 +982,8 @@ int koemi_moe_router_balance_loss_backward(const float* assignment_counts, const
  * segment_offsets, pair_positions); pair_weights [tokens, top_k] fp32 in token order
  * (NULL: 1 / top_k). Pairs past the valid ones count nothing, a token without any gets
  * zeros. saved (NULL: no gradients wanted) keeps koemi_moe_experts_saved_bytes for the
- * backward. Workspace: koemi_moe_experts_workspace_bytes, no zeroing needed. */
+ * backward. Workspace: koemi_moe_experts_workspace_bytes, no zeroing needed; both 16-byte
+ * aligned. */
 size_t koemi_moe_experts_saved_bytes(int64_t tokens, int64_t top_k, int64_t width, int64_t hidden,
                                      int64_t expert_count, int dtype);
 size_t koemi_moe_experts_workspace_bytes(int64_t tokens, int64_t top_k, int64_t width, int64_t hidden,

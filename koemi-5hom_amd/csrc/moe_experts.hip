@@ -364,22 +364,47 @@ __global__ __launch_bounds__(split_gemm::kThreads, 2) void any_input_gradient_ke
         }
 }
 
-// One expert's C[m, n] = sum over its pairs of A[pair, m] B[pair, n] (rows lda and ldb
-// apart), in type T; zeros for an expert without pairs.
+// Every expert's C[m, n] = sum over its pairs of A[pair, m] B[pair, n] (rows lda and ldb
+// apart), in type T; zeros for an expert without pairs. Up to three products of the same
+// types in one launch, since small ones leave CUs idle (fp32 500 tokens, 201 -> 333: three
+// launches 26 us, one 15; fp16 3000, 768 -> 2000: two 150, one 131).
+template <typename T, typename TA, typename TB>
+struct WeightProducts {
+    struct One {
+        const TA* a;
+        const TB* b;
+        T* c;
+        int64_t M, N, lda, ldb;
+        uint32_t end, n_tiles;  // of an expert's tiles, those of this product and the ones before it
+    } one[3];
+    int count = 0;
+    void add(const TA* a, const TB* b, void* c, int64_t M, int64_t N, int64_t lda, int64_t ldb, int64_t side) {
+        const uint32_t nt = static_cast<uint32_t>(ceil_div(N, side)), mt = static_cast<uint32_t>(ceil_div(M, side));
+        one[count] = {a, b, static_cast<T*>(c), M, N, lda, ldb, tiles() + mt * nt, nt};
+        ++count;
+    }
+    uint32_t tiles() const { return count ? one[count - 1].end : 0; }
+};
 template <typename T, typename TA, typename TB, int BM, int A_LIES, int B_LIES>
 __global__ __launch_bounds__(split_gemm::kThreads, 2) void any_weight_gradient_kernel(
-    const TA* __restrict__ A, const TB* __restrict__ B, const int64_t* __restrict__ offsets, T* __restrict__ C,
-    int64_t pairs, int64_t M, int64_t N, int64_t lda, int64_t ldb, uint32_t m_tiles, uint32_t n_tiles) {
+    WeightProducts<T, TA, TB> products, uint32_t per, const int64_t* __restrict__ offsets, int64_t pairs) {
     using G = split_gemm::Tile<TA, TB, BM, BM, A_LIES, B_LIES, BM == 64 ? 2 : 1>;
     constexpr int kRegion = split_gemm::store_bytes<T, 1>();
     __shared__ __attribute__((aligned(16))) char lds[any_lds<G>(kRegion)];
-    const uint32_t per = m_tiles * n_tiles, e = blockIdx.x / per, within = blockIdx.x % per;
-    const int64_t m0 = static_cast<int64_t>(within / n_tiles) * BM, n0 = static_cast<int64_t>(within % n_tiles) * BM;
+    const uint32_t e = blockIdx.x / per;
+    uint32_t within = blockIdx.x % per;
+    int which = 0;
+    while (which + 1 < products.count && within >= products.one[which].end) ++which;
+    if (which) within -= products.one[which - 1].end;
+    const auto& one = products.one[which];
+    const int64_t M = one.M, N = one.N, lda = one.lda, ldb = one.ldb;
+    T* const C = one.c;
+    const int64_t m0 = static_cast<int64_t>(within / one.n_tiles) * BM, n0 = static_cast<int64_t>(within % one.n_tiles) * BM;
     const int64_t lo = min(max(offsets[e], int64_t(0)), pairs), K = min(max(offsets[e + 1], lo), pairs) - lo;
     const int wave = threadIdx.x / kWave, wm = wave >> 1, wn = wave & 1;
     T* out = C + static_cast<int64_t>(e) * M * N;
-    const TA* a = A + lo * lda;
-    const TB* b = B + lo * ldb;
+    const TA* a = one.a + lo * lda;
+    const TB* b = one.b + lo * ldb;
     G tile;
     uint64_t chains = 0;
     if (K > 0) {
@@ -985,23 +1010,32 @@ __global__ __launch_bounds__(256) void combine_rows_kernel(const float* __restri
 }
 
 // The rows of x and dout that the pairs came from, in sorted order (either NULL: not
-// wanted), and <dout, b_o> of each pair. A wave per pair.
-template <typename T>
+// wanted), and <dout, b_o> of each pair. A wave per pair, a lane VEC columns at a time (fp16
+// 3000 tokens of 768: one 18 us, eight 9).
+template <typename T, int VEC>
 __global__ __launch_bounds__(256) void gather_pairs_kernel(const T* __restrict__ x, const T* __restrict__ d_out,
                                                            const int64_t* __restrict__ rows, const int64_t* __restrict__ offsets,
                                                            int64_t experts, const T* __restrict__ bo,
                                                            const int64_t* __restrict__ pair_experts, T* __restrict__ xs,
                                                            T* __restrict__ ds, float* __restrict__ dot, int64_t pairs,
                                                            int64_t tokens, int64_t width) {
+    struct alignas(sizeof(T) * VEC) Piece {
+        T v[VEC];
+    };
     const int64_t p = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / kWave;
     if (p >= pairs || p >= offsets[experts]) return;
     const int64_t t = min(max(rows[p], int64_t(0)), tokens - 1), e = min(max(pair_experts[p], int64_t(0)), experts - 1);
     float sum = 0.0f;
-    for (int64_t c = lane_id(); c < width; c += kWave) {
-        if (xs) xs[p * width + c] = x[t * width + c];
-        const T d = d_out[t * width + c];
-        if (ds) ds[p * width + c] = d;
-        if (dot) sum = fmaf(to_f32(d), to_f32(bo[e * width + c]), sum);
+    for (int64_t c = lane_id() * VEC; c < width; c += kWave * VEC) {
+        auto piece = [&](const T* from) { return *reinterpret_cast<const Piece*>(from + c); };
+        if (xs) *reinterpret_cast<Piece*>(xs + p * width + c) = piece(x + t * width);
+        const Piece d = piece(d_out + t * width);
+        if (ds) *reinterpret_cast<Piece*>(ds + p * width + c) = d;
+        if (dot) {
+            const Piece b = piece(bo + e * width);
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) sum = fmaf(to_f32(d.v[v]), to_f32(b.v[v]), sum);
+        }
     }
     if (dot) {
         sum = wave_sum_xor(sum);
@@ -1022,8 +1056,14 @@ __global__ __launch_bounds__(256) void weight_gradient_kernel(const float* __res
     if (p >= pairs) return;
     float sum = 0.0f;
     if (p < *valid_end) {
-#pragma unroll 4
-        for (int j = 0; j < parts; ++j) sum += part[j * pairs + p];
+        constexpr int kAhead = 16;  // loads under way at once
+        for (int j = 0; j < parts; j += kAhead) {
+            float v[kAhead];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) v[i] = part[min(j + i, parts - 1) * pairs + p];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) sum += j + i < parts ? v[i] : 0.0f;
+        }
         for (int j = 0; j < dot_parts; ++j) sum += dot[j * pairs + p];
     }
     const int64_t t = min(max(rows[p], int64_t(0)), pairs / top_k - 1);
@@ -1048,6 +1088,7 @@ template <typename TA>
 __device__ __forceinline__ float column_sum(const TA* a, int64_t lda, const float* weights, float share, bool weighted,
                                             int64_t begin, int64_t end) {
     float sum = 0.0f;
+#pragma unroll 8
     for (int64_t r = begin; r < end; r += 4)
         sum = fmaf(weighted ? (weights ? weights[r] : share) : 1.0f, to_f32(a[r * lda]), sum);
     return sum;
@@ -1125,8 +1166,22 @@ struct Carver {
         return o;
     }
 };
-struct ForwardSpace {
+// What the forward keeps: g, v and the slots.
+struct SavedSpace {
+    float* keep;
     Slots slots;
+    size_t bytes;
+};
+inline SavedSpace saved_space(const Shape& s, void* base) {
+    Carver c{static_cast<char*>(base)};
+    SavedSpace w;
+    w.keep = c.take<float>(2 * kept_floats(s));
+    w.slots = c.slots(s);
+    w.bytes = c.used;
+    return w;
+}
+struct ForwardSpace {
+    Slots slots;  // in `saved` where that is given
     float *h, *y;
     size_t bytes;
 };
@@ -1140,7 +1195,7 @@ inline ForwardSpace forward_space(const Shape& s, void* base) {
     return w;
 }
 struct BackwardSpace {
-    Slots slots;
+    Slots slots;  // the forward's, in `saved`
     float *dg, *dv, *wh, *dx, *dw_part, *dot, *sums, *out_sums;
     void *xs, *ds;
     size_t bytes;
@@ -1149,7 +1204,6 @@ inline BackwardSpace backward_space(const Shape& s, void* base) {
     Carver c{static_cast<char*>(base)};
     BackwardSpace w;
     const int64_t ld = padded_hidden(s.hidden), rows = gathered_rows(s);
-    w.slots = c.slots(s);
     if (tile_shape(s)) {  // dg and dv as bf16 side by side, w h bf16
         w.dg = c.take<float>(rows * s.hidden);
         w.dv = nullptr;
@@ -1197,6 +1251,12 @@ template <typename F>
 void by_rows(const Shape& s, F f) {
     if (any_rows(s.pairs, s.experts) == 64) f(std::integral_constant<int, 64>{});
     else f(std::integral_constant<int, 128>{});
+}
+// Whether 16 bytes can be read and written at once from each.
+inline bool aligned16(std::initializer_list<const void*> pointers) {
+    uintptr_t all = 0;
+    for (const void* p : pointers) all |= reinterpret_cast<uintptr_t>(p);
+    return all % 16 == 0;
 }
 // Whether the rows of an operand across K can be read eight columns at once.
 template <typename T>
@@ -1275,12 +1335,17 @@ int any_backward(const Shape& s, const void* d_out, const void* x, const int64_t
     const float share = 1.0f / static_cast<float>(s.top_k);
     const T* dy = static_cast<const T*>(d_out);
     T *xs = static_cast<T*>(w.xs), *ds = static_cast<T*>(w.ds);
-    find_slots(s, offsets, w.slots, q);
     const bool want_in = d.Wg || d.Wv, want_out = d.Wo || d.bo;
-    if (want_in || want_out || d.weights)
-        hipLaunchKernelGGL(gather_pairs_kernel<T>, dim3(grid_for(s.pairs, 4)), dim3(256), 0, q, static_cast<const T*>(x), dy,
-                           rows, offsets, s.experts, static_cast<const T*>(m.bo), pair_experts, want_in ? xs : nullptr,
-                           want_out ? ds : nullptr, d.weights ? w.dot : nullptr, s.pairs, s.tokens, s.width);
+    if (want_in || want_out || d.weights) {
+        auto gather = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3(grid_for(s.pairs, 4)), dim3(256), 0, q, static_cast<const T*>(x), dy, rows, offsets,
+                               s.experts, static_cast<const T*>(m.bo), pair_experts, want_in ? xs : nullptr,
+                               want_out ? ds : nullptr, d.weights ? w.dot : nullptr, s.pairs, s.tokens, s.width);
+        };
+        constexpr int kPiece = 16 / sizeof(T);
+        if (s.width % kPiece == 0 && aligned16({x, d_out, m.bo})) gather(gather_pairs_kernel<T, kPiece>);
+        else gather(gather_pairs_kernel<T, 1>);
+    }
     const uint32_t h_tiles = static_cast<uint32_t>(ceil_div(s.hidden, kGradientCols));
     const uint32_t w_tiles = static_cast<uint32_t>(ceil_div(s.width, kGradientCols));
     by_rows(s, [&](auto rows_tag) {
@@ -1309,23 +1374,33 @@ int any_backward(const Shape& s, const void* d_out, const void* x, const int64_t
                            static_cast<int>(s.top_k));
     // tiles of 64 x 64 where those of 128 x 128 would leave CUs idle
     const int side = s.experts * ceil_div(s.width, 128) * ceil_div(s.hidden, 128) < 256 ? 64 : 128;
-    auto product = [&](auto* a, auto* b, void* c, int64_t M, int64_t N, int64_t lda, int64_t ldb) {
-        using TA = std::remove_pointer_t<decltype(a)>;
-        using TB = std::remove_pointer_t<decltype(b)>;
-        const uint32_t mt = static_cast<uint32_t>(ceil_div(M, side)), nt = static_cast<uint32_t>(ceil_div(N, side));
-        auto launch = [&](auto kernel) {
-            hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(s.experts * mt * nt)), dim3(split_gemm::kThreads), 0, q, a, b,
-                               offsets, static_cast<T*>(c), s.pairs, M, N, lda, ldb, mt, nt);
+    auto multiply = [&](const auto& products) {
+        using P = std::decay_t<decltype(products)>;
+        using TA = std::remove_const_t<std::remove_pointer_t<decltype(products.one[0].a)>>;
+        using TB = std::remove_const_t<std::remove_pointer_t<decltype(products.one[0].b)>>;
+        if (!products.count) return;
+        auto launch = [&](void (*kernel)(P, uint32_t, const int64_t*, int64_t)) {
+            hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(s.experts * products.tiles())), dim3(split_gemm::kThreads), 0, q,
+                               products, products.tiles(), offsets, s.pairs);
         };
-        by_lies(octets<TA>(a, M, lda) && octets<TB>(b, N, ldb), [&](auto lies) {
+        // the workspace's rows are aligned: both widths in whole octets, or none read as such
+        by_lies(s.hidden % 8 == 0 && s.width % 8 == 0, [&](auto lies) {
             constexpr int kLies = decltype(lies)::value;
             if (side == 64) launch(any_weight_gradient_kernel<T, TA, TB, 64, kLies, kLies>);
             else launch(any_weight_gradient_kernel<T, TA, TB, 128, kLies, kLies>);
         });
     };
-    if (d.Wg) product(between<T>(w.dg), xs, d.Wg, s.hidden, s.width, ld, s.width);
-    if (d.Wv) product(between<T>(w.dv), xs, d.Wv, s.hidden, s.width, ld, s.width);
-    if (d.Wo) product(ds, between<T>(w.wh), d.Wo, s.width, s.hidden, s.width, ld);
+    WeightProducts<T, Between<T>, T> in;
+    WeightProducts<T, T, Between<T>> out;
+    if (d.Wg) in.add(between<T>(w.dg), xs, d.Wg, s.hidden, s.width, ld, s.width, side);
+    if (d.Wv) in.add(between<T>(w.dv), xs, d.Wv, s.hidden, s.width, ld, s.width, side);
+    if constexpr (std::is_same<T, float>::value) {
+        if (d.Wo) in.add(ds, w.wh, d.Wo, s.width, s.hidden, s.width, ld, side);
+    } else if (d.Wo) {
+        out.add(ds, between<T>(w.wh), d.Wo, s.width, s.hidden, s.width, ld, side);
+    }
+    multiply(in);
+    if constexpr (!std::is_same<T, float>::value) multiply(out);
     if (d.bg || d.bv || d.bo) {
         const int64_t most = std::max(s.hidden, s.width);
         const ThreeSums sums{{{w.dg, w.sums, d.bg, ld, 2 * s.hidden, s.hidden, 1},
@@ -1366,7 +1441,6 @@ int tile_backward(const Shape& s, const void* d_out, const void* x, const int64_
     bf16 *xs = static_cast<bf16*>(w.xs), *ds = static_cast<bf16*>(w.ds);
     bf16 *dgv = reinterpret_cast<bf16*>(w.dg), *wh = reinterpret_cast<bf16*>(w.wh);
     const dim3 threads(mfma_stage::kThreads);
-    find_slots(s, offsets, w.slots, q);
     const unsigned blocks = static_cast<unsigned>(ceil_div(s.width, kGatherColumns));
     hipLaunchKernelGGL(tile_gather_kernel, dim3(static_cast<unsigned>(padded / kGatherRows), blocks), dim3(256), 0, q,
                        static_cast<const bf16*>(x), static_cast<const bf16*>(d_out), rows, static_cast<const bf16*>(m.bo),
@@ -1401,13 +1475,6 @@ int tile_backward(const Shape& s, const void* d_out, const void* x, const int64_
     return check_launch("koemi_moe_experts_backward(tiles)");
 }
 
-// The tiles' copies take 16 bytes of a row at once.
-inline bool aligned16(std::initializer_list<const void*> pointers) {
-    uintptr_t all = 0;
-    for (const void* p : pointers) all |= reinterpret_cast<uintptr_t>(p);
-    return all % 16 == 0;
-}
-
 }  // namespace
 }  // namespace koemi
 
@@ -1417,7 +1484,7 @@ extern "C" size_t koemi_moe_experts_saved_bytes(int64_t tokens, int64_t top_k, i
                                                 int64_t expert_count, int dtype) {
     const Shape s{tokens * top_k, tokens, width, hidden, expert_count, top_k, dtype};
     if (check_shape("koemi_moe_experts_saved_bytes", s) != KOEMI_OK) return 0;
-    return static_cast<size_t>(2 * kept_floats(s)) * sizeof(float);
+    return saved_space(s, nullptr).bytes;
 }
 
 extern "C" size_t koemi_moe_experts_workspace_bytes(int64_t tokens, int64_t top_k, int64_t width, int64_t hidden,
@@ -1442,12 +1509,18 @@ extern "C" int koemi_moe_experts_forward(const void* context, const int64_t* sor
     if (!context || !sorted_rows || !segment_offsets || !pair_positions || !m.Wg || !m.bg || !m.Wv || !m.bv || !m.Wo ||
         !m.bo || !output)
         return fail(KOEMI_ERR_INVALID, "%s: null pointer", what);
-    const ForwardSpace w = forward_space(s, workspace);
+    ForwardSpace w = forward_space(s, workspace);
     if (!workspace || workspace_bytes < w.bytes) return fail(KOEMI_ERR_INVALID, "%s: workspace too small", what);
-    float* keep = static_cast<float*>(saved);
+    if (!aligned16({saved, workspace})) return fail(KOEMI_ERR_INVALID, "%s: saved and workspace must be 16-byte aligned", what);
+    float* keep = nullptr;
+    if (saved) {
+        const SavedSpace space = saved_space(s, saved);
+        keep = space.keep;
+        w.slots = space.slots;
+    }
     hipStream_t q = as_stream(stream);
     const bool few = !saved && few_rows_mlp_fits(s.pairs, width, hidden, expert_count, dtype);
-    if ((tile_shape(s) || few) && !aligned16({context, m.Wg, m.Wv, m.Wo, saved, workspace}))
+    if ((tile_shape(s) || few) && !aligned16({context, m.Wg, m.Wv, m.Wo}))
         return fail(KOEMI_ERR_INVALID, "%s: operands must be 16-byte aligned", what);
     if (few) {  // a decode step: bound by the weights, read once
         const int rc = few_rows_mlp(context, sorted_rows, tokens, segment_offsets, m.Wg, m.bg, m.Wv, m.bv, m.Wo, m.bo, w.h, w.y,
@@ -1485,12 +1558,15 @@ extern "C" int koemi_moe_experts_backward(const void* grad_output, const void* c
         return fail(KOEMI_ERR_INVALID, "%s: null pointer", what);
     const Gradients d{grad_context,       grad_gate_weights,   grad_gate_biases,   grad_value_weights,
                       grad_value_biases,  grad_output_weights, grad_output_biases, grad_pair_weights};
-    const BackwardSpace w = backward_space(s, workspace);
+    BackwardSpace w = backward_space(s, workspace);
     if (!workspace || workspace_bytes < w.bytes) return fail(KOEMI_ERR_INVALID, "%s: workspace too small", what);
-    const float* keep = static_cast<const float*>(saved);
+    if (!aligned16({saved, workspace})) return fail(KOEMI_ERR_INVALID, "%s: saved and workspace must be 16-byte aligned", what);
+    const SavedSpace space = saved_space(s, const_cast<void*>(saved));  // read alone
+    const float* keep = space.keep;
+    w.slots = space.slots;
     hipStream_t q = as_stream(stream);
     if (tile_shape(s)) {
-        if (!aligned16({grad_output, context, m.Wg, m.Wv, m.Wo, m.bo, saved, workspace, d.Wg, d.Wv, d.Wo}))
+        if (!aligned16({grad_output, context, m.Wg, m.Wv, m.Wo, m.bo, d.Wg, d.Wv, d.Wo}))
             return fail(KOEMI_ERR_INVALID, "%s: operands must be 16-byte aligned", what);
         return tile_backward(s, grad_output, context, sorted_rows, segment_offsets, pair_positions, sorted_weights, m, keep, d, w,
                              q);
