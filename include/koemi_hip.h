@@ -919,7 +919,8 @@ int koemi_herm_combine_norm_fusion(const void* expert_outputs, const int64_t* pa
  * [batch, koemi_gated_recurrence_kept_rows(length), width] fp32 receives the
  * states that the backward starts from. `workspace` holds the maps of a sequence cut
  * into parts (0 bytes where the batch's columns alone fill the chip). What lies in
- * masked positions does not matter, NaN included. */
+ * masked positions does not matter, NaN included. Refused: batch ceil(width / 64)
+ * from 2^23 on, rows of 2^22 elements or more. */
 int64_t koemi_gated_recurrence_kept_rows(int64_t length);
 size_t koemi_gated_recurrence_workspace_bytes(int64_t batch, int64_t length, int64_t width);
 int koemi_gated_recurrence_forward(const void* preactivations, int64_t batch_stride, int64_t row_stride, int dtype,
@@ -983,7 +984,9 @@ int koemi_moe_router_balance_loss_backward(const float* assignment_counts, const
  * (NULL: 1 / top_k). Pairs past the valid ones count nothing, a token without any gets
  * zeros. saved (NULL: no gradients wanted) keeps koemi_moe_experts_saved_bytes for the
  * backward. Workspace: koemi_moe_experts_workspace_bytes, no zeroing needed; both 16-byte
- * aligned. */
+ * aligned. Refused (the queries give 0): 2^26 pairs, 2^34 context values or 2^22 blocks of
+ * 64 x 64 parameters and more. bf16 of widths in multiples of 64 needs 16-byte aligned
+ * operands. */
 size_t koemi_moe_experts_saved_bytes(int64_t tokens, int64_t top_k, int64_t width, int64_t hidden,
                                      int64_t expert_count, int dtype);
 size_t koemi_moe_experts_workspace_bytes(int64_t tokens, int64_t top_k, int64_t width, int64_t hidden,
