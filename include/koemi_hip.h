@@ -910,14 +910,14 @@ int koemi_herm_combine_norm_fusion(const void* expert_outputs, const int64_t* pa
  * BoundedRecurrentState.gates (model/memory.py:14-30), the masking and scan of
  * network.py:306-310, and the gradients that autograd forms through them in the
  * reference. preactivations (F32, F16 or BF16): row (b, t) starts at
- * b batch_stride + t row_stride (elements) and holds u W_r^T + b_r in its first
- * `width` columns and u W_c^T + b_c in the next. a = 2^-8 + (1 - 2^-7) sigmoid,
- * b = (1 - a) tanh, (1, 0) where valid [batch, length] is 0 (NULL: all valid),
- * h_t = a_t h_{t-1} + b_t in fp32 from initial [batch, width] fp32 (NULL:
- * zeros). states [batch, length, width] in the input's type, final_states
- * [batch, width] fp32 (length 0: the initial states). kept (NULL: not wanted)
- * [batch, koemi_gated_recurrence_kept_rows(length), width] fp32 receives the
- * states that the backward starts from. `workspace` holds the maps of a sequence cut
+ * b batch_stride + t row_stride (elements; any row_stride for a length of 1) and
+ * holds u W_r^T + b_r in its first `width` columns and u W_c^T + b_c in the next.
+ * a = 2^-8 + (1 - 2^-7) sigmoid, b = (1 - a) tanh, (1, 0) where valid [batch,
+ * length] is 0 (NULL: all valid), h_t = a_t h_{t-1} + b_t in fp32 from initial
+ * [batch, width] fp32 (NULL: zeros). states [batch, length, width] in the input's
+ * type, final_states [batch, width] fp32 (length 0: the initial states). kept
+ * (NULL: not wanted) [batch, koemi_gated_recurrence_kept_rows(length), width] fp32
+ * receives the states that the backward starts from. `workspace` holds the maps of a sequence cut
  * into parts (0 bytes where the batch's columns alone fill the chip). What lies in
  * masked positions does not matter, NaN included. Refused: batch ceil(width / 64)
  * from 2^23 on, rows of 2^22 elements or more. */

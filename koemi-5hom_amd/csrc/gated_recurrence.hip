@@ -712,6 +712,7 @@ extern "C" int koemi_gated_recurrence_forward(const void* preactivations, int64_
     const char* what = "koemi_gated_recurrence_forward";
     const int st = check_sequence(what, preactivations, batch_stride, row_stride, dtype, batch, length, width);
     if (st != KOEMI_OK || batch == 0 || width == 0) return st;
+    if (length <= 1) row_stride = 2 * width;  // a single row has no next one: Rows takes its size from the stride
     if (!final_states || (length > 0 && !states)) return fail(KOEMI_ERR_INVALID, "%s: null output", what);
     const bool pairs = pairs_fit(preactivations, batch_stride, row_stride, width, dtype, states, nullptr, kept);
     const Plan p = plan_of(batch, length, width, pairs ? 2 : 1, dtype == KOEMI_F32 ? 4 : 2, kForwardFill);
@@ -734,6 +735,7 @@ extern "C" int koemi_gated_recurrence_backward(const void* preactivations, int64
     const char* what = "koemi_gated_recurrence_backward";
     const int st = check_sequence(what, preactivations, batch_stride, row_stride, dtype, batch, length, width);
     if (st != KOEMI_OK || batch == 0 || width == 0) return st;
+    if (length <= 1) row_stride = 2 * width;  // a single row has no next one: Rows takes its size from the stride
     if (length > 0 && (!kept || !grad_preactivations)) return fail(KOEMI_ERR_INVALID, "%s: null pointer", what);
     // fp32 takes one column a lane: two spill ([1, 32768, 512] 101 us against 81 in strips as wide; bf16 [8, 2048, 1024] 57 with one, 47 with two)
     const bool pairs = dtype != KOEMI_F32 && pairs_fit(preactivations, batch_stride, row_stride, width, dtype, grad_states,
