@@ -34,3 +34,51 @@ def test_one_position_of_any_row_stride(layout, width, dtype):
     for got, want in zip(run(other), run(z)):
         assert torch.equal(got, want)
     recurrence_tests.check(other, None, initial, d_states, d_final)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("scale", [0.3, 0.1, 1e-2, 1e-3, 1e-4, 1e-5])
+def test_candidates_next_to_zero_keep_their_precision(scale, dtype):
+    """One position from zero: h = k u, dr = -g u (1 - 2^-7) s (1 - s), dc = g k (1 - u^2), each relative to itself.
+
+    In units of 2^-24 for |r| <= 1: the exponential's argument is rounded (1) and it and the reciprocal are off by 2
+    each, so 1 - s and k by at most 10 with their products and s (1 - s) by 16; tanh takes 8 more (c <= 0.3: a product
+    of its argument and a polynomial within 3, or 1 - 2^(-2 c log2 e) within 8), products and sums 4: 32 units, 2^-19.
+    """
+    batch, width = 64, 96
+    gen = torch.Generator(device="cuda").manual_seed(17)
+    r = torch.rand((batch, 1, width), device="cuda", generator=gen) * 2.0 - 1.0
+    c = (torch.rand((batch, 1, width), device="cuda", generator=gen) * 0.9 + 0.1) * scale
+    z = torch.cat([r, c * torch.sign(r)], dim=-1).to(dtype).requires_grad_()
+    states, final = recurrent.gated_recurrence(z)
+    d_final = torch.randn((batch, width), device="cuda", generator=gen)
+    (d_z,) = torch.autograd.grad(final, z, d_final)
+    z64 = z.detach().double()[:, 0].requires_grad_()
+    s, u = torch.sigmoid(z64[:, :width]), torch.tanh(z64[:, width:])
+    want = (1.0 - (recurrence_tests.MIN_RETENTION + recurrence_tests.SPAN * s)) * u
+    (d_want,) = torch.autograd.grad(want, z64, d_final.double())
+    recurrence_tests.close(final, want, 2.0 ** -19 * want.detach().abs(), "final")
+    recurrence_tests.close(states[:, 0], want, 2.0 ** -19 * want.detach().abs(), "states")
+    recurrence_tests.close(d_z[:, 0], d_want, 2.0 ** -19 * d_want.abs(), "d_z")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [1e-2, 1e-4, 1e-6])
+@pytest.mark.parametrize("length", [40, 4100])
+def test_sequences_of_candidates_next_to_zero(length, scale):
+    """The bound of the recurrence's own tests without its absolute part: EPS of what the states add up to."""
+    z, valid, _, d_states, _ = recurrence_tests.draw((2, length, 70), torch.float32, 23, "random")
+    z[..., 70:] *= scale
+    z.requires_grad_()
+    states, _ = recurrent.gated_recurrence(z, valid)
+    want, _, d_want, _, _, d_bound, _ = recurrence_tests.reference(z, valid, None, d_states, None)
+    with torch.no_grad():
+        z64 = torch.where(valid[..., None], z.detach().double(), 0.0)
+        a, b = recurrence_tests.gates(z64, valid)
+        none = torch.zeros_like(b[:, 0])
+        size = recurrence_tests.scan(a, b.abs(), none)
+        bound = 4 * recurrence_tests.EPS * recurrence_tests.scan(a, size, none)
+    recurrence_tests.close(states, want, bound, "states")
+    (d_z,) = torch.autograd.grad(states, z, d_states)
+    recurrence_tests.close(d_z, d_want, d_bound, "d_z")
