@@ -58,7 +58,7 @@ __device__ __forceinline__ void exp_pair(float r, float c, float& e, float& d) {
     d = __builtin_amdgcn_exp2f(fabsf(c) * -2.88539008177792682f);
 }
 // s = 1 / (1 + e) and 1 - s = e / (1 + e), so that k (down to 2^-8) loses nothing to a
-// subtraction from 1: a and k within 10 units of 2^-24 (the product with log2 e is rounded,
+// subtraction from 1: a and k within 7 units of 2^-24 (the product with log2 e is rounded,
 // which costs s or 1 - s |r| units more where that one is small, and 2^-8 is not).
 // u = (1 - d) / (1 + d), which cancels next to zero; below 3/8 it is c + c^3 P(c^2), P of
 // degree 2 with the least largest error of tanh (7e-8 of it). u is within 2.3 units of 2^-24
@@ -586,6 +586,7 @@ struct Fill {
 };
 constexpr Fill kForwardFill{512, 3}, kBackwardFill{256, 2};
 constexpr int64_t kPartFill = 256;
+constexpr int64_t kMostGroups = (int64_t(1) << 23) - 8;  // a launch has fewer than 2^32 threads, of 512 a workgroup
 
 inline Plan plan_of(int64_t batch, int64_t length, int64_t width, int vec, int size, Fill fill) {
     Plan p;
@@ -596,6 +597,7 @@ inline Plan plan_of(int64_t batch, int64_t length, int64_t width, int vec, int s
     };
     int64_t least = 0;
     for (int lpc = 1; lpc <= 4; lpc *= 2) {  // rounds of the chip times columns
+        if (lpc > 1 && batch * strips_of(lpc) > kMostGroups) break;  // the widest strips always fit (check_sequence)
         const int64_t cost = (batch * strips_of(lpc) + fill.whole - 1) / fill.whole * (kWave / lpc);
         if (lpc == 1 || cost < least) p.lpc = lpc, least = cost;
     }
@@ -638,8 +640,8 @@ int check_sequence(const char* what, const void* z, int64_t z_batch, int64_t z_r
     if (length > 1 && z_row < 2 * width) return fail(KOEMI_ERR_INVALID, "%s: pre-activation rows overlap", what);
     const __int128 cells = static_cast<__int128>(batch) * width * (length + 1) * 8;
     if (cells > (static_cast<__int128>(1) << 60)) return fail(KOEMI_ERR_INVALID, "%s: too many elements", what);
-    // a launch has fewer than 2^32 threads: 2^23 workgroups, strips of 64 columns or more where many fill the chip
-    if (static_cast<__int128>(batch) * ((width + 63) / 64) > (int64_t(1) << 23) - 8)
+    // plan_of takes strips of 64 columns or more where narrower ones would be too many
+    if (static_cast<__int128>(batch) * ((width + 63) / 64) > kMostGroups)
         return fail(KOEMI_ERR_UNSUPPORTED, "%s: more than 2^23 strips of 64 columns", what);
     // offsets inside a chunk of four lane groups of kKeep rows have 32 bits
     const int64_t row = std::max<int64_t>(length > 1 ? z_row : 0, 2 * width);

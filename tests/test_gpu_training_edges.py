@@ -82,3 +82,25 @@ def test_sequences_of_candidates_next_to_zero(length, scale):
     recurrence_tests.close(states, want, bound, "states")
     (d_z,) = torch.autograd.grad(states, z, d_states)
     recurrence_tests.close(d_z, d_want, d_bound, "d_z")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("width,batch", [(33, (1 << 23) - 8), (65, ((1 << 23) - 8) // 2), (130, ((1 << 23) - 8) // 3)])
+def test_the_largest_batches_that_are_accepted(width, batch):
+    """Widths just above whole strips, where narrow strips would be more than a launch takes."""
+    small, _, initial, d_states, d_final = recurrence_tests.draw((400, 1, width), torch.bfloat16, width, None)
+    at = torch.cat([torch.arange(200, device="cuda"), torch.arange(batch - 200, batch, device="cuda")])
+    z = torch.zeros((batch, 1, 2 * width), device="cuda", dtype=torch.bfloat16)
+    h0, up = torch.zeros((batch, width), device="cuda"), torch.zeros((batch, width), device="cuda")
+    z[at], h0[at], up[at] = small, initial, d_final
+    z.requires_grad_()
+    h0.requires_grad_()
+    states, final = recurrent.gated_recurrence(z, None, h0)
+    d_z, d_h0 = torch.autograd.grad(final, (z, h0), up)
+    want = recurrence_tests.reference(small, None, initial, None, d_final)
+    recurrence_tests.close(states[at], want[0], want[4], "states")
+    recurrence_tests.close(final[at], want[1], want[4][:, -1], "final")
+    recurrence_tests.close(d_z[at], want[2], want[5], "d_z")
+    recurrence_tests.close(d_h0[at], want[3], want[6], "d_initial")
+    for t in (states, final, d_z, d_h0):
+        assert not t[200:-200].any()
