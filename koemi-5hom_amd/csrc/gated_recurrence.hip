@@ -59,7 +59,7 @@ __device__ __forceinline__ void exp_pair(float r, float c, float& e, float& d) {
 }
 // s = 1 / (1 + e) and 1 - s = e / (1 + e), so that k (down to 2^-8) loses nothing to a
 // subtraction from 1: a and k within 7 units of 2^-24 (the product with log2 e is rounded,
-// which costs s or 1 - s |r| units more where that one is small, and 2^-8 is not).
+// which costs s or 1 - s 1.3 |r| units more where that one is small, and 2^-8 is not).
 // u = (1 - d) / (1 + d), which cancels next to zero; below 3/8 it is c + c^3 P(c^2), P of
 // degree 2 with the least largest error of tanh (7e-8 of it). u is within 2.3 units of 2^-24
 // of itself below and 4.2 above; the quotient alone is off by 1.5 / c units ([8, 2048, 1024]

@@ -39,13 +39,15 @@ inline size_t align256(size_t x) { return (x + 255) & ~static_cast<size_t>(255);
 __host__ __device__ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline int64_t padded_hidden(int64_t hidden) { return (hidden + 7) / 8 * 8; }  // rows of whole 32-byte octets
 
-// sigmoid and 1 - sigmoid, each to fp32's relative precision; the exponential stays
-// finite, NaN stays NaN.
+// sigmoid and 1 - sigmoid. The exponential stays finite (an infinite one would make 0 x inf of
+// 1 - s); past its end s is 0, so that g s vanishes however far below zero g lies. NaN stays
+// NaN. The product with log2 e is rounded: s for g < 0 and 1 - s for g > 0 are within
+// 1.3 |g| + 8 units of 2^-24 of themselves, the other within 4.
 __device__ __forceinline__ void sigmoid_pair(float g, float& s, float& rest) {
     const float x = g * -1.44269504088896341f;
-    const float e = __builtin_amdgcn_exp2f(x > 126.0f ? 126.0f : x);
-    s = __builtin_amdgcn_rcpf(1.0f + e);
-    rest = e * s;
+    const float e = __builtin_amdgcn_exp2f(x > 126.0f ? 126.0f : x), r = __builtin_amdgcn_rcpf(1.0f + e);
+    s = x > 126.0f ? 0.0f : r;
+    rest = e * r;
 }
 __device__ __forceinline__ float glu(float g, float v) {
     float s, rest;

@@ -6,6 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+import test_gpu_experts_training as experts_tests
 import test_gpu_recurrence_training as recurrence_tests
 from koemi_amd import recurrent
 
@@ -104,3 +105,51 @@ def test_the_largest_batches_that_are_accepted(width, batch):
     recurrence_tests.close(d_h0[at], want[3], want[6], "d_initial")
     for t in (states, final, d_z, d_h0):
         assert not t[200:-200].any()
+
+
+FAR = (-3e38, -1e30, -1e4, -200.0, -110.0, -89.0, -60.0, -20.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("tokens,width,hidden", [(6, 20, 24), (40, 64, 64), (300, 64, 64)])
+def test_gates_far_below_zero_vanish(tokens, width, hidden, dtype):
+    """g = b_g alone (W_g = 0), each row of FAR in turn: silu(g) and its slope go to 0, however far below zero g lies.
+
+    The sigmoid of g is within 1.3 |g| + 8 units of 2^-24 of itself, 2^-17 of it down to -87 where it passes 2^-126, and
+    may be 0 below: 110 x 2^-126 of silu covers that. Products of K terms in float32 add (K + 64) 2^-24 of their terms'
+    sizes twice, and the bf16 tiles' rows between products 2^-8."""
+    gen = torch.Generator(device="cuda").manual_seed(tokens)
+
+    def normal(*shape):
+        return (torch.randn(shape, device="cuda", generator=gen) * 0.25).to(dtype)
+
+    g = torch.tensor(FAR, device="cuda").repeat(hidden // len(FAR)).to(dtype)
+    case = {"context": normal(tokens, width), "assignments": torch.zeros((tokens, 1), device="cuda", dtype=torch.int64),
+            "pair_weights": torch.ones((tokens, 1), device="cuda"), "valid": torch.ones(tokens, device="cuda", dtype=torch.bool),
+            "gate_weights": torch.zeros((1, hidden, width), device="cuda", dtype=dtype), "gate_biases": g[None],
+            "value_weights": normal(1, hidden, width), "value_biases": normal(1, hidden),
+            "output_weights": normal(1, width, hidden), "output_biases": torch.zeros((1, width), device="cuda", dtype=dtype)}
+    d_out = normal(tokens, width)
+    case, leaves, names = experts_tests.leaves_of(case)
+    y = experts_tests.call(case)
+    grads = dict(zip(names, torch.autograd.grad(y, leaves, d_out)))
+    with torch.no_grad():
+        plain = experts_tests.call(case)
+        x, wv, bv, wo = (case[n].detach().double().squeeze(0) for n in ("context", "value_weights", "value_biases", "output_weights"))
+        g, d = g.double(), d_out.double()
+        between = 2.0 ** -8 if dtype == torch.bfloat16 else 0.0
+        s, tiny, units = torch.sigmoid(g), 110 * 2.0 ** -126, 2.0 ** -17 + between + (max(width, hidden, tokens) + 64) * 2.0 ** -23
+        silu, slope = g * s, s * (1.0 + g * torch.sigmoid(-g))
+        v, v_size = x @ wv.T + bv, x.abs() @ wv.abs().T + bv.abs()
+        up, up_size = d @ wo, d.abs() @ wo.abs()
+
+        def like(got, want, size, what):
+            experts_tests.close(got, want, size, what)
+
+        h_size = (silu.abs() * units + tiny) * v_size
+        like(y, (silu * v) @ wo.T, h_size @ wo.abs().T, "out")
+        like(plain, (silu * v) @ wo.T, h_size @ wo.abs().T, "out without gradients")
+        like(grads["gate_biases"], (up * v * slope).sum(0), (up_size * v_size * (slope.abs() * units + tiny)).sum(0), "d gate_biases")
+        like(grads["value_biases"], (up * silu).sum(0), (up_size * (silu.abs() * units + tiny)).sum(0), "d value_biases")
+        like(grads["pair_weights"], (up * silu * v).sum(1), (up_size * h_size).sum(1), "d pair_weights")
