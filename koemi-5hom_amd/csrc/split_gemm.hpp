@@ -41,9 +41,11 @@ typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16;
 constexpr int kThreads = 256;  // four waves, 2 x 2 over the block tile
 
 // An fp32 operand of a product whose result is rounded to 16 bits: two planes, and beside
-// fp16 (two planes of its own) the product of the second ones is dropped. What is missing
-// stays below 2^-17 of a term, of either sign, 64 times less than half a step of fp16; it
-// saves a third of the products beside bf16 and two of five beside fp16.
+// fp16 (two planes of its own) the product of the second ones is dropped. The missing third
+// plane is at most 2^-17 of a term. A second plane is at most 2^-8 of its value (1 + 2^-8 lies
+// halfway between two bf16 values), so the dropped product is at most 2^-16 more, of one sign
+// where all terms have such values: 3 x 2^-17 in all beside fp16, 21 times less than half a
+// step of it. It saves a third of the products beside bf16 and two of five beside fp16.
 struct coarse_f32 {
     float v;
     __device__ operator float() const { return v; }

@@ -153,3 +153,31 @@ def test_gates_far_below_zero_vanish(tokens, width, hidden, dtype):
         like(grads["gate_biases"], (up * v * slope).sum(0), (up_size * v_size * (slope.abs() * units + tiny)).sum(0), "d gate_biases")
         like(grads["value_biases"], (up * silu).sum(0), (up_size * (silu.abs() * units + tiny)).sum(0), "d value_biases")
         like(grads["pair_weights"], (up * silu * v).sum(1), (up_size * h_size).sum(1), "d pair_weights")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [20, 400])
+def test_fp16_terms_at_the_worst_rounding(tokens):
+    """h = W_o = 1 + 2^-8 in every term: halfway between two bf16 values, so both second planes are 2^-8 and their
+    dropped product is 2^-16 of each term, all of one sign. The third plane would add 2^-17 at most, sums of 96 terms
+    in float32 (96 + 64) 2^-24; b_o takes most of the sum away, so that the output's own half step shows it."""
+    width, hidden = 40, 96
+    one = 1.0 + 2.0 ** -8
+    half = torch.float16
+
+    def full(value, *shape):
+        return torch.full(shape, value, device="cuda", dtype=half)
+
+    b_o = full(-hidden * one * one, 1, width)
+    case = {"context": full(1.0, tokens, width), "assignments": torch.zeros((tokens, 1), device="cuda", dtype=torch.int64),
+            "pair_weights": torch.ones((tokens, 1), device="cuda"), "valid": torch.ones(tokens, device="cuda", dtype=torch.bool),
+            "gate_weights": full(0.0, 1, hidden, width), "gate_biases": full(32.0, 1, hidden),  # silu(32) = 32 in float32
+            "value_weights": full(0.0, 1, hidden, width), "value_biases": full(one / 32.0, 1, hidden),
+            "output_weights": full(one, 1, width, hidden), "output_biases": b_o}
+    want = (hidden * one * one + b_o.double()).expand(tokens, width)
+    terms = hidden * one * one
+    bound = torch.full_like(want, (2.0 ** -16 + 2.0 ** -17 + (hidden + 64) * 2.0 ** -24) * terms)
+    with torch.no_grad():
+        experts_tests.close(experts_tests.call(case), want, bound, "out")
+    trained, _, _ = experts_tests.leaves_of(case)
+    experts_tests.close(experts_tests.call(trained), want, bound, "out with what the gradients need")
