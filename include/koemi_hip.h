@@ -942,13 +942,14 @@ int koemi_gated_recurrence_backward(const void* preactivations, int64_t batch_st
 
 /* LearnedExpertMixture.forward's route and RouterStatistics (model/router.py:11-22,
  * 43-59), to be trained. router_logits F32, F16 or BF16, rows row_stride elements
- * apart, expert_count <= 1024. assignments [tokens, top_k] are the experts of the
- * top_k largest logits in descending order (ties to the lower expert) and weights
- * their softmax probabilities; -1 and 0 for an invalid token, and for an expert whose
- * logit is minus infinity: it is never chosen, and a token with no other logit counts
- * as invalid. probability_mass, assignment_counts [expert_count], valid_count [1] and
- * balance_loss [1] as koemi_moe_route_learned_stats. Sums run in a fixed order.
- * Workspace: koemi_moe_route_balanced_workspace_bytes bytes, no zeroing needed. */
+ * apart, expert_count <= 1024, fewer than 2^32 choices. assignments [tokens, top_k]
+ * are the experts of the top_k largest logits in descending order (ties to the lower
+ * expert) and weights their softmax probabilities; -1 and 0 for an invalid token, and
+ * for an expert whose logit is minus infinity: it is never chosen, and a token with no
+ * other logit counts as invalid. probability_mass, assignment_counts [expert_count],
+ * valid_count [1] and balance_loss [1] as koemi_moe_route_learned_stats. Sums run in a
+ * fixed order. Workspace: koemi_moe_route_balanced_workspace_bytes bytes, no zeroing
+ * needed. */
 size_t koemi_moe_route_balanced_workspace_bytes(int64_t tokens, int64_t expert_count);
 int koemi_moe_route_balanced_forward(const void* router_logits, int dtype, int64_t row_stride,
                                      const uint8_t* valid_mask, int64_t* assignments, float* weights,

@@ -397,6 +397,8 @@ int check_route(const char* what, const void* logits, int dtype, int64_t row_str
     if (tokens < 0 || experts < 1 || top_k < 1) return fail(KOEMI_ERR_INVALID, "%s: bad dimension", what);
     if (experts > kMaxExperts) return fail(KOEMI_ERR_UNSUPPORTED, "%s: more than %d experts", what, kMaxExperts);
     if (top_k > experts) return fail(KOEMI_ERR_INVALID, "%s: top_k exceeds the experts", what);
+    if (tokens > ((int64_t(1) << 32) - 1) / top_k)  // their counts have 32 bits
+        return fail(KOEMI_ERR_UNSUPPORTED, "%s: 2^32 choices or more", what);
     if (tokens > 0 && !logits) return fail(KOEMI_ERR_INVALID, "%s: null logits", what);
     if (tokens > 1 && row_stride < experts) return fail(KOEMI_ERR_INVALID, "%s: logit rows overlap", what);
     return KOEMI_OK;

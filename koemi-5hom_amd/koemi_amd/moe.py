@@ -379,7 +379,7 @@ def route_topk_balanced(router_logits: Tensor, valid_mask: Tensor, *, top_k: int
     """The learned softmax top-k gate of router.py:43-59 with first-order autograd.
 
     ``router_logits`` ``[..., E]`` float32, float16 or bfloat16 (any strides; E at
-    most 1024), ``valid_mask`` bool of the leading shape. Returns int64 assignments
+    most 1024, fewer than 2^32 choices), ``valid_mask`` bool of the leading shape. Returns int64 assignments
     and float32 weights of shape ``[..., top_k]`` and the ``RouterStatistics``: the
     experts of the ``top_k`` largest logits in descending order (ties to the lower
     index) with their softmax probabilities, -1 and 0 for an invalid token. An expert
@@ -405,6 +405,8 @@ def route_topk_balanced(router_logits: Tensor, valid_mask: Tensor, *, top_k: int
     top_k = _require_positive_bounded(top_k, "top_k", 1024)
     if top_k > expert_count:
         raise CudaMoeValidationError("top_k must not exceed expert_count")
+    if valid_mask.numel() * top_k >= 1 << 32:
+        raise CudaMoeValidationError("tokens x top_k must be below 2^32")
     _require_library()
     assignments, weights, mass, counts, valid_count, loss = _RouteBalanced.apply(router_logits, valid_mask, top_k)
     return assignments, weights, RouterStatistics(mass, counts, valid_count, loss)

@@ -8,7 +8,7 @@ import torch
 
 import test_gpu_experts_training as experts_tests
 import test_gpu_recurrence_training as recurrence_tests
-from koemi_amd import recurrent
+from koemi_amd import _native, moe, recurrent
 
 
 @pytest.mark.gpu
@@ -181,3 +181,19 @@ def test_fp16_terms_at_the_worst_rounding(tokens):
         experts_tests.close(experts_tests.call(case), want, bound, "out")
     trained, _, _ = experts_tests.leaves_of(case)
     experts_tests.close(experts_tests.call(trained), want, bound, "out with what the gradients need")
+
+
+def test_routes_of_2_32_choices_are_refused():
+    """Their counts would pass 32 bits."""
+    for name, pointers in (("koemi_moe_route_balanced_forward", 7), ("koemi_moe_route_balanced_backward", 8)):
+        tail = (None, 0, None) if name.endswith("forward") else (None,)
+        with pytest.raises(_native.NativeCallError, match="2\\^32"):
+            _native.call(name, None, _native.dtype_code(torch.bfloat16), 2, *([None] * pointers), 1 << 31, 2, 2, *tail)
+
+
+@pytest.mark.gpu
+def test_routes_of_2_32_choices_are_refused_by_the_front():
+    logits = torch.zeros((1, 2), device="cuda", dtype=torch.bfloat16).expand(1 << 31, 2)
+    valid = torch.ones(1, device="cuda", dtype=torch.bool).expand(1 << 31)
+    with pytest.raises(moe.CudaMoeValidationError, match="2\\^32"):
+        moe.route_topk_balanced(logits, valid, top_k=2)
