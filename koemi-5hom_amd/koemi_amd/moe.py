@@ -1033,6 +1033,9 @@ def expert_mixture(
             3 * experts * -(-width // 64) * -(-hidden // 64) > (1 << 24) - 8:
         raise CudaMoeValidationError("tokens x width must be below 2^34 and the parameters' 64 x 64 blocks below 2^22 each")
     _require_library()
+    if tokens and not _size("koemi_moe_experts_workspace_bytes", tokens, top_k, width, hidden, experts,
+                            _native.dtype_code(context.dtype), 0):
+        raise CudaMoeValidationError("the pairs' rows in tiles of 64 to 256, times the wider side's 64 columns, must be below 2^24")
     if validate and tokens:
         flat, mask = assignments.reshape(-1, top_k).contiguous(), valid_mask.reshape(-1)
         # a slot of -1 is no expert: it takes one past the catalog of its own, which repeats nothing

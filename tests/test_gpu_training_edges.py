@@ -197,3 +197,21 @@ def test_routes_of_2_32_choices_are_refused_by_the_front():
     valid = torch.ones(1, device="cuda", dtype=torch.bool).expand(1 << 31)
     with pytest.raises(moe.CudaMoeValidationError, match="2\\^32"):
         moe.route_topk_balanced(logits, valid, top_k=2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("validate", [False, True])
+def test_experts_of_more_tiles_than_a_launch_takes_are_refused_at_once(validate):
+    def t(*shape, dtype=torch.float16):
+        return torch.zeros(shape, device="cuda", dtype=dtype)
+
+    tokens, width, hidden = 1 << 24, 512, 8192
+    matrix = t(4, hidden, width)
+    args = [t(1, width).expand(tokens, width), torch.arange(2, device="cuda").expand(tokens, 2), None,
+            t(1, dtype=torch.bool).expand(tokens), matrix, t(4, hidden), matrix, t(4, hidden), matrix.transpose(1, 2), t(4, width)]
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    with pytest.raises(moe.CudaMoeValidationError, match="2\\^24"):
+        moe.expert_mixture(*args, validate=validate)
+    assert torch.cuda.max_memory_allocated() == before
