@@ -15,8 +15,9 @@
 //
 // A lane always holds the same experts, so the mass adds up in its registers over
 // the workgroup's tokens, then over its groups through LDS, then over the workgroups in
-// a second launch: every order is fixed (the counts are whole numbers). Bound by memory for many experts, by the two
-// launches' latency for a few tokens.
+// a second launch: every order is fixed (the counts are whole numbers). Bound by the latency
+// of a token's reductions for many experts (two waves a SIMD in the forward), by the two
+// launches' for a few tokens.
 #include "common.hpp"
 
 #include <algorithm>
@@ -82,6 +83,16 @@ __device__ __forceinline__ float key_value(uint32_t k) {
     } else {
         return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
     }
+}
+
+// n values `step` apart, in eight sums and those in pairs: 64 in a row are off by twice as
+// much ([64, 16] fp32, the mass: 1.2e-7 of itself, 5e-8 so).
+__device__ __forceinline__ float spaced_sum(const float* p, int step, int n) {
+    float s[8] = {};
+    for (int i = 0; i < n; i += 8)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[j] += i + j < n ? p[(i + j) * step] : 0.0f;
+    return ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
 }
 
 // The layout of a token: G lanes of VPL experts each.
@@ -208,8 +219,7 @@ __global__ __launch_bounds__(kThreads) void route_balanced_kernel(
     for (int v = 0; v < VPL; ++v) mass_sh[group * (G * VPL) + e0 + v] = mass[v];
     __syncthreads();
     for (int e = tid; e < experts; e += kThreads) {
-        float m = 0.0f;
-        for (int g = 0; g < K::kPerBlock; ++g) m += mass_sh[g * (G * VPL) + e];
+        const float m = spaced_sum(mass_sh + e, G * VPL, K::kPerBlock);
         part_mass[static_cast<int64_t>(blockIdx.x) * experts + e] = m;
         part_counts[static_cast<int64_t>(blockIdx.x) * experts + e] = counts_sh[e];
     }
@@ -258,8 +268,10 @@ __global__ __launch_bounds__(kFinishThreads) void route_balanced_finish_kernel(
     counts_sh[tid] = c;
     const uint32_t routed = block_sum<uint32_t, kFinishThreads>(n, count_scratch);  // (joins: the slices are in LDS)
     m = 0.0f, c = 0;
-    if (tid < experts)
-        for (int s = 0; s < slices; ++s) m += mass_sh[s * padded + tid], c += counts_sh[s * padded + tid];
+    if (tid < experts) {
+        m = spaced_sum(mass_sh + tid, padded, slices);
+        for (int s = 0; s < slices; ++s) c += counts_sh[s * padded + tid];
+    }
     const uint32_t total = block_sum<uint32_t, kFinishThreads>(c, count_scratch);
     const float share = tid < experts ? m / fmaxf(static_cast<float>(routed), 1.0f) *
                                             (static_cast<float>(c) / fmaxf(static_cast<float>(total), 1.0f)) : 0.0f;

@@ -215,3 +215,16 @@ def test_experts_of_more_tiles_than_a_launch_takes_are_refused_at_once(validate)
     with pytest.raises(moe.CudaMoeValidationError, match="2\\^24"):
         moe.expert_mixture(*args, validate=validate)
     assert torch.cuda.max_memory_allocated() == before
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("experts", [5, 10, 11, 17, 26, 31, 33, 62])
+def test_mass_of_equal_probabilities(experts):
+    """p = 1 / E in every token, one token for each lane group of a workgroup: p is off by one unit of 2^-24 with its
+    reciprocal, the eight sums of k equal values by (k + 1) / 2 (step i rounds i p of k p), and joining equal sums is
+    exact. k = 1 / 8 of the 128 groups of two lanes, 64 of four and 32 of eight."""
+    tokens = 256 // (2 if experts <= 8 else 4 if experts <= 16 else 8)
+    logits, valid = torch.zeros((tokens, experts), device="cuda"), torch.ones(tokens, device="cuda", dtype=torch.bool)
+    _, _, statistics = moe.route_topk_balanced(logits, valid, top_k=1)
+    off = (statistics.probability_mass.double() * experts / tokens - 1.0).abs().max().item()
+    assert off <= ((tokens / 8 + 1) / 2 + 2) * 2.0 ** -24, off * 2.0 ** 24
