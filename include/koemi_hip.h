@@ -987,8 +987,9 @@ int koemi_moe_router_balance_loss_backward(const float* assignment_counts, const
  * backward. Workspace: koemi_moe_experts_workspace_bytes, no zeroing needed; both 16-byte
  * aligned. Refused (the queries give 0): 2^26 pairs, 2^34 context values or 2^22 blocks of
  * 64 x 64 parameters and more, or 2^24 tiles of the pairs' rows (64, 128 or, bf16 of widths
- * in multiples of 64, 256) by 64 columns of the wider side. bf16 of widths in multiples of 64 needs 16-byte aligned
- * operands. */
+ * in multiples of 64, 256) by 64 columns of the wider side. bf16 of widths in multiples of
+ * 64 needs 16-byte aligned operands and rounds h and its gradients to bf16 between the
+ * products (from 64 pairs an expert on, and without `saved` below that too); sums are fp32. */
 size_t koemi_moe_experts_saved_bytes(int64_t tokens, int64_t top_k, int64_t width, int64_t hidden,
                                      int64_t expert_count, int dtype);
 size_t koemi_moe_experts_workspace_bytes(int64_t tokens, int64_t top_k, int64_t width, int64_t hidden,

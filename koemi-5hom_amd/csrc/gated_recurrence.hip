@@ -63,7 +63,8 @@ __device__ __forceinline__ void exp_pair(float r, float c, float& e, float& d) {
 // u = (1 - d) / (1 + d), which cancels next to zero; below 3/8 it is c + c^3 P(c^2), P of
 // degree 2 with the least largest error of tanh (7e-8 of it). u is within 2.3 units of 2^-24
 // of itself below and 4.2 above; the quotient alone is off by 1.5 / c units ([8, 2048, 1024]
-// bf16 forward: 32 us with the quotient alone, 35 with P of degree 1 below 3/16 or with this).
+// bf16 forward: 32 us with the quotient alone, 35 with P of degree 1 below 3/16 or with this;
+// [1, 32768, 512] fp32 forward 44 and 47 beside its fold).
 template <bool GRADIENTS>
 __device__ __forceinline__ Gates gates_of(float r, float c) {
     Gates o;
@@ -578,6 +579,7 @@ struct Plan {
 };
 // whole: workgroups that run at once on 256 CUs. The registers let two of the forward's share
 // a CU and one of the backward's (bf16 [16, 2048, 1024] backward: 82 us as 256, 92 as 512).
+// Strips have 16 lanes at least, so that [8, 2048, 1024] has 256 workgroups forward too.
 // parts: from how many on they pay for the fold (bf16 [4, 2048, 1024] in two: forward 12 + 16 us
 // against 26, backward 8 + 23 against 38). They fill the chip once: more only hand on more maps
 // (bf16 [1, 32768, 512] backward: 43 us in 32 parts of eight strips, 55 in 64).

@@ -443,8 +443,10 @@ __global__ __launch_bounds__(split_gemm::kThreads, 2) void any_weight_gradient_k
 // ------------------------------------------------------------ the bf16 tiles ---
 // Width and hidden multiples of 64: 256 x 256 tiles of mfma_stage.hpp and mfma_across.hpp
 // (four waves in 2 x 2, 128 x 128 outputs each, operands through a ring of four LDS
-// stages filled by direct copies). What lies between two products is bf16, g, v, y and dx
-// are fp32. A slot is up to 256 pairs of one expert; the backward works on rows padded to
+// stages filled by direct copies). What lies between two products (h, dg, dv, w h) is bf16: as
+// two planes it would double four of the six products, for 1.7e-3 from float64 (the results'
+// own rounding) instead of 2.3e-3; bf16 torch operations, which round g, v, silu and y too, are at
+// 4.7e-3 to 5.8e-3 (4096 tokens, 1024 -> 2048). g, v, y, dx and every sum are fp32. A slot is up to 256 pairs of one expert; the backward works on rows padded to
 // whole slots (row 256 slot + r), so that sums over an expert's pairs take whole K steps:
 // rows past its pairs are zeros.
 using mfma_stage::across_fragment;
@@ -1448,7 +1450,7 @@ int tile_backward(const Shape& s, const void* d_out, const void* x, const int64_
                        static_cast<const bf16*>(x), static_cast<const bf16*>(d_out), rows, static_cast<const bf16*>(m.bo),
                        sorted_w, share, d.Wg || d.Wv ? xs : nullptr, ds, d.weights ? w.dot : nullptr,
                        d.bo ? w.out_sums : nullptr, w.slots, slots, s.pairs, s.tokens, s.width);
-        hipLaunchKernelGGL(tile_hidden_gradient_kernel, dim3(tiles_grid(slots, h_tiles)), threads, 0, q, ds,
+    hipLaunchKernelGGL(tile_hidden_gradient_kernel, dim3(tiles_grid(slots, h_tiles)), threads, 0, q, ds,
                        static_cast<const bf16*>(m.Wo), keep, keep + kept_floats(s), sorted_w, share, dgv, wh, w.dw_part,
                        d.bg || d.bv ? w.sums : nullptr, w.slots, slots, s.pairs, s.width, s.hidden, h_tiles);
     if (d.x) {

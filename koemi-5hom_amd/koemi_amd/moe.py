@@ -988,7 +988,15 @@ def expert_mixture(
     Returns ``context``'s shape and dtype: the sum over a token's slots of
     ``w (W_o (silu(W_g x + b_g) * (W_v x + b_v)) + b_o)``, zeros without any. All
     floating arguments are differentiable (``koemi_moe_experts_backward``); sums are
-    float32, in a fixed order."""
+    float32, in a fixed order.
+
+    What lies between two products is float32 too, except in bfloat16 with width and
+    hidden multiples of 64: from 64 pairs an expert on the product ``h`` of the gates and
+    its gradients are rounded to bfloat16, and without gradients ``h`` below that as well.
+    Results are then 2.3e-3 from float64 in the relative norm, where rounding them alone
+    is 1.7e-3 (and bfloat16 torch operations 4.7e-3 to 5.8e-3). Refused: 2^26 pairs, 2^34
+    context values, 2^22 blocks of 64 x 64 parameters, or 2^24 tiles of 64 to 256 pairs by
+    64 columns of the wider side, and more."""
 
     params = {"gate_weights": gate_weights, "gate_biases": gate_biases, "value_weights": value_weights,
               "value_biases": value_biases, "output_weights": output_weights, "output_biases": output_biases}
