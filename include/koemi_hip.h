@@ -1015,6 +1015,41 @@ int koemi_moe_experts_backward(const void* grad_output, const void* context, con
                                int64_t tokens, int64_t top_k, int64_t width, int64_t hidden, int64_t expert_count,
                                int dtype, void* workspace, size_t workspace_bytes, koemi_stream_t stream);
 
+/* Multi-head attention over a window of positions and the first ones (sinks), the
+ * sliding-window read of LocalKeyValueMemory (model/memory.py:332-383) with heads, to be
+ * trained. queries [batch, length, heads, width], keys and values [batch, total, groups,
+ * width] in one type (F32, F16, BF16), columns contiguous; strides: nine element
+ * strides on the host (batch, position and head of queries, keys and values). groups divides
+ * heads, query head h reads key head h / (heads / groups); the queries stand at the last
+ * `length` of `total` positions. Query i sees j <= i with i - j < window or j < sinks.
+ * valid [batch, total] (NULL: all): a position with 0 is neither read nor reads, whatever its
+ * tensors hold. A query that sees nothing gets zeros. scale (positive): of the scores.
+ * output [batch, length, heads, width], contiguous; rest (NULL: no gradients wanted; not
+ * for F32) like it: what the output was rounded off by; lse [batch, groups, length x heads /
+ * groups] fp32 (NULL: no gradients wanted): log2 of the sum of 2^(score log2 e), infinite
+ * where nothing is seen. Workspace: koemi_window_attention_workspace_bytes, no zeroing
+ * needed, 4-byte aligned. Refused: widths over 256, 2^29 rows (positions x heads / groups)
+ * of a key head and 2^24 tiles of 128 of them and more. */
+size_t koemi_window_attention_workspace_bytes(int64_t batch, int64_t length, int64_t total, int64_t heads, int64_t groups,
+                                              int64_t width, int64_t window, int64_t sinks, int dtype);
+int koemi_window_attention_forward(const void* queries, const void* keys, const void* values, const uint8_t* valid,
+                                   const int64_t* strides, void* output, void* rest, float* lse, int64_t batch,
+                                   int64_t length, int64_t total, int64_t heads, int64_t groups, int64_t width, int64_t window,
+                                   int64_t sinks, float scale, int dtype, void* workspace, size_t workspace_bytes,
+                                   koemi_stream_t stream);
+
+/* Its gradients, each contiguous in its input's shape, NULL where not wanted. output,
+ * rest, lse: the forward's; grad_output contiguous. Sums run in a fixed order. */
+size_t koemi_window_attention_backward_workspace_bytes(int64_t batch, int64_t length, int64_t total, int64_t heads,
+                                                       int64_t groups, int64_t width, int64_t window, int64_t sinks,
+                                                       int dtype);
+int koemi_window_attention_backward(const void* queries, const void* keys, const void* values, const uint8_t* valid,
+                                    const int64_t* strides, const void* output, const void* rest, const float* lse,
+                                    const void* grad_output, void* grad_queries, void* grad_keys, void* grad_values, int64_t batch, int64_t length,
+                                    int64_t total, int64_t heads, int64_t groups, int64_t width, int64_t window,
+                                    int64_t sinks, float scale, int dtype, void* workspace, size_t workspace_bytes,
+                                    koemi_stream_t stream);
+
 /* Measurement only (no counterpart in the reference): reads `bytes` (a
  * multiple of 16) from `src` with `grid` workgroups of `block` threads, each
  * thread issuing `unroll` (1, 2, 4 or 8) 16-byte loads per pass of a

@@ -1,0 +1,313 @@
+// What the kernels of the windowed attention with sinks share (window_attention.hip,
+// window_attention_grad.hip): the call's shape, tiles of rows staged through LDS, and the
+// matrix products on them.
+//
+// Position i of the keys sees j if both are valid, j <= i, and i - j < window or j <
+// sinks. Queries stand at the last `length` of `total` positions. The `shared` query heads
+// of one key head are rows of one matrix: row m is position m / shared, head m % shared,
+// so heads that share keys share every tile of them, whatever `shared` is.
+//
+// Products are v_mfma_f32_32x32x16 (16-bit types) and v_mfma_f32_32x32x2f32 (fp32, whole
+// products): lane l holds column l % 32 of a result, rows 8 (r / 4) + 4 (l / 32) + r % 4
+// in register r. A product over the columns of a staged tile reads its rows as they lie (16
+// bytes a lane, mma_rows). A product over the tile's rows takes the other operand straight
+// from a result's registers: the rows a lane holds there are the K values it brings,
+// whatever their order, as long as the tile's operand is read in the same one
+// (mma_acc; 16-bit through ds_read_b64_tr_b16, which hands each lane four rows of a column).
+#pragma once
+
+#include "common.hpp"
+
+#include <type_traits>
+
+namespace koemi {
+namespace window_attention {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / kWave;
+constexpr int kRows = 32 * kWaves;  // rows (or keys) of a workgroup, 32 a wave
+constexpr float kLog2e = 1.44269504088896341f;
+
+struct Strides {
+    int64_t batch, position, head;
+};
+
+struct Shape {
+    const void* q;
+    const void* k;
+    const void* v;
+    const uint8_t* valid;  // [batch, total] or null
+    Strides qs, ks, vs;
+    int batch, length, total, groups, shared, width;
+    int window, sinks;  // at most total
+    float scale;        // of the scores
+    uint32_t magic;     // rows / shared = (rows * magic >> 32) >> shift, rows below 2^31
+    int shift;
+    int vector;         // rows are whole, aligned 16-byte pieces
+};
+
+// The position of row m, and its head among those that share.
+__device__ __forceinline__ int position_of(const Shape& a, int m) {
+    return a.shared == 1 ? m : static_cast<int>(__umulhi(static_cast<uint32_t>(m), a.magic) >> a.shift);
+}
+
+// Probabilities of fp16 calls are kept times 2^8: what is below 2^-14 of the largest would lose bits.
+template <typename T> inline constexpr float kLift = 0.0f;
+template <> inline constexpr float kLift<f16> = 8.0f;
+
+template <typename T> inline constexpr int kPer16 = 16 / static_cast<int>(sizeof(T));  // values in 16 bytes
+
+// NB: blocks of 32 columns that a head's width fills. A staged row is a power of two of bytes.
+template <typename T, int NB>
+struct Tile {
+    static constexpr int kBytes = NB * 32 * static_cast<int>(sizeof(T));
+    static constexpr int kUnits = kBytes / 16;
+    static constexpr int kStride = kBytes <= 64 ? 64 : kBytes <= 128 ? 128 : kBytes <= 256 ? 256 : kBytes <= 512 ? 512 : 1024;
+    static constexpr int kFrags = kUnits / 2;  // 16-byte pieces of a row that a lane brings to mma_rows
+    // 16-byte unit u of row r lies at unit u ^ turn(r): the sixteen rows that sixteen lanes
+    // read at one unit, and the four rows by 64 bytes of a transposed read, fill all banks.
+    static __device__ __forceinline__ int turn(int r) {
+        return kStride >= 256 ? ((r & 3) << 2) | ((r >> 2) & 3) : kStride == 128 ? ((r & 2) << 1) | ((r >> 2) & 3) : (r >> 2) & 3;
+    }
+    static __device__ __forceinline__ int at(int r, int unit) { return r * kStride + ((unit ^ turn(r)) << 4); }
+};
+
+template <typename T> __device__ __forceinline__ bool any_nonfinite(const uint4& x) {
+    constexpr uint32_t E = sizeof(T) == 4 ? 0x7f800000u : std::is_same<T, f16>::value ? 0x7c00u : 0x7f80u;
+    bool bad = false;
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        bad |= (w[i] & E) == E;
+        if (sizeof(T) == 2) bad |= ((w[i] >> 16) & E) == E;
+    }
+    return bad;
+}
+
+// 16 bytes of a row from column 16 / sizeof(T) * unit on, zeros past the width.
+template <typename T>
+__device__ __forceinline__ uint4 load_unit(const T* row, int unit, int width, bool vector) {
+    constexpr int E = kPer16<T>;
+    const int c = unit * E;
+    uint4 out = make_uint4(0, 0, 0, 0);
+    if (vector) {
+        if (c < width) out = *reinterpret_cast<const uint4*>(row + c);
+    } else {
+        alignas(16) T e[E];
+#pragma unroll
+        for (int i = 0; i < E; ++i) e[i] = c + i < width ? row[c + i] : static_cast<T>(0.0f);
+        out = *reinterpret_cast<const uint4*>(e);
+    }
+    return out;
+}
+
+// A tile's rows on their way from memory to LDS. row(i) gives row i's address, null for zeros.
+template <typename T, int NB, int ROWS>
+struct Staged {
+    using L = Tile<T, NB>;
+    static constexpr int kPieces = ROWS * L::kUnits;
+    static constexpr int kEach = (kPieces + kThreads - 1) / kThreads;
+    uint4 piece[kEach];
+
+    template <typename Row>
+    __device__ __forceinline__ void load(Row row, int width, bool vector) {
+#pragma unroll
+        for (int n = 0; n < kEach; ++n) {
+            const int i = static_cast<int>(threadIdx.x) + n * kThreads;
+            piece[n] = make_uint4(0, 0, 0, 0);
+            if (kPieces % kThreads == 0 || i < kPieces) {
+                const T* p = row(i / L::kUnits);
+                if (p) piece[n] = load_unit<T>(p, i % L::kUnits, width, vector);
+            }
+        }
+    }
+    __device__ __forceinline__ void store(char* tile) const {
+#pragma unroll
+        for (int n = 0; n < kEach; ++n) {
+            const int i = static_cast<int>(threadIdx.x) + n * kThreads;
+            if (kPieces % kThreads == 0 || i < kPieces)
+                *reinterpret_cast<uint4*>(tile + L::at(i / L::kUnits, i % L::kUnits)) = piece[n];
+        }
+    }
+    __device__ __forceinline__ bool bad() const {
+        bool b = false;
+#pragma unroll
+        for (int n = 0; n < kEach; ++n) b |= any_nonfinite<T>(piece[n]);
+        return b;
+    }
+};
+
+template <typename T>
+__device__ __forceinline__ f32x16 mfma16(const uint4& a, const uint4& b, f32x16 c) {
+    if constexpr (std::is_same<T, bf16>::value)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+}
+
+// acc[tile row first + ...][column] += tile row . frag, frag being the lane's pieces of column l % 32's row.
+template <typename T, int NB>
+__device__ __forceinline__ void mma_rows(f32x16& acc, const char* tile, int first, const uint4 (&frag)[Tile<T, NB>::kFrags]) {
+    using L = Tile<T, NB>;
+    const int lane = lane_id(), r = first + (lane & 31);
+    const char* base = tile + r * L::kStride;
+    const int turned = ((lane >> 5) ^ L::turn(r)) << 4;
+#pragma unroll
+    for (int s = 0; s < L::kFrags; ++s) {
+        const uint4 a = *reinterpret_cast<const uint4*>(base + (turned ^ (s << 5)));
+        if constexpr (sizeof(T) == 4) {
+            const float* x = reinterpret_cast<const float*>(&a);
+            const float* y = reinterpret_cast<const float*>(&frag[s]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(x[c], y[c], acc, 0, 0, 0);
+        } else {
+            acc = mfma16<T>(a, frag[s], acc);
+        }
+    }
+}
+
+// acc[n][32 n + ...][column] += sum over the tile's rows first .. first + 31 of row[32 n + ...] coef[row][column].
+template <typename T, int NB>
+__device__ __forceinline__ void mma_acc(f32x16 (&acc)[NB], const char* tile, int first, const f32x16& coef) {
+    using L = Tile<T, NB>;
+    const int lane = lane_id(), half = lane >> 5;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int row = first + 8 * (r / 4) + 4 * half + r % 4;
+            const char* base = tile + row * L::kStride + (lane & 3) * 4;
+            const int unit = ((lane & 31) >> 2) ^ L::turn(row);
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+                acc[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(*reinterpret_cast<const float*>(base + ((unit ^ (8 * n)) << 4)),
+                                                              coef[r], acc[n], 0, 0, 0);
+        }
+    } else {
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+        const int j = (lane & 15) >> 2, unit = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            alignas(16) T e[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) e[i] = static_cast<T>(coef[8 * s + i]);
+            const uint4 b = *reinterpret_cast<const uint4*>(e);
+            const char* base[2];
+            int turned[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int row = first + 16 * s + 8 * i + 4 * half + j;
+                base[i] = tile + row * L::kStride + (lane & 1) * 8;
+                turned[i] = (unit ^ L::turn(row)) << 4;
+            }
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                union {
+                    s16x4 part[2];
+                    uint4 whole;
+                } a;
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    a.part[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(base[i] + (turned[i] ^ (n << 6))));
+                acc[n] = mfma16<T>(a.whole, b, acc[n]);
+            }
+        }
+    }
+}
+
+// mma_acc for a block that holds an infinity or NaN and is masked in places: 0 times one of
+// them is not 0, so only what a column sees is added, one row after another. `seen`: the
+// lane's column's 32 rows. `scratch`: 32 x 32 floats of this wave's own.
+template <typename T, int NB>
+__device__ __forceinline__ void seen_acc(f32x16 (&acc)[NB], const char* tile, int first, const f32x16& coef, uint32_t seen, float* scratch) {
+    using L = Tile<T, NB>;
+    const int lane = lane_id(), half = lane >> 5, col = lane & 31;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) scratch[(8 * (r / 4) + 4 * half + r % 4) * 32 + col] = coef[r];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll 1
+    for (int k = 0; k < 32; ++k) {
+        const float c = scratch[k * 32 + col];
+        if (!((seen >> k) & 1u)) continue;
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int d = 32 * n + 8 * q + 4 * half;
+                const T* x = reinterpret_cast<const T*>(tile + L::at(first + k, d / kPer16<T>) + (d % kPer16<T>) * sizeof(T));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[n][4 * q + i] = fmaf(c, to_f32(x[i]), acc[n][4 * q + i]);
+            }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
+
+// Both halves of the wave hold a part of a column's maximum or sum.
+__device__ __forceinline__ float max_of_halves(float x) {
+    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+}
+__device__ __forceinline__ float sum_of_halves(float x) {
+    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(both[0]) + __uint_as_float(both[1]);
+}
+
+// The lowest n bits, n of any sign.
+__device__ __forceinline__ uint64_t low_bits(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; }
+
+// Of the 64 keys from key0 on, those that a query at `place` sees by position.
+__device__ __forceinline__ uint64_t keys_seen(const Shape& a, int place, int key0) {
+    const int rel = place - key0;
+    return low_bits(rel + 1) & (~low_bits(rel - a.window + 1) | low_bits(a.sinks - key0));
+}
+
+// The 16 bits of a 32-row block's mask that the lane's registers hold, from bit 0 on.
+__device__ __forceinline__ bool bit_of(uint32_t seen_half, int r) { return (seen_half >> (8 * (r / 4) + r % 4)) & 1u; }
+
+// A workgroup's place: consecutive workgroups go to the eight XCDs in turn, so those that
+// share keys (neighbours) are given to one of them.
+__device__ __forceinline__ int by_xcd(int id, int count) {
+    const int even = count & ~7;
+    return id < even ? (id & 7) * (even >> 3) + (id >> 3) : id;
+}
+
+// Key tiles of KT that rows at places first .. last (of the keys' positions) see: the
+// sinks' before the window, then the window's.
+template <int KT>
+struct KeyTiles {
+    int lead, skip, count;
+    __device__ __forceinline__ KeyTiles(const Shape& a, int first, int last) {
+        const int low = max(first - a.window + 1, 0) / KT;
+        lead = min((a.sinks + KT - 1) / KT, low);
+        skip = low - lead;
+        count = lead + last / KT - low + 1;
+    }
+    __device__ __forceinline__ int operator[](int t) const { return t < lead ? t : t + skip; }
+};
+
+// Checks, and the shape as the kernels take it (window_attention.hip).
+int shape_of(const char* what, const void* queries, const void* keys, const void* values, const uint8_t* valid,
+             const int64_t* strides, int64_t batch, int64_t length, int64_t total, int64_t heads, int64_t groups,
+             int64_t width, int64_t window, int64_t sinks, float scale, int dtype, Shape& s);
+
+// Four consecutive values of a row of `width` from column d on.
+template <typename T>
+__device__ __forceinline__ void store_four(T* row, int d, int width, const float (&x)[4]) {
+    alignas(16) T e[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[i] = from_f32<T>(x[i]);
+    if (width % 4 == 0) {
+        if (d < width) __builtin_memcpy(__builtin_assume_aligned(row + d, 4 * sizeof(T)), e, 4 * sizeof(T));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (d + i < width) row[d + i] = e[i];
+    }
+}
+
+}  // namespace window_attention
+}  // namespace koemi

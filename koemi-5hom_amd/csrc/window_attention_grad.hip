@@ -1,0 +1,471 @@
+// Gradients of the attention over a window and the first positions (sinks):
+//
+//   p_ij = 2^(c s_ij - lse_i) again from the kept lse,  D_i = sum_d dout_id out_id
+//   dp_ij = dout_i . v_j,  ds_ij = p_ij (dp_ij - D_i)
+//   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i,  dv_j = sum_i p_ij dout_i
+//
+// Two kernels, each owning what it sums, so that no sum depends on an order of arrival: one
+// holds 128 rows (positions x shared heads) and walks the keys for dq and D, one holds 128
+// keys and walks the rows for dk and dv, all heads that share the keys among them. That
+// forms s and dp twice (seven products of a pair instead of five). The sinks are seen by every
+// later row: what lies beyond their window is cut into chunks of rows that run beside the
+// others, and the sinks' own workgroups add the chunks' sums in order.
+#include "window_attention.hpp"
+
+#include <algorithm>
+
+namespace koemi {
+namespace window_attention {
+namespace {
+
+struct Backward {
+    Shape s;
+    const void* out;
+    const void* rest;   // what out was rounded off by, or null: D is a small difference of large terms
+    const void* d_out;  // each [batch, length, heads, width]
+    const float* lse;
+    float* delta;       // D: [batch, groups, rows]
+    void* dq;
+    void* dk;
+    void* dv;
+    float* far_parts;   // [chunks, batch, groups, 128 x far_tiles keys, 2, width]
+    int row_tiles, key_tiles;
+    int far_tiles, far_chunks, far_first, far_rows;  // sinks' key tiles; rows past their window: first, and of a chunk
+};
+
+template <typename T> constexpr int kKeys = sizeof(T) == 4 ? 32 : 64;  // of a tile that dq walks
+
+__device__ __forceinline__ float largest(const f32x16& x) {
+    float m = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) m = fmaxf(m, fabsf(x[r]));
+    return max_of_halves(m);
+}
+
+// fp16 products of ds: its size is the loss's, so each column's ds is brought to about 2^10
+// by a power of two, which is lowered (the sums with it) where a later block exceeds 2^14.
+template <typename T, int NB>
+struct Range {
+    float by = 0.0f;
+    __device__ __forceinline__ void fit(f32x16& ds, f32x16 (&acc)[NB]) {
+        if constexpr (std::is_same<T, f16>::value) {
+            const float high = largest(ds);
+            const bool over = high * by > 16384.0f || (by == 0.0f && high > 0.0f);
+            if (__any(over)) {
+                const int e = static_cast<int>(__float_as_uint(high) >> 23);
+                const float to = over ? __uint_as_float(static_cast<uint32_t>(min(264 - e, 254)) << 23) : by;
+                const float change = over && by != 0.0f ? to / by : 1.0f;
+#pragma unroll
+                for (int n = 0; n < NB; ++n) acc[n] *= change;
+                by = to;
+            }
+            ds *= by;
+        }
+    }
+    __device__ __forceinline__ float back() const {
+        if constexpr (std::is_same<T, f16>::value) return by == 0.0f ? 1.0f : 1.0f / by;
+        return 1.0f;
+    }
+};
+
+template <typename T, int NB>
+__global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void window_dq_kernel(Backward f) {
+    using L = Tile<T, NB>;
+    constexpr int KT = kKeys<T>, KB = KT / 32;
+    __shared__ __attribute__((aligned(1024))) char k_tile[KT * L::kStride];
+    __shared__ __attribute__((aligned(1024))) char v_tile[KT * L::kStride];
+    __shared__ float scratch[kWaves][32 * 32];
+    __shared__ int bad_tile, any_row;
+    const Shape& a = f.s;
+    const int lane = lane_id(), wave = static_cast<int>(threadIdx.x) / kWave, half = lane >> 5, col = lane & 31;
+    int id = by_xcd(static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x));
+    const int tile = id % f.row_tiles;
+    id /= f.row_tiles;
+    const int g = id % a.groups, b = id / a.groups;
+    const int rows = a.length * a.shared, before = a.total - a.length;
+    const int row = tile * kRows + wave * 32 + col, last_row = min(tile * kRows + kRows, rows) - 1;
+    const int position = position_of(a, min(row, rows - 1)), place = before + position;
+    const int head = g * a.shared + min(row, rows - 1) - position * a.shared;
+    const int first = before + position_of(a, tile * kRows), last = before + position_of(a, last_row);
+    const uint8_t* valid = a.valid ? a.valid + static_cast<int64_t>(b) * a.total : nullptr;
+    const bool row_ok = row < rows && (!valid || valid[place]);
+    const int64_t at = (static_cast<int64_t>(b) * a.groups + g) * rows + row;
+    const int64_t cell = ((static_cast<int64_t>(b) * a.length + position) * a.groups * a.shared + head) * a.width;
+    if (threadIdx.x == 0) bad_tile = -1, any_row = 0;
+    __syncthreads();
+    if (__ballot(row_ok) && lane == 0) any_row = 1;
+    __syncthreads();
+
+    f32x16 acc[NB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) acc[n] = f32x16(0.0f);
+    Range<T, NB> range;
+    float delta = 0.0f;
+    const float c = a.scale * kLog2e;
+    if (any_row) {
+        const T* q = static_cast<const T*>(a.q) + b * a.qs.batch + position * a.qs.position + head * a.qs.head;
+        const T* k = static_cast<const T*>(a.k) + b * a.ks.batch + g * a.ks.head;
+        const T* v = static_cast<const T*>(a.v) + b * a.vs.batch + g * a.vs.head;
+        const bool plain = a.width % kPer16<T> == 0;  // out, d_out: contiguous rows
+        uint4 qf[L::kFrags], gf[L::kFrags];
+#pragma unroll
+        for (int s = 0; s < L::kFrags; ++s) {
+            qf[s] = gf[s] = make_uint4(0, 0, 0, 0);
+            if (row_ok) {
+                qf[s] = load_unit<T>(q, 2 * s + half, a.width, a.vector);
+                gf[s] = load_unit<T>(static_cast<const T*>(f.d_out) + cell, 2 * s + half, a.width, plain);
+                const uint4 o = load_unit<T>(static_cast<const T*>(f.out) + cell, 2 * s + half, a.width, plain);
+                uint4 l = make_uint4(0, 0, 0, 0);
+                if (f.rest) l = load_unit<T>(static_cast<const T*>(f.rest) + cell, 2 * s + half, a.width, plain);
+                const T* x = reinterpret_cast<const T*>(&gf[s]);
+                const T* y = reinterpret_cast<const T*>(&o);
+                const T* z = reinterpret_cast<const T*>(&l);
+#pragma unroll
+                for (int i = 0; i < kPer16<T>; ++i) delta = fmaf(to_f32(x[i]), to_f32(y[i]) + to_f32(z[i]), delta);
+            }
+        }
+        delta = sum_of_halves(delta);
+        const float lse = row_ok ? f.lse[at] : INFINITY;
+        const KeyTiles<KT> tiles(a, first, last);
+        const int wave_row = tile * kRows + wave * 32;
+        const int wave_first = before + position_of(a, min(wave_row, rows - 1));
+        const int wave_last = before + position_of(a, min(wave_row + 31, rows - 1));
+        const bool wave_rows = __ballot(row_ok) != 0;
+        Staged<T, NB, KT> next_k, next_v;
+        bool next_ok = false;
+        auto fetch = [&](int t) {
+            const int key0 = tiles[t] * KT;
+            next_ok = lane < KT && key0 + lane < a.total && (!valid || valid[key0 + lane]);
+            auto from = [&](const T* base, int64_t stride) {
+                return [=](int r) -> const T* {
+                    const int key = key0 + r;
+                    return key < a.total && (!valid || valid[key]) ? base + key * stride : nullptr;
+                };
+            };
+            next_k.load(from(k, a.ks.position), a.width, a.vector);
+            next_v.load(from(v, a.vs.position), a.width, a.vector);
+        };
+        fetch(0);
+        for (int t = 0; t < tiles.count; ++t) {
+            const int key0 = tiles[t] * KT;
+            const uint64_t shown = __ballot(next_ok), every = low_bits(KT);
+            auto whole = [&](int lo, int hi) {  // rows at places lo .. hi see all of the tile
+                return shown == every && key0 + KT - 1 <= lo && (hi - key0 < a.window || key0 + KT <= a.sinks);
+            };
+            __syncthreads();
+            if (!whole(first, last) && next_k.bad()) bad_tile = t;
+            next_k.store(k_tile);
+            next_v.store(v_tile);
+            __syncthreads();
+            if (t + 1 < tiles.count) fetch(t + 1);
+            if (!shown || !wave_rows || key0 > wave_last || (key0 + KT <= wave_first - a.window + 1 && key0 >= a.sinks)) continue;
+            const bool masked = !whole(wave_first, wave_last);
+            const uint64_t seen = !masked ? every : row_ok ? keys_seen(a, place, key0) & shown : 0ull;
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+                f32x16 s = f32x16(0.0f), d = f32x16(0.0f);
+                mma_rows<T, NB>(s, k_tile, kb * 32, qf);
+                mma_rows<T, NB>(d, v_tile, kb * 32, gf);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) d[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse)) * (d[r] - delta);
+                if (masked) {
+                    const uint32_t mine = static_cast<uint32_t>(seen >> (32 * kb)) >> (4 * half);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) d[r] = bit_of(mine, r) ? d[r] : 0.0f;
+                }
+                range.fit(d, acc);
+                if (masked && bad_tile == t)
+                    seen_acc<T, NB>(acc, k_tile, kb * 32, d, static_cast<uint32_t>(seen >> (32 * kb)), scratch[wave]);
+                else
+                    mma_acc<T, NB>(acc, k_tile, kb * 32, d);
+            }
+        }
+    }
+    if (row >= rows) return;
+    if (half == 0) f.delta[at] = delta;
+    if (!f.dq) return;
+    const float by = a.scale * range.back();
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            float x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = row_ok ? acc[n][4 * q + i] * by : 0.0f;
+            store_four(static_cast<T*>(f.dq) + cell, 32 * n + 8 * q + 4 * half, a.width, x);
+        }
+}
+
+// FAR: the sinks' keys against a chunk of the rows past their window, sums to far_parts.
+template <typename T, int NB, bool FAR>
+__global__ __launch_bounds__(kThreads, NB <= 2 ? 2 : 1) void window_dkv_kernel(Backward f) {
+    using L = Tile<T, NB>;
+    constexpr int RT = 32;  // rows of a tile
+    __shared__ __attribute__((aligned(1024))) char q_tile[RT * L::kStride];
+    __shared__ __attribute__((aligned(1024))) char g_tile[RT * L::kStride];
+    __shared__ __attribute__((aligned(16))) float stats[2][RT];  // lse, D
+    __shared__ float scratch[kWaves][32 * 32];
+    __shared__ int bad_tile;
+    const Shape& a = f.s;
+    const int lane = lane_id(), wave = static_cast<int>(threadIdx.x) / kWave, half = lane >> 5, col = lane & 31;
+    int id = by_xcd(static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x));
+    int tile, chunk = 0;
+    if (FAR) {
+        chunk = id % f.far_chunks;
+        id /= f.far_chunks;
+        tile = id % f.far_tiles;
+        id /= f.far_tiles;
+    } else {
+        tile = id % f.key_tiles;
+        id /= f.key_tiles;
+    }
+    const int g = id % a.groups, b = id / a.groups;
+    const int rows = a.length * a.shared, before = a.total - a.length;
+    const int key = tile * kRows + wave * 32 + col;
+    const uint8_t* valid = a.valid ? a.valid + static_cast<int64_t>(b) * a.total : nullptr;
+    const bool key_ok = key < a.total && (!valid || valid[key]) && (!FAR || key < a.sinks);
+    const T* q = static_cast<const T*>(a.q) + b * a.qs.batch + g * a.shared * a.qs.head;
+    const T* k = static_cast<const T*>(a.k) + b * a.ks.batch + key * a.ks.position + g * a.ks.head;
+    const T* v = static_cast<const T*>(a.v) + b * a.vs.batch + key * a.vs.position + g * a.vs.head;
+    const int64_t out_row = static_cast<int64_t>(a.groups) * a.shared * a.width;
+    const T* d_out = static_cast<const T*>(f.d_out) + b * a.length * out_row + static_cast<int64_t>(g) * a.shared * a.width;
+    const int64_t stat = (static_cast<int64_t>(b) * a.groups + g) * rows;
+    if (threadIdx.x == 0) bad_tile = -1;
+
+    uint4 kf[L::kFrags], vf[L::kFrags];
+#pragma unroll
+    for (int s = 0; s < L::kFrags; ++s) {
+        kf[s] = key_ok ? load_unit<T>(k, 2 * s + half, a.width, a.vector) : make_uint4(0, 0, 0, 0);
+        vf[s] = key_ok ? load_unit<T>(v, 2 * s + half, a.width, a.vector) : make_uint4(0, 0, 0, 0);
+    }
+    f32x16 dk[NB], dv[NB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) dk[n] = dv[n] = f32x16(0.0f);
+    Range<T, NB> range;
+    const float c = a.scale * kLog2e;
+    const bool plain = a.width % kPer16<T> == 0;
+    // rows that any key of the workgroup is seen by, and of a wave's keys
+    auto begins = [&](int j) { return max(j - before, 0) * a.shared; };             // first row at or past key j
+    auto ends = [&](int j) { return max(j - before + a.window, 0) * a.shared; };    // first row past its window
+    const int key0 = tile * kRows, wave_key = key0 + wave * 32;
+    int m_first, m_end;
+    if (FAR) {
+        m_first = f.far_first + chunk * f.far_rows;
+        m_end = min(m_first + f.far_rows, rows);
+    } else {
+        m_first = begins(key0);
+        m_end = min(ends(min(key0 + kRows, a.total) - 1), rows);
+    }
+    m_first &= ~(RT - 1);
+    const int own_first = FAR ? f.far_first + chunk * f.far_rows : 0;
+    const bool wave_keys = __ballot(key_ok) != 0, wave_whole = __ballot(key_ok) == ~0ull;
+    const int key_begin = begins(key), key_end = ends(key);
+    const int wave_begin = begins(wave_key), wave_end = ends(wave_key), wave_last_begin = begins(wave_key + 31), wave_last_end = ends(wave_key + 31);
+
+    Staged<T, NB, RT> next_q, next_g;
+    bool next_ok = false;
+    float next_stat = 0.0f;
+    auto fetch = [&](int m0) {
+        auto row_shown = [&](int m) { return m < rows && (!valid || valid[before + position_of(a, m)]); };
+        next_ok = lane < RT && row_shown(m0 + lane);
+        if (threadIdx.x < 2 * RT) {
+            const int m = m0 + (lane & (RT - 1));
+            next_stat = m < rows ? (lane < RT ? f.lse : f.delta)[stat + m] : 0.0f;
+        }
+        next_q.load([&](int r) -> const T* {
+            const int m = m0 + r;
+            if (!row_shown(m)) return nullptr;
+            const int p = position_of(a, m);
+            return q + p * a.qs.position + (m - p * a.shared) * a.qs.head;
+        }, a.width, a.vector);
+        next_g.load([&](int r) -> const T* {
+            const int m = m0 + r;
+            if (!row_shown(m)) return nullptr;
+            const int p = position_of(a, m);
+            return d_out + p * out_row + static_cast<int64_t>(m - p * a.shared) * a.width;
+        }, a.width, plain);
+    };
+    if (m_first < m_end) fetch(m_first);
+    for (int m0 = m_first; m0 < m_end; m0 += RT) {
+        const uint32_t shown = static_cast<uint32_t>(__ballot(next_ok));
+        // every key of the workgroup is seen by every row of the tile
+        const bool all = !FAR && shown == ~0u && !valid && m0 >= begins(key0 + kRows - 1) && m0 + RT <= ends(key0) && key0 + kRows <= a.total;
+        __syncthreads();
+        if (!all && (next_q.bad() || next_g.bad())) bad_tile = m0;
+        next_q.store(q_tile);
+        next_g.store(g_tile);
+        if (threadIdx.x < 2 * RT) stats[lane >> 5][lane & 31] = next_stat;
+        __syncthreads();
+        if (m0 + RT < m_end) fetch(m0 + RT);
+        if (!shown || !wave_keys) continue;
+        if (FAR ? m0 + RT <= wave_end : (m0 + RT <= wave_begin || m0 >= wave_last_end)) continue;
+        const bool masked = FAR || !(shown == ~0u && wave_whole && m0 >= wave_last_begin && m0 + RT <= wave_end);
+        uint32_t seen = ~0u;
+        if (masked) {
+            uint64_t range_seen = FAR ? ~low_bits(max(key_end, own_first) - m0) & low_bits(m_end - m0)
+                                      : ~low_bits(key_begin - m0) & low_bits(key_end - m0);
+            seen = key_ok ? static_cast<uint32_t>(range_seen) & shown : 0u;
+        }
+        f32x16 s = f32x16(0.0f), d = f32x16(0.0f);
+        mma_rows<T, NB>(s, q_tile, 0, kf);
+        mma_rows<T, NB>(d, g_tile, 0, vf);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            const float4 lse = *reinterpret_cast<const float4*>(&stats[0][8 * n + 4 * half]);
+            const float4 del = *reinterpret_cast<const float4*>(&stats[1][8 * n + 4 * half]);
+            const float x[4] = {lse.x, lse.y, lse.z, lse.w}, y[4] = {del.x, del.y, del.z, del.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                s[4 * n + i] = __builtin_amdgcn_exp2f(fmaf(s[4 * n + i], c, kLift<T> - x[i]));
+                d[4 * n + i] = s[4 * n + i] * (d[4 * n + i] - y[i]);
+            }
+        }
+        if (masked) {
+            const uint32_t mine = seen >> (4 * half);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[r] = bit_of(mine, r) ? s[r] : 0.0f;
+                d[r] = bit_of(mine, r) ? d[r] : 0.0f;
+            }
+        }
+        range.fit(d, dk);
+        if (masked && bad_tile == m0) {
+            seen_acc<T, NB>(dv, g_tile, 0, s, seen, scratch[wave]);
+            seen_acc<T, NB>(dk, q_tile, 0, d, seen, scratch[wave]);
+        } else {
+            mma_acc<T, NB>(dv, g_tile, 0, s);
+            mma_acc<T, NB>(dk, q_tile, 0, d);
+        }
+    }
+    const float unlift = std::is_same<T, f16>::value ? 1.0f / 256.0f : 1.0f;
+    const float by = a.scale * range.back() * unlift;
+    const int64_t far_keys = static_cast<int64_t>(f.far_tiles) * kRows;
+    if (FAR) {
+        float* part = f.far_parts + ((((static_cast<int64_t>(chunk) * a.batch + b) * a.groups + g) * far_keys + key) * 2) * a.width;
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int e = 32 * n + 8 * (r / 4) + 4 * half + r % 4;
+                if (e < a.width) part[e] = dk[n][r] * by, part[a.width + e] = dv[n][r] * unlift;
+            }
+        return;
+    }
+    if (key >= a.total) return;
+    const int parts = tile < f.far_tiles ? f.far_chunks : 0;
+    const int64_t cell = ((static_cast<int64_t>(b) * a.total + key) * a.groups + g) * a.width;
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int qd = 0; qd < 4; ++qd) {
+            const int e = 32 * n + 8 * qd + 4 * half;
+            float x[4], y[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = dk[n][4 * qd + i] * by, y[i] = dv[n][4 * qd + i] * unlift;
+            for (int p = 0; p < parts; ++p) {
+                const float* part = f.far_parts + ((((static_cast<int64_t>(p) * a.batch + b) * a.groups + g) * far_keys + key) * 2) * a.width;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (e + i < a.width) x[i] += part[e + i], y[i] += part[a.width + e + i];
+            }
+            if (f.dk) store_four(static_cast<T*>(f.dk) + cell, e, a.width, x);
+            if (f.dv) store_four(static_cast<T*>(f.dv) + cell, e, a.width, y);
+        }
+}
+
+// Rows past the sinks' window, in chunks of about what the other workgroups walk.
+void far_of(const Shape& s, Backward& f) {
+    const int64_t rows = static_cast<int64_t>(s.length) * s.shared, before = s.total - s.length;
+    const int64_t first = std::max<int64_t>(s.window - before, 0) * s.shared;
+    if (s.sinks == 0 || first >= rows) return;
+    f.far_tiles = (s.sinks + kRows - 1) / kRows;
+    f.far_first = static_cast<int>(first);
+    const int64_t per = std::max<int64_t>(static_cast<int64_t>(s.window) * s.shared, 1024);
+    f.far_chunks = static_cast<int>(std::min<int64_t>(64, (rows - first + per - 1) / per));
+    const int64_t each = (rows - first + f.far_chunks - 1) / f.far_chunks;
+    f.far_rows = static_cast<int>((each + 31) / 32 * 32);
+    f.far_chunks = static_cast<int>((rows - first + f.far_rows - 1) / f.far_rows);
+}
+
+size_t far_values(const Shape& s, const Backward& f) {
+    return static_cast<size_t>(f.far_chunks) * s.batch * s.groups * f.far_tiles * kRows * 2 * s.width;
+}
+
+template <typename T, int NB>
+int run(const Backward& f, hipStream_t stream) {
+    const int64_t heads = static_cast<int64_t>(f.s.batch) * f.s.groups;
+    const char* what = "koemi_window_attention_backward";
+    int rc = KOEMI_OK;
+    if (f.row_tiles) {
+        hipLaunchKernelGGL((window_dq_kernel<T, NB>), dim3(static_cast<unsigned>(heads * f.row_tiles)), dim3(kThreads), 0, stream, f);
+        rc = check_launch(what);
+    }
+    if (rc != KOEMI_OK || (!f.dk && !f.dv)) return rc;
+    if (f.far_chunks) {
+        hipLaunchKernelGGL((window_dkv_kernel<T, NB, true>), dim3(static_cast<unsigned>(heads * f.far_tiles * f.far_chunks)),
+                           dim3(kThreads), 0, stream, f);
+        rc = check_launch(what);
+        if (rc != KOEMI_OK) return rc;
+    }
+    hipLaunchKernelGGL((window_dkv_kernel<T, NB, false>), dim3(static_cast<unsigned>(heads * f.key_tiles)), dim3(kThreads), 0, stream, f);
+    return check_launch(what);
+}
+
+template <typename T>
+int by_width(const Backward& f, hipStream_t stream) {
+    const int nb = (f.s.width + 31) / 32;
+    if (nb <= 1) return run<T, 1>(f, stream);
+    if (nb <= 2) return run<T, 2>(f, stream);
+    if (nb <= 3) return run<T, 3>(f, stream);
+    if (nb <= 4) return run<T, 4>(f, stream);
+    if (nb <= 6) return run<T, 6>(f, stream);
+    return run<T, 8>(f, stream);
+}
+
+}  // namespace
+}  // namespace window_attention
+}  // namespace koemi
+
+using namespace koemi;
+using namespace koemi::window_attention;
+
+extern "C" size_t koemi_window_attention_backward_workspace_bytes(int64_t batch, int64_t length, int64_t total, int64_t heads,
+                                                                  int64_t groups, int64_t width, int64_t window, int64_t sinks,
+                                                                  int dtype) {
+    Backward f{};
+    if (shape_of("koemi_window_attention_backward_workspace_bytes", nullptr, nullptr, nullptr, nullptr, nullptr, 0, length, total,
+                 heads, groups, width, window, sinks, 1.0f, dtype, f.s) != KOEMI_OK || batch < 1) {
+        clear_error();
+        return 0;
+    }
+    f.s.batch = static_cast<int>(batch);
+    far_of(f.s, f);
+    return (static_cast<size_t>(batch) * heads * length + far_values(f.s, f)) * 4;
+}
+
+extern "C" int koemi_window_attention_backward(const void* queries, const void* keys, const void* values, const uint8_t* valid,
+                                               const int64_t* strides, const void* output, const void* rest, const float* lse,
+                                               const void* grad_output, void* grad_queries, void* grad_keys, void* grad_values,
+                                               int64_t batch, int64_t length, int64_t total, int64_t heads, int64_t groups,
+                                               int64_t width, int64_t window, int64_t sinks, float scale, int dtype,
+                                               void* workspace, size_t workspace_bytes, koemi_stream_t stream) {
+    clear_error();
+    const char* what = "koemi_window_attention_backward";
+    Backward f{};
+    const int rc = shape_of(what, queries, keys, values, valid, strides, batch, length, total, heads, groups, width, window, sinks,
+                            scale, dtype, f.s);
+    if (rc != KOEMI_OK || batch == 0 || total == 0) return rc;
+    if (length && (!output || !lse || !grad_output)) return fail(KOEMI_ERR_INVALID, "%s: null pointer", what);
+    f.out = output, f.rest = dtype == KOEMI_F32 ? nullptr : rest, f.lse = lse, f.d_out = grad_output, f.dq = grad_queries, f.dk = grad_keys, f.dv = grad_values;
+    f.row_tiles = static_cast<int>((length * f.s.shared + kRows - 1) / kRows);
+    f.key_tiles = static_cast<int>((total + kRows - 1) / kRows);
+    far_of(f.s, f);
+    const size_t cells = static_cast<size_t>(batch) * heads * length;
+    const size_t need = (cells + far_values(f.s, f)) * 4;
+    if (need && (!workspace || workspace_bytes < need)) return fail(KOEMI_ERR_INVALID, "%s: workspace too small", what);
+    f.delta = static_cast<float*>(workspace);
+    f.far_parts = f.delta + cells;
+    if (dtype == KOEMI_F32) return by_width<float>(f, as_stream(stream));
+    if (dtype == KOEMI_F16) return by_width<f16>(f, as_stream(stream));
+    return by_width<bf16>(f, as_stream(stream));
+}

@@ -48,6 +48,8 @@ SOURCES = (
     "gated_recurrence.hip",
     "stream_probe.hip",
     "refine.hip",
+    "window_attention.hip",
+    "window_attention_grad.hip",
 )
 
 ARCH = "gfx950"

@@ -91,6 +91,16 @@ _SIGNATURES: dict[str, tuple[Any, tuple[Any, ...]]] = {
         (_P, _P, _P, _P, _P, _P, _P, _P, c_int64, c_int64, c_int64, _P, c_size_t, _P),
     ),
     "koemi_moe_router_balance_loss": (c_int, (_P, _P, _P, c_int64, _P, _P)),
+    "koemi_window_attention_workspace_bytes": (c_size_t, (c_int64,) * 8 + (c_int,)),
+    "koemi_window_attention_forward": (
+        c_int,
+        (_P,) * 8 + (c_int64,) * 8 + (c_float, c_int, _P, c_size_t, _P),
+    ),
+    "koemi_window_attention_backward_workspace_bytes": (c_size_t, (c_int64,) * 8 + (c_int,)),
+    "koemi_window_attention_backward": (
+        c_int,
+        (_P,) * 12 + (c_int64,) * 8 + (c_float, c_int, _P, c_size_t, _P),
+    ),
     "koemi_stream_read": (c_int, (_P, c_int64, c_int, c_int, c_int64, _P, _P)),
     "koemi_herm_sample_tokens": (c_int, (_P, c_int64, c_int64, c_int64, c_int64, c_float, c_int64, _P, _P, _P, _P)),
     "koemi_moe_check_assignments": (c_int, (_P, c_int, _P, _P, c_int64, c_int64, c_int64, _P)),
