@@ -22,7 +22,7 @@ struct Forward {
     Shape s;
     void* out;
     void* rest;       // what 16-bit outputs are rounded off by, in their type, or null
-    float* lse;       // [batch, groups, length * shared] or null
+    float* lse;       // [batch, heads, length] or null
     float* parts;     // one of several parts of the keys: [parts, batch, groups, rows, width] sums, null for one part
     float* part_lse;  // [parts, batch, groups, rows]
     int row_tiles, splits;
@@ -82,15 +82,11 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void window_forward_kern
         auto fetch = [&](int t) {
             const int key0 = tiles[t] * KT;
             next_ok = lane < KT && key0 + lane < a.total && (!valid || valid[key0 + lane]);
-            auto from = [&](const T* base, int64_t stride) {
-                return [=](int r) -> const T* {
-                    const int key = key0 + r;
-                    return key < a.total && (!valid || valid[key]) ? base + key * stride : nullptr;
-                };
-            };
-            next_k.load(from(k, a.ks.position), a.width, a.vector);
-            next_v.load(from(v, a.vs.position), a.width, a.vector);
+            next_k.load(k + key0 * a.ks.position, a.ks.position, a.total - key0, a.width, a.vector);
+            next_v.load(v + key0 * a.vs.position, a.vs.position, a.total - key0, a.width, a.vector);
         };
+        next_k.prepare(a.ks.position, a.width);
+        next_v.prepare(a.vs.position, a.width);
         if (t0 < t1) fetch(t0);
         for (int t = t0; t < t1; ++t) {
             const int key0 = tiles[t] * KT;
@@ -99,7 +95,10 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void window_forward_kern
                 return shown == every && key0 + KT - 1 <= lo && (hi - key0 < a.window || key0 + KT <= a.sinks);
             };
             __syncthreads();
-            if (!whole(first, last) && next_v.bad()) bad_tile = t;
+            if (!whole(first, last)) {
+                next_k.keep(shown);
+                if (next_v.keep(shown)) bad_tile = t;
+            }
             next_k.store(k_tile);
             next_v.store(v_tile);
             __syncthreads();
@@ -158,9 +157,9 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void window_forward_kern
     const bool none = sum == 0.0f || !row_ok;  // nothing seen: zeros (a masked row's sums are of a zero query)
     const float invert = none ? 0.0f : 1.0f / sum;
     const float lse = none ? INFINITY : top * c - kLift<T> + __builtin_amdgcn_logf(sum);
-    const int64_t at = (static_cast<int64_t>(b) * a.groups + g) * rows + row;
+    const int64_t at = (static_cast<int64_t>(b) * a.groups * a.shared + head) * a.length + position;
     if (f.parts) {
-        const int64_t cell = at + static_cast<int64_t>(split) * a.batch * a.groups * rows;
+        const int64_t cell = (static_cast<int64_t>(b) * a.groups + g) * rows + row + static_cast<int64_t>(split) * a.batch * a.groups * rows;
         if (half == 0) f.part_lse[cell] = lse;
         float* o = f.parts + cell * a.width;
 #pragma unroll
@@ -210,10 +209,10 @@ __global__ __launch_bounds__(kThreads) void window_join_kernel(Forward f) {
         if (x != INFINITY) sum += __builtin_amdgcn_exp2f(x - top);
     }
     const float invert = sum == 0.0f ? 0.0f : 1.0f / sum;
-    if (f.lse && lane == 0) f.lse[cell] = sum == 0.0f ? INFINITY : top + __builtin_amdgcn_logf(sum);
     const int64_t row = cell % rows, g = cell / rows % a.groups, b = cell / rows / a.groups;
-    T* o = static_cast<T*>(f.out) +
-           ((b * a.length + row / a.shared) * a.groups * a.shared + g * a.shared + row % a.shared) * a.width;
+    const int64_t position = row / a.shared, head = g * a.shared + row % a.shared, heads = static_cast<int64_t>(a.groups) * a.shared;
+    if (f.lse && lane == 0) f.lse[(b * heads + head) * a.length + position] = sum == 0.0f ? INFINITY : top + __builtin_amdgcn_logf(sum);
+    T* o = static_cast<T*>(f.out) + ((b * a.length + position) * heads + head) * a.width;
     for (int d = lane; d < a.width; d += kWave) {
         float x = 0.0f;
         for (int p = 0; p < f.splits; ++p) {
@@ -289,7 +288,8 @@ int shape_of(const char* what, const void* queries, const void* keys, const void
         s.ks = {strides[3], strides[4], strides[5]};
         s.vs = {strides[6], strides[7], strides[8]};
         bool aligned = width * size % 16 == 0;
-        for (int i = 0; i < 9; ++i) aligned = aligned && strides[i] * size % 16 == 0;
+        for (int i = 0; i < 9; ++i) aligned = aligned && strides[i] * size % 16 == 0 && strides[i] >= 0;
+        for (int i = 1; i < 9; i += 3) aligned = aligned && strides[i] * size < (1 << 24);
         for (const void* p : {queries, keys, values}) aligned = aligned && reinterpret_cast<uintptr_t>(p) % 16 == 0;
         s.vector = aligned;
     }

@@ -47,7 +47,7 @@ struct Shape {
     float scale;        // of the scores
     uint32_t magic;     // rows / shared = (rows * magic >> 32) >> shift, rows below 2^31
     int shift;
-    int vector;         // rows are whole, aligned 16-byte pieces
+    int vector;         // rows are whole, aligned 16-byte pieces, less than 2^24 bytes apart
 };
 
 // The position of row m, and its head among those that share.
@@ -105,39 +105,58 @@ __device__ __forceinline__ uint4 load_unit(const T* row, int unit, int width, bo
     return out;
 }
 
-// A tile's rows on their way from memory to LDS. row(i) gives row i's address, null for zeros.
+// A tile's rows on their way from memory to LDS: each thread brings the same pieces of
+// every tile, at offsets that it forms once (vector: a row's stride is below 2^24 bytes).
 template <typename T, int NB, int ROWS>
 struct Staged {
     using L = Tile<T, NB>;
     static constexpr int kPieces = ROWS * L::kUnits;
     static constexpr int kEach = (kPieces + kThreads - 1) / kThreads;
+    static constexpr bool kEven = kThreads % L::kUnits == 0;  // a thread's pieces are one unit of rows a fixed step apart
+    static constexpr uint32_t kNone = ~0u;
     uint4 piece[kEach];
+    uint32_t off[kEven ? 1 : kEach];
 
-    template <typename Row>
-    __device__ __forceinline__ void load(Row row, int width, bool vector) {
+    static __device__ __forceinline__ int row(int n) { return (static_cast<int>(threadIdx.x) + n * kThreads) / L::kUnits; }
+    static __device__ __forceinline__ int unit(int n) { return (static_cast<int>(threadIdx.x) + n * kThreads) % L::kUnits; }
+    __device__ __forceinline__ void prepare(int64_t stride, int width) {
 #pragma unroll
-        for (int n = 0; n < kEach; ++n) {
-            const int i = static_cast<int>(threadIdx.x) + n * kThreads;
-            piece[n] = make_uint4(0, 0, 0, 0);
-            if (kPieces % kThreads == 0 || i < kPieces) {
-                const T* p = row(i / L::kUnits);
-                if (p) piece[n] = load_unit<T>(p, i % L::kUnits, width, vector);
+        for (int n = 0; n < (kEven ? 1 : kEach); ++n)
+            off[n] = row(n) < ROWS && unit(n) * kPer16<T> < width
+                         ? row(n) * static_cast<uint32_t>(stride * static_cast<int64_t>(sizeof(T))) + unit(n) * 16 : kNone;
+    }
+    // Rows 0 .. count - 1 of the tile from `first`, a uniform address; the others are zeros.
+    __device__ __forceinline__ void load(const T* first, int64_t stride, int count, int width, bool vector) {
+        if (vector && count >= ROWS) {
+#pragma unroll
+            for (int n = 0; n < kEach; ++n) {
+                const char* from = reinterpret_cast<const char*>(kEven ? first + n * (kThreads / L::kUnits) * stride : first);
+                const uint32_t at = off[kEven ? 0 : n];
+                piece[n] = make_uint4(0, 0, 0, 0);
+                if (at != kNone) piece[n] = *reinterpret_cast<const uint4*>(from + at);
+            }
+        } else {
+#pragma unroll
+            for (int n = 0; n < kEach; ++n) {
+                piece[n] = make_uint4(0, 0, 0, 0);
+                if (row(n) < min(count, ROWS)) piece[n] = load_unit<T>(first + row(n) * stride, unit(n), width, vector);
             }
         }
     }
-    __device__ __forceinline__ void store(char* tile) const {
+    // Zeros for the rows without a bit; true if what is left holds an infinity or NaN.
+    __device__ __forceinline__ bool keep(uint64_t rows) {
+        bool bad = false;
 #pragma unroll
         for (int n = 0; n < kEach; ++n) {
-            const int i = static_cast<int>(threadIdx.x) + n * kThreads;
-            if (kPieces % kThreads == 0 || i < kPieces)
-                *reinterpret_cast<uint4*>(tile + L::at(i / L::kUnits, i % L::kUnits)) = piece[n];
+            if (!((rows >> (row(n) & 63)) & 1ull)) piece[n] = make_uint4(0, 0, 0, 0);
+            bad |= any_nonfinite<T>(piece[n]);
         }
+        return bad;
     }
-    __device__ __forceinline__ bool bad() const {
-        bool b = false;
+    __device__ __forceinline__ void store(char* tile) const {
 #pragma unroll
-        for (int n = 0; n < kEach; ++n) b |= any_nonfinite<T>(piece[n]);
-        return b;
+        for (int n = 0; n < kEach; ++n)
+            if (kPieces % kThreads == 0 || row(n) < ROWS) *reinterpret_cast<uint4*>(tile + L::at(row(n), unit(n))) = piece[n];
     }
 };
 

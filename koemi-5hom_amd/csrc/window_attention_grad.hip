@@ -24,13 +24,13 @@ struct Backward {
     const void* rest;   // what out was rounded off by, or null: D is a small difference of large terms
     const void* d_out;  // each [batch, length, heads, width]
     const float* lse;
-    float* delta;       // D: [batch, groups, rows]
+    float* delta;       // D: [batch, heads, length]
     void* dq;
     void* dk;
     void* dv;
-    float* far_parts;   // [chunks, batch, groups, 128 x far_tiles keys, 2, width]
+    float* far_parts;   // [chunks, batch, groups, 32 x far_tiles keys, 2, width]
     int row_tiles, key_tiles;
-    int far_tiles, far_chunks, far_first, far_rows;  // sinks' key tiles; rows past their window: first, and of a chunk
+    int far_tiles, far_chunks, far_first, far_rows;  // tiles of 32 sinks; positions past their window: first, and of a chunk
 };
 
 template <typename T> constexpr int kKeys = sizeof(T) == 4 ? 32 : 64;  // of a tile that dq walks
@@ -89,7 +89,7 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void window_dq_kernel(Ba
     const int first = before + position_of(a, tile * kRows), last = before + position_of(a, last_row);
     const uint8_t* valid = a.valid ? a.valid + static_cast<int64_t>(b) * a.total : nullptr;
     const bool row_ok = row < rows && (!valid || valid[place]);
-    const int64_t at = (static_cast<int64_t>(b) * a.groups + g) * rows + row;
+    const int64_t at = (static_cast<int64_t>(b) * a.groups * a.shared + head) * a.length + position;
     const int64_t cell = ((static_cast<int64_t>(b) * a.length + position) * a.groups * a.shared + head) * a.width;
     if (threadIdx.x == 0) bad_tile = -1, any_row = 0;
     __syncthreads();
@@ -136,15 +136,11 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void window_dq_kernel(Ba
         auto fetch = [&](int t) {
             const int key0 = tiles[t] * KT;
             next_ok = lane < KT && key0 + lane < a.total && (!valid || valid[key0 + lane]);
-            auto from = [&](const T* base, int64_t stride) {
-                return [=](int r) -> const T* {
-                    const int key = key0 + r;
-                    return key < a.total && (!valid || valid[key]) ? base + key * stride : nullptr;
-                };
-            };
-            next_k.load(from(k, a.ks.position), a.width, a.vector);
-            next_v.load(from(v, a.vs.position), a.width, a.vector);
+            next_k.load(k + key0 * a.ks.position, a.ks.position, a.total - key0, a.width, a.vector);
+            next_v.load(v + key0 * a.vs.position, a.vs.position, a.total - key0, a.width, a.vector);
         };
+        next_k.prepare(a.ks.position, a.width);
+        next_v.prepare(a.vs.position, a.width);
         fetch(0);
         for (int t = 0; t < tiles.count; ++t) {
             const int key0 = tiles[t] * KT;
@@ -153,7 +149,10 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void window_dq_kernel(Ba
                 return shown == every && key0 + KT - 1 <= lo && (hi - key0 < a.window || key0 + KT <= a.sinks);
             };
             __syncthreads();
-            if (!whole(first, last) && next_k.bad()) bad_tile = t;
+            if (!whole(first, last)) {
+                next_v.keep(shown);
+                if (next_k.keep(shown)) bad_tile = t;
+            }
             next_k.store(k_tile);
             next_v.store(v_tile);
             __syncthreads();
@@ -196,13 +195,15 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void window_dq_kernel(Ba
         }
 }
 
-// FAR: the sinks' keys against a chunk of the rows past their window, sums to far_parts.
+// The rows of one head after another, in tiles of 64 positions (fp32: 32). FAR: the sinks'
+// keys against a chunk of the positions past their window: the waves share 32 keys and take the
+// tiles in turn, and their sums, added in order, go to far_parts.
 template <typename T, int NB, bool FAR>
 __global__ __launch_bounds__(kThreads, NB <= 2 ? 2 : 1) void window_dkv_kernel(Backward f) {
     using L = Tile<T, NB>;
-    constexpr int RT = 32;  // rows of a tile
-    __shared__ __attribute__((aligned(1024))) char q_tile[RT * L::kStride];
-    __shared__ __attribute__((aligned(1024))) char g_tile[RT * L::kStride];
+    constexpr int RT = kKeys<T>, RB = RT / 32;
+    __shared__ __attribute__((aligned(1024))) char tiles[2 * RT * L::kStride];
+    char *const q_tile = tiles, *const g_tile = tiles + RT * L::kStride;
     __shared__ __attribute__((aligned(16))) float stats[2][RT];  // lse, D
     __shared__ float scratch[kWaves][32 * 32];
     __shared__ int bad_tile;
@@ -220,8 +221,8 @@ __global__ __launch_bounds__(kThreads, NB <= 2 ? 2 : 1) void window_dkv_kernel(B
         id /= f.key_tiles;
     }
     const int g = id % a.groups, b = id / a.groups;
-    const int rows = a.length * a.shared, before = a.total - a.length;
-    const int key = tile * kRows + wave * 32 + col;
+    const int before = a.total - a.length;
+    const int wave_key = FAR ? tile * 32 : tile * kRows + wave * 32, key = wave_key + col;
     const uint8_t* valid = a.valid ? a.valid + static_cast<int64_t>(b) * a.total : nullptr;
     const bool key_ok = key < a.total && (!valid || valid[key]) && (!FAR || key < a.sinks);
     const T* q = static_cast<const T*>(a.q) + b * a.qs.batch + g * a.shared * a.qs.head;
@@ -229,7 +230,7 @@ __global__ __launch_bounds__(kThreads, NB <= 2 ? 2 : 1) void window_dkv_kernel(B
     const T* v = static_cast<const T*>(a.v) + b * a.vs.batch + key * a.vs.position + g * a.vs.head;
     const int64_t out_row = static_cast<int64_t>(a.groups) * a.shared * a.width;
     const T* d_out = static_cast<const T*>(f.d_out) + b * a.length * out_row + static_cast<int64_t>(g) * a.shared * a.width;
-    const int64_t stat = (static_cast<int64_t>(b) * a.groups + g) * rows;
+    const int64_t stat = (static_cast<int64_t>(b) * a.groups + g) * a.shared * a.length;
     if (threadIdx.x == 0) bad_tile = -1;
 
     uint4 kf[L::kFrags], vf[L::kFrags];
@@ -243,116 +244,135 @@ __global__ __launch_bounds__(kThreads, NB <= 2 ? 2 : 1) void window_dkv_kernel(B
     for (int n = 0; n < NB; ++n) dk[n] = dv[n] = f32x16(0.0f);
     Range<T, NB> range;
     const float c = a.scale * kLog2e;
-    const bool plain = a.width % kPer16<T> == 0;
-    // rows that any key of the workgroup is seen by, and of a wave's keys
-    auto begins = [&](int j) { return max(j - before, 0) * a.shared; };             // first row at or past key j
-    auto ends = [&](int j) { return max(j - before + a.window, 0) * a.shared; };    // first row past its window
-    const int key0 = tile * kRows, wave_key = key0 + wave * 32;
-    int m_first, m_end;
+    const bool plain = a.width % kPer16<T> == 0 && out_row * static_cast<int64_t>(sizeof(T)) < (1 << 24);
+    // queries that see key j: from begins(j) on, up to ends(j)
+    auto begins = [&](int j) { return max(j - before, 0); };
+    auto ends = [&](int j) { return max(j - before + a.window, 0); };
+    const int key0 = tile * kRows;
+    int from, to;
     if (FAR) {
-        m_first = f.far_first + chunk * f.far_rows;
-        m_end = min(m_first + f.far_rows, rows);
+        from = f.far_first + chunk * f.far_rows;
+        to = min(from + f.far_rows, a.length);
     } else {
-        m_first = begins(key0);
-        m_end = min(ends(min(key0 + kRows, a.total) - 1), rows);
+        from = begins(key0);
+        to = min(ends(min(key0 + kRows, a.total) - 1), a.length);
     }
-    m_first &= ~(RT - 1);
-    const int own_first = FAR ? f.far_first + chunk * f.far_rows : 0;
     const bool wave_keys = __ballot(key_ok) != 0, wave_whole = __ballot(key_ok) == ~0ull;
     const int key_begin = begins(key), key_end = ends(key);
-    const int wave_begin = begins(wave_key), wave_end = ends(wave_key), wave_last_begin = begins(wave_key + 31), wave_last_end = ends(wave_key + 31);
+    const int wave_begin = begins(wave_key), wave_end = ends(wave_key);
+    const int wave_last_begin = begins(wave_key + 31), wave_last_end = ends(wave_key + 31);
+    const int first = from & ~(RT - 1), walk = to > from ? (to - first + RT - 1) / RT : 0, steps = walk * a.shared;
 
     Staged<T, NB, RT> next_q, next_g;
     bool next_ok = false;
     float next_stat = 0.0f;
-    auto fetch = [&](int m0) {
-        auto row_shown = [&](int m) { return m < rows && (!valid || valid[before + position_of(a, m)]); };
-        next_ok = lane < RT && row_shown(m0 + lane);
+    next_q.prepare(a.qs.position, a.width);
+    next_g.prepare(out_row, a.width);
+    int next_head = 0, next_p = first;  // of the tile to fetch
+    auto fetch = [&]() {
+        const int p0 = next_p;
+        next_ok = lane < RT && p0 + lane < a.length && (!valid || valid[before + p0 + lane]);
         if (threadIdx.x < 2 * RT) {
-            const int m = m0 + (lane & (RT - 1));
-            next_stat = m < rows ? (lane < RT ? f.lse : f.delta)[stat + m] : 0.0f;
+            const int r = static_cast<int>(threadIdx.x) % RT;
+            next_stat = p0 + r < a.length
+                            ? (static_cast<int>(threadIdx.x) < RT ? f.lse : f.delta)[stat + static_cast<int64_t>(next_head) * a.length + p0 + r]
+                            : 0.0f;
         }
-        next_q.load([&](int r) -> const T* {
-            const int m = m0 + r;
-            if (!row_shown(m)) return nullptr;
-            const int p = position_of(a, m);
-            return q + p * a.qs.position + (m - p * a.shared) * a.qs.head;
-        }, a.width, a.vector);
-        next_g.load([&](int r) -> const T* {
-            const int m = m0 + r;
-            if (!row_shown(m)) return nullptr;
-            const int p = position_of(a, m);
-            return d_out + p * out_row + static_cast<int64_t>(m - p * a.shared) * a.width;
-        }, a.width, plain);
+        next_q.load(q + next_head * a.qs.head + p0 * a.qs.position, a.qs.position, a.length - p0, a.width, a.vector);
+        next_g.load(d_out + static_cast<int64_t>(next_head) * a.width + p0 * out_row, out_row, a.length - p0, a.width, plain);
+        next_p += RT;
+        if (next_p >= to) next_p = first, ++next_head;
     };
-    if (m_first < m_end) fetch(m_first);
-    for (int m0 = m_first; m0 < m_end; m0 += RT) {
-        const uint32_t shown = static_cast<uint32_t>(__ballot(next_ok));
+    if (steps) fetch();
+    int p0 = first;
+    for (int t = 0; t < steps; ++t, p0 = p0 + RT >= to ? first : p0 + RT) {
+        const uint64_t shown = __ballot(next_ok), every = low_bits(RT);
         // every key of the workgroup is seen by every row of the tile
-        const bool all = !FAR && shown == ~0u && !valid && m0 >= begins(key0 + kRows - 1) && m0 + RT <= ends(key0) && key0 + kRows <= a.total;
+        const bool all = !FAR && shown == every && !valid && p0 >= begins(key0 + kRows - 1) && p0 + RT <= ends(key0) && key0 + kRows <= a.total;
         __syncthreads();
-        if (!all && (next_q.bad() || next_g.bad())) bad_tile = m0;
+        if (!all) {
+            const bool bad_q = next_q.keep(shown), bad_g = next_g.keep(shown);
+            if (bad_q || bad_g) bad_tile = t;
+        }
         next_q.store(q_tile);
         next_g.store(g_tile);
-        if (threadIdx.x < 2 * RT) stats[lane >> 5][lane & 31] = next_stat;
+        if (threadIdx.x < 2 * RT) stats[static_cast<int>(threadIdx.x) / RT][static_cast<int>(threadIdx.x) % RT] = next_stat;
         __syncthreads();
-        if (m0 + RT < m_end) fetch(m0 + RT);
+        if (t + 1 < steps) fetch();
         if (!shown || !wave_keys) continue;
-        if (FAR ? m0 + RT <= wave_end : (m0 + RT <= wave_begin || m0 >= wave_last_end)) continue;
-        const bool masked = FAR || !(shown == ~0u && wave_whole && m0 >= wave_last_begin && m0 + RT <= wave_end);
-        uint32_t seen = ~0u;
+        if (FAR ? (t % kWaves != wave || p0 + RT <= wave_end) : (p0 + RT <= wave_begin || p0 >= wave_last_end)) continue;
+        const bool masked = FAR || !(shown == every && wave_whole && p0 >= wave_last_begin && p0 + RT <= wave_end);
+        uint64_t seen = every;
         if (masked) {
-            uint64_t range_seen = FAR ? ~low_bits(max(key_end, own_first) - m0) & low_bits(m_end - m0)
-                                      : ~low_bits(key_begin - m0) & low_bits(key_end - m0);
-            seen = key_ok ? static_cast<uint32_t>(range_seen) & shown : 0u;
+            const uint64_t by_place = FAR ? ~low_bits(max(key_end, from) - p0) & low_bits(to - p0)
+                                          : ~low_bits(key_begin - p0) & low_bits(key_end - p0);
+            seen = key_ok ? by_place & shown : 0ull;
         }
-        f32x16 s = f32x16(0.0f), d = f32x16(0.0f);
-        mma_rows<T, NB>(s, q_tile, 0, kf);
-        mma_rows<T, NB>(d, g_tile, 0, vf);
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-            const float4 lse = *reinterpret_cast<const float4*>(&stats[0][8 * n + 4 * half]);
-            const float4 del = *reinterpret_cast<const float4*>(&stats[1][8 * n + 4 * half]);
-            const float x[4] = {lse.x, lse.y, lse.z, lse.w}, y[4] = {del.x, del.y, del.z, del.w};
+        for (int rb = 0; rb < RB; ++rb) {
+            f32x16 s = f32x16(0.0f), d = f32x16(0.0f);
+            mma_rows<T, NB>(s, q_tile, rb * 32, kf);
+            mma_rows<T, NB>(d, g_tile, rb * 32, vf);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                s[4 * n + i] = __builtin_amdgcn_exp2f(fmaf(s[4 * n + i], c, kLift<T> - x[i]));
-                d[4 * n + i] = s[4 * n + i] * (d[4 * n + i] - y[i]);
+            for (int n = 0; n < 4; ++n) {
+                const float4 lse = *reinterpret_cast<const float4*>(&stats[0][rb * 32 + 8 * n + 4 * half]);
+                const float4 del = *reinterpret_cast<const float4*>(&stats[1][rb * 32 + 8 * n + 4 * half]);
+                const float x[4] = {lse.x, lse.y, lse.z, lse.w}, y[4] = {del.x, del.y, del.z, del.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[4 * n + i] = __builtin_amdgcn_exp2f(fmaf(s[4 * n + i], c, kLift<T> - x[i]));
+                    d[4 * n + i] = s[4 * n + i] * (d[4 * n + i] - y[i]);
+                }
             }
-        }
-        if (masked) {
-            const uint32_t mine = seen >> (4 * half);
+            const uint32_t block = static_cast<uint32_t>(seen >> (32 * rb));
+            if (masked) {
+                const uint32_t mine = block >> (4 * half);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                s[r] = bit_of(mine, r) ? s[r] : 0.0f;
-                d[r] = bit_of(mine, r) ? d[r] : 0.0f;
+                for (int r = 0; r < 16; ++r) {
+                    s[r] = bit_of(mine, r) ? s[r] : 0.0f;
+                    d[r] = bit_of(mine, r) ? d[r] : 0.0f;
+                }
             }
-        }
-        range.fit(d, dk);
-        if (masked && bad_tile == m0) {
-            seen_acc<T, NB>(dv, g_tile, 0, s, seen, scratch[wave]);
-            seen_acc<T, NB>(dk, q_tile, 0, d, seen, scratch[wave]);
-        } else {
-            mma_acc<T, NB>(dv, g_tile, 0, s);
-            mma_acc<T, NB>(dk, q_tile, 0, d);
+            range.fit(d, dk);
+            if (masked && bad_tile == t) {
+                seen_acc<T, NB>(dv, g_tile, rb * 32, s, block, scratch[wave]);
+                seen_acc<T, NB>(dk, q_tile, rb * 32, d, block, scratch[wave]);
+            } else {
+                mma_acc<T, NB>(dv, g_tile, rb * 32, s);
+                mma_acc<T, NB>(dk, q_tile, rb * 32, d);
+            }
         }
     }
     const float unlift = std::is_same<T, f16>::value ? 1.0f / 256.0f : 1.0f;
     const float by = a.scale * range.back() * unlift;
-    const int64_t far_keys = static_cast<int64_t>(f.far_tiles) * kRows;
+    const int64_t far_keys = static_cast<int64_t>(f.far_tiles) * 32;
     if (FAR) {
-        float* part = f.far_parts + ((((static_cast<int64_t>(chunk) * a.batch + b) * a.groups + g) * far_keys + key) * 2) * a.width;
+        // [32 keys][2][32 NB] floats fill the tiles' LDS
+        static_assert(2 * RT * L::kStride >= 32 * 2 * 32 * NB * 4, "the waves' sums need the tiles' room");
+        float* sums = reinterpret_cast<float*>(tiles);
+        for (int w = 0; w < kWaves; ++w) {
+            __syncthreads();
+            if (w != wave) continue;
 #pragma unroll
-        for (int n = 0; n < NB; ++n)
+            for (int n = 0; n < NB; ++n)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int e = 32 * n + 8 * (r / 4) + 4 * half + r % 4;
-                if (e < a.width) part[e] = dk[n][r] * by, part[a.width + e] = dv[n][r] * unlift;
-            }
+                for (int r = 0; r < 16; ++r) {
+                    float* x = sums + col * (64 * NB) + 32 * n + 8 * (r / 4) + 4 * half + r % 4;
+                    const float k0 = w ? x[0] : 0.0f, v0 = w ? x[32 * NB] : 0.0f;
+                    x[0] = k0 + dk[n][r] * by;
+                    x[32 * NB] = v0 + dv[n][r] * unlift;
+                }
+        }
+        __syncthreads();
+        float* part = f.far_parts + (((static_cast<int64_t>(chunk) * a.batch + b) * a.groups + g) * far_keys + wave_key) * 2 * a.width;
+        for (int i = threadIdx.x; i < 64 * a.width; i += kThreads) {
+            const int line = i / a.width;
+            part[i] = sums[line * 32 * NB + i - line * a.width];
+        }
         return;
     }
     if (key >= a.total) return;
-    const int parts = tile < f.far_tiles ? f.far_chunks : 0;
+    const float* far = f.far_parts + (((static_cast<int64_t>(b) * a.groups + g) * far_keys + key) * 2) * a.width;
     const int64_t cell = ((static_cast<int64_t>(b) * a.total + key) * a.groups + g) * a.width;
 #pragma unroll
     for (int n = 0; n < NB; ++n)
@@ -362,34 +382,43 @@ __global__ __launch_bounds__(kThreads, NB <= 2 ? 2 : 1) void window_dkv_kernel(B
             float x[4], y[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[i] = dk[n][4 * qd + i] * by, y[i] = dv[n][4 * qd + i] * unlift;
-            for (int p = 0; p < parts; ++p) {
-                const float* part = f.far_parts + ((((static_cast<int64_t>(p) * a.batch + b) * a.groups + g) * far_keys + key) * 2) * a.width;
+            if (key < far_keys) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (e + i < a.width) x[i] += part[e + i], y[i] += part[a.width + e + i];
+                    if (e + i < a.width) x[i] += far[e + i], y[i] += far[a.width + e + i];
             }
             if (f.dk) store_four(static_cast<T*>(f.dk) + cell, e, a.width, x);
             if (f.dv) store_four(static_cast<T*>(f.dv) + cell, e, a.width, y);
         }
 }
 
-// Rows past the sinks' window, in chunks of about what the other workgroups walk.
-void far_of(const Shape& s, Backward& f) {
-    const int64_t rows = static_cast<int64_t>(s.length) * s.shared, before = s.total - s.length;
-    const int64_t first = std::max<int64_t>(s.window - before, 0) * s.shared;
-    if (s.sinks == 0 || first >= rows) return;
-    f.far_tiles = (s.sinks + kRows - 1) / kRows;
-    f.far_first = static_cast<int>(first);
-    const int64_t per = std::max<int64_t>(static_cast<int64_t>(s.window) * s.shared, 1024);
-    f.far_chunks = static_cast<int>(std::min<int64_t>(64, (rows - first + per - 1) / per));
-    const int64_t each = (rows - first + f.far_chunks - 1) / f.far_chunks;
-    f.far_rows = static_cast<int>((each + 31) / 32 * 32);
-    f.far_chunks = static_cast<int>((rows - first + f.far_rows - 1) / f.far_rows);
+// The chunks' sums of the sinks' keys, added in order into the first chunk's.
+__global__ __launch_bounds__(kThreads) void window_far_kernel(float* parts, int chunks, int64_t each) {
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+    if (i >= each) return;
+    float sum = parts[i];
+#pragma unroll 8
+    for (int p = 1; p < chunks; ++p) sum += parts[p * each + i];
+    parts[i] = sum;
 }
 
-size_t far_values(const Shape& s, const Backward& f) {
-    return static_cast<size_t>(f.far_chunks) * s.batch * s.groups * f.far_tiles * kRows * 2 * s.width;
+// Positions past the sinks' window, in chunks: two workgroups for each compute unit where
+// the rows suffice, none under four tiles.
+void far_of(const Shape& s, Backward& f) {
+    const int64_t before = s.total - s.length, first = std::max<int64_t>(s.window - before, 0);
+    if (s.sinks == 0 || first >= s.length) return;
+    f.far_tiles = (s.sinks + 31) / 32;
+    f.far_first = static_cast<int>(first);
+    const int64_t span = s.length - first, heads = static_cast<int64_t>(s.batch) * s.groups * f.far_tiles;
+    const int64_t chunks = std::max<int64_t>(1, std::min<int64_t>((span + 255) / 256, (512 + heads - 1) / heads));
+    f.far_rows = static_cast<int>(((span + chunks - 1) / chunks + 63) / 64 * 64);
+    f.far_chunks = static_cast<int>((span + f.far_rows - 1) / f.far_rows);
 }
+
+int64_t far_each(const Shape& s, const Backward& f) {
+    return static_cast<int64_t>(s.batch) * s.groups * f.far_tiles * 32 * 2 * s.width;
+}
+size_t far_values(const Shape& s, const Backward& f) { return static_cast<size_t>(f.far_chunks) * far_each(s, f); }
 
 template <typename T, int NB>
 int run(const Backward& f, hipStream_t stream) {
@@ -406,6 +435,12 @@ int run(const Backward& f, hipStream_t stream) {
                            dim3(kThreads), 0, stream, f);
         rc = check_launch(what);
         if (rc != KOEMI_OK) return rc;
+        if (f.far_chunks > 1) {
+            const int64_t each = far_each(f.s, f);
+            hipLaunchKernelGGL(window_far_kernel, dim3(grid_for(each, kThreads)), dim3(kThreads), 0, stream, f.far_parts, f.far_chunks, each);
+            rc = check_launch(what);
+            if (rc != KOEMI_OK) return rc;
+        }
     }
     hipLaunchKernelGGL((window_dkv_kernel<T, NB, false>), dim3(static_cast<unsigned>(heads * f.key_tiles)), dim3(kThreads), 0, stream, f);
     return check_launch(what);

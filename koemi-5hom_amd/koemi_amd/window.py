@@ -135,7 +135,7 @@ class _WindowAttention(torch.autograd.Function):
         mask = valid_mask.contiguous() if valid_mask is not None else None
         output = torch.empty((batch, length, heads, width), device=device, dtype=queries.dtype)
         rest = torch.empty_like(output) if trained and queries.dtype != torch.float32 else None
-        lse = torch.empty((batch, length * heads), device=device, dtype=torch.float32) if trained else None
+        lse = torch.empty((batch, heads, length), device=device, dtype=torch.float32) if trained else None
         shape = (batch, length, total, heads, groups, width, window, sinks)
         need = _workspace_bytes(*shape, code)[0]
         workspace = _bytes(need, device)
