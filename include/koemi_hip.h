@@ -1049,6 +1049,43 @@ int koemi_window_attention_backward(const void* queries, const void* keys, const
                                     int64_t sinks, float scale, int dtype, void* workspace, size_t workspace_bytes,
                                     koemi_stream_t stream);
 
+/* The 8-bit cache of that attention for single positions: the first `sinks` entries of a
+ * row and a ring of its last `window` others (LocalKeyValueMemory.tail, model/memory.py:385-403,
+ * with heads and in 8 bits). keys, values: codes [batch, groups, window + sinks, stored], stored
+ * being width rounded up to 32, zeros behind it, 16-byte aligned; key_scales,
+ * value_scales [batch, groups, window + sinks] fp32; code 0 int8, 1 e4m3 (OCP). Entry p lies
+ * at slot p < sinks ? p : sinks + (p - sinks) mod window. A row x is held as x / scale
+ * rounded to nearest even, scale = max(max |x| times 1 / 127 or
+ * 1 / 448 in fp32, 2^-126); one that is not
+ * finite as codes 0 with a NaN scale. lengths [batch] int64: the entries that a row holds before
+ * the call (the caller advances them); a negative one takes no part.
+ *
+ * _write appends the first counts[b] (NULL: all) of `length` new rows [batch, length, groups,
+ * width]; strides: six on the host (batch, position, head of new keys, new values). _entries
+ * gives the sinks and the last `window` entries, in their order and at the end of
+ * [batch, window + sinks, groups, width] (16-byte aligned), as the values they stand for, and
+ * present [batch, window + sinks]; absent places hold zeros. _step appends one row [batch,
+ * groups, width] (NULL keys and values: none) and answers queries [batch, heads, width] from
+ * what the row then holds: output [batch, heads, width], zeros for a row that holds nothing
+ * or has 0 in active [batch] (NULL: all; nothing is written there either); strides: batch and
+ * head of queries, new keys, new values. dtype: of new rows, queries and results. Workspace of
+ * _step: koemi_window_cache_step_workspace_bytes, no zeroing needed. */
+int koemi_window_cache_write(void* keys, float* key_scales, void* values, float* value_scales, int code,
+                             const void* new_keys, const void* new_values, const int64_t* strides, const int64_t* lengths,
+                             const int64_t* counts, int64_t batch, int64_t length, int64_t groups, int64_t width,
+                             int64_t window, int64_t sinks, int dtype, koemi_stream_t stream);
+int koemi_window_cache_entries(const void* keys, const float* key_scales, const void* values, const float* value_scales,
+                               int code, const int64_t* lengths, void* out_keys, void* out_values, uint8_t* present,
+                               int64_t batch, int64_t groups, int64_t width, int64_t window, int64_t sinks, int dtype,
+                               koemi_stream_t stream);
+size_t koemi_window_cache_step_workspace_bytes(int64_t batch, int64_t heads, int64_t groups, int64_t width, int64_t window,
+                                               int64_t sinks);
+int koemi_window_cache_step(void* keys, float* key_scales, void* values, float* value_scales, int code, const void* queries,
+                            const void* new_keys, const void* new_values, const int64_t* strides, const int64_t* lengths,
+                            const uint8_t* active, void* output, int64_t batch, int64_t heads, int64_t groups, int64_t width,
+                            int64_t window, int64_t sinks, float scale, int dtype, void* workspace, size_t workspace_bytes,
+                            koemi_stream_t stream);
+
 /* Measurement only (no counterpart in the reference): reads `bytes` (a
  * multiple of 16) from `src` with `grid` workgroups of `block` threads, each
  * thread issuing `unroll` (1, 2, 4 or 8) 16-byte loads per pass of a

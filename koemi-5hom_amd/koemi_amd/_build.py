@@ -50,6 +50,7 @@ SOURCES = (
     "refine.hip",
     "window_attention.hip",
     "window_attention_grad.hip",
+    "window_cache.hip",
 )
 
 ARCH = "gfx950"

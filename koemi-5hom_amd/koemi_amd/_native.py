@@ -101,6 +101,19 @@ _SIGNATURES: dict[str, tuple[Any, tuple[Any, ...]]] = {
         c_int,
         (_P,) * 12 + (c_int64,) * 8 + (c_float, c_int, _P, c_size_t, _P),
     ),
+    "koemi_window_cache_write": (
+        c_int,
+        (_P, _P, _P, _P, c_int, _P, _P, _P, _P, _P) + (c_int64,) * 6 + (c_int, _P),
+    ),
+    "koemi_window_cache_entries": (
+        c_int,
+        (_P, _P, _P, _P, c_int, _P, _P, _P, _P) + (c_int64,) * 5 + (c_int, _P),
+    ),
+    "koemi_window_cache_step_workspace_bytes": (c_size_t, (c_int64,) * 6),
+    "koemi_window_cache_step": (
+        c_int,
+        (_P, _P, _P, _P, c_int) + (_P,) * 7 + (c_int64,) * 6 + (c_float, c_int, _P, c_size_t, _P),
+    ),
     "koemi_stream_read": (c_int, (_P, c_int64, c_int, c_int, c_int64, _P, _P)),
     "koemi_herm_sample_tokens": (c_int, (_P, c_int64, c_int64, c_int64, c_int64, c_float, c_int64, _P, _P, _P, _P)),
     "koemi_moe_check_assignments": (c_int, (_P, c_int, _P, _P, c_int64, c_int64, c_int64, _P)),

@@ -3,14 +3,18 @@
 The local memory of the reference reads a sliding window with one head as wide as the
 model (model/memory.py:332-383). ``window_attention`` is that read with heads, for
 prompts and training: position i sees the last ``window`` positions up to its own and the
-first ``sinks`` ones, which stay visible. It runs ``koemi_window_attention_forward`` and
-``koemi_window_attention_backward``; there is no torch fallback.
+first ``sinks`` ones, which stay visible. ``WindowCache`` holds what such a window needs of
+a sequence in 8 bits, for chunks of a prompt (``window_cache_write``,
+``window_cache_entries``) and for single positions (``window_cache_step``,
+``window_cache_read``), as the reference's ring does in full (memory.py:385-403). They run
+``koemi_window_attention_*`` and ``koemi_window_cache_*``; there is no torch fallback.
 """
 
 from __future__ import annotations
 
 import ctypes
 import math
+from dataclasses import dataclass
 from functools import lru_cache
 
 import torch
@@ -20,10 +24,12 @@ from torch.autograd.function import once_differentiable
 from koemi_amd import _native
 from koemi_amd.think import CudaThinkUnavailableError, CudaThinkValidationError
 
-__all__ = ["window_attention"]
+__all__ = ["WindowCache", "window_attention", "window_cache", "window_cache_entries", "window_cache_read",
+           "window_cache_step", "window_cache_write"]
 
 _SUPPORTED_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 _MAX_WIDTH = 256
+_CODES = {torch.int8: 0, torch.float8_e4m3fn: 1}
 
 
 def _whole(name: str, value: object, least: int) -> int:
@@ -169,3 +175,220 @@ class _WindowAttention(torch.autograd.Function):
                          _native.ptr(d_q), _native.ptr(d_k), _native.ptr(d_v), *shape, scale, code,
                          _native.ptr(workspace), need, _native.stream_of(device))
         return d_q, d_k, d_v, None, None, None, None, None
+
+
+@dataclass(frozen=True)
+class WindowCache:
+    """Keys and values of a window and its sinks, in 8 bits.
+
+    ``keys``, ``values``: codes ``[B, G, window + sinks, stored]``, int8 or float8_e4m3fn,
+    ``stored`` being the head width rounded up to 32 (zeros behind it); ``key_scales``,
+    ``value_scales`` ``[B, G, window + sinks]`` float32: an entry's row stands for ``codes *
+    scale``. Entry p of a row lies at slot p, from ``sinks`` on at ``sinks + (p - sinks) %
+    window``. How many entries a row holds is the caller's count, one for all layers. All
+    contiguous; ``window_cache`` makes an empty one.
+    """
+
+    keys: Tensor
+    key_scales: Tensor
+    values: Tensor
+    value_scales: Tensor
+    width: int
+    window: int
+    sinks: int = 0
+
+    def __post_init__(self) -> None:
+        window, sinks = _whole("window", self.window, 1), _whole("sinks", self.sinks, 0)
+        if not 1 <= _whole("width", self.width, 1) <= _MAX_WIDTH:
+            raise CudaThinkValidationError(f"heads must be 1 to {_MAX_WIDTH} wide")
+        tensors = (self.keys, self.key_scales, self.values, self.value_scales)
+        if not all(isinstance(t, Tensor) for t in tensors):
+            raise CudaThinkValidationError("a cache is made of four tensors")
+        shape = self.keys.shape
+        if (self.keys.ndim != 4 or shape[2] != window + sinks or shape[3] != -(-self.width // 32) * 32
+                or self.values.shape != shape or self.key_scales.shape != shape[:3] or self.value_scales.shape != shape[:3]):
+            raise CudaThinkValidationError("a cache's codes must be [batch, key heads, window + sinks, width rounded up to 32] "
+                                           "and its scales [batch, key heads, window + sinks]")
+        if self.keys.dtype not in _CODES or self.values.dtype != self.keys.dtype:
+            raise CudaThinkValidationError("a cache's codes must be int8 or float8_e4m3fn")
+        if self.key_scales.dtype != torch.float32 or self.value_scales.dtype != torch.float32:
+            raise CudaThinkValidationError("a cache's scales must be float32")
+        if any(t.device != self.keys.device for t in tensors) or not all(t.is_contiguous() for t in tensors):
+            raise CudaThinkValidationError("a cache's tensors must be contiguous and on the same device")
+        if self.keys.numel() and (self.keys.data_ptr() % 16 or self.values.data_ptr() % 16):
+            raise CudaThinkValidationError("a cache's codes must be 16-byte aligned")
+
+    def buffers(self) -> tuple[int, int, int, int, int]:
+        """The entry points' first arguments."""
+
+        return (self.keys.data_ptr(), self.key_scales.data_ptr(), self.values.data_ptr(), self.value_scales.data_ptr(),
+                _CODES[self.keys.dtype])
+
+
+def window_cache(batch: int, heads: int, width: int, *, window: int, sinks: int = 0, dtype: torch.dtype = torch.int8,
+                 device: torch.device | str = "cuda") -> WindowCache:
+    """An empty cache of ``heads`` key heads of ``width`` for ``batch`` rows (int8 or float8_e4m3fn codes)."""
+
+    batch, heads, width = _whole("batch", batch, 0), _whole("heads", heads, 1), _whole("width", width, 1)
+    window, sinks = _whole("window", window, 1), _whole("sinks", sinks, 0)
+    if dtype not in _CODES:
+        raise CudaThinkValidationError("a cache's codes must be int8 or float8_e4m3fn")
+    if width > _MAX_WIDTH:
+        raise CudaThinkValidationError(f"heads must be 1 to {_MAX_WIDTH} wide")
+    shape = (batch, heads, window + sinks)
+
+    def codes() -> Tensor:
+        return torch.zeros((*shape, -(-width // 32) * 32), device=device, dtype=torch.int8).view(dtype)
+
+    return WindowCache(codes(), torch.zeros(shape, device=device), codes(), torch.zeros(shape, device=device),
+                       width=width, window=window, sinks=sinks)
+
+
+def _check_cache(cache: object) -> WindowCache:
+    if not isinstance(cache, WindowCache):
+        raise CudaThinkValidationError("cache must be a WindowCache")
+    if cache.keys.device.type != "cuda":
+        raise CudaThinkValidationError("cache must be on CUDA")
+    return cache
+
+
+def _check_rows(cache: WindowCache, name: str, tensor: object, shape: tuple[int, ...], dtype: torch.dtype | None) -> None:
+    """A tensor of rows of the cache's heads in one of the three types."""
+
+    if not isinstance(tensor, Tensor):
+        raise CudaThinkValidationError(f"{name} must be a torch.Tensor")
+    if tensor.shape != shape:
+        raise CudaThinkValidationError(f"{name} must have shape {list(shape)}")
+    if tensor.dtype not in _SUPPORTED_DTYPES or (dtype is not None and tensor.dtype != dtype):
+        raise CudaThinkValidationError(f"{name} must be float32, float16 or bfloat16, one type for all")
+    if tensor.device != cache.keys.device:
+        raise CudaThinkValidationError(f"{name} must be on the cache's device")
+
+
+def _check_counts(cache: WindowCache, name: str, tensor: object) -> Tensor:
+    batch = cache.keys.shape[0]
+    if not isinstance(tensor, Tensor) or tensor.dtype != torch.int64 or tensor.shape != (batch,) \
+            or tensor.device != cache.keys.device:
+        raise CudaThinkValidationError(f"{name} must be an int64 [batch] tensor on the cache's device")
+    return tensor.contiguous()
+
+
+def _in_rows(tensor: Tensor) -> Tensor:
+    return tensor if tensor.stride(-1) == 1 or tensor.shape[-1] == 1 else tensor.contiguous()
+
+
+def window_cache_write(cache: WindowCache, keys: Tensor, values: Tensor, lengths: Tensor, counts: Tensor | None = None) -> None:
+    """Append rows to the cache, in place.
+
+    ``keys``, ``values`` ``[B, L, G, D]`` (float32, float16 or bfloat16, any strides);
+    ``lengths`` ``[B]`` int64: the entries that each row holds already (the caller
+    adds what was appended afterwards; a row with a negative one is left as it is);
+    ``counts`` ``[B]`` int64: how many of the L each row appends, from the first on (all, when
+    omitted; what the others hold does not matter). Of more rows than the ring holds the last
+    ones stay. A row's largest absolute value gets the largest code; codes are rounded to
+    nearest even; a row that is not finite stands for NaN.
+    """
+
+    cache = _check_cache(cache)
+    batch, groups = cache.keys.shape[:2]
+    length = keys.shape[1] if isinstance(keys, Tensor) and keys.ndim == 4 else -1
+    _check_rows(cache, "keys", keys, (batch, max(length, 0), groups, cache.width), None)
+    _check_rows(cache, "values", values, (batch, length, groups, cache.width), keys.dtype)
+    lengths = _check_counts(cache, "lengths", lengths)
+    counts = _check_counts(cache, "counts", counts) if counts is not None else None
+    _load()
+    k, v = _in_rows(keys.detach()), _in_rows(values.detach())
+    with _native.device_guard(k.device):
+        _native.call("koemi_window_cache_write", *cache.buffers(), k.data_ptr(), v.data_ptr(), _strides(k, v),
+                     lengths.data_ptr(), _native.ptr(counts), batch, length, groups, cache.width, cache.window, cache.sinks,
+                     _native.dtype_code(k.dtype), _native.stream_of(k.device))
+
+
+def window_cache_entries(cache: WindowCache, lengths: Tensor, *, dtype: torch.dtype) -> tuple[Tensor, Tensor, Tensor]:
+    """What the cache holds, as the values it stands for.
+
+    Returns ``(keys, values, present)``: ``[B, sinks + window, G, D]`` in ``dtype`` and
+    ``[B, sinks + window]`` bool: the sinks, then the last ``window`` other entries in their
+    order, the latest at the end; places without an entry hold zeros. Put before the next
+    chunk's keys, values and mask, ``window_attention`` reads them as the chunk's own past.
+    """
+
+    cache = _check_cache(cache)
+    lengths = _check_counts(cache, "lengths", lengths)
+    if dtype not in _SUPPORTED_DTYPES:
+        raise CudaThinkValidationError("dtype must be float32, float16 or bfloat16")
+    _load()
+    batch, groups, slots, _ = cache.keys.shape
+    device = cache.keys.device
+    keys = torch.empty((batch, slots, groups, cache.width), device=device, dtype=dtype)
+    values = torch.empty_like(keys)
+    present = torch.empty((batch, slots), device=device, dtype=torch.bool)
+    with _native.device_guard(device):
+        _native.call("koemi_window_cache_entries", *cache.buffers(), lengths.data_ptr(), keys.data_ptr(), values.data_ptr(),
+                     present.data_ptr(), batch, groups, cache.width, cache.window, cache.sinks, _native.dtype_code(dtype),
+                     _native.stream_of(device))
+    return keys, values, present
+
+
+@lru_cache(maxsize=256)
+def _step_bytes(batch: int, heads: int, groups: int, width: int, window: int, sinks: int) -> int:
+    return _native.query("koemi_window_cache_step_workspace_bytes", batch, heads, groups, width, window, sinks)
+
+
+def _step(cache: WindowCache, queries: Tensor, keys: Tensor | None, values: Tensor | None, lengths: Tensor,
+          active: Tensor | None, scale: float | None) -> Tensor:
+    cache = _check_cache(cache)
+    batch, groups = cache.keys.shape[:2]
+    heads = queries.shape[1] if isinstance(queries, Tensor) and queries.ndim == 3 else 0
+    _check_rows(cache, "queries", queries, (batch, heads, cache.width), None)
+    if heads < 1 or heads % groups:
+        raise CudaThinkValidationError("the key heads must divide the query heads")
+    if keys is not None or values is not None:
+        _check_rows(cache, "keys", keys, (batch, groups, cache.width), queries.dtype)
+        _check_rows(cache, "values", values, (batch, groups, cache.width), queries.dtype)
+    lengths = _check_counts(cache, "lengths", lengths)
+    device = queries.device
+    if active is not None and (not isinstance(active, Tensor) or active.dtype != torch.bool or active.shape != (batch,)
+                               or active.device != device):
+        raise CudaThinkValidationError("active must be a bool [batch] tensor on the cache's device")
+    scale = _scale(scale, cache.width)
+    _load()
+    q = _in_rows(queries.detach())
+    k = _in_rows(keys.detach()) if keys is not None else None
+    v = _in_rows(values.detach()) if values is not None else None
+    flat = [s for t in (q, k, v) for s in (t.stride()[:2] if t is not None else (0, 0))]
+    mask = active.contiguous() if active is not None else None
+    output = torch.empty((batch, heads, cache.width), device=device, dtype=q.dtype)
+    need = _step_bytes(batch, heads, groups, cache.width, cache.window, cache.sinks)
+    workspace = _bytes(need, device)
+    with _native.device_guard(device):
+        _native.call("koemi_window_cache_step", *cache.buffers(), q.data_ptr(), _native.ptr(k), _native.ptr(v),
+                     (ctypes.c_int64 * 6)(*flat), lengths.data_ptr(), _native.ptr(mask), output.data_ptr(), batch, heads,
+                     groups, cache.width, cache.window, cache.sinks, scale, _native.dtype_code(q.dtype),
+                     _native.ptr(workspace), need, _native.stream_of(device))
+    return output
+
+
+def window_cache_step(cache: WindowCache, queries: Tensor, keys: Tensor, values: Tensor, lengths: Tensor,
+                      active: Tensor | None = None, *, scale: float | None = None) -> Tensor:
+    """One position of every row: its key and value appended, in place, and its queries answered.
+
+    ``queries`` ``[B, H, D]``, ``keys`` and ``values`` ``[B, G, D]`` in one type (float32,
+    float16 or bfloat16), G a divisor of H; ``lengths`` ``[B]`` int64: the entries that
+    each row holds before the step. Returns ``[B, H, D]``: the softmax read over the sinks
+    and the last ``window`` entries, this one among them, as the cache holds them (what
+    ``window_attention`` reads at this position, the rounding to 8 bits apart). Rows with
+    False in ``active`` ``[B]`` bool, or with a negative length, are left as they are and
+    read zeros. Queries and probabilities keep 22 bits or more, sums are float32, in a fixed
+    order. Nothing is read back to the host, so a step can be captured in a graph; without
+    gradients.
+    """
+
+    return _step(cache, queries, keys, values, lengths, active, scale)
+
+
+def window_cache_read(cache: WindowCache, queries: Tensor, lengths: Tensor, active: Tensor | None = None, *,
+                      scale: float | None = None) -> Tensor:
+    """``window_cache_step`` without a new entry: the queries of the last of ``lengths`` entries."""
+
+    return _step(cache, queries, None, None, lengths, active, scale)
