@@ -1086,6 +1086,21 @@ int koemi_window_cache_step(void* keys, float* key_scales, void* values, float* 
                             int64_t window, int64_t sinks, float scale, int dtype, void* workspace, size_t workspace_bytes,
                             koemi_stream_t stream);
 
+/* The next id of every row of logits [rows, vocab] (F32, F16 or BF16, rows row_stride apart, 0:
+ * vocab) from its uniform number in [0, 1): the non-greedy TokenSampler step
+ * (runtime/fast_decode.py:57-95) with top-p and min-p, for vocabularies up to 2^19. Ids
+ * without a score: `exclude` (negative: none), -inf and NaN. With w = exp((z - max z) /
+ * temperature), kept are: the top_k largest (0: all), equals of the last among them; of
+ * those the ids whose strictly better ones weigh less than top_p (0 < top_p <= 1) of their
+ * sum; and of those w >= min_p (0 <= min_p <= 1). ids [rows]: the first whose running sum,
+ * in the ids' order, exceeds uniform x the kept sum; 0 for a row without a score. A row with
+ * +inf draws among those. probabilities [rows, vocab] fp32 (NULL: none): the distribution
+ * drawn from. Weights are formed in 64 bits and added as whole multiples of 2^-44, in any
+ * order the same. */
+int koemi_sample_filtered(const void* logits, int dtype, int64_t row_stride, int64_t rows, int64_t vocab, int64_t exclude,
+                          double temperature, int64_t top_k, double top_p, double min_p, const float* uniforms,
+                          int64_t* ids, float* probabilities, koemi_stream_t stream);
+
 /* Measurement only (no counterpart in the reference): reads `bytes` (a
  * multiple of 16) from `src` with `grid` workgroups of `block` threads, each
  * thread issuing `unroll` (1, 2, 4 or 8) 16-byte loads per pass of a

@@ -51,6 +51,7 @@ SOURCES = (
     "window_attention.hip",
     "window_attention_grad.hip",
     "window_cache.hip",
+    "sampling.hip",
 )
 
 ARCH = "gfx950"

@@ -1577,6 +1577,13 @@ class DecodeGraph:
         logits, _ = _stack_decode(self.params, self.settings, self.ids, src, dst)
         if self.policy is None:
             _greedy_tokens(logits, out=self.ids)
+        elif self.policy.top_p is not None or self.policy.min_p is not None:
+            policy, last = self.policy, logits[:, -1]
+            vocab = last.shape[1]
+            _native.call("koemi_sample_filtered", _native.ptr(last), _native.dtype_code(last.dtype), logits.stride(0),
+                         last.shape[0], vocab, PAD_TOKEN_ID if vocab > PAD_TOKEN_ID else -1, float(policy.temperature),
+                         int(policy.top_k or 0), 1.0 if policy.top_p is None else float(policy.top_p), float(policy.min_p or 0.0),
+                         _native.ptr(self.uniforms), _native.ptr(self.ids), None, _native.stream_of(logits.device))
         else:
             last = logits[:, -1]
             _native.call("koemi_herm_sample_tokens", _native.ptr(last), logits.stride(0), last.shape[0],
