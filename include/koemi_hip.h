@@ -1025,10 +1025,12 @@ int koemi_moe_experts_backward(const void* grad_output, const void* context, con
  * valid [batch, total] (NULL: all): a position with 0 is neither read nor reads, whatever its
  * tensors hold. A query that sees nothing gets zeros. scale (positive): of the scores.
  * output [batch, length, heads, width], contiguous; rest (NULL: no gradients wanted; not
- * for F32) like it: what the output was rounded off by; lse [batch, heads, length] fp32 (NULL: no gradients wanted): log2 of the sum of 2^(score log2 e), infinite
- * where nothing is seen. Workspace: koemi_window_attention_workspace_bytes, no zeroing
+ * for F32) like it: what the output was rounded off by; lse [batch,
+ * heads, length] fp32 (NULL: no gradients wanted): log2 of the sum of 2^(score log2 e),
+ * infinite where nothing is seen. Workspace: koemi_window_attention_workspace_bytes, no zeroing
  * needed, 4-byte aligned. Refused: widths over 256, 2^29 rows (positions x heads / groups)
- * of a key head and 2^24 tiles of 128 of them and more. */
+ * of a key head and 2^24 tiles of 128 of them and more, rows (width, strides, pointers) that
+ * are not whole 16-byte pieces, 16-byte aligned and less than 2^25 bytes apart. */
 size_t koemi_window_attention_workspace_bytes(int64_t batch, int64_t length, int64_t total, int64_t heads, int64_t groups,
                                               int64_t width, int64_t window, int64_t sinks, int dtype);
 int koemi_window_attention_forward(const void* queries, const void* keys, const void* values, const uint8_t* valid,

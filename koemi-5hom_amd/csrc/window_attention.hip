@@ -51,6 +51,7 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void window_forward_kern
     const int first = before + position_of(a, tile * kRows), last = before + position_of(a, last_row);
     const uint8_t* valid = a.valid ? a.valid + static_cast<int64_t>(b) * a.total : nullptr;
     const bool row_ok = row < rows && (!valid || valid[place]);
+    const uint8_t* shown_at = valid ? valid : static_cast<const uint8_t*>(a.k);  // any byte where all are valid
     if (threadIdx.x == 0) bad_tile = -1, any_row = 0;
     __syncthreads();
     if (__ballot(row_ok) && lane == 0) any_row = 1;
@@ -68,7 +69,7 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void window_forward_kern
         uint4 qf[L::kFrags];
 #pragma unroll
         for (int s = 0; s < L::kFrags; ++s)
-            qf[s] = row_ok ? load_unit<T>(q, 2 * s + half, a.width, a.vector) : make_uint4(0, 0, 0, 0);
+            qf[s] = row_ok ? load_unit<T>(q, 2 * s + half, a.width) : make_uint4(0, 0, 0, 0);
         const KeyTiles<KT> tiles(a, first, last);
         const int t0 = static_cast<int>(static_cast<int64_t>(tiles.count) * split / f.splits);
         const int t1 = static_cast<int>(static_cast<int64_t>(tiles.count) * (split + 1) / f.splits);
@@ -78,19 +79,17 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void window_forward_kern
         const int wave_last = before + position_of(a, min(wave_row + 31, rows - 1));
         const bool wave_rows = __ballot(row_ok) != 0;
         Staged<T, NB, KT> next_k, next_v;
-        bool next_ok = false;
+        uint8_t next_ok = 0;
         auto fetch = [&](int t) {
-            const int key0 = tiles[t] * KT;
-            next_ok = lane < KT && key0 + lane < a.total && (!valid || valid[key0 + lane]);
-            next_k.load(k + key0 * a.ks.position, a.ks.position, a.total - key0, a.width, a.vector);
-            next_v.load(v + key0 * a.vs.position, a.vs.position, a.total - key0, a.width, a.vector);
+            const int key0 = tiles[t] * KT, last = a.total - 1 - key0;
+            next_ok = shown_at[valid ? min(key0 + lane, a.total - 1) : 0];
+            next_k.load(k + key0 * a.ks.position, a.ks.position, last, a.width);
+            next_v.load(v + key0 * a.vs.position, a.vs.position, last, a.width);
         };
-        next_k.prepare(a.ks.position, a.width);
-        next_v.prepare(a.vs.position, a.width);
         if (t0 < t1) fetch(t0);
         for (int t = t0; t < t1; ++t) {
             const int key0 = tiles[t] * KT;
-            const uint64_t shown = __ballot(next_ok), every = low_bits(KT);
+            const uint64_t shown = __ballot(lane < KT && key0 + lane < a.total && (!valid || next_ok)), every = low_bits(KT);
             auto whole = [&](int lo, int hi) {  // rows at places lo .. hi see all of the tile
                 return shown == every && key0 + KT - 1 <= lo && (hi - key0 < a.window || key0 + KT <= a.sinks);
             };
@@ -99,8 +98,8 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void window_forward_kern
                 next_k.keep(shown);
                 if (next_v.keep(shown)) bad_tile = t;
             }
-            next_k.store(k_tile);
-            next_v.store(v_tile);
+            next_k.store(k_tile, a.width);
+            next_v.store(v_tile, a.width);
             __syncthreads();
             if (t + 1 < t1) fetch(t + 1);
             if (!shown || !wave_rows || key0 > wave_last || (key0 + KT <= wave_first - a.window + 1 && key0 >= a.sinks)) continue;
@@ -287,11 +286,12 @@ int shape_of(const char* what, const void* queries, const void* keys, const void
         s.qs = {strides[0], strides[1], strides[2]};
         s.ks = {strides[3], strides[4], strides[5]};
         s.vs = {strides[6], strides[7], strides[8]};
-        bool aligned = width * size % 16 == 0;
-        for (int i = 0; i < 9; ++i) aligned = aligned && strides[i] * size % 16 == 0 && strides[i] >= 0;
-        for (int i = 1; i < 9; i += 3) aligned = aligned && strides[i] * size < (1 << 24);
-        for (const void* p : {queries, keys, values}) aligned = aligned && reinterpret_cast<uintptr_t>(p) % 16 == 0;
-        s.vector = aligned;
+        bool fits = width * size % 16 == 0 && heads * width * size < (1 << 25);
+        for (int i = 0; i < 9; ++i) fits = fits && strides[i] * size % 16 == 0 && strides[i] >= 0;
+        for (int i = 1; i < 9; i += 3) fits = fits && strides[i] * size < (1 << 25);
+        for (const void* p : {queries, keys, values}) fits = fits && reinterpret_cast<uintptr_t>(p) % 16 == 0;
+        if (!fits)
+            return fail(KOEMI_ERR_UNSUPPORTED, "%s: rows must be whole 16-byte pieces, 16-byte aligned and less than 2^25 bytes apart", what);
     }
     s.batch = static_cast<int>(batch), s.length = static_cast<int>(length), s.total = static_cast<int>(total);
     s.groups = static_cast<int>(groups), s.shared = static_cast<int>(shared), s.width = static_cast<int>(width);

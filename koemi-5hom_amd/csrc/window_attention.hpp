@@ -37,6 +37,7 @@ struct Strides {
 };
 
 struct Shape {
+    // rows are whole, aligned 16-byte pieces, less than 2^25 bytes apart
     const void* q;
     const void* k;
     const void* v;
@@ -47,7 +48,6 @@ struct Shape {
     float scale;        // of the scores
     uint32_t magic;     // rows / shared = (rows * magic >> 32) >> shift, rows below 2^31
     int shift;
-    int vector;         // rows are whole, aligned 16-byte pieces, less than 2^24 bytes apart
 };
 
 // The position of row m, and its head among those that share.
@@ -90,57 +90,31 @@ template <typename T> __device__ __forceinline__ bool any_nonfinite(const uint4&
 
 // 16 bytes of a row from column 16 / sizeof(T) * unit on, zeros past the width.
 template <typename T>
-__device__ __forceinline__ uint4 load_unit(const T* row, int unit, int width, bool vector) {
-    constexpr int E = kPer16<T>;
-    const int c = unit * E;
-    uint4 out = make_uint4(0, 0, 0, 0);
-    if (vector) {
-        if (c < width) out = *reinterpret_cast<const uint4*>(row + c);
-    } else {
-        alignas(16) T e[E];
-#pragma unroll
-        for (int i = 0; i < E; ++i) e[i] = c + i < width ? row[c + i] : static_cast<T>(0.0f);
-        out = *reinterpret_cast<const uint4*>(e);
-    }
-    return out;
+__device__ __forceinline__ uint4 load_unit(const T* row, int unit, int width) {
+    const int c = unit * kPer16<T>;
+    return c < width ? *reinterpret_cast<const uint4*>(row + c) : make_uint4(0, 0, 0, 0);
 }
 
 // A tile's rows on their way from memory to LDS: each thread brings the same pieces of
-// every tile, at offsets that it forms once (vector: a row's stride is below 2^24 bytes).
+// every tile. The loads are unconditional (rows past the last one read that one again, pieces
+// past the width the row's first), so that nothing waits for them before store(), which
+// puts zeros in those places.
 template <typename T, int NB, int ROWS>
 struct Staged {
     using L = Tile<T, NB>;
-    static constexpr int kPieces = ROWS * L::kUnits;
-    static constexpr int kEach = (kPieces + kThreads - 1) / kThreads;
-    static constexpr bool kEven = kThreads % L::kUnits == 0;  // a thread's pieces are one unit of rows a fixed step apart
-    static constexpr uint32_t kNone = ~0u;
+    static constexpr int kEach = ROWS * L::kUnits / kThreads;
+    static_assert(ROWS * L::kUnits % kThreads == 0, "whole pieces a thread");
     uint4 piece[kEach];
-    uint32_t off[kEven ? 1 : kEach];
 
     static __device__ __forceinline__ int row(int n) { return (static_cast<int>(threadIdx.x) + n * kThreads) / L::kUnits; }
     static __device__ __forceinline__ int unit(int n) { return (static_cast<int>(threadIdx.x) + n * kThreads) % L::kUnits; }
-    __device__ __forceinline__ void prepare(int64_t stride, int width) {
+    // `first`: the tile's first row, a uniform address; `last`: the last row to read.
+    __device__ __forceinline__ void load(const T* first, int64_t stride, int last, int width) {
+        const uint32_t bytes = static_cast<uint32_t>(stride) * static_cast<uint32_t>(sizeof(T));
 #pragma unroll
-        for (int n = 0; n < (kEven ? 1 : kEach); ++n)
-            off[n] = row(n) < ROWS && unit(n) * kPer16<T> < width
-                         ? row(n) * static_cast<uint32_t>(stride * static_cast<int64_t>(sizeof(T))) + unit(n) * 16 : kNone;
-    }
-    // Rows 0 .. count - 1 of the tile from `first`, a uniform address; the others are zeros.
-    __device__ __forceinline__ void load(const T* first, int64_t stride, int count, int width, bool vector) {
-        if (vector && count >= ROWS) {
-#pragma unroll
-            for (int n = 0; n < kEach; ++n) {
-                const char* from = reinterpret_cast<const char*>(kEven ? first + n * (kThreads / L::kUnits) * stride : first);
-                const uint32_t at = off[kEven ? 0 : n];
-                piece[n] = make_uint4(0, 0, 0, 0);
-                if (at != kNone) piece[n] = *reinterpret_cast<const uint4*>(from + at);
-            }
-        } else {
-#pragma unroll
-            for (int n = 0; n < kEach; ++n) {
-                piece[n] = make_uint4(0, 0, 0, 0);
-                if (row(n) < min(count, ROWS)) piece[n] = load_unit<T>(first + row(n) * stride, unit(n), width, vector);
-            }
+        for (int n = 0; n < kEach; ++n) {
+            const uint32_t at = static_cast<uint32_t>(min(row(n), last)) * bytes + (unit(n) * kPer16<T> < width ? unit(n) * 16u : 0u);
+            piece[n] = *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(first) + at);
         }
     }
     // Zeros for the rows without a bit; true if what is left holds an infinity or NaN.
@@ -153,10 +127,14 @@ struct Staged {
         }
         return bad;
     }
-    __device__ __forceinline__ void store(char* tile) const {
+    __device__ __forceinline__ void store(char* tile, int width) {
+        if (width < 32 * NB) {
 #pragma unroll
-        for (int n = 0; n < kEach; ++n)
-            if (kPieces % kThreads == 0 || row(n) < ROWS) *reinterpret_cast<uint4*>(tile + L::at(row(n), unit(n))) = piece[n];
+            for (int n = 0; n < kEach; ++n)
+                if (unit(n) * kPer16<T> >= width) piece[n] = make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int n = 0; n < kEach; ++n) *reinterpret_cast<uint4*>(tile + L::at(row(n), unit(n))) = piece[n];
     }
 };
 
@@ -313,19 +291,13 @@ int shape_of(const char* what, const void* queries, const void* keys, const void
              const int64_t* strides, int64_t batch, int64_t length, int64_t total, int64_t heads, int64_t groups,
              int64_t width, int64_t window, int64_t sinks, float scale, int dtype, Shape& s);
 
-// Four consecutive values of a row of `width` from column d on.
+// Four consecutive values of a row of `width` (a multiple of four) from column d on.
 template <typename T>
 __device__ __forceinline__ void store_four(T* row, int d, int width, const float (&x)[4]) {
     alignas(16) T e[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) e[i] = from_f32<T>(x[i]);
-    if (width % 4 == 0) {
-        if (d < width) __builtin_memcpy(__builtin_assume_aligned(row + d, 4 * sizeof(T)), e, 4 * sizeof(T));
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (d + i < width) row[d + i] = e[i];
-    }
+    if (d < width) __builtin_memcpy(__builtin_assume_aligned(row + d, 4 * sizeof(T)), e, 4 * sizeof(T));
 }
 
 }  // namespace window_attention

@@ -89,6 +89,7 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void window_dq_kernel(Ba
     const int first = before + position_of(a, tile * kRows), last = before + position_of(a, last_row);
     const uint8_t* valid = a.valid ? a.valid + static_cast<int64_t>(b) * a.total : nullptr;
     const bool row_ok = row < rows && (!valid || valid[place]);
+    const uint8_t* shown_at = valid ? valid : static_cast<const uint8_t*>(a.k);  // any byte where all are valid
     const int64_t at = (static_cast<int64_t>(b) * a.groups * a.shared + head) * a.length + position;
     const int64_t cell = ((static_cast<int64_t>(b) * a.length + position) * a.groups * a.shared + head) * a.width;
     if (threadIdx.x == 0) bad_tile = -1, any_row = 0;
@@ -106,17 +107,16 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void window_dq_kernel(Ba
         const T* q = static_cast<const T*>(a.q) + b * a.qs.batch + position * a.qs.position + head * a.qs.head;
         const T* k = static_cast<const T*>(a.k) + b * a.ks.batch + g * a.ks.head;
         const T* v = static_cast<const T*>(a.v) + b * a.vs.batch + g * a.vs.head;
-        const bool plain = a.width % kPer16<T> == 0;  // out, d_out: contiguous rows
         uint4 qf[L::kFrags], gf[L::kFrags];
 #pragma unroll
         for (int s = 0; s < L::kFrags; ++s) {
             qf[s] = gf[s] = make_uint4(0, 0, 0, 0);
             if (row_ok) {
-                qf[s] = load_unit<T>(q, 2 * s + half, a.width, a.vector);
-                gf[s] = load_unit<T>(static_cast<const T*>(f.d_out) + cell, 2 * s + half, a.width, plain);
-                const uint4 o = load_unit<T>(static_cast<const T*>(f.out) + cell, 2 * s + half, a.width, plain);
+                qf[s] = load_unit<T>(q, 2 * s + half, a.width);
+                gf[s] = load_unit<T>(static_cast<const T*>(f.d_out) + cell, 2 * s + half, a.width);
+                const uint4 o = load_unit<T>(static_cast<const T*>(f.out) + cell, 2 * s + half, a.width);
                 uint4 l = make_uint4(0, 0, 0, 0);
-                if (f.rest) l = load_unit<T>(static_cast<const T*>(f.rest) + cell, 2 * s + half, a.width, plain);
+                if (f.rest) l = load_unit<T>(static_cast<const T*>(f.rest) + cell, 2 * s + half, a.width);
                 const T* x = reinterpret_cast<const T*>(&gf[s]);
                 const T* y = reinterpret_cast<const T*>(&o);
                 const T* z = reinterpret_cast<const T*>(&l);
@@ -132,19 +132,17 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void window_dq_kernel(Ba
         const int wave_last = before + position_of(a, min(wave_row + 31, rows - 1));
         const bool wave_rows = __ballot(row_ok) != 0;
         Staged<T, NB, KT> next_k, next_v;
-        bool next_ok = false;
+        uint8_t next_ok = 0;
         auto fetch = [&](int t) {
-            const int key0 = tiles[t] * KT;
-            next_ok = lane < KT && key0 + lane < a.total && (!valid || valid[key0 + lane]);
-            next_k.load(k + key0 * a.ks.position, a.ks.position, a.total - key0, a.width, a.vector);
-            next_v.load(v + key0 * a.vs.position, a.vs.position, a.total - key0, a.width, a.vector);
+            const int key0 = tiles[t] * KT, last = a.total - 1 - key0;
+            next_ok = shown_at[valid ? min(key0 + lane, a.total - 1) : 0];
+            next_k.load(k + key0 * a.ks.position, a.ks.position, last, a.width);
+            next_v.load(v + key0 * a.vs.position, a.vs.position, last, a.width);
         };
-        next_k.prepare(a.ks.position, a.width);
-        next_v.prepare(a.vs.position, a.width);
         fetch(0);
         for (int t = 0; t < tiles.count; ++t) {
             const int key0 = tiles[t] * KT;
-            const uint64_t shown = __ballot(next_ok), every = low_bits(KT);
+            const uint64_t shown = __ballot(lane < KT && key0 + lane < a.total && (!valid || next_ok)), every = low_bits(KT);
             auto whole = [&](int lo, int hi) {  // rows at places lo .. hi see all of the tile
                 return shown == every && key0 + KT - 1 <= lo && (hi - key0 < a.window || key0 + KT <= a.sinks);
             };
@@ -153,8 +151,8 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void window_dq_kernel(Ba
                 next_v.keep(shown);
                 if (next_k.keep(shown)) bad_tile = t;
             }
-            next_k.store(k_tile);
-            next_v.store(v_tile);
+            next_k.store(k_tile, a.width);
+            next_v.store(v_tile, a.width);
             __syncthreads();
             if (t + 1 < tiles.count) fetch(t + 1);
             if (!shown || !wave_rows || key0 > wave_last || (key0 + KT <= wave_first - a.window + 1 && key0 >= a.sinks)) continue;
@@ -236,15 +234,14 @@ __global__ __launch_bounds__(kThreads, NB <= 2 ? 2 : 1) void window_dkv_kernel(B
     uint4 kf[L::kFrags], vf[L::kFrags];
 #pragma unroll
     for (int s = 0; s < L::kFrags; ++s) {
-        kf[s] = key_ok ? load_unit<T>(k, 2 * s + half, a.width, a.vector) : make_uint4(0, 0, 0, 0);
-        vf[s] = key_ok ? load_unit<T>(v, 2 * s + half, a.width, a.vector) : make_uint4(0, 0, 0, 0);
+        kf[s] = key_ok ? load_unit<T>(k, 2 * s + half, a.width) : make_uint4(0, 0, 0, 0);
+        vf[s] = key_ok ? load_unit<T>(v, 2 * s + half, a.width) : make_uint4(0, 0, 0, 0);
     }
     f32x16 dk[NB], dv[NB];
 #pragma unroll
     for (int n = 0; n < NB; ++n) dk[n] = dv[n] = f32x16(0.0f);
     Range<T, NB> range;
     const float c = a.scale * kLog2e;
-    const bool plain = a.width % kPer16<T> == 0 && out_row * static_cast<int64_t>(sizeof(T)) < (1 << 24);
     // queries that see key j: from begins(j) on, up to ends(j)
     auto begins = [&](int j) { return max(j - before, 0); };
     auto ends = [&](int j) { return max(j - before + a.window, 0); };
@@ -264,29 +261,24 @@ __global__ __launch_bounds__(kThreads, NB <= 2 ? 2 : 1) void window_dkv_kernel(B
     const int first = from & ~(RT - 1), walk = to > from ? (to - first + RT - 1) / RT : 0, steps = walk * a.shared;
 
     Staged<T, NB, RT> next_q, next_g;
-    bool next_ok = false;
+    const uint8_t* shown_at = valid ? valid + before : static_cast<const uint8_t*>(a.q);  // any byte where all are valid
+    const float* stat_at = (static_cast<int>(threadIdx.x) / RT % 2 ? f.delta : f.lse) + stat;
+    uint8_t next_ok = 0;
     float next_stat = 0.0f;
-    next_q.prepare(a.qs.position, a.width);
-    next_g.prepare(out_row, a.width);
     int next_head = 0, next_p = first;  // of the tile to fetch
     auto fetch = [&]() {
-        const int p0 = next_p;
-        next_ok = lane < RT && p0 + lane < a.length && (!valid || valid[before + p0 + lane]);
-        if (threadIdx.x < 2 * RT) {
-            const int r = static_cast<int>(threadIdx.x) % RT;
-            next_stat = p0 + r < a.length
-                            ? (static_cast<int>(threadIdx.x) < RT ? f.lse : f.delta)[stat + static_cast<int64_t>(next_head) * a.length + p0 + r]
-                            : 0.0f;
-        }
-        next_q.load(q + next_head * a.qs.head + p0 * a.qs.position, a.qs.position, a.length - p0, a.width, a.vector);
-        next_g.load(d_out + static_cast<int64_t>(next_head) * a.width + p0 * out_row, out_row, a.length - p0, a.width, plain);
+        const int p0 = next_p, last = a.length - 1 - p0;
+        next_ok = shown_at[valid ? min(p0 + lane, a.length - 1) : 0];
+        next_stat = stat_at[static_cast<int64_t>(next_head) * a.length + p0 + min(static_cast<int>(threadIdx.x) % RT, last)];
+        next_q.load(q + next_head * a.qs.head + p0 * a.qs.position, a.qs.position, last, a.width);
+        next_g.load(d_out + static_cast<int64_t>(next_head) * a.width + p0 * out_row, out_row, last, a.width);
         next_p += RT;
         if (next_p >= to) next_p = first, ++next_head;
     };
     if (steps) fetch();
     int p0 = first;
     for (int t = 0; t < steps; ++t, p0 = p0 + RT >= to ? first : p0 + RT) {
-        const uint64_t shown = __ballot(next_ok), every = low_bits(RT);
+        const uint64_t shown = __ballot(lane < RT && p0 + lane < a.length && (!valid || next_ok)), every = low_bits(RT);
         // every key of the workgroup is seen by every row of the tile
         const bool all = !FAR && shown == every && !valid && p0 >= begins(key0 + kRows - 1) && p0 + RT <= ends(key0) && key0 + kRows <= a.total;
         __syncthreads();
@@ -294,8 +286,8 @@ __global__ __launch_bounds__(kThreads, NB <= 2 ? 2 : 1) void window_dkv_kernel(B
             const bool bad_q = next_q.keep(shown), bad_g = next_g.keep(shown);
             if (bad_q || bad_g) bad_tile = t;
         }
-        next_q.store(q_tile);
-        next_g.store(g_tile);
+        next_q.store(q_tile, a.width);
+        next_g.store(g_tile, a.width);
         if (threadIdx.x < 2 * RT) stats[static_cast<int>(threadIdx.x) / RT][static_cast<int>(threadIdx.x) % RT] = next_stat;
         __syncthreads();
         if (t + 1 < steps) fetch();
@@ -385,7 +377,7 @@ __global__ __launch_bounds__(kThreads, NB <= 2 ? 2 : 1) void window_dkv_kernel(B
             if (key < far_keys) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (e + i < a.width) x[i] += far[e + i], y[i] += far[a.width + e + i];
+                    if (e < a.width) x[i] += far[e + i], y[i] += far[a.width + e + i];
             }
             if (f.dk) store_four(static_cast<T*>(f.dk) + cell, e, a.width, x);
             if (f.dv) store_four(static_cast<T*>(f.dv) + cell, e, a.width, y);

@@ -105,8 +105,22 @@ def window_attention(queries: Tensor, keys: Tensor, values: Tensor, valid_mask: 
         raise CudaThinkValidationError("valid_mask must be a bool [batch, total] tensor on the same device")
     window, sinks, scale = _whole("window", window, 1), _whole("sinks", sinks, 0), _scale(scale, width)
     _load()
-    trained = torch.is_grad_enabled() and any(t.requires_grad for t in tensors.values())
-    return _WindowAttention.apply(queries, keys, values, valid_mask, window, sinks, scale, trained)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors.values()):
+        return _WindowAttention.apply(queries, keys, values, valid_mask, window, sinks, scale)
+    return _forward(queries, keys, values, valid_mask, window, sinks, scale, False)[0]
+
+
+def _pieces(tensor: Tensor) -> Tensor:
+    """``tensor`` [B, L, H, D] where the kernels can read its rows as they lie (whole, aligned
+    16-byte pieces, less than 2^25 bytes apart), else a copy that they can, its width padded
+    with zeros."""
+
+    size, strides = tensor.element_size(), tensor.stride()
+    if (strides[3] == 1 and tensor.shape[3] * size % 16 == 0 and tensor.data_ptr() % 16 == 0
+            and all(s * size % 16 == 0 for s in strides[:3]) and strides[1] * size < 1 << 25):
+        return tensor
+    short = -tensor.shape[3] % (16 // size)
+    return torch.nn.functional.pad(tensor, (0, short)) if short else tensor.contiguous()
 
 
 @lru_cache(maxsize=256)
@@ -130,43 +144,54 @@ def _bytes(need: int, device: torch.device) -> Tensor | None:
     return torch.empty(need, device=device, dtype=torch.uint8) if need else None
 
 
+def _forward(queries: Tensor, keys: Tensor, values: Tensor, valid_mask: Tensor | None, window: int, sinks: int,
+             scale: float, trained: bool) -> tuple:
+    """The output, and with ``trained`` what the gradients need."""
+
+    batch, length, heads, width = queries.shape
+    total, groups = keys.shape[1:3]
+    device, code = queries.device, _native.dtype_code(queries.dtype)
+    q, k, v = _pieces(queries.detach()), _pieces(keys.detach()), _pieces(values.detach())
+    if not q.shape[3] == k.shape[3] == v.shape[3]:
+        raise CudaThinkValidationError("heads must share a width")
+    mask = valid_mask.contiguous() if valid_mask is not None else None
+    output = torch.empty((batch, length, heads, q.shape[3]), device=device, dtype=queries.dtype)
+    rest = torch.empty_like(output) if trained and queries.dtype != torch.float32 else None
+    lse = torch.empty((batch, heads, length), device=device, dtype=torch.float32) if trained else None
+    shape = (batch, length, total, heads, groups, q.shape[3], window, sinks)
+    need = _workspace_bytes(*shape, code)[0]
+    workspace = _bytes(need, device)
+    with _native.device_guard(device):
+        _native.call("koemi_window_attention_forward", q.data_ptr(), k.data_ptr(), v.data_ptr(), _native.ptr(mask),
+                     _strides(q, k, v), output.data_ptr(), _native.ptr(rest), _native.ptr(lse), *shape, scale, code,
+                     _native.ptr(workspace), need, _native.stream_of(device))
+    result = output if q.shape[3] == width else output[..., :width].contiguous()
+    return (result, q, k, v, mask, output, rest, lse) if trained else (result,)
+
+
 class _WindowAttention(torch.autograd.Function):
     @staticmethod
     def forward(context, queries: Tensor, keys: Tensor, values: Tensor, valid_mask: Tensor | None,  # type: ignore[override]
-                window: int, sinks: int, scale: float, trained: bool) -> Tensor:
-        batch, length, heads, width = queries.shape
-        total, groups = keys.shape[1:3]
-        device, code = queries.device, _native.dtype_code(queries.dtype)
-        q, k, v = (t if t.stride(3) == 1 or width == 1 else t.contiguous() for t in (queries, keys, values))
-        mask = valid_mask.contiguous() if valid_mask is not None else None
-        output = torch.empty((batch, length, heads, width), device=device, dtype=queries.dtype)
-        rest = torch.empty_like(output) if trained and queries.dtype != torch.float32 else None
-        lse = torch.empty((batch, heads, length), device=device, dtype=torch.float32) if trained else None
-        shape = (batch, length, total, heads, groups, width, window, sinks)
-        need = _workspace_bytes(*shape, code)[0]
-        workspace = _bytes(need, device)
-        with _native.device_guard(device):
-            _native.call("koemi_window_attention_forward", q.data_ptr(), k.data_ptr(), v.data_ptr(), _native.ptr(mask),
-                         _strides(q, k, v), output.data_ptr(), _native.ptr(rest), _native.ptr(lse), *shape, scale, code,
-                         _native.ptr(workspace), need, _native.stream_of(device))
-        if trained:
-            context.save_for_backward(q, k, v, mask, output, rest, lse)
-            context.window = (window, sinks, scale)
-        return output
+                window: int, sinks: int, scale: float) -> Tensor:
+        result, *kept = _forward(queries, keys, values, valid_mask, window, sinks, scale, True)
+        context.save_for_backward(*kept)
+        context.window = (window, sinks, scale, queries.shape[3])
+        return result
 
     @staticmethod
     @once_differentiable
     def backward(context, d_output: Tensor):  # type: ignore[override]
         q, k, v, mask, output, rest, lse = context.saved_tensors
-        window, sinks, scale = context.window
-        batch, length, heads, width = q.shape
+        window, sinks, scale, width = context.window
+        batch, length, heads, padded = q.shape
         total, groups = k.shape[1:3]
         device, code = q.device, _native.dtype_code(q.dtype)
-        d_output = d_output.contiguous()
-        wanted = context.needs_input_grad
+        d_output = torch.nn.functional.pad(d_output, (0, padded - width)) if padded > width else d_output.contiguous()
+        if d_output.data_ptr() % 16:
+            d_output = d_output.clone()
         d_q, d_k, d_v = (torch.empty(t.shape, device=device, dtype=t.dtype) if need else None
-                         for t, need in zip((q, k, v), wanted))
-        shape = (batch, length, total, heads, groups, width, window, sinks)
+                         for t, need in zip((q, k, v), context.needs_input_grad))
+        shape = (batch, length, total, heads, groups, padded, window, sinks)
         need = _workspace_bytes(*shape, code)[1]
         workspace = _bytes(need, device)
         with _native.device_guard(device):
@@ -174,7 +199,8 @@ class _WindowAttention(torch.autograd.Function):
                          _strides(q, k, v), output.data_ptr(), _native.ptr(rest), lse.data_ptr(), d_output.data_ptr(),
                          _native.ptr(d_q), _native.ptr(d_k), _native.ptr(d_v), *shape, scale, code,
                          _native.ptr(workspace), need, _native.stream_of(device))
-        return d_q, d_k, d_v, None, None, None, None, None
+        grads = (g if g is None or padded == width else g[..., :width].contiguous() for g in (d_q, d_k, d_v))
+        return (*grads, None, None, None, None)
 
 
 @dataclass(frozen=True)
