@@ -29,12 +29,12 @@ struct Forward {
 };
 
 template <typename T, int NB>
-__global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void window_forward_kernel(Forward f) {
+__global__ __launch_bounds__(kThreads, NB == 1 ? 4 : NB == 2 ? 3 : NB <= 4 ? 2 : 1) void window_forward_kernel(Forward f) {
     using L = Tile<T, NB>;
     constexpr int KT = kKeys<T>, KB = KT / 32;
     __shared__ __attribute__((aligned(1024))) char k_tile[KT * L::kStride];
     __shared__ __attribute__((aligned(1024))) char v_tile[KT * L::kStride];
-    __shared__ float scratch[kWaves][32 * 32];
+    __shared__ float scratch[kWaves][kScratch];
     __shared__ int bad_tile, any_row;
     const Shape& a = f.s;
     const int lane = lane_id(), wave = static_cast<int>(threadIdx.x) / kWave, half = lane >> 5, col = lane & 31;
@@ -95,8 +95,8 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void window_forward_kern
             };
             __syncthreads();
             if (!whole(first, last)) {
-                next_k.keep(shown);
-                if (next_v.keep(shown)) bad_tile = t;
+                next_k.keep({shown});
+                if (next_v.keep({shown})) bad_tile = t;
             }
             next_k.store(k_tile, a.width);
             next_v.store(v_tile, a.width);

@@ -76,17 +76,31 @@ struct Tile {
     static __device__ __forceinline__ int at(int r, int unit) { return r * kStride + ((unit ^ turn(r)) << 4); }
 };
 
-template <typename T> __device__ __forceinline__ bool any_nonfinite(const uint4& x) {
-    constexpr uint32_t E = sizeof(T) == 4 ? 0x7f800000u : std::is_same<T, f16>::value ? 0x7c00u : 0x7f80u;
-    bool bad = false;
-    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+// The lowest n bits, n of any sign.
+__device__ __forceinline__ uint64_t low_bits(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; }
+
+// The largest sizes, by their bits, of values seen so far: an infinity or NaN among them?
+template <typename T>
+struct Largest {
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    uint32_t bits = 0;
+    __device__ __forceinline__ void add(const uint4& x) {
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        bad |= (w[i] & E) == E;
-        if (sizeof(T) == 2) bad |= ((w[i] >> 16) & E) == E;
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 4)
+                bits = max(bits, w[i] & 0x7fffffffu);
+            else
+                bits = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, bits),
+                                                                              __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu)));
+        }
     }
-    return bad;
-}
+    __device__ __forceinline__ bool nonfinite() const {
+        if constexpr (sizeof(T) == 4) return bits >= 0x7f800000u;
+        constexpr uint32_t E = std::is_same<T, f16>::value ? 0x7c00u : 0x7f80u;
+        return (bits & 0xffffu) >= E || bits >> 16 >= E;
+    }
+};
 
 // 16 bytes of a row from column 16 / sizeof(T) * unit on, zeros past the width.
 template <typename T>
@@ -118,14 +132,19 @@ struct Staged {
         }
     }
     // Zeros for the rows without a bit; true if what is left holds an infinity or NaN.
-    __device__ __forceinline__ bool keep(uint64_t rows) {
-        bool bad = false;
+    __device__ __forceinline__ bool keep(const uint64_t (&rows)[(ROWS + 63) / 64]) {
+        Largest<T> largest;
+        bool every = true;
 #pragma unroll
-        for (int n = 0; n < kEach; ++n) {
-            if (!((rows >> (row(n) & 63)) & 1ull)) piece[n] = make_uint4(0, 0, 0, 0);
-            bad |= any_nonfinite<T>(piece[n]);
+        for (int w = 0; w < (ROWS + 63) / 64; ++w) every = every && rows[w] == low_bits(ROWS - 64 * w);
+        if (!every) {
+#pragma unroll
+            for (int n = 0; n < kEach; ++n)
+                if (!((rows[ROWS > 64 && row(n) >= 64 ? 1 : 0] >> (row(n) & 63)) & 1ull)) piece[n] = make_uint4(0, 0, 0, 0);
         }
-        return bad;
+#pragma unroll
+        for (int n = 0; n < kEach; ++n) largest.add(piece[n]);
+        return largest.nonfinite();
     }
     __device__ __forceinline__ void store(char* tile, int width) {
         if (width < 32 * NB) {
@@ -218,29 +237,33 @@ __device__ __forceinline__ void mma_acc(f32x16 (&acc)[NB], const char* tile, int
 
 // mma_acc for a block that holds an infinity or NaN and is masked in places: 0 times one of
 // them is not 0, so only what a column sees is added, one row after another. `seen`: the
-// lane's column's 32 rows. `scratch`: 32 x 32 floats of this wave's own.
+// lane's column's 32 rows. `scratch`: kScratch floats of this wave's own.
+constexpr int kScratch = 16 * 32;
 template <typename T, int NB>
 __device__ __forceinline__ void seen_acc(f32x16 (&acc)[NB], const char* tile, int first, const f32x16& coef, uint32_t seen, float* scratch) {
     using L = Tile<T, NB>;
     const int lane = lane_id(), half = lane >> 5, col = lane & 31;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) scratch[(8 * (r / 4) + 4 * half + r % 4) * 32 + col] = coef[r];
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r) scratch[(8 * (r / 4) + 4 * half + r % 4) * 32 + col] = coef[8 * h + r];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll 1
-    for (int k = 0; k < 32; ++k) {
-        const float c = scratch[k * 32 + col];
-        if (!((seen >> k) & 1u)) continue;
+        for (int k = 0; k < 16; ++k) {
+            const float c = scratch[k * 32 + col];
+            if (!((seen >> (16 * h + k)) & 1u)) continue;
 #pragma unroll
-        for (int n = 0; n < NB; ++n)
+            for (int n = 0; n < NB; ++n)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int d = 32 * n + 8 * q + 4 * half;
-                const T* x = reinterpret_cast<const T*>(tile + L::at(first + k, d / kPer16<T>) + (d % kPer16<T>) * sizeof(T));
+                for (int q = 0; q < 4; ++q) {
+                    const int d = 32 * n + 8 * q + 4 * half;
+                    const T* x = reinterpret_cast<const T*>(tile + L::at(first + 16 * h + k, d / kPer16<T>) + (d % kPer16<T>) * sizeof(T));
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[n][4 * q + i] = fmaf(c, to_f32(x[i]), acc[n][4 * q + i]);
-            }
+                    for (int i = 0; i < 4; ++i) acc[n][4 * q + i] = fmaf(c, to_f32(x[i]), acc[n][4 * q + i]);
+                }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
 
 // Both halves of the wave hold a part of a column's maximum or sum.
@@ -252,9 +275,6 @@ __device__ __forceinline__ float sum_of_halves(float x) {
     const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return __uint_as_float(both[0]) + __uint_as_float(both[1]);
 }
-
-// The lowest n bits, n of any sign.
-__device__ __forceinline__ uint64_t low_bits(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; }
 
 // Of the 64 keys from key0 on, those that a query at `place` sees by position.
 __device__ __forceinline__ uint64_t keys_seen(const Shape& a, int place, int key0) {

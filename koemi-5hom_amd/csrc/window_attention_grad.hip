@@ -29,8 +29,8 @@ struct Backward {
     void* dk;
     void* dv;
     float* far_parts;   // [chunks, batch, groups, 32 x far_tiles keys, 2, width]
-    int row_tiles, key_tiles;
-    int far_tiles, far_chunks, far_first, far_rows;  // tiles of 32 sinks; positions past their window: first, and of a chunk
+    int row_tiles;
+    int far_tiles, far_chunks, far_first;  // tiles of 32 sinks; the first position past the first one's window
 };
 
 template <typename T> constexpr int kKeys = sizeof(T) == 4 ? 32 : 64;  // of a tile that dq walks
@@ -69,12 +69,12 @@ struct Range {
 };
 
 template <typename T, int NB>
-__global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void window_dq_kernel(Backward f) {
+__global__ __launch_bounds__(kThreads, NB == 1 ? 4 : NB == 2 && sizeof(T) == 2 ? 3 : NB <= 4 ? 2 : 1) void window_dq_kernel(Backward f) {
     using L = Tile<T, NB>;
     constexpr int KT = kKeys<T>, KB = KT / 32;
     __shared__ __attribute__((aligned(1024))) char k_tile[KT * L::kStride];
     __shared__ __attribute__((aligned(1024))) char v_tile[KT * L::kStride];
-    __shared__ float scratch[kWaves][32 * 32];
+    __shared__ float scratch[kWaves][kScratch];
     __shared__ int bad_tile, any_row;
     const Shape& a = f.s;
     const int lane = lane_id(), wave = static_cast<int>(threadIdx.x) / kWave, half = lane >> 5, col = lane & 31;
@@ -148,8 +148,8 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void window_dq_kernel(Ba
             };
             __syncthreads();
             if (!whole(first, last)) {
-                next_v.keep(shown);
-                if (next_k.keep(shown)) bad_tile = t;
+                next_v.keep({shown});
+                if (next_k.keep({shown})) bad_tile = t;
             }
             next_k.store(k_tile, a.width);
             next_v.store(v_tile, a.width);
@@ -193,36 +193,36 @@ __global__ __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) void window_dq_kernel(Ba
         }
 }
 
-// The rows of one head after another, in tiles of 64 positions (fp32: 32). FAR: the sinks'
-// keys against a chunk of the positions past their window: the waves share 32 keys and take the
-// tiles in turn, and their sums, added in order, go to far_parts.
-template <typename T, int NB, bool FAR>
-__global__ __launch_bounds__(kThreads, NB <= 2 ? 2 : 1) void window_dkv_kernel(Backward f) {
+// Rows of a tile where the waves share their keys: 32 a wave, or what LDS holds.
+template <typename T, int NB> constexpr int kShareRows = Tile<T, NB>::kStride > 512 ? 64 : 32 * kWaves;
+
+// The rows of one head after another, in tiles. Each wave holds 32 keys of its own (SHARE
+// false: 128 a workgroup), or all hold the same 32 and take blocks of 32 rows in turn, their
+// sums added in their order: four times the workgroups, each with a quarter of the work, for
+// calls of few keys, and (far) for the sinks against a chunk of the tiles past their window,
+// whose sums go to far_parts.
+template <typename T, int NB, bool SHARE>
+__global__ __launch_bounds__(kThreads, NB <= 2 ? 2 : 1) void window_dkv_kernel(Backward f, int far) {
     using L = Tile<T, NB>;
-    constexpr int RT = kKeys<T>, RB = RT / 32;
+    constexpr int RT = SHARE ? kShareRows<T, NB> : kKeys<T>, RB = RT / 32, RW = (RT + 63) / 64;
+    constexpr int kOwn = SHARE ? 32 : kRows;  // keys of the workgroup
     __shared__ __attribute__((aligned(1024))) char tiles[2 * RT * L::kStride];
     char *const q_tile = tiles, *const g_tile = tiles + RT * L::kStride;
     __shared__ __attribute__((aligned(16))) float stats[2][RT];  // lse, D
-    __shared__ float scratch[kWaves][32 * 32];
+    __shared__ float scratch[kWaves][kScratch];
     __shared__ int bad_tile;
     const Shape& a = f.s;
     const int lane = lane_id(), wave = static_cast<int>(threadIdx.x) / kWave, half = lane >> 5, col = lane & 31;
     int id = by_xcd(static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x));
-    int tile, chunk = 0;
-    if (FAR) {
-        chunk = id % f.far_chunks;
-        id /= f.far_chunks;
-        tile = id % f.far_tiles;
-        id /= f.far_tiles;
-    } else {
-        tile = id % f.key_tiles;
-        id /= f.key_tiles;
-    }
+    const int chunks = SHARE && far ? f.far_chunks : 1, chunk = id % chunks;
+    id /= chunks;
+    const int count = SHARE && far ? f.far_tiles : (a.total + kOwn - 1) / kOwn, tile = id % count;
+    id /= count;
     const int g = id % a.groups, b = id / a.groups;
     const int before = a.total - a.length;
-    const int wave_key = FAR ? tile * 32 : tile * kRows + wave * 32, key = wave_key + col;
+    const int key0 = tile * kOwn, wave_key = SHARE ? key0 : key0 + wave * 32, key = wave_key + col;
     const uint8_t* valid = a.valid ? a.valid + static_cast<int64_t>(b) * a.total : nullptr;
-    const bool key_ok = key < a.total && (!valid || valid[key]) && (!FAR || key < a.sinks);
+    const bool key_ok = key < a.total && (!valid || valid[key]) && (!(SHARE && far) || key < a.sinks);
     const T* q = static_cast<const T*>(a.q) + b * a.qs.batch + g * a.shared * a.qs.head;
     const T* k = static_cast<const T*>(a.k) + b * a.ks.batch + key * a.ks.position + g * a.ks.head;
     const T* v = static_cast<const T*>(a.v) + b * a.vs.batch + key * a.vs.position + g * a.vs.head;
@@ -245,42 +245,49 @@ __global__ __launch_bounds__(kThreads, NB <= 2 ? 2 : 1) void window_dkv_kernel(B
     // queries that see key j: from begins(j) on, up to ends(j)
     auto begins = [&](int j) { return max(j - before, 0); };
     auto ends = [&](int j) { return max(j - before + a.window, 0); };
-    const int key0 = tile * kRows;
-    int from, to;
-    if (FAR) {
-        from = f.far_first + chunk * f.far_rows;
-        to = min(from + f.far_rows, a.length);
-    } else {
-        from = begins(key0);
-        to = min(ends(min(key0 + kRows, a.total) - 1), a.length);
-    }
+    const int from = SHARE && far ? f.far_first : begins(key0);
+    const int to = SHARE && far ? a.length : min(ends(min(key0 + kOwn, a.total) - 1), a.length);
     const bool wave_keys = __ballot(key_ok) != 0, wave_whole = __ballot(key_ok) == ~0ull;
     const int key_begin = begins(key), key_end = ends(key);
     const int wave_begin = begins(wave_key), wave_end = ends(wave_key);
     const int wave_last_begin = begins(wave_key + 31), wave_last_end = ends(wave_key + 31);
-    const int first = from & ~(RT - 1), walk = to > from ? (to - first + RT - 1) / RT : 0, steps = walk * a.shared;
+    const int first = from & ~(RT - 1), walk = to > from ? (to - first + RT - 1) / RT : 0;
+    const int64_t whole = static_cast<int64_t>(walk) * a.shared;
+    const int t0 = static_cast<int>(whole * chunk / chunks), t1 = static_cast<int>(whole * (chunk + 1) / chunks);
 
     Staged<T, NB, RT> next_q, next_g;
     const uint8_t* shown_at = valid ? valid + before : static_cast<const uint8_t*>(a.q);  // any byte where all are valid
-    const float* stat_at = (static_cast<int>(threadIdx.x) / RT % 2 ? f.delta : f.lse) + stat;
-    uint8_t next_ok = 0;
-    float next_stat = 0.0f;
-    int next_head = 0, next_p = first;  // of the tile to fetch
+    constexpr int SE = (2 * RT + kThreads - 1) / kThreads;  // statistics a thread brings
+    uint8_t next_ok[RW] = {};
+    float next_stat[SE] = {};
+    int next_head = walk ? t0 / walk : 0, next_p = first + (walk ? t0 % walk : 0) * RT;  // of the tile to fetch
     auto fetch = [&]() {
         const int p0 = next_p, last = a.length - 1 - p0;
-        next_ok = shown_at[valid ? min(p0 + lane, a.length - 1) : 0];
-        next_stat = stat_at[static_cast<int64_t>(next_head) * a.length + p0 + min(static_cast<int>(threadIdx.x) % RT, last)];
+#pragma unroll
+        for (int w = 0; w < RW; ++w) next_ok[w] = shown_at[valid ? min(p0 + 64 * w + lane, a.length - 1) : 0];
+#pragma unroll
+        for (int i = 0; i < SE; ++i) {
+            const int n = static_cast<int>(threadIdx.x) + i * kThreads;
+            next_stat[i] = (n / RT % 2 ? f.delta : f.lse)[stat + static_cast<int64_t>(next_head) * a.length + p0 + min(n % RT, last)];
+        }
         next_q.load(q + next_head * a.qs.head + p0 * a.qs.position, a.qs.position, last, a.width);
         next_g.load(d_out + static_cast<int64_t>(next_head) * a.width + p0 * out_row, out_row, last, a.width);
         next_p += RT;
         if (next_p >= to) next_p = first, ++next_head;
     };
-    if (steps) fetch();
-    int p0 = first;
-    for (int t = 0; t < steps; ++t, p0 = p0 + RT >= to ? first : p0 + RT) {
-        const uint64_t shown = __ballot(lane < RT && p0 + lane < a.length && (!valid || next_ok)), every = low_bits(RT);
+    int p0 = next_p;
+    if (t0 < t1) fetch();
+    for (int t = t0; t < t1; ++t, p0 = p0 + RT >= to ? first : p0 + RT) {
+        uint64_t shown[RW];
+        bool every = true, some = false;
+#pragma unroll
+        for (int w = 0; w < RW; ++w) {
+            const int r = 64 * w + lane;
+            shown[w] = __ballot(r < RT && p0 + r < a.length && (!valid || next_ok[w]));
+            every = every && shown[w] == low_bits(RT - 64 * w), some = some || shown[w];
+        }
         // every key of the workgroup is seen by every row of the tile
-        const bool all = !FAR && shown == every && !valid && p0 >= begins(key0 + kRows - 1) && p0 + RT <= ends(key0) && key0 + kRows <= a.total;
+        const bool all = !far && every && !valid && p0 >= begins(key0 + kOwn - 1) && p0 + RT <= ends(key0) && key0 + kOwn <= a.total;
         __syncthreads();
         if (!all) {
             const bool bad_q = next_q.keep(shown), bad_g = next_g.keep(shown);
@@ -288,26 +295,29 @@ __global__ __launch_bounds__(kThreads, NB <= 2 ? 2 : 1) void window_dkv_kernel(B
         }
         next_q.store(q_tile, a.width);
         next_g.store(g_tile, a.width);
-        if (threadIdx.x < 2 * RT) stats[static_cast<int>(threadIdx.x) / RT][static_cast<int>(threadIdx.x) % RT] = next_stat;
-        __syncthreads();
-        if (t + 1 < steps) fetch();
-        if (!shown || !wave_keys) continue;
-        if (FAR ? (t % kWaves != wave || p0 + RT <= wave_end) : (p0 + RT <= wave_begin || p0 >= wave_last_end)) continue;
-        const bool masked = FAR || !(shown == every && wave_whole && p0 >= wave_last_begin && p0 + RT <= wave_end);
-        uint64_t seen = every;
-        if (masked) {
-            const uint64_t by_place = FAR ? ~low_bits(max(key_end, from) - p0) & low_bits(to - p0)
-                                          : ~low_bits(key_begin - p0) & low_bits(key_end - p0);
-            seen = key_ok ? by_place & shown : 0ull;
-        }
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
+        for (int i = 0; i < SE; ++i) {
+            const int n = static_cast<int>(threadIdx.x) + i * kThreads;
+            if (n < 2 * RT) stats[n / RT][n % RT] = next_stat[i];
+        }
+        __syncthreads();
+        if (t + 1 < t1) fetch();
+        if (!some || !wave_keys) continue;
+        auto block = [&](int rb, uint32_t block_shown) {
+            const int pb = p0 + rb * 32;
+            if (far ? pb + 32 <= wave_end : (pb + 32 <= wave_begin || pb >= wave_last_end)) return;
+            const bool masked = far || !(block_shown == ~0u && wave_whole && pb >= wave_last_begin && pb + 32 <= wave_end);
+            uint32_t seen = ~0u;
+            if (masked) {
+                const uint64_t by_place = far ? ~low_bits(key_end - pb) : ~low_bits(key_begin - pb) & low_bits(key_end - pb);
+                seen = key_ok ? static_cast<uint32_t>(by_place) & block_shown : 0u;
+            }
             f32x16 s = f32x16(0.0f), d = f32x16(0.0f);
             mma_rows<T, NB>(s, q_tile, rb * 32, kf);
             mma_rows<T, NB>(d, g_tile, rb * 32, vf);
 #pragma unroll
             for (int n = 0; n < 4; ++n) {
-                const float4 lse = *reinterpret_cast<const float4*>(&stats[0][rb * 32 + 8 * n + 4 * half]);
+            const float4 lse = *reinterpret_cast<const float4*>(&stats[0][rb * 32 + 8 * n + 4 * half]);
                 const float4 del = *reinterpret_cast<const float4*>(&stats[1][rb * 32 + 8 * n + 4 * half]);
                 const float x[4] = {lse.x, lse.y, lse.z, lse.w}, y[4] = {del.x, del.y, del.z, del.w};
 #pragma unroll
@@ -316,9 +326,8 @@ __global__ __launch_bounds__(kThreads, NB <= 2 ? 2 : 1) void window_dkv_kernel(B
                     d[4 * n + i] = s[4 * n + i] * (d[4 * n + i] - y[i]);
                 }
             }
-            const uint32_t block = static_cast<uint32_t>(seen >> (32 * rb));
             if (masked) {
-                const uint32_t mine = block >> (4 * half);
+                const uint32_t mine = seen >> (4 * half);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     s[r] = bit_of(mine, r) ? s[r] : 0.0f;
@@ -327,19 +336,26 @@ __global__ __launch_bounds__(kThreads, NB <= 2 ? 2 : 1) void window_dkv_kernel(B
             }
             range.fit(d, dk);
             if (masked && bad_tile == t) {
-                seen_acc<T, NB>(dv, g_tile, rb * 32, s, block, scratch[wave]);
-                seen_acc<T, NB>(dk, q_tile, rb * 32, d, block, scratch[wave]);
+                seen_acc<T, NB>(dv, g_tile, rb * 32, s, seen, scratch[wave]);
+                seen_acc<T, NB>(dk, q_tile, rb * 32, d, seen, scratch[wave]);
             } else {
                 mma_acc<T, NB>(dv, g_tile, rb * 32, s);
                 mma_acc<T, NB>(dk, q_tile, rb * 32, d);
             }
+        };
+        if (SHARE) {
+            const int rb = (wave - t * RB) & (kWaves - 1);
+            if (rb < RB) block(rb, static_cast<uint32_t>(shown[RW > 1 ? rb / 2 : 0] >> (32 * (rb & 1))));
+        } else {
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) block(rb, static_cast<uint32_t>(shown[0] >> (32 * rb)));
         }
     }
     const float unlift = std::is_same<T, f16>::value ? 1.0f / 256.0f : 1.0f;
     const float by = a.scale * range.back() * unlift;
     const int64_t far_keys = static_cast<int64_t>(f.far_tiles) * 32;
-    if (FAR) {
-        // [32 keys][2][32 NB] floats fill the tiles' LDS
+    if constexpr (SHARE) {
+        // [32 keys][2][32 NB] floats in the tiles' place
         static_assert(2 * RT * L::kStride >= 32 * 2 * 32 * NB * 4, "the waves' sums need the tiles' room");
         float* sums = reinterpret_cast<float*>(tiles);
         for (int w = 0; w < kWaves; ++w) {
@@ -356,15 +372,28 @@ __global__ __launch_bounds__(kThreads, NB <= 2 ? 2 : 1) void window_dkv_kernel(B
                 }
         }
         __syncthreads();
-        float* part = f.far_parts + (((static_cast<int64_t>(chunk) * a.batch + b) * a.groups + g) * far_keys + wave_key) * 2 * a.width;
-        for (int i = threadIdx.x; i < 64 * a.width; i += kThreads) {
-            const int line = i / a.width;
-            part[i] = sums[line * 32 * NB + i - line * a.width];
+        if (far) {
+            float* part = f.far_parts + (((static_cast<int64_t>(chunk) * a.batch + b) * a.groups + g) * far_keys + wave_key) * 2 * a.width;
+            for (int i = threadIdx.x; i < 64 * a.width; i += kThreads) {
+                const int line = i / a.width;
+                part[i] = sums[line * 32 * NB + i - line * a.width];
+            }
+            return;
+        }
+        const float* part = f.far_parts + ((static_cast<int64_t>(b) * a.groups + g) * far_keys + key0) * 2 * a.width;
+        for (int i = threadIdx.x; i < 64 * (8 * NB); i += kThreads) {  // four columns of a key's dk or dv each
+            const int line = i / (8 * NB), e = i % (8 * NB) * 4, at = key0 + line / 2;
+            T* out = static_cast<T*>(line % 2 ? f.dv : f.dk);
+            if (at >= a.total || e >= a.width || !out) continue;
+            float x[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = sums[line * 32 * NB + e + j] + (key0 < far_keys ? part[line * a.width + e + j] : 0.0f);
+            store_four(out + ((static_cast<int64_t>(b) * a.total + at) * a.groups + g) * a.width, e, a.width, x);
         }
         return;
     }
     if (key >= a.total) return;
-    const float* far = f.far_parts + (((static_cast<int64_t>(b) * a.groups + g) * far_keys + key) * 2) * a.width;
+    const float* part = f.far_parts + (((static_cast<int64_t>(b) * a.groups + g) * far_keys + key) * 2) * a.width;
     const int64_t cell = ((static_cast<int64_t>(b) * a.total + key) * a.groups + g) * a.width;
 #pragma unroll
     for (int n = 0; n < NB; ++n)
@@ -374,10 +403,9 @@ __global__ __launch_bounds__(kThreads, NB <= 2 ? 2 : 1) void window_dkv_kernel(B
             float x[4], y[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[i] = dk[n][4 * qd + i] * by, y[i] = dv[n][4 * qd + i] * unlift;
-            if (key < far_keys) {
+            if (key < far_keys && e < a.width) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (e < a.width) x[i] += far[e + i], y[i] += far[a.width + e + i];
+                for (int i = 0; i < 4; ++i) x[i] += part[e + i], y[i] += part[a.width + e + i];
             }
             if (f.dk) store_four(static_cast<T*>(f.dk) + cell, e, a.width, x);
             if (f.dv) store_four(static_cast<T*>(f.dv) + cell, e, a.width, y);
@@ -394,23 +422,22 @@ __global__ __launch_bounds__(kThreads) void window_far_kernel(float* parts, int 
     parts[i] = sum;
 }
 
-// Positions past the sinks' window, in chunks: two workgroups for each compute unit where
-// the rows suffice, none under four tiles.
+// The sinks' rows past their window, in chunks: two workgroups for each compute unit where
+// the rows suffice, none under two tiles of 128.
 void far_of(const Shape& s, Backward& f) {
     const int64_t before = s.total - s.length, first = std::max<int64_t>(s.window - before, 0);
     if (s.sinks == 0 || first >= s.length) return;
     f.far_tiles = (s.sinks + 31) / 32;
     f.far_first = static_cast<int>(first);
-    const int64_t span = s.length - first, heads = static_cast<int64_t>(s.batch) * s.groups * f.far_tiles;
-    const int64_t chunks = std::max<int64_t>(1, std::min<int64_t>((span + 255) / 256, (512 + heads - 1) / heads));
-    f.far_rows = static_cast<int>(((span + chunks - 1) / chunks + 63) / 64 * 64);
-    f.far_chunks = static_cast<int>((span + f.far_rows - 1) / f.far_rows);
+    const int64_t span = (s.length - first) * s.shared, heads = static_cast<int64_t>(s.batch) * s.groups * f.far_tiles;
+    f.far_chunks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((span + 255) / 256, (512 + heads - 1) / heads)));
 }
 
 int64_t far_each(const Shape& s, const Backward& f) {
     return static_cast<int64_t>(s.batch) * s.groups * f.far_tiles * 32 * 2 * s.width;
 }
 size_t far_values(const Shape& s, const Backward& f) { return static_cast<size_t>(f.far_chunks) * far_each(s, f); }
+
 
 template <typename T, int NB>
 int run(const Backward& f, hipStream_t stream) {
@@ -424,7 +451,7 @@ int run(const Backward& f, hipStream_t stream) {
     if (rc != KOEMI_OK || (!f.dk && !f.dv)) return rc;
     if (f.far_chunks) {
         hipLaunchKernelGGL((window_dkv_kernel<T, NB, true>), dim3(static_cast<unsigned>(heads * f.far_tiles * f.far_chunks)),
-                           dim3(kThreads), 0, stream, f);
+                           dim3(kThreads), 0, stream, f, 1);
         rc = check_launch(what);
         if (rc != KOEMI_OK) return rc;
         if (f.far_chunks > 1) {
@@ -434,7 +461,14 @@ int run(const Backward& f, hipStream_t stream) {
             if (rc != KOEMI_OK) return rc;
         }
     }
-    hipLaunchKernelGGL((window_dkv_kernel<T, NB, false>), dim3(static_cast<unsigned>(heads * f.key_tiles)), dim3(kThreads), 0, stream, f);
+    // Shared keys cost about 1.7 times the work on a full chip ([1, 16384], 256 wide workgroups: 1347 us against 771)
+    // and spread it where the wide ones leave compute units idle (70 of them at [5, 777]: 31.6 us against 45.7).
+    const int64_t wide = heads * ((f.s.total + kRows - 1) / kRows);
+    if (wide < 160)
+        hipLaunchKernelGGL((window_dkv_kernel<T, NB, true>), dim3(static_cast<unsigned>(heads * ((f.s.total + 31) / 32))),
+                           dim3(kThreads), 0, stream, f, 0);
+    else
+        hipLaunchKernelGGL((window_dkv_kernel<T, NB, false>), dim3(static_cast<unsigned>(wide)), dim3(kThreads), 0, stream, f, 0);
     return check_launch(what);
 }
 
@@ -485,7 +519,6 @@ extern "C" int koemi_window_attention_backward(const void* queries, const void* 
     if (length && (!output || !lse || !grad_output)) return fail(KOEMI_ERR_INVALID, "%s: null pointer", what);
     f.out = output, f.rest = dtype == KOEMI_F32 ? nullptr : rest, f.lse = lse, f.d_out = grad_output, f.dq = grad_queries, f.dk = grad_keys, f.dv = grad_values;
     f.row_tiles = static_cast<int>((length * f.s.shared + kRows - 1) / kRows);
-    f.key_tiles = static_cast<int>((total + kRows - 1) / kRows);
     far_of(f.s, f);
     const size_t cells = static_cast<size_t>(batch) * heads * length;
     const size_t need = (cells + far_values(f.s, f)) * 4;
