@@ -1030,7 +1030,7 @@ int koemi_moe_experts_backward(const void* grad_output, const void* context, con
  * infinite where nothing is seen. Workspace: koemi_window_attention_workspace_bytes, no zeroing
  * needed, 4-byte aligned. Refused: widths over 256, 2^29 rows (positions x heads / groups)
  * of a key head and 2^24 tiles of 128 of them and more, rows (width, strides, pointers) that
- * are not whole 16-byte pieces, 16-byte aligned and less than 2^25 bytes apart. */
+ * are not whole 16-byte pieces, 16-byte aligned and less than 2^24 bytes apart. */
 size_t koemi_window_attention_workspace_bytes(int64_t batch, int64_t length, int64_t total, int64_t heads, int64_t groups,
                                               int64_t width, int64_t window, int64_t sinks, int dtype);
 int koemi_window_attention_forward(const void* queries, const void* keys, const void* values, const uint8_t* valid,

@@ -38,12 +38,9 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 4 : NB == 2 ? 3 : NB <= 4 ? 2 :
     __shared__ int bad_tile, any_row;
     const Shape& a = f.s;
     const int lane = lane_id(), wave = static_cast<int>(threadIdx.x) / kWave, half = lane >> 5, col = lane & 31;
-    int id = by_xcd(static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x));
-    const int split = id % f.splits;
-    id /= f.splits;
-    const int tile = id % f.row_tiles;
-    id /= f.row_tiles;
-    const int g = id % a.groups, b = id / a.groups;
+    const Place at_work(static_cast<int>(blockIdx.x), a.batch * a.groups, f.row_tiles * f.splits);
+    const int split = at_work.part % f.splits, tile = at_work.part / f.splits;
+    const int g = at_work.head % a.groups, b = at_work.head / a.groups;
     const int rows = a.length * a.shared, before = a.total - a.length;
     const int row = tile * kRows + wave * 32 + col, last_row = min(tile * kRows + kRows, rows) - 1;
     const int position = position_of(a, min(row, rows - 1)), place = before + position;
@@ -117,7 +114,7 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 4 : NB == 2 ? 3 : NB <= 4 ? 2 :
                 for (int kb = 0; kb < KB; ++kb) {
                     const uint32_t mine = static_cast<uint32_t>(seen >> (32 * kb)) >> (4 * half);
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[kb][r] = bit_of(mine, r) ? s[kb][r] : -INFINITY;
+                    for (int r = 0; r < 16; ++r) s[kb][r] = where_seen(mine, r, s[kb][r], -INFINITY);
                 }
             }
             float high = s[0][0];
@@ -126,7 +123,8 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 4 : NB == 2 ? 3 : NB <= 4 ? 2 :
 #pragma unroll
                 for (int r = 0; r < 16; ++r) high = fmaxf(high, s[kb][r]);
             high = fmaxf(top, max_of_halves(high));
-            if (__any(high > top)) {
+            // The maximum only keeps the exponentials in range: while no row's grows by 2^6, all keep the one they have.
+            if (__any(high * c > top * c + 6.0f || (top == -INFINITY && high > top))) {
                 const float shrink = high > top ? __builtin_amdgcn_exp2f((top - high) * c) : 1.0f;
 #pragma unroll
                 for (int n = 0; n < NB; ++n) acc[n] *= shrink;
@@ -286,12 +284,12 @@ int shape_of(const char* what, const void* queries, const void* keys, const void
         s.qs = {strides[0], strides[1], strides[2]};
         s.ks = {strides[3], strides[4], strides[5]};
         s.vs = {strides[6], strides[7], strides[8]};
-        bool fits = width * size % 16 == 0 && heads * width * size < (1 << 25);
+        bool fits = width * size % 16 == 0 && heads * width * size < (1 << 24);
         for (int i = 0; i < 9; ++i) fits = fits && strides[i] * size % 16 == 0 && strides[i] >= 0;
-        for (int i = 1; i < 9; i += 3) fits = fits && strides[i] * size < (1 << 25);
+        for (int i = 1; i < 9; i += 3) fits = fits && strides[i] * size < (1 << 24);
         for (const void* p : {queries, keys, values}) fits = fits && reinterpret_cast<uintptr_t>(p) % 16 == 0;
         if (!fits)
-            return fail(KOEMI_ERR_UNSUPPORTED, "%s: rows must be whole 16-byte pieces, 16-byte aligned and less than 2^25 bytes apart", what);
+            return fail(KOEMI_ERR_UNSUPPORTED, "%s: rows must be whole 16-byte pieces, 16-byte aligned and less than 2^24 bytes apart", what);
     }
     s.batch = static_cast<int>(batch), s.length = static_cast<int>(length), s.total = static_cast<int>(total);
     s.groups = static_cast<int>(groups), s.shared = static_cast<int>(shared), s.width = static_cast<int>(width);

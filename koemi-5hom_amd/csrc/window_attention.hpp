@@ -37,7 +37,7 @@ struct Strides {
 };
 
 struct Shape {
-    // rows are whole, aligned 16-byte pieces, less than 2^25 bytes apart
+    // rows are whole, aligned 16-byte pieces, less than 2^24 bytes apart
     const void* q;
     const void* k;
     const void* v;
@@ -77,7 +77,10 @@ struct Tile {
 };
 
 // The lowest n bits, n of any sign.
-__device__ __forceinline__ uint64_t low_bits(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; }
+__device__ __forceinline__ uint32_t low_bits32(int n) { return n >= 32 ? ~0u : (1u << (max(n, 0) & 31)) - 1u; }
+__device__ __forceinline__ uint64_t low_bits(int n) {
+    return static_cast<uint64_t>(low_bits32(n)) | static_cast<uint64_t>(low_bits32(n < 32 ? 0 : n - 32)) << 32;
+}
 
 // The largest sizes, by their bits, of values seen so far: an infinity or NaN among them?
 template <typename T>
@@ -127,7 +130,7 @@ struct Staged {
         const uint32_t bytes = static_cast<uint32_t>(stride) * static_cast<uint32_t>(sizeof(T));
 #pragma unroll
         for (int n = 0; n < kEach; ++n) {
-            const uint32_t at = static_cast<uint32_t>(min(row(n), last)) * bytes + (unit(n) * kPer16<T> < width ? unit(n) * 16u : 0u);
+            const uint32_t at = __umul24(static_cast<uint32_t>(min(row(n), last)), bytes) + (unit(n) * kPer16<T> < width ? unit(n) * 16u : 0u);
             piece[n] = *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(first) + at);
         }
     }
@@ -282,15 +285,33 @@ __device__ __forceinline__ uint64_t keys_seen(const Shape& a, int place, int key
     return low_bits(rel + 1) & (~low_bits(rel - a.window + 1) | low_bits(a.sinks - key0));
 }
 
-// The 16 bits of a 32-row block's mask that the lane's registers hold, from bit 0 on.
-__device__ __forceinline__ bool bit_of(uint32_t seen_half, int r) { return (seen_half >> (8 * (r / 4) + r % 4)) & 1u; }
-
-// A workgroup's place: consecutive workgroups go to the eight XCDs in turn, so those that
-// share keys (neighbours) are given to one of them.
-__device__ __forceinline__ int by_xcd(int id, int count) {
-    const int even = count & ~7;
-    return id < even ? (id & 7) * (even >> 3) + (id >> 3) : id;
+// x where the lane's register r of a 32-row block is seen (seen_half: the block's mask from
+// the lane's half on), else `other`.
+__device__ __forceinline__ float where_seen(uint32_t seen_half, int r, float x, float other) {
+    const uint32_t all = static_cast<uint32_t>(__builtin_amdgcn_sbfe(static_cast<int>(seen_half), 8 * (r / 4) + r % 4, 1));
+    return __uint_as_float((all & __float_as_uint(x)) | (~all & __float_as_uint(other)));
 }
+
+// A workgroup's key head (of `heads` in all, batch rows times key heads) and its part of it.
+// Consecutive workgroups go to the eight XCDs in turn, and parts of a head read the same
+// keys: so each XCD takes whole heads, every eighth one (rows of a batch differ in
+// length), and the heads left over are cut into eight runs of parts.
+struct Place {
+    int head, part;
+    __device__ __forceinline__ Place(int id, int heads, int parts) {
+        const int even = (heads & ~7) * parts;
+        if (id < even) {
+            head = (id >> 3) / parts * 8 + (id & 7);
+            part = (id >> 3) % parts;
+        } else {
+            const int rest = heads * parts - even, whole = rest & ~7;
+            id -= even;
+            id = id < whole ? (id & 7) * (whole >> 3) + (id >> 3) : id;
+            head = (heads & ~7) + id / parts;
+            part = id % parts;
+        }
+    }
+};
 
 // Key tiles of KT that rows at places first .. last (of the keys' positions) see: the
 // sinks' before the window, then the window's.

@@ -78,10 +78,8 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 4 : NB == 2 && sizeof(T) == 2 ?
     __shared__ int bad_tile, any_row;
     const Shape& a = f.s;
     const int lane = lane_id(), wave = static_cast<int>(threadIdx.x) / kWave, half = lane >> 5, col = lane & 31;
-    int id = by_xcd(static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x));
-    const int tile = id % f.row_tiles;
-    id /= f.row_tiles;
-    const int g = id % a.groups, b = id / a.groups;
+    const Place at_work(static_cast<int>(blockIdx.x), a.batch * a.groups, f.row_tiles);
+    const int tile = at_work.part, g = at_work.head % a.groups, b = at_work.head / a.groups;
     const int rows = a.length * a.shared, before = a.total - a.length;
     const int row = tile * kRows + wave * 32 + col, last_row = min(tile * kRows + kRows, rows) - 1;
     const int position = position_of(a, min(row, rows - 1)), place = before + position;
@@ -168,7 +166,7 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 4 : NB == 2 && sizeof(T) == 2 ?
                 if (masked) {
                     const uint32_t mine = static_cast<uint32_t>(seen >> (32 * kb)) >> (4 * half);
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) d[r] = bit_of(mine, r) ? d[r] : 0.0f;
+                    for (int r = 0; r < 16; ++r) d[r] = where_seen(mine, r, d[r], 0.0f);
                 }
                 range.fit(d, acc);
                 if (masked && bad_tile == t)
@@ -213,12 +211,10 @@ __global__ __launch_bounds__(kThreads, NB <= 2 ? 2 : 1) void window_dkv_kernel(B
     __shared__ int bad_tile;
     const Shape& a = f.s;
     const int lane = lane_id(), wave = static_cast<int>(threadIdx.x) / kWave, half = lane >> 5, col = lane & 31;
-    int id = by_xcd(static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x));
-    const int chunks = SHARE && far ? f.far_chunks : 1, chunk = id % chunks;
-    id /= chunks;
-    const int count = SHARE && far ? f.far_tiles : (a.total + kOwn - 1) / kOwn, tile = id % count;
-    id /= count;
-    const int g = id % a.groups, b = id / a.groups;
+    const int chunks = SHARE && far ? f.far_chunks : 1, own_tiles = SHARE && far ? f.far_tiles : (a.total + kOwn - 1) / kOwn;
+    const Place at_work(static_cast<int>(blockIdx.x), a.batch * a.groups, own_tiles * chunks);
+    const int chunk = at_work.part % chunks, tile = at_work.part / chunks;
+    const int g = at_work.head % a.groups, b = at_work.head / a.groups;
     const int before = a.total - a.length;
     const int key0 = tile * kOwn, wave_key = SHARE ? key0 : key0 + wave * 32, key = wave_key + col;
     const uint8_t* valid = a.valid ? a.valid + static_cast<int64_t>(b) * a.total : nullptr;
@@ -330,8 +326,8 @@ __global__ __launch_bounds__(kThreads, NB <= 2 ? 2 : 1) void window_dkv_kernel(B
                 const uint32_t mine = seen >> (4 * half);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    s[r] = bit_of(mine, r) ? s[r] : 0.0f;
-                    d[r] = bit_of(mine, r) ? d[r] : 0.0f;
+                    s[r] = where_seen(mine, r, s[r], 0.0f);
+                    d[r] = where_seen(mine, r, d[r], 0.0f);
                 }
             }
             range.fit(d, dk);

@@ -112,12 +112,12 @@ def window_attention(queries: Tensor, keys: Tensor, values: Tensor, valid_mask: 
 
 def _pieces(tensor: Tensor) -> Tensor:
     """``tensor`` [B, L, H, D] where the kernels can read its rows as they lie (whole, aligned
-    16-byte pieces, less than 2^25 bytes apart), else a copy that they can, its width padded
+    16-byte pieces, less than 2^24 bytes apart), else a copy that they can, its width padded
     with zeros."""
 
     size, strides = tensor.element_size(), tensor.stride()
     if (strides[3] == 1 and tensor.shape[3] * size % 16 == 0 and tensor.data_ptr() % 16 == 0
-            and all(s * size % 16 == 0 for s in strides[:3]) and strides[1] * size < 1 << 25):
+            and all(s * size % 16 == 0 for s in strides[:3]) and strides[1] * size < 1 << 24):
         return tensor
     short = -tensor.shape[3] % (16 // size)
     return torch.nn.functional.pad(tensor, (0, short)) if short else tensor.contiguous()
