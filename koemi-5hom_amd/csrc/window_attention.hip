@@ -132,20 +132,25 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 4 : NB == 2 ? 3 : NB <= 4 ? 2 :
                 top = high;
             }
             const float base = (top == -INFINITY ? 0.0f : top * c) - kLift<T>;
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
+            auto terms = [&](int kb) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     s[kb][r] = __builtin_amdgcn_exp2f(fmaf(s[kb][r], c, -base));
                     sum += s[kb][r];
                 }
+            };
             if (masked && bad_tile == t) {
 #pragma unroll
-                for (int kb = 0; kb < KB; ++kb)
+                for (int kb = 0; kb < KB; ++kb) {
+                    terms(kb);
                     seen_acc<T, NB>(acc, v_tile, kb * 32, s[kb], static_cast<uint32_t>(seen >> (32 * kb)), scratch[wave]);
-            } else {
+                }
+            } else {  // one block's products run beside the next one's exponentials
 #pragma unroll
-                for (int kb = 0; kb < KB; ++kb) mma_acc<T, NB>(acc, v_tile, kb * 32, s[kb]);
+                for (int kb = 0; kb < KB; ++kb) {
+                    terms(kb);
+                    mma_acc<T, NB>(acc, v_tile, kb * 32, s[kb]);
+                }
             }
         }
     }

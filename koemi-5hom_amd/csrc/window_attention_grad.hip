@@ -163,14 +163,14 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 4 : NB == 2 && sizeof(T) == 2 ?
                 mma_rows<T, NB>(d, v_tile, kb * 32, gf);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) d[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse)) * (d[r] - delta);
+                const uint32_t block = static_cast<uint32_t>(seen >> (32 * kb));
                 if (masked) {
-                    const uint32_t mine = static_cast<uint32_t>(seen >> (32 * kb)) >> (4 * half);
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) d[r] = where_seen(mine, r, d[r], 0.0f);
+                    for (int r = 0; r < 16; ++r) d[r] = where_seen(block >> (4 * half), r, d[r], 0.0f);
                 }
                 range.fit(d, acc);
                 if (masked && bad_tile == t)
-                    seen_acc<T, NB>(acc, k_tile, kb * 32, d, static_cast<uint32_t>(seen >> (32 * kb)), scratch[wave]);
+                    seen_acc<T, NB>(acc, k_tile, kb * 32, d, block, scratch[wave]);
                 else
                     mma_acc<T, NB>(acc, k_tile, kb * 32, d);
             }
@@ -299,21 +299,15 @@ __global__ __launch_bounds__(kThreads, NB <= 2 ? 2 : 1) void window_dkv_kernel(B
         __syncthreads();
         if (t + 1 < t1) fetch();
         if (!some || !wave_keys) continue;
-        auto block = [&](int rb, uint32_t block_shown) {
-            const int pb = p0 + rb * 32;
-            if (far ? pb + 32 <= wave_end : (pb + 32 <= wave_begin || pb >= wave_last_end)) return;
-            const bool masked = far || !(block_shown == ~0u && wave_whole && pb >= wave_last_begin && pb + 32 <= wave_end);
-            uint32_t seen = ~0u;
-            if (masked) {
-                const uint64_t by_place = far ? ~low_bits(key_end - pb) : ~low_bits(key_begin - pb) & low_bits(key_end - pb);
-                seen = key_ok ? static_cast<uint32_t>(by_place) & block_shown : 0u;
-            }
-            f32x16 s = f32x16(0.0f), d = f32x16(0.0f);
+        auto products = [&](int rb, f32x16& s, f32x16& d) {
+            s = d = f32x16(0.0f);
             mma_rows<T, NB>(s, q_tile, rb * 32, kf);
             mma_rows<T, NB>(d, g_tile, rb * 32, vf);
+        };
+        auto terms = [&](int rb, f32x16& s, f32x16& d) {
 #pragma unroll
             for (int n = 0; n < 4; ++n) {
-            const float4 lse = *reinterpret_cast<const float4*>(&stats[0][rb * 32 + 8 * n + 4 * half]);
+                const float4 lse = *reinterpret_cast<const float4*>(&stats[0][rb * 32 + 8 * n + 4 * half]);
                 const float4 del = *reinterpret_cast<const float4*>(&stats[1][rb * 32 + 8 * n + 4 * half]);
                 const float x[4] = {lse.x, lse.y, lse.z, lse.w}, y[4] = {del.x, del.y, del.z, del.w};
 #pragma unroll
@@ -322,7 +316,18 @@ __global__ __launch_bounds__(kThreads, NB <= 2 ? 2 : 1) void window_dkv_kernel(B
                     d[4 * n + i] = s[4 * n + i] * (d[4 * n + i] - y[i]);
                 }
             }
+        };
+        auto block = [&](int rb, uint32_t block_shown) {
+            const int pb = p0 + rb * 32;
+            if (far ? pb + 32 <= wave_end : (pb + 32 <= wave_begin || pb >= wave_last_end)) return;
+            const bool masked = far || !(block_shown == ~0u && wave_whole && pb >= wave_last_begin && pb + 32 <= wave_end);
+            f32x16 s, d;
+            products(rb, s, d);
+            terms(rb, s, d);
+            uint32_t seen = ~0u;
             if (masked) {
+                const uint64_t by_place = far ? ~low_bits(key_end - pb) : ~low_bits(key_begin - pb) & low_bits(key_end - pb);
+                seen = key_ok ? static_cast<uint32_t>(by_place) & block_shown : 0u;
                 const uint32_t mine = seen >> (4 * half);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
@@ -342,6 +347,22 @@ __global__ __launch_bounds__(kThreads, NB <= 2 ? 2 : 1) void window_dkv_kernel(B
         if (SHARE) {
             const int rb = (wave - t * RB) & (kWaves - 1);
             if (rb < RB) block(rb, static_cast<uint32_t>(shown[RW > 1 ? rb / 2 : 0] >> (32 * (rb & 1))));
+        } else if (NB <= 2 && every && wave_whole && p0 >= wave_last_begin && p0 + RT <= wave_end) {
+            // all seen: without a branch, so that one block's products run beside the other's terms (heads of 64: 115 ->
+            // 109 us; wider ones have no registers for both blocks)
+            f32x16 s[RB], d[RB];
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) products(rb, s[rb], d[rb]);
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+                terms(rb, s[rb], d[rb]);
+                range.fit(d[rb], dk);
+                mma_acc<T, NB>(dv, g_tile, rb * 32, s[rb]);
+                mma_acc<T, NB>(dk, q_tile, rb * 32, d[rb]);
+            }
+        } else if (NB <= 2) {
+#pragma unroll 1
+            for (int rb = 0; rb < RB; ++rb) block(rb, static_cast<uint32_t>(shown[0] >> (32 * rb)));
         } else {
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) block(rb, static_cast<uint32_t>(shown[0] >> (32 * rb)));

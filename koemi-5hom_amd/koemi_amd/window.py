@@ -16,6 +16,7 @@ import ctypes
 import math
 from dataclasses import dataclass
 from functools import lru_cache
+from typing import NamedTuple
 
 import torch
 from torch import Tensor
@@ -40,7 +41,7 @@ def _whole(name: str, value: object, least: int) -> int:
 
 def _scale(scale: object, width: int) -> float:
     if scale is None:
-        return 1.0 / math.sqrt(width)
+        return 1.0 / math.sqrt(max(width, 1))
     if isinstance(scale, bool) or not isinstance(scale, (int, float)) or not 2.0 ** -126 <= scale < 2.0 ** 127:
         raise CudaThinkValidationError("scale must be a positive finite number")
     return float(scale)
@@ -75,23 +76,51 @@ def window_attention(queries: Tensor, keys: Tensor, values: Tensor, valid_mask: 
     inputs' type between two products. Sums run in a fixed order.
     """
 
-    tensors = {"queries": queries, "keys": keys, "values": values}
-    for name, tensor in tensors.items():
+    for name, tensor in (("queries", queries), ("keys", keys), ("values", values)):
         if not isinstance(tensor, Tensor):
             raise CudaThinkValidationError(f"{name} must be a torch.Tensor")
-        if tensor.ndim != 4:
-            raise CudaThinkValidationError(f"{name} must have shape [batch, length, heads, width]")
-        if tensor.dtype not in _SUPPORTED_DTYPES:
-            raise CudaThinkValidationError(f"{name} must be float32, float16 or bfloat16")
-        if tensor.device.type != "cuda":
-            raise CudaThinkValidationError(f"{name} must be on CUDA")
-    if len({t.device for t in tensors.values()}) != 1 or len({t.dtype for t in tensors.values()}) != 1:
+    device, dtype = queries.device, queries.dtype
+    if keys.device != device or values.device != device or keys.dtype != dtype or values.dtype != dtype:
         raise CudaThinkValidationError("queries, keys and values must share a dtype and a device")
-    batch, length, heads, width = queries.shape
-    if keys.shape != values.shape or keys.shape[0] != batch or keys.shape[3] != width:
+    width = queries.shape[-1] if queries.ndim else 1
+    plan = _plan(queries.shape, keys.shape, values.shape, queries.stride(), keys.stride(), values.stride(), dtype, device.type,
+                 _whole("window", window, 1), _whole("sinks", sinks, 0), _scale(scale, width))
+    if valid_mask is not None and (not isinstance(valid_mask, Tensor) or valid_mask.dtype != torch.bool
+                                   or valid_mask.shape != keys.shape[:2] or valid_mask.device != device):
+        raise CudaThinkValidationError("valid_mask must be a bool [batch, total] tensor on the same device")
+    if torch.is_grad_enabled() and (queries.requires_grad or keys.requires_grad or values.requires_grad):
+        return _WindowAttention.apply(queries, keys, values, valid_mask, plan)
+    return _forward(queries, keys, values, valid_mask, plan, False)[0]
+
+
+class _Plan(NamedTuple):
+    """What a call's shapes and numbers come to."""
+
+    sizes: tuple[int, ...]      # batch, length, total, heads, groups, padded width, window, sinks
+    width: int                  # of the heads
+    scale: float
+    code: int                   # of the dtype
+    workspace: tuple[int, int]  # bytes, forward and backward
+    strides: ctypes.Array | None  # of the inputs as they lie, None where one of them has to be copied
+
+
+@lru_cache(maxsize=1024)
+def _plan(query: tuple, key: tuple, value: tuple, query_stride: tuple, key_stride: tuple, value_stride: tuple,
+          dtype: torch.dtype, device: str, window: int, sinks: int, scale: float) -> _Plan:
+    """A call's shapes checked, and what follows from them."""
+
+    for name, shape in (("queries", query), ("keys", key), ("values", value)):
+        if len(shape) != 4:
+            raise CudaThinkValidationError(f"{name} must have shape [batch, length, heads, width]")
+    if dtype not in _SUPPORTED_DTYPES:
+        raise CudaThinkValidationError("queries, keys and values must be float32, float16 or bfloat16")
+    if device != "cuda":
+        raise CudaThinkValidationError("queries, keys and values must be on CUDA")
+    batch, length, heads, width = query
+    if key != value or key[0] != batch or key[3] != width:
         raise CudaThinkValidationError("keys and values must have the same shape [batch, total, key heads, width], "
                                        "batch and width being the queries'")
-    total, groups = keys.shape[1:3]
+    total, groups = key[1:3]
     if total < length:
         raise CudaThinkValidationError("there must be no fewer keys than queries")
     if heads < 1 or groups < 1 or heads % groups:
@@ -100,37 +129,28 @@ def window_attention(queries: Tensor, keys: Tensor, values: Tensor, valid_mask: 
         raise CudaThinkValidationError(f"heads must be 1 to {_MAX_WIDTH} wide")
     if total * (heads // groups) >= 1 << 29 or batch * groups * -(-max(length * heads // groups, total) // 128) >= 1 << 24:
         raise CudaThinkValidationError("too many positions: 2^29 rows of a key head and 2^24 tiles of 128 rows at most")
-    if valid_mask is not None and (not isinstance(valid_mask, Tensor) or valid_mask.dtype != torch.bool
-                                   or valid_mask.shape != (batch, total) or valid_mask.device != queries.device):
-        raise CudaThinkValidationError("valid_mask must be a bool [batch, total] tensor on the same device")
-    window, sinks, scale = _whole("window", window, 1), _whole("sinks", sinks, 0), _scale(scale, width)
+    size = dtype.itemsize
+    if heads * (width + 8) * size >= 1 << 24:
+        raise CudaThinkValidationError("too many heads: a position's must be less than 2^24 bytes")
     _load()
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors.values()):
-        return _WindowAttention.apply(queries, keys, values, valid_mask, window, sinks, scale)
-    return _forward(queries, keys, values, valid_mask, window, sinks, scale, False)[0]
+    padded = -(-width * size // 16) * 16 // size
+    code = _native.dtype_code(dtype)
+    sizes = (batch, length, total, heads, groups, padded, window, sinks)
+    need = (_native.query("koemi_window_attention_workspace_bytes", *sizes, code),
+            _native.query("koemi_window_attention_backward_workspace_bytes", *sizes, code))
+    strides = (query_stride, key_stride, value_stride)
+    in_place = padded == width and all(
+        s[3] == 1 and all(x * size % 16 == 0 for x in s[:3]) and s[1] * size < 1 << 24 for s in strides)
+    flat = [x for s in strides for x in s[:3]]
+    return _Plan(sizes, width, scale, code, need, (ctypes.c_int64 * 9)(*flat) if in_place else None)
 
 
-def _pieces(tensor: Tensor) -> Tensor:
-    """``tensor`` [B, L, H, D] where the kernels can read its rows as they lie (whole, aligned
-    16-byte pieces, less than 2^24 bytes apart), else a copy that they can, its width padded
-    with zeros."""
+def _rows(tensor: Tensor, width: int) -> Tensor:
+    """A copy of ``tensor`` [B, L, H, D] that the kernels can read: contiguous, its width
+    padded with zeros to whole 16-byte pieces, aligned."""
 
-    size, strides = tensor.element_size(), tensor.stride()
-    if (strides[3] == 1 and tensor.shape[3] * size % 16 == 0 and tensor.data_ptr() % 16 == 0
-            and all(s * size % 16 == 0 for s in strides[:3]) and strides[1] * size < 1 << 24):
-        return tensor
-    short = -tensor.shape[3] % (16 // size)
-    return torch.nn.functional.pad(tensor, (0, short)) if short else tensor.contiguous()
-
-
-@lru_cache(maxsize=256)
-def _workspace_bytes(batch: int, length: int, total: int, heads: int, groups: int, width: int, window: int, sinks: int,
-                     dtype: int) -> tuple[int, int]:
-    """Bytes of workspace of a shape: forward, backward."""
-
-    shape = (batch, length, total, heads, groups, width, window, sinks, dtype)
-    return (_native.query("koemi_window_attention_workspace_bytes", *shape),
-            _native.query("koemi_window_attention_backward_workspace_bytes", *shape))
+    short = width - tensor.shape[3]
+    return torch.nn.functional.pad(tensor, (0, short)) if short else tensor.clone(memory_format=torch.contiguous_format)
 
 
 def _strides(*tensors: Tensor) -> ctypes.Array:
@@ -140,67 +160,59 @@ def _strides(*tensors: Tensor) -> ctypes.Array:
     return (ctypes.c_int64 * len(flat))(*flat)
 
 
-def _bytes(need: int, device: torch.device) -> Tensor | None:
-    return torch.empty(need, device=device, dtype=torch.uint8) if need else None
-
-
-def _forward(queries: Tensor, keys: Tensor, values: Tensor, valid_mask: Tensor | None, window: int, sinks: int,
-             scale: float, trained: bool) -> tuple:
+def _forward(queries: Tensor, keys: Tensor, values: Tensor, valid_mask: Tensor | None, plan: _Plan, trained: bool) -> tuple:
     """The output, and with ``trained`` what the gradients need."""
 
-    batch, length, heads, width = queries.shape
-    total, groups = keys.shape[1:3]
-    device, code = queries.device, _native.dtype_code(queries.dtype)
-    q, k, v = _pieces(queries.detach()), _pieces(keys.detach()), _pieces(values.detach())
-    if not q.shape[3] == k.shape[3] == v.shape[3]:
-        raise CudaThinkValidationError("heads must share a width")
+    batch, length, total, heads, groups, padded, window, sinks = plan.sizes
+    device = queries.device
+    q, k, v, strides = queries, keys, values, plan.strides
+    at = (q.data_ptr(), k.data_ptr(), v.data_ptr())
+    if strides is None or at[0] % 16 or at[1] % 16 or at[2] % 16:
+        q, k, v = (_rows(t.detach(), padded) for t in (q, k, v))
+        strides, at = _strides(q, k, v), (q.data_ptr(), k.data_ptr(), v.data_ptr())
     mask = valid_mask.contiguous() if valid_mask is not None else None
-    output = torch.empty((batch, length, heads, q.shape[3]), device=device, dtype=queries.dtype)
-    rest = torch.empty_like(output) if trained and queries.dtype != torch.float32 else None
+    output = torch.empty((batch, length, heads, padded), device=device, dtype=q.dtype)
+    rest = torch.empty_like(output) if trained and q.dtype != torch.float32 else None
     lse = torch.empty((batch, heads, length), device=device, dtype=torch.float32) if trained else None
-    shape = (batch, length, total, heads, groups, q.shape[3], window, sinks)
-    need = _workspace_bytes(*shape, code)[0]
-    workspace = _bytes(need, device)
+    need = plan.workspace[0]
+    workspace = torch.empty(need, device=device, dtype=torch.uint8) if need else None
     with _native.device_guard(device):
-        _native.call("koemi_window_attention_forward", q.data_ptr(), k.data_ptr(), v.data_ptr(), _native.ptr(mask),
-                     _strides(q, k, v), output.data_ptr(), _native.ptr(rest), _native.ptr(lse), *shape, scale, code,
+        _native.call("koemi_window_attention_forward", *at, _native.ptr(mask), strides, output.data_ptr(), _native.ptr(rest),
+                     _native.ptr(lse), batch, length, total, heads, groups, padded, window, sinks, plan.scale, plan.code,
                      _native.ptr(workspace), need, _native.stream_of(device))
-    result = output if q.shape[3] == width else output[..., :width].contiguous()
+    result = output if padded == plan.width else output[..., :plan.width].contiguous()
     return (result, q, k, v, mask, output, rest, lse) if trained else (result,)
 
 
 class _WindowAttention(torch.autograd.Function):
     @staticmethod
     def forward(context, queries: Tensor, keys: Tensor, values: Tensor, valid_mask: Tensor | None,  # type: ignore[override]
-                window: int, sinks: int, scale: float) -> Tensor:
-        result, *kept = _forward(queries, keys, values, valid_mask, window, sinks, scale, True)
+                plan: _Plan) -> Tensor:
+        result, *kept = _forward(queries, keys, values, valid_mask, plan, True)
         context.save_for_backward(*kept)
-        context.window = (window, sinks, scale, queries.shape[3])
+        context.plan = plan
         return result
 
     @staticmethod
     @once_differentiable
     def backward(context, d_output: Tensor):  # type: ignore[override]
         q, k, v, mask, output, rest, lse = context.saved_tensors
-        window, sinks, scale, width = context.window
-        batch, length, heads, padded = q.shape
-        total, groups = k.shape[1:3]
-        device, code = q.device, _native.dtype_code(q.dtype)
-        d_output = torch.nn.functional.pad(d_output, (0, padded - width)) if padded > width else d_output.contiguous()
-        if d_output.data_ptr() % 16:
-            d_output = d_output.clone()
+        plan = context.plan
+        batch, length, total, heads, groups, padded, window, sinks = plan.sizes
+        device, width = q.device, plan.width
+        if padded > width or not d_output.is_contiguous() or d_output.data_ptr() % 16:
+            d_output = _rows(d_output, padded)
         d_q, d_k, d_v = (torch.empty(t.shape, device=device, dtype=t.dtype) if need else None
                          for t, need in zip((q, k, v), context.needs_input_grad))
-        shape = (batch, length, total, heads, groups, padded, window, sinks)
-        need = _workspace_bytes(*shape, code)[1]
-        workspace = _bytes(need, device)
+        need = plan.workspace[1]
+        workspace = torch.empty(need, device=device, dtype=torch.uint8) if need else None
         with _native.device_guard(device):
             _native.call("koemi_window_attention_backward", q.data_ptr(), k.data_ptr(), v.data_ptr(), _native.ptr(mask),
                          _strides(q, k, v), output.data_ptr(), _native.ptr(rest), lse.data_ptr(), d_output.data_ptr(),
-                         _native.ptr(d_q), _native.ptr(d_k), _native.ptr(d_v), *shape, scale, code,
-                         _native.ptr(workspace), need, _native.stream_of(device))
+                         _native.ptr(d_q), _native.ptr(d_k), _native.ptr(d_v), batch, length, total, heads, groups, padded,
+                         window, sinks, plan.scale, plan.code, _native.ptr(workspace), need, _native.stream_of(device))
         grads = (g if g is None or padded == width else g[..., :width].contiguous() for g in (d_q, d_k, d_v))
-        return (*grads, None, None, None, None)
+        return (*grads, None, None)
 
 
 @dataclass(frozen=True)
@@ -225,23 +237,26 @@ class WindowCache:
 
     def __post_init__(self) -> None:
         window, sinks = _whole("window", self.window, 1), _whole("sinks", self.sinks, 0)
-        if not 1 <= _whole("width", self.width, 1) <= _MAX_WIDTH:
+        width = _whole("width", self.width, 1)
+        if width > _MAX_WIDTH:
             raise CudaThinkValidationError(f"heads must be 1 to {_MAX_WIDTH} wide")
-        tensors = (self.keys, self.key_scales, self.values, self.value_scales)
-        if not all(isinstance(t, Tensor) for t in tensors):
-            raise CudaThinkValidationError("a cache is made of four tensors")
-        shape = self.keys.shape
-        if (self.keys.ndim != 4 or shape[2] != window + sinks or shape[3] != -(-self.width // 32) * 32
-                or self.values.shape != shape or self.key_scales.shape != shape[:3] or self.value_scales.shape != shape[:3]):
+        keys, key_scales, values, value_scales = tensors = (self.keys, self.key_scales, self.values, self.value_scales)
+        for t in tensors:
+            if not isinstance(t, Tensor):
+                raise CudaThinkValidationError("a cache is made of four tensors")
+        shape, device = keys.shape, keys.device
+        if (len(shape) != 4 or shape[2] != window + sinks or shape[3] != -(-width // 32) * 32
+                or values.shape != shape or key_scales.shape != shape[:3] or value_scales.shape != shape[:3]):
             raise CudaThinkValidationError("a cache's codes must be [batch, key heads, window + sinks, width rounded up to 32] "
                                            "and its scales [batch, key heads, window + sinks]")
-        if self.keys.dtype not in _CODES or self.values.dtype != self.keys.dtype:
+        if keys.dtype not in _CODES or values.dtype != keys.dtype:
             raise CudaThinkValidationError("a cache's codes must be int8 or float8_e4m3fn")
-        if self.key_scales.dtype != torch.float32 or self.value_scales.dtype != torch.float32:
+        if key_scales.dtype != torch.float32 or value_scales.dtype != torch.float32:
             raise CudaThinkValidationError("a cache's scales must be float32")
-        if any(t.device != self.keys.device for t in tensors) or not all(t.is_contiguous() for t in tensors):
-            raise CudaThinkValidationError("a cache's tensors must be contiguous and on the same device")
-        if self.keys.numel() and (self.keys.data_ptr() % 16 or self.values.data_ptr() % 16):
+        for t in tensors:
+            if t.device != device or not t.is_contiguous():
+                raise CudaThinkValidationError("a cache's tensors must be contiguous and on the same device")
+        if keys.data_ptr() % 16 or values.data_ptr() % 16:
             raise CudaThinkValidationError("a cache's codes must be 16-byte aligned")
 
     def buffers(self) -> tuple[int, int, int, int, int]:
@@ -278,22 +293,24 @@ def _check_cache(cache: object) -> WindowCache:
     return cache
 
 
-def _check_rows(cache: WindowCache, name: str, tensor: object, shape: tuple[int, ...], dtype: torch.dtype | None) -> None:
-    """A tensor of rows of the cache's heads in one of the three types."""
-
+def _check_tensor(cache: WindowCache, name: str, tensor: object) -> None:
     if not isinstance(tensor, Tensor):
         raise CudaThinkValidationError(f"{name} must be a torch.Tensor")
-    if tensor.shape != shape:
-        raise CudaThinkValidationError(f"{name} must have shape {list(shape)}")
-    if tensor.dtype not in _SUPPORTED_DTYPES or (dtype is not None and tensor.dtype != dtype):
-        raise CudaThinkValidationError(f"{name} must be float32, float16 or bfloat16, one type for all")
     if tensor.device != cache.keys.device:
         raise CudaThinkValidationError(f"{name} must be on the cache's device")
 
 
+def _check_rows(name: str, shape: tuple[int, ...], wanted: tuple[int, ...], dtype: torch.dtype, same: torch.dtype) -> None:
+    """Rows of the cache's heads in one of the three types."""
+
+    if tuple(shape) != wanted:
+        raise CudaThinkValidationError(f"{name} must have shape {list(wanted)}")
+    if dtype not in _SUPPORTED_DTYPES or dtype != same:
+        raise CudaThinkValidationError(f"{name} must be float32, float16 or bfloat16, one type for all")
+
+
 def _check_counts(cache: WindowCache, name: str, tensor: object) -> Tensor:
-    batch = cache.keys.shape[0]
-    if not isinstance(tensor, Tensor) or tensor.dtype != torch.int64 or tensor.shape != (batch,) \
+    if not isinstance(tensor, Tensor) or tensor.dtype != torch.int64 or tensor.shape != cache.keys.shape[:1] \
             or tensor.device != cache.keys.device:
         raise CudaThinkValidationError(f"{name} must be an int64 [batch] tensor on the cache's device")
     return tensor.contiguous()
@@ -316,10 +333,13 @@ def window_cache_write(cache: WindowCache, keys: Tensor, values: Tensor, lengths
     """
 
     cache = _check_cache(cache)
+    _check_tensor(cache, "keys", keys)
+    _check_tensor(cache, "values", values)
     batch, groups = cache.keys.shape[:2]
-    length = keys.shape[1] if isinstance(keys, Tensor) and keys.ndim == 4 else -1
-    _check_rows(cache, "keys", keys, (batch, max(length, 0), groups, cache.width), None)
-    _check_rows(cache, "values", values, (batch, length, groups, cache.width), keys.dtype)
+    length = keys.shape[1] if keys.ndim == 4 else 0
+    wanted = (batch, length, groups, cache.width)
+    _check_rows("keys", keys.shape, wanted, keys.dtype, keys.dtype)
+    _check_rows("values", values.shape, wanted, values.dtype, keys.dtype)
     lengths = _check_counts(cache, "lengths", lengths)
     counts = _check_counts(cache, "counts", counts) if counts is not None else None
     _load()
@@ -356,42 +376,59 @@ def window_cache_entries(cache: WindowCache, lengths: Tensor, *, dtype: torch.dt
     return keys, values, present
 
 
-@lru_cache(maxsize=256)
-def _step_bytes(batch: int, heads: int, groups: int, width: int, window: int, sinks: int) -> int:
-    return _native.query("koemi_window_cache_step_workspace_bytes", batch, heads, groups, width, window, sinks)
+@lru_cache(maxsize=1024)
+def _step_plan(cache: tuple, width: int, window: int, sinks: int, scale: float | None, query: tuple, query_stride: tuple,
+               dtype: torch.dtype, key: tuple | None, key_stride: tuple | None, key_dtype: torch.dtype | None,
+               value: tuple | None, value_stride: tuple | None, value_dtype: torch.dtype | None) -> tuple:
+    """A step's shapes checked: heads, scale, dtype code, bytes of workspace, and the strides of
+    the rows as they lie (None where one of them has to be copied)."""
+
+    batch, groups = cache[:2]
+    heads = query[1] if len(query) == 3 else 0
+    _check_rows("queries", query, (batch, heads, width), dtype, dtype)
+    if heads < 1 or heads % groups:
+        raise CudaThinkValidationError("the key heads must divide the query heads")
+    if key is not None:
+        _check_rows("keys", key, (batch, groups, width), key_dtype, dtype)
+        _check_rows("values", value, (batch, groups, width), value_dtype, dtype)
+    _load()
+    need = _native.query("koemi_window_cache_step_workspace_bytes", batch, heads, groups, width, window, sinks)
+    strides = (query_stride, key_stride or (0, 0, 1), value_stride or (0, 0, 1))
+    flat = (ctypes.c_int64 * 6)(*(x for s in strides for x in s[:2]))
+    in_place = width == 1 or all(s[2] == 1 for s in strides)
+    return heads, _scale(scale, width), _native.dtype_code(dtype), need, flat if in_place else None
 
 
 def _step(cache: WindowCache, queries: Tensor, keys: Tensor | None, values: Tensor | None, lengths: Tensor,
           active: Tensor | None, scale: float | None) -> Tensor:
     cache = _check_cache(cache)
-    batch, groups = cache.keys.shape[:2]
-    heads = queries.shape[1] if isinstance(queries, Tensor) and queries.ndim == 3 else 0
-    _check_rows(cache, "queries", queries, (batch, heads, cache.width), None)
-    if heads < 1 or heads % groups:
-        raise CudaThinkValidationError("the key heads must divide the query heads")
-    if keys is not None or values is not None:
-        _check_rows(cache, "keys", keys, (batch, groups, cache.width), queries.dtype)
-        _check_rows(cache, "values", values, (batch, groups, cache.width), queries.dtype)
+    _check_tensor(cache, "queries", queries)
+    if scale is not None:
+        scale = _scale(scale, cache.width)
+    writes = keys is not None or values is not None
+    if writes:
+        _check_tensor(cache, "keys", keys)
+        _check_tensor(cache, "values", values)
+    shape, width, window, sinks = cache.keys.shape, cache.width, cache.window, cache.sinks
+    new = (keys.shape, keys.stride(), keys.dtype, values.shape, values.stride(), values.dtype) if writes else (None,) * 6
+    heads, scale, code, need, strides = _step_plan(shape, width, window, sinks, scale, queries.shape, queries.stride(),
+                                                   queries.dtype, *new)
     lengths = _check_counts(cache, "lengths", lengths)
     device = queries.device
-    if active is not None and (not isinstance(active, Tensor) or active.dtype != torch.bool or active.shape != (batch,)
-                               or active.device != device):
-        raise CudaThinkValidationError("active must be a bool [batch] tensor on the cache's device")
-    scale = _scale(scale, cache.width)
-    _load()
-    q = _in_rows(queries.detach())
-    k = _in_rows(keys.detach()) if keys is not None else None
-    v = _in_rows(values.detach()) if values is not None else None
-    flat = [s for t in (q, k, v) for s in (t.stride()[:2] if t is not None else (0, 0))]
-    mask = active.contiguous() if active is not None else None
-    output = torch.empty((batch, heads, cache.width), device=device, dtype=q.dtype)
-    need = _step_bytes(batch, heads, groups, cache.width, cache.window, cache.sinks)
-    workspace = _bytes(need, device)
+    if active is not None:
+        if not isinstance(active, Tensor) or active.dtype != torch.bool or active.shape != shape[:1] or active.device != device:
+            raise CudaThinkValidationError("active must be a bool [batch] tensor on the cache's device")
+        active = active.contiguous()
+    q, k, v = queries, keys, values
+    if strides is None:
+        q, k, v = (_in_rows(t.detach()) if t is not None else None for t in (q, k, v))
+        strides = (ctypes.c_int64 * 6)(*(x for t in (q, k, v) for x in (t.stride()[:2] if t is not None else (0, 0))))
+    output = torch.empty((shape[0], heads, width), device=device, dtype=q.dtype)
+    workspace = torch.empty(need, device=device, dtype=torch.uint8) if need else None
     with _native.device_guard(device):
-        _native.call("koemi_window_cache_step", *cache.buffers(), q.data_ptr(), _native.ptr(k), _native.ptr(v),
-                     (ctypes.c_int64 * 6)(*flat), lengths.data_ptr(), _native.ptr(mask), output.data_ptr(), batch, heads,
-                     groups, cache.width, cache.window, cache.sinks, scale, _native.dtype_code(q.dtype),
-                     _native.ptr(workspace), need, _native.stream_of(device))
+        _native.call("koemi_window_cache_step", *cache.buffers(), q.data_ptr(), _native.ptr(k), _native.ptr(v), strides,
+                     lengths.data_ptr(), _native.ptr(active), output.data_ptr(), shape[0], heads, shape[1], width, window,
+                     sinks, scale, code, _native.ptr(workspace), need, _native.stream_of(device))
     return output
 
 

@@ -19,6 +19,7 @@ import math
 import pytest
 import torch
 
+from koemi_amd import _native
 from koemi_amd import window as W
 from koemi_amd.think import CudaThinkValidationError
 
@@ -167,7 +168,7 @@ def test_long_windows_are_read_in_parts(device, code):
     batch, heads, groups, width, window, sinks = 2, 6, 2, 128, 5000, 16
     gen = torch.Generator(device="cuda").manual_seed(3)
     cache = W.window_cache(batch, groups, width, window=window, sinks=sinks, dtype=code, device=device)
-    assert W._step_bytes(batch, heads, groups, width, window, sinks) > 0
+    assert _native.query("koemi_window_cache_step_workspace_bytes", batch, heads, groups, width, window, sinks) > 0
     lengths = torch.tensor([0, 0], device=device)
     keys, values = (rows(gen, batch, 9000, groups, width, dtype=torch.bfloat16) for _ in range(2))
     counts = torch.tensor([9000, 1700], device=device)
