@@ -27,11 +27,11 @@ struct Cache {
     uint8_t* values;
     float* key_scales;      // [batch, groups, slots]
     float* value_scales;
-    int64_t window, sinks;
+    int window, sinks;      // together below 2^31
     int batch, groups, width, stored, kind;
-    __host__ __device__ int64_t slots() const { return window + sinks; }
-    __device__ __forceinline__ int64_t slot_of(int64_t entry) const {
-        return entry < sinks ? entry : sinks + (entry - sinks) % window;
+    __host__ __device__ int slots() const { return window + sinks; }
+    __device__ __forceinline__ int slot_of(int64_t entry) const {
+        return entry < sinks ? static_cast<int>(entry) : sinks + static_cast<int>((entry - sinks) % window);
     }
 };
 
@@ -111,39 +111,37 @@ struct Write {
     int64_t kb, kp, kh, vb, vp, vh;
     const int64_t* lengths;
     const int64_t* counts;  // or null: length
-    int64_t length;
-    int lanes, vector;
+    int length, lanes, vector, per_batch;  // per_batch: workgroups of a batch row
 };
 
 // `lanes` lanes quantise a row of a key head. Of the rows that this call appends only
-// those that stay are written, so no two go to one slot.
+// those that stay are written, so no two go to one slot. Bound by memory; the batch row's
+// ring position is a workgroup's own, so that a row needs no 64-bit division.
 template <typename T, int KIND>
 __global__ __launch_bounds__(kThreads) void window_cache_write_kernel(Write f) {
     const Cache& c = f.c;
     const int per = kThreads / f.lanes, i = static_cast<int>(threadIdx.x) % f.lanes;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * per + threadIdx.x / f.lanes;
-    const int64_t rows = c.batch * f.length * c.groups;
-    const int g = static_cast<int>(row % c.groups);
-    const int64_t t = row / c.groups % f.length, b = row / c.groups / f.length;
-    bool kept = row < rows;
-    int64_t slot = 0;
-    if (kept) {
-        const int64_t before = f.lengths[b], count = f.counts ? min(f.counts[b], f.length) : f.length;
-        const int64_t entry = before + t;
-        kept = before >= 0 && t < count && (entry < c.sinks || entry >= before + count - c.window);
-        if (kept) slot = c.slot_of(entry);
-    }
-    if (!kept) return;  // a whole row's lanes at once
-    const int64_t at = (b * c.groups + g) * c.slots() + slot;
+    const int b = static_cast<int>(blockIdx.x) / f.per_batch;
+    const int row = (static_cast<int>(blockIdx.x) - b * f.per_batch) * per + static_cast<int>(threadIdx.x) / f.lanes;
+    const int t = row / c.groups, g = row - t * c.groups;
+    const int64_t before = f.lengths[b], count = f.counts ? min(f.counts[b], static_cast<int64_t>(f.length)) : f.length;
+    const int64_t entry = before + t;
+    // a whole row's lanes at once
+    if (before < 0 || t >= count || !(entry < c.sinks || entry >= before + count - c.window)) return;
+    const uint32_t turn = before >= c.sinks ? static_cast<uint32_t>((before - c.sinks) % c.window) : 0u;
+    const uint32_t along = static_cast<uint32_t>(before >= c.sinks ? t : entry - c.sinks);
+    const int slot = entry < c.sinks ? static_cast<int>(entry) : c.sinks + static_cast<int>((turn + along) % static_cast<uint32_t>(c.window));
+    const int64_t at = (static_cast<int64_t>(b) * c.groups + g) * c.slots() + slot;
+    const T* x[2] = {static_cast<const T*>(f.keys) + b * f.kb + t * f.kp + g * f.kh,
+                     static_cast<const T*>(f.values) + b * f.vb + t * f.vp + g * f.vh};
+    float e[2][8];
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) load_eight(x[kv], i, c.width, f.vector, e[kv]);
 #pragma unroll
     for (int kv = 0; kv < 2; ++kv) {
-        const T* x = kv ? static_cast<const T*>(f.values) + b * f.vb + t * f.vp + g * f.vh
-                        : static_cast<const T*>(f.keys) + b * f.kb + t * f.kp + g * f.kh;
-        float e[8];
-        load_eight(x, i, c.width, f.vector, e);
         bool fine;
-        const float scale = scale_of<KIND>(e, f.lanes, fine);
-        const uint2 w = encode<KIND>(e, scale, fine);
+        const float scale = scale_of<KIND>(e[kv], f.lanes, fine);
+        const uint2 w = encode<KIND>(e[kv], scale, fine);
         if (8 * i < c.stored) *reinterpret_cast<uint2*>((kv ? c.values : c.keys) + at * c.stored + 8 * i) = w;
         if (i == 0) (kv ? c.value_scales : c.key_scales)[at] = fine ? scale : NAN;
     }
@@ -155,32 +153,43 @@ struct Entries {
     void* keys;    // [batch, slots, groups, width]
     void* values;
     uint8_t* present;  // [batch, slots]
-    int lanes;
+    int lanes, per_batch;
 };
 
 // The sinks, then the last `window` entries in their order, as the values they stand for.
 template <typename T, int KIND>
 __global__ __launch_bounds__(kThreads) void window_cache_entries_kernel(Entries f) {
     const Cache& c = f.c;
-    const int per = kThreads / f.lanes, i = static_cast<int>(threadIdx.x) % f.lanes;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * per + threadIdx.x / f.lanes, slots = c.slots();
-    if (row >= c.batch * slots * c.groups) return;
-    const int g = static_cast<int>(row % c.groups);
-    const int64_t place = row / c.groups % slots, b = row / c.groups / slots, held = f.lengths[b];
-    const int64_t entry = place < c.sinks ? place : held - slots + place;
+    const int per = kThreads / f.lanes, i = static_cast<int>(threadIdx.x) % f.lanes, slots = c.slots();
+    const int b = static_cast<int>(blockIdx.x) / f.per_batch;
+    const int row = (static_cast<int>(blockIdx.x) - b * f.per_batch) * per + static_cast<int>(threadIdx.x) / f.lanes;
+    const int place = row / c.groups, g = row - place * c.groups;
+    if (place >= slots) return;
+    const int64_t held = f.lengths[b], entry = place < c.sinks ? place : held - slots + place;
     const bool here = entry < held && (place < c.sinks || entry >= c.sinks);
-    const int64_t at = (b * c.groups + g) * slots + (here ? c.slot_of(entry) : 0);
-    if (g == 0 && i == 0) f.present[b * slots + place] = here;
+    // entry - sinks = (held - sinks) + (place - sinks) - window
+    const uint32_t turn = held >= c.sinks ? static_cast<uint32_t>((held - c.sinks) % c.window) : 0u;
+    uint32_t ring = turn + static_cast<uint32_t>(place - c.sinks);
+    if (held >= c.sinks && ring >= static_cast<uint32_t>(c.window)) ring -= static_cast<uint32_t>(c.window);
+    const int slot = !here ? 0 : place < c.sinks ? place : c.sinks + static_cast<int>(ring);
+    const int64_t at = (static_cast<int64_t>(b) * c.groups + g) * slots + slot;
+    if (g == 0 && i == 0) f.present[static_cast<int64_t>(b) * slots + place] = here;
     if (8 * i >= c.width) return;
+    uint2 w[2];
+    float scale[2];
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+        w[kv] = *reinterpret_cast<const uint2*>((kv ? c.values : c.keys) + at * c.stored + 8 * i);
+        scale[kv] = (kv ? c.value_scales : c.key_scales)[at];
+    }
 #pragma unroll
     for (int kv = 0; kv < 2; ++kv) {
         float x[8];
-        decode<KIND>(*reinterpret_cast<const uint2*>((kv ? c.values : c.keys) + at * c.stored + 8 * i), x);
-        const float scale = (kv ? c.value_scales : c.key_scales)[at];
-        T* o = static_cast<T*>(kv ? f.values : f.keys) + row * c.width + 8 * i;
+        decode<KIND>(w[kv], x);
+        T* o = static_cast<T*>(kv ? f.values : f.keys) + (static_cast<int64_t>(b) * slots * c.groups + row) * c.width + 8 * i;
         alignas(16) T e[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) e[j] = here ? from_f32<T>(x[j] * scale) : static_cast<T>(0.0f);
+        for (int j = 0; j < 8; ++j) e[j] = here ? from_f32<T>(x[j] * scale[kv]) : static_cast<T>(0.0f);
         if (c.width % 8 == 0) {
 #pragma unroll
             for (int h = 0; h < static_cast<int>(sizeof(T)) / 2; ++h) reinterpret_cast<uint4*>(o)[h] = reinterpret_cast<const uint4*>(e)[h];
@@ -236,14 +245,19 @@ __device__ __forceinline__ f16x8 widen8(uint32_t lo, uint32_t hi) {  // eight by
     return f16x8{p[0][0], p[0][1], p[1][0], p[1][1], p[2][0], p[2][1], p[3][0], p[3][1]};
 }
 
-// The largest of the four lane groups that hold a query.
+// Over the four lane groups (of sixteen) that hold a query.
+template <typename Op>
+__device__ __forceinline__ float over_groups(float x, Op op) {
+    const auto odd = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = op(__uint_as_float(odd[0]), __uint_as_float(odd[1]));
+    const auto high = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return op(__uint_as_float(high[0]), __uint_as_float(high[1]));
+}
 __device__ __forceinline__ float max_of_groups(float x) {
-    x = fmaxf(x, __shfl_xor(x, 16, kWave));
-    return fmaxf(x, __shfl_xor(x, 32, kWave));
+    return over_groups(x, [](float a, float b) { return fmaxf(a, b); });
 }
 __device__ __forceinline__ float sum_of_groups(float x) {
-    x += __shfl_xor(x, 16, kWave);
-    return x + __shfl_xor(x, 32, kWave);
+    return over_groups(x, [](float a, float b) { return a + b; });
 }
 
 template <int NB>
@@ -377,15 +391,19 @@ struct Walk {
     }
 };
 
+// Waves of a workgroup: eight where two of them fit a SIMD's registers.
+template <int NB> constexpr int kStepWaves = NB <= 4 ? 8 : 4;
+
 // A workgroup answers sixteen query heads of one key head from one part of the slots, its
 // waves 32 slots each in turn. The new entry is quantised by the first part's workgroups
 // (of every sixteen heads), which read it from LDS; the others leave its slot out.
 template <typename T, int NB, int KIND>
-__global__ __launch_bounds__(kThreads) void window_cache_step_kernel(Step f) {
+__global__ __launch_bounds__(kStepWaves<NB> * kWave) void window_cache_step_kernel(Step f) {
+    constexpr int kWaves = kStepWaves<NB>, kThreads = kWaves * kWave;
     const Cache& c = f.c;
     __shared__ __attribute__((aligned(16))) uint8_t fresh[2][NB * 32];
     __shared__ float fresh_scale[2];
-    __shared__ float sums[kWaves][16][NB * 32];
+    __shared__ float sums[kWaves][16][NB * 32 + 1];
     __shared__ float tops[kWaves][16], totals[kWaves][16];
     const int lane = lane_id(), wave = static_cast<int>(threadIdx.x) / kWave, m = lane >> 4, col = lane & 15;
     int64_t id = blockIdx.x;
@@ -405,6 +423,46 @@ __global__ __launch_bounds__(kThreads) void window_cache_step_kernel(Step f) {
     const float* key_scales = c.key_scales + base;
     const float* value_scales = c.value_scales + base;
 
+    const int64_t chunks = (held + 31) / 32;
+    const int c0 = static_cast<int>(chunks * split / f.splits), c1 = static_cast<int>(chunks * (split + 1) / f.splits);
+    uint32_t kw[2][2 * NB];
+    Bytes<NB> vw[8];
+    float ks[8], vs[8];
+    // chunk n's loads; past the last entry that one again
+    auto fetch = [&](int n) {
+        const int s0 = n * 32, end = static_cast<int>(held) - 1;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int64_t s = min(s0 + 16 * h + col, end);
+            const uint32_t* p = reinterpret_cast<const uint32_t*>(keys + s * c.stored + m * 8 * NB);
+#pragma unroll
+            for (int i = 0; i < 2 * NB; ++i) kw[h][i] = p[i];
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int64_t s = min(s0 + 16 * (j / 4) + 4 * m + j % 4, end);
+            vw[j] = *reinterpret_cast<const Bytes<NB>*>(values + s * c.stored + col * 2 * NB);
+        }
+        if (s0 + 32 <= static_cast<int>(held)) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {  // four at once, at any place
+                __builtin_memcpy(&ks[4 * h], key_scales + s0 + 16 * h + 4 * m, 16);
+                __builtin_memcpy(&vs[4 * h], value_scales + s0 + 16 * h + 4 * m, 16);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int s = min(s0 + 16 * (j / 4) + 4 * m + j % 4, end);
+                ks[j] = key_scales[s], vs[j] = value_scales[s];
+            }
+        }
+    };
+    if (c0 + wave < c1) fetch(c0 + wave);
+    const int head = block * 16 + col;
+    const bool head_ok = live && head < f.shared;
+    Walk<NB, KIND> walk;
+    walk.begin(static_cast<const T*>(f.queries) + b * f.qb + (static_cast<int64_t>(g) * f.shared + head) * f.qh, c.width, head_ok, f.vector, f.scale);
+
     if (writes && split == 0 && wave < 2) {  // wave 0 the key, wave 1 the value
         const T* x = wave ? static_cast<const T*>(f.new_values) + b * f.vb + g * f.vh : static_cast<const T*>(f.new_keys) + b * f.kb + g * f.kh;
         float e[8];
@@ -421,33 +479,22 @@ __global__ __launch_bounds__(kThreads) void window_cache_step_kernel(Step f) {
             if (block == 0) (wave ? c.value_scales : c.key_scales)[base + slot] = fine ? scale : NAN;
         }
     }
-    Walk<NB, KIND> walk;
-    const int head = block * 16 + col;
-    const bool head_ok = live && head < f.shared;
-    walk.begin(static_cast<const T*>(f.queries) + b * f.qb + (static_cast<int64_t>(g) * f.shared + head) * f.qh, c.width, head_ok, f.vector, f.scale);
-
-    uint32_t kw[2][2 * NB];
-    Bytes<NB> vw[8];
-    float ks[8], vs[8];
-    const int64_t chunks = (held + 31) / 32, c0 = chunks * split / f.splits, c1 = chunks * (split + 1) / f.splits;
-    for (int64_t n = c0 + wave; n < c1; n += kWaves) {
-        const int64_t s0 = n * 32;
-        uint32_t ok = 0;
+    for (int n = c0 + wave; n < c1; n += kWaves) {
+        uint32_t kn[2][2 * NB], ok = 0;
+        Bytes<NB> vn[8];
+        float ksn[8], vsn[8];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int64_t s = min(s0 + 16 * h + col, held - 1);
-            const uint32_t* p = reinterpret_cast<const uint32_t*>(keys + s * c.stored + m * 8 * NB);
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int i = 0; i < 2 * NB; ++i) kw[h][i] = p[i];
-        }
+            for (int i = 0; i < 2 * NB; ++i) kn[h][i] = kw[h][i];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const int64_t at = s0 + 16 * (j / 4) + 4 * m + j % 4, s = min(at, held - 1);
-            vw[j] = *reinterpret_cast<const Bytes<NB>*>(values + s * c.stored + col * 2 * NB);
-            ks[j] = key_scales[s], vs[j] = value_scales[s];
+            vn[j] = vw[j], ksn[j] = ks[j], vsn[j] = vs[j];
+            const int at = n * 32 + 16 * (j / 4) + 4 * m + j % 4;
             ok |= static_cast<uint32_t>(at < held && at != slot) << j;
         }
-        walk.chunk(kw, vw, ks, vs, ok);
+        fetch(min(n + kWaves, c1 - 1));
+        walk.chunk(kn, vn, ksn, vsn, ok);
     }
     if (writes && split == 0) {
         __syncthreads();
@@ -518,21 +565,24 @@ __global__ __launch_bounds__(kThreads) void window_cache_join_kernel(Step f) {
     share = all == 0.0f ? 0.0f : share / all;
     for (int d = lane; d < width; d += kWave) {
         float x = 0.0f;
+#pragma unroll 8
         for (int p = 0; p < f.splits; ++p) x = fmaf(f.parts[(cell + p * cells) * width + d], __shfl(share, p, kWave), x);
         static_cast<T*>(f.out)[cell * width + d] = from_f32<T>(x);
     }
 }
 
-// Parts of the slots: about four workgroups for each compute unit, none under 256 slots.
+// Parts of the slots: one workgroup for each compute unit, none under 256 slots. A workgroup's start and end cost
+// as much as a few chunks: [64] rows of 4 key heads, 1028 slots: 16.2 us in 256 workgroups, 19.8 (and 3.9 for the join) in
+// 512, 29.4 in 1024; [8] of 8, 32784 slots: 93.8 + 5.5, 100.4 + 8.8, 111.6 + 12.0.
 int splits_for(int64_t batch, int64_t heads, int64_t groups, int64_t slots) {
     const int64_t wide = batch * groups * ((heads / groups + 15) / 16);
-    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({64, slots / 256, 1024 / std::max<int64_t>(wide, 1)})));
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({64, slots / 256, 256 / std::max<int64_t>(wide, 1)})));
 }
 
 template <typename T, int NB, int KIND>
 int run_step(const Step& f, hipStream_t stream) {
     const int64_t grid = static_cast<int64_t>(f.c.batch) * f.c.groups * f.blocks16 * f.splits;
-    hipLaunchKernelGGL((window_cache_step_kernel<T, NB, KIND>), dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, stream, f);
+    hipLaunchKernelGGL((window_cache_step_kernel<T, NB, KIND>), dim3(static_cast<unsigned>(grid)), dim3(kStepWaves<NB> * kWave), 0, stream, f);
     const int rc = check_launch("koemi_window_cache_step");
     if (rc != KOEMI_OK || f.splits == 1) return rc;
     hipLaunchKernelGGL((window_cache_join_kernel<T>), dim3(grid_for(static_cast<int64_t>(f.c.batch) * f.c.groups * f.shared, kWaves)),
@@ -559,14 +609,14 @@ int cache_of(const char* what, void* keys, float* key_scales, void* values, floa
         return fail(KOEMI_ERR_INVALID, "%s: sizes must be positive, batch and sinks not negative", what);
     if (width > 256) return fail(KOEMI_ERR_UNSUPPORTED, "%s: heads are at most 256 wide", what);
     if (code != kInt8 && code != kE4m3) return fail(KOEMI_ERR_UNSUPPORTED, "%s: codes are int8 (0) or e4m3 (1)", what);
-    if (window >= (int64_t(1) << 40) || sinks >= (int64_t(1) << 40) || batch >= (1 << 24) || groups >= (1 << 20) ||
-        (batch && (window + sinks) >= (int64_t(1) << 38) / (batch * groups)))
-        return fail(KOEMI_ERR_UNSUPPORTED, "%s: at most 2^38 entries of a key head", what);
+    if (window >= (int64_t(1) << 31) || sinks >= (int64_t(1) << 31) - window || batch >= (1 << 24) || groups >= (1 << 20) ||
+        (window + sinks) * groups >= (int64_t(1) << 31))
+        return fail(KOEMI_ERR_UNSUPPORTED, "%s: at most 2^31 entries x key heads, 2^20 key heads and 2^24 rows", what);
     if (batch && (!keys || !key_scales || !values || !value_scales)) return fail(KOEMI_ERR_INVALID, "%s: null pointer", what);
     if (reinterpret_cast<uintptr_t>(keys) % 16 || reinterpret_cast<uintptr_t>(values) % 16)
         return fail(KOEMI_ERR_INVALID, "%s: the codes must be 16-byte aligned", what);
-    c = Cache{static_cast<uint8_t*>(keys), static_cast<uint8_t*>(values), key_scales, value_scales, window, sinks,
-              static_cast<int>(batch), static_cast<int>(groups), static_cast<int>(width), static_cast<int>((width + 31) / 32 * 32), code};
+    c = Cache{static_cast<uint8_t*>(keys), static_cast<uint8_t*>(values), key_scales, value_scales, static_cast<int>(window),
+              static_cast<int>(sinks), static_cast<int>(batch), static_cast<int>(groups), static_cast<int>(width), static_cast<int>((width + 31) / 32 * 32), code};
     return KOEMI_OK;
 }
 
@@ -603,12 +653,15 @@ extern "C" int koemi_window_cache_write(void* keys, float* key_scales, void* val
     if (length < 0) return fail(KOEMI_ERR_INVALID, "%s: length must not be negative", what);
     if (batch == 0 || length == 0) return KOEMI_OK;
     if (!new_keys || !new_values || !strides || !lengths) return fail(KOEMI_ERR_INVALID, "%s: null pointer", what);
-    f.keys = new_keys, f.values = new_values, f.lengths = lengths, f.counts = counts, f.length = length;
+    f.keys = new_keys, f.values = new_values, f.lengths = lengths, f.counts = counts, f.length = static_cast<int>(length);
     f.kb = strides[0], f.kp = strides[1], f.kh = strides[2], f.vb = strides[3], f.vp = strides[4], f.vh = strides[5];
     f.lanes = lanes_of(f.c.stored);
     f.vector = aligned16(new_keys, size_of(dtype), {f.kb, f.kp, f.kh}) && aligned16(new_values, size_of(dtype), {f.vb, f.vp, f.vh});
-    if (length >= (int64_t(1) << 34) / (batch * groups)) return fail(KOEMI_ERR_UNSUPPORTED, "%s: at most 2^34 rows", what);
-    const dim3 grid(grid_for(batch * length * groups, kThreads / f.lanes));
+    if (length >= (int64_t(1) << 31) / groups - 256) return fail(KOEMI_ERR_UNSUPPORTED, "%s: at most 2^31 new entries x key heads", what);
+    const int64_t per_batch = (length * groups * f.lanes + kThreads - 1) / kThreads;
+    if (batch * per_batch >= (int64_t(1) << 31)) return fail(KOEMI_ERR_UNSUPPORTED, "%s: too many rows", what);
+    f.per_batch = static_cast<int>(per_batch);
+    const dim3 grid(static_cast<unsigned>(batch * per_batch));
     auto launch = [&](auto type, auto kind) {
         hipLaunchKernelGGL((window_cache_write_kernel<decltype(type), decltype(kind)::value>), grid, dim3(kThreads), 0, as_stream(stream), f);
     };
@@ -639,8 +692,10 @@ extern "C" int koemi_window_cache_entries(const void* keys, const float* key_sca
         return fail(KOEMI_ERR_INVALID, "%s: the outputs must be 16-byte aligned", what);
     f.lengths = lengths, f.keys = out_keys, f.values = out_values, f.present = present;
     f.lanes = lanes_of(f.c.stored);
-    if (window + sinks >= (int64_t(1) << 34) / (batch * groups)) return fail(KOEMI_ERR_UNSUPPORTED, "%s: at most 2^34 rows", what);
-    const dim3 grid(grid_for(batch * (window + sinks) * groups, kThreads / f.lanes));
+    const int64_t per_batch = ((window + sinks) * groups * f.lanes + kThreads - 1) / kThreads;
+    if (batch * per_batch >= (int64_t(1) << 31)) return fail(KOEMI_ERR_UNSUPPORTED, "%s: too many rows", what);
+    f.per_batch = static_cast<int>(per_batch);
+    const dim3 grid(static_cast<unsigned>(batch * per_batch));
     auto launch = [&](auto type, auto kind) {
         hipLaunchKernelGGL((window_cache_entries_kernel<decltype(type), decltype(kind)::value>), grid, dim3(kThreads), 0, as_stream(stream), f);
     };
