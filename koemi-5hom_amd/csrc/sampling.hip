@@ -21,8 +21,8 @@
 namespace koemi {
 namespace {
 
-constexpr int kBins = 2048;
-constexpr int kList = 4096;        // scores of one step that fit LDS
+constexpr int kBins = 2048;        // steps of the histogram
+constexpr int kList = 4096;        // scores of one step that LDS holds
 constexpr int kTile = 512;         // scores of a wave and step: eight a lane
 constexpr int64_t kMaxVocab = 1 << 19;  // 2^44 x 2^19 fits 64 bits
 constexpr double kLog2eD = 1.4426950408889634074;
@@ -90,10 +90,13 @@ struct Row {
         const double e = (static_cast<double>(x) - top) * slope;
         return e > -100.0 ? pow2(e) : 0.0;
     }
-    static __device__ __forceinline__ uint64_t whole(double w) { return static_cast<uint64_t>(fma(w, 17592186044416.0, 0.5)); }
+    // w in steps of 2^-44, 0 <= w <= 1: the last bits of 2^52 plus it.
+    static __device__ __forceinline__ uint64_t whole(double w) {
+        return __builtin_bit_cast(uint64_t, fma(w, 17592186044416.0, 4503599627370496.0)) & 0xfffffffffffffull;
+    }
     // The histogram's step: falls with the score, never rises.
     __device__ __forceinline__ int bin(float x) const {
-        const float e = (static_cast<float>(top) - x) * (static_cast<float>(slope) * 32.0f);
+        const float e = (static_cast<float>(top) - x) * (static_cast<float>(slope) * (kBins / 64.0f));
         return e < static_cast<float>(kBins - 1) ? static_cast<int>(e) : kBins - 1;
     }
 };
@@ -110,6 +113,7 @@ struct Shared {
     uint64_t mass[kBins];
     uint32_t count[kBins];
     uint32_t list[kList];
+    float gathered[THREADS / kWave][kTile];
     uint64_t scan[THREADS / kWave];
     float wave_top[THREADS / kWave];
     uint64_t before;
@@ -151,9 +155,8 @@ __device__ float limit(const Row<T>& row, Shared<THREADS>& sh, double target) {
     constexpr int kWaves = THREADS / kWave;
     const int lane = lane_id(), wave = static_cast<int>(threadIdx.x) / kWave;
     uint64_t before;
-    const int bin = reach<THREADS>(sh, kBins, [&](int i) { return MASS ? sh.mass[i] : static_cast<uint64_t>(sh.count[i]); }, target, 0, before);
-    const uint32_t many = sh.count[bin];
-    const bool listed = many <= kList;
+    const int bin = reach<THREADS>(sh, kBins, [&](int i) { return MASS ? sh.mass[i] : static_cast<uint64_t>(sh.count[i]); },
+                                   target, 0, before);
     if (threadIdx.x == 0) sh.listed = 0;
     __syncthreads();
     auto each = [&](auto take) {  // every score of the step
@@ -165,7 +168,12 @@ __device__ float limit(const Row<T>& row, Shared<THREADS>& sh, double target) {
                 if (x[i] != -INFINITY && row.bin(x[i]) == bin) take(x[i]);
         }
     };
-    if (listed) each([&](float x) { sh.list[atomicAdd(&sh.listed, 1)] = rank_of(x); });
+    each([&](float x) {
+        const int at = atomicAdd(&sh.listed, 1);
+        if (at < kList) sh.list[at] = rank_of(x);
+    });
+    __syncthreads();
+    const int many = sh.listed;
     __shared__ unsigned long long digits[256];
     uint32_t prefix = 0;
     for (int shift = 24; shift >= 0; shift -= 8) {
@@ -175,8 +183,8 @@ __device__ float limit(const Row<T>& row, Shared<THREADS>& sh, double target) {
             if (shift == 24 || r >> (shift + 8) == prefix >> (shift + 8))
                 atomicAdd(&digits[255 - ((r >> shift) & 255)], MASS ? Row<T>::whole(row.weight(score_of(r))) : 1ull);
         };
-        if (listed) {
-            for (int i = threadIdx.x; i < static_cast<int>(many); i += THREADS) add(sh.list[i]);
+        if (many <= kList) {
+            for (int i = threadIdx.x; i < many; i += THREADS) add(sh.list[i]);
         } else {
             each([&](float x) { add(rank_of(x)); });
         }
@@ -221,7 +229,7 @@ __global__ __launch_bounds__(THREADS) void sample_filtered_kernel(Draw f) {
             for (int i = 0; i < 8; ++i)
                 if (x[i] != -INFINITY) {
                     const int b = row.bin(x[i]);
-                    atomicAdd(&sh.count[b], 1u);
+                    if (by_k) atomicAdd(&sh.count[b], 1u);
                     if (by_p) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.mass[b]), static_cast<unsigned long long>(Row<T>::whole(row.weight(x[i]))));
                 }
         }
@@ -250,7 +258,8 @@ __global__ __launch_bounds__(THREADS) void sample_filtered_kernel(Draw f) {
             least = fmaxf(least, limit<THREADS, true>(row, sh, f.top_p * static_cast<double>(total)));
         }
     }
-    // the kept weights of every tile, in the histogram's place
+    // the kept weights of every tile, in the histogram's place: a wave first gathers its tile's
+    // kept scores, often few, so that their exponentials fill its lanes
     __syncthreads();
     auto kept = [&](float x) {
         if (x == -INFINITY || x < least) return 0.0;
@@ -261,8 +270,17 @@ __global__ __launch_bounds__(THREADS) void sample_filtered_kernel(Draw f) {
         float x[8];
         row.load(t * kTile + lane * 8, x);
         uint64_t sum = 0;
+        int count = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum += Row<T>::whole(kept(x[i]));
+        for (int i = 0; i < 8; ++i) {
+            const bool in = x[i] != -INFINITY && x[i] >= least;
+            const uint64_t mask = __ballot(in);
+            if (in) sh.gathered[wave][count + __popcll(mask & lanemask_lt())] = x[i];
+            count += __popcll(mask);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        for (int i = lane; i < count; i += kWave) sum += Row<T>::whole(kept(sh.gathered[wave][i]));
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
         for (int off = kWave / 2; off > 0; off >>= 1) sum += __shfl_xor(sum, off, kWave);
         if (lane == 0) sh.mass[t] = sum;
@@ -313,10 +331,134 @@ __global__ __launch_bounds__(THREADS) void sample_filtered_kernel(Draw f) {
     if (lane == 0) f.ids[r] = none ? 0 : chosen;
 }
 
+// Over a wave's 64 lanes, the result in each: neighbours, quads, half rows and rows by
+// data-parallel moves, then the rows of sixteen and the halves.
+template <typename V, typename Op>
+__device__ __forceinline__ V over_wave(V x, Op op) {
+    constexpr int N = sizeof(V) / 4;
+    struct Words {
+        int w[N];
+    };
+    auto step = [&](auto move) {
+        Words a = __builtin_bit_cast(Words, x);
+#pragma unroll
+        for (int i = 0; i < N; ++i) a.w[i] = move(a.w[i]);
+        x = op(x, __builtin_bit_cast(V, a));
+    };
+    step([](int w) { return __builtin_amdgcn_update_dpp(0, w, 0xb1, 0xf, 0xf, true); });   // lane ^ 1
+    step([](int w) { return __builtin_amdgcn_update_dpp(0, w, 0x4e, 0xf, 0xf, true); });   // lane ^ 2
+    step([](int w) { return __builtin_amdgcn_update_dpp(0, w, 0x141, 0xf, 0xf, true); });  // 7 - lane in eight
+    step([](int w) { return __builtin_amdgcn_update_dpp(0, w, 0x140, 0xf, 0xf, true); });  // 15 - lane in sixteen
+    auto halves = [&](auto swap) {
+        const Words a = __builtin_bit_cast(Words, x);
+        Words lo, hi;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const auto both = swap(static_cast<uint32_t>(a.w[i]));
+            lo.w[i] = static_cast<int>(both[0]), hi.w[i] = static_cast<int>(both[1]);
+        }
+        x = op(__builtin_bit_cast(V, lo), __builtin_bit_cast(V, hi));
+    };
+    halves([](uint32_t w) { return __builtin_amdgcn_permlane16_swap(w, w, false, false); });
+    halves([](uint32_t w) { return __builtin_amdgcn_permlane32_swap(w, w, false, false); });
+    return x;
+}
+
+// Rows of one tile: a wave holds all scores, and finds the limits bit by bit from how many
+// scores, or what weight, lie at or above a candidate. 2^44 x 512 = 2^53: sums of whole
+// weights are exact in double.
+template <typename T>
+__global__ __launch_bounds__(kWave) void sample_narrow_kernel(Draw f) {
+    const int lane = lane_id(), j = lane * 8;
+    const int64_t r = blockIdx.x;
+    Row<T> row{static_cast<const T*>(f.logits) + r * f.row_stride, f.vocab, static_cast<int>(f.exclude), f.vector != 0, false, 0.0, f.slope};
+    const float u = f.uniforms[r];
+    float x[8], top = -INFINITY;
+    row.load(j, x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, x[i]);
+    top = over_wave(top, [](float a, float b) { return fmaxf(a, b); });
+    if (top == INFINITY) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = x[i] == INFINITY ? 0.0f : -INFINITY;
+        top = 0.0f;
+    }
+    row.top = static_cast<double>(top);
+    const auto add = [](double a, double b) { return a + b; };
+    uint32_t rank[8];
+    double exact[8], w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const bool here = x[i] != -INFINITY;
+        rank[i] = here ? rank_of(x[i]) : 0u;
+        exact[i] = here ? row.weight(x[i]) : 0.0;
+        w[i] = static_cast<double>(Row<T>::whole(exact[i]));
+    }
+    uint32_t least = 1;  // of the kept ranks; no score has rank 0
+    if (f.top_k > 0 && f.top_k < f.vocab) {
+        uint32_t at = 0;
+        for (int bit = 31; bit >= 0; --bit) {
+            const uint32_t next = at | 1u << bit;
+            int64_t count = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) count += __popcll(__ballot(rank[i] >= next));
+            if (count >= f.top_k) at = next;
+        }
+        least = max(at, 1u);
+    }
+    if (f.top_p < 1.0) {
+        double total = 0.0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) total += rank[i] >= least ? w[i] : 0.0;
+        const double target = f.top_p * over_wave(total, add);
+        uint32_t at = 0;
+        for (int bit = 31; bit >= 0; --bit) {
+            const uint32_t next = at | 1u << bit;
+            double sum = 0.0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum += rank[i] >= next ? w[i] : 0.0;
+            if (!(over_wave(sum, add) < target)) at = next;
+        }
+        least = max(least, at);
+    }
+    double own = 0.0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if (rank[i] < least || !(exact[i] >= f.min_p)) exact[i] = w[i] = 0.0;
+        own += w[i];
+    }
+    double run = own;
+#pragma unroll
+    for (int off = 1; off < kWave; off <<= 1) {
+        const double up = __shfl_up(run, off, kWave);
+        if (lane >= off) run += up;
+    }
+    const double total = __shfl(run, kWave - 1, kWave);
+    run -= own;
+    if (f.probabilities) {
+        const double share = total > 0.0 ? 17592186044416.0 / total : 0.0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (j + i < f.vocab) f.probabilities[r * f.vocab + j + i] = static_cast<float>(exact[i] * share);
+    }
+    const double target = static_cast<double>(u > 0.0f ? fminf(u, 0.999999940395355f) : 0.0f) * total;
+    int id = -1;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        run += w[i];
+        if (id < 0 && run > target) id = j + i;
+    }
+    const uint64_t hit = __ballot(id >= 0);
+    const int chosen = hit ? __shfl(id, __ffsll(static_cast<unsigned long long>(hit)) - 1, kWave) : 0;
+    if (lane == 0) f.ids[r] = chosen;
+}
+
 template <typename T>
 int draw(const Draw& f, int64_t rows, hipStream_t stream) {
     // a wave takes 512 scores a step: sixteen waves where a row has more than four such tiles
-    if (f.vocab <= 2048)
+    if (f.vocab <= kTile)
+        hipLaunchKernelGGL((sample_narrow_kernel<T>), dim3(static_cast<unsigned>(rows)), dim3(kWave), 0, stream, f);
+    else if (f.vocab <= 2048)
         hipLaunchKernelGGL((sample_filtered_kernel<256, T>), dim3(static_cast<unsigned>(rows)), dim3(256), 0, stream, f);
     else
         hipLaunchKernelGGL((sample_filtered_kernel<1024, T>), dim3(static_cast<unsigned>(rows)), dim3(1024), 0, stream, f);
