@@ -563,11 +563,15 @@ __global__ __launch_bounds__(kThreads) void window_cache_join_kernel(Step f) {
     float share = some ? __builtin_amdgcn_exp2f(own - top) : 0.0f;
     const float all = wave_sum_xor(share);
     share = all == 0.0f ? 0.0f : share / all;
-    for (int d = lane; d < width; d += kWave) {
+    for (int d0 = 0; d0 < width; d0 += kWave) {  // all lanes in every round: each holds a part's share
+        const int d = d0 + lane;
         float x = 0.0f;
 #pragma unroll 8
-        for (int p = 0; p < f.splits; ++p) x = fmaf(f.parts[(cell + p * cells) * width + d], __shfl(share, p, kWave), x);
-        static_cast<T*>(f.out)[cell * width + d] = from_f32<T>(x);
+        for (int p = 0; p < f.splits; ++p) {
+            const float part = f.parts[(cell + p * cells) * width + min(d, width - 1)];
+            x = fmaf(part, __shfl(share, p, kWave), x);
+        }
+        if (d < width) static_cast<T*>(f.out)[cell * width + d] = from_f32<T>(x);
     }
 }
 

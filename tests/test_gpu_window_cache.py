@@ -163,9 +163,10 @@ def test_chunks_and_steps(device, batch, heads, groups, width, window, sinks, dt
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("width", [8, 32, 72, 96, 128, 200])
 @pytest.mark.parametrize("code", CODES)
-def test_long_windows_are_read_in_parts(device, code):
-    batch, heads, groups, width, window, sinks = 2, 6, 2, 128, 5000, 16
+def test_long_windows_are_read_in_parts(device, code, width):
+    batch, heads, groups, window, sinks = 2, 6, 2, 5000, 16
     gen = torch.Generator(device="cuda").manual_seed(3)
     cache = W.window_cache(batch, groups, width, window=window, sinks=sinks, dtype=code, device=device)
     assert _native.query("koemi_window_cache_step_workspace_bytes", batch, heads, groups, width, window, sinks) > 0
