@@ -24,7 +24,7 @@ struct Backward {
     const void* rest;   // what out was rounded off by, or null: D is a small difference of large terms
     const void* d_out;  // each [batch, length, heads, width]
     const float* lse;
-    float* delta;       // D: [batch, heads, length]
+    float* delta;       // D: [batch, heads, length], infinite for a row that sees one key
     void* dq;
     void* dk;
     void* dv;
@@ -68,7 +68,7 @@ struct Range {
     }
 };
 
-template <typename T, int NB>
+template <typename T, int NB, int PLANES>
 __global__ __launch_bounds__(kThreads, NB == 1 ? 4 : NB == 2 && sizeof(T) == 2 ? 3 : NB <= 4 ? 2 : 1) void window_dq_kernel(Backward f) {
     using L = Tile<T, NB>;
     constexpr int KT = kKeys<T>, KB = KT / 32;
@@ -100,6 +100,7 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 4 : NB == 2 && sizeof(T) == 2 ?
     for (int n = 0; n < NB; ++n) acc[n] = f32x16(0.0f);
     Range<T, NB> range;
     float delta = 0.0f;
+    int sees = 0;  // keys
     const float c = a.scale * kLog2e;
     if (any_row) {
         const T* q = static_cast<const T*>(a.q) + b * a.qs.batch + position * a.qs.position + head * a.qs.head;
@@ -156,6 +157,7 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 4 : NB == 2 && sizeof(T) == 2 ?
             if (!shown || !wave_rows || key0 > wave_last || (key0 + KT <= wave_first - a.window + 1 && key0 >= a.sinks)) continue;
             const bool masked = !whole(wave_first, wave_last);
             const uint64_t seen = !masked ? every : row_ok ? keys_seen(a, place, key0) & shown : 0ull;
+            sees += __popcll(seen);
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
                 f32x16 s = f32x16(0.0f), d = f32x16(0.0f);
@@ -172,12 +174,14 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 4 : NB == 2 && sizeof(T) == 2 ?
                 if (masked && bad_tile == t)
                     seen_acc<T, NB>(acc, k_tile, kb * 32, d, block, scratch[wave]);
                 else
-                    mma_acc<T, NB>(acc, k_tile, kb * 32, d);
+                    mma_acc<T, NB, PLANES>(acc, k_tile, kb * 32, d);
             }
         }
     }
     if (row >= rows) return;
-    if (half == 0) f.delta[at] = delta;
+    // A row that sees one key has p = 1 whatever the score: no gradient, to the bit. Its D says so to the other kernel.
+    const bool alone = sees <= 1;
+    if (half == 0) f.delta[at] = alone ? INFINITY : delta;
     if (!f.dq) return;
     const float by = a.scale * range.back();
 #pragma unroll
@@ -186,7 +190,7 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 4 : NB == 2 && sizeof(T) == 2 ?
         for (int q = 0; q < 4; ++q) {
             float x[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = row_ok ? acc[n][4 * q + i] * by : 0.0f;
+            for (int i = 0; i < 4; ++i) x[i] = row_ok && !alone ? acc[n][4 * q + i] * by : 0.0f;
             store_four(static_cast<T*>(f.dq) + cell, 32 * n + 8 * q + 4 * half, a.width, x);
         }
 }
@@ -199,7 +203,7 @@ template <typename T, int NB> constexpr int kShareRows = Tile<T, NB>::kStride > 
 // sums added in their order: four times the workgroups, each with a quarter of the work, for
 // calls of few keys, and (far) for the sinks against a chunk of the tiles past their window,
 // whose sums go to far_parts.
-template <typename T, int NB, bool SHARE>
+template <typename T, int NB, int PLANES, bool SHARE>
 __global__ __launch_bounds__(kThreads, NB <= 2 ? 2 : 1) void window_dkv_kernel(Backward f, int far) {
     using L = Tile<T, NB>;
     constexpr int RT = SHARE ? kShareRows<T, NB> : kKeys<T>, RB = RT / 32, RW = (RT + 63) / 64;
@@ -255,12 +259,17 @@ __global__ __launch_bounds__(kThreads, NB <= 2 ? 2 : 1) void window_dkv_kernel(B
     const uint8_t* shown_at = valid ? valid + before : static_cast<const uint8_t*>(a.q);  // any byte where all are valid
     constexpr int SE = (2 * RT + kThreads - 1) / kThreads;  // statistics a thread brings
     uint8_t next_ok[RW] = {};
+    float next_delta[RW] = {};
     float next_stat[SE] = {};
     int next_head = walk ? t0 / walk : 0, next_p = first + (walk ? t0 % walk : 0) * RT;  // of the tile to fetch
     auto fetch = [&]() {
         const int p0 = next_p, last = a.length - 1 - p0;
 #pragma unroll
-        for (int w = 0; w < RW; ++w) next_ok[w] = shown_at[valid ? min(p0 + 64 * w + lane, a.length - 1) : 0];
+        for (int w = 0; w < RW; ++w) {
+            const int p = min(p0 + 64 * w + lane, a.length - 1);
+            next_ok[w] = shown_at[valid ? p : 0];
+            next_delta[w] = f.delta[stat + static_cast<int64_t>(next_head) * a.length + p];
+        }
 #pragma unroll
         for (int i = 0; i < SE; ++i) {
             const int n = static_cast<int>(threadIdx.x) + i * kThreads;
@@ -274,13 +283,14 @@ __global__ __launch_bounds__(kThreads, NB <= 2 ? 2 : 1) void window_dkv_kernel(B
     int p0 = next_p;
     if (t0 < t1) fetch();
     for (int t = t0; t < t1; ++t, p0 = p0 + RT >= to ? first : p0 + RT) {
-        uint64_t shown[RW];
-        bool every = true, some = false;
+        uint64_t shown[RW], alone[RW];  // alone: see one key
+        bool every = true, some = false, any_alone = false;
 #pragma unroll
         for (int w = 0; w < RW; ++w) {
             const int r = 64 * w + lane;
             shown[w] = __ballot(r < RT && p0 + r < a.length && (!valid || next_ok[w]));
-            every = every && shown[w] == low_bits(RT - 64 * w), some = some || shown[w];
+            alone[w] = __ballot(next_delta[w] == INFINITY);
+            every = every && shown[w] == low_bits(RT - 64 * w), some = some || shown[w], any_alone = any_alone || alone[w];
         }
         // every key of the workgroup is seen by every row of the tile
         const bool all = !far && every && !valid && p0 >= begins(key0 + kOwn - 1) && p0 + RT <= ends(key0) && key0 + kOwn <= a.total;
@@ -317,10 +327,10 @@ __global__ __launch_bounds__(kThreads, NB <= 2 ? 2 : 1) void window_dkv_kernel(B
                 }
             }
         };
-        auto block = [&](int rb, uint32_t block_shown) {
+        auto block = [&](int rb, uint32_t block_shown, uint32_t block_alone) {
             const int pb = p0 + rb * 32;
             if (far ? pb + 32 <= wave_end : (pb + 32 <= wave_begin || pb >= wave_last_end)) return;
-            const bool masked = far || !(block_shown == ~0u && wave_whole && pb >= wave_last_begin && pb + 32 <= wave_end);
+            const bool masked = far || !(block_shown == ~0u && !block_alone && wave_whole && pb >= wave_last_begin && pb + 32 <= wave_end);
             f32x16 s, d;
             products(rb, s, d);
             terms(rb, s, d);
@@ -328,26 +338,27 @@ __global__ __launch_bounds__(kThreads, NB <= 2 ? 2 : 1) void window_dkv_kernel(B
             if (masked) {
                 const uint64_t by_place = far ? ~low_bits(key_end - pb) : ~low_bits(key_begin - pb) & low_bits(key_end - pb);
                 seen = key_ok ? static_cast<uint32_t>(by_place) & block_shown : 0u;
-                const uint32_t mine = seen >> (4 * half);
+                const uint32_t mine = seen >> (4 * half), moved = (seen & ~block_alone) >> (4 * half);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     s[r] = where_seen(mine, r, s[r], 0.0f);
-                    d[r] = where_seen(mine, r, d[r], 0.0f);
+                    d[r] = where_seen(moved, r, d[r], 0.0f);
                 }
             }
             range.fit(d, dk);
             if (masked && bad_tile == t) {
                 seen_acc<T, NB>(dv, g_tile, rb * 32, s, seen, scratch[wave]);
-                seen_acc<T, NB>(dk, q_tile, rb * 32, d, seen, scratch[wave]);
+                seen_acc<T, NB>(dk, q_tile, rb * 32, d, seen & ~block_alone, scratch[wave]);
             } else {
-                mma_acc<T, NB>(dv, g_tile, rb * 32, s);
-                mma_acc<T, NB>(dk, q_tile, rb * 32, d);
+                mma_acc<T, NB, PLANES>(dv, g_tile, rb * 32, s);
+                mma_acc<T, NB, PLANES>(dk, q_tile, rb * 32, d);
             }
         };
         if (SHARE) {
             const int rb = (wave - t * RB) & (kWaves - 1);
-            if (rb < RB) block(rb, static_cast<uint32_t>(shown[RW > 1 ? rb / 2 : 0] >> (32 * (rb & 1))));
-        } else if (NB <= 2 && every && wave_whole && p0 >= wave_last_begin && p0 + RT <= wave_end) {
+            const int w = RW > 1 ? rb / 2 : 0;
+            if (rb < RB) block(rb, static_cast<uint32_t>(shown[w] >> (32 * (rb & 1))), static_cast<uint32_t>(alone[w] >> (32 * (rb & 1))));
+        } else if (NB <= 2 && every && !any_alone && wave_whole && p0 >= wave_last_begin && p0 + RT <= wave_end) {
             // all seen: without a branch, so that one block's products run beside the other's terms (heads of 64: 115 ->
             // 109 us; wider ones have no registers for both blocks)
             f32x16 s[RB], d[RB];
@@ -357,15 +368,15 @@ __global__ __launch_bounds__(kThreads, NB <= 2 ? 2 : 1) void window_dkv_kernel(B
             for (int rb = 0; rb < RB; ++rb) {
                 terms(rb, s[rb], d[rb]);
                 range.fit(d[rb], dk);
-                mma_acc<T, NB>(dv, g_tile, rb * 32, s[rb]);
-                mma_acc<T, NB>(dk, q_tile, rb * 32, d[rb]);
+                mma_acc<T, NB, PLANES>(dv, g_tile, rb * 32, s[rb]);
+                mma_acc<T, NB, PLANES>(dk, q_tile, rb * 32, d[rb]);
             }
         } else if (NB <= 2) {
 #pragma unroll 1
-            for (int rb = 0; rb < RB; ++rb) block(rb, static_cast<uint32_t>(shown[0] >> (32 * rb)));
+            for (int rb = 0; rb < RB; ++rb) block(rb, static_cast<uint32_t>(shown[0] >> (32 * rb)), static_cast<uint32_t>(alone[0] >> (32 * rb)));
         } else {
 #pragma unroll
-            for (int rb = 0; rb < RB; ++rb) block(rb, static_cast<uint32_t>(shown[0] >> (32 * rb)));
+            for (int rb = 0; rb < RB; ++rb) block(rb, static_cast<uint32_t>(shown[0] >> (32 * rb)), static_cast<uint32_t>(alone[0] >> (32 * rb)));
         }
     }
     const float unlift = std::is_same<T, f16>::value ? 1.0f / 256.0f : 1.0f;
@@ -456,18 +467,18 @@ int64_t far_each(const Shape& s, const Backward& f) {
 size_t far_values(const Shape& s, const Backward& f) { return static_cast<size_t>(f.far_chunks) * far_each(s, f); }
 
 
-template <typename T, int NB>
-int run(const Backward& f, hipStream_t stream) {
+template <typename T, int NB, int PLANES>
+int run_planes(const Backward& f, hipStream_t stream) {
     const int64_t heads = static_cast<int64_t>(f.s.batch) * f.s.groups;
     const char* what = "koemi_window_attention_backward";
     int rc = KOEMI_OK;
     if (f.row_tiles) {
-        hipLaunchKernelGGL((window_dq_kernel<T, NB>), dim3(static_cast<unsigned>(heads * f.row_tiles)), dim3(kThreads), 0, stream, f);
+        hipLaunchKernelGGL((window_dq_kernel<T, NB, PLANES>), dim3(static_cast<unsigned>(heads * f.row_tiles)), dim3(kThreads), 0, stream, f);
         rc = check_launch(what);
     }
     if (rc != KOEMI_OK || (!f.dk && !f.dv)) return rc;
     if (f.far_chunks) {
-        hipLaunchKernelGGL((window_dkv_kernel<T, NB, true>), dim3(static_cast<unsigned>(heads * f.far_tiles * f.far_chunks)),
+        hipLaunchKernelGGL((window_dkv_kernel<T, NB, PLANES, true>), dim3(static_cast<unsigned>(heads * f.far_tiles * f.far_chunks)),
                            dim3(kThreads), 0, stream, f, 1);
         rc = check_launch(what);
         if (rc != KOEMI_OK) return rc;
@@ -482,11 +493,17 @@ int run(const Backward& f, hipStream_t stream) {
     // and spread it where the wide ones leave compute units idle (70 of them at [5, 777]: 31.6 us against 45.7).
     const int64_t wide = heads * ((f.s.total + kRows - 1) / kRows);
     if (wide < 160)
-        hipLaunchKernelGGL((window_dkv_kernel<T, NB, true>), dim3(static_cast<unsigned>(heads * ((f.s.total + 31) / 32))),
+        hipLaunchKernelGGL((window_dkv_kernel<T, NB, PLANES, true>), dim3(static_cast<unsigned>(heads * ((f.s.total + 31) / 32))),
                            dim3(kThreads), 0, stream, f, 0);
     else
-        hipLaunchKernelGGL((window_dkv_kernel<T, NB, false>), dim3(static_cast<unsigned>(wide)), dim3(kThreads), 0, stream, f, 0);
+        hipLaunchKernelGGL((window_dkv_kernel<T, NB, PLANES, false>), dim3(static_cast<unsigned>(wide)), dim3(kThreads), 0, stream, f, 0);
     return check_launch(what);
+}
+
+template <typename T, int NB>
+int run(const Backward& f, hipStream_t stream) {
+    if (sizeof(T) == 2 && two_planes(f.s, sizeof(T))) return run_planes<T, NB, sizeof(T) == 2 ? 2 : 1>(f, stream);
+    return run_planes<T, NB, 1>(f, stream);
 }
 
 template <typename T>

@@ -162,3 +162,18 @@ def test_against_float64(device, batch, length, heads, groups, width, window, si
 def test_keys_carried_before_the_queries(device, length, total, window, sinks, mask, dtype):
     args = make((2, length, 4, 2, 64), dtype, length, mask, total=total)
     check(*args, window, sinks)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("length, total, window, sinks, mask", [
+    (1, 1, 5, 2, None), (77, 77, 1, 0, None), (130, 160, 1, 0, "random"), (3, 3, 9, 0, "single"), (400, 400, 1, 0, "tail")])
+def test_one_visible_key_has_no_gradient_through_its_score(device, length, total, window, sinks, mask, dtype):
+    q, k, v, valid, d_out = make((2, length, 4, 2, 48), dtype, 5, None if mask == "single" else mask, total=total)
+    if mask == "single":
+        valid = torch.arange(total, device=device)[None].expand(2, -1) == 1
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = W.window_attention(*leaves, valid, window=window, sinks=sinks)
+    d_q, d_k, d_v = torch.autograd.grad(out, leaves, d_out)
+    assert not d_q.any() and not d_k.any()
+    check(q, k, v, valid, d_out, window, sinks)
