@@ -613,8 +613,8 @@ int cache_of(const char* what, void* keys, float* key_scales, void* values, floa
         return fail(KOEMI_ERR_INVALID, "%s: sizes must be positive, batch and sinks not negative", what);
     if (width > 256) return fail(KOEMI_ERR_UNSUPPORTED, "%s: heads are at most 256 wide", what);
     if (code != kInt8 && code != kE4m3) return fail(KOEMI_ERR_UNSUPPORTED, "%s: codes are int8 (0) or e4m3 (1)", what);
-    if (window >= (int64_t(1) << 31) || sinks >= (int64_t(1) << 31) - window || batch >= (1 << 24) || groups >= (1 << 20) ||
-        (window + sinks) * groups >= (int64_t(1) << 31))
+    if (window >= (int64_t(1) << 31) || sinks >= (int64_t(1) << 31) || batch >= (1 << 24) || groups >= (1 << 20) ||
+        (window + sinks) * groups >= (int64_t(1) << 31) - 256)
         return fail(KOEMI_ERR_UNSUPPORTED, "%s: at most 2^31 entries x key heads, 2^20 key heads and 2^24 rows", what);
     if (batch && (!keys || !key_scales || !values || !value_scales)) return fail(KOEMI_ERR_INVALID, "%s: null pointer", what);
     if (reinterpret_cast<uintptr_t>(keys) % 16 || reinterpret_cast<uintptr_t>(values) % 16)

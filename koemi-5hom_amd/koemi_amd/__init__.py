@@ -10,6 +10,8 @@ Module map (reference front -> this package):
 * ``koemi.model.memory`` (BoundedRecurrentState.gates, + network.py:306-310 scan) -> ``koemi_amd.recurrent``
 * ``koemi.cuda_kernels.moe``    -> ``koemi_amd.moe``       (route/permute/grouped MLP/combine)
 * ``koemi.cuda_kernels.loader`` -> ``koemi_amd.loader``
+* ``koemi.runtime.fast_decode`` (TokenSampler) -> ``koemi_amd.sampling``
+* the local memory with heads, trained and served (no module of the reference): ``koemi_amd.window``
 
 Every operator runs from ``libkoemi_hip.so`` (C ABI in ``include/koemi_hip.h``):
 hand-written HIP kernels, with rocBLAS for the plain GEMMs of the salient read
@@ -33,9 +35,20 @@ from koemi_amd.moe import (
     route_topk_modulo,
     route_topk_valid,
 )
+from koemi_amd.sampling import sample_tokens
 from koemi_amd.think import benchmark_causal_surprise, causal_surprise, salience_admission, surprise_from_logits
+from koemi_amd.window import (
+    WindowCache,
+    window_attention,
+    window_cache,
+    window_cache_entries,
+    window_cache_read,
+    window_cache_step,
+    window_cache_write,
+)
 
 __all__ = [
+    "WindowCache",
     "benchmark_causal_surprise",
     "causal_surprise",
     "combine_topk",
@@ -61,5 +74,12 @@ __all__ = [
     "recurrent_gates",
     "recurrent_scan",
     "salient_tail",
+    "sample_tokens",
     "surprise_from_logits",
+    "window_attention",
+    "window_cache",
+    "window_cache_entries",
+    "window_cache_read",
+    "window_cache_step",
+    "window_cache_write",
 ]

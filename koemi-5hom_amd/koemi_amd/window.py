@@ -114,8 +114,6 @@ def _plan(query: tuple, key: tuple, value: tuple, query_stride: tuple, key_strid
             raise CudaThinkValidationError(f"{name} must have shape [batch, length, heads, width]")
     if dtype not in _SUPPORTED_DTYPES:
         raise CudaThinkValidationError("queries, keys and values must be float32, float16 or bfloat16")
-    if device != "cuda":
-        raise CudaThinkValidationError("queries, keys and values must be on CUDA")
     batch, length, heads, width = query
     if key != value or key[0] != batch or key[3] != width:
         raise CudaThinkValidationError("keys and values must have the same shape [batch, total, key heads, width], "
@@ -132,6 +130,8 @@ def _plan(query: tuple, key: tuple, value: tuple, query_stride: tuple, key_strid
     size = dtype.itemsize
     if heads * (width + 8) * size >= 1 << 24:
         raise CudaThinkValidationError("too many heads: a position's must be less than 2^24 bytes")
+    if device != "cuda":
+        raise CudaThinkValidationError("queries, keys and values must be on CUDA")
     _load()
     padded = -(-width * size // 16) * 16 // size
     code = _native.dtype_code(dtype)
@@ -288,9 +288,12 @@ def window_cache(batch: int, heads: int, width: int, *, window: int, sinks: int 
 def _check_cache(cache: object) -> WindowCache:
     if not isinstance(cache, WindowCache):
         raise CudaThinkValidationError("cache must be a WindowCache")
+    return cache
+
+
+def _check_cuda(cache: WindowCache) -> None:
     if cache.keys.device.type != "cuda":
         raise CudaThinkValidationError("cache must be on CUDA")
-    return cache
 
 
 def _check_tensor(cache: WindowCache, name: str, tensor: object) -> None:
@@ -342,6 +345,7 @@ def window_cache_write(cache: WindowCache, keys: Tensor, values: Tensor, lengths
     _check_rows("values", values.shape, wanted, values.dtype, keys.dtype)
     lengths = _check_counts(cache, "lengths", lengths)
     counts = _check_counts(cache, "counts", counts) if counts is not None else None
+    _check_cuda(cache)
     _load()
     k, v = _in_rows(keys.detach()), _in_rows(values.detach())
     with _native.device_guard(k.device):
@@ -363,6 +367,7 @@ def window_cache_entries(cache: WindowCache, lengths: Tensor, *, dtype: torch.dt
     lengths = _check_counts(cache, "lengths", lengths)
     if dtype not in _SUPPORTED_DTYPES:
         raise CudaThinkValidationError("dtype must be float32, float16 or bfloat16")
+    _check_cuda(cache)
     _load()
     batch, groups, slots, _ = cache.keys.shape
     device = cache.keys.device
@@ -419,6 +424,7 @@ def _step(cache: WindowCache, queries: Tensor, keys: Tensor | None, values: Tens
         if not isinstance(active, Tensor) or active.dtype != torch.bool or active.shape != shape[:1] or active.device != device:
             raise CudaThinkValidationError("active must be a bool [batch] tensor on the cache's device")
         active = active.contiguous()
+    _check_cuda(cache)
     q, k, v = queries, keys, values
     if strides is None:
         q, k, v = (_in_rows(t.detach()) if t is not None else None for t in (q, k, v))

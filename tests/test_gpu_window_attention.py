@@ -177,3 +177,299 @@ def test_one_visible_key_has_no_gradient_through_its_score(device, length, total
     d_q, d_k, d_v = torch.autograd.grad(out, leaves, d_out)
     assert not d_q.any() and not d_k.any()
     check(q, k, v, valid, d_out, window, sinks)
+
+
+def together(leaves, out, d_out, wanted):
+    return torch.autograd.grad(out, [t for t, w in zip(leaves, wanted) if w], d_out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("layout", ["fused", "heads first", "shared keys", "odd start", "odd columns", "reversed columns", "one row for all"])
+def test_any_strides(device, layout, dtype):
+    """Views of one projection, transposed and broadcast inputs, starts and strides off 16 bytes: as contiguous copies."""
+
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    draw = lambda *shape: torch.randn(shape, device=device, generator=gen).to(dtype)  # noqa: E731
+    B, L, H, G, D = 2, 90, 4, 2, 64
+    if layout == "fused":
+        wide = draw(B, L, (H + 2 * G) * D)
+        q, k, v = (t.unflatten(-1, (-1, D)) for t in wide.split([H * D, G * D, G * D], dim=-1))
+    elif layout == "heads first":
+        q, k, v = draw(B, H, L, D).transpose(1, 2), draw(B, G, L, D).transpose(1, 2), draw(B, G, L, D).transpose(1, 2)
+    elif layout == "shared keys":
+        q, k, v = draw(B, L, H, D), draw(B, L, 1, D).expand(-1, -1, H, -1), draw(1, L, 1, D).expand(B, -1, H, -1)
+    elif layout == "odd start":
+        q, k, v = draw(B, L, H, D), draw(B * L * G * D + 1)[1:].view(B, L, G, D), draw(B, L, G, D)
+    elif layout == "odd columns":
+        q, k, v = draw(B, L, H, D + 3)[..., 1:D + 1], draw(B, L, G, D), draw(B, L, G, D + 1)[..., :D]
+    elif layout == "reversed columns":
+        q, k, v = draw(B, L, H, D), draw(B, L, D, G).transpose(2, 3), draw(B, L, G, 2 * D)[..., ::2]
+    else:
+        q, k, v = draw(B, 1, 1, D).expand(-1, L, H, -1), draw(B, L, G, D), draw(1, L, G, D).expand(B, -1, -1, -1)
+    d_out = draw(B, 1, 1, D).expand(-1, L, H, -1)
+    straight = [t.contiguous().detach().requires_grad_() for t in (q, k, v)]
+    want = W.window_attention(*straight, window=20, sinks=2)
+    want_grads = torch.autograd.grad(want, straight, d_out.contiguous())
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    got = W.window_attention(*leaves, window=20, sinks=2)
+    assert torch.equal(got, want)
+    for a, b in zip(torch.autograd.grad(got, leaves, d_out), want_grads):
+        assert torch.equal(a, b)
+    check(q.contiguous(), k.contiguous(), v.contiguous(), None, d_out.contiguous(), 20, 2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("wanted", [(True, False, False), (False, True, False), (False, False, True), (True, False, True)])
+def test_gradients_of_some_inputs(device, wanted):
+    q, k, v, valid, d_out = make((2, 100, 4, 2, 64), torch.bfloat16, 9, "tail")
+    every = [t.detach().requires_grad_() for t in (q, k, v)]
+    want = torch.autograd.grad(W.window_attention(*every, valid, window=30, sinks=3), every, d_out)
+    leaves = [t.detach().requires_grad_(w) for t, w in zip((q, k, v), wanted)]
+    got = together(leaves, W.window_attention(*leaves, valid, window=30, sinks=3), d_out, wanted)
+    for a, b in zip(got, [t for t, w in zip(want, wanted) if w]):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_what_is_not_finite_reaches_only_those_who_see_it(device, value, dtype):
+    """NaN and infinities at valid positions: rows that do not see them, and the gradients of keys that their rows do
+    not see, are what they are without them, within the bounds of any order of their sums."""
+
+    window, sinks, length, at = 40, 2, 200, 90
+    q, k, v, _, d_out = make((1, length, 4, 2, 64), dtype, 3, None)
+    want, bounds = reference(q, k, v, None, window, sinks, 0.125, d_out)
+
+    def unmoved(got, n, rows, name):
+        close(got[:, rows], want[n][:, rows], bounds[n][:, rows], (name, n))
+
+    i = torch.arange(length, device=device)
+    sees = (i >= at) & (i - at < window)          # queries that see position `at`
+    seen = ((i <= at) & (at - i < window)) | (i < sinks)  # keys that the query there sees
+    for name in ("keys", "values", "queries", "d_out"):
+        t = {"queries": q.clone(), "keys": k.clone(), "values": v.clone(), "d_out": d_out.clone()}
+        t[name][0, at, :, 5] = value
+        leaves = [t[n].requires_grad_() for n in ("queries", "keys", "values")]
+        out = W.window_attention(*leaves, window=window, sinks=sinks)
+        grads = torch.autograd.grad(out, leaves, t["d_out"])
+        hit = sees if name in ("keys", "values") else (i == at) & (name == "queries")
+        unmoved(out, 0, ~hit, name)
+        assert not hit.any() or not torch.isfinite(out[0, hit]).all(), name
+        rows = sees if name in ("keys", "values") else i == at
+        unmoved(grads[0], 1, ~rows, name)
+        # keys seen by any row that holds something not finite
+        reached = seen if name in ("queries", "d_out") else (i > at - window) & (i < at + window) | (i < sinks)
+        unmoved(grads[1], 2, ~reached, name)
+        unmoved(grads[2], 3, ~reached, name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [2.0 ** -24, 2.0 ** -16, 1.0, 2.0 ** 10])
+def test_half_precision_gradients_of_any_size(device, size):
+    """fp16 derivatives far below and above one keep their digits between the products: the gradients are those of d_out =
+    1 times size, as far as fp16 holds them."""
+
+    q, k, v, valid, d_out = make((1, 200, 2, 1, 64), torch.float16, 21, "tail")
+    d_out = (d_out.float() * size).half()
+    check(q, k, v, valid, d_out, 64, 2)
+
+
+@pytest.mark.gpu
+def test_gradients_against_differences(device):
+    """Central differences of the float32 output along random directions: with steps h of 2^-6 the cubic term is below 2^-11 of
+    the slope's size here (scores move by under 1/2), rounding (2^-20 of the output's sum of sizes, over h) below 2^-12."""
+
+    q, k, v, valid, d_out = make((2, 60, 4, 2, 32), torch.float32, 4, "tail", junk=False)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    grads = torch.autograd.grad(W.window_attention(*leaves, valid, window=17, sinks=2), leaves, d_out)
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    h = 2.0 ** -6
+    for n in range(3):
+        along = torch.randn(leaves[n].shape, device=device, generator=gen)
+        ends = []
+        for sign in (1.0, -1.0):
+            moved = [t.detach() + (sign * h * along if m == n else 0.0) for m, t in enumerate(leaves)]
+            ends.append(W.window_attention(*moved, valid, window=17, sinks=2).double())
+        slope = ((ends[0] - ends[1]) * d_out.double()).sum() / (2 * h)
+        want = (grads[n].double() * along.double()).sum()
+        size = (grads[n].double() * along.double()).norm()
+        assert abs(slope - want) <= 2.0 ** -5 * size, (n, slope.item(), want.item(), size.item())
+
+
+@pytest.mark.gpu
+def test_the_same_bits_every_time_and_on_two_streams(device):
+    args = [make((2, 700, 8, 2, 64), torch.bfloat16, seed, "tail") for seed in (1, 2)]
+
+    def step(q, k, v, valid, d_out):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        out = W.window_attention(*leaves, valid, window=100, sinks=4)
+        return (out, *torch.autograd.grad(out, leaves, d_out))
+
+    want = [step(*a) for a in args]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in args]
+    for _ in range(3):
+        got = []
+        for a, s in zip(args, streams):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                got.append(step(*a))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.gpu
+def test_captured_forward_and_backward(device):
+    """A training step in a graph: replays with new inputs, with eager work between them, equal eager steps."""
+
+    q, k, v, valid, d_out = make((2, 300, 4, 2, 64), torch.bfloat16, 1, "tail")
+    static = [t.detach().clone().requires_grad_() for t in (q, k, v)]
+    up, mask = d_out.clone(), valid.clone()
+
+    def step(leaves, m, d):
+        out = W.window_attention(*leaves, m, window=60, sinks=4)
+        return (out.detach(), *torch.autograd.grad(out, leaves, d))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(static, mask, up)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step(static, mask, up)
+    for seed in range(4):
+        new = make((2, 300, 4, 2, 64), torch.bfloat16, 30 + seed, "random")
+        with torch.no_grad():
+            for s, t in zip((*static, mask, up), new):
+                s.copy_(t)
+        graph.replay()
+        leaves = [t.detach().requires_grad_() for t in new[:3]]
+        want = step(leaves, new[3], new[4])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(captured, want)), seed
+
+
+@pytest.mark.gpu
+def test_past_2_31_elements(device):
+    """A key tensor of more than 2^31 elements: the last queries, whose window and sinks are its ends."""
+
+    total, groups, width, window, sinks, length = 270000, 64, 128, 96, 3, 70
+    assert total * groups * width > 1 << 31
+    near = window + length
+    q, k, v, _, d_out = make((1, length, groups, groups, width), torch.bfloat16, 6, None, total=near + sinks)
+    big = [torch.full((1, total, groups, width), float("nan"), device=device, dtype=torch.bfloat16) for _ in range(2)]
+    for full, part in zip(big, (k, v)):
+        full[:, :sinks], full[:, total - near:] = part[:, :sinks], part[:, sinks:]
+    leaves = [t.requires_grad_() for t in (q, *big)]
+    out = W.window_attention(*leaves, window=window, sinks=sinks)
+    d_q, d_k, d_v = torch.autograd.grad(out, leaves, d_out)
+    # in a short call the same pairs are seen: the sinks far behind the window are the first keys
+    want, bounds = reference(q, k, v, None, window, sinks, 1.0 / math.sqrt(width), d_out)
+    close(out, want[0], bounds[0], "out")
+    close(d_q, want[1], bounds[1], "d_queries")
+    for got, w, b, name in ((d_k, want[2], bounds[2], "d_keys"), (d_v, want[3], bounds[3], "d_values")):
+        close(got[:, :sinks], w[:, :sinks], b[:, :sinks], name)
+        close(got[:, total - near:], w[:, sinks:], b[:, sinks:], name)
+        assert not got[:, sinks:total - near].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch, length, total", [(0, 5, 5), (2, 0, 0), (2, 0, 9)])
+def test_nothing_to_do(device, batch, length, total):
+    q = torch.zeros(batch, length, 4, 32, device=device, requires_grad=True)
+    k, v = (torch.zeros(batch, total, 2, 32, device=device, requires_grad=True) for _ in range(2))
+    out = W.window_attention(q, k, v, window=3, sinks=1)
+    grads = torch.autograd.grad(out, (q, k, v), torch.ones_like(out))
+    assert out.shape == q.shape and all(g.shape == t.shape and not g.any() for g, t in zip(grads, (q, k, v)))
+
+
+@pytest.mark.gpu
+def test_windows_and_sinks_past_the_length_and_other_scales(device):
+    q, k, v, valid, d_out = make((2, 120, 4, 2, 64), torch.bfloat16, 14, "random")
+    whole = W.window_attention(q, k, v, valid, window=120)
+    for window, sinks in ((1 << 40, 0), (1, 1 << 40), (7, 120)):
+        close(W.window_attention(q, k, v, valid, window=window, sinks=sinks),
+              *reference(q, k, v, valid, min(window, 1 << 30), min(sinks, 1 << 30), 0.125), (window, sinks))
+    assert torch.equal(W.window_attention(q, k, v, valid, window=1 << 40, scale=0.125), whole)
+    check(q, k, v, valid, d_out, 50, 3, scale=1.0)
+    check(q, k, v, valid, d_out, 50, 3, scale=2.0 ** -20)
+
+
+REFUSED = [
+    (dict(q=(2, 5, 4)), "shape"), (dict(k=(2, 5, 2, 16)), "same shape"), (dict(q=(2, 6, 4, 8)), "no fewer keys"),
+    (dict(k=(2, 5, 3, 8), v=(2, 5, 3, 8)), "divide"), (dict(q=(2, 5, 4, 300), k=(2, 5, 2, 300), v=(2, 5, 2, 300)), "wide"),
+    (dict(dtype=torch.float64), "float32, float16 or bfloat16"), (dict(window=0), "window must be a positive integer"),
+    (dict(window=True), "window must be a positive integer"), (dict(window=2.0), "window must be a positive integer"),
+    (dict(sinks=-1), "sinks must be a non-negative integer"), (dict(scale=0.0), "scale must be"), (dict(scale=True), "scale must be"),
+    (dict(scale=float("inf")), "scale must be"), (dict(scale=float("nan")), "scale must be"), (dict(), "must be on CUDA"),
+]
+
+
+@pytest.mark.parametrize("change, message", REFUSED)
+def test_refusals(change, message):
+    shapes = {"q": (2, 5, 4, 8), "k": (2, 5, 2, 8), "v": (2, 5, 2, 8)} | {n: s for n, s in change.items() if n in "qkv"}
+    q, k, v = (torch.zeros(shapes[n], dtype=change.get("dtype", torch.float32)) for n in "qkv")
+    numbers = {"window": 4} | {n: x for n, x in change.items() if n in ("window", "sinks", "scale")}
+    with pytest.raises(CudaThinkValidationError, match=message):
+        W.window_attention(q, k, v, **numbers)
+
+
+def test_refusals_of_mixed_inputs():
+    q, k = torch.zeros(2, 5, 4, 8), torch.zeros(2, 5, 2, 8)
+    with pytest.raises(CudaThinkValidationError, match="torch.Tensor"):
+        W.window_attention(q, k, None, window=3)
+    with pytest.raises(CudaThinkValidationError, match="share a dtype"):
+        W.window_attention(q, k, k.half(), window=3)
+
+
+@pytest.mark.gpu
+def test_masks_that_are_refused(device):
+    q, k = torch.zeros(2, 5, 4, 8, device=device), torch.zeros(2, 6, 2, 8, device=device)
+    for mask in (torch.ones(2, 5, dtype=torch.bool, device=device), torch.ones(2, 6, device=device), torch.ones(2, 6, dtype=torch.bool)):
+        with pytest.raises(CudaThinkValidationError, match="valid_mask"):
+            W.window_attention(q, k, k, mask, window=3)
+
+
+def test_the_library_refuses_what_its_kernels_cannot_take():
+    """Checked on the host, before any launch: addresses and strides off 16 bytes, sizes past the indices."""
+
+    import ctypes
+
+    from koemi_amd import _native
+
+    strides = (ctypes.c_int64 * 9)(*[64 * 4, 64, 16] * 3)
+
+    def call(q=16, stride=strides, batch=1, length=4, total=4, heads=4, groups=4, width=16, window=2, sinks=0, scale=1.0, out=16):
+        return lambda: _native.call("koemi_window_attention_forward", q, 16, 16, None, stride, out, None, None, batch, length, total,
+                                    heads, groups, width, window, sinks, scale, _native.F32, None, 0, None)
+
+    odd = (ctypes.c_int64 * 9)(*[64 * 4, 64, 17] * 3)
+    far = (ctypes.c_int64 * 9)(*[1 << 30, 1 << 23, 16] * 3)
+    for bad, message in ((call(q=20), "aligned"), (call(stride=odd), "aligned"), (call(stride=far), "2\\^24 bytes"), (call(width=18), "pieces"),
+                         (call(width=320), "256"), (call(heads=3), "divide"), (call(window=0), "window"), (call(scale=-1.0), "scale"),
+                         (call(total=3), "no fewer keys"), (call(length=1 << 30, total=1 << 30), "2\\^29"), (call(out=None), "null pointer")):
+        with pytest.raises(_native.NativeCallError, match=message):
+            bad()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("width, mask", [(32, "random"), (64, "tail"), (64, None), (96, "tail"), (128, None), (160, "random"), (256, "tail")])
+def test_many_rows(device, width, mask, dtype):
+    """Calls of many rows: probabilities in one plane, 128 keys a workgroup."""
+
+    args = make((160, 130, 4, 1, width), dtype, width, mask)
+    check(*args, 40, 3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_long_rows(device, dtype):
+    """Whole tiles between the window's ends, sinks with many rows past their window."""
+
+    args = make((2, 2300, 16, 4, 64), dtype, 2, "tail")
+    check(*args, 700, 5)
