@@ -1098,10 +1098,13 @@ int koemi_window_cache_step(void* keys, float* key_scales, void* values, float* 
  * in the ids' order, exceeds uniform x the kept sum; 0 for a row without a score. A row with
  * +inf draws among those. probabilities [rows, vocab] fp32 (NULL: none): the distribution
  * drawn from. Weights are formed in 64 bits and added as whole multiples of 2^-44, in any
- * order the same. */
+ * order the same. Workspace: koemi_sample_filtered_workspace_bytes (0 for short rows),
+ * 8-byte aligned, no zeroing needed. */
+size_t koemi_sample_filtered_workspace_bytes(int64_t rows, int64_t vocab);
 int koemi_sample_filtered(const void* logits, int dtype, int64_t row_stride, int64_t rows, int64_t vocab, int64_t exclude,
                           double temperature, int64_t top_k, double top_p, double min_p, const float* uniforms,
-                          int64_t* ids, float* probabilities, koemi_stream_t stream);
+                          int64_t* ids, float* probabilities, void* workspace, size_t workspace_bytes,
+                          koemi_stream_t stream);
 
 /* Measurement only (no counterpart in the reference): reads `bytes` (a
  * multiple of 16) from `src` with `grid` workgroups of `block` threads, each

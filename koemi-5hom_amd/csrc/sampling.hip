@@ -12,10 +12,14 @@
 // histogram of counts and weights over 2048 steps of (max - z) / T; the step that a
 // limit falls into, whose scores are then ranked by their bits, eight at a time, from a list
 // in LDS (or from the row where they are too many); the tiles' kept weights; the tile that
-// u falls into. A row stays in its XCD's L2 between the walks. Bound by the two passes of
-// exponentials (about 25 64-bit operations a score).
+// u falls into. A row stays in its XCD's L2 between the walks. Few long rows are walked by
+// several workgroups each, one launch a phase; a row of one tile stays in a wave's registers.
+// Bound by the two passes of exponentials: 128 rows of 131072 bf16 scores with top-p and min-p
+// take 7 us for the maximum, 26 the histogram, 38 the limit, 20 the kept weights, 7 the pick;
+// one read of the scores takes 7.
 #include "common.hpp"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace koemi {
@@ -59,6 +63,22 @@ __device__ __forceinline__ double pow2(double x) {
     return ldexp(p, static_cast<int>(n));
 }
 
+// The same from 2^(i / 32), i < 32: the series of 2^(f / 32) to the 5th power (the 6th adds below
+// 2^-48). Fourteen 64-bit operations a weight instead of twenty-one.
+constexpr int kTable = 32;
+__device__ __forceinline__ double pow2(double x, const double* table) {
+    constexpr double c = 0.69314718055994530942 / kTable;
+    const double y = x * kTable, n = __builtin_rint(y), f = y - n;
+    const int i = static_cast<int>(n);
+    double p = c * c * c * c * c / 120.0;
+    p = fma(p, f, c * c * c * c / 24.0);
+    p = fma(p, f, c * c * c / 6.0);
+    p = fma(p, f, c * c / 2.0);
+    p = fma(p, f, c);
+    p = fma(p, f, 1.0);
+    return ldexp(p * table[i & (kTable - 1)], i >> 5);
+}
+
 // A row's scores, in tiles.
 template <typename T>
 struct Row {
@@ -66,29 +86,46 @@ struct Row {
     int vocab, exclude;
     bool vector, infinite;  // infinite: the largest is +inf, and only such ones count
     double top, slope;
+    const double* table;    // 2^(i / 32), or null
 
-    // Scores 8 i .. 8 i + 7 of a tile's lane, -inf where there is none.
+    static constexpr int kWords = static_cast<int>(sizeof(T)) / 2;  // of 16 bytes, for eight scores
+
+    // Scores as they count: -inf where there is none, zeros of one sign.
+    __device__ __forceinline__ void clean(int j, float (&x)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            x[i] = x[i] != x[i] || j + i == exclude ? -INFINITY : x[i] + 0.0f;
+            if (infinite) x[i] = x[i] == INFINITY ? 0.0f : -INFINITY;
+        }
+    }
+    // Scores j .. j + 7.
     __device__ __forceinline__ void load(int j, float (&x)[8]) const {
         alignas(16) T e[8];
         if (vector && j + 8 <= vocab) {
 #pragma unroll
-            for (int h = 0; h < static_cast<int>(sizeof(T)) / 2; ++h)
-                reinterpret_cast<uint4*>(e)[h] = reinterpret_cast<const uint4*>(z + j)[h];
+            for (int h = 0; h < kWords; ++h) reinterpret_cast<uint4*>(e)[h] = reinterpret_cast<const uint4*>(z + j)[h];
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = to_f32(e[i]);
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = j + i < vocab ? to_f32(z[j + i]) : -INFINITY;
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            x[i] = x[i] != x[i] || j + i == exclude ? -INFINITY : x[i] + 0.0f;  // no negative zero
-            if (infinite) x[i] = x[i] == INFINITY ? 0.0f : -INFINITY;
+        clean(j, x);
+    }
+    // take(tile, a lane's eight scores) for tiles first, first + step .. below last. Tiles loaded
+    // ahead gain nothing: the exponentials bound the walks, not the loads.
+    template <typename Take>
+    __device__ __forceinline__ void walk(int first, int last, int step, Take take) const {
+#pragma unroll 1
+        for (int t = first; t < last; t += step) {
+            float x[8];
+            load(t * kTile + lane_id() * 8, x);
+            take(t, x);
         }
     }
     __device__ __forceinline__ double weight(float x) const {
         const double e = (static_cast<double>(x) - top) * slope;
-        return e > -100.0 ? pow2(e) : 0.0;
+        return e > -100.0 ? (table ? pow2(e, table) : pow2(e)) : 0.0;
     }
     // w in steps of 2^-44, 0 <= w <= 1: the last bits of 2^52 plus it.
     static __device__ __forceinline__ uint64_t whole(double w) {
@@ -111,6 +148,7 @@ __device__ __forceinline__ float score_of(uint32_t r) { return __uint_as_float(r
 template <int THREADS>
 struct Shared {
     uint64_t mass[kBins];
+    double table[kTable];
     uint32_t count[kBins];
     uint32_t list[kList];
     float gathered[THREADS / kWave][kTile];
@@ -153,20 +191,18 @@ __device__ __forceinline__ int reach(Shared<THREADS>& sh, int n, Value value, do
 template <int THREADS, bool MASS, typename T>
 __device__ float limit(const Row<T>& row, Shared<THREADS>& sh, double target) {
     constexpr int kWaves = THREADS / kWave;
-    const int lane = lane_id(), wave = static_cast<int>(threadIdx.x) / kWave;
+    const int wave = static_cast<int>(threadIdx.x) / kWave;
     uint64_t before;
     const int bin = reach<THREADS>(sh, kBins, [&](int i) { return MASS ? sh.mass[i] : static_cast<uint64_t>(sh.count[i]); },
                                    target, 0, before);
     if (threadIdx.x == 0) sh.listed = 0;
     __syncthreads();
     auto each = [&](auto take) {  // every score of the step
-        for (int t = wave; t * kTile < row.vocab; t += kWaves) {
-            float x[8];
-            row.load(t * kTile + lane * 8, x);
+        row.walk(wave, (row.vocab + kTile - 1) / kTile, kWaves, [&](int, const float (&x)[8]) {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 if (x[i] != -INFINITY && row.bin(x[i]) == bin) take(x[i]);
-        }
+        });
     };
     each([&](float x) {
         const int at = atomicAdd(&sh.listed, 1);
@@ -195,36 +231,48 @@ __device__ float limit(const Row<T>& row, Shared<THREADS>& sh, double target) {
     return score_of(prefix);
 }
 
+// What the phases of a row share: the largest score found, the limits, the kept weights.
 template <int THREADS, typename T>
-__global__ __launch_bounds__(THREADS) void sample_filtered_kernel(Draw f) {
-    constexpr int kWaves = THREADS / kWave;
-    __shared__ Shared<THREADS> sh;
-    const int lane = lane_id(), wave = static_cast<int>(threadIdx.x) / kWave;
-    const int64_t r = blockIdx.x;
-    Row<T> row{static_cast<const T*>(f.logits) + r * f.row_stride, f.vocab, static_cast<int>(f.exclude), f.vector != 0, false, 0.0, f.slope};
-    const int tiles = (f.vocab + kTile - 1) / kTile;
-    float top = -INFINITY;
-    for (int t = wave; t < tiles; t += kWaves) {
-        float x[8];
-        row.load(t * kTile + lane * 8, x);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, x[i]);
+struct Phases {
+    static constexpr int kWaves = THREADS / kWave;
+    const Draw& f;
+    Shared<THREADS>& sh;
+    Row<T> row;
+    int64_t r;
+    int tiles, lane, wave;
+    bool none, by_k, by_p;
+
+    __device__ __forceinline__ Phases(const Draw& draw, Shared<THREADS>& shared, int64_t index)
+        : f(draw), sh(shared),
+          row{static_cast<const T*>(draw.logits) + index * draw.row_stride, draw.vocab, static_cast<int>(draw.exclude), draw.vector != 0, false, 0.0, draw.slope, shared.table},
+          r(index), tiles((draw.vocab + kTile - 1) / kTile), lane(lane_id()), wave(static_cast<int>(threadIdx.x) / kWave) {
+        if (threadIdx.x < kTable) sh.table[threadIdx.x] = pow2(-1.0 + threadIdx.x / static_cast<double>(kTable)) * 2.0;
+        __syncthreads();
     }
-    top = wave_max_xor(top);
-    if (lane == 0) sh.wave_top[wave] = top;
-    __syncthreads();
-    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, sh.wave_top[w]);
-    row.infinite = top == INFINITY;
-    row.top = row.infinite ? 0.0 : static_cast<double>(top);
-    const bool none = top == -INFINITY;
-    const bool by_k = !none && f.top_k > 0 && f.top_k < f.vocab, by_p = !none && f.top_p < 1.0;
-    float least = -INFINITY;  // of the kept scores
-    if (by_k || by_p) {
+
+    // The largest of tiles first .. last - 1, in every thread.
+    __device__ __forceinline__ float largest(int first, int last) {
+        float top = -INFINITY;
+        row.walk(first + wave, last, kWaves, [&](int, const float (&x)[8]) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = fmaxf(top, x[i]);
+        });
+        top = wave_max_xor(top);
+        if (lane == 0) sh.wave_top[wave] = top;
+        __syncthreads();
+        for (int w = 0; w < kWaves; ++w) top = fmaxf(top, sh.wave_top[w]);
+        return top;
+    }
+    __device__ __forceinline__ void begin(float top) {
+        row.infinite = top == INFINITY;
+        row.top = row.infinite ? 0.0 : static_cast<double>(top);
+        none = top == -INFINITY;
+        by_k = !none && f.top_k > 0 && f.top_k < f.vocab, by_p = !none && f.top_p < 1.0;
+    }
+    __device__ __forceinline__ void histogram(int first, int last) {
         for (int i = threadIdx.x; i < kBins; i += THREADS) sh.mass[i] = 0, sh.count[i] = 0;
         __syncthreads();
-        for (int t = wave; t < tiles; t += kWaves) {
-            float x[8];
-            row.load(t * kTile + lane * 8, x);
+        row.walk(first + wave, last, kWaves, [&](int, const float (&x)[8]) {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 if (x[i] != -INFINITY) {
@@ -232,103 +280,223 @@ __global__ __launch_bounds__(THREADS) void sample_filtered_kernel(Draw f) {
                     if (by_k) atomicAdd(&sh.count[b], 1u);
                     if (by_p) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.mass[b]), static_cast<unsigned long long>(Row<T>::whole(row.weight(x[i]))));
                 }
-        }
+        });
         __syncthreads();
+    }
+    // The least kept score by top-k and top-p, from the whole row's histogram.
+    __device__ __forceinline__ float least() {
+        float at = -INFINITY;
         if (by_k) {
             uint64_t own = 0, available;
             for (int i = threadIdx.x; i < kBins; i += THREADS) own += sh.count[i];
             block_exclusive_scan<THREADS, uint64_t>(own, sh.scan, available);
-            if (static_cast<uint64_t>(f.top_k) < available) least = limit<THREADS, false>(row, sh, static_cast<double>(f.top_k));
+            if (static_cast<uint64_t>(f.top_k) < available) at = limit<THREADS, false>(row, sh, static_cast<double>(f.top_k));
         }
         if (by_p) {
             // the sum that p is of: of what top-k leaves
             uint64_t own = 0, total;
-            const int edge = least == -INFINITY ? kBins : row.bin(least);
+            const int edge = at == -INFINITY ? kBins : row.bin(at);
             for (int i = threadIdx.x; i < edge; i += THREADS) own += sh.mass[i];
             if (edge < kBins) {
-                for (int t = wave; t < tiles; t += kWaves) {
-                    float x[8];
-                    row.load(t * kTile + lane * 8, x);
+                row.walk(wave, tiles, kWaves, [&](int, const float (&x)[8]) {
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
-                        if (x[i] >= least && row.bin(x[i]) == edge) own += Row<T>::whole(row.weight(x[i]));
-                }
+                        if (x[i] >= at && row.bin(x[i]) == edge) own += Row<T>::whole(row.weight(x[i]));
+                });
             }
             block_exclusive_scan<THREADS, uint64_t>(own, sh.scan, total);
-            least = fmaxf(least, limit<THREADS, true>(row, sh, f.top_p * static_cast<double>(total)));
+            at = fmaxf(at, limit<THREADS, true>(row, sh, f.top_p * static_cast<double>(total)));
         }
+        return at;
     }
-    // the kept weights of every tile, in the histogram's place: a wave first gathers its tile's
-    // kept scores, often few, so that their exponentials fill its lanes
-    __syncthreads();
-    auto kept = [&](float x) {
+    __device__ __forceinline__ double kept(float x, float least) const {
         if (x == -INFINITY || x < least) return 0.0;
         const double w = row.weight(x);
         return w >= f.min_p ? w : 0.0;
-    };
-    for (int t = wave; t < tiles; t += kWaves) {
-        float x[8];
-        row.load(t * kTile + lane * 8, x);
-        uint64_t sum = 0;
-        int count = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const bool in = x[i] != -INFINITY && x[i] >= least;
-            const uint64_t mask = __ballot(in);
-            if (in) sh.gathered[wave][count + __popcll(mask & lanemask_lt())] = x[i];
-            count += __popcll(mask);
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        for (int i = lane; i < count; i += kWave) sum += Row<T>::whole(kept(sh.gathered[wave][i]));
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll
-        for (int off = kWave / 2; off > 0; off >>= 1) sum += __shfl_xor(sum, off, kWave);
-        if (lane == 0) sh.mass[t] = sum;
     }
-    __syncthreads();
-    uint64_t own = 0, total;
-    for (int t = threadIdx.x; t < tiles; t += THREADS) own += sh.mass[t];
-    block_exclusive_scan<THREADS, uint64_t>(own, sh.scan, total);
-    if (f.probabilities) {
+    // The kept weight of tiles first .. last - 1, to `sums`: a wave first gathers its tile's kept
+    // scores, often few, so that their exponentials fill its lanes.
+    __device__ __forceinline__ void tile_sums(int first, int last, float least, uint64_t* sums) {
+        row.walk(first + wave, last, kWaves, [&](int t, const float (&x)[8]) {
+            uint64_t sum = 0;
+            int count = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const bool in = x[i] != -INFINITY && x[i] >= least;
+                const uint64_t mask = __ballot(in);
+                if (in) sh.gathered[wave][count + __popcll(mask & lanemask_lt())] = x[i];
+                count += __popcll(mask);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            for (int i = lane; i < count; i += kWave) sum += Row<T>::whole(kept(sh.gathered[wave][i], least));
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+            for (int off = kWave / 2; off > 0; off >>= 1) sum += __shfl_xor(sum, off, kWave);
+            if (lane == 0) sums[t] = sum;
+        });
+    }
+    __device__ __forceinline__ uint64_t whole_sum(const uint64_t* sums) {
+        uint64_t own = 0, total;
+        for (int t = threadIdx.x; t < tiles; t += THREADS) own += sums[t];
+        block_exclusive_scan<THREADS, uint64_t>(own, sh.scan, total);
+        return total;
+    }
+    __device__ __forceinline__ void distribution(int first, int last, float least, uint64_t total) {
         const double share = total ? 17592186044416.0 / static_cast<double>(total) : 0.0;
         float* out = f.probabilities + r * f.vocab;
-        for (int t = wave; t < tiles; t += kWaves) {
-            float x[8];
+        row.walk(first + wave, last, kWaves, [&](int t, const float (&x)[8]) {
             const int j = t * kTile + lane * 8;
-            row.load(j, x);
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                if (j + i < f.vocab) out[j + i] = static_cast<float>(kept(x[i]) * share);
+                if (j + i < f.vocab) out[j + i] = static_cast<float>(kept(x[i], least) * share);
+        });
+    }
+    // The first running sum beyond u of the whole; sums are whole, so beyond it means not below the next double.
+    __device__ __forceinline__ void pick(float least, const uint64_t* sums, uint64_t total) {
+        const float u = f.uniforms[r];
+        const double target = static_cast<double>(u > 0.0f ? fminf(u, 0.999999940395355f) : 0.0f) * static_cast<double>(total);
+        uint64_t before;
+        const int tile = reach<THREADS>(sh, tiles, [&](int i) { return sums[i]; }, nextafter(target, 1e300), 0, before);
+        if (wave) return;
+        float x[8];
+        const int j = tile * kTile + lane * 8;
+        row.load(j, x);
+        uint64_t w[8], sum = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = Row<T>::whole(kept(x[i], least)), sum += w[i];
+        uint64_t incl = sum;
+#pragma unroll
+        for (int off = 1; off < kWave; off <<= 1) {
+            const uint64_t up = __shfl_up(incl, off, kWave);
+            if (lane >= off) incl += up;
         }
-    }
-    // the first running sum beyond u of the whole; sums are whole, so beyond it means not below the next double
-    const float u = f.uniforms[r];
-    const double target = static_cast<double>(u > 0.0f ? fminf(u, 0.999999940395355f) : 0.0f) * static_cast<double>(total);
-    uint64_t before;
-    const int tile = reach<THREADS>(sh, tiles, [&](int i) { return sh.mass[i]; }, nextafter(target, 1e300), 0, before);
-    if (wave) return;
-    float x[8];
-    const int j = tile * kTile + lane * 8;
-    row.load(j, x);
-    uint64_t w[8], sum = 0;
+        uint64_t run = before + incl - sum;
+        int id = -1;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = Row<T>::whole(kept(x[i])), sum += w[i];
-    uint64_t incl = sum;
-#pragma unroll
-    for (int off = 1; off < kWave; off <<= 1) {
-        const uint64_t up = __shfl_up(incl, off, kWave);
-        if (lane >= off) incl += up;
+        for (int i = 0; i < 8; ++i) {
+            run += w[i];
+            if (id < 0 && static_cast<double>(run) > target) id = j + i;
+        }
+        const uint64_t hit = __ballot(id >= 0);
+        const int chosen = hit ? __shfl(id, __ffsll(static_cast<unsigned long long>(hit)) - 1, kWave) : 0;
+        if (lane == 0) f.ids[r] = none ? 0 : chosen;
     }
-    uint64_t run = before + incl - sum;
-    int id = -1;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        run += w[i];
-        if (id < 0 && static_cast<double>(run) > target) id = j + i;
+};
+
+// A row in one workgroup.
+template <int THREADS, typename T>
+__global__ __launch_bounds__(THREADS) void sample_filtered_kernel(Draw f) {
+    __shared__ Shared<THREADS> sh;
+    Phases<THREADS, T> p(f, sh, blockIdx.x);
+    p.begin(p.largest(0, p.tiles));
+    float least = -INFINITY;
+    if (p.by_k || p.by_p) {
+        p.histogram(0, p.tiles);
+        least = p.least();
     }
-    const uint64_t hit = __ballot(id >= 0);
-    const int chosen = hit ? __shfl(id, __ffsll(static_cast<unsigned long long>(hit)) - 1, kWave) : 0;
-    if (lane == 0) f.ids[r] = none ? 0 : chosen;
+    __syncthreads();
+    p.tile_sums(0, p.tiles, least, sh.mass);  // in the histogram's place
+    __syncthreads();
+    const uint64_t total = p.whole_sum(sh.mass);
+    if (f.probabilities) p.distribution(0, p.tiles, least, total);
+    p.pick(least, sh.mass, total);
+}
+
+// A long row in several workgroups, a launch for each phase. `parts` of a row's tiles each.
+struct Parted {
+    Draw f;
+    int parts;
+    float* tops;      // [rows, parts]
+    float* least;     // [rows]
+    uint64_t* total;  // [rows]
+    uint64_t* mass;   // [rows, parts, kBins]
+    uint32_t* count;  // [rows, parts, kBins]
+    uint64_t* sums;   // [rows, tiles]
+};
+constexpr int kPartThreads = 1024;
+
+template <typename T>
+__device__ __forceinline__ void begin_part(Phases<kPartThreads, T>& p, const Parted& d) {
+    float top = -INFINITY;
+    for (int i = 0; i < d.parts; ++i) top = fmaxf(top, d.tops[p.r * d.parts + i]);
+    p.begin(top);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kPartThreads) void sample_top_kernel(Parted d) {
+    __shared__ Shared<kPartThreads> sh;
+    Phases<kPartThreads, T> p(d.f, sh, blockIdx.x / d.parts);
+    const int part = static_cast<int>(blockIdx.x % d.parts);
+    const float top = p.largest(p.tiles * part / d.parts, p.tiles * (part + 1) / d.parts);
+    if (threadIdx.x == 0) d.tops[blockIdx.x] = top;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kPartThreads) void sample_histogram_kernel(Parted d) {
+    __shared__ Shared<kPartThreads> sh;
+    Phases<kPartThreads, T> p(d.f, sh, blockIdx.x / d.parts);
+    const int part = static_cast<int>(blockIdx.x % d.parts);
+    begin_part(p, d);
+    p.histogram(p.tiles * part / d.parts, p.tiles * (part + 1) / d.parts);
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * kBins;
+    for (int i = threadIdx.x; i < kBins; i += kPartThreads) {
+        if (p.by_p) d.mass[at + i] = sh.mass[i];
+        if (p.by_k) d.count[at + i] = sh.count[i];
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(1024) void sample_least_kernel(Parted d) {
+    __shared__ Shared<1024> sh;
+    Phases<1024, T> p(d.f, sh, blockIdx.x);
+    float top = -INFINITY;
+    for (int i = 0; i < d.parts; ++i) top = fmaxf(top, d.tops[p.r * d.parts + i]);
+    p.begin(top);
+    for (int i = threadIdx.x; i < kBins; i += 1024) {
+        uint64_t mass = 0;
+        uint32_t count = 0;
+        for (int part = 0; part < d.parts; ++part) {
+            const int64_t at = (p.r * d.parts + part) * kBins + i;
+            if (p.by_p) mass += d.mass[at];
+            if (p.by_k) count += d.count[at];
+        }
+        sh.mass[i] = mass, sh.count[i] = count;
+    }
+    __syncthreads();
+    const float least = p.least();
+    if (threadIdx.x == 0) d.least[p.r] = least;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kPartThreads) void sample_kept_kernel(Parted d) {
+    __shared__ Shared<kPartThreads> sh;
+    Phases<kPartThreads, T> p(d.f, sh, blockIdx.x / d.parts);
+    const int part = static_cast<int>(blockIdx.x % d.parts);
+    begin_part(p, d);
+    const float least = p.by_k || p.by_p ? d.least[p.r] : -INFINITY;
+    p.tile_sums(p.tiles * part / d.parts, p.tiles * (part + 1) / d.parts, least, d.sums + p.r * p.tiles);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kPartThreads) void sample_pick_kernel(Parted d) {
+    __shared__ Shared<kPartThreads> sh;
+    Phases<kPartThreads, T> p(d.f, sh, blockIdx.x);
+    begin_part(p, d);
+    const float least = p.by_k || p.by_p ? d.least[p.r] : -INFINITY;
+    const uint64_t* sums = d.sums + p.r * p.tiles;
+    const uint64_t total = p.whole_sum(sums);
+    if (threadIdx.x == 0) d.total[p.r] = total;
+    p.pick(least, sums, total);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kPartThreads) void sample_distribution_kernel(Parted d) {
+    __shared__ Shared<kPartThreads> sh;
+    Phases<kPartThreads, T> p(d.f, sh, blockIdx.x / d.parts);
+    const int part = static_cast<int>(blockIdx.x % d.parts);
+    begin_part(p, d);
+    const float least = p.by_k || p.by_p ? d.least[p.r] : -INFINITY;
+    p.distribution(p.tiles * part / d.parts, p.tiles * (part + 1) / d.parts, least, d.total[p.r]);
 }
 
 // Over a wave's 64 lanes, the result in each: neighbours, quads, half rows and rows by
@@ -371,7 +539,7 @@ template <typename T>
 __global__ __launch_bounds__(kWave) void sample_narrow_kernel(Draw f) {
     const int lane = lane_id(), j = lane * 8;
     const int64_t r = blockIdx.x;
-    Row<T> row{static_cast<const T*>(f.logits) + r * f.row_stride, f.vocab, static_cast<int>(f.exclude), f.vector != 0, false, 0.0, f.slope};
+    Row<T> row{static_cast<const T*>(f.logits) + r * f.row_stride, f.vocab, static_cast<int>(f.exclude), f.vector != 0, false, 0.0, f.slope, nullptr};
     const float u = f.uniforms[r];
     float x[8], top = -INFINITY;
     row.load(j, x);
@@ -453,16 +621,64 @@ __global__ __launch_bounds__(kWave) void sample_narrow_kernel(Draw f) {
     if (lane == 0) f.ids[r] = chosen;
 }
 
+// Workgroups of a row in the walks: one, or for at most 128 rows of 65536 scores and more so many
+// that all rows have about 512, none under eight tiles. Five launches instead of one, in us with
+// top-p and min-p, parted against one workgroup a row: 8 x 131072 77 | 119, 128 x 131072 95 | 124,
+// 64 x 65536 59 | 72, 128 x 65536 65 | 71, but 128 x 32768 52 | 46 and 256 x 131072 132 | 130.
+int parts_for(int64_t rows, int64_t vocab) {
+    if (vocab < 65536 || rows > 128) return 1;
+    const int64_t tiles = (vocab + kTile - 1) / kTile;
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({64, tiles / 8, 512 / std::max<int64_t>(rows, 1)})));
+}
+
+size_t align256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
+
+// The parted form's workspace from `base` on; returns its bytes.
+size_t lay_out(Parted& d, char* base, int64_t rows, int64_t vocab) {
+    const size_t tiles = (vocab + kTile - 1) / kTile, cells = static_cast<size_t>(rows) * d.parts;
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        char* p = base + at;
+        at += align256(bytes);
+        return p;
+    };
+    d.total = reinterpret_cast<uint64_t*>(take(rows * 8));
+    d.sums = reinterpret_cast<uint64_t*>(take(rows * tiles * 8));
+    d.mass = reinterpret_cast<uint64_t*>(take(cells * kBins * 8));
+    d.count = reinterpret_cast<uint32_t*>(take(cells * kBins * 4));
+    d.tops = reinterpret_cast<float*>(take(cells * 4));
+    d.least = reinterpret_cast<float*>(take(rows * 4));
+    return at;
+}
+
 template <typename T>
-int draw(const Draw& f, int64_t rows, hipStream_t stream) {
-    // a wave takes 512 scores a step: sixteen waves where a row has more than four such tiles
-    if (f.vocab <= kTile)
-        hipLaunchKernelGGL((sample_narrow_kernel<T>), dim3(static_cast<unsigned>(rows)), dim3(kWave), 0, stream, f);
-    else if (f.vocab <= 2048)
-        hipLaunchKernelGGL((sample_filtered_kernel<256, T>), dim3(static_cast<unsigned>(rows)), dim3(256), 0, stream, f);
-    else
-        hipLaunchKernelGGL((sample_filtered_kernel<1024, T>), dim3(static_cast<unsigned>(rows)), dim3(1024), 0, stream, f);
-    return check_launch("koemi_sample_filtered");
+int draw(const Draw& f, int64_t rows, void* workspace, hipStream_t stream) {
+    const char* what = "koemi_sample_filtered";
+    const unsigned grid = static_cast<unsigned>(rows);
+    Parted d{};
+    d.f = f;
+    d.parts = parts_for(rows, f.vocab);
+    if (d.parts == 1) {
+        // a wave takes 512 scores a step: sixteen waves where a row has more than four such tiles
+        if (f.vocab <= kTile)
+            hipLaunchKernelGGL((sample_narrow_kernel<T>), dim3(grid), dim3(kWave), 0, stream, f);
+        else if (f.vocab <= 2048)
+            hipLaunchKernelGGL((sample_filtered_kernel<256, T>), dim3(grid), dim3(256), 0, stream, f);
+        else
+            hipLaunchKernelGGL((sample_filtered_kernel<1024, T>), dim3(grid), dim3(1024), 0, stream, f);
+        return check_launch(what);
+    }
+    lay_out(d, static_cast<char*>(workspace), rows, f.vocab);
+    const dim3 wide(static_cast<unsigned>(rows * d.parts)), threads(kPartThreads);
+    hipLaunchKernelGGL((sample_top_kernel<T>), wide, threads, 0, stream, d);
+    if ((f.top_k > 0 && f.top_k < f.vocab) || f.top_p < 1.0) {
+        hipLaunchKernelGGL((sample_histogram_kernel<T>), wide, threads, 0, stream, d);
+        hipLaunchKernelGGL((sample_least_kernel<T>), dim3(grid), dim3(1024), 0, stream, d);
+    }
+    hipLaunchKernelGGL((sample_kept_kernel<T>), wide, threads, 0, stream, d);
+    hipLaunchKernelGGL((sample_pick_kernel<T>), dim3(grid), threads, 0, stream, d);
+    if (f.probabilities) hipLaunchKernelGGL((sample_distribution_kernel<T>), wide, threads, 0, stream, d);
+    return check_launch(what);
 }
 
 }  // namespace
@@ -470,9 +686,17 @@ int draw(const Draw& f, int64_t rows, hipStream_t stream) {
 
 using namespace koemi;
 
+extern "C" size_t koemi_sample_filtered_workspace_bytes(int64_t rows, int64_t vocab) {
+    if (rows < 1 || vocab < 1 || vocab > kMaxVocab || rows > 0x7fffffff) return 0;
+    Parted d{};
+    d.parts = parts_for(rows, vocab);
+    return d.parts == 1 ? 0 : lay_out(d, nullptr, rows, vocab);
+}
+
 extern "C" int koemi_sample_filtered(const void* logits, int dtype, int64_t row_stride, int64_t rows, int64_t vocab,
                                      int64_t exclude, double temperature, int64_t top_k, double top_p, double min_p,
-                                     const float* uniforms, int64_t* ids, float* probabilities, koemi_stream_t stream) {
+                                     const float* uniforms, int64_t* ids, float* probabilities, void* workspace,
+                                     size_t workspace_bytes, koemi_stream_t stream) {
     clear_error();
     const char* what = "koemi_sample_filtered";
     if (rows < 0 || vocab < 1) return fail(KOEMI_ERR_INVALID, "%s: rows must not be negative and the vocabulary positive", what);
@@ -492,7 +716,9 @@ extern "C" int koemi_sample_filtered(const void* logits, int dtype, int64_t row_
     f.uniforms = uniforms, f.ids = ids, f.probabilities = probabilities;
     f.slope = kLog2eD / temperature, f.top_p = top_p, f.min_p = min_p, f.top_k = top_k, f.vocab = static_cast<int>(vocab);
     f.vector = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && (rows == 1 || row_stride * size % 16 == 0);
-    if (dtype == KOEMI_F32) return draw<float>(f, rows, as_stream(stream));
-    if (dtype == KOEMI_F16) return draw<f16>(f, rows, as_stream(stream));
-    return draw<bf16>(f, rows, as_stream(stream));
+    const size_t need = koemi_sample_filtered_workspace_bytes(rows, vocab);
+    if (need && (!workspace || workspace_bytes < need)) return fail(KOEMI_ERR_INVALID, "%s: workspace too small", what);
+    if (dtype == KOEMI_F32) return draw<float>(f, rows, workspace, as_stream(stream));
+    if (dtype == KOEMI_F16) return draw<f16>(f, rows, workspace, as_stream(stream));
+    return draw<bf16>(f, rows, workspace, as_stream(stream));
 }

@@ -116,8 +116,9 @@ _SIGNATURES: dict[str, tuple[Any, tuple[Any, ...]]] = {
     ),
     "koemi_sample_filtered": (
         c_int,
-        (_P, c_int, c_int64, c_int64, c_int64, c_int64, c_double, c_int64, c_double, c_double, _P, _P, _P, _P),
+        (_P, c_int, c_int64, c_int64, c_int64, c_int64, c_double, c_int64, c_double, c_double, _P, _P, _P, _P, c_size_t, _P),
     ),
+    "koemi_sample_filtered_workspace_bytes": (c_size_t, (c_int64, c_int64)),
     "koemi_stream_read": (c_int, (_P, c_int64, c_int, c_int, c_int64, _P, _P)),
     "koemi_herm_sample_tokens": (c_int, (_P, c_int64, c_int64, c_int64, c_int64, c_float, c_int64, _P, _P, _P, _P)),
     "koemi_moe_check_assignments": (c_int, (_P, c_int, _P, _P, c_int64, c_int64, c_int64, _P)),

@@ -60,6 +60,7 @@ from torch import Tensor
 from torch.nn import functional
 
 from koemi_amd import _native, linear, memory, moe, recurrent, think
+from koemi_amd.sampling import sample_tokens
 
 __all__ = [
     "DecodeGraph",
@@ -1579,11 +1580,9 @@ class DecodeGraph:
             _greedy_tokens(logits, out=self.ids)
         elif self.policy.top_p is not None or self.policy.min_p is not None:
             policy, last = self.policy, logits[:, -1]
-            vocab = last.shape[1]
-            _native.call("koemi_sample_filtered", _native.ptr(last), _native.dtype_code(last.dtype), logits.stride(0),
-                         last.shape[0], vocab, PAD_TOKEN_ID if vocab > PAD_TOKEN_ID else -1, float(policy.temperature),
-                         int(policy.top_k or 0), 1.0 if policy.top_p is None else float(policy.top_p), float(policy.min_p or 0.0),
-                         _native.ptr(self.uniforms), _native.ptr(self.ids), None, _native.stream_of(logits.device))
+            self.ids.copy_(sample_tokens(last, self.uniforms, temperature=policy.temperature, top_k=policy.top_k,
+                                         top_p=policy.top_p, min_p=policy.min_p,
+                                         exclude=PAD_TOKEN_ID if last.shape[1] > PAD_TOKEN_ID else None))
         else:
             last = logits[:, -1]
             _native.call("koemi_herm_sample_tokens", _native.ptr(last), logits.stride(0), last.shape[0],

@@ -19,6 +19,7 @@ a static buffer before each replay). Nothing is read back to the host.
 from __future__ import annotations
 
 from dataclasses import dataclass
+from functools import lru_cache
 
 import torch
 from torch import Tensor
@@ -31,6 +32,11 @@ PAD_TOKEN_ID = 256  # configuration/settings.py:10-11
 _NARROW = 4096  # columns that koemi_herm_sample_tokens takes
 _MAX_VOCAB = 1 << 19
 _LOGIT_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
+@lru_cache(maxsize=256)
+def _workspace_bytes(rows: int, vocab: int) -> int:
+    return _native.query("koemi_sample_filtered_workspace_bytes", rows, vocab)
 
 
 def _check_share(name: str, value: float | None, zero: bool) -> None:
@@ -82,11 +88,14 @@ def sample_tokens(logits: Tensor, uniforms: Tensor, *, temperature: float = 1.0,
     uniforms = uniforms.contiguous()
     ids = torch.empty((rows, 1), device=z.device, dtype=torch.int64)
     probabilities = torch.empty((rows, vocab), device=z.device, dtype=torch.float32) if with_probabilities else None
+    need = _workspace_bytes(rows, vocab)
+    workspace = torch.empty(need, device=z.device, dtype=torch.uint8) if need else None
     with _native.device_guard(z.device):
         _native.call("koemi_sample_filtered", z.data_ptr(), _native.dtype_code(z.dtype), z.stride(0) if rows > 1 else vocab,
                      rows, vocab, -1 if exclude is None else exclude, float(temperature), min(top_k or 0, 1 << 40),
                      1.0 if top_p is None else float(top_p), 0.0 if min_p is None else float(min_p),
-                     uniforms.data_ptr(), ids.data_ptr(), _native.ptr(probabilities), _native.stream_of(z.device))
+                     uniforms.data_ptr(), ids.data_ptr(), _native.ptr(probabilities), _native.ptr(workspace), need,
+                     _native.stream_of(z.device))
     return (ids, probabilities) if with_probabilities else ids
 
 

@@ -104,6 +104,73 @@ def test_equal_scores_and_odd_values(device, limits):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("limits", LIMITS)
+@pytest.mark.parametrize("vocab, dtype", [(65536, torch.float32), (70001, torch.bfloat16), (1 << 19, torch.float16)])
+def test_long_rows_against_float64(device, vocab, dtype, limits):
+    """Rows in several workgroups. Of 2^19 running sums one lies within 2^-24 of u in a row of sixteen, of
+    top-p's border in as many: of eight rows four are hardly ever left out."""
+
+    gen = torch.Generator(device="cuda").manual_seed(vocab + 1)
+    z = (3.0 * torch.randn(8, vocab, device=device, generator=gen)).to(dtype)
+    check(z, torch.rand(8, device=device, generator=gen), most_skipped=0.5, exclude=vocab - 1, **limits)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("limits", [{}, {"top_k": 7}, {"top_p": 0.6}, {"min_p": 0.5}, {"top_k": 300, "top_p": 0.3}])
+def test_long_rows_of_equal_scores_and_odd_values(device, limits):
+    vocab = 70003
+    z = torch.zeros(8, vocab, device=device)
+    z[1] = (torch.arange(vocab, device=device) % 3).float()
+    z[2, ::2] = -0.0
+    z[3, 17::1000] = float("inf")
+    z[4] = float("-inf")
+    z[4, 70002] = -3.0e38
+    z[5, ::3] = float("nan")
+    z[6] = torch.linspace(-3e38, 3e38, vocab, device=device)
+    z[7] = float("-inf")
+    u = torch.tensor([0.0, 0.4999, 0.75, 0.55, 0.999, 1.0 - 2.0 ** -24, 0.5, 0.3], device=device)
+    check(z, u, **limits)
+    assert int(S.sample_tokens(z, u, **limits)[7]) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("limits", [{}, {"top_p": 0.9, "min_p": 0.01}, {"top_k": 50, "top_p": 0.8, "temperature": 0.7}])
+def test_one_workgroup_a_row_and_several_agree(device, limits):
+    """129 rows take one workgroup each, fewer take several: the same bits, also on another stream."""
+
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    z = (2.0 * torch.randn(129, 66000, device=device, generator=gen)).bfloat16()
+    u = torch.rand(129, device=device, generator=gen)
+    ids, probabilities = S.sample_tokens(z, u, with_probabilities=True, **limits)
+    other = torch.cuda.Stream()
+    other.wait_stream(torch.cuda.current_stream())
+    for rows in (1, 5, 128):
+        with torch.cuda.stream(other):
+            got, p = S.sample_tokens(z[:rows], u[:rows], with_probabilities=True, **limits)
+        other.synchronize()
+        assert torch.equal(got, ids[:rows])
+        assert torch.equal(p, probabilities[:rows])
+
+
+@pytest.mark.gpu
+def test_long_rows_in_a_graph(device):
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    z = torch.randn(4, 65536, device=device, generator=gen)
+    u = torch.rand(4, device=device, generator=gen)
+    S.sample_tokens(z, u, top_k=40, top_p=0.9)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ids = S.sample_tokens(z, u, top_k=40, top_p=0.9)
+    for _ in range(3):
+        z.normal_(generator=gen)
+        u.uniform_(generator=gen)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(S.sample_tokens(z, u, top_k=40, top_p=0.9), ids)
+
+
+@pytest.mark.gpu
 def test_rows_apart_and_no_rows(device):
     gen = torch.Generator(device="cuda").manual_seed(1)
     wide = torch.randn(6, 1003, device=device, generator=gen)
