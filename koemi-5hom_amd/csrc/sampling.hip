@@ -533,8 +533,8 @@ __device__ __forceinline__ V over_wave(V x, Op op) {
 }
 
 // Rows of one tile: a wave holds all scores, and finds the limits bit by bit from how many
-// scores, or what weight, lie at or above a candidate. 2^44 x 512 = 2^53: sums of whole
-// weights are exact in double.
+// scores, or what weight, lie at or above a candidate, until only one score lies between what
+// is known to be kept and what is not. 2^44 x 512 = 2^53: sums of whole weights are exact in double.
 template <typename T>
 __global__ __launch_bounds__(kWave) void sample_narrow_kernel(Draw f) {
     const int lane = lane_id(), j = lane * 8;
@@ -562,15 +562,20 @@ __global__ __launch_bounds__(kWave) void sample_narrow_kernel(Draw f) {
         exact[i] = here ? row.weight(x[i]) : 0.0;
         w[i] = static_cast<double>(Row<T>::whole(exact[i]));
     }
+    const auto at_least = [&](uint32_t candidate) {
+        int count = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) count += __popcll(__ballot(rank[i] >= candidate));
+        return count;
+    };
     uint32_t least = 1;  // of the kept ranks; no score has rank 0
     if (f.top_k > 0 && f.top_k < f.vocab) {
         uint32_t at = 0;
         for (int bit = 31; bit >= 0; --bit) {
             const uint32_t next = at | 1u << bit;
-            int64_t count = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) count += __popcll(__ballot(rank[i] >= next));
+            const int count = at_least(next);
             if (count >= f.top_k) at = next;
+            if (count == f.top_k) break;  // the same scores lie at or above the k-th
         }
         least = max(at, 1u);
     }
@@ -580,12 +585,19 @@ __global__ __launch_bounds__(kWave) void sample_narrow_kernel(Draw f) {
         for (int i = 0; i < 8; ++i) total += rank[i] >= least ? w[i] : 0.0;
         const double target = f.top_p * over_wave(total, add);
         uint32_t at = 0;
+        int above = 0, from = at_least(0);  // scores known to lie above the border, and at or above `at`
         for (int bit = 31; bit >= 0; --bit) {
             const uint32_t next = at | 1u << bit;
-            double sum = 0.0;
+            double part[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum += rank[i] >= next ? w[i] : 0.0;
-            if (!(over_wave(sum, add) < target)) at = next;
+            for (int i = 0; i < 8; ++i) part[i] = rank[i] >= next ? w[i] : 0.0;
+            const double sum = ((part[0] + part[1]) + (part[2] + part[3])) + ((part[4] + part[5]) + (part[6] + part[7]));
+            const int count = at_least(next);
+            if (!(over_wave(sum, add) < target))
+                at = next, from = count;
+            else
+                above = count;
+            if (from == above + 1) break;
         }
         least = max(least, at);
     }
