@@ -227,8 +227,8 @@ __global__ __launch_bounds__(kThreads) void window_join_kernel(Forward f) {
     }
 }
 
-// Parts the keys are cut into where the rows alone leave compute units idle: at most 16
-// tiles' worth of the longest walk each, and no part under four tiles.
+// Parts the keys are cut into where the rows alone leave compute units idle: so many that there are
+// about 512 workgroups, at most 64, and no part under four tiles.
 int splits_of(int64_t workgroups, int64_t tiles) {
     int64_t n = std::min<int64_t>(tiles / 4, 512 / std::max<int64_t>(workgroups, 1));
     return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(n, 64)));

@@ -204,7 +204,7 @@ template <typename T, int NB> constexpr int kShareRows = Tile<T, NB>::kStride > 
 // calls of few keys, and (far) for the sinks against a chunk of the tiles past their window,
 // whose sums go to far_parts.
 template <typename T, int NB, int PLANES, bool SHARE>
-__global__ __launch_bounds__(kThreads, NB <= 2 ? 2 : 1) void window_dkv_kernel(Backward f, int far) {
+__global__ __launch_bounds__(kThreads, NB == 1 || (NB == 2 && !(SHARE && sizeof(T) == 4)) ? 2 : 1) void window_dkv_kernel(Backward f, int far) {
     using L = Tile<T, NB>;
     constexpr int RT = SHARE ? kShareRows<T, NB> : kKeys<T>, RB = RT / 32, RW = (RT + 63) / 64;
     constexpr int kOwn = SHARE ? 32 : kRows;  // keys of the workgroup
