@@ -10,6 +10,12 @@
 // forms s and dp twice (seven products of a pair instead of five). The sinks are seen by every
 // later row: what lies beyond their window is cut into chunks of rows that run beside the
 // others, and the sinks' own workgroups add the chunks' sums in order.
+//
+// Bound by the products, the exponentials and, at heads of 128, by one wave a SIMD (dk, dv, p and
+// ds take 467 registers). bf16, 16 heads on 4, [8, 2048] of 64, window 512: dq 58 us, dk and dv 113, the sinks'
+// far rows 21, their sums 5. 8 heads on 2, [1, 16384] of 128, window 4096: 513, 797, 40, 11 (a large
+// product's rate would take 750 for forward and gradients). fp32, 4 heads on 1, [2, 1500] of 48, window
+// 256: 40 and 80.
 #include "window_attention.hpp"
 
 #include <algorithm>
@@ -202,7 +208,8 @@ template <typename T, int NB> constexpr int kShareRows = Tile<T, NB>::kStride > 
 // false: 128 a workgroup), or all hold the same 32 and take blocks of 32 rows in turn, their
 // sums added in their order: four times the workgroups, each with a quarter of the work, for
 // calls of few keys, and (far) for the sinks against a chunk of the tiles past their window,
-// whose sums go to far_parts.
+// whose sums go to far_parts. fp32 heads of 33 to 64 that share: with all registers of a SIMD to a wave
+// 80 us at [2, 1500], with half of them and 153 spilled 108.
 template <typename T, int NB, int PLANES, bool SHARE>
 __global__ __launch_bounds__(kThreads, NB == 1 || (NB == 2 && !(SHARE && sizeof(T) == 4)) ? 2 : 1) void window_dkv_kernel(Backward f, int far) {
     using L = Tile<T, NB>;
