@@ -15,7 +15,7 @@
 // u falls into. A row stays in its XCD's L2 between the walks. Few long rows are walked by
 // several workgroups each, one launch a phase; a row of one tile stays in a wave's registers.
 // Bound by the two passes of exponentials: 128 rows of 131072 bf16 scores with top-p and min-p
-// take 7 us for the maximum, 26 the histogram, 38 the limit, 20 the kept weights, 7 the pick;
+// take 7 us for the maximum, 26 the histogram, 9 + 13 + 9 the limit, 20 the kept weights, 6 the pick;
 // one read of the scores takes 7.
 #include "common.hpp"
 
@@ -186,30 +186,39 @@ __device__ __forceinline__ int reach(Shared<THREADS>& sh, int n, Value value, do
     return found;
 }
 
-// The score at which the running sum (of ones, or of weights) over falling scores
-// reaches target.
-template <int THREADS, bool MASS, typename T>
-__device__ float limit(const Row<T>& row, Shared<THREADS>& sh, double target) {
-    constexpr int kWaves = THREADS / kWave;
-    const int wave = static_cast<int>(threadIdx.x) / kWave;
-    uint64_t before;
-    const int bin = reach<THREADS>(sh, kBins, [&](int i) { return MASS ? sh.mass[i] : static_cast<uint64_t>(sh.count[i]); },
-                                   target, 0, before);
+// take(score) for every score of a step among tiles first .. last - 1.
+template <int THREADS, typename T, typename Take>
+__device__ __forceinline__ void of_step(const Row<T>& row, int bin, int first, int last, Take take) {
+    row.walk(first + static_cast<int>(threadIdx.x) / kWave, last, THREADS / kWave, [&](int, const float (&x)[8]) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (x[i] != -INFINITY && row.bin(x[i]) == bin) take(x[i]);
+    });
+}
+
+// The step in which the running sum (of ones, or of weights) over falling scores reaches
+// target, and the sum before it.
+template <int THREADS, bool MASS>
+__device__ __forceinline__ int step_of(Shared<THREADS>& sh, double target, uint64_t& before) {
+    return reach<THREADS>(sh, kBins, [&](int i) { return MASS ? sh.mass[i] : static_cast<uint64_t>(sh.count[i]); }, target, 0, before);
+}
+
+// The ranks of a step's scores among tiles first .. last - 1 into the list, as many as fit; how many there are.
+template <int THREADS, typename T>
+__device__ __forceinline__ int list_step(const Row<T>& row, Shared<THREADS>& sh, int bin, int first, int last) {
     if (threadIdx.x == 0) sh.listed = 0;
     __syncthreads();
-    auto each = [&](auto take) {  // every score of the step
-        row.walk(wave, (row.vocab + kTile - 1) / kTile, kWaves, [&](int, const float (&x)[8]) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (x[i] != -INFINITY && row.bin(x[i]) == bin) take(x[i]);
-        });
-    };
-    each([&](float x) {
+    of_step<THREADS>(row, bin, first, last, [&](float x) {
         const int at = atomicAdd(&sh.listed, 1);
         if (at < kList) sh.list[at] = rank_of(x);
     });
     __syncthreads();
-    const int many = sh.listed;
+    return sh.listed;
+}
+
+// The score of a step at which that sum reaches target; `many` scores, from the list where it holds them all.
+template <int THREADS, bool MASS, typename T>
+__device__ float score_in(const Row<T>& row, Shared<THREADS>& sh, int bin, int many, double target, uint64_t before) {
     __shared__ unsigned long long digits[256];
     uint32_t prefix = 0;
     for (int shift = 24; shift >= 0; shift -= 8) {
@@ -222,7 +231,7 @@ __device__ float limit(const Row<T>& row, Shared<THREADS>& sh, double target) {
         if (many <= kList) {
             for (int i = threadIdx.x; i < many; i += THREADS) add(sh.list[i]);
         } else {
-            each([&](float x) { add(rank_of(x)); });
+            of_step<THREADS>(row, bin, 0, (row.vocab + kTile - 1) / kTile, [&](float x) { add(rank_of(x)); });
         }
         __syncthreads();
         const int digit = reach<THREADS>(sh, 256, [&](int i) { return static_cast<uint64_t>(digits[i]); }, target, before, before);
@@ -283,29 +292,45 @@ struct Phases {
         });
         __syncthreads();
     }
+    // Scores counted in the whole row's histogram.
+    __device__ __forceinline__ uint64_t available() {
+        uint64_t own = 0, all;
+        for (int i = threadIdx.x; i < kBins; i += THREADS) own += sh.count[i];
+        block_exclusive_scan<THREADS, uint64_t>(own, sh.scan, all);
+        return all;
+    }
+    // The weight of all scores from the limit `at` up, which lies in step `edge` (kBins: no limit); `many`
+    // of that step are listed.
+    __device__ __forceinline__ uint64_t mass_from(float at, int edge, int many) {
+        uint64_t own = 0, total;
+        for (int i = threadIdx.x; i < edge; i += THREADS) own += sh.mass[i];
+        auto add = [&](float x) {
+            if (x >= at) own += Row<T>::whole(row.weight(x));
+        };
+        if (edge < kBins && many <= kList) {
+            for (int i = threadIdx.x; i < many; i += THREADS) add(score_of(sh.list[i]));
+        } else if (edge < kBins) {
+            of_step<THREADS>(row, edge, 0, tiles, add);
+        }
+        block_exclusive_scan<THREADS, uint64_t>(own, sh.scan, total);
+        return total;
+    }
     // The least kept score by top-k and top-p, from the whole row's histogram.
     __device__ __forceinline__ float least() {
         float at = -INFINITY;
-        if (by_k) {
-            uint64_t own = 0, available;
-            for (int i = threadIdx.x; i < kBins; i += THREADS) own += sh.count[i];
-            block_exclusive_scan<THREADS, uint64_t>(own, sh.scan, available);
-            if (static_cast<uint64_t>(f.top_k) < available) at = limit<THREADS, false>(row, sh, static_cast<double>(f.top_k));
+        int edge = kBins, many = 0;
+        uint64_t before;
+        if (by_k && static_cast<uint64_t>(f.top_k) < available()) {
+            const double target = static_cast<double>(f.top_k);
+            edge = step_of<THREADS, false>(sh, target, before);
+            many = list_step<THREADS>(row, sh, edge, 0, tiles);
+            at = score_in<THREADS, false>(row, sh, edge, many, target, before);
         }
         if (by_p) {
-            // the sum that p is of: of what top-k leaves
-            uint64_t own = 0, total;
-            const int edge = at == -INFINITY ? kBins : row.bin(at);
-            for (int i = threadIdx.x; i < edge; i += THREADS) own += sh.mass[i];
-            if (edge < kBins) {
-                row.walk(wave, tiles, kWaves, [&](int, const float (&x)[8]) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (x[i] >= at && row.bin(x[i]) == edge) own += Row<T>::whole(row.weight(x[i]));
-                });
-            }
-            block_exclusive_scan<THREADS, uint64_t>(own, sh.scan, total);
-            at = fmaxf(at, limit<THREADS, true>(row, sh, f.top_p * static_cast<double>(total)));
+            const double target = f.top_p * static_cast<double>(mass_from(at, edge, many));
+            const int step = step_of<THREADS, true>(sh, target, before);
+            if (step != edge) many = list_step<THREADS>(row, sh, step, 0, tiles);
+            at = fmaxf(at, score_in<THREADS, true>(row, sh, step, many, target, before));
         }
         return at;
     }
@@ -402,21 +427,32 @@ __global__ __launch_bounds__(THREADS) void sample_filtered_kernel(Draw f) {
     p.pick(least, sh.mass, total);
 }
 
+// The limit that a row looks for: the running sum (of weights, or of ones) that reaches target in step
+// `bin` (-1: none), of which `listed` scores were found.
+struct Limit {
+    double target;
+    uint64_t before;
+    int bin, listed, mass;
+};
+
 // A long row in several workgroups, a launch for each phase. `parts` of a row's tiles each.
 struct Parted {
     Draw f;
     int parts;
     float* tops;      // [rows, parts]
-    float* least;     // [rows]
+    float* least;     // [rows]: of the limits found so far
+    Limit* limits;    // [rows]
+    uint32_t* list;   // [rows, kList]: ranks of a step's scores
     uint64_t* total;  // [rows]
     uint64_t* mass;   // [rows, parts, kBins]
     uint32_t* count;  // [rows, parts, kBins]
     uint64_t* sums;   // [rows, tiles]
 };
-constexpr int kPartThreads = 1024;
+constexpr int kPartThreads = 1024;  // of a part; a row's own steps are chains of barriers, cheaper among four waves
+constexpr int kRowThreads = 256;
 
-template <typename T>
-__device__ __forceinline__ void begin_part(Phases<kPartThreads, T>& p, const Parted& d) {
+template <int THREADS, typename T>
+__device__ __forceinline__ void begin_part(Phases<THREADS, T>& p, const Parted& d) {
     float top = -INFINITY;
     for (int i = 0; i < d.parts; ++i) top = fmaxf(top, d.tops[p.r * d.parts + i]);
     p.begin(top);
@@ -445,26 +481,80 @@ __global__ __launch_bounds__(kPartThreads) void sample_histogram_kernel(Parted d
     }
 }
 
+// The parts' histograms added into the first one's, and the step of the first limit.
 template <typename T>
-__global__ __launch_bounds__(1024) void sample_least_kernel(Parted d) {
-    __shared__ Shared<1024> sh;
-    Phases<1024, T> p(d.f, sh, blockIdx.x);
-    float top = -INFINITY;
-    for (int i = 0; i < d.parts; ++i) top = fmaxf(top, d.tops[p.r * d.parts + i]);
-    p.begin(top);
-    for (int i = threadIdx.x; i < kBins; i += 1024) {
+__global__ __launch_bounds__(kPartThreads) void sample_step_kernel(Parted d) {
+    __shared__ Shared<kPartThreads> sh;
+    Phases<kPartThreads, T> p(d.f, sh, blockIdx.x);
+    begin_part(p, d);
+    for (int i = threadIdx.x; i < kBins; i += kPartThreads) {
+        const int64_t first = p.r * d.parts * kBins + i;
         uint64_t mass = 0;
         uint32_t count = 0;
+#pragma unroll 4
         for (int part = 0; part < d.parts; ++part) {
-            const int64_t at = (p.r * d.parts + part) * kBins + i;
-            if (p.by_p) mass += d.mass[at];
-            if (p.by_k) count += d.count[at];
+            if (p.by_p) mass += d.mass[first + static_cast<int64_t>(part) * kBins];
+            if (p.by_k) count += d.count[first + static_cast<int64_t>(part) * kBins];
         }
         sh.mass[i] = mass, sh.count[i] = count;
+        if (p.by_p) d.mass[first] = mass;
     }
     __syncthreads();
-    const float least = p.least();
-    if (threadIdx.x == 0) d.least[p.r] = least;
+    Limit limit{0.0, 0, -1, 0, 0};
+    if (p.by_k && static_cast<uint64_t>(d.f.top_k) < p.available()) {
+        limit.target = static_cast<double>(d.f.top_k);
+        limit.bin = step_of<kPartThreads, false>(sh, limit.target, limit.before);
+    } else if (p.by_p) {
+        limit.mass = 1;
+        limit.target = d.f.top_p * static_cast<double>(p.mass_from(-INFINITY, kBins, 0));
+        limit.bin = step_of<kPartThreads, true>(sh, limit.target, limit.before);
+    }
+    if (threadIdx.x == 0) d.limits[p.r] = limit, d.least[p.r] = -INFINITY;
+}
+
+// That step's scores, in any order: what is summed of them is whole.
+template <typename T>
+__global__ __launch_bounds__(kPartThreads) void sample_list_kernel(Parted d) {
+    __shared__ Shared<kPartThreads> sh;
+    __shared__ int base;
+    Phases<kPartThreads, T> p(d.f, sh, blockIdx.x / d.parts);
+    const int part = static_cast<int>(blockIdx.x % d.parts);
+    Limit& limit = d.limits[p.r];
+    if (limit.bin < 0) return;
+    begin_part(p, d);
+    const int many = list_step<kPartThreads>(p.row, sh, limit.bin, p.tiles * part / d.parts, p.tiles * (part + 1) / d.parts);
+    if (threadIdx.x == 0) base = many ? atomicAdd(&limit.listed, many) : 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < min(many, kList) && base + i < kList; i += kPartThreads) d.list[p.r * kList + base + i] = sh.list[i];
+}
+
+// The limit among them; after top-k's, top-p's or the step of it, if that is another one.
+template <typename T>
+__global__ __launch_bounds__(kRowThreads) void sample_limit_kernel(Parted d) {
+    __shared__ Shared<kRowThreads> sh;
+    Phases<kRowThreads, T> p(d.f, sh, blockIdx.x);
+    Limit limit = d.limits[p.r];
+    if (limit.bin < 0) return;
+    begin_part(p, d);
+    const int many = limit.listed;
+    if (many <= kList)
+        for (int i = threadIdx.x; i < many; i += kRowThreads) sh.list[i] = d.list[p.r * kList + i];
+    const bool then = !limit.mass && p.by_p;
+    if (then)
+        for (int i = threadIdx.x; i < kBins; i += kRowThreads) sh.mass[i] = d.mass[p.r * d.parts * kBins + i];
+    __syncthreads();
+    float at = limit.mass ? score_in<kRowThreads, true>(p.row, sh, limit.bin, many, limit.target, limit.before)
+                          : score_in<kRowThreads, false>(p.row, sh, limit.bin, many, limit.target, limit.before);
+    Limit next{0.0, 0, -1, 0, 1};
+    if (then) {
+        next.target = d.f.top_p * static_cast<double>(p.mass_from(at, limit.bin, many));
+        next.bin = step_of<kRowThreads, true>(sh, next.target, next.before);
+        if (next.bin == limit.bin) {
+            at = fmaxf(at, score_in<kRowThreads, true>(p.row, sh, next.bin, many, next.target, next.before));
+            next.bin = -1;
+        }
+    }
+    if (threadIdx.x == 0) d.limits[p.r] = next, d.least[p.r] = fmaxf(d.least[p.r], at);
 }
 
 template <typename T>
@@ -478,9 +568,9 @@ __global__ __launch_bounds__(kPartThreads) void sample_kept_kernel(Parted d) {
 }
 
 template <typename T>
-__global__ __launch_bounds__(kPartThreads) void sample_pick_kernel(Parted d) {
-    __shared__ Shared<kPartThreads> sh;
-    Phases<kPartThreads, T> p(d.f, sh, blockIdx.x);
+__global__ __launch_bounds__(kRowThreads) void sample_pick_kernel(Parted d) {
+    __shared__ Shared<kRowThreads> sh;
+    Phases<kRowThreads, T> p(d.f, sh, blockIdx.x);
     begin_part(p, d);
     const float least = p.by_k || p.by_p ? d.least[p.r] : -INFINITY;
     const uint64_t* sums = d.sums + p.r * p.tiles;
@@ -634,9 +724,9 @@ __global__ __launch_bounds__(kWave) void sample_narrow_kernel(Draw f) {
 }
 
 // Workgroups of a row in the walks: one, or for at most 128 rows of 65536 scores and more so many
-// that all rows have about 512, none under eight tiles. Five launches instead of one, in us with
-// top-p and min-p, parted against one workgroup a row: 8 x 131072 77 | 119, 128 x 131072 95 | 124,
-// 64 x 65536 59 | 72, 128 x 65536 65 | 71, but 128 x 32768 52 | 46 and 256 x 131072 132 | 130.
+// that all rows have about 512, none under eight tiles. Seven launches instead of one, in us with
+// top-p and min-p, parted against one workgroup a row: 8 x 131072 67 | 119, 128 x 131072 87 | 124,
+// 64 x 65536 56 | 72, 128 x 65536 62 | 71, but 8 x 32768 42 | 45, 128 x 32768 52 | 46 and 256 x 131072 131 | 130.
 int parts_for(int64_t rows, int64_t vocab) {
     if (vocab < 65536 || rows > 128) return 1;
     const int64_t tiles = (vocab + kTile - 1) / kTile;
@@ -660,6 +750,8 @@ size_t lay_out(Parted& d, char* base, int64_t rows, int64_t vocab) {
     d.count = reinterpret_cast<uint32_t*>(take(cells * kBins * 4));
     d.tops = reinterpret_cast<float*>(take(cells * 4));
     d.least = reinterpret_cast<float*>(take(rows * 4));
+    d.limits = reinterpret_cast<Limit*>(take(rows * sizeof(Limit)));
+    d.list = reinterpret_cast<uint32_t*>(take(rows * kList * 4));
     return at;
 }
 
@@ -683,12 +775,17 @@ int draw(const Draw& f, int64_t rows, void* workspace, hipStream_t stream) {
     lay_out(d, static_cast<char*>(workspace), rows, f.vocab);
     const dim3 wide(static_cast<unsigned>(rows * d.parts)), threads(kPartThreads);
     hipLaunchKernelGGL((sample_top_kernel<T>), wide, threads, 0, stream, d);
-    if ((f.top_k > 0 && f.top_k < f.vocab) || f.top_p < 1.0) {
+    const int limits = (f.top_k > 0 && f.top_k < f.vocab) + (f.top_p < 1.0);
+    if (limits) {
         hipLaunchKernelGGL((sample_histogram_kernel<T>), wide, threads, 0, stream, d);
-        hipLaunchKernelGGL((sample_least_kernel<T>), dim3(grid), dim3(1024), 0, stream, d);
+        hipLaunchKernelGGL((sample_step_kernel<T>), dim3(grid), threads, 0, stream, d);
+    }
+    for (int i = 0; i < limits; ++i) {
+        hipLaunchKernelGGL((sample_list_kernel<T>), wide, threads, 0, stream, d);
+        hipLaunchKernelGGL((sample_limit_kernel<T>), dim3(grid), dim3(kRowThreads), 0, stream, d);
     }
     hipLaunchKernelGGL((sample_kept_kernel<T>), wide, threads, 0, stream, d);
-    hipLaunchKernelGGL((sample_pick_kernel<T>), dim3(grid), threads, 0, stream, d);
+    hipLaunchKernelGGL((sample_pick_kernel<T>), dim3(grid), dim3(kRowThreads), 0, stream, d);
     if (f.probabilities) hipLaunchKernelGGL((sample_distribution_kernel<T>), wide, threads, 0, stream, d);
     return check_launch(what);
 }
