@@ -18,6 +18,7 @@
 
 #include "common.hpp"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace koemi {
@@ -336,9 +337,15 @@ struct KeyTiles {
 // Probabilities and their derivatives enter their products rounded to the inputs' type,
 // which about doubles a 16-bit result's squared error against rounding it alone (1.41 times the
 // error). Calls of few rows, whose time is launches and not products, take them in two
-// planes instead: [5, 777], 6 heads of 80, fp16: 0.00030 -> 0.00021 from float64.
+// planes instead: [5, 777], 6 heads of 80, fp16: 0.00030 -> 0.00021 from float64. So do rows that
+// see few keys: there the output's error, which the scores' gradients take in through D, is
+// no average of many roundings (1.5 to 1.8 times the error with 2 to 27 keys), and tiles are few; and
+// heads of fewer than 32 columns (1.5 times at 9 to 12, whatever the keys). [8, 2048], 16 heads on 4,
+// with gradients: 211 us against 190 in one plane at 64 columns and a window of 60, 425 against 402 at 128.
+constexpr int kFewKeys = 64, kFewColumns = 32;
 inline bool two_planes(const Shape& s, int size) {
-    return size == 2 && static_cast<int64_t>(s.batch) * s.groups * s.shared * s.length < (1 << 16);
+    return size == 2 && (s.width < kFewColumns || static_cast<int64_t>(s.batch) * s.groups * s.shared * s.length < (1 << 16) ||
+                         std::min<int64_t>(s.total, static_cast<int64_t>(s.window) + s.sinks) <= kFewKeys);
 }
 
 // Checks, and the shape as the kernels take it (window_attention.hip).

@@ -473,3 +473,35 @@ def test_long_rows(device, dtype):
 
     args = make((2, 2300, 16, 4, 64), dtype, 2, "tail")
     check(*args, 700, 5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("width, mask", [(32, "tail"), (64, "random"), (96, None), (128, "tail"), (160, None), (256, "random")])
+def test_many_rows_that_see_many_keys(device, width, mask, dtype):
+    """More keys than those that keep two planes of probabilities."""
+
+    args = make((160, 130, 4, 1, width), dtype, width + 1, mask)
+    check(*args, 100, 3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("window, sinks", [(1, 1), (3, 1), (2, 4), (21, 6)])
+def test_few_visible_keys_keep_the_types_precision(device, window, sinks, dtype):
+    """Many rows of few keys are off by their own rounding and little more.
+
+    A rounding's error is spread over H = half a step of 1 either way for values from 1 to 2, so a
+    result's error is at most H / sqrt(3) of its norm over many elements, were all at their
+    binade's start; at 2^-16 of a row's largest size, two planes add less than 1% of H. One
+    plane adds an error of about the same size again, and more through D.
+    """
+
+    q, k, v, _, d_out = make((64, 128, 16, 4, 32), dtype, 3, None)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    out = W.window_attention(*leaves, window=window, sinks=sinks)
+    grads = torch.autograd.grad(out, leaves, d_out)
+    want, _ = reference(q, k, v, None, window, sinks, 1.0 / math.sqrt(32), d_out)
+    for name, got, w in zip(("out", "d_queries", "d_keys", "d_values"), (out, *grads), want):
+        off = ((got.detach().double() - w).norm() / w.norm()).item()
+        assert off <= HALF_STEP[dtype] * (1 / math.sqrt(3) + 0.01), (name, off)
