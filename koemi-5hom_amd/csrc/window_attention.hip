@@ -33,7 +33,7 @@ struct Forward {
     int row_tiles, splits;
 };
 
-template <typename T, int NB, int PLANES>
+template <typename T, int NB>
 __global__ __launch_bounds__(kThreads, NB == 1 ? 4 : NB == 2 ? 3 : NB <= 4 ? 2 : 1) void window_forward_kernel(Forward f) {
     using L = Tile<T, NB>;
     constexpr int KT = kKeys<T>, KB = KT / 32;
@@ -154,7 +154,7 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 4 : NB == 2 ? 3 : NB <= 4 ? 2 :
 #pragma unroll
                 for (int kb = 0; kb < KB; ++kb) {
                     terms(kb);
-                    mma_acc<T, NB, PLANES>(acc, v_tile, kb * 32, s[kb]);
+                    mma_acc<T, NB>(acc, v_tile, kb * 32, s[kb]);
                 }
             }
         }
@@ -250,10 +250,7 @@ int splits_for(int64_t batch, int64_t length, int64_t total, int64_t heads, int6
 template <typename T, int NB>
 int run(const Forward& f, hipStream_t stream) {
     const int64_t grid = workgroups_of(f.s.batch, f.s.groups, static_cast<int64_t>(f.s.length) * f.s.shared) * f.splits;
-    if (sizeof(T) == 2 && two_planes(f.s, sizeof(T)))
-        hipLaunchKernelGGL((window_forward_kernel<T, NB, sizeof(T) == 2 ? 2 : 1>), dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, stream, f);
-    else
-        hipLaunchKernelGGL((window_forward_kernel<T, NB, 1>), dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, stream, f);
+    hipLaunchKernelGGL((window_forward_kernel<T, NB>), dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, stream, f);
     int rc = check_launch("koemi_window_attention_forward");
     if (rc != KOEMI_OK || f.splits == 1) return rc;
     const int64_t cells = static_cast<int64_t>(f.s.length) * f.s.shared * f.s.batch * f.s.groups;

@@ -191,8 +191,10 @@ __device__ __forceinline__ void mma_rows(f32x16& acc, const char* tile, int firs
 }
 
 // acc[n][32 n + ...][column] += sum over the tile's rows first .. first + 31 of row[32 n + ...] coef[row][column],
-// coef rounded to T, or (PLANES 2) as two values of T that sum to it within 2^-17 or 2^-22.
-template <typename T, int NB, int PLANES>
+// coef (a probability, or its derivative) of 16-bit calls as two values of T that sum to it within 2^-17 or
+// 2^-22. Rounded to T alone it would add an error as large as the result's own rounding (1.41 times the error; 1.5
+// to 1.8 times where few keys are seen, whose output D takes in), whatever the call's size.
+template <typename T, int NB>
 __device__ __forceinline__ void mma_acc(f32x16 (&acc)[NB], const char* tile, int first, const f32x16& coef) {
     using L = Tile<T, NB>;
     const int lane = lane_id(), half = lane >> 5;
@@ -218,7 +220,7 @@ __device__ __forceinline__ void mma_acc(f32x16 (&acc)[NB], const char* tile, int
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 e[i] = static_cast<T>(coef[8 * s + i]);
-                if (PLANES == 2) low[i] = static_cast<T>(coef[8 * s + i] - to_f32(e[i]));
+                low[i] = static_cast<T>(coef[8 * s + i] - to_f32(e[i]));
             }
             const uint4 b = *reinterpret_cast<const uint4*>(e);
             const char* base[2];
@@ -239,7 +241,7 @@ __device__ __forceinline__ void mma_acc(f32x16 (&acc)[NB], const char* tile, int
                 for (int i = 0; i < 2; ++i)
                     a.part[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(base[i] + (turned[i] ^ (n << 6))));
                 acc[n] = mfma16<T>(a.whole, b, acc[n]);
-                if (PLANES == 2) acc[n] = mfma16<T>(a.whole, *reinterpret_cast<const uint4*>(low), acc[n]);
+                acc[n] = mfma16<T>(a.whole, *reinterpret_cast<const uint4*>(low), acc[n]);
             }
         }
     }
@@ -333,20 +335,6 @@ struct KeyTiles {
     }
     __device__ __forceinline__ int operator[](int t) const { return t < lead ? t : t + skip; }
 };
-
-// Probabilities and their derivatives enter their products rounded to the inputs' type,
-// which about doubles a 16-bit result's squared error against rounding it alone (1.41 times the
-// error). Calls of few rows, whose time is launches and not products, take them in two
-// planes instead: [5, 777], 6 heads of 80, fp16: 0.00030 -> 0.00021 from float64. So do rows that
-// see few keys: there the output's error, which the scores' gradients take in through D, is
-// no average of many roundings (1.5 to 1.8 times the error with 2 to 27 keys), and tiles are few; and
-// heads of fewer than 32 columns (1.5 times at 9 to 12, whatever the keys). [8, 2048], 16 heads on 4,
-// with gradients: 211 us against 190 in one plane at 64 columns and a window of 60, 425 against 402 at 128.
-constexpr int kFewKeys = 64, kFewColumns = 32;
-inline bool two_planes(const Shape& s, int size) {
-    return size == 2 && (s.width < kFewColumns || static_cast<int64_t>(s.batch) * s.groups * s.shared * s.length < (1 << 16) ||
-                         std::min<int64_t>(s.total, static_cast<int64_t>(s.window) + s.sinks) <= kFewKeys);
-}
 
 // Checks, and the shape as the kernels take it (window_attention.hip).
 int shape_of(const char* what, const void* queries, const void* keys, const void* values, const uint8_t* valid,

@@ -74,7 +74,7 @@ struct Range {
     }
 };
 
-template <typename T, int NB, int PLANES>
+template <typename T, int NB>
 __global__ __launch_bounds__(kThreads, NB == 1 ? 4 : NB == 2 && sizeof(T) == 2 ? 3 : NB <= 4 ? 2 : 1) void window_dq_kernel(Backward f) {
     using L = Tile<T, NB>;
     constexpr int KT = kKeys<T>, KB = KT / 32;
@@ -180,7 +180,7 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 4 : NB == 2 && sizeof(T) == 2 ?
                 if (masked && bad_tile == t)
                     seen_acc<T, NB>(acc, k_tile, kb * 32, d, block, scratch[wave]);
                 else
-                    mma_acc<T, NB, PLANES>(acc, k_tile, kb * 32, d);
+                    mma_acc<T, NB>(acc, k_tile, kb * 32, d);
             }
         }
     }
@@ -210,7 +210,7 @@ template <typename T, int NB> constexpr int kShareRows = Tile<T, NB>::kStride > 
 // calls of few keys, and (far) for the sinks against a chunk of the tiles past their window,
 // whose sums go to far_parts. fp32 heads of 33 to 64 that share: with all registers of a SIMD to a wave
 // 80 us at [2, 1500], with half of them and 153 spilled 108.
-template <typename T, int NB, int PLANES, bool SHARE>
+template <typename T, int NB, bool SHARE>
 __global__ __launch_bounds__(kThreads, NB == 1 || (NB == 2 && !(SHARE && sizeof(T) == 4)) ? 2 : 1) void window_dkv_kernel(Backward f, int far) {
     using L = Tile<T, NB>;
     constexpr int RT = SHARE ? kShareRows<T, NB> : kKeys<T>, RB = RT / 32, RW = (RT + 63) / 64;
@@ -357,8 +357,8 @@ __global__ __launch_bounds__(kThreads, NB == 1 || (NB == 2 && !(SHARE && sizeof(
                 seen_acc<T, NB>(dv, g_tile, rb * 32, s, seen, scratch[wave]);
                 seen_acc<T, NB>(dk, q_tile, rb * 32, d, seen & ~block_alone, scratch[wave]);
             } else {
-                mma_acc<T, NB, PLANES>(dv, g_tile, rb * 32, s);
-                mma_acc<T, NB, PLANES>(dk, q_tile, rb * 32, d);
+                mma_acc<T, NB>(dv, g_tile, rb * 32, s);
+                mma_acc<T, NB>(dk, q_tile, rb * 32, d);
             }
         };
         if (SHARE) {
@@ -375,8 +375,8 @@ __global__ __launch_bounds__(kThreads, NB == 1 || (NB == 2 && !(SHARE && sizeof(
             for (int rb = 0; rb < RB; ++rb) {
                 terms(rb, s[rb], d[rb]);
                 range.fit(d[rb], dk);
-                mma_acc<T, NB, PLANES>(dv, g_tile, rb * 32, s[rb]);
-                mma_acc<T, NB, PLANES>(dk, q_tile, rb * 32, d[rb]);
+                mma_acc<T, NB>(dv, g_tile, rb * 32, s[rb]);
+                mma_acc<T, NB>(dk, q_tile, rb * 32, d[rb]);
             }
         } else if (NB <= 2) {
 #pragma unroll 1
@@ -474,18 +474,18 @@ int64_t far_each(const Shape& s, const Backward& f) {
 size_t far_values(const Shape& s, const Backward& f) { return static_cast<size_t>(f.far_chunks) * far_each(s, f); }
 
 
-template <typename T, int NB, int PLANES>
-int run_planes(const Backward& f, hipStream_t stream) {
+template <typename T, int NB>
+int run(const Backward& f, hipStream_t stream) {
     const int64_t heads = static_cast<int64_t>(f.s.batch) * f.s.groups;
     const char* what = "koemi_window_attention_backward";
     int rc = KOEMI_OK;
     if (f.row_tiles) {
-        hipLaunchKernelGGL((window_dq_kernel<T, NB, PLANES>), dim3(static_cast<unsigned>(heads * f.row_tiles)), dim3(kThreads), 0, stream, f);
+        hipLaunchKernelGGL((window_dq_kernel<T, NB>), dim3(static_cast<unsigned>(heads * f.row_tiles)), dim3(kThreads), 0, stream, f);
         rc = check_launch(what);
     }
     if (rc != KOEMI_OK || (!f.dk && !f.dv)) return rc;
     if (f.far_chunks) {
-        hipLaunchKernelGGL((window_dkv_kernel<T, NB, PLANES, true>), dim3(static_cast<unsigned>(heads * f.far_tiles * f.far_chunks)),
+        hipLaunchKernelGGL((window_dkv_kernel<T, NB, true>), dim3(static_cast<unsigned>(heads * f.far_tiles * f.far_chunks)),
                            dim3(kThreads), 0, stream, f, 1);
         rc = check_launch(what);
         if (rc != KOEMI_OK) return rc;
@@ -500,17 +500,11 @@ int run_planes(const Backward& f, hipStream_t stream) {
     // and spread it where the wide ones leave compute units idle (70 of them at [5, 777]: 31.6 us against 45.7).
     const int64_t wide = heads * ((f.s.total + kRows - 1) / kRows);
     if (wide < 160)
-        hipLaunchKernelGGL((window_dkv_kernel<T, NB, PLANES, true>), dim3(static_cast<unsigned>(heads * ((f.s.total + 31) / 32))),
+        hipLaunchKernelGGL((window_dkv_kernel<T, NB, true>), dim3(static_cast<unsigned>(heads * ((f.s.total + 31) / 32))),
                            dim3(kThreads), 0, stream, f, 0);
     else
-        hipLaunchKernelGGL((window_dkv_kernel<T, NB, PLANES, false>), dim3(static_cast<unsigned>(wide)), dim3(kThreads), 0, stream, f, 0);
+        hipLaunchKernelGGL((window_dkv_kernel<T, NB, false>), dim3(static_cast<unsigned>(wide)), dim3(kThreads), 0, stream, f, 0);
     return check_launch(what);
-}
-
-template <typename T, int NB>
-int run(const Backward& f, hipStream_t stream) {
-    if (sizeof(T) == 2 && two_planes(f.s, sizeof(T))) return run_planes<T, NB, sizeof(T) == 2 ? 2 : 1>(f, stream);
-    return run_planes<T, NB, 1>(f, stream);
 }
 
 template <typename T>

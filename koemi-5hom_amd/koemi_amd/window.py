@@ -72,10 +72,8 @@ def window_attention(queries: Tensor, keys: Tensor, values: Tensor, valid_mask: 
     batches are padded at their end.
 
     Returns ``[B, L, H, D]`` in the inputs' type. Sums and softmax statistics are float32;
-    16-bit calls of 2^16 rows of heads (B L H) and more, heads wider than 24 and more than 64
-    visible keys (window + sinks, T) round the probabilities (and, for the gradients, their
-    derivatives) to the inputs' type between two products, the others keep twice the
-    bits. Sums run in a fixed order.
+    16-bit calls keep the probabilities and, for the gradients, their derivatives to twice the
+    inputs' bits between two products. Sums run in a fixed order.
     """
 
     for name, tensor in (("queries", queries), ("keys", keys), ("values", values)):
