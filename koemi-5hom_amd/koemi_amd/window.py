@@ -146,11 +146,14 @@ def _plan(query: tuple, key: tuple, value: tuple, query_stride: tuple, key_strid
 
 
 def _rows(tensor: Tensor, width: int) -> Tensor:
-    """A copy of ``tensor`` [B, L, H, D] that the kernels can read: contiguous, its width
-    padded with zeros to whole 16-byte pieces, aligned."""
+    """A copy of ``tensor`` [B, L, H, D] that the kernels can read: contiguous whatever the layout (``pad`` and
+    ``clone`` may keep one with other columns inside), its width padded with zeros to whole 16-byte pieces, aligned."""
 
-    short = width - tensor.shape[3]
-    return torch.nn.functional.pad(tensor, (0, short)) if short else tensor.clone(memory_format=torch.contiguous_format)
+    rows = tensor.new_empty((*tensor.shape[:3], width))
+    rows[..., :tensor.shape[3]].copy_(tensor)
+    if width > tensor.shape[3]:
+        rows[..., tensor.shape[3]:].zero_()
+    return rows
 
 
 def _strides(*tensors: Tensor) -> ctypes.Array:

@@ -40,3 +40,70 @@ def test_calls_of_many_rows_and_keys_keep_the_types_precision(device, width, win
         attention.close(got, w, b, name)
         off = ((got.detach().double() - w).norm() / w.norm()).item()
         assert off <= half * (1 / math.sqrt(3) + 0.01), (name, off)
+
+
+def positions_last(t):
+    """The same values in the layout that an operator over positions hands back: neighbours along the positions."""
+
+    return t.permute(0, 2, 3, 1).contiguous().permute(0, 3, 1, 2)
+
+
+def stray_stride(t):
+    """A single position whose stride, which nothing steps by, is odd."""
+
+    t = t.contiguous()
+    return t.as_strided(t.shape, (t.stride(0), 1, t.stride(2), t.stride(3)))
+
+
+@pytest.mark.parametrize("width, padded", [(10, 16), (16, 16), (3, 4)])
+def test_copies_of_rows_are_contiguous(width, padded):
+    t = torch.arange(2 * 7 * 3 * width, dtype=torch.float32).reshape(2, 7, 3, width)
+    for rows in (t, positions_last(t), t.transpose(1, 2), t[:, :1], stray_stride(t[:, :1]), t[:1, :, :1], t[:0]):
+        got = W._rows(rows, padded)
+        shape = (*rows.shape[:3], padded)
+        assert got.shape == shape and got.stride() == torch.empty(shape).stride()
+        assert torch.equal(got[..., :width], rows) and not got[..., width:].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("width", [10, 64, 100])
+@pytest.mark.parametrize("layout", ["gradient", "inputs", "both", "one position"])
+def test_rows_whose_neighbours_lie_along_the_positions(device, layout, width, dtype):
+    """The gradient that an operator over positions hands back, and such inputs, at widths on and off 16 bytes."""
+
+    length = 1 if layout == "one position" else 90
+    q, k, v, valid, d_out = attention.make((2, length, 4, 2, width), dtype, 17, "tail", total=90)
+    inputs, up = [q, k, v], d_out
+    if layout in ("inputs", "both"):
+        inputs = [positions_last(t) for t in inputs]
+    if layout in ("gradient", "both"):
+        up = positions_last(up)
+    if layout == "one position":
+        inputs, up = [stray_stride(q), k, v], stray_stride(d_out)
+
+    def step(tensors, up):
+        leaves = [t.detach().requires_grad_() for t in tensors]
+        out = W.window_attention(*leaves, valid, window=20, sinks=2)
+        return (out, *torch.autograd.grad(out, leaves, up))
+
+    want = step([t.contiguous() for t in (q, k, v)], d_out)
+    assert all(torch.equal(a, b) for a, b in zip(step(inputs, up), want))
+    attention.check(q, k, v, valid, d_out, 20, 2)
+
+
+@pytest.mark.gpu
+def test_a_convolution_over_positions_behind_heads_of_ten(device):
+    """The same layout from a real graph: what follows the heads runs over channels first."""
+
+    q, k, v, _, _ = attention.make((2, 60, 3, 1, 10), torch.float32, 4, None)
+    weight = torch.randn(5, 30, 3, device=device)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    out = W.window_attention(*leaves, window=9, sinks=1)
+    got = []
+    out.register_hook(lambda g: got.append(g))
+    loss = torch.nn.functional.conv1d(out.flatten(2).transpose(1, 2), weight).square().sum()
+    grads = torch.autograd.grad(loss, leaves)
+    want, bounds = attention.reference(q, k, v, None, 9, 1, 1.0 / math.sqrt(10), got[0])
+    for g, w, b, name in zip(grads, want[1:], bounds[1:], ("d_queries", "d_keys", "d_values")):
+        attention.close(g, w, b, name)
