@@ -30,7 +30,7 @@ struct Backward {
     const void* rest;   // what out was rounded off by, or null: D is a small difference of large terms
     const void* d_out;  // each [batch, length, heads, width]
     const float* lse;
-    float* delta;       // D: [batch, heads, length], infinite for a row that sees one key
+    float* delta;       // D: [batch, heads, length], kAlone for a row that sees one key
     void* dq;
     void* dk;
     void* dv;
@@ -40,6 +40,13 @@ struct Backward {
 };
 
 template <typename T> constexpr int kKeys = sizeof(T) == 4 ? 32 : 64;  // of a tile that dq walks
+
+// D in place of a number: the row sees one key. A NaN that no sum is stored as: D may be infinite or NaN by
+// itself, and has to reach the keys' gradients then.
+constexpr uint32_t kAlone = 0x7fffffffu;
+__device__ __forceinline__ float stored_delta(float delta, bool alone) {
+    return __uint_as_float(alone ? kAlone : delta != delta ? 0x7fc00000u : __float_as_uint(delta));
+}
 
 __device__ __forceinline__ float largest(const f32x16& x) {
     float m = 0.0f;
@@ -187,7 +194,7 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 4 : NB == 2 && sizeof(T) == 2 ?
     if (row >= rows) return;
     // A row that sees one key has p = 1 whatever the score: no gradient, to the bit. Its D says so to the other kernel.
     const bool alone = sees <= 1;
-    if (half == 0) f.delta[at] = alone ? INFINITY : delta;
+    if (half == 0) f.delta[at] = stored_delta(delta, alone);
     if (!f.dq) return;
     const float by = a.scale * range.back();
 #pragma unroll
@@ -296,7 +303,7 @@ __global__ __launch_bounds__(kThreads, NB == 1 || (NB == 2 && !(SHARE && sizeof(
         for (int w = 0; w < RW; ++w) {
             const int r = 64 * w + lane;
             shown[w] = __ballot(r < RT && p0 + r < a.length && (!valid || next_ok[w]));
-            alone[w] = __ballot(next_delta[w] == INFINITY);
+            alone[w] = __ballot(__float_as_uint(next_delta[w]) == kAlone);
             every = every && shown[w] == low_bits(RT - 64 * w), some = some || shown[w], any_alone = any_alone || alone[w];
         }
         // every key of the workgroup is seen by every row of the tile

@@ -107,3 +107,42 @@ def test_a_convolution_over_positions_behind_heads_of_ten(device):
     want, bounds = attention.reference(q, k, v, None, 9, 1, 1.0 / math.sqrt(10), got[0])
     for g, w, b, name in zip(grads, want[1:], bounds[1:], ("d_queries", "d_keys", "d_values")):
         attention.close(g, w, b, name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("batch, sinks", [(2, 2), (90, 2), (2, 0)])
+@pytest.mark.parametrize("value", ["inf", "-inf", "nan", "overflow"])
+def test_an_infinite_gradient_reaches_every_key_that_its_row_sees(device, value, batch, sinks, dtype):
+    """D, the sum of d_out times out, of any size and sign: a row whose D is infinite counts like any other.
+
+    Column 5 of the values is positive, so with d_out = +-inf there D is, too, and every ds of the row NaN. With
+    overflow it is finite: the columns 5 and 6 of values are 0 or 3 (in fp16, whose largest D is far below fp32's, this
+    one has no infinite D and is left out), so that D = 2^127 (out_5 + out_6) passes 2^128 in heads where out_5 + out_6 >= 2.
+    Where it does not, keys of zeros have finite derivatives.
+    """
+
+    if value == "overflow" and dtype == torch.float16:
+        return
+    window, length, at = 40, 200, 130
+    q, k, v, _, d_out = attention.make((batch, length, 4, 2, 64), dtype, 3, None)
+    v[..., 5] = v[..., 5].abs() + 1.0
+    i = torch.arange(length, device=device)
+    if value == "overflow":
+        v[..., 5:7] = 3.0 * (i % 2 == 0)[None, :, None, None]
+        d_out[0, at, :, 5:7] = 2.0 ** 127
+    else:
+        d_out[0, at, :, 5] = float(value)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    out = W.window_attention(*leaves, window=window, sinks=sinks)
+    d_q, d_k, d_v = torch.autograd.grad(out, leaves, d_out)
+    seen = ((i <= at) & (at - i < window)) | (i < sinks)
+    assert torch.isfinite(out).all() and not torch.isfinite(d_q[0, at]).any()
+    reached = torch.ones(2, dtype=torch.bool, device=device)  # key heads
+    if value == "overflow":
+        reached = (out[0, at, :, 5].double() + out[0, at, :, 6].double() >= 2.0).view(2, 2).any(dim=1)
+        assert reached.any()
+    assert not torch.isfinite(d_k[0, seen][:, reached]).any()
+    assert torch.isfinite(d_k[0, ~seen]).all() and torch.isfinite(d_k[1:]).all() and torch.isfinite(d_q[0, i != at]).all()
+    if value != "overflow":
+        assert not torch.isfinite(d_v[0, seen][..., 5]).any() and torch.isfinite(d_v[0, ~seen]).all()
