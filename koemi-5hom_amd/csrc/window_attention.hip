@@ -158,6 +158,53 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 4 : NB == 2 ? 3 : NB <= 4 ? 2 :
                 }
             }
         }
+        if constexpr (sizeof(T) == 2) {
+            // An infinite value times two planes may be NaN, by a second plane of 0 or of the other sign. Where such sums
+            // are NaN and the probabilities are not, they are what the infinities and NaN among the values seen add up to.
+            bool nan = false;
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) nan = nan || acc[n][r] != acc[n][r];
+            const float all = sum_of_halves(sum);
+            nan = nan && row_ok && all == all;
+            if (__any(nan)) {
+                uint32_t lost[NB];
+#pragma unroll
+                for (int n = 0; n < NB; ++n) {
+                    lost[n] = 0;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (nan && acc[n][r] != acc[n][r]) acc[n][r] = 0.0f, lost[n] |= 1u << r;
+                }
+#pragma unroll 1
+                for (int t = t0; t < t1; ++t)
+#pragma unroll 1
+                    for (int key = tiles[t] * KT; key < min(tiles[t] * KT + KT, a.total); ++key) {
+                        if (!nan || key > place || (place - key >= a.window && key >= a.sinks) || (valid && !valid[key])) continue;
+                        const T* x = v + key * a.vs.position;
+#pragma unroll
+                        for (int n = 0; n < NB; ++n)
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) {
+                                const int d = 32 * n + 8 * q + 4 * half;
+                                if (d >= a.width) continue;
+                                alignas(8) T e[4];
+                                *reinterpret_cast<uint2*>(e) = *reinterpret_cast<const uint2*>(x + d);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    const float y = to_f32(e[i]);
+                                    acc[n][4 * q + i] += fabsf(y) < INFINITY ? 0.0f : y;
+                                }
+                            }
+                    }
+#pragma unroll
+                for (int n = 0; n < NB; ++n)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if ((lost[n] >> r & 1u) && acc[n][r] == 0.0f) acc[n][r] = NAN;
+            }
+        }
     }
     sum = sum_of_halves(sum);
     if (row >= rows) return;
@@ -191,7 +238,7 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 4 : NB == 2 ? 3 : NB <= 4 ? 2 :
             store_four(o, d, a.width, x);
             if (f.rest) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] -= to_f32(from_f32<T>(x[i]));
+                for (int i = 0; i < 4; ++i) x[i] = fabsf(x[i]) < INFINITY ? x[i] - to_f32(from_f32<T>(x[i])) : 0.0f;
                 store_four(static_cast<T*>(f.rest) + (o - static_cast<T*>(f.out)), d, a.width, x);
             }
         }
@@ -228,7 +275,8 @@ __global__ __launch_bounds__(kThreads) void window_join_kernel(Forward f) {
         }
         x *= invert;
         o[d] = from_f32<T>(x);
-        if (f.rest) static_cast<T*>(f.rest)[o - static_cast<T*>(f.out) + d] = from_f32<T>(x - to_f32(from_f32<T>(x)));
+        if (f.rest)
+            static_cast<T*>(f.rest)[o - static_cast<T*>(f.out) + d] = from_f32<T>(fabsf(x) < INFINITY ? x - to_f32(from_f32<T>(x)) : 0.0f);
     }
 }
 

@@ -73,7 +73,8 @@ def window_attention(queries: Tensor, keys: Tensor, values: Tensor, valid_mask: 
 
     Returns ``[B, L, H, D]`` in the inputs' type. Sums and softmax statistics are float32;
     16-bit calls keep the probabilities and, for the gradients, their derivatives to twice the
-    inputs' bits between two products. Sums run in a fixed order.
+    inputs' bits between two products. Sums run in a fixed order. What a value or gradient that is not
+    finite reaches is not finite either; an infinity among the gradients may read as NaN there.
     """
 
     for name, tensor in (("queries", queries), ("keys", keys), ("values", values)):

@@ -146,3 +146,37 @@ def test_an_infinite_gradient_reaches_every_key_that_its_row_sees(device, value,
     assert torch.isfinite(d_k[0, ~seen]).all() and torch.isfinite(d_k[1:]).all() and torch.isfinite(d_q[0, i != at]).all()
     if value != "overflow":
         assert not torch.isfinite(d_v[0, seen][..., 5]).any() and torch.isfinite(d_v[0, ~seen]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("batch, length, window", [(2, 200, 40), (90, 200, 150), (1, 2000, 1200)])
+@pytest.mark.parametrize("value", [float("inf"), float("-inf")])
+def test_an_infinity_that_a_row_sees_is_an_infinity(device, value, batch, length, window, dtype):
+    """A sum with one infinite term is infinite, of the term's sign: outputs over an infinite value. The gradients of
+    values under an infinite d_out are not finite. Rows and keys that see none stay within their bounds.
+    Scores are small, so that no probability vanishes."""
+
+    sinks, at = 1, 130
+    q, k, v, _, d_out = attention.make((batch, length, 4, 2, 64), dtype, 5, None)
+    i = torch.arange(length, device=device)
+    sees = (i >= at) & (i - at < window)
+    seen = ((i <= at) & (at - i < window)) | (i < sinks)
+    one = slice(0, 1)
+    want, bounds = attention.reference(q[one], k[one], v[one], None, window, sinks, 0.125, d_out[one])
+    bad = v.clone()
+    bad[0, at, :, 9] = value
+    for train in (False, True):
+        leaves = [t.clone().requires_grad_(train) for t in (q, k, bad)]
+        out = W.window_attention(*leaves, window=window, sinks=sinks)[0]
+        assert (out[sees][..., 9] == value).all()
+        others = [c for c in range(64) if c != 9]
+        attention.close(out[..., others], want[0][0][..., others], bounds[0][0][..., others], "out")
+        attention.close(out[~sees], want[0][0][~sees], bounds[0][0][~sees], "out")
+    up = d_out.clone()
+    up[0, at, :, 9] = value
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    d_v = torch.autograd.grad(W.window_attention(*leaves, window=window, sinks=sinks), leaves, up)[2][0]
+    assert not torch.isfinite(d_v[seen][..., 9]).any()
+    attention.close(d_v[..., others], want[3][0][..., others], bounds[3][0][..., others], "d_values")
+    attention.close(d_v[~seen], want[3][0][~seen], bounds[3][0][~seen], "d_values")
