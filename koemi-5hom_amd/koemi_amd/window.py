@@ -20,6 +20,7 @@ from typing import NamedTuple
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from koemi_amd import _native
@@ -56,7 +57,7 @@ def _load() -> None:
 
 def window_attention(queries: Tensor, keys: Tensor, values: Tensor, valid_mask: Tensor | None = None, *, window: int,
                      sinks: int = 0, scale: float | None = None) -> Tensor:
-    """Windowed attention with sinks, with first-order autograd.
+    """Windowed attention with sinks, with first-order autograd (reverse mode; forward mode is refused).
 
     ``queries`` ``[B, L, H, D]``, ``keys`` and ``values`` ``[B, T, G, D]`` in one type
     (float32, float16 or bfloat16), D at most 256, G a divisor of H (query head h reads
@@ -83,6 +84,9 @@ def window_attention(queries: Tensor, keys: Tensor, values: Tensor, valid_mask: 
     device, dtype = queries.device, queries.dtype
     if keys.device != device or values.device != device or keys.dtype != dtype or values.dtype != dtype:
         raise CudaThinkValidationError("queries, keys and values must share a dtype and a device")
+    # asked only while a level is open: each question takes 0.7 us
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in (queries, keys, values)):
+        raise CudaThinkValidationError("window_attention has no forward-mode derivative")
     width = queries.shape[-1] if queries.ndim else 1
     plan = _plan(queries.shape, keys.shape, values.shape, queries.stride(), keys.stride(), values.stride(), dtype, device.type,
                  _whole("window", window, 1), _whole("sinks", sinks, 0), _scale(scale, width))

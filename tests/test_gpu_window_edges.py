@@ -13,6 +13,7 @@ import torch
 
 import test_gpu_window_attention as attention
 from koemi_amd import window as W
+from koemi_amd.think import CudaThinkValidationError
 
 
 @pytest.mark.gpu
@@ -180,3 +181,17 @@ def test_an_infinity_that_a_row_sees_is_an_infinity(device, value, batch, length
     assert not torch.isfinite(d_v[seen][..., 9]).any()
     attention.close(d_v[..., others], want[3][0][..., others], bounds[3][0][..., others], "d_values")
     attention.close(d_v[~seen], want[3][0][~seen], bounds[3][0][~seen], "d_values")
+
+
+@pytest.mark.parametrize("which", ["queries", "keys", "values"])
+def test_forward_mode_is_refused(which):
+    """A tangent is not dropped: there is no forward-mode derivative. On the CPU, before anything runs."""
+
+    tensors = {"queries": torch.zeros(2, 5, 4, 8), "keys": torch.zeros(2, 5, 2, 8), "values": torch.zeros(2, 5, 2, 8)}
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(CudaThinkValidationError, match="must be on CUDA"):  # an open level alone refuses nothing
+            W.window_attention(*tensors.values(), window=3)
+        tensors[which] = torch.autograd.forward_ad.make_dual(tensors[which], torch.ones_like(tensors[which]))
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad), pytest.raises(CudaThinkValidationError, match="forward-mode"):
+                W.window_attention(*tensors.values(), window=3)
