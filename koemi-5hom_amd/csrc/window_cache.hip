@@ -279,7 +279,9 @@ struct alignas(2) Bytes {
 template <int NB, int KIND>
 struct Walk {
     f32x4 acc[2 * NB];
-    float top = -INFINITY, sum = 0.0f, by = 0.0f;
+    float top = -INFINITY, sum = 0.0f;
+    float peak = 0.0f;  // the largest probability times its value's scale, in units of the top as `acc`
+    int power = 0;      // acc is held times 2^power
     f16x8 q[2][NB];
     float factor;  // of a product of codes and planes, to a score in powers of two
 
@@ -337,33 +339,36 @@ struct Walk {
         high = fmaxf(top, max_of_groups(high));
         const bool higher = high > top;
         const float shrink = higher ? __builtin_amdgcn_exp2f(top - high) : 1.0f;
-        const float base = high == -INFINITY ? 0.0f : high;
+        const float base = high == -INFINITY ? 0.0f : high, was = top;
         top = high;
         sum *= shrink;
-        float x[8], most = 0.0f;
+        float prob[8], v[8], most = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float p = __builtin_amdgcn_exp2f(s[j] - base);
-            sum += p;
-            x[j] = (ok >> j) & 1u ? p * vs[j] : 0.0f;
-            most = fmaxf(most, fabsf(x[j]));
+            prob[j] = __builtin_amdgcn_exp2f(s[j] - base);
+            sum += prob[j];
+            v[j] = (ok >> j) & 1u ? vs[j] : 0.0f;
+            most = fmaxf(most, fabsf(prob[j] * v[j]));
         }
-        // fp16 planes of x: a power of two brings their largest to 2^13 .. 2^14, anew with every new top
-        most = max_of_groups(most);
-        const bool move = higher || most * by > 32768.0f || (by == 0.0f && most > 0.0f);
-        if (__any(move)) {
-            const int e = min(max(static_cast<int>(__float_as_uint(most) >> 23), 64), 254);
-            float to = move && most > 0.0f ? __uint_as_float(static_cast<uint32_t>(267 - e) << 23) : by;
-            if (by != 0.0f) to = fminf(to, by * 1.15292150e18f);  // 2^60: the sums' change stays finite
-            const float change = (move && by != 0.0f && most > 0.0f ? to / by : 1.0f) * shrink;
-            by = to;
+        // fp16 planes of p v: a power of two holds the largest so far at 2^13 to 2^15 (2^126 at most: scales from 2^-126 on
+        // stay above 1). It falls with the probabilities when the top rises, so the sums' change stays under 2^2.
+        peak = fmaxf(peak * shrink, max_of_groups(most));
+        const int want = min(140 - static_cast<int>(__float_as_uint(peak) >> 23), 126);
+        const bool move = peak > 0.0f && (want < power - 1 || want > power);
+        if (__any(higher || move)) {
+            const int next = move ? want : power;
+            const float change = shrink > 0.0f ? __builtin_amdgcn_exp2f((higher ? was - high : 0.0f) + static_cast<float>(next - power)) : 0.0f;
+            power = next;
 #pragma unroll
             for (int n = 0; n < 2 * NB; ++n) acc[n] *= change;
         }
+        // up to the scale before the value, down after it: neither passes the range on the way
+        const float up = __uint_as_float(static_cast<uint32_t>(127 + max(power, 0)) << 23);
+        const float down = __uint_as_float(static_cast<uint32_t>(127 + min(power, 0)) << 23);
         f16x8 p[2];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float y = x[j] * by;
+            const float y = prob[j] * up * v[j] * down;
             const _Float16 h = static_cast<_Float16>(y);
             p[0][j] = h;
             p[1][j] = static_cast<_Float16>(y - static_cast<float>(h));
@@ -517,13 +522,14 @@ __global__ __launch_bounds__(kStepWaves<NB> * kWave) void window_cache_step_kern
             walk.chunk(kw, vw, ks, vs, m == 0 ? 1u : 0u);
         }
     }
-    // the waves' sums joined in their order
-    const float total = sum_of_groups(walk.sum), back = walk.by == 0.0f ? 1.0f : 1.0f / walk.by;
+    // the waves' means joined in their order, by their shares of the whole: sums of large values would pass the range
+    const float total = sum_of_groups(walk.sum), invert = total == 0.0f ? 0.0f : 1.0f / total;
+    const float back = __uint_as_float(static_cast<uint32_t>(127 - walk.power) << 23);
     if (m == 0) tops[wave][col] = walk.top, totals[wave][col] = total;
 #pragma unroll
     for (int n = 0; n < 2 * NB; ++n)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) sums[wave][col][(4 * m + r) * 2 * NB + n] = walk.acc[n][r] * back;
+        for (int r = 0; r < 4; ++r) sums[wave][col][(4 * m + r) * 2 * NB + n] = walk.acc[n][r] * invert * back;
     __syncthreads();
     for (int i = threadIdx.x; i < 16 * NB * 32; i += kThreads) {
         const int h = i / (NB * 32), d = i % (NB * 32), hd = block * 16 + h;
@@ -531,16 +537,18 @@ __global__ __launch_bounds__(kStepWaves<NB> * kWave) void window_cache_step_kern
         float top = -INFINITY;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) top = tops[w][h] > top || tops[w][h] != tops[w][h] ? tops[w][h] : top;
-        float all = 0.0f, x = 0.0f;
+        float share[kWaves], all = 0.0f, x = 0.0f;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
-            if (tops[w][h] == -INFINITY && totals[w][h] == 0.0f) continue;
-            const float share = __builtin_amdgcn_exp2f(tops[w][h] - top);
-            all = fmaf(totals[w][h], share, all);
-            x = fmaf(sums[w][h][d], share, x);
+            const bool empty = tops[w][h] == -INFINITY && totals[w][h] == 0.0f;
+            share[w] = empty ? 0.0f : totals[w][h] * __builtin_amdgcn_exp2f(tops[w][h] - top);
+            all += share[w];
         }
         const bool none = all == 0.0f;
-        x = none ? 0.0f : x / all;
+        const float whole = 1.0f / all;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) x = fmaf(share[w] * whole, sums[w][h][d], x);
+        if (none) x = 0.0f;
         const int64_t cell = b * heads + static_cast<int64_t>(g) * f.shared + hd;
         if (f.splits == 1) {
             static_cast<T*>(f.out)[cell * c.width + d] = from_f32<T>(x);

@@ -12,6 +12,7 @@ import pytest
 import torch
 
 import test_gpu_window_attention as attention
+import test_gpu_window_cache as caching
 from koemi_amd import window as W
 from koemi_amd.think import CudaThinkValidationError
 
@@ -195,3 +196,87 @@ def test_forward_mode_is_refused(which):
         for grad in (True, False):
             with torch.set_grad_enabled(grad), pytest.raises(CudaThinkValidationError, match="forward-mode"):
                 W.window_attention(*tensors.values(), window=3)
+
+
+def held_cache(code, keys, values, window, sinks=0):
+    """A cache that holds these rows [batch, n, groups, width], its plain form, and the counts."""
+
+    batch, n, groups, width = keys.shape
+    cache = W.window_cache(batch, groups, width, window=window, sinks=sinks, dtype=code, device=keys.device)
+    none = torch.zeros(batch, dtype=torch.int64, device=keys.device)
+    W.window_cache_write(cache, keys, values, none)
+    return cache, caching.Plain(cache), none + n
+
+
+def read_and_step(cache, plain, counts, queries, key, value, scale):
+    """window_cache_read and _step against float64 over what the cache stands for."""
+
+    n = int(counts[0])
+    read = W.window_cache_read(cache, queries, counts, scale=scale)
+    for b in range(queries.shape[0]):
+        want, bound = plain.read(b, n, queries[b], scale)
+        caching.close(read[b], want, bound, ("read", b))
+    out = W.window_cache_step(cache, queries, key, value, counts, scale=scale)
+    for b in range(queries.shape[0]):
+        plain.append(b, n, key[b], value[b])
+        want, bound = plain.read(b, n + 1, queries[b], scale)
+        caching.close(out[b], want, bound, ("step", b))
+    plain.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code", caching.CODES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("entries, width", [(20, 40), (700, 64), (5000, 128)])
+@pytest.mark.parametrize("size", [2.0 ** -124, 1e-35, 1e-31, 1e-27, 1e-10, 1e10, 1e30, 3e37])
+def test_values_of_any_size_are_read(device, size, entries, width, dtype, code):
+    """Values from the smallest scale to the largest: bounds are relative to them, and their sum before it is divided passes the range."""
+
+    gen = torch.Generator(device="cuda").manual_seed(entries)
+    keys, values = (torch.randn(2, entries, 2, width, device=device, generator=gen) for _ in range(2))
+    if size > 1.0:  # one sign, so that the unscaled sum is large
+        values = values.abs()
+    values = (values * size).clamp(max=3e38).to(dtype)
+    cache, plain, counts = held_cache(code, keys.to(dtype), values, 5000)
+    queries = torch.randn(2, 6, width, device=device, generator=gen).to(dtype)
+    key = torch.randn(2, 2, width, device=device, generator=gen).to(dtype)
+    value = (torch.randn(2, 2, width, device=device, generator=gen).abs() * size).clamp(max=3e38).to(dtype)
+    read_and_step(cache, plain, counts, queries, key, value, 1.0 / math.sqrt(width))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code", caching.CODES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("size", [1e-31, 1.0, 1e17, 1e20, 1e37])
+def test_rows_of_zeros_with_rising_scores_after_values_of_any_size(device, size, dtype, code):
+    """One wave's chunks lie 256 slots apart: values first, then chunks of zero rows (whose scale is 2^-126), each of which brings a new
+    largest score, and a last chunk of small values. Scores rise by 1 a chunk, so that the first values stay in the result."""
+
+    width, chunks = 64, 8
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    i = torch.arange(256 * chunks, device=device)
+    keys = torch.zeros(1, 256 * chunks, 1, width, device=device)
+    keys[0, :, 0, 0] = (i // 256).float()
+    values = torch.randn(1, 256 * chunks, 1, width, device=device, generator=gen) * size
+    values[0, 256:-256] = 0.0
+    values[0, -256:] *= 2.0 ** -20
+    queries = torch.zeros(1, 3, width, device=device)
+    queries[0, :, 0] = torch.tensor([1.0, 0.5, -1.0], device=device)
+    cache, plain, counts = held_cache(code, keys.to(dtype), values.to(dtype), 4096)
+    read_and_step(cache, plain, counts, queries.to(dtype), keys[:, -1].to(dtype), values[:, 0].to(dtype), 1.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code", caching.CODES)
+@pytest.mark.parametrize("seed", range(6))
+def test_values_of_mixed_sizes(device, seed, code):
+    """Rows whose sizes are spread over sixty binary orders of magnitude, with scores over some tens."""
+
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    entries, width = 1500, 32
+    spread = torch.exp2(torch.rand(2, entries, 2, 1, device=device, generator=gen) * 60.0 - 30.0)
+    keys = torch.randn(2, entries, 2, width, device=device, generator=gen)
+    values = torch.randn(2, entries, 2, width, device=device, generator=gen) * spread
+    cache, plain, counts = held_cache(code, keys, values, 1024, sinks=3)
+    queries = torch.randn(2, 4, width, device=device, generator=gen)
+    read_and_step(cache, plain, counts, queries, keys[:, 5], values[:, 7], 0.5)
