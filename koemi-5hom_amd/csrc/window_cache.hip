@@ -283,7 +283,9 @@ struct Walk {
     float peak = 0.0f;  // the largest probability times its value's scale, in units of the top as `acc`
     int power = 0;      // acc is held times 2^power
     f16x8 q[2][NB];
-    float factor;  // of a product of codes and planes, to a score in powers of two
+    // of a product of codes and planes, and of a key's scale, to a score in powers of two: half of the queries' power each, so
+    // that neither large keys under small queries nor the reverse pass the range on the way
+    float factor, key_factor;
 
     template <typename T>
     __device__ __forceinline__ void begin(const T* row, int width, bool ok, bool vector, float scale) {
@@ -301,8 +303,10 @@ struct Walk {
         high = max_of_groups(high);
         // the largest comes to 2^14 .. 2^15, so that what the second plane has no digits for is below 2^-39 of it
         const int e = min(max(static_cast<int>(__float_as_uint(high) >> 23), 16), 254);
-        const float lift = __uint_as_float(static_cast<uint32_t>(min(268 - e, 254)) << 23);
-        factor = scale * kLog2e / lift;
+        const int power = 141 - e;
+        const float lift = __uint_as_float(static_cast<uint32_t>(127 + power) << 23);
+        factor = scale * kLog2e * __uint_as_float(static_cast<uint32_t>(127 - power / 2) << 23);
+        key_factor = __uint_as_float(static_cast<uint32_t>(127 - (power - power / 2)) << 23);
 #pragma unroll
         for (int s = 0; s < NB; ++s)
 #pragma unroll
@@ -331,7 +335,7 @@ struct Walk {
                 d = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q[1][n], d, 0, 0, 0);
             }
 #pragma unroll
-            for (int r = 0; r < 4; ++r) s[4 * h + r] = (ok >> (4 * h + r)) & 1u ? d[r] * ks[4 * h + r] * factor : -INFINITY;
+            for (int r = 0; r < 4; ++r) s[4 * h + r] = (ok >> (4 * h + r)) & 1u ? (d[r] * factor) * (ks[4 * h + r] * key_factor) : -INFINITY;
         }
         float high = s[0];
 #pragma unroll

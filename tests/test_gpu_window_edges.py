@@ -280,3 +280,20 @@ def test_values_of_mixed_sizes(device, seed, code):
     cache, plain, counts = held_cache(code, keys, values, 1024, sinks=3)
     queries = torch.randn(2, 4, width, device=device, generator=gen)
     read_and_step(cache, plain, counts, queries, keys[:, 5], values[:, 7], 0.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code", caching.CODES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("key_size", [2.0 ** -100, 2.0 ** -60, 2.0 ** 60, 2.0 ** 100, 2.0 ** 122])
+def test_keys_of_any_size_are_scored(device, key_size, dtype, code):
+    """Large keys under small queries and the reverse: scores of order one, whose factors alone pass the range."""
+
+    width, entries = 64, 300
+    gen = torch.Generator(device="cuda").manual_seed(13)
+    keys = (torch.randn(2, entries, 2, width, device=device, generator=gen) * key_size).to(dtype)
+    values = torch.randn(2, entries, 2, width, device=device, generator=gen).to(dtype)
+    queries = (torch.randn(2, 4, width, device=device, generator=gen) / min(key_size, 2.0 ** 110)).to(dtype)
+    cache, plain, counts = held_cache(code, keys, values, 512)
+    scale = 0.125 * min(1.0, 2.0 ** 110 / key_size)
+    read_and_step(cache, plain, counts, queries, keys[:, 3], values[:, 4], scale)
