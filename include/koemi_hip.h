@@ -1039,6 +1039,16 @@ int koemi_window_attention_forward(const void* queries, const void* keys, const 
                                    int64_t sinks, float scale, int dtype, void* workspace, size_t workspace_bytes,
                                    koemi_stream_t stream);
 
+/* The same for a chunk of a sequence behind an 8-bit cache of its past (below): keys and values [batch, window + sinks +
+ * length, groups, width] are the cache's entries as koemi_window_cache_entries gives them, then the chunk's own; valid
+ * (needed) says which are there. held [batch] int64: the entries that a row had. A row that had fewer than
+ * `sinks` has the others among the chunk's first positions, and they stay visible like those of the cache. No
+ * gradients. Workspace: koemi_window_attention_workspace_bytes of that total. */
+int koemi_window_attention_chunk(const void* queries, const void* keys, const void* values, const uint8_t* valid,
+                                 const int64_t* strides, const int64_t* held, void* output, int64_t batch, int64_t length,
+                                 int64_t heads, int64_t groups, int64_t width, int64_t window, int64_t sinks, float scale,
+                                 int dtype, void* workspace, size_t workspace_bytes, koemi_stream_t stream);
+
 /* Its gradients, each contiguous in its input's shape, NULL where not wanted. output,
  * rest, lse: the forward's; grad_output contiguous. Sums run in a fixed order. */
 size_t koemi_window_attention_backward_workspace_bytes(int64_t batch, int64_t length, int64_t total, int64_t heads,

@@ -30,10 +30,13 @@ struct Forward {
     float* lse;       // [batch, heads, length] or null
     float* parts;     // one of several parts of the keys: [parts, batch, groups, rows, width] sums, null for one part
     float* part_lse;  // [parts, batch, groups, rows]
+    const int64_t* held;  // [batch]: entries of the cache that the keys begin with, or null
     int row_tiles, splits;
 };
 
-template <typename T, int NB>
+// LATE: the keys begin with a cache's entries (as many as it has slots), and rows that held fewer than their sinks have
+// the others among the first of the queries' own positions.
+template <typename T, int NB, bool LATE>
 __global__ __launch_bounds__(kThreads, NB == 1 ? 4 : NB == 2 ? 3 : NB <= 4 ? 2 : 1) void window_forward_kernel(Forward f) {
     using L = Tile<T, NB>;
     constexpr int KT = kKeys<T>, KB = KT / 32;
@@ -54,6 +57,8 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 4 : NB == 2 ? 3 : NB <= 4 ? 2 :
     const uint8_t* valid = a.valid ? a.valid + static_cast<int64_t>(b) * a.total : nullptr;
     const bool row_ok = row < rows && (!valid || valid[place]);
     const uint8_t* shown_at = valid ? valid : static_cast<const uint8_t*>(a.k);  // any byte where all are valid
+    const int late = LATE ? static_cast<int>(max(a.sinks - max(f.held[b], int64_t{0}), int64_t{0})) : 0;
+    const int late_from = LATE ? before : 0, late_to = LATE ? before + min(late, a.length) : 0;
     if (threadIdx.x == 0) bad_tile = -1, any_row = 0;
     __syncthreads();
     if (__ballot(row_ok) && lane == 0) any_row = 1;
@@ -72,7 +77,7 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 4 : NB == 2 ? 3 : NB <= 4 ? 2 :
 #pragma unroll
         for (int s = 0; s < L::kFrags; ++s)
             qf[s] = row_ok ? load_unit<T>(q, 2 * s + half, a.width) : make_uint4(0, 0, 0, 0);
-        const KeyTiles<KT> tiles(a, first, last);
+        const KeyTiles<KT> tiles(a, first, last, late_from, late_to);
         const int t0 = static_cast<int>(static_cast<int64_t>(tiles.count) * split / f.splits);
         const int t1 = static_cast<int>(static_cast<int64_t>(tiles.count) * (split + 1) / f.splits);
         // the wave's own rows
@@ -93,7 +98,7 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 4 : NB == 2 ? 3 : NB <= 4 ? 2 :
             const int key0 = tiles[t] * KT;
             const uint64_t shown = __ballot(lane < KT && key0 + lane < a.total && (!valid || next_ok)), every = low_bits(KT);
             auto whole = [&](int lo, int hi) {  // rows at places lo .. hi see all of the tile
-                return shown == every && key0 + KT - 1 <= lo && (hi - key0 < a.window || key0 + KT <= a.sinks);
+                return shown == every && key0 + KT - 1 <= lo && (hi - key0 < a.window || key0 + KT <= a.sinks || (LATE && key0 >= late_from && key0 + KT <= late_to));
             };
             __syncthreads();
             if (!whole(first, last)) {
@@ -104,7 +109,8 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 4 : NB == 2 ? 3 : NB <= 4 ? 2 :
             next_v.store(v_tile, a.width);
             __syncthreads();
             if (t + 1 < t1) fetch(t + 1);
-            if (!shown || !wave_rows || key0 > wave_last || (key0 + KT <= wave_first - a.window + 1 && key0 >= a.sinks)) continue;
+            if (!shown || !wave_rows || key0 > wave_last || (key0 + KT <= wave_first - a.window + 1 && key0 >= a.sinks && !(LATE && key0 < late_to && key0 + KT > late_from)))
+                continue;
             f32x16 s[KB];
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
@@ -114,7 +120,7 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 4 : NB == 2 ? 3 : NB <= 4 ? 2 :
             const bool masked = !whole(wave_first, wave_last);
             uint64_t seen = every;
             if (masked) {
-                seen = row_ok ? keys_seen(a, place, key0) & shown : 0ull;
+                seen = row_ok ? keys_seen(a, place, key0, late_from, late_to) & shown : 0ull;
 #pragma unroll
                 for (int kb = 0; kb < KB; ++kb) {
                     const uint32_t mine = static_cast<uint32_t>(seen >> (32 * kb)) >> (4 * half);
@@ -181,7 +187,7 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 4 : NB == 2 ? 3 : NB <= 4 ? 2 :
                 for (int t = t0; t < t1; ++t)
 #pragma unroll 1
                     for (int key = tiles[t] * KT; key < min(tiles[t] * KT + KT, a.total); ++key) {
-                        if (!nan || key > place || (place - key >= a.window && key >= a.sinks) || (valid && !valid[key])) continue;
+                        if (!nan || key > place || (place - key >= a.window && key >= a.sinks && !(LATE && key >= late_from && key < late_to)) || (valid && !valid[key])) continue;
                         const T* x = v + key * a.vs.position;
 #pragma unroll
                         for (int n = 0; n < NB; ++n)
@@ -298,7 +304,10 @@ int splits_for(int64_t batch, int64_t length, int64_t total, int64_t heads, int6
 template <typename T, int NB>
 int run(const Forward& f, hipStream_t stream) {
     const int64_t grid = workgroups_of(f.s.batch, f.s.groups, static_cast<int64_t>(f.s.length) * f.s.shared) * f.splits;
-    hipLaunchKernelGGL((window_forward_kernel<T, NB>), dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, stream, f);
+    if (f.held)
+        hipLaunchKernelGGL((window_forward_kernel<T, NB, true>), dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, stream, f);
+    else
+        hipLaunchKernelGGL((window_forward_kernel<T, NB, false>), dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, stream, f);
     int rc = check_launch("koemi_window_attention_forward");
     if (rc != KOEMI_OK || f.splits == 1) return rc;
     const int64_t cells = static_cast<int64_t>(f.s.length) * f.s.shared * f.s.batch * f.s.groups;
@@ -381,19 +390,18 @@ extern "C" size_t koemi_window_attention_workspace_bytes(int64_t batch, int64_t 
     return n == 1 ? 0 : static_cast<size_t>(n) * batch * heads * length * (width + 1) * 4;
 }
 
-extern "C" int koemi_window_attention_forward(const void* queries, const void* keys, const void* values, const uint8_t* valid,
-                                              const int64_t* strides, void* output, void* rest, float* lse, int64_t batch, int64_t length,
-                                              int64_t total, int64_t heads, int64_t groups, int64_t width, int64_t window,
-                                              int64_t sinks, float scale, int dtype, void* workspace, size_t workspace_bytes,
-                                              koemi_stream_t stream) {
-    clear_error();
-    const char* what = "koemi_window_attention_forward";
+namespace {
+
+int forward(const char* what, const void* queries, const void* keys, const void* values, const uint8_t* valid, const int64_t* strides,
+            const int64_t* held, void* output, void* rest, float* lse, int64_t batch, int64_t length, int64_t total, int64_t heads,
+            int64_t groups, int64_t width, int64_t window, int64_t sinks, float scale, int dtype, void* workspace,
+            size_t workspace_bytes, koemi_stream_t stream) {
     Forward f{};
     const int rc = shape_of(what, queries, keys, values, valid, strides, batch, length, total, heads, groups, width, window, sinks,
                             scale, dtype, f.s);
     if (rc != KOEMI_OK || batch == 0 || length == 0) return rc;
     if (!output) return fail(KOEMI_ERR_INVALID, "%s: null pointer", what);
-    f.out = output, f.rest = dtype == KOEMI_F32 ? nullptr : rest, f.lse = lse;
+    f.out = output, f.rest = dtype == KOEMI_F32 ? nullptr : rest, f.lse = lse, f.held = held;
     f.row_tiles = static_cast<int>((length * f.s.shared + kRows - 1) / kRows);
     f.splits = splits_for(batch, length, total, heads, groups, window, sinks, dtype);
     if (f.splits > 1) {
@@ -405,4 +413,30 @@ extern "C" int koemi_window_attention_forward(const void* queries, const void* k
     if (dtype == KOEMI_F32) return by_width<float>(f, as_stream(stream));
     if (dtype == KOEMI_F16) return by_width<f16>(f, as_stream(stream));
     return by_width<bf16>(f, as_stream(stream));
+}
+
+}  // namespace
+
+extern "C" int koemi_window_attention_forward(const void* queries, const void* keys, const void* values, const uint8_t* valid,
+                                              const int64_t* strides, void* output, void* rest, float* lse, int64_t batch, int64_t length,
+                                              int64_t total, int64_t heads, int64_t groups, int64_t width, int64_t window,
+                                              int64_t sinks, float scale, int dtype, void* workspace, size_t workspace_bytes,
+                                              koemi_stream_t stream) {
+    clear_error();
+    return forward("koemi_window_attention_forward", queries, keys, values, valid, strides, nullptr, output, rest, lse, batch, length, total,
+                   heads, groups, width, window, sinks, scale, dtype, workspace, workspace_bytes, stream);
+}
+
+extern "C" int koemi_window_attention_chunk(const void* queries, const void* keys, const void* values, const uint8_t* valid,
+                                            const int64_t* strides, const int64_t* held, void* output, int64_t batch, int64_t length,
+                                            int64_t heads, int64_t groups, int64_t width, int64_t window, int64_t sinks, float scale,
+                                            int dtype, void* workspace, size_t workspace_bytes, koemi_stream_t stream) {
+    clear_error();
+    const char* what = "koemi_window_attention_chunk";
+    if (length < 0 || window < 1 || sinks < 0) return fail(KOEMI_ERR_INVALID, "%s: window must be positive, length and sinks not negative", what);
+    if (length >= (1 << 29) || window >= (1 << 29) || sinks >= (1 << 29))
+        return fail(KOEMI_ERR_UNSUPPORTED, "%s: at most 2^29 positions", what);
+    if (batch > 0 && length > 0 && (!valid || !held)) return fail(KOEMI_ERR_INVALID, "%s: null pointer", what);
+    return forward(what, queries, keys, values, valid, strides, held, output, nullptr, nullptr, batch, length, window + sinks + length, heads,
+                   groups, width, window, sinks, scale, dtype, workspace, workspace_bytes, stream);
 }

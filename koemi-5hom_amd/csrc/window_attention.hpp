@@ -288,10 +288,10 @@ __device__ __forceinline__ float sum_of_halves(float x) {
     return __uint_as_float(both[0]) + __uint_as_float(both[1]);
 }
 
-// Of the 64 keys from key0 on, those that a query at `place` sees by position.
-__device__ __forceinline__ uint64_t keys_seen(const Shape& a, int place, int key0) {
+// Of the 64 keys from key0 on, those that a query at `place` sees by position. Keys from..to - 1 are sinks as well.
+__device__ __forceinline__ uint64_t keys_seen(const Shape& a, int place, int key0, int from = 0, int to = 0) {
     const int rel = place - key0;
-    return low_bits(rel + 1) & (~low_bits(rel - a.window + 1) | low_bits(a.sinks - key0));
+    return low_bits(rel + 1) & (~low_bits(rel - a.window + 1) | low_bits(a.sinks - key0) | (low_bits(to - key0) & ~low_bits(from - key0)));
 }
 
 // x where the lane's register r of a 32-row block is seen (seen_half: the block's mask from
@@ -323,17 +323,20 @@ struct Place {
 };
 
 // Key tiles of KT that rows at places first .. last (of the keys' positions) see: the
-// sinks' before the window, then the window's.
+// sinks' before the window, then the window's; between them those of keys from..to - 1, sinks as well.
 template <int KT>
 struct KeyTiles {
-    int lead, skip, count;
-    __device__ __forceinline__ KeyTiles(const Shape& a, int first, int last) {
+    int lead, middle, jump, skip, count;
+    __device__ __forceinline__ KeyTiles(const Shape& a, int first, int last, int from = 0, int to = 0) {
         const int low = max(first - a.window + 1, 0) / KT;
         lead = min((a.sinks + KT - 1) / KT, low);
-        skip = low - lead;
-        count = lead + last / KT - low + 1;
+        const int end = min((to + KT - 1) / KT, low), begin = max(from / KT, lead);
+        middle = to > from ? max(end - begin, 0) : 0;
+        jump = begin - lead;
+        skip = low - lead - middle;
+        count = lead + middle + last / KT - low + 1;
     }
-    __device__ __forceinline__ int operator[](int t) const { return t < lead ? t : t + skip; }
+    __device__ __forceinline__ int operator[](int t) const { return t < lead ? t : t < lead + middle ? t + jump : t + skip; }
 };
 
 // Checks, and the shape as the kernels take it (window_attention.hip).

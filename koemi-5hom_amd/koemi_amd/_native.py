@@ -96,6 +96,10 @@ _SIGNATURES: dict[str, tuple[Any, tuple[Any, ...]]] = {
         c_int,
         (_P,) * 8 + (c_int64,) * 8 + (c_float, c_int, _P, c_size_t, _P),
     ),
+    "koemi_window_attention_chunk": (
+        c_int,
+        (_P,) * 7 + (c_int64,) * 7 + (c_float, c_int, _P, c_size_t, _P),
+    ),
     "koemi_window_attention_backward_workspace_bytes": (c_size_t, (c_int64,) * 8 + (c_int,)),
     "koemi_window_attention_backward": (
         c_int,

@@ -56,7 +56,7 @@ def _load() -> None:
 
 
 def window_attention(queries: Tensor, keys: Tensor, values: Tensor, valid_mask: Tensor | None = None, *, window: int,
-                     sinks: int = 0, scale: float | None = None) -> Tensor:
+                     sinks: int = 0, scale: float | None = None, lengths: Tensor | None = None) -> Tensor:
     """Windowed attention with sinks, with first-order autograd (reverse mode; forward mode is refused).
 
     ``queries`` ``[B, L, H, D]``, ``keys`` and ``values`` ``[B, T, G, D]`` in one type
@@ -71,6 +71,11 @@ def window_attention(queries: Tensor, keys: Tensor, values: Tensor, valid_mask: 
     its tensors hold does not matter, it reads zeros and its gradients are zeros. A query
     that sees nothing reads zeros. Positions count from the first row of ``keys``, so
     batches are padded at their end.
+
+    ``lengths`` ``[B]`` int64, for a chunk behind a cache: ``keys``, ``values`` and ``valid_mask`` are what
+    ``window_cache_entries`` gives for these lengths, then the chunk's own (T = sinks + window + L). Rows
+    that held fewer than ``sinks`` entries have the others among the chunk's first positions; without ``lengths`` those
+    would leave the sight with the window. Without gradients.
 
     Returns ``[B, L, H, D]`` in the inputs' type. Sums and softmax statistics are float32;
     16-bit calls keep the probabilities and, for the gradients, their derivatives to twice the
@@ -87,15 +92,25 @@ def window_attention(queries: Tensor, keys: Tensor, values: Tensor, valid_mask: 
     # asked only while a level is open: each question takes 0.7 us
     if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in (queries, keys, values)):
         raise CudaThinkValidationError("window_attention has no forward-mode derivative")
+    trained = torch.is_grad_enabled() and (queries.requires_grad or keys.requires_grad or values.requires_grad)
+    window, sinks = _whole("window", window, 1), _whole("sinks", sinks, 0)
+    if lengths is not None:
+        if not isinstance(lengths, Tensor) or lengths.dtype != torch.int64 or lengths.shape != queries.shape[:1] or lengths.device != device:
+            raise CudaThinkValidationError("lengths must be an int64 [batch] tensor on the same device")
+        if valid_mask is None or (queries.ndim == keys.ndim == 4 and keys.shape[1] - queries.shape[1] != window + sinks):
+            raise CudaThinkValidationError("with lengths, keys, values and a valid_mask must be a cache's sinks + window entries "
+                                           "and the queries' own positions")
+        if trained:
+            raise CudaThinkValidationError("window_attention has no gradients with lengths: a cache's entries have none")
     width = queries.shape[-1] if queries.ndim else 1
     plan = _plan(queries.shape, keys.shape, values.shape, queries.stride(), keys.stride(), values.stride(), dtype, device.type,
-                 _whole("window", window, 1), _whole("sinks", sinks, 0), _scale(scale, width))
+                 window, sinks, _scale(scale, width))
     if valid_mask is not None and (not isinstance(valid_mask, Tensor) or valid_mask.dtype != torch.bool
                                    or valid_mask.shape != keys.shape[:2] or valid_mask.device != device):
         raise CudaThinkValidationError("valid_mask must be a bool [batch, total] tensor on the same device")
-    if torch.is_grad_enabled() and (queries.requires_grad or keys.requires_grad or values.requires_grad):
+    if trained:
         return _WindowAttention.apply(queries, keys, values, valid_mask, plan)
-    return _forward(queries, keys, values, valid_mask, plan, False)[0]
+    return _forward(queries, keys, values, valid_mask, plan, False, lengths)[0]
 
 
 class _Plan(NamedTuple):
@@ -168,7 +183,8 @@ def _strides(*tensors: Tensor) -> ctypes.Array:
     return (ctypes.c_int64 * len(flat))(*flat)
 
 
-def _forward(queries: Tensor, keys: Tensor, values: Tensor, valid_mask: Tensor | None, plan: _Plan, trained: bool) -> tuple:
+def _forward(queries: Tensor, keys: Tensor, values: Tensor, valid_mask: Tensor | None, plan: _Plan, trained: bool,
+             lengths: Tensor | None = None) -> tuple:
     """The output, and with ``trained`` what the gradients need."""
 
     batch, length, total, heads, groups, padded, window, sinks = plan.sizes
@@ -184,6 +200,13 @@ def _forward(queries: Tensor, keys: Tensor, values: Tensor, valid_mask: Tensor |
     lse = torch.empty((batch, heads, length), device=device, dtype=torch.float32) if trained else None
     need = plan.workspace[0]
     workspace = torch.empty(need, device=device, dtype=torch.uint8) if need else None
+    if lengths is not None:
+        lengths = lengths.contiguous()
+        with _native.device_guard(device):
+            _native.call("koemi_window_attention_chunk", *at, _native.ptr(mask), strides, lengths.data_ptr(), output.data_ptr(),
+                         batch, length, heads, groups, padded, window, sinks, plan.scale, plan.code, _native.ptr(workspace),
+                         need, _native.stream_of(device))
+        return (output if padded == plan.width else output[..., :plan.width].contiguous(),)
     with _native.device_guard(device):
         _native.call("koemi_window_attention_forward", *at, _native.ptr(mask), strides, output.data_ptr(), _native.ptr(rest),
                      _native.ptr(lse), batch, length, total, heads, groups, padded, window, sinks, plan.scale, plan.code,
@@ -368,7 +391,8 @@ def window_cache_entries(cache: WindowCache, lengths: Tensor, *, dtype: torch.dt
     Returns ``(keys, values, present)``: ``[B, sinks + window, G, D]`` in ``dtype`` and
     ``[B, sinks + window]`` bool: the sinks, then the last ``window`` other entries in their
     order, the latest at the end; places without an entry hold zeros. Put before the next
-    chunk's keys, values and mask, ``window_attention`` reads them as the chunk's own past.
+    chunk's keys, values and mask, ``window_attention`` with the same ``lengths`` reads them as the
+    chunk's own past.
     """
 
     cache = _check_cache(cache)

@@ -297,3 +297,130 @@ def test_keys_of_any_size_are_scored(device, key_size, dtype, code):
     cache, plain, counts = held_cache(code, keys, values, 512)
     scale = 0.125 * min(1.0, 2.0 ** 110 / key_size)
     read_and_step(cache, plain, counts, queries, keys[:, 3], values[:, 4], scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("width, window, sinks, chunks", [
+    (64, 50, 3, (70, 20, 9)),          # a first chunk longer than the window
+    (64, 30, 5, (2, 1, 3, 40, 40)),    # chunks shorter than the sinks
+    (128, 40, 130, (100, 90, 200)),    # sinks of more than two tiles, filled over two chunks
+    (10, 20, 4, (33, 300)),
+    (32, 16, 1, (900, 30)),            # many tiles between the late sinks and the window
+    (64, 100, 0, (150, 20)),
+    (256, 25, 70, (60, 130)),
+])
+def test_chunks_behind_a_cache_whatever_its_rows_hold(device, width, window, sinks, chunks, dtype):
+    """Every row's chunks against float64 over its own entries in one sequence: rows that are behind with their sinks, fresh
+    ones among old ones, rows that pause. The sinks are a row's first entries, in the cache or in the chunk."""
+
+    batch, heads, groups = 4, 6, 2
+    gen = torch.Generator(device="cuda").manual_seed(width + sinks)
+    cache = W.window_cache(batch, groups, width, window=window, sinks=sinks, device=device)
+    plain = caching.Plain(cache)
+    lengths = torch.zeros(batch, dtype=torch.int64, device=device)
+    scale = 1.0 / math.sqrt(width)
+    for turn, length in enumerate(chunks):
+        q = torch.randn(batch, length, heads, width, device=device, generator=gen).to(dtype)
+        k, v = (torch.randn(batch, length, groups, width, device=device, generator=gen).to(dtype) for _ in range(2))
+        counts = torch.tensor([length, max(1, length - 13), min(2, length), 0 if turn == 0 else length], device=device)
+        held_k, held_v, present = W.window_cache_entries(cache, lengths, dtype=dtype)
+        chunk = torch.arange(length, device=device)[None] < counts[:, None]
+        out = W.window_attention(q, torch.cat([held_k, k], 1), torch.cat([held_v, v], 1), torch.cat([present, chunk], 1),
+                                 window=window, sinks=sinks, lengths=lengths)
+        for b in range(batch):
+            n, count = int(lengths[b]), int(counts[b])
+            assert not out[b, count:].any()
+            if not count:
+                continue
+            entries = plain.held(n)
+            at = [plain.slot(p) for p in entries]
+            past = [plain.stands_for(name, b, at, torch.float32).to(dtype).transpose(0, 1) for name in ("keys", "values")]
+            kk, vv = (torch.cat([p, new[b, :count]]).double().repeat_interleave(heads // groups, 1).transpose(0, 1)
+                      for p, new in zip(past, (k, v)))
+            places = torch.tensor(entries + list(range(n, n + count)), device=device)
+            i, j = places[len(entries):, None], places[None]
+            see = (j <= i) & ((i - j < window) | (j < sinks))
+            qq = q[b, :count].double().transpose(0, 1)
+            s = torch.matmul(qq, kk.transpose(1, 2).contiguous()) * scale
+            size = torch.where(see, torch.matmul(qq.abs(), kk.abs().transpose(1, 2).contiguous()) * scale, 0.0).amax(dim=-1, keepdim=True)
+            p = torch.softmax(s.masked_fill(~see, float("-inf")), dim=-1)
+            half = attention.HALF_STEP[dtype]
+            bound = torch.matmul((half * half + 2.0 ** -17 * (1.0 + size)) * p, vv.abs())
+            attention.close(out[b, :count], torch.matmul(p, vv).transpose(0, 1), bound.transpose(0, 1), (length, b))
+        W.window_cache_write(cache, k, v, lengths, counts)
+        for b in range(batch):
+            for t in range(int(counts[b])):
+                plain.append(b, int(lengths[b]) + t, k[b, t], v[b, t])
+        lengths = lengths + counts
+
+
+@pytest.mark.gpu
+def test_a_chunk_of_one_position_and_full_rows(device):
+    """With all sinks held, or none to hold, `lengths` changes nothing, whatever else it says; negative ones hold nothing."""
+
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    for length, window, sinks in ((1, 30, 4), (70, 30, 4), (40, 600, 2), (5, 3, 0)):
+        q = torch.randn(3, length, 4, 64, device=device, generator=gen).bfloat16()
+        k, v = (torch.randn(3, sinks + window + length, 2, 64, device=device, generator=gen).bfloat16() for _ in range(2))
+        valid = torch.rand(3, sinks + window + length, device=device, generator=gen) < 0.8
+        want = W.window_attention(q, k, v, valid, window=window, sinks=sinks)
+        for held in ([sinks, sinks + 9, 1 << 40], torch.tensor([[sinks, 0], [1 << 62, 0], [sinks, 0]])[:, 0]):
+            held = torch.as_tensor(held).to(device)
+            assert torch.equal(W.window_attention(q, k, v, valid, window=window, sinks=sinks, lengths=held), want)
+        none, less = (W.window_attention(q, k, v, valid, window=window, sinks=sinks, lengths=torch.full((3,), n, device=device)) for n in (0, -5))
+        assert torch.equal(none, less)
+
+
+@pytest.mark.gpu
+def test_chunks_in_a_graph(device):
+    """The counts are read on the device: replays with others."""
+
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    q = torch.randn(2, 40, 4, 64, device=device, generator=gen).bfloat16()
+    k, v = (torch.randn(2, 56, 2, 64, device=device, generator=gen).bfloat16() for _ in range(2))
+    valid, held = torch.ones(2, 56, dtype=torch.bool, device=device), torch.zeros(2, dtype=torch.int64, device=device)
+    run = lambda: W.window_attention(q, k, v, valid, window=10, sinks=6, lengths=held)  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for a, b in ((0, 3), (6, 1), (2, 100), (0, 0)):
+        held.copy_(torch.tensor([a, b]))
+        graph.replay()
+        assert torch.equal(out, run())
+
+
+def test_chunks_that_are_refused():
+    q, k, n = torch.zeros(2, 5, 4, 8), torch.zeros(2, 12, 2, 8), torch.zeros(2, dtype=torch.int64)
+    valid = torch.ones(2, 12, dtype=torch.bool)
+
+    def call(lengths=n, mask=valid, sinks=3, queries=q):
+        return lambda: W.window_attention(queries, k, k, mask, window=4, sinks=sinks, lengths=lengths)
+
+    for bad, message in ((call(lengths=n.int()), "lengths must be an int64"), (call(lengths=n[:1]), "lengths must be an int64"),
+                         (call(lengths=[0, 0]), "lengths must be an int64"), (call(mask=None), "with lengths"), (call(sinks=2), "with lengths"),
+                         (call(queries=q.clone().requires_grad_()), "no gradients with lengths"), (call(), "must be on CUDA")):
+        with pytest.raises(CudaThinkValidationError, match=message):
+            bad()
+
+
+def test_the_library_refuses_chunks_that_it_cannot_take():
+    import ctypes
+
+    from koemi_amd import _native
+
+    strides = (ctypes.c_int64 * 9)(*[64 * 4, 64, 16] * 3)
+
+    def call(valid=16, held=16, length=4, window=2, sinks=1, width=16):
+        return lambda: _native.call("koemi_window_attention_chunk", 16, 16, 16, valid, strides, held, 16, 1, length, 4, 4, width, window,
+                                    sinks, 1.0, _native.F32, None, 0, None)
+
+    for bad, message in ((call(valid=None), "null pointer"), (call(held=None), "null pointer"), (call(length=-1), "not negative"),
+                         (call(window=0), "window"), (call(sinks=-1), "window"), (call(window=1 << 40), "2\\^29"), (call(width=320), "256")):
+        with pytest.raises(_native.NativeCallError, match=message):
+            bad()
