@@ -437,12 +437,11 @@ def _step_plan(cache: tuple, width: int, window: int, sinks: int, scale: float |
 
 
 def _step(cache: WindowCache, queries: Tensor, keys: Tensor | None, values: Tensor | None, lengths: Tensor,
-          active: Tensor | None, scale: float | None) -> Tensor:
+          active: Tensor | None, scale: float | None, writes: bool) -> Tensor:
     cache = _check_cache(cache)
     _check_tensor(cache, "queries", queries)
     if scale is not None:
         scale = _scale(scale, cache.width)
-    writes = keys is not None or values is not None
     if writes:
         _check_tensor(cache, "keys", keys)
         _check_tensor(cache, "values", values)
@@ -485,11 +484,11 @@ def window_cache_step(cache: WindowCache, queries: Tensor, keys: Tensor, values:
     gradients.
     """
 
-    return _step(cache, queries, keys, values, lengths, active, scale)
+    return _step(cache, queries, keys, values, lengths, active, scale, True)
 
 
 def window_cache_read(cache: WindowCache, queries: Tensor, lengths: Tensor, active: Tensor | None = None, *,
                       scale: float | None = None) -> Tensor:
     """``window_cache_step`` without a new entry: the queries of the last of ``lengths`` entries."""
 
-    return _step(cache, queries, None, None, lengths, active, scale)
+    return _step(cache, queries, None, None, lengths, active, scale, False)

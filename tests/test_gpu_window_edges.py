@@ -424,3 +424,14 @@ def test_the_library_refuses_chunks_that_it_cannot_take():
                          (call(window=0), "window"), (call(sinks=-1), "window"), (call(window=1 << 40), "2\\^29"), (call(width=320), "256")):
         with pytest.raises(_native.NativeCallError, match=message):
             bad()
+
+
+def test_a_step_without_a_key_and_a_value_is_refused():
+    """A step appends; reading alone is another call."""
+
+    cache = W.window_cache(2, 2, 8, window=4, device="cpu")
+    q, n = torch.zeros(2, 4, 8), torch.zeros(2, dtype=torch.int64)
+    with pytest.raises(CudaThinkValidationError, match="keys must be a torch.Tensor"):
+        W.window_cache_step(cache, q, None, None, n)
+    with pytest.raises(CudaThinkValidationError, match="keys must be a torch.Tensor"):
+        W.window_cache_step(cache, q, None, q[:, :2], n)
