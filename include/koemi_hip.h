@@ -1050,7 +1050,8 @@ int koemi_window_attention_chunk(const void* queries, const void* keys, const vo
                                  int dtype, void* workspace, size_t workspace_bytes, koemi_stream_t stream);
 
 /* Its gradients, each contiguous in its input's shape, NULL where not wanted. output,
- * rest, lse: the forward's; grad_output contiguous. Sums run in a fixed order. */
+ * rest, lse: the forward's; grad_output contiguous. Sums run in a fixed order. Refused beside the forward's: 2^24 tiles
+ * of 32 sinks (batch x groups). */
 size_t koemi_window_attention_backward_workspace_bytes(int64_t batch, int64_t length, int64_t total, int64_t heads,
                                                        int64_t groups, int64_t width, int64_t window, int64_t sinks,
                                                        int dtype);
@@ -1081,7 +1082,8 @@ int koemi_window_attention_backward(const void* queries, const void* keys, const
  * what the row then holds: output [batch, heads, width], zeros for a row that holds nothing
  * or has 0 in active [batch] (NULL: all; nothing is written there either); strides: batch and
  * head of queries, new keys, new values. dtype: of new rows, queries and results. Workspace of
- * _step: koemi_window_cache_step_workspace_bytes, no zeroing needed. */
+ * _step: koemi_window_cache_step_workspace_bytes, no zeroing needed. Refused: what a launch of fewer than 2^32
+ * threads does not take (2^24 workgroups of up to 32 rows; in _step 2^23 of sixteen query heads of a key head). */
 int koemi_window_cache_write(void* keys, float* key_scales, void* values, float* value_scales, int code,
                              const void* new_keys, const void* new_values, const int64_t* strides, const int64_t* lengths,
                              const int64_t* counts, int64_t batch, int64_t length, int64_t groups, int64_t width,
@@ -1107,7 +1109,8 @@ int koemi_window_cache_step(void* keys, float* key_scales, void* values, float* 
  * sum; and of those w >= min_p (0 <= min_p <= 1). ids [rows]: the first whose running sum,
  * in the ids' order, exceeds uniform x the kept sum; 0 for a row without a score. A row with
  * +inf draws among those. probabilities [rows, vocab] fp32 (NULL: none): the distribution
- * drawn from. Weights are formed in 64 bits and added as whole multiples of 2^-44, in any
+ * drawn from. Refused: 2^32 threads (64 a row of at most 512 scores, 256 to 2048, 1024 above). Weights are formed in
+ * 64 bits and added as whole multiples of 2^-44, in any
  * order the same. Workspace: koemi_sample_filtered_workspace_bytes (0 for short rows),
  * 8-byte aligned, no zeroing needed. */
 size_t koemi_sample_filtered_workspace_bytes(int64_t rows, int64_t vocab);

@@ -755,6 +755,9 @@ size_t lay_out(Parted& d, char* base, int64_t rows, int64_t vocab) {
     return at;
 }
 
+// Threads of a row in one workgroup: a wave takes 512 scores a step, sixteen waves where a row has more than four such tiles.
+int threads_for(int64_t vocab) { return vocab <= kTile ? kWave : vocab <= 2048 ? 256 : 1024; }
+
 template <typename T>
 int draw(const Draw& f, int64_t rows, void* workspace, hipStream_t stream) {
     const char* what = "koemi_sample_filtered";
@@ -763,10 +766,9 @@ int draw(const Draw& f, int64_t rows, void* workspace, hipStream_t stream) {
     d.f = f;
     d.parts = parts_for(rows, f.vocab);
     if (d.parts == 1) {
-        // a wave takes 512 scores a step: sixteen waves where a row has more than four such tiles
-        if (f.vocab <= kTile)
+        if (threads_for(f.vocab) == kWave)
             hipLaunchKernelGGL((sample_narrow_kernel<T>), dim3(grid), dim3(kWave), 0, stream, f);
-        else if (f.vocab <= 2048)
+        else if (threads_for(f.vocab) == 256)
             hipLaunchKernelGGL((sample_filtered_kernel<256, T>), dim3(grid), dim3(256), 0, stream, f);
         else
             hipLaunchKernelGGL((sample_filtered_kernel<1024, T>), dim3(grid), dim3(1024), 0, stream, f);
@@ -811,7 +813,8 @@ extern "C" int koemi_sample_filtered(const void* logits, int dtype, int64_t row_
     if (rows < 0 || vocab < 1) return fail(KOEMI_ERR_INVALID, "%s: rows must not be negative and the vocabulary positive", what);
     if (!float_dtype(dtype)) return fail(KOEMI_ERR_UNSUPPORTED, "%s: float32, float16 or bfloat16, not %s", what, dtype_name(dtype));
     if (vocab > kMaxVocab) return fail(KOEMI_ERR_UNSUPPORTED, "%s: at most 2^19 ids", what);
-    if (rows > 0x7fffffff) return fail(KOEMI_ERR_UNSUPPORTED, "%s: too many rows", what);
+    if (rows >= (int64_t(1) << 32) / threads_for(vocab))
+        return fail(KOEMI_ERR_UNSUPPORTED, "%s: too many rows: a launch has fewer than 2^32 threads", what);
     if (!(temperature >= 1e-30 && temperature <= 1e30)) return fail(KOEMI_ERR_INVALID, "%s: temperature must be positive and finite", what);
     if (top_k < 0 || !(top_p > 0.0 && top_p <= 1.0) || !(min_p >= 0.0 && min_p <= 1.0))
         return fail(KOEMI_ERR_INVALID, "%s: top_k must not be negative, top_p above 0 and min_p from 0, both at most 1", what);

@@ -562,6 +562,8 @@ extern "C" int koemi_window_attention_backward(const void* queries, const void* 
     f.out = output, f.rest = dtype == KOEMI_F32 ? nullptr : rest, f.lse = lse, f.d_out = grad_output, f.dq = grad_queries, f.dk = grad_keys, f.dv = grad_values;
     f.row_tiles = static_cast<int>((length * f.s.shared + kRows - 1) / kRows);
     far_of(f.s, f);
+    if (batch * groups * f.far_tiles * f.far_chunks >= (int64_t(1) << 32) / kThreads)
+        return fail(KOEMI_ERR_UNSUPPORTED, "%s: too many sinks for gradients: a launch has fewer than 2^32 threads", what);
     const size_t cells = static_cast<size_t>(batch) * heads * length;
     const size_t need = (cells + far_values(f.s, f)) * 4;
     if (need && (!workspace || workspace_bytes < need)) return fail(KOEMI_ERR_INVALID, "%s: workspace too small", what);

@@ -24,6 +24,7 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr int kInt8 = 0, kE4m3 = 1;
+constexpr int64_t kMostThreads = int64_t(1) << 32;  // a launch has fewer
 
 struct Cache {
     uint8_t* keys;          // [batch, groups, slots, stored]
@@ -678,7 +679,7 @@ extern "C" int koemi_window_cache_write(void* keys, float* key_scales, void* val
     f.vector = aligned16(new_keys, size_of(dtype), {f.kb, f.kp, f.kh}) && aligned16(new_values, size_of(dtype), {f.vb, f.vp, f.vh});
     if (length >= (int64_t(1) << 31) / groups - 256) return fail(KOEMI_ERR_UNSUPPORTED, "%s: at most 2^31 new entries x key heads", what);
     const int64_t per_batch = (length * groups * f.lanes + kThreads - 1) / kThreads;
-    if (batch * per_batch >= (int64_t(1) << 31)) return fail(KOEMI_ERR_UNSUPPORTED, "%s: too many rows", what);
+    if (batch * per_batch >= kMostThreads / kThreads) return fail(KOEMI_ERR_UNSUPPORTED, "%s: too many rows: a launch has fewer than 2^32 threads", what);
     f.per_batch = static_cast<int>(per_batch);
     const dim3 grid(static_cast<unsigned>(batch * per_batch));
     auto launch = [&](auto type, auto kind) {
@@ -712,7 +713,7 @@ extern "C" int koemi_window_cache_entries(const void* keys, const float* key_sca
     f.lengths = lengths, f.keys = out_keys, f.values = out_values, f.present = present;
     f.lanes = lanes_of(f.c.stored);
     const int64_t per_batch = ((window + sinks) * groups * f.lanes + kThreads - 1) / kThreads;
-    if (batch * per_batch >= (int64_t(1) << 31)) return fail(KOEMI_ERR_UNSUPPORTED, "%s: too many rows", what);
+    if (batch * per_batch >= kMostThreads / kThreads) return fail(KOEMI_ERR_UNSUPPORTED, "%s: too many rows: a launch has fewer than 2^32 threads", what);
     f.per_batch = static_cast<int>(per_batch);
     const dim3 grid(static_cast<unsigned>(batch * per_batch));
     auto launch = [&](auto type, auto kind) {
@@ -759,6 +760,8 @@ extern "C" int koemi_window_cache_step(void* keys, float* key_scales, void* valu
     f.scale = scale;
     f.shared = static_cast<int>(heads / groups), f.blocks16 = (f.shared + 15) / 16;
     f.splits = splits_for(batch, heads, groups, window + sinks);
+    if (batch * groups * f.blocks16 * f.splits >= kMostThreads / (f.c.stored <= 128 ? kStepWaves<4> * kWave : kStepWaves<8> * kWave))
+        return fail(KOEMI_ERR_UNSUPPORTED, "%s: too many rows of heads: a launch has fewer than 2^32 threads", what);
     if (f.splits > 1) {
         const size_t cells = static_cast<size_t>(f.splits) * batch * heads;
         if (!workspace || workspace_bytes < cells * (width + 1) * 4) return fail(KOEMI_ERR_INVALID, "%s: workspace too small", what);

@@ -435,3 +435,37 @@ def test_a_step_without_a_key_and_a_value_is_refused():
         W.window_cache_step(cache, q, None, None, n)
     with pytest.raises(CudaThinkValidationError, match="keys must be a torch.Tensor"):
         W.window_cache_step(cache, q, None, q[:, :2], n)
+
+
+def test_sizes_past_a_launch_are_refused():
+    """On the host, before any launch: a launch takes fewer than 2^32 threads. Addresses are never followed."""
+
+    import ctypes
+
+    from koemi_amd import _native
+
+    six = (ctypes.c_int64 * 6)(*[8] * 6)
+    nine = (ctypes.c_int64 * 9)(*[16, 8, 8] * 3)
+
+    def write(batch, length):
+        return "koemi_window_cache_write", (16, 16, 16, 16, 0, 16, 16, six, 16, None, batch, length, 1, 8, 2, 0, _native.BF16, None)
+
+    def entries(batch, window):
+        return "koemi_window_cache_entries", (16, 16, 16, 16, 0, 16, 16, 16, 16, batch, 1, 8, window, 0, _native.BF16, None)
+
+    def step(batch, heads, width):
+        return "koemi_window_cache_step", (16, 16, 16, 16, 0, 16, None, None, six, 16, None, 16, batch, heads, heads, width, 1, 0, 1.0,
+                                           _native.BF16, None, 0, None)
+
+    def draw(rows, vocab):
+        return "koemi_sample_filtered", (16, _native.F32, vocab, rows, vocab, -1, 1.0, 0, 1.0, 0.0, 16, 16, None, None, 0, None)
+
+    def sinks(batch, total, window):
+        need = _native.query("koemi_window_attention_backward_workspace_bytes", batch, total, total, 1, 1, 8, window, total, _native.BF16)
+        return "koemi_window_attention_backward", (16, 16, 16, None, nine, 16, None, 16, 16, 16, 16, 16, batch, total, total, 1, 1, 8,
+                                                   window, total, 1.0, _native.BF16, 16, need, None)
+
+    for name, args in (write(1 << 20, 1024), entries(1 << 20, 1024), step(1 << 23, 1, 64), step(1 << 20, 8, 64), step(1 << 22, 4, 256),
+                       draw(1 << 26, 2), draw(1 << 24, 600), draw(1 << 22, 5000), sinks(1 << 15, 1 << 14, 1)):
+        with pytest.raises(_native.NativeCallError, match="2\\^32 threads"):
+            _native.call(name, *args)
