@@ -15,7 +15,7 @@
 // u falls into. A row stays in its XCD's L2 between the walks. Few long rows are walked by
 // several workgroups each, one launch a phase; a row of one tile stays in a wave's registers.
 // Bound by the two passes of exponentials: 128 rows of 131072 bf16 scores with top-p and min-p
-// take 7 us for the maximum, 26 the histogram, 9 + 13 + 9 the limit, 20 the kept weights, 6 the pick;
+// take 7 us for the maximum, 26 the histogram, 9 + 13 + 10 the limit, 20 the kept weights, 6 the pick;
 // one read of the scores takes 7.
 #include "common.hpp"
 
@@ -726,7 +726,9 @@ __global__ __launch_bounds__(kWave) void sample_narrow_kernel(Draw f) {
 // Workgroups of a row in the walks: one, or for at most 128 rows of 65536 scores and more so many
 // that all rows have about 512, none under eight tiles. Seven launches instead of one, in us with
 // top-p and min-p, parted against one workgroup a row: 8 x 131072 67 | 119, 128 x 131072 87 | 124,
-// 64 x 65536 56 | 72, 128 x 65536 62 | 71, but 8 x 32768 42 | 45, 128 x 32768 52 | 46 and 256 x 131072 131 | 130.
+// 64 x 65536 56 | 72, 128 x 65536 62 | 71, but 8 x 32768 42 | 45, 128 x 32768 52 | 46. Past 128 rows three parts (to
+// 170 rows) would still gain, two (192 and more) no longer: 129 x 131072 98 | 126, 160 x 131072 99 | 129, 192 x 131072 127 | 129,
+// 256 x 131072 130 | 130, 129 x 65536 66 | 73, 160 x 65536 67 | 75, 192 x 65536 83 | 75, 256 x 65536 83 | 71.
 int parts_for(int64_t rows, int64_t vocab) {
     if (vocab < 65536 || rows > 128) return 1;
     const int64_t tiles = (vocab + kTile - 1) / kTile;

@@ -8,10 +8,10 @@
 // them sees; a wave holds 32 rows as the columns of its products, so a row's maximum, sum
 // and rescaling are a lane's own (two lanes a row).
 // 128 rows and 64 keys: 16-bit heads of 64 leave registers for three waves a SIMD, of 128 for two; more
-// rows a wave or a second tile in flight spilled. Bound by the products and, beside them, an
-// exponential for each 2 D multiply-adds: bf16, 16 heads on 4, [1, 16384] of 128, window 2048 behind 2052
-// carried keys 338 us (0.82 PFLOP/s; a large product 1.12), [8, 2048] of 64, window 512, 48 us. The smallest calls
-// are a chain of latencies: [1, 16] 6 us.
+// rows a wave or a second tile in flight spilled. Bound by the products (three of a pair: the probabilities are two planes)
+// and, beside them, an exponential for each 3 D multiply-adds: bf16, 16 heads on 4, [1, 16384] of 128, window 2048 behind 2052
+// carried keys 445 us a call (0.62 PFLOP/s of the two products that count, 0.93 of the three; a large product 1.12),
+// [8, 2048] of 64, window 512, 56 us. The smallest calls are a chain of latencies: [1, 16] 6.5 us.
 #include "window_attention.hpp"
 
 #include <algorithm>

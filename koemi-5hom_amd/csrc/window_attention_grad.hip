@@ -7,15 +7,15 @@
 // Two kernels, each owning what it sums, so that no sum depends on an order of arrival: one
 // holds 128 rows (positions x shared heads) and walks the keys for dq and D, one holds 128
 // keys and walks the rows for dk and dv, all heads that share the keys among them. That
-// forms s and dp twice (seven products of a pair instead of five). The sinks are seen by every
+// forms s and dp twice (seven products of a pair instead of five; in 16 bits, where p and ds are two planes, ten). The sinks are seen by every
 // later row: what lies beyond their window is cut into chunks of rows that run beside the
 // others, and the sinks' own workgroups add the chunks' sums in order.
 //
 // Bound by the products, the exponentials and, at heads of 128, by one wave a SIMD (dk, dv, p and
-// ds take 467 registers). bf16, 16 heads on 4, [8, 2048] of 64, window 512: dq 58 us, dk and dv 113, the sinks'
-// far rows 21, their sums 5. 8 heads on 2, [1, 16384] of 128, window 4096: 513, 797, 40, 11 (a large
-// product's rate would take 750 for forward and gradients). fp32, 4 heads on 1, [2, 1500] of 48, window
-// 256: 40 and 80.
+// ds take 467 registers). bf16, 16 heads on 4, [8, 2048] of 64, window 512: dq 65 us, dk and dv 148, the sinks'
+// far rows 22, their sums 5. 8 heads on 2, [1, 16384] of 128, window 4096: 570, 979, 42, 11 (a large
+// product's rate would take 750 for forward and gradients of seven products). fp32, 4 heads on 1, [2, 1500] of 48, window
+// 256: 40 and 79.
 #include "window_attention.hpp"
 
 #include <algorithm>
@@ -373,8 +373,8 @@ __global__ __launch_bounds__(kThreads, NB == 1 || (NB == 2 && !(SHARE && sizeof(
             const int w = RW > 1 ? rb / 2 : 0;
             if (rb < RB) block(rb, static_cast<uint32_t>(shown[w] >> (32 * (rb & 1))), static_cast<uint32_t>(alone[w] >> (32 * (rb & 1))));
         } else if (NB <= 2 && every && !any_alone && wave_whole && p0 >= wave_last_begin && p0 + RT <= wave_end) {
-            // all seen: without a branch, so that one block's products run beside the other's terms (heads of 64: 115 ->
-            // 109 us; wider ones have no registers for both blocks)
+            // all seen: without a branch, so that one block's products run beside the other's terms (heads of 64: 158 ->
+            // 153 us; wider ones have no registers for both blocks)
             f32x16 s[RB], d[RB];
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) products(rb, s[rb], d[rb]);
@@ -503,8 +503,9 @@ int run(const Backward& f, hipStream_t stream) {
             if (rc != KOEMI_OK) return rc;
         }
     }
-    // Shared keys cost about 1.7 times the work on a full chip ([1, 16384], 256 wide workgroups: 1347 us against 771)
-    // and spread it where the wide ones leave compute units idle (70 of them at [5, 777]: 31.6 us against 45.7).
+    // Shared keys cost about 1.5 times the work on a full chip ([1, 16384], 256 wide workgroups: 1598 us against 1063)
+    // and spread it where the wide ones leave compute units idle (70 of them at [5, 777]: 35.5 us against 52.5; 24 at
+    // [2, 1500] in fp32: 80 against 256).
     const int64_t wide = heads * ((f.s.total + kRows - 1) / kRows);
     if (wide < 160)
         hipLaunchKernelGGL((window_dkv_kernel<T, NB, true>), dim3(static_cast<unsigned>(heads * ((f.s.total + 31) / 32))),
