@@ -1083,7 +1083,7 @@ int koemi_window_attention_backward(const void* queries, const void* keys, const
  * or has 0 in active [batch] (NULL: all; nothing is written there either); strides: batch and
  * head of queries, new keys, new values. dtype: of new rows, queries and results. Workspace of
  * _step: koemi_window_cache_step_workspace_bytes, no zeroing needed. Refused: what a launch of fewer than 2^32
- * threads does not take (2^24 workgroups of up to 32 rows; in _step 2^23 of sixteen query heads of a key head). */
+ * threads does not take (2^24 workgroups of 8 to 64 rows; in _step 2^23 of sixteen query heads of a key head). */
 int koemi_window_cache_write(void* keys, float* key_scales, void* values, float* value_scales, int code,
                              const void* new_keys, const void* new_values, const int64_t* strides, const int64_t* lengths,
                              const int64_t* counts, int64_t batch, int64_t length, int64_t groups, int64_t width,

@@ -1,6 +1,7 @@
 """Calls of the windowed attention and its cache at the edges of what they take.
 
-Large calls that keep the precision of small ones, against float64 with the bounds of
+Precision that does not depend on a call's size, layouts of padded rows, infinities, values and keys of any size,
+chunks behind a cache whose rows lack their sinks, and what is refused; against float64 with the bounds of
 test_gpu_window_attention.py and of test_gpu_window_cache.py.
 """
 
