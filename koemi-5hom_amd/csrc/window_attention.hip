@@ -167,14 +167,15 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 4 : NB == 2 ? 3 : NB <= 4 ? 2 :
         if constexpr (sizeof(T) == 2) {
             // An infinite value times two planes may be NaN, by a second plane of 0 or of the other sign. Where such sums
             // are NaN and the probabilities are not, they are what the infinities and NaN among the values seen add up to.
-            bool nan = false;
+            float any[4] = {};  // NaN if one of the sums is
 #pragma unroll
             for (int n = 0; n < NB; ++n)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) nan = nan || acc[n][r] != acc[n][r];
+                for (int r = 0; r < 16; ++r) any[r % 4] += acc[n][r];
+            any[0] = (any[0] + any[1]) + (any[2] + any[3]);
             const float all = sum_of_halves(sum);
-            nan = nan && row_ok && all == all;
-            if (__any(nan)) {
+            const bool nan = row_ok && any[0] != any[0] && all == all;
+            if (__builtin_expect(__any(nan), 0)) {
                 uint32_t lost[NB];
 #pragma unroll
                 for (int n = 0; n < NB; ++n) {

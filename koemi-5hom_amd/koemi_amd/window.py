@@ -166,13 +166,16 @@ def _plan(query: tuple, key: tuple, value: tuple, query_stride: tuple, key_strid
 
 
 def _rows(tensor: Tensor, width: int) -> Tensor:
-    """A copy of ``tensor`` [B, L, H, D] that the kernels can read: contiguous whatever the layout (``pad`` and
-    ``clone`` may keep one with other columns inside), its width padded with zeros to whole 16-byte pieces, aligned."""
+    """A copy of ``tensor`` [B, L, H, D] that the kernels can read: contiguous whatever the layout, its width
+    padded with zeros to whole 16-byte pieces, aligned."""
 
-    rows = tensor.new_empty((*tensor.shape[:3], width))
-    rows[..., :tensor.shape[3]].copy_(tensor)
-    if width > tensor.shape[3]:
-        rows[..., tensor.shape[3]:].zero_()
+    batch, length, heads, short = *tensor.shape[:3], width - tensor.shape[3]
+    if not short:
+        return tensor.clone(memory_format=torch.contiguous_format)
+    rows = torch.nn.functional.pad(tensor, (0, short))
+    if rows.stride() != (length * heads * width, heads * width, width, 1):  # a layout that pad kept
+        rows = tensor.new_zeros((batch, length, heads, width))
+        rows[..., :tensor.shape[3]].copy_(tensor)
     return rows
 
 
