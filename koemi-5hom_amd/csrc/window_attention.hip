@@ -10,8 +10,8 @@
 // 128 rows and 64 keys: 16-bit heads of 64 leave registers for three waves a SIMD, of 128 for two; more
 // rows a wave or a second tile in flight spilled. Bound by the products (three of a pair: the probabilities are two planes)
 // and, beside them, an exponential for each 3 D multiply-adds: bf16, 16 heads on 4, [1, 16384] of 128, window 2048 behind 2052
-// carried keys 445 us a call (0.62 PFLOP/s of the two products that count, 0.93 of the three; a large product 1.12),
-// [8, 2048] of 64, window 512, 56 us. The smallest calls are a chain of latencies: [1, 16] 6.5 us.
+// carried keys 434 us a call (0.63 PFLOP/s of the two products that count, 0.95 of the three; a large product 1.12),
+// [8, 2048] of 64, window 512, 57 us. The smallest calls are a chain of latencies: [1, 16] 6.1 us.
 #include "window_attention.hpp"
 
 #include <algorithm>

@@ -12,8 +12,8 @@
 // others, and the sinks' own workgroups add the chunks' sums in order.
 //
 // Bound by the products, the exponentials and, at heads of 128, by one wave a SIMD (dk, dv, p and
-// ds take 467 registers). bf16, 16 heads on 4, [8, 2048] of 64, window 512: dq 65 us, dk and dv 148, the sinks'
-// far rows 22, their sums 5. 8 heads on 2, [1, 16384] of 128, window 4096: 570, 979, 42, 11 (a large
+// ds take 467 registers). bf16, 16 heads on 4, [8, 2048] of 64, window 512: dq 65 us, dk and dv 149, the sinks'
+// far rows 22, their sums 5. 8 heads on 2, [1, 16384] of 128, window 4096: 547, 939, 43, 11 (a large
 // product's rate would take 750 for forward and gradients of seven products). fp32, 4 heads on 1, [2, 1500] of 48, window
 // 256: 40 and 79.
 #include "window_attention.hpp"

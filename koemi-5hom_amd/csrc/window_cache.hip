@@ -9,8 +9,8 @@
 //
 // Rows of codes are whole blocks of 32 bytes, zeros behind the head's width.
 // All three are bound by bytes, the small ones by one pass of their workgroups: [8, 2048, 4, 64] bf16 written
-// in 13 us, read back in 9; a step of 8 rows over up to 32784 entries of 8 key heads of 128 in e4m3 94 to 97 us a call
-// (471 MB, 4.9 TB/s), of 64 rows over 1028 entries of 4 of 64 in int8 16 (36 MB).
+// in 13 us, read back in 9; a step of 8 rows over up to 32784 entries of 8 key heads of 128 in e4m3 94 to 104 us a call
+// (471 MB, 4.5 to 5.0 TB/s), of 64 rows over 1028 entries of 4 of 64 in int8 16 (36 MB).
 #include "common.hpp"
 
 #include <algorithm>
